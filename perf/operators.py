@@ -252,8 +252,10 @@ def _step_outputs(s):
 def run(state: dict):
     s, kind = state, state["case"]["kind"]
     if own:
-        from aeris_gb_b200.ops import orthogonalise as OR
-        from aeris_gb_b200.ops import qk_norm as QN
+        if kind.startswith("norm"):
+            from aeris_gb_b200.ops import qk_norm as QN
+        else:
+            from aeris_gb_b200.ops import orthogonalise as OR
         if kind == "norm":
             return QN.qk_norm_fwd(s["q"], s["k"], s["wq"], s["wk"], s["cos"], s["sin"], eps=EPS, positions=s["positions"])
         if kind == "norm-grad":
