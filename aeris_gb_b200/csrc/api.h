@@ -181,6 +181,28 @@ int aeris_block_backward(const AerisBlock* b, const AerisBlockGrad* g);
 // aeris_block_forward of `n` records in a row, each with `mod + mod_offset` and on `stream`; same result codes.
 int aeris_blocks_forward(const AerisBlock* blocks, int n, long long mod_offset, void* stream);
 
+
+// Norms of queries and keys by head with the position rotation (csrc/qk_norm.cu; mirrored in ops/qk_norm.py). Strides in
+// elements; a head's channels lie side by side.
+typedef struct AerisHeads {
+  const void* ptr;
+  long long row, head;
+} AerisHeads;
+typedef struct AerisQkNorm {
+  AerisHeads q, k, dq, dk, q_out, k_out;  // q_out, k_out: results (backward: gradients of q, k); may be the inputs themselves
+  const void *wq, *wk;              // [d], bf16 or fp32
+  const float *cos, *sin;           // [L, rot / 2], or null with rot = 0
+  const void* pos;                  // table row of every row (int32 or int64), null: row mod L. Outside [0, L): recorded in
+                                    // the status word, the row's results are not written
+  float *dwq, *dwk, *sums;          // backward: [d] each; scratch [sum_rows, 2, d]
+  int* status;
+  long long rows;
+  int L, heads, kv_heads, d, rot, f32, w_bf16, pos64, add_dw, sum_rows;   // add_dw: dwq, dwk are added to
+  float eps;
+} AerisQkNorm;
+int aeris_qk_norm_fwd(const AerisQkNorm* a, void* stream);
+int aeris_qk_norm_bwd(const AerisQkNorm* a, void* stream);      // returns the number of kernels launched, or a negative code
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ pure-PyTorch oracle in :mod:`aeris_gb_b200.models.oracle` instead and never reac
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -45,6 +46,16 @@ def raw_stream() -> int:
 
 def stream_ptr() -> _c_void_p:
     return _c_void_p(raw_stream())
+
+
+def require_cuda(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"the kernels take tensors on a GPU, got one on {t.device}")
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one; 2 us where it is not already."""
+    return contextlib.nullcontext() if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _STATUS: dict[int, torch.Tensor] = {}

@@ -1,0 +1,85 @@
+"""Refusals of the norms of queries and keys: made on the host, before anything is launched."""
+import pytest
+import torch
+
+from aeris_gb_b200.ops import qk_norm as QN
+
+ROWS, H, HK, D, L = 6, 4, 2, 16, 3
+
+
+def args(**over):
+    a = dict(q=torch.randn(ROWS, H, D), k=torch.randn(ROWS, HK, D), wq=torch.ones(D), wk=torch.ones(D),
+             cos=torch.ones(L, D // 2), sin=torch.zeros(L, D // 2), positions=None, q_out=None, k_out=None)
+    a.update(over)
+    return a
+
+
+def forward(a):
+    return QN.qk_norm_fwd(a["q"], a["k"], a["wq"], a["wk"], a["cos"], a["sin"], eps=1e-6, positions=a["positions"],
+                          q_out=a["q_out"], k_out=a["k_out"])
+
+
+BAD = {
+    "rows differ": dict(k=torch.randn(ROWS + 1, HK, D)),
+    "widths differ": dict(k=torch.randn(ROWS, HK, D + 2)),
+    "two dimensions": dict(q=torch.randn(ROWS, H * D)),
+    "odd width": dict(q=torch.randn(ROWS, H, 15), k=torch.randn(ROWS, HK, 15)),
+    "too wide": dict(q=torch.randn(ROWS, H, 258), k=torch.randn(ROWS, HK, 258)),
+    "no heads": dict(k=torch.randn(ROWS, 0, D)),
+    "half": dict(q=torch.randn(ROWS, H, D).half(), k=torch.randn(ROWS, HK, D).half()),
+    "types differ": dict(k=torch.randn(ROWS, HK, D).bfloat16()),
+    "channels apart": dict(q=torch.randn(ROWS, D, H).transpose(1, 2)),
+    "weight of another width": dict(wq=torch.ones(D + 2)),
+    "weight types differ": dict(wk=torch.ones(D).bfloat16()),
+    "weight with gaps": dict(wk=torch.ones(2 * D)[::2]),
+    "sin without cos": dict(cos=None),
+    "positions without angles": dict(cos=None, sin=None, positions=torch.zeros(ROWS, dtype=torch.int32)),
+    "angles in bf16": dict(cos=torch.ones(L, D // 2).bfloat16(), sin=torch.ones(L, D // 2).bfloat16()),
+    "more angles than pairs": dict(cos=torch.ones(L, D), sin=torch.ones(L, D)),
+    "angles of unlike length": dict(sin=torch.ones(L + 1, D // 2)),
+    "empty table": dict(cos=torch.ones(0, D // 2), sin=torch.ones(0, D // 2)),
+    "positions of another length": dict(positions=torch.zeros(ROWS + 1, dtype=torch.int32)),
+    "positions in floating point": dict(positions=torch.zeros(ROWS)),
+    "positions with gaps": dict(positions=torch.zeros(2 * ROWS, dtype=torch.int64)[::2]),
+    "result of another shape": dict(q_out=torch.empty(ROWS, H + 1, D)),
+    "result of another type": dict(k_out=torch.empty(ROWS, HK, D).bfloat16()),
+    "expanded result": dict(q_out=torch.empty(1, H, D).expand(ROWS, H, D)),
+    "result with overlapping heads": dict(q_out=torch.empty(ROWS * H * D).as_strided((ROWS, H, D), (H * D, D // 2, 1))),
+}
+
+
+@pytest.mark.parametrize("what", BAD)
+def test_refused(what):
+    with pytest.raises(ValueError):
+        forward(args(**BAD[what]))
+
+
+def test_cpu_tensors_are_refused_and_not_computed_elsewhere():
+    with pytest.raises(ValueError, match="GPU"):
+        forward(args())
+
+
+@pytest.mark.parametrize("bad", [dict(dq=torch.randn(ROWS, H, D + 2)), dict(dk=torch.randn(ROWS, HK, D).bfloat16()),
+                                 dict(dwq=torch.zeros(D)), dict(dwq=torch.zeros(D), dwk=torch.zeros(D + 1)),
+                                 dict(dwq=torch.zeros(D), dwk=torch.zeros(D).bfloat16()),
+                                 dict(dq_out=torch.empty(ROWS, 1, D).expand(ROWS, H, D))])
+def test_backward_refuses(bad):
+    a = args()
+    g = dict(dq=torch.randn(ROWS, H, D), dk=torch.randn(ROWS, HK, D), dwq=None, dwk=None, dq_out=None)
+    g.update(bad)
+    with pytest.raises(ValueError):
+        QN.qk_norm_bwd(g["dq"], g["dk"], a["q"], a["k"], a["wq"], a["wk"], a["cos"], a["sin"], eps=1e-6, dwq=g["dwq"],
+                       dwk=g["dwk"], dq_out=g["dq_out"])
+
+
+@pytest.mark.parametrize("shape,strides,fine", [((5, 3, 8), (24, 8, 1), True), ((5, 3, 8), (8, 40, 1), True),
+                                                ((5, 3, 8), (100, 8, 1), True), ((1, 3, 8), (0, 8, 1), True),
+                                                ((5, 1, 8), (8, 0, 1), True), ((5, 3, 8), (20, 8, 1), False),
+                                                ((5, 3, 8), (0, 8, 1), False), ((5, 3, 8), (8, 36, 1), False)])
+def test_overlap_of_results(shape, strides, fine):
+    t = torch.empty(1000).as_strided(shape, strides)
+    if fine:
+        QN._writable("t", t)
+    else:
+        with pytest.raises(ValueError):
+            QN._writable("t", t)
