@@ -203,6 +203,43 @@ typedef struct AerisQkNorm {
 int aeris_qk_norm_fwd(const AerisQkNorm* a, void* stream);
 int aeris_qk_norm_bwd(const AerisQkNorm* a, void* stream);      // returns the number of kernels launched, or a negative code
 
+// Orthogonalisation of matrices (csrc/orthogonalise.cu; mirrored in ops/orthogonalise.py). A batch: `count` matrices of rows x
+// cols with row pitch ld, matrix i at element offsets[i] (device memory, int64, ascending, no two overlapping, inside [0,
+// numel): else the status word is set and the matrix left out) or, with offsets null, at i * stride. X: fp16 workspace, one
+// [min(rows, cols), longer side rounded up to 64] per matrix. At most 65535 matrices a call.
+typedef struct AerisOrthoIn {
+  const void* x;                    // fp32 or bf16, or null with grad and momentum (flat fp32 buffers, offsets needed)
+  float *grad, *momentum;
+  const double* norm_sq;            // as aeris_adamw
+  const void* offsets;
+  void* X;
+  double* partial;                  // [count, 128]
+  int* status;
+  double eps;
+  long long stride, numel;
+  int rows, cols, ld, count, behind, bf16, nesterov, zero_grad;   // behind: offsets[-1] is the matrix before the first one
+  float beta, grad_scale, max_norm;
+} AerisOrthoIn;
+typedef struct AerisOrthoOut {
+  const void* X;
+  void* out;                        // bf16, or null with master
+  float *master, *ema;              // flat fp32 buffers; ema may be null
+  void* weights;                    // flat bf16 buffer or null
+  const void* offsets;
+  int* status;
+  long long stride, numel;
+  int rows, cols, ld, count, behind;
+  float decay, rate, ema_beta;      // master * decay - rate * X
+} AerisOrthoOut;
+int aeris_ortho_in(const AerisOrthoIn* a, void* stream);        // two kernels
+int aeris_ortho_out(const AerisOrthoOut* a, void* stream);
+// X: [2, count] matrices d x K, the first `count` the input; S: aeris_ortho_buffers() * count matrices d x d of pitch d rounded
+// up to 64, both fp16. Returns the number of kernels launched, or a negative code. The result is in the half of X that
+// aeris_ortho_updates() changes of side lead to.
+int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, int steps, int* status, void* stream);
+int aeris_ortho_buffers();
+int aeris_ortho_updates(int d, int K, int steps);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,47 @@
+"""Refusals of the orthogonalisation and of the optimizer step on it: made on the host, before anything is launched."""
+import pytest
+import torch
+
+from aeris_gb_b200.ops import orthogonalise as OR
+
+
+@pytest.mark.parametrize("x,kw", [
+    (torch.randn(4), {}), (torch.randn(2, 2, 4, 4), {}), (torch.randn(4, 4).half(), {}), (torch.randn(4, 4).double(), {}),
+    (torch.randn(4, 4), dict(steps=0)), (torch.randn(4, 4), dict(steps=21)), (torch.randn(4, 4), dict(steps=2.0)),
+    (torch.randn(4, 4), dict(out=torch.empty(4, 4))), (torch.randn(4, 4), dict(out=torch.empty(4, 5).bfloat16())),
+    (torch.randn(4, 4), dict(out=torch.empty(1, 4).bfloat16().expand(4, 4))),
+    (torch.randn(2, 4, 4), dict(out=torch.empty(1, 4, 4).bfloat16().expand(2, 4, 4))),
+    (torch.randn(4, 4), dict(out=torch.empty(4, 4).bfloat16().t())),
+    (torch.randn(4, 4), {}),                                                     # not on a GPU
+])
+def test_orthogonalise_refuses(x, kw):
+    with pytest.raises(ValueError):
+        OR.orthogonalise(x, **kw)
+
+
+N = 64
+
+
+def step(**over):
+    a = dict(master=torch.zeros(N), grad=torch.zeros(N), momentum=torch.zeros(N), weights=torch.zeros(N).bfloat16(),
+             ema=torch.zeros(N), norm_sq=torch.zeros(1, dtype=torch.float64), groups=[(4, 4, torch.tensor([0, 16]))])
+    kw = dict(lr=1e-3, beta=0.9, nesterov=True, weight_decay=0.1, scale=0.2, grad_scale=1.0, max_norm=1.0, ema_beta=0.5)
+    for k, v in over.items():
+        (a if k in a else kw)[k] = v
+    groups = a.pop("groups")
+    OR.orthogonal_step(*a.values(), groups=groups, **kw)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(master=torch.zeros(8, 8)), dict(master=torch.zeros(N).bfloat16()), dict(master=torch.zeros(2 * N)[::2]),
+    dict(master=torch.zeros(N + 1)[1:]), dict(grad=torch.zeros(N + 1)), dict(grad=torch.zeros(N).bfloat16()),
+    dict(momentum=torch.zeros(2 * N)[::2]), dict(momentum=torch.zeros(N + 1)[1:]), dict(weights=torch.zeros(N)),
+    dict(ema=torch.zeros(N - 1)), dict(norm_sq=torch.zeros(1)), dict(norm_sq=torch.zeros(2, dtype=torch.float64)),
+    dict(groups=[(0, 4, torch.tensor([0]))]), dict(groups=[(4, 4, torch.tensor([0], dtype=torch.int32))]),
+    dict(groups=[(4, 4, torch.tensor([[0]]))]), dict(groups=[(4, 4, torch.tensor([0, 1, 2, 3])[::2])]),
+    dict(groups=[(4, 4, torch.tensor([0, 16, 32, 48, 64]))]), dict(groups=[(9, 9, torch.tensor([0]))]), dict(steps=0),
+    {},                                                                           # not on a GPU
+])
+def test_step_refuses(bad):
+    with pytest.raises(ValueError):
+        step(**bad)
