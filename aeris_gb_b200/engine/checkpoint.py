@@ -83,8 +83,9 @@ def _torch_optim_state(names: list[str], exp_avg: dict, exp_avg_sq: dict, opt) -
     state = {}
     for i, n in enumerate(names):
         if n in exp_avg:
-            state[i] = {"step": torch.tensor(float(opt.step_count)), "exp_avg": exp_avg[n].cpu(),
-                        "exp_avg_sq": exp_avg_sq[n].cpu()}
+            state[i] = {"step": torch.tensor(float(opt.step_count)), "exp_avg": exp_avg[n].cpu()}
+            if n in exp_avg_sq:          # matrices with orthogonalised updates have a momentum alone
+                state[i]["exp_avg_sq"] = exp_avg_sq[n].cpu()
     group = {"lr": float(getattr(opt, "last_lr", c.lr)), "betas": tuple(c.betas), "eps": c.eps,
              "weight_decay": c.weight_decay, "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
              "differentiable": False, "fused": None, "params": list(range(len(names)))}
@@ -106,9 +107,20 @@ def _read_optim_state(osd: dict, names: list[str]) -> tuple[int, dict, dict]:
     m, v, step = {}, {}, 0
     for i, st in osd["state"].items():
         name = by_index[int(i)]
-        m[name], v[name] = st["exp_avg"], st["exp_avg_sq"]
+        m[name] = st["exp_avg"]
+        if "exp_avg_sq" in st:
+            v[name] = st["exp_avg_sq"]
         step = max(step, int(float(st["step"])))
     return step, m, v
+
+
+def check_methods(opt, exp_avg: dict, exp_avg_sq: dict) -> None:
+    """Raises before anything is touched where the state is not of ``opt``'s kind: matrices with orthogonalised updates have a
+    momentum alone, without second moments AdamW would divide by nothing, and its first moments have another scale."""
+    alone = opt.momentum_only() if hasattr(opt, "momentum_only") else set()
+    for n in exp_avg:
+        if (n in exp_avg_sq) == (n in alone):
+            raise ValueError(f"optimizer state of {n} was written with another method than {opt.cfg.method!r}")
 
 
 def _stage_param_names(module) -> dict[int, list[str]]:
@@ -208,6 +220,7 @@ def load_stage_checkpoint(directory: str | None, module, opt, device) -> bool:
             logging.getLogger(__name__).warning("checkpoint of stage %d in %s not loaded: %s", stage, directory, e)
             return False
     first = next(iter(loaded.values()))
+    check_methods(opt, m, v)
     # parameters are views of the optimizer's flat buffers, so loading the masters refreshes the model copies too;
     # buffers and frozen parameters come from the model state dict
     own = module.state_dict()

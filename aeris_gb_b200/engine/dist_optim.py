@@ -14,11 +14,12 @@ import os
 import torch
 import torch.distributed as dist
 
-from .optim import FlatOptimizer, OptimConfig, ema_beta_at, lr_at
+from .optim import FlatOptimizer, OptimConfig, ema_beta_at, lr_at, require_adamw
 
 
 class DistOptimizer(FlatOptimizer):
     def __init__(self, model, cfg: OptimConfig, group, rs_grads: bool = True):
+        require_adamw(cfg, "the sharded optimizer")
         super().__init__(model, cfg)
         self.group = group
         self.rs_grads = rs_grads

@@ -21,7 +21,7 @@ import torch.nn as nn
 
 from ..ops import elementwise as E
 from ..ops import lib as L
-from .optim import OptimConfig, ema_beta_at, lr_at, no_decay_names
+from .optim import OptimConfig, ema_beta_at, lr_at, no_decay_names, require_adamw
 
 
 def _ptr_array(ptrs):
@@ -56,6 +56,7 @@ class FusedShardedOptimizer:
     def __init__(self, model: nn.Module, cfg: OptimConfig, group, device, use_multicast: bool = True, params=None):
         """``params``: the (name, parameter) pairs to manage; default: every trainable parameter of ``model``."""
         import torch.distributed._symmetric_memory as symm_mem
+        require_adamw(cfg, "the sharded peer-memory optimizer")
         self.cfg, self.group, self.device = cfg, group, torch.device(device)
         self.world, self.rank = dist.get_world_size(group), dist.get_rank(group)
         self.step_count, self.cur_nimg = 0, 0

@@ -43,6 +43,9 @@ def init_params(model: nn.Module, cfg, policy: dict | None = None) -> None:
         if not isinstance(m, (nn.Linear, nn.RMSNorm)):
             continue
         w = m.weight
+        if name.rsplit(".", 1)[-1] in ("q_norm", "k_norm"):      # not in the reference: what they norm enters as it is
+            nn.init.ones_(w)
+            continue
         if tp > 1:
             from ..parallel.tensor import tp_kind
             kind = tp_kind(name + ".weight", w)

@@ -6,6 +6,9 @@ What the reference does (src/aeris/parallelism/parallel_engine.py): a flat fp32 
 and the EMA on the CPU with a full D2H/H2D round trip per step (:727-738, :862-884); piecewise LR schedule
 (:799-830). Here everything stays on the GPU: one fused kernel per segment applies scale, clip, NaN guard, AdamW on
 the fp32 master, the bf16 weight refresh and the EMA update, and zeroes the gradient.
+
+With ``method = "muon"`` the blocks' matrices take orthogonalised momentum instead (ops/orthogonalise.py; absent from the
+reference); everything else keeps AdamW.
 """
 from __future__ import annotations
 
@@ -34,6 +37,13 @@ class OptimConfig:
     ema_halflife_img: int = 100_000
     ema_rampup_ratio: float | None = 0.05
     use_ema: bool = True
+    # "adamw", or "muon": the attention and MLP matrices of the blocks are updated with their orthogonalised momentum, at the
+    # same learning rate and decay (``muon_scale`` gives their updates the root mean square of AdamW's)
+    method: str = "adamw"
+    muon_beta: float = 0.95
+    muon_nesterov: bool = True
+    muon_steps: int = 5
+    muon_scale: float = 0.2
 
 
 def lr_at(cur_nimg: int, base_lr: float, c: OptimConfig) -> float:
@@ -79,6 +89,30 @@ def no_decay_names(model: nn.Module, policy: str) -> set[str]:
     return set()
 
 
+def block_matrices(model: nn.Module) -> dict[str, list[tuple[int, int, int]]]:
+    """The parameters of ``model`` that take orthogonalised updates, by name: (element offset, rows, columns) of the matrices
+    in each. q, k and v are three matrices, and so are the gate and up halves of an MLP's first layer two: they are
+    different maps that share a tensor. The modulation MLPs are not among them: their gradients have the rank of the
+    batch."""
+    from ..models.aeris import AttentionParams, FeedForwardParams
+    out = {}
+    for name, m in model.named_modules():
+        parts = ({"to_qkv": 3, "wo": 1} if isinstance(m, AttentionParams) else
+                 {"w1": 2, "w2": 1} if isinstance(m, FeedForwardParams) else {})
+        for k, n in parts.items():
+            w = getattr(m, k).weight
+            if w.requires_grad:
+                rows, cols = w.shape[0] // n, w.shape[1]
+                out[f"{name}.{k}.weight" if name else f"{k}.weight"] = [(i * rows * cols, rows, cols) for i in range(n)]
+    return out
+
+
+def require_adamw(cfg: OptimConfig, what: str) -> None:
+    """Sharded optimizers cut matrices into pieces, of which none can be orthogonalised by itself."""
+    if cfg.method != "adamw":
+        raise ValueError(f"optimizer method {cfg.method!r} needs whole matrices on every rank: {what} takes \"adamw\" only")
+
+
 @dataclass
 class _Segment:
     name: str
@@ -93,6 +127,7 @@ class _Segment:
     v: torch.Tensor | None = None
     ema: torch.Tensor | None = None
     model_flat: torch.Tensor | None = None   # bf16 flat buffer the module parameters view (low_precision only)
+    groups: list | None = None               # orthogonalised updates: (rows, cols, element offsets); ``m`` is the momentum
 
 
 class FlatOptimizer:
@@ -109,13 +144,17 @@ class FlatOptimizer:
         self.model = model
         self.step_count = 0
         self.cur_nimg = 0
+        if cfg.method not in ("adamw", "muon"):
+            raise ValueError(f"optimizer method {cfg.method!r}: \"adamw\" or \"muon\"")
         nd = no_decay_names(model, cfg.decay_policy)
-        segs: dict[tuple[bool, bool], _Segment] = {}
+        matrices = block_matrices(model) if cfg.method == "muon" else {}
+        segs: dict[tuple[bool, bool, bool], _Segment] = {}
         for n, p in (params if params is not None else model.named_parameters()):
             if not p.requires_grad:
                 continue
-            key = (p.dtype != torch.float32, n not in nd)
-            seg = segs.setdefault(key, _Segment(name=f"{'lp' if key[0] else 'fp32'}_{'decay' if key[1] else 'nodecay'}",
+            key = (p.dtype != torch.float32, n not in nd, n in matrices)
+            seg = segs.setdefault(key, _Segment(name=f"{'lp' if key[0] else 'fp32'}_{'decay' if key[1] else 'nodecay'}"
+                                                     f"{'_matrices' if key[2] else ''}",
                                                 decay=key[1], low_precision=key[0]))
             seg.params.append(p)
             seg.names.append(n)
@@ -132,7 +171,11 @@ class FlatOptimizer:
             seg.master = torch.zeros(total, dtype=torch.float32, device=dev)
             seg.grad = torch.zeros(total, dtype=torch.float32, device=dev)
             seg.m = torch.zeros(total, dtype=torch.float32, device=dev)
-            seg.v = torch.zeros(total, dtype=torch.float32, device=dev)
+            if seg.names[0] in matrices:
+                seg.groups = self._groups([(off + o, rows, cols) for n, off in zip(seg.names, offs)
+                                           for o, rows, cols in matrices[n]], dev)
+            else:
+                seg.v = torch.zeros(total, dtype=torch.float32, device=dev)
             if seg.low_precision:
                 seg.model_flat = torch.zeros(total, dtype=seg.params[0].dtype, device=dev)
             for p, off in zip(seg.params, offs):
@@ -146,6 +189,14 @@ class FlatOptimizer:
                 self._hooks.append(p.register_post_accumulate_grad_hook(self._fold_grad))
             seg.ema = seg.master.clone() if cfg.use_ema else None
         self._norm_sq = None
+
+    @staticmethod
+    def _groups(matrices: list[tuple[int, int, int]], dev) -> list:
+        """(element offset, rows, cols) in ascending order -> (rows, cols, offsets) per shape."""
+        shapes: dict[tuple[int, int], list[int]] = {}
+        for off, rows, cols in matrices:
+            shapes.setdefault((rows, cols), []).append(off)
+        return [(rows, cols, torch.tensor(offs, dtype=torch.int64, device=dev)) for (rows, cols), offs in shapes.items()]
 
     @staticmethod
     def _fold_grad(p: torch.Tensor):
@@ -186,7 +237,9 @@ class FlatOptimizer:
         max_norm = c.grad_clip_max_norm if (c.grad_clip and norm_sq is not None) else 0.0
         for s in self.segments:
             wd = c.weight_decay if s.decay else 0.0
-            if s.master.is_cuda:
+            if s.groups is not None:
+                self._step_matrices(s, lr, wd, grad_scale, max_norm, norm_sq, beta)
+            elif s.master.is_cuda:
                 from ..ops import elementwise as E
                 E.adamw(s.master, s.grad, s.m, s.v, s.model_flat, s.ema if beta is not None else None, norm_sq,
                         lr=lr, betas=c.betas, eps=c.eps, weight_decay=wd, step=self.step_count,
@@ -195,6 +248,16 @@ class FlatOptimizer:
                 self._step_cpu(s, lr, wd, grad_scale, max_norm, norm_sq, beta)
         self.cur_nimg += batch_img
         self.last_lr = lr
+
+    def _step_matrices(self, s: _Segment, lr, wd, grad_scale, max_norm, norm_sq, beta):
+        c = self.cfg
+        kw = dict(groups=s.groups, lr=lr, beta=c.muon_beta, nesterov=c.muon_nesterov, weight_decay=wd, scale=c.muon_scale,
+                  grad_scale=grad_scale, max_norm=max_norm, ema_beta=beta if beta is not None else -1.0, steps=c.muon_steps)
+        if s.master.is_cuda:
+            from ..ops.orthogonalise import orthogonal_step
+        else:
+            from ..models.oracle import orthogonal_step
+        orthogonal_step(s.master, s.grad, s.m, s.model_flat, s.ema, norm_sq, **kw)
 
     def _step_cpu(self, s: _Segment, lr, wd, grad_scale, max_norm, norm_sq, beta):
         c = self.cfg
@@ -239,7 +302,14 @@ class FlatOptimizer:
                 "exp_avg": {k: v.clone() for k, v in self._named_views("m").items()},
                 "exp_avg_sq": {k: v.clone() for k, v in self._named_views("v").items()}}
 
+    def momentum_only(self) -> set[str]:
+        """Parameters whose state is a momentum without second moments."""
+        return {n for s in self.segments if s.groups is not None for n in s.names}
+
     def load_state_dict(self, sd: dict, master: dict | None = None, ema: dict | None = None):
+        from .checkpoint import check_methods
+        check_methods(self, {n: t for s in self.segments for n in s.names if (t := sd["exp_avg"].get(n)) is not None},
+                      sd["exp_avg_sq"])
         self.step_count, self.cur_nimg = sd["step"], sd["cur_nimg"]
         for which, src in (("m", sd["exp_avg"]), ("v", sd["exp_avg_sq"]), ("master", master), ("ema", ema)):
             if src is None:

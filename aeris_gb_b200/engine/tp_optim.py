@@ -21,12 +21,13 @@ import torch.distributed as dist
 import torch.nn as nn
 
 from ..parallel.tensor import fit_to_shard, full_state_dict, tp_kind
-from .optim import FlatOptimizer, OptimConfig
+from .optim import FlatOptimizer, OptimConfig, require_adamw
 
 
 class TPOptimizer:
     def __init__(self, model: nn.Module, cfg: OptimConfig, device, weight_group, tp_group, ortho_group=None,
                  fused: bool = False, use_multicast: bool = False):
+        require_adamw(cfg, "a model with tensor-parallel shards")
         self.cfg, self.device = cfg, torch.device(device)
         self.weight_group, self.tp_group, self.ortho_group = weight_group, tp_group, ortho_group
         self.tp, self.tp_rank = dist.get_world_size(tp_group), dist.get_rank(tp_group)

@@ -71,9 +71,11 @@ class Trainer:
         self.dp_size, self.dp_rank = dp_size, dp_rank
         torch.manual_seed(seed)   # identical initial weights on every rank
         self.model = (model or AerisModel(model_cfg)).to(self.device)
-        # weight-group collectives: this library's peer-memory kernels (default on GPUs with > 1 rank) or NCCL
+        # weight-group collectives: this library's peer-memory kernels (default on GPUs with > 1 rank) or NCCL (orthogonalised
+        # updates, which need whole matrices)
         n_replicas = self.wp_size * dp_size
-        self.fused_dp = (n_replicas > 1 and self.device.type == "cuda") if fused_dp is None else fused_dp
+        self.fused_dp = (n_replicas > 1 and self.device.type == "cuda" and optim_cfg.method == "adamw") \
+            if fused_dp is None else fused_dp
         if self.tp_group is not None:
             from .tp_optim import TPOptimizer
             self.opt = TPOptimizer(self.model, optim_cfg, self.device, self.weight_group, self.tp_group, tp_ortho_group,

@@ -63,6 +63,9 @@ class AerisConfig:
     recompute: bool = False
     use_rope: bool = False          # axial 2-D rotary embedding on q, k inside every window (the reference's is inert)
     rope_base: float = 10_000.0
+    # RMS norm of every head's q and k before the rotation, weights shared by a block's heads (absent from the reference):
+    # keeps the attention scores bounded where weights grow, as under orthogonalised updates
+    qk_norm: bool = False
     # model mode (parallel_swin.py:367-376, 394-397, 474-486): ``diffusion`` conditions every block on the noise level,
     # ``rit`` (random time interval) on an embedding of the forecast interval; with neither the blocks are plain
     # pre-norm transformer blocks and the model is a deterministic regressor
@@ -92,7 +95,7 @@ class AerisConfig:
     def param_count(self) -> int:
         d, hd, f = self.dim, self.heads * self.head_dim, self.mlp_dim
         mod = ((d * d + d if self.layerwise_t_emb else 0) + d * 6 * d + 6 * d) if self.conditioned else 0
-        block = 2 * d + hd + 3 * hd * d + d * hd + 3 * d * f + mod
+        block = 2 * d + hd + 3 * hd * d + d * hd + 3 * d * f + mod + (2 * self.head_dim if self.qk_norm else 0)
         inp = self.in_channels * d + d + 2 * (d * d + d)
         outp = d + (d * d + d if self.layerwise_t_emb else 0) + d * 2 * d + 2 * d + d * self.out_channels
         return block * self.n_blocks + inp + outp
@@ -210,10 +213,11 @@ class ApeBuffer(nn.Module):
 class AttentionParams(nn.Module):
     """``norm``: ``"unused"`` = present in the reference's diffusion checkpoints but never applied (kept frozen for
     key parity, parallel_swin.py:231-232, 265-266), ``"own"`` = the block's pre-norm in the plain mode, ``None`` = absent
-    (rit)."""
+    (rit). ``qk_norm``: norms of q and k by head."""
 
-    def __init__(self, dim, heads, head_dim, norm: str | None = "unused"):
+    def __init__(self, dim, heads, head_dim, norm: str | None = "unused", qk_norm: bool = False):
         super().__init__()
+        self.q_norm, self.k_norm = (nn.RMSNorm(head_dim), nn.RMSNorm(head_dim)) if qk_norm else (None, None)
         if norm is not None:
             self.norm = nn.RMSNorm(dim)
             if norm == "unused":
@@ -337,7 +341,7 @@ class SwinLayer(nn.Module):
             self.modulelist = nn.ModuleList([
                 nn.ModuleList([
                     nn.RMSNorm(d),
-                    AttentionParams(d, cfg.heads, cfg.head_dim, None if cfg.rit else "unused"),
+                    AttentionParams(d, cfg.heads, cfg.head_dim, None if cfg.rit else "unused", cfg.qk_norm),
                     nn.RMSNorm(d),
                     FeedForwardParams(d, cfg.mlp_dim, tp=cfg.tp, tp_rank=cfg.tp_rank),
                     ModulationLinear(d, 6 * d, cfg.layerwise_t_emb),
@@ -345,11 +349,11 @@ class SwinLayer(nn.Module):
             ])
         elif cfg.sublayers > 1:         # plain pre-norm blocks, module names as in parallel_swin.py:446-451
             self.modulelist = nn.ModuleList([
-                nn.ModuleList([AttentionParams(d, cfg.heads, cfg.head_dim, "own"),
+                nn.ModuleList([AttentionParams(d, cfg.heads, cfg.head_dim, "own", cfg.qk_norm),
                                FeedForwardParams(d, cfg.mlp_dim, own_norm=True, tp=cfg.tp, tp_rank=cfg.tp_rank)])
                 for _ in range(cfg.sublayers)])
         else:
-            self.attn = AttentionParams(d, cfg.heads, cfg.head_dim, "own")
+            self.attn = AttentionParams(d, cfg.heads, cfg.head_dim, "own", cfg.qk_norm)
             self.ff = FeedForwardParams(d, cfg.mlp_dim, own_norm=True, tp=cfg.tp, tp_rank=cfg.tp_rank)
 
     def blocks(self):
@@ -396,7 +400,7 @@ class SwinLayer(nn.Module):
                                        eps, cfg.chunk_windows, sp=ctx.sp_exchange if ctx.grid.sp > 1 else None,
                                        rope=ctx.rope(x.device), tp=ctx.tp_exchange if cfg.tp > 1 else None,
                                        keep=keep_from is not None and j >= keep_from,
-                                       min_chunk_bytes=cfg.min_chunk_bytes)
+                                       min_chunk_bytes=cfg.min_chunk_bytes, qk_norm=cfg.qk_norm)
                 if cfg.tp > 1 and ctx.tp_exchange is None:
                     raise RuntimeError("tensor parallelism on CUDA needs StreamContext.tp_exchange (tensor.TPExchange)")
                 rg = None
@@ -406,8 +410,9 @@ class SwinLayer(nn.Module):
                 alloc = None
                 if publish_out and j == len(blocks) - 1:
                     alloc = fused._pool_alloc(ctx.peer_fn)
+                qk = (attn.q_norm.weight, attn.k_norm.weight) if cfg.qk_norm else ()
                 x = fused.run_block(x, m, meta, n1w, attn.to_qkv.weight, attn.wo.weight, n2w,
-                                    ff.w1.weight, ff.w2.weight, rg, alloc)
+                                    ff.w1.weight, ff.w2.weight, rg, alloc, *qk)
             else:
                 m = mod(dt.to(mod.modulation[-1].weight.dtype)) if mod is not None else \
                     self._plain_modulation(ctx.batch, x.device, x.dtype)
@@ -416,7 +421,9 @@ class SwinLayer(nn.Module):
                 p = {"n1": n1w, "to_qkv": attn.to_qkv.weight, "wo": attn.wo.weight, "n2": n2w,
                      "w1": ff.w1.weight, "w2": ff.w2.weight}
                 rope = ctx.rope(x.device)
-                inner = (lambda q_, nw, nl, H, d: O.window_attention(q_, nw, nl, H, d, rope=rope)) if rope else None
+                qk = (attn.q_norm.weight, attn.k_norm.weight, eps) if cfg.qk_norm else None
+                inner = (lambda q_, nw, nl, H, d, qk=qk: O.window_attention(q_, nw, nl, H, d, rope=rope, qk=qk)) \
+                    if rope or qk else None
                 attn = inner
                 if ctx.sp_group is not None and ctx.grid.sp > 1:
                     from ..parallel.sequence import sp_window_attention
@@ -604,7 +611,7 @@ class AerisModel(nn.Module):
         from . import fused
         wins, L = ctx.grid.windows_per_rank, ctx.grid.n_local
         meta = fused.BlockMeta(wins, L, cfg.heads, cfg.head_dim, E.MODE_MOD_THEN_NORM, cfg.eps(x.dtype), cfg.chunk_windows,
-                               min_chunk_bytes=cfg.min_chunk_bytes)
+                               min_chunk_bytes=cfg.min_chunk_bytes, qk_norm=cfg.qk_norm)
         return n_blocks - fused.plan_kept_blocks(meta, x.shape[0] // (wins * L), cfg.dim, cfg.mlp_dim, n_blocks, x.device)
 
     def trunk(self, x: torch.Tensor, dt: torch.Tensor, ctx: StreamContext) -> torch.Tensor:

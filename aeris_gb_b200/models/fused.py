@@ -22,6 +22,7 @@ from torch.autograd import forward_ad
 from ..ops import attention as A
 from ..ops import elementwise as E
 from ..ops import gemm as G
+from ..ops import qk_norm as QN
 from . import block as NB
 
 
@@ -39,6 +40,7 @@ class BlockMeta:
     tp: object | None = None           # parallel.tensor.TPExchange: w1 / w2 are this rank's shards of the MLP weights
     keep: bool = False                 # forward keeps its internals for the backward pass (see plan_kept_blocks)
     min_chunk_bytes: int | None = None  # chunks with fewer bytes of internals are merged; None: MIN_CHUNK_BYTES
+    qk_norm: bool = False              # q and k are normed by head; the weights go beside the block's others
 
     @property
     def chunk_floor(self) -> int:
@@ -140,7 +142,39 @@ def _rope_qk_(qkv: torch.Tensor, meta: BlockMeta, nw: int, inverse: bool = False
     E.rope_qk_(qkv, cos.float().contiguous(), sin.float().contiguous(), meta.L, meta.heads, meta.head_dim, inverse)
 
 
+def _qk_sections(meta: BlockMeta, rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The q and k sections of rows [T, 2 * heads * d or more] as [T, heads, d]."""
+    HD = meta.heads * meta.head_dim
+    return tuple(rows[:, i * HD:(i + 1) * HD].unflatten(1, (meta.heads, meta.head_dim)) for i in (0, 1))
+
+
+def _angles(meta: BlockMeta) -> tuple:
+    return (None, None) if meta.rope is None else tuple(t.float().contiguous() for t in meta.rope)
+
+
+def _normed_qkv(meta: BlockMeta, h1, wqkv, qk, raw, qkv) -> None:
+    """``qkv`` with normed (and rotated) q and k; ``raw`` receives them as the projection gives them, for the backward pass.
+    Two products instead of one, so that neither v nor the raw values are copied."""
+    n = 2 * meta.heads * meta.head_dim
+    G.gemm(h1, wqkv[:n], out=raw)
+    G.gemm(h1, wqkv[n:], out=qkv[:, n:])
+    q_out, k_out = _qk_sections(meta, qkv)
+    QN.qk_norm_fwd(*_qk_sections(meta, raw), *qk, *_angles(meta), eps=meta.eps, q_out=q_out, k_out=k_out)
+
+
+def _check_qk(meta: BlockMeta, qk) -> None:
+    if meta.qk_norm != (qk is not None):
+        raise ValueError("a block with qk_norm takes the weights of both norms, one without takes none")
+    if qk is not None and meta.sp is not None:
+        raise ValueError("norms of q and k are not combined with sequence parallelism")
+
+
 KEPT = ("h1", "qkv", "o", "lse", "x1", "h2", "act", "u")
+KEPT_QK = (*KEPT, "qk")      # with norms of q and k: both as they were before
+
+
+def _qk_shape(T: int, HD: int):
+    return {"qk": ((T, 2 * HD), torch.bfloat16)}
 
 
 def _kept_shapes(T: int, D: int, HD: int, heads: int, F: int) -> dict[str, tuple[tuple[int, ...], torch.dtype]]:
@@ -223,7 +257,7 @@ def plan_kept_blocks(meta: BlockMeta, batch: int, D: int, F: int, n_blocks: int,
     they do not count as free."""
     HD = meta.heads * meta.head_dim
     T = batch * meta.n_win_per_sample * meta.L
-    per_block = kept_bytes(T, D, HD, meta.heads, F)
+    per_block = kept_bytes(T, D, HD, meta.heads, F) + (4 * T * HD if meta.qk_norm else 0)
     step = chunk_step(meta, D, F)
     rows = step * meta.L
     fwd_rows = max(nw for _, _, nw, _ in _forward_spans(meta, batch, step, D, F, False)) * meta.L
@@ -353,7 +387,7 @@ def _chunk_views(bufs: dict[str, torch.Tensor], r0: int, n: int, heads: int):
 
 def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv, wo, wn2, w1, w2,
                   out: torch.Tensor | None = None, gather=None,
-                  kept: dict[str, torch.Tensor] | None = None) -> torch.Tensor:
+                  kept: dict[str, torch.Tensor] | None = None, qk=None) -> torch.Tensor:
     """x: [B * n_win * L, D] bf16 window-major; mod: [B, 6D] fp32 (shift1, scale1, gate1, shift2, scale2, gate2).
 
     ``gather = (table, peer_ptrs, src)``: ``x`` is then an EMPTY buffer in this block's window layout; the first
@@ -361,7 +395,8 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
     re-partition / halo exchange of a shifted layer) and writes them into ``x`` on the way.
 
     ``kept``: full-size buffers (:func:`_kept_shapes`) that receive the block's internals; without it they live in chunk
-    workspaces and are gone afterwards."""
+    workspaces and are gone afterwards. ``qk``: weights of the norms of q and k (``meta.qk_norm``)."""
+    _check_qk(meta, qk)
     T, D = x.shape
     B = mod.shape[0]
     F = w2.shape[1]
@@ -375,7 +410,7 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
     weights = (wn1, wqkv, wo, wn2, w1, w2)
     table = gather[0] if gather is not None else None
     rows = () if out is None else (out,)
-    native = (NB.takes(meta, x, mod, (*weights, *rows)) and NB.fits(meta, x, mod, weights, rows, table=table)
+    native = (qk is None and NB.takes(meta, x, mod, (*weights, *rows)) and NB.fits(meta, x, mod, weights, rows, table=table)
               and (kept is None or type(kept) is FreshKept or _all_whole(kept, T, D, HD, meta.heads, F, x.get_device())))
     if not native:
         NB.refuse_misfits(meta, x, mod, weights, table=table)
@@ -383,6 +418,8 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
         cmax = max(nw for _, _, nw, _ in spans) * meta.L
         tpn = meta.tp.tp if meta.tp is not None else 1   # gathered rows x local features: the same element count
         shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn)
+        if qk is not None:
+            shapes.update(_qk_shape(cmax, HD))
         get = ws.whole if native else ws.get
         chunk_bufs = {k: get(k, *sh, dev) for k, sh in shapes.items() if k != "h2"}
         chunk_bufs["h1"] = chunk_bufs["h2"] = chunk_bufs.pop("h")
@@ -406,9 +443,12 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
         else:
             E.modnorm_fwd(xc, sc1, sh1, wn1, mode=meta.mode, eps=meta.eps, batch=nb, out=h1)
         if meta.sp is None:
-            G.gemm(h1, wqkv, out=qkv)
-            if meta.rope is not None:
-                _rope_qk_(qkv, meta, nw)
+            if qk is not None:
+                _normed_qkv(meta, h1, wqkv, qk, kept["qk"][r0:r0 + n] if kept is not None else chunk_bufs["qk"][:n], qkv)
+            else:
+                G.gemm(h1, wqkv, out=qkv)
+                if meta.rope is not None:
+                    _rope_qk_(qkv, meta, nw)
             A.attn_fwd(qkv, nw, meta.L, meta.heads, meta.head_dim, out=o, lse=lse.view(nw, meta.heads, meta.L))
             oc = o
         else:
@@ -428,10 +468,11 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
 
 def block_backward(x: torch.Tensor, mod: torch.Tensor, dy: torch.Tensor, meta: BlockMeta, wn1, wqkv, wo, wn2, w1, w2,
                    grads: dict[str, torch.Tensor], dx: torch.Tensor | None = None,
-                   kept: dict[str, torch.Tensor] | None = None):
+                   kept: dict[str, torch.Tensor] | None = None, qk=None):
     """Recompute-and-backpropagate; with ``kept`` (what :func:`block_forward` stored) nothing is recomputed and ``kept`` is
-    only read. ``grads`` maps n1, to_qkv, wo, n2, w1, w2 to fp32 accumulators (+=).
+    only read. ``grads`` maps n1, to_qkv, wo, n2, w1, w2 to fp32 accumulators (+=), with ``qk`` qn and kn too.
     Returns (dx bf16, dmod [B, 6D] fp32). ``dx`` may alias ``dy``."""
+    _check_qk(meta, qk)
     T, D = x.shape
     B = mod.shape[0]
     F = w2.shape[1]
@@ -444,15 +485,20 @@ def block_backward(x: torch.Tensor, mod: torch.Tensor, dy: torch.Tensor, meta: B
     tpn = tp.tp if tp is not None else 1
     weights = (wn1, wqkv, wo, wn2, w1, w2)
     rows = (dy,) if dx is None else (dy, dx)
-    native = NB.takes(meta, x, mod, (*weights, *rows), grads.values()) and NB.fits(meta, x, mod, weights, rows, grads)
+    native = qk is None and NB.takes(meta, x, mod, (*weights, *rows), grads.values()) and NB.fits(meta, x, mod, weights, rows, grads)
     if not native:
         NB.refuse_misfits(meta, x, mod, weights, dx, grads)
     get = ws.whole if native else ws.get
     if kept is not None:
-        if not _all_whole(kept, T, D, HD, meta.heads, F, x.get_device()):
+        if qk is not None:
+            kept = _whole_kept(kept, {**_kept_shapes(T, D, HD, meta.heads, F), **_qk_shape(T, HD)}, dev)
+        elif not _all_whole(kept, T, D, HD, meta.heads, F, x.get_device()):
             kept = _whole_kept(kept, _kept_shapes(T, D, HD, meta.heads, F), dev)
     else:
-        chunk_bufs = {k: get(k, *sh, dev) for k, sh in _chunk_shapes(cmax, D, HD, meta.heads, F, tpn).items()}
+        shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn)
+        if qk is not None:
+            shapes.update(_qk_shape(cmax, HD))
+        chunk_bufs = {k: get(k, *sh, dev) for k, sh in shapes.items()}
         chunk_bufs["h1"], act_b = chunk_bufs.pop("h"), chunk_bufs["act"]
     work = {k: get(k, *sh, dev) for k, sh in _grad_shapes(cmax, D, HD, meta.heads, F, tpn).items()}
     if native:
@@ -482,15 +528,19 @@ def block_backward(x: torch.Tensor, mod: torch.Tensor, dy: torch.Tensor, meta: B
             h1, qkv, o, x1, h2, act, lse = _chunk_views(kept, r0, n, meta.heads) if kept is not None else \
                 _chunk_views(chunk_bufs, 0, n, meta.heads)
             lse_c = lse.view(nw, meta.heads, meta.L)
+            raw = (None if qk is None else kept["qk"][r0:r0 + n] if kept is not None else chunk_bufs["qk"][:n])
             oc, du = o, du_b[:n]
             u = kept["u"][r0:r0 + n] if kept is not None else du
             if kept is None:
                 # ---- recompute the chunk's forward internals
                 E.modnorm_fwd(xc, sc1, sh1, wn1, mode=meta.mode, eps=meta.eps, out=h1)
                 if meta.sp is None:
-                    G.gemm(h1, wqkv, out=qkv)
-                    if meta.rope is not None:
-                        _rope_qk_(qkv, meta, nw)
+                    if qk is not None:
+                        _normed_qkv(meta, h1, wqkv, qk, raw, qkv)
+                    else:
+                        G.gemm(h1, wqkv, out=qkv)
+                        if meta.rope is not None:
+                            _rope_qk_(qkv, meta, nw)
                     A.attn_fwd(qkv, nw, meta.L, meta.heads, meta.head_dim, out=o, lse=lse_c)
                 else:
                     oc, sp_state = _sp_attention_fwd(meta, h1, wqkv, nw, keep_local=True)
@@ -529,7 +579,11 @@ def block_backward(x: torch.Tensor, mod: torch.Tensor, dy: torch.Tensor, meta: B
                 G.gemm(dx1[:n], wog, b_t=True, out=d_o[:n])                            # do = (dx1 * g1) @ wo
                 A.attn_bwd(qkv, o, d_o[:n], lse_c, nw, meta.L, meta.heads, meta.head_dim, dqkv=dqkv[:n],
                            delta=delta[:n * meta.heads].view(nw, meta.heads, meta.L))
-                if meta.rope is not None:
+                if qk is not None:
+                    dq, dk = _qk_sections(meta, dqkv[:n])
+                    QN.qk_norm_bwd(dq, dk, *_qk_sections(meta, raw), *qk, *_angles(meta), eps=meta.eps, dq_out=dq, dk_out=dk,
+                                   dwq=grads["qn"], dwk=grads["kn"])
+                elif meta.rope is not None:
                     _rope_qk_(dqkv[:n], meta, nw, inverse=True)
                 dq_c = dqkv[:n]
             else:
@@ -562,22 +616,23 @@ def recorded() -> bool:
             or _tracing_state() is not None)
 
 
-def run_block(x, mod, meta: BlockMeta, wn1, wqkv, wo, wn2, w1, w2, regroup=None, out_alloc=None) -> torch.Tensor:
+def run_block(x, mod, meta: BlockMeta, wn1, wqkv, wo, wn2, w1, w2, regroup=None, out_alloc=None, *qk) -> torch.Tensor:
     """:class:`FusedBlock` where something is recorded, else its forward pass by itself."""
     if recorded():
-        return FusedBlock.apply(x, mod, meta, wn1, wqkv, wo, wn2, w1, w2, regroup, out_alloc)
-    return _block_output(x, mod, meta, (wn1, wqkv, wo, wn2, w1, w2), regroup, out_alloc, None)[1]
+        return FusedBlock.apply(x, mod, meta, wn1, wqkv, wo, wn2, w1, w2, regroup, out_alloc, *qk)
+    return _block_output(x, mod, meta, (wn1, wqkv, wo, wn2, w1, w2), regroup, out_alloc, None, qk)[1]
 
 
-def _block_output(x, mod, meta: BlockMeta, weights, regroup, out_alloc, kept):
+def _block_output(x, mod, meta: BlockMeta, weights, regroup, out_alloc, kept, qk=()):
     """(block input in the block's own window layout, output); see :meth:`FusedBlock.forward`."""
+    more = {"qk": qk} if qk else {}
     out = out_alloc(x.shape[0], x.shape[1], x.dtype) if out_alloc is not None else None
     if regroup is None:
-        return x, block_forward(x, mod.float(), meta, *weights, out=out, kept=kept)
+        return x, block_forward(x, mod.float(), meta, *weights, out=out, kept=kept, **more)
     table_fwd, _, peer_fn = regroup
     peers = peer_fn(x, "fwd") if peer_fn is not None else [x.data_ptr()]
     xg = torch.empty((table_fwd.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
-    return xg, block_forward(xg, mod.float(), meta, *weights, out=out, gather=(table_fwd, peers, x), kept=kept)
+    return xg, block_forward(xg, mod.float(), meta, *weights, out=out, gather=(table_fwd, peers, x), kept=kept, **more)
 
 
 class FusedBlock(torch.autograd.Function):
@@ -585,30 +640,38 @@ class FusedBlock(torch.autograd.Function):
     ``param.main_grad`` (fp32) when the engine provides one, otherwise they are returned to autograd."""
 
     @staticmethod
-    def forward(ctx, x, mod, meta, wn1, wqkv, wo, wn2, w1, w2, regroup=None, out_alloc=None):
+    def forward(ctx, x, mod, meta, wn1, wqkv, wo, wn2, w1, w2, regroup=None, out_alloc=None, *qk):
         """``regroup = (table_fwd, table_bwd, peer_fn)`` fuses the preceding window re-partition into this block: the
         incoming stream ``x`` is in the previous layout (published to the WP peers when ``peer_fn`` is given) and the
         first modulate+norm kernel gathers this block's rows from it. ``out_alloc(rows, cols, dtype)``: where to put the
-        output when the caller knows that it will be re-partitioned next (a peer-readable buffer: no publish copy)."""
+        output when the caller knows that it will be re-partitioned next (a peer-readable buffer: no publish copy). ``qk``:
+        the weights of the norms of q and k, if any."""
         ctx.meta = meta
         ctx.regroup = regroup
         kept = None
         if meta.keep and any(ctx.needs_input_grad):        # a frozen block has no backward pass to keep anything for
             shapes = _kept_shapes(regroup[0].numel() if regroup is not None else x.shape[0], x.shape[1],
                                   meta.heads * meta.head_dim, meta.heads, w2.shape[1])
+            if qk:
+                shapes = {**shapes, **_qk_shape(shapes["qkv"][0][0], meta.heads * meta.head_dim)}
             try:
                 kept = FreshKept({k: torch.empty(shape, dtype=dt, device=x.device) for k, (shape, dt) in shapes.items()})
             except torch.OutOfMemoryError:
                 kept = None            # free in sum but not in pieces of this size: recompute instead
-        x, y = _block_output(x, mod, meta, (wn1, wqkv, wo, wn2, w1, w2), regroup, out_alloc, kept)
-        ctx.save_for_backward(x, mod, wn1, wqkv, wo, wn2, w1, w2, *([kept[k] for k in KEPT] if kept is not None else ()))
+        x, y = _block_output(x, mod, meta, (wn1, wqkv, wo, wn2, w1, w2), regroup, out_alloc, kept, qk)
+        ctx.save_for_backward(x, mod, wn1, wqkv, wo, wn2, w1, w2, *qk,
+                              *([kept[k] for k in (KEPT_QK if qk else KEPT)] if kept is not None else ()))
         return y
 
     @staticmethod
     def backward(ctx, dy):
         x, mod, wn1, wqkv, wo, wn2, w1, w2, *rest = ctx.saved_tensors
-        kept = dict(zip(KEPT, rest)) if rest else None
         params = {"n1": wn1, "to_qkv": wqkv, "wo": wo, "n2": wn2, "w1": w1, "w2": w2}
+        more = {}
+        if ctx.meta.qk_norm:
+            params["qn"], params["kn"], *rest = rest
+            more = {"qk": (params["qn"], params["kn"])}
+        kept = dict(zip(KEPT_QK if more else KEPT, rest)) if rest else None
         grads, ret = {}, {}
         for k, p in params.items():
             mg = getattr(p, "main_grad", None)
@@ -619,7 +682,7 @@ class FusedBlock(torch.autograd.Function):
                 grads[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 ret[k] = grads[k]
         x, dy = x.contiguous(), dy.contiguous()        # a saved-tensor hook may hand back other strides
-        dx, dmod = block_backward(x, mod.float(), dy, ctx.meta, wn1, wqkv, wo, wn2, w1, w2, grads, dx=dy, kept=kept)
+        dx, dmod = block_backward(x, mod.float(), dy, ctx.meta, wn1, wqkv, wo, wn2, w1, w2, grads, dx=dy, kept=kept, **more)
         if ctx.regroup is not None:
             _, table_bwd, peer_fn = ctx.regroup
             peers = peer_fn(dx, "bwd") if peer_fn is not None else [dx.data_ptr()]
@@ -630,9 +693,8 @@ class FusedBlock(torch.autograd.Function):
                     torch.empty((table_bwd.numel(), dx.shape[1]), dtype=dx.dtype, device=dx.device))
             E.gather_rows(table_bwd, peers, back, src_rows=dx.shape[0])
             dx = back
-        out = [ret[k].to(params[k].dtype) if ret[k] is not None else None
-               for k in ("n1", "to_qkv", "wo", "n2", "w1", "w2")]
-        return (dx, dmod.to(mod.dtype), None, *out, None, None)
+        out = [ret[k].to(params[k].dtype) if ret[k] is not None else None for k in params]
+        return (dx, dmod.to(mod.dtype), None, *out[:6], None, None, *out[6:])
 
 
 class GemvLinearFn(torch.autograd.Function):

@@ -95,16 +95,58 @@ def apply_rope_2d(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, inverse
     return out.flatten(-2).to(x.dtype)
 
 
-def window_attention(qkv: torch.Tensor, n_win: int, L: int, heads: int, head_dim: int, rope=None) -> torch.Tensor:
+def window_attention(qkv: torch.Tensor, n_win: int, L: int, heads: int, head_dim: int, rope=None, qk=None) -> torch.Tensor:
     """softmax(q k^T / sqrt(d)) v per window and head, no mask (parallel_swin.py:257-258). qkv: [n_win*L, 3*h*d]
     with columns ordered (q|k|v, head, d) as produced by ``to_qkv`` (model.py:300). ``rope = (cos, sin)`` applies the
     2-D rotary embedding to q and k first (the reference computes it and then attends on the un-rotated tensors,
-    parallel_swin.py:292-294, so parity with it needs ``rope=None``)."""
+    parallel_swin.py:292-294, so parity with it needs ``rope=None``). ``qk = (wq, wk, eps)``: every head's q and k are RMS-normed
+    before that, with weights [head_dim] (absent from the reference)."""
     q, k, v = qkv.view(n_win, L, 3, heads, head_dim).permute(2, 0, 3, 1, 4)
+    if qk is not None:
+        q, k = rms_norm(q, qk[0], qk[2]), rms_norm(k, qk[1], qk[2])
     if rope is not None:
         q, k = apply_rope_2d(q, *rope), apply_rope_2d(k, *rope)
     o = F.scaled_dot_product_attention(q, k, v, is_causal=False)
     return o.permute(0, 2, 1, 3).reshape(n_win * L, heads * head_dim)
+
+
+ORTHO_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalise(x: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> torch.Tensor:
+    """fp32 matrices [.., rows, cols] with their singular values pushed to around 1 by the polynomial a x + b x^3 + c x^5,
+    ``steps`` times, after division by the Frobenius norm. Absent from the reference."""
+    if x.shape[-2] > x.shape[-1]:
+        return orthogonalise(x.mT, steps, eps).mT
+    a, b, c = ORTHO_COEFFICIENTS
+    x = x.float()
+    x = x / x.double().square().sum((-2, -1), keepdim=True).sqrt().clamp_min(eps).float()
+    for _ in range(steps):
+        s = x @ x.mT
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x
+
+
+def orthogonal_step(master, grad, momentum, weights, ema, norm_sq, *, groups, lr, beta, nesterov, weight_decay, scale, grad_scale,
+                    max_norm, ema_beta, steps: int = 5, eps: float = 1e-7, zero_grad: bool = True) -> None:
+    """The optimizer step of :func:`..ops.orthogonalise.orthogonal_step`, matrix by matrix."""
+    clip = 1.0
+    if max_norm > 0 and norm_sq is not None:
+        clip = min(1.0, max_norm / (float(norm_sq.sqrt()) + 1e-6))
+    for rows, cols, offsets in groups:
+        for o in offsets.tolist():
+            sl = slice(o, o + rows * cols)
+            g = torch.nan_to_num(grad[sl] * (grad_scale * clip), nan=0.0, posinf=1e5, neginf=-1e5)
+            momentum[sl] = beta * momentum[sl] + (1 - beta) * g
+            u = beta * momentum[sl] + (1 - beta) * g if nesterov else momentum[sl]
+            x = orthogonalise(u.view(rows, cols), steps, eps).reshape(-1)
+            master[sl] = master[sl] * (1 - lr * weight_decay) - lr * scale * math.sqrt(max(rows, cols)) * x
+            if weights is not None:
+                weights[sl] = master[sl].to(weights.dtype)
+            if ema is not None and ema_beta >= 0:
+                ema[sl] = master[sl].lerp(ema[sl], ema_beta)
+            if zero_grad:
+                grad[sl] = 0
 
 
 def swiglu(u: torch.Tensor) -> torch.Tensor:

@@ -39,7 +39,7 @@ class Evaluations:
     @classmethod
     def prepare(cls, model, c_img, levels: list[float], ctx, plan, slots: int, x_img) -> "Evaluations | None":
         """None where the evaluations have to go one by one: parallel ranks, objectives without a noise level or with a
-        shared embedding, what the native call does not take, anything that watches or replaces a part of the model, and
+        shared embedding, what the native call does not take (norms of q and k too), anything that watches or replaces a part of the model, and
         where all buffers at once do not fit."""
         from . import aeris as A
         cfg, grid, M, D = model.cfg, ctx.grid, plan.geom.B, model.cfg.dim
@@ -49,7 +49,7 @@ class Evaluations:
                 or _hooked(model.layers)
                 or grid.n_ranks != 1 or ctx.peer_fn is not None or cfg.tp != 1 or ctx.batch != M
                 or not (cfg.diffusion and cfg.conditioned and cfg.layerwise_t_emb) or cfg.model_dtype != torch.bfloat16
-                or cfg.data_dtype != torch.float32 or D % 8 or not DF.gemv_ok(M, D) or fused.recorded()
+                or cfg.data_dtype != torch.float32 or cfg.qk_norm or D % 8 or not DF.gemv_ok(M, D) or fused.recorded()
                 or not A.use_fused(x_img)):
             return None
         try:

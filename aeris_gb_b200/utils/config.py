@@ -254,7 +254,7 @@ def model_config(cfg: Config):
         chunk_windows=int(m.get("chunk_windows", 64)), min_chunk_bytes=m.get("min_chunk_bytes"), norm_eps=m.get("norm_eps"),
         shift_layers=m.get("shift_mode", "odd"), diffusion=bool(m.get("diffusion", True)),
         rit=bool(m.get("rit", False)), emb_norm=bool(m.get("emb_norm", False)) and bool(m.get("rit", False)),
-        tp=int(m.get("TP", 1)),
+        tp=int(m.get("TP", 1)), qk_norm=bool(m.get("qk_norm", False)),
         # model.act_ckpt: every block recomputes its internals in the backward pass. Without it the PyTorch path keeps
         # them all, the CUDA path those that fit the free memory
         oracle_checkpoint=bool(m.get("act_ckpt", False)), recompute=bool(m.get("act_ckpt", False)))
@@ -265,8 +265,9 @@ def optim_config(cfg: Config):
     t, o, m = cfg.trainer, cfg.optimizer, cfg.model
     policy = "custom_decay5" if m.get("custom_decay5") else ("custom_decay" if m.get("custom_decay") else "all")
     target = str(o.get("_target_", "torch.optim.AdamW"))
-    if target.rsplit(".", 1)[-1] not in ("AdamW", "Adam"):
-        raise ValueError(f"optimizer._target_ = {target}: the fused update implements Adam / AdamW")
+    family = target.rsplit(".", 1)[-1]
+    if family not in ("AdamW", "Adam", "Muon"):
+        raise ValueError(f"optimizer._target_ = {target}: the fused updates implement Adam / AdamW and Muon")
     if target.endswith(".Adam") and float(o.weight_decay) != 0.0:
         # torch.optim.Adam adds weight_decay * w to the gradient (L2); the fused kernels decay the weights directly
         warnings.warn("optimizer._target_ is torch.optim.Adam with a non-zero weight_decay: the decoupled (AdamW) "
@@ -279,7 +280,11 @@ def optim_config(cfg: Config):
         lr_rampdown_length=int(t.get("lr_rampdown_length", 1)),
         lr_rampdown_ema_min_ratio=float(t.get("lr_rampdown_ema_min_ratio", 1.0)),
         ema_halflife_img=int(t.ema_halflife_kimg * 1000), ema_rampup_ratio=t.get("ema_rampup_ratio", 0.05),
-        use_ema=not bool(m.get("dist_optimizer", False)))
+        use_ema=not bool(m.get("dist_optimizer", False)),
+        # Muon: momentum, nesterov, ns_steps and update_scale for the blocks' matrices, betas and eps for everything else
+        method="muon" if family == "Muon" else "adamw", muon_beta=float(o.get("momentum", 0.95)),
+        muon_nesterov=bool(o.get("nesterov", True)), muon_steps=int(o.get("ns_steps", 5)),
+        muon_scale=float(o.get("update_scale", 0.2)))
 
 
 def diffusion_config(cfg: Config):
