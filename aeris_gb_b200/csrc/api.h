@@ -233,11 +233,11 @@ typedef struct AerisOrthoOut {
 } AerisOrthoOut;
 int aeris_ortho_in(const AerisOrthoIn* a, void* stream);        // two kernels
 int aeris_ortho_out(const AerisOrthoOut* a, void* stream);
-// X: [2, count] matrices d x K, the first `count` the input; S: aeris_ortho_buffers() * count matrices d x d of pitch d rounded
-// up to 64, both fp16. Returns the number of kernels launched, or a negative code. The result is in the half of X that
-// aeris_ortho_updates() changes of side lead to.
+// X: [2, count] matrices d x K, the first `count` the input; S: [aeris_ortho_buffers(), count] matrices d x d of pitch d rounded
+// up to 64, both fp16; 1 to 20 steps. Returns the number of kernels launched, or a negative code. The result is in the half of
+// X that aeris_ortho_updates() changes of side lead to.
 int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, int steps, int* status, void* stream);
-int aeris_ortho_buffers();
+int aeris_ortho_buffers(int d, int K, int steps);
 int aeris_ortho_updates(int d, int K, int steps);
 
 #ifdef __cplusplus

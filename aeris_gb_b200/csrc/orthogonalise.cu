@@ -12,6 +12,7 @@
 // A batch holds matrices whose shorter side is d and whose longer side is K; upright ones are transposed on the way in and
 // out, so that the products see one layout: X [d, K] and symmetric factors [d, d], rows of whole 128 bytes.
 #include "api.h"
+#include "cluster.cuh"
 #include "common.cuh"
 #include "host.h"
 
@@ -21,7 +22,6 @@ namespace aeris {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float NS_SCALE = 512.f;             // stored = NS_SCALE * value, for X and for the [d, d] factors
-constexpr int NS_BUFFERS = 2;                 // [d, d] factors per matrix: S and a I + b S + c S^2
 
 constexpr int NS_PARTS = 128;                 // blocks per matrix that its squares are summed in, at most
 
@@ -334,6 +334,19 @@ __host__ __device__ constexpr uint32_t make_idesc_fp16(int M, int N, int b_mn) {
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Bounded waits that only their own time-out ends. Nothing here waits for another kernel's work, and a status word that is
+// already set keeps results back (`keep`) without two CTAs or roles having to give up at the same place.
+__device__ __forceinline__ bool own_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  if (mbar_wait(bar, parity, nullptr, 0)) return true;
+  if (status) atomicCAS(status, 0, code);
+  return false;
+}
+__device__ __forceinline__ bool own_poll(uint64_t* bar, uint32_t parity, int* status, int code) {
+  if (mbar_wait_poll(bar, parity, nullptr, 0)) return true;
+  if (status) atomicCAS(status, 0, code);
+  return false;
+}
+
 // Tile `t` of one matrix: row by row, or the t-th on and below the diagonal.
 __device__ __forceinline__ void ortho_tile(int t, int sym, int n_tiles, int& ti, int& tj) {
   if (!sym) {
@@ -347,6 +360,54 @@ __device__ __forceinline__ void ortho_tile(int t, int sym, int n_tiles, int& ti,
   tj = t - ti * (ti + 1) / 2;
 }
 
+// One thread's row of a tile: NCOL accumulator columns from `taddr` on are columns col0 .. of row `row`.
+template <int NCOL>
+__device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, uint32_t taddr, int mat, int row, int col0, bool keep,
+                                               bool mirror) {
+  const long long at = mat * p.c_stride;
+  __half* C = p.C + at;
+  const __half* R = p.R ? p.R + at : nullptr;
+#pragma unroll 1
+  for (int c = 0; c < NCOL; c += 32) {
+    const int col = col0 + c;
+    if (col >= p.ldc) break;
+    uint32_t v[32];
+    tmem_ld32(taddr + c, v);
+    tmem_wait_ld();
+    if (!keep || row >= p.M) continue;
+    float f[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
+    if (R) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 w = *reinterpret_cast<const uint4*>(R + static_cast<long long>(row) * p.ldc + col + 8 * j);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 r2 = __half22float2(*reinterpret_cast<const __half2*>(&ww[i]));
+          f[8 * j + 2 * i] += p.beta * r2.x;
+          f[8 * j + 2 * i + 1] += p.beta * r2.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (row == col + j) f[j] += p.gamma;
+    __half2 h[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+    uint4* dst = reinterpret_cast<uint4*>(C + static_cast<long long>(row) * p.ldc + col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[j] = reinterpret_cast<uint4*>(h)[j];
+    if (p.sym && mirror) {                 // the mirror image: for one column after the other, 32 rows side by side
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col + j < p.N) C[static_cast<long long>(col + j) * p.ldc + row] = j & 1 ? __high2half(h[j / 2]) : __low2half(h[j / 2]);
+    }
+  }
+}
+
 template <int B_MN>
 __global__ void __launch_bounds__(OG_THREADS, 1)
 ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const OrthoGemm p) {
@@ -358,12 +419,6 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   uint64_t* tempty_bar = tfull_bar + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  {
-    __shared__ int s_abort;
-    if (threadIdx.x == 0) s_abort = failed(p.status);
-    __syncthreads();
-    if (s_abort) { chain_point(); return; }
-  }
   const int m_tiles = (p.M + OG_TILE - 1) / OG_TILE, n_tiles = (p.N + OG_TILE - 1) / OG_TILE;
   const int per_matrix = p.sym ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles;
   const int total = per_matrix * p.count;
@@ -401,7 +456,7 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         int ti, tj;
         ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
         for (int kb = 0; kb < kb_total; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
+          if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
           uint8_t* sa = smem + stage * OG_STAGE;
           uint8_t* sb = sa + OG_OPERAND;
           mbar_expect_tx(&full_bar[stage], OG_STAGE);
@@ -419,11 +474,11 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       // every stage filled has been consumed, or at least arrived, before the CTA leaves
       for (int s = 0; s < OG_STAGES; ++s) {
         if (ok) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) break;
+          if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) break;
           if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         } else {
           if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
-          if (!mbar_wait(&full_bar[stage], phase, nullptr, 0)) break;
+          if (!own_wait(&full_bar[stage], phase, nullptr, 0)) break;
         }
       }
     }
@@ -434,11 +489,11 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
+        if (!own_wait(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
         const uint32_t tmem_acc = tmem_base + acc * OG_TILE;
         for (int kb = 0; kb < kb_total; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
+          if (!own_wait(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * OG_STAGE), sb = sa + OG_OPERAND;
 #pragma unroll
@@ -455,7 +510,7 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       }
       // the last products have completed before the tensor memory goes back (a stage never filled counts as done)
       if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
-      mbar_wait(&empty_bar[stage], phase, nullptr, 0);
+      own_wait(&empty_bar[stage], phase, nullptr, 0);
     }
   } else {
     const int q = warp & 3;
@@ -466,51 +521,11 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       const int mat = tile / per_matrix;
       int ti, tj;
       ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
-      if (!__all_sync(0xffffffffu, mbar_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
+      if (!__all_sync(0xffffffffu, own_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
       const int row = ti * OG_TILE + q * 32 + lane;
       const uint32_t taddr = tmem_base + acc * OG_TILE + (static_cast<uint32_t>(q * 32) << 16);
-      __half* C = p.C + mat * p.c_stride;
-      const __half* R = p.R ? p.R + mat * p.c_stride : nullptr;
-#pragma unroll 1
-      for (int c = 0; c < OG_TILE; c += 32) {
-        const int col = tj * OG_TILE + c;
-        if (col >= p.ldc) break;
-        uint32_t v[32];
-        tmem_ld32(taddr + c, v);
-        tmem_wait_ld();
-        if (!keep || row >= p.M) continue;
-        float f[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
-        if (R) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 w = *reinterpret_cast<const uint4*>(R + static_cast<long long>(row) * p.ldc + col + 8 * j);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 r2 = __half22float2(*reinterpret_cast<const __half2*>(&ww[i]));
-              f[8 * j + 2 * i] += p.beta * r2.x;
-              f[8 * j + 2 * i + 1] += p.beta * r2.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (row == col + j) f[j] += p.gamma;
-        __half2 h[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-        uint4* dst = reinterpret_cast<uint4*>(C + static_cast<long long>(row) * p.ldc + col);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j] = reinterpret_cast<uint4*>(h)[j];
-        if (p.sym && ti != tj) {             // the mirror image: for one column after the other, 32 rows side by side
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < p.N) C[static_cast<long long>(col + j) * p.ldc + row] = j & 1 ? __high2half(h[j / 2]) : __low2half(h[j / 2]);
-        }
-      }
+      ortho_epilogue<OG_TILE>(p, taddr, mat, row, tj * OG_TILE, keep, ti != tj);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[acc]);
@@ -523,14 +538,175 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   if (warp == 1) tmem_dealloc(tmem_base, 2 * OG_TILE);
 }
 
+// The same on CTA pairs: a cluster of two computes a 256 x 256 tile, each CTA staging its 128 rows of A and half of B's columns
+// (csrc/gemm2.cu has the scheme). Per product a third less shared memory and L2 traffic than a 128 x 128 tile needs half of.
+constexpr int OP_BM = 128, OP_BN = 256, OP_STAGES = 6;
+constexpr int OP_OPERAND = 128 * OG_BK * 2;
+constexpr int OP_STAGE = 2 * OP_OPERAND;
+constexpr int OP_SMEM = OP_STAGES * OP_STAGE + 256 + 1024;
+
+template <int B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(OG_THREADS, 1)
+ortho_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const OrthoGemm p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + OP_STAGES * OP_STAGE);      // the leader's: both CTAs' bytes
+  uint64_t* empty_bar = full_bar + OP_STAGES;
+  uint64_t* tfull_bar = empty_bar + OP_STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;                                               // the leader's: both CTAs' warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const int m_tiles = (p.M + 2 * OP_BM - 1) / (2 * OP_BM), n_tiles = (p.N + OP_BN - 1) / OP_BN;
+  const int per_matrix = p.sym ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles;
+  const int total = per_matrix * p.count;
+  const int kb_total = (p.K + OG_BK - 1) / OG_BK;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    for (int s = 0; s < OP_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 8);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc2(tmem_slot, 2 * OP_BN);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_point();
+
+  if (warp == 0) {
+    if (elect_one_sync()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < total && ok; tile += clusters) {
+        const int mat = tile / per_matrix;
+        int ti, tj;
+        ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
+        const int m0 = ti * 2 * OP_BM + crank * OP_BM, n0 = tj * OP_BN + crank * (OP_BN / 2);
+        for (int kb = 0; kb < kb_total; ++kb) {
+          if (!own_poll(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
+          uint8_t* sa = smem + stage * OP_STAGE;
+          uint8_t* sb = sa + OP_OPERAND;
+          if (crank == 0) mbar_expect_tx(&full_bar[stage], 2 * OP_STAGE);
+          const uint32_t fb = map_to_cta(smem_u32(&full_bar[stage]), 0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            tma_load_3d_pair(sa + j * 8192, &tmap_a, fb, kb * OG_BK, m0 + j * 64, p.a0 + mat);
+            if (B_MN)
+              tma_load_3d_pair(sb + j * 8192, &tmap_b, fb, n0 + j * 64, kb * OG_BK, p.b0 + mat);
+            else
+              tma_load_3d_pair(sb + j * 8192, &tmap_b, fb, kb * OG_BK, n0 + j * 64, p.b0 + mat);
+          }
+          if (++stage == OP_STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // tiles that the issuer did not take, of both CTAs (a stage never filled counts as there)
+      for (int s = 0; s < OP_STAGES && !ok && crank == 0; ++s) {
+        if (--stage < 0) { stage = OP_STAGES - 1; phase ^= 1; }
+        if (!own_poll(&full_bar[stage], phase, nullptr, 0)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (crank == 0 && elect_one_sync()) {
+      constexpr uint32_t idesc = make_idesc_fp16(2 * OP_BM, OP_BN, B_MN);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < total && ok; tile += clusters) {
+        if (!own_poll(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
+        tc_fence_after();
+        const uint32_t tmem_acc = tmem_base + acc * OP_BN;
+        for (int kb = 0; kb < kb_total; ++kb) {
+          if (!own_poll(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * OP_STAGE), sb = sa + OP_OPERAND;
+#pragma unroll
+          for (int kk = 0; kk < OG_BK / 16; ++kk)
+            umma2_ss(tmem_acc, make_smem_desc(sa + kk * 32, 0, 1024),
+                     B_MN ? make_smem_desc(sb + kk * 2048, 8192, 1024) : make_smem_desc(sb + kk * 32, 0, 1024), idesc,
+                     kb > 0 || kk > 0);
+          tc_commit2_mc(&empty_bar[stage], 0x3);
+          if (++stage == OP_STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tc_commit2_mc(&tfull_bar[acc], 0x3);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      // the last products have completed before the CTAs leave
+      if (--stage < 0) { stage = OP_STAGES - 1; phase ^= 1; }
+      own_poll(&empty_bar[stage], phase, nullptr, 0);
+    }
+  } else {
+    const int q = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const bool keep = !failed(p.status);
+    const uint32_t leader_tempty = map_to_cta(smem_u32(&tempty_bar[0]), 0);
+    for (int tile = cluster; tile < total; tile += clusters) {
+      const int mat = tile / per_matrix;
+      int ti, tj;
+      ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
+      if (!__all_sync(0xffffffffu, own_poll(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
+      tc_fence_after();
+      const int row = ti * 2 * OP_BM + crank * OP_BM + q * 32 + lane;
+      ortho_epilogue<OP_BN>(p, tmem_base + acc * OP_BN + (static_cast<uint32_t>(q * 32) << 16), mat, row, tj * OP_BN, keep,
+                            ti != tj);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(leader_tempty + acc * 8);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc2(tmem_base, 2 * OP_BN);
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 namespace {
 
 int pitch(int n) { return (n + 63) / 64 * 64; }
 bool on_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+// How the steps are grouped. One step by itself is a Gram matrix of X, its square and an update of X: in units of d^3, with
+// symmetric products at half and r = K / d, 3 r + 1. Two steps can share the update: the Gram matrix alone goes on (S <- P S P
+// with P = a I + b S + c S^2, all symmetric and commuting) and X is multiplied by the product of both P at the end: 3 r + 5
+// instead of 6 r + 2, the less for every oblong matrix. Groups of three would cost 3 r + 9, but a Gram matrix's rounding error
+// (2^-12 of its norm) grows by a^2 a step in directions that hold little of the norm, and is not small against them any more:
+// error on 127 x 640 gradients with half as much noise as signal 6e-4 by single steps and in groups (2, 2, 1), 1.8e-3 in (3, 2); on
+// 320 x 2000 5.5e-4, 6.5e-4, 9e-4; a group of five diverges. Below GROUP_FROM rows single steps: the products are shorter than
+// their launches, of which groups have two more, and a handful of rows does not average the roundings (5 x 9: up to three times
+// the error of single steps).
+constexpr int GROUP_FROM = 256;
+struct Groups {
+  int n, size[20];
+};
+Groups groups_of(int d, int K, int steps) {
+  Groups g = {0, {}};
+  for (int left = steps, most = K > d && d >= GROUP_FROM ? 2 : 1; left > 0; left -= g.size[g.n++]) g.size[g.n] = left < most ? left : most;
+  return g;
+}
+int buffers_of(const Groups& g) { return g.size[0] == 1 ? 2 : 4; }
+
+enum Factor { F_S, F_P0, F_T, F_P1 };    // where the [d, d] factors of a batch are
+
 struct Products {
-  CUtensorMap x, s;                           // 2 * count matrices X, NS_BUFFERS * count factors
+  CUtensorMap x, s;                           // 2 * count matrices X, and all factors
   __half *X, *S;
   int count, d, K;
   int* status;
@@ -539,14 +715,15 @@ struct Products {
 
   long long x_stride() const { return static_cast<long long>(d) * pitch(K); }
   long long s_stride() const { return static_cast<long long>(d) * pitch(d); }
+  __half* at(int f) const { return S + f * count * s_stride(); }
 
   template <int B_MN>
   void launch(const CUtensorMap& a, const CUtensorMap& b, OrthoGemm p) {
     if (rc) return;
     static bool configured = false;
-    auto kern = ortho_gemm_kernel<B_MN>;
     if (!configured) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess) {
+      if (cudaFuncSetAttribute(ortho_gemm_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
+          cudaFuncSetAttribute(ortho_gemm_pair_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OP_SMEM) != cudaSuccess) {
         rc = -20;
         return;
       }
@@ -554,38 +731,58 @@ struct Products {
     }
     p.count = count;
     p.status = status;
-    const long long m = (p.M + OG_TILE - 1) / OG_TILE, n = (p.N + OG_TILE - 1) / OG_TILE;
-    const long long tiles = (p.sym ? m * (m + 1) / 2 : m * n) * count;
-    if (tiles > 0x7fffffff) {
+    auto tiles_of = [&](int tile) {
+      const long long m = (p.M + tile - 1) / tile, n = (p.N + tile - 1) / tile;
+      return (p.sym ? m * (m + 1) / 2 : m * n) * count;
+    };
+    const long long small = tiles_of(OG_TILE), large = tiles_of(2 * OG_TILE);
+    if (small > 0x7fffffff) {
       rc = -5;
       return;
     }
-    rc = launch_chained(kern, static_cast<int>(tiles < num_sms() ? tiles : num_sms()), OG_THREADS, OG_SMEM, stream, a, b, p);
+    // rounds of tiles; a pair's tile has twice the work per multiprocessor of a single one's and takes about as long
+    const int sms = num_sms(), pairs = sms / 2;
+    if ((large + pairs - 1) / pairs <= (small + sms - 1) / sms)
+      rc = launch_chained(ortho_gemm_pair_kernel<B_MN>, 2 * static_cast<int>(large < pairs ? large : pairs), OG_THREADS, OP_SMEM,
+                          stream, a, b, p);
+    else
+      rc = launch_chained(ortho_gemm_kernel<B_MN>, static_cast<int>(small < sms ? small : sms), OG_THREADS, OG_SMEM, stream, a, b,
+                          p);
     ++launches;
   }
-  // factor `out` = alpha * (factor i) (factor j) + beta * (factor r) + gamma I, in values
-  void factor(int out, int i, int j, float alpha, int r = -1, float beta = 0.f, float gamma = 0.f) {
+  void product(int out, int i, int j) {       // factor `out` = (factor i) (factor j)
     OrthoGemm p{};
     p.M = p.N = p.K = d;
     p.sym = 1;
     p.a0 = i * count;
     p.b0 = j * count;
-    p.C = S + out * count * s_stride();
-    p.R = r < 0 ? nullptr : S + r * count * s_stride();
+    p.C = at(out);
     p.c_stride = s_stride();
     p.ldc = pitch(d);
-    p.alpha = alpha / NS_SCALE;
-    p.beta = beta;
-    p.gamma = gamma * NS_SCALE;
+    p.alpha = 1.f / NS_SCALE;
     launch<0>(s, s, p);
   }
-  void gram(int out, int from) {              // factor `out` = X X^T
+  void polynomial(int out) {                  // factor `out` = a I + b S + c S^2
+    OrthoGemm p{};
+    p.M = p.N = p.K = d;
+    p.sym = 1;
+    p.a0 = p.b0 = F_S * count;
+    p.C = at(out);
+    p.R = at(F_S);
+    p.c_stride = s_stride();
+    p.ldc = pitch(d);
+    p.alpha = NS_C / NS_SCALE;
+    p.beta = NS_B;
+    p.gamma = NS_A * NS_SCALE;
+    launch<0>(s, s, p);
+  }
+  void gram(int from) {                       // S = X X^T
     OrthoGemm p{};
     p.M = p.N = d;
     p.K = K;
     p.sym = 1;
     p.a0 = p.b0 = from * count;
-    p.C = S + out * count * s_stride();
+    p.C = at(F_S);
     p.c_stride = s_stride();
     p.ldc = pitch(d);
     p.alpha = 1.f / NS_SCALE;
@@ -603,6 +800,16 @@ struct Products {
     p.alpha = 1.f / NS_SCALE;
     launch<1>(s, x, p);
   }
+  void group(int from, int steps) {           // one or two steps on X number `from`, into the other one
+    gram(from);
+    polynomial(F_P0);
+    if (steps == 1) return update(from, F_P0);
+    product(F_T, F_P0, F_S);
+    product(F_S, F_T, F_P0);                  // S after the first step
+    polynomial(F_P1);
+    product(F_T, F_P1, F_P0);
+    update(from, F_T);
+  }
 };
 
 }  // namespace
@@ -610,9 +817,13 @@ struct Products {
 
 using namespace aeris;
 
-extern "C" int aeris_ortho_buffers() { return NS_BUFFERS; }
+extern "C" int aeris_ortho_buffers(int d, int K, int steps) {
+  return d <= 0 || K < d || steps < 1 || steps > 20 ? -1 : buffers_of(groups_of(d, K, steps));
+}
 
-extern "C" int aeris_ortho_updates(int d, int K, int steps) { return steps; }
+extern "C" int aeris_ortho_updates(int d, int K, int steps) {
+  return d <= 0 || K < d || steps < 1 || steps > 20 ? -1 : groups_of(d, K, steps).n;
+}
 
 extern "C" int aeris_ortho_in(const AerisOrthoIn* a, void* stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
@@ -644,7 +855,8 @@ extern "C" int aeris_ortho_in(const AerisOrthoIn* a, void* stream_) {
 }
 
 extern "C" int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, int steps, int* status, void* stream) {
-  if (!X || !S || !status || count <= 0 || d <= 0 || K < d || steps < 0) return -1;
+  if (!X || !S || !status || count <= 0 || d <= 0 || K < d || steps < 1 || steps > 20) return -1;
+  const Groups groups = groups_of(d, K, steps);
   Products p;
   p.X = reinterpret_cast<__half*>(X);
   p.S = reinterpret_cast<__half*>(S);
@@ -654,12 +866,8 @@ extern "C" int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, in
   p.status = status;
   p.stream = reinterpret_cast<cudaStream_t>(stream);
   if (const int r = make_tmap_3d_fp16(&p.x, X, K, d, 2ull * count, pitch(K), 64)) return r;
-  if (const int r = make_tmap_3d_fp16(&p.s, S, d, d, static_cast<uint64_t>(NS_BUFFERS) * count, pitch(d), 64)) return r;
-  for (int k = 0; k < steps; ++k) {
-    p.gram(0, k & 1);
-    p.factor(1, 0, 0, NS_C, 0, NS_B, NS_A);
-    p.update(k & 1, 1);
-  }
+  if (const int r = make_tmap_3d_fp16(&p.s, S, d, d, static_cast<uint64_t>(buffers_of(groups)) * count, pitch(d), 64)) return r;
+  for (int k = 0; k < groups.n; ++k) p.group(k & 1, groups.size[k]);
   return p.rc ? p.rc : p.launches;
 }
 

@@ -44,31 +44,31 @@ def _pitch(n: int) -> int:
 class _Batch:
     """Workspaces of ``count`` matrices of shorter side ``d`` and longer side ``k``, and the products on them."""
 
-    def __init__(self, count: int, d: int, k: int, device):
-        self.count, self.d, self.k = count, d, k
+    def __init__(self, count: int, d: int, k: int, steps: int, device):
+        self.count, self.d, self.k, self.steps = count, d, k, steps
         self.x_size, self.half = d * _pitch(k), count * d * _pitch(k)
-        s = _l.lib().aeris_ortho_buffers() * count * d * _pitch(d)
+        s = _l.lib().aeris_ortho_buffers(d, k, steps) * count * d * _pitch(d)
         self.x = torch.empty(2 * self.half, dtype=torch.float16, device=device)
         self.s = torch.empty(s, dtype=torch.float16, device=device)
         self.partial = torch.empty(count * PARTS, dtype=torch.float64, device=device)
 
     @staticmethod
-    def most(d: int, k: int) -> int:
+    def most(d: int, k: int, steps: int) -> int:
         """Matrices of one batch."""
-        per = 2 * (2 * d * _pitch(k) + _l.lib().aeris_ortho_buffers() * d * _pitch(d))
+        per = 2 * (2 * d * _pitch(k) + _l.lib().aeris_ortho_buffers(d, k, steps) * d * _pitch(d))
         return max(1, min(MAX_COUNT, WORKSPACE_BYTES // per))
 
     def load(self, first: int, a: _In) -> None:
         a.X, a.partial = self.x.data_ptr() + 2 * first * self.x_size, self.partial.data_ptr()
         _l.check(_l.lib().aeris_ortho_in(ctypes.byref(a), _l.stream_ptr()), "aeris_ortho_in", kernels=2)
 
-    def iterate(self, steps: int) -> None:
+    def iterate(self) -> None:
         """Leaves the result in ``self.result``."""
         lib = _l.lib()
-        rc = lib.aeris_ortho_iterate(_l.ptr(self.x), _l.ptr(self.s), self.count, self.d, self.k, steps, _l.ptr(_l.status_word()),
-                                     _l.stream_ptr())
+        rc = lib.aeris_ortho_iterate(_l.ptr(self.x), _l.ptr(self.s), self.count, self.d, self.k, self.steps,
+                                     _l.ptr(_l.status_word()), _l.stream_ptr())
         _l.check(min(rc, 0), "aeris_ortho_iterate", kernels=max(rc, 0))
-        self.result = self.x.data_ptr() + 2 * self.half * (lib.aeris_ortho_updates(self.d, self.k, steps) & 1)
+        self.result = self.x.data_ptr() + 2 * self.half * (lib.aeris_ortho_updates(self.d, self.k, self.steps) & 1)
 
     def store(self, first: int, a: _Out) -> None:
         a.X = self.result + 2 * first * self.x_size
@@ -118,14 +118,14 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, eps: float = 1e-7, out: to
     d, k = min(rows, cols), max(rows, cols)
     with _l.on_device(x.device):
         status = _l.status_word().data_ptr()
-        most = _Batch.most(d, k)
+        most = _Batch.most(d, k, steps)
         for i in range(0, count, most):
             n = min(most, count - i)
-            b = _Batch(n, d, k, x.device)
+            b = _Batch(n, d, k, steps, x.device)
             a = _In(x=xs.data_ptr() + i * xs.stride(0) * xs.element_size(), bf16=xs.dtype == torch.bfloat16, stride=xs.stride(0),
                     rows=rows, cols=cols, ld=_row_pitch(xs), count=n, eps=eps, status=status)
             b.load(0, a)
-            b.iterate(steps)
+            b.iterate()
             b.store(0, _Out(out=os.data_ptr() + i * os.stride(0) * 2, stride=os.stride(0), rows=rows, cols=cols,
                             ld=_row_pitch(os), count=n, status=status))
     return out
@@ -141,11 +141,11 @@ def _check_flat(name: str, t: torch.Tensor, like: torch.Tensor, dtype: torch.dty
 def _step_batches(d, k, parts, master, grad, momentum, weights, ema, norm_sq, status, steps, settings, rates) -> None:
     """All matrices of sides ``d`` and ``k``, upright and wide ones in the same products, as many at a time as fit a batch."""
     todo = [(rows, cols, off.data_ptr(), 0, off.numel()) for rows, cols, off in parts]
-    left, most = sum(n for *_, n in todo), _Batch.most(d, k)
+    left, most = sum(n for *_, n in todo), _Batch.most(d, k, steps)
     batch, taken = None, []
     while left:
         if batch is None:
-            batch, room = _Batch(min(most, left), d, k, master.device), min(most, left)
+            batch, room = _Batch(min(most, left), d, k, steps, master.device), min(most, left)
             first, taken = 0, []
         rows, cols, table, start, n = todo.pop(0)
         m = min(n, room)
@@ -158,7 +158,7 @@ def _step_batches(d, k, parts, master, grad, momentum, weights, ema, norm_sq, st
         if m < n:
             todo.insert(0, (rows, cols, table, start + m, n - m))
         if not room:
-            batch.iterate(steps)
+            batch.iterate()
             for i, where in taken:
                 batch.store(i, _Out(master=master.data_ptr(), weights=0 if weights is None else weights.data_ptr(),
                                     ema=0 if ema is None else ema.data_ptr(), **where, **rates))
