@@ -203,42 +203,33 @@ typedef struct AerisQkNorm {
 int aeris_qk_norm_fwd(const AerisQkNorm* a, void* stream);
 int aeris_qk_norm_bwd(const AerisQkNorm* a, void* stream);      // returns the number of kernels launched, or a negative code
 
-// Orthogonalisation of matrices (csrc/orthogonalise.cu; mirrored in ops/orthogonalise.py). A batch: `count` matrices of rows x
-// cols with row pitch ld, matrix i at element offsets[i] (device memory, int64, ascending, no two overlapping, inside [0,
-// numel): else the status word is set and the matrix left out) or, with offsets null, at i * stride. X: fp16 workspace, one
-// [min(rows, cols), longer side rounded up to 64] per matrix. At most 65535 matrices a call.
-typedef struct AerisOrthoIn {
-  const void* x;                    // fp32 or bf16, or null with grad and momentum (flat fp32 buffers, offsets needed)
-  float *grad, *momentum;
-  const double* norm_sq;            // as aeris_adamw
+// Orthogonalisation of matrices (csrc/orthogonalise.cu; mirrored in ops/orthogonalise.py): a batch of up to ORTHO_GROUPS groups
+// whose matrices have one shorter side and at most two different longer ones. Matrix i of a group has rows x cols elements
+// with row pitch ld and lies at element offsets[i] (device memory, int64, ascending, no two overlapping, inside [0, numel):
+// else the status word is set and the matrix left out) or, with offsets null, at i * stride.
+#define ORTHO_GROUPS 4
+typedef struct AerisOrthoGroup {
   const void* offsets;
-  void* X;
-  double* partial;                  // [count, 128]
+  long long stride, out_stride;     // out_stride, ld_out: where the results of `out` lie
+  int rows, cols, ld, ld_out, count, behind;    // behind: offsets[-1] is the matrix before the first one
+  float rate;                       // master * decay - rate * result
+} AerisOrthoGroup;
+typedef struct AerisOrtho {
+  AerisOrthoGroup group[ORTHO_GROUPS];
+  const void* x;                    // a tensor, fp32 or bf16, and its bf16 results
+  void* out;
+  float *grad, *momentum, *master, *ema;        // or flat buffers of an optimizer (x and out null); ema may be null
+  void* weights;                    // bf16, may be null
+  const double* norm_sq;            // as aeris_adamw
+  void* work;                       // workspace from a 1024-byte boundary on
   int* status;
   double eps;
-  long long stride, numel;
-  int rows, cols, ld, count, behind, bf16, nesterov, zero_grad;   // behind: offsets[-1] is the matrix before the first one
-  float beta, grad_scale, max_norm;
-} AerisOrthoIn;
-typedef struct AerisOrthoOut {
-  const void* X;
-  void* out;                        // bf16, or null with master
-  float *master, *ema;              // flat fp32 buffers; ema may be null
-  void* weights;                    // flat bf16 buffer or null
-  const void* offsets;
-  int* status;
-  long long stride, numel;
-  int rows, cols, ld, count, behind;
-  float decay, rate, ema_beta;      // master * decay - rate * X
-} AerisOrthoOut;
-int aeris_ortho_in(const AerisOrthoIn* a, void* stream);        // two kernels
-int aeris_ortho_out(const AerisOrthoOut* a, void* stream);
-// X: [2, count] matrices d x K, the first `count` the input; S: [aeris_ortho_buffers(), count] matrices d x d of pitch d rounded
-// up to 64, both fp16; 1 to 20 steps. Returns the number of kernels launched, or a negative code. The result is in the half of
-// X that aeris_ortho_updates() changes of side lead to.
-int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, int steps, int* status, void* stream);
-int aeris_ortho_buffers(int d, int K, int steps);
-int aeris_ortho_updates(int d, int K, int steps);
+  long long numel, work_bytes;
+  int groups, steps, bf16, nesterov, zero_grad; // 1 to 20 steps
+  float beta, grad_scale, max_norm, decay, ema_beta;
+} AerisOrtho;
+long long aeris_ortho_work_bytes(const AerisOrtho* a);          // of its groups and steps, or a negative code
+int aeris_orthogonalise(const AerisOrtho* a, void* stream);     // the number of kernels launched, or a negative code
 
 #ifdef __cplusplus
 }

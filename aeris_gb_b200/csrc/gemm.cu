@@ -275,16 +275,17 @@ int make_tmap_heads32_bf16(CUtensorMap* out, const void* base, int d, int heads,
 }
 
 int make_tmap_3d_fp16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint64_t count, uint64_t ld,
-                      uint32_t box_rows) {
+                      uint32_t box_cols, uint32_t box_rows) {
   PFN_encodeTiled enc = get_encode();
   if (!enc) return -10;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || ((ld * 2) & 15)) return -11;
   cuuint64_t dims[3] = {inner, rows, count};
   cuuint64_t strides[2] = {ld * 2, rows * ld * 2};
-  cuuint32_t box[3] = {64, box_rows, 1};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -12;
 }

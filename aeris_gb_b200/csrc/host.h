@@ -16,9 +16,10 @@ int make_tmap_heads_bf16(CUtensorMap* out, const void* base, int d, int heads, i
 // The same dims with box {32, 1, box_rows, 1} and the 64-byte swizzle: for tiled stores of 32 columns.
 int make_tmap_heads32_bf16(CUtensorMap* out, const void* base, int d, int heads, int tokens, int windows, uint64_t ld,
                            uint32_t box_rows);
-// 3-D fp16 map with 128-byte swizzle: `count` matrices of `rows` rows of pitch `ld`, one behind the other; box {64, box_rows, 1}.
+// 3-D fp16 map: `count` matrices of `rows` rows of pitch `ld`, one behind the other; box {box_cols, box_rows, 1} of 64 columns
+// with the 128-byte swizzle or 32 with the 64-byte one.
 int make_tmap_3d_fp16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint64_t count, uint64_t ld,
-                      uint32_t box_rows);
+                      uint32_t box_cols, uint32_t box_rows);
 int num_sms();
 // Slices of an accumulating product's reduction over `kb_total` blocks of 64: see gemm.cu.
 int choose_k_splits(int tiles, int kb_total, int units, int most, int want);

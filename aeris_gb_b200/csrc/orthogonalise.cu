@@ -24,29 +24,52 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float NS_SCALE = 512.f;             // stored = NS_SCALE * value, for X and for the [d, d] factors
 
 constexpr int NS_PARTS = 128;                 // blocks per matrix that its squares are summed in, at most
+constexpr int NS_GROUPS = ORTHO_GROUPS, NS_CLASSES = 2;
 
 // ------------------------------------------------------------------------------------------------ in and out
-// Where matrix i of a batch lies: element offset offsets[i] (checked against [0, numel) and for ascending order) or i * stride;
-// rows of pitch ld.
-struct MatrixAt {
+// `count` matrices of one shape, from number `first` of their table on. Matrix i lies at element offsets[i] (checked against
+// [0, numel) and for ascending order) or i * stride, with rows of pitch ld; its X [d, K] at x + i * x_stride with pitch ldx.
+struct OrthoGroup {
   const long long* offsets;
-  long long stride, numel;
-  int rows, cols, ld, behind;                 // behind: offsets[-1] is the matrix before the first one
-  int aligned;                                // four elements from the buffers' starts on are one vector
-  int* status;
-  __device__ bool vectors(long long at) const { return aligned && cols % 4 == 0 && ld % 4 == 0 && at % 4 == 0; }
-  __device__ bool find(int i, long long& at) const {
-    if (!offsets) {
-      at = i * stride;
-      return true;
-    }
-    at = offsets[i];
-    const long long size = static_cast<long long>(rows) * cols;
-    if (at >= 0 && at + size <= numel && ((i == 0 && !behind) || at >= offsets[i - 1] + size)) return true;
-    if (threadIdx.x == 0) atomicCAS(status, 0, ERR_BOUNDS);
-    return false;
-  }
+  long long stride, x_stride;
+  __half* x;
+  double* partial;                            // [parts] per matrix
+  int rows, cols, ld, ldx, behind, first, count, blocks, parts;      // behind: offsets[-1] is the matrix before the first one
+  float rate;
 };
+struct OrthoGroups {
+  OrthoGroup g[NS_GROUPS];
+  long long numel;
+  int n, aligned;                             // aligned: four elements from the buffers' starts on are one vector
+  int* status;
+};
+
+struct OrthoPlace {
+  int group, matrix, block;                   // matrix: its number in the table
+  long long at;
+  bool found, four;                           // four: rows are whole vectors of four
+};
+__device__ __forceinline__ OrthoPlace ortho_place(const OrthoGroups& a) {
+  OrthoPlace p;
+  int b = blockIdx.x;
+  p.group = 0;
+  while (p.group + 1 < a.n && b >= a.g[p.group].count * a.g[p.group].blocks) b -= a.g[p.group].count * a.g[p.group].blocks, ++p.group;
+  const OrthoGroup& g = a.g[p.group];
+  p.matrix = g.first + b / g.blocks;
+  p.block = b % g.blocks;
+  p.found = true;
+  if (!g.offsets) {
+    p.at = p.matrix * g.stride;
+  } else {
+    p.at = g.offsets[p.matrix];
+    const long long size = static_cast<long long>(g.rows) * g.cols;
+    p.found = p.at >= 0 && p.at + size <= a.numel &&
+              ((p.matrix == 0 && !g.behind) || p.at >= g.offsets[p.matrix - 1] + size);
+    if (!p.found && threadIdx.x == 0) atomicCAS(a.status, 0, ERR_BOUNDS);
+  }
+  p.four = a.aligned && g.cols % 4 == 0 && g.ld % 4 == 0 && p.at % 4 == 0;
+  return p;
+}
 
 // What is orthogonalised: a tensor (fp32 or bf16), or the momentum of an optimizer.
 struct OrthoInput {
@@ -84,11 +107,12 @@ __device__ __forceinline__ float4 in_value4(const OrthoInput& in, long long e) {
 // optimizer's momentum is brought up to date on the way: M = beta M + (1 - beta) g; what is summed is M, or beta M + (1 -
 // beta) g with nesterov.
 template <bool STEP>
-__global__ void __launch_bounds__(256) ortho_squares_kernel(const MatrixAt m, const OrthoInput in, double* __restrict__ partial) {
+__global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a, const OrthoInput in) {
   chain_point();
-  long long at;
+  const OrthoPlace p = ortho_place(a);
+  const OrthoGroup& m = a.g[p.group];
   double sum = 0;
-  if (m.find(blockIdx.y, at)) {
+  if (p.found) {
     const float gs = STEP ? step_scale(in) : 0.f;
     auto value = [&](float g, float& mom) {
       g = clean(g * gs);
@@ -97,12 +121,11 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const MatrixAt m, co
     };
     const bool flat = m.ld == m.cols;
     const long long n = static_cast<long long>(m.rows) * m.cols;
-    const long long step = static_cast<long long>(gridDim.x) * 256, first = blockIdx.x * 256ll + threadIdx.x;
-    const bool four = m.vectors(at);
-    if (four) {
+    const long long step = m.blocks * 256ll, first = p.block * 256ll + threadIdx.x;
+    if (p.four) {
       const int per_row = m.cols / 4;
       for (long long v = first; v < n / 4; v += step) {
-        const long long e = flat ? at + 4 * v : at + v / per_row * m.ld + 4 * (v % per_row);
+        const long long e = flat ? p.at + 4 * v : p.at + v / per_row * m.ld + 4 * (v % per_row);
         float4 u;
         if (STEP) {
           const float4 g = *reinterpret_cast<const float4*>(in.grad + e);
@@ -117,7 +140,7 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const MatrixAt m, co
       }
     } else {
       for (long long v = first; v < n; v += step) {
-        const long long e = flat ? at + v : at + v / m.cols * m.ld + v % m.cols;
+        const long long e = flat ? p.at + v : p.at + v / m.cols * m.ld + v % m.cols;
         float u;
         if (STEP) {
           float mo = in.momentum[e];
@@ -136,24 +159,23 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const MatrixAt m, co
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 8; ++i) sum += red[i];
-    partial[blockIdx.y * static_cast<long long>(gridDim.x) + blockIdx.x] = sum;
+    m.partial[p.matrix * static_cast<long long>(m.parts) + p.block] = sum;
   }
 }
 
-// Normed, scaled and rounded to fp16 into X [d, K] (pitch ldx), through shared memory where the matrix is upright: one 64 x 64
-// tile per block. An optimizer's value is computed again from gradient and momentum, which were read a moment before.
-template <bool STEP, bool UPRIGHT>
-__global__ void __launch_bounds__(256) ortho_pack_kernel(const MatrixAt m, const OrthoInput in, const double* __restrict__ partial,
-                                                         int parts, double eps, __half* __restrict__ X, long long x_stride,
-                                                         int ldx) {
-  __shared__ float tile[UPRIGHT ? 64 : 1][65];
+// Normed, scaled and rounded to fp16 into X [d, K], through shared memory where the matrix is upright: one 64 x 64 tile per
+// block. An optimizer's value is computed again from gradient and momentum, which were read a moment before.
+template <bool STEP>
+__global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, const OrthoInput in, double eps) {
+  __shared__ float tile[64][65];
   __shared__ float s_scale;
   chain_point();
-  long long at;
-  if (!m.find(blockIdx.y, at)) return;
+  const OrthoPlace p = ortho_place(a);
+  const OrthoGroup& m = a.g[p.group];
+  if (!p.found) return;
   if (threadIdx.x < 32) {
     double sum = 0;
-    for (int i = threadIdx.x; i < parts; i += 32) sum += partial[blockIdx.y * static_cast<long long>(parts) + i];
+    for (int i = threadIdx.x; i < m.parts; i += 32) sum += m.partial[p.matrix * static_cast<long long>(m.parts) + i];
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const double norm = sqrt(sum);
     if (threadIdx.x == 0) s_scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
@@ -161,10 +183,10 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const MatrixAt m, const
   __syncthreads();
   const float scale = s_scale, gs = STEP ? step_scale(in) : 0.f;
   const int tiles_c = (m.cols + 63) / 64;
-  const int r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
+  const int r0 = p.block / tiles_c * 64, c0 = p.block % tiles_c * 64;
   const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
-  X += blockIdx.y * x_stride;
-  const bool four = m.vectors(at);
+  __half* X = m.x + p.matrix * m.x_stride;
+  const bool upright = m.rows > m.cols;
   auto value = [&](float g, float mom) {
     g = clean(g * gs);
     return scale * (in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom);
@@ -174,8 +196,8 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const MatrixAt m, const
     const int r = r0 + tr + 16 * k, c = c0 + tc;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (r < m.rows && c < m.cols) {
-      const long long e = at + static_cast<long long>(r) * m.ld + c;
-      if (four) {
+      const long long e = p.at + static_cast<long long>(r) * m.ld + c;
+      if (p.four) {
         if (STEP) {
           const float4 g = *reinterpret_cast<const float4*>(in.grad + e);
           const float4 mo = *reinterpret_cast<const float4*>(in.momentum + e);
@@ -198,23 +220,23 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const MatrixAt m, const
         }
       }
     }
-    if (UPRIGHT) {
+    if (upright) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) tile[tr + 16 * k][tc + j] = v[j];
-    } else if (r < m.rows && c < ldx) {
+    } else if (r < m.rows && c < m.ldx) {
       __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
-      *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * ldx + c) = *reinterpret_cast<uint2*>(h);
+      *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * m.ldx + c) = *reinterpret_cast<uint2*>(h);
     }
   }
-  if (UPRIGHT) {
+  if (upright) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = c0 + tr + 16 * k, c = r0 + tc;          // row and column of X
-      if (r < m.cols && c < ldx) {
+      if (r < m.cols && c < m.ldx) {
         __half2 h[2] = {__floats2half2_rn(tile[tc][tr + 16 * k], tile[tc + 1][tr + 16 * k]),
                         __floats2half2_rn(tile[tc + 2][tr + 16 * k], tile[tc + 3][tr + 16 * k])};
-        *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * ldx + c) = *reinterpret_cast<uint2*>(h);
+        *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * m.ldx + c) = *reinterpret_cast<uint2*>(h);
       }
     }
   }
@@ -225,78 +247,80 @@ struct OrthoOutput {
   __nv_bfloat16* out;
   float *master, *ema;                        // optimizer: master set
   __nv_bfloat16* weights;                     // may be null
-  float decay, rate, ema_beta;                // master * decay - rate * X; ema_beta < 0: no running average
+  float decay, ema_beta;                      // master * decay - rate * X; ema_beta < 0: no running average
 };
 
-template <bool STEP, bool UPRIGHT>
-__global__ void __launch_bounds__(256) ortho_finish_kernel(const MatrixAt m, const OrthoOutput o, const __half* __restrict__ X,
-                                                           long long x_stride, int ldx, const int* status) {
-  __shared__ float tile[UPRIGHT ? 64 : 1][65];
+__device__ __forceinline__ void load_x4(const __half* p, float (&v)[4]) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+
+template <bool STEP>
+__global__ void __launch_bounds__(256) ortho_finish_kernel(const OrthoGroups a, const OrthoOutput o) {
+  __shared__ float tile[64][65];
   chain_point();
-  long long at;
-  if (!m.find(blockIdx.y, at) || failed(status)) return;      // what a kernel that gave up left behind is not applied
+  const OrthoPlace p = ortho_place(a);
+  const OrthoGroup& m = a.g[p.group];
+  if (!p.found || failed(a.status)) return;   // what a kernel that gave up left behind is not applied
   const int tiles_c = (m.cols + 63) / 64;
-  const int r0 = blockIdx.x / tiles_c * 64, c0 = blockIdx.x % tiles_c * 64;
+  const int r0 = p.block / tiles_c * 64, c0 = p.block % tiles_c * 64;
   const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
-  X += blockIdx.y * x_stride;
-  if (UPRIGHT) {
+  const __half* X = m.x + p.matrix * m.x_stride;
+  const bool upright = m.rows > m.cols;
+  if (upright) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = c0 + tr + 16 * k, c = r0 + tc;
-      if (r < m.cols && c < ldx) {
-        const uint2 w = *reinterpret_cast<const uint2*>(X + static_cast<long long>(r) * ldx + c);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-        tile[tc][tr + 16 * k] = a.x; tile[tc + 1][tr + 16 * k] = a.y;
-        tile[tc + 2][tr + 16 * k] = b.x; tile[tc + 3][tr + 16 * k] = b.y;
+      if (r < m.cols && c < m.ldx) {
+        float v[4];
+        load_x4(X + static_cast<long long>(r) * m.ldx + c, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tile[tc + j][tr + 16 * k] = v[j];
       }
     }
     __syncthreads();
   }
-  const bool four = m.vectors(at);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int r = r0 + tr + 16 * k, c = c0 + tc;
     if (r >= m.rows || c >= m.cols) continue;
-    const long long e = at + static_cast<long long>(r) * m.ld + c;
+    const long long e = p.at + static_cast<long long>(r) * m.ld + c;
     float v[4];
-    if (UPRIGHT) {
+    if (upright) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = tile[tr + 16 * k][tc + j];
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(X + static_cast<long long>(r) * ldx + c);
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+      load_x4(X + static_cast<long long>(r) * m.ldx + c, v);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= 1.f / NS_SCALE;
     if (!STEP) {
-      if (four) {
+      if (p.four) {
         *reinterpret_cast<uint2*>(o.out + e) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
       } else {
         for (int j = 0; j < 4 && c + j < m.cols; ++j) o.out[e + j] = __float2bfloat16_rn(v[j]);
       }
       continue;
     }
-    if (four) {
+    if (p.four) {
       const float4 p4 = *reinterpret_cast<const float4*>(o.master + e);
-      const float p[4] = {p4.x * o.decay - o.rate * v[0], p4.y * o.decay - o.rate * v[1], p4.z * o.decay - o.rate * v[2],
-                          p4.w * o.decay - o.rate * v[3]};
-      *reinterpret_cast<float4*>(o.master + e) = make_float4(p[0], p[1], p[2], p[3]);
-      if (o.weights) *reinterpret_cast<uint2*>(o.weights + e) = make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
+      const float w[4] = {p4.x * o.decay - m.rate * v[0], p4.y * o.decay - m.rate * v[1], p4.z * o.decay - m.rate * v[2],
+                          p4.w * o.decay - m.rate * v[3]};
+      *reinterpret_cast<float4*>(o.master + e) = make_float4(w[0], w[1], w[2], w[3]);
+      if (o.weights) *reinterpret_cast<uint2*>(o.weights + e) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
       if (o.ema && o.ema_beta >= 0.f) {
-        float4 a = *reinterpret_cast<const float4*>(o.ema + e);
-        a.x = p[0] + o.ema_beta * (a.x - p[0]); a.y = p[1] + o.ema_beta * (a.y - p[1]);
-        a.z = p[2] + o.ema_beta * (a.z - p[2]); a.w = p[3] + o.ema_beta * (a.w - p[3]);
-        *reinterpret_cast<float4*>(o.ema + e) = a;
+        float4 x = *reinterpret_cast<const float4*>(o.ema + e);
+        x.x = w[0] + o.ema_beta * (x.x - w[0]); x.y = w[1] + o.ema_beta * (x.y - w[1]);
+        x.z = w[2] + o.ema_beta * (x.z - w[2]); x.w = w[3] + o.ema_beta * (x.w - w[3]);
+        *reinterpret_cast<float4*>(o.ema + e) = x;
       }
     } else {
       for (int j = 0; j < 4 && c + j < m.cols; ++j) {
-        const float p = o.master[e + j] * o.decay - o.rate * v[j];
-        o.master[e + j] = p;
-        if (o.weights) o.weights[e + j] = __float2bfloat16_rn(p);
-        if (o.ema && o.ema_beta >= 0.f) o.ema[e + j] = p + o.ema_beta * (o.ema[e + j] - p);
+        const float w = o.master[e + j] * o.decay - m.rate * v[j];
+        o.master[e + j] = w;
+        if (o.weights) o.weights[e + j] = __float2bfloat16_rn(w);
+        if (o.ema && o.ema_beta >= 0.f) o.ema[e + j] = w + o.ema_beta * (o.ema[e + j] - w);
       }
     }
   }
@@ -305,22 +329,38 @@ __global__ void __launch_bounds__(256) ortho_finish_kernel(const MatrixAt m, con
 // ------------------------------------------------------------------------------------------------ products
 // C = alpha A B^T + beta R + gamma I for every matrix of a batch (B stored [K, N] with B_MN); fp16 in and out, fp32 sums.
 // `sym`: the result is symmetric, only tiles on and below the diagonal are computed and the others are their mirror images.
-// One CTA per 128 x 128 tile at a time: a TMA producer, an issuer of tcgen05.mma, four epilogue warps, two accumulators.
+// A batch has up to two classes of matrices, of longer sides of their own, so that all matrices with d rows share a launch.
+//
+// Two kernels of one scheme, a TMA producer, an issuer of tcgen05.mma, eight epilogue warps (two for the 32 rows of tensor memory
+// each can read, with half of the columns) and two accumulators: 128 x 128 tiles on single CTAs, and 256 x 256 tiles on CTA
+// pairs, each CTA staging its 128 rows of A and half of B's columns (csrc/gemm2.cu has the scheme), which need half the shared
+// memory and L2 traffic per product. Results leave by 32 x 32 pieces through shared memory as tiled stores, their mirror images
+// transposed by pairs of lanes on the way: with 2-byte stores of the mirror image the epilogue of a 256 x 256 tile took twice as
+// long as its products (252 tiles of 1536: 55 us, 31 of which are products).
+struct OrthoClass {
+  int tiles, count, N, K;                     // tiles per matrix
+  int a0, b0, c0;                             // first matrix of the class in the tensor maps of A, B and C
+};
 struct OrthoGemm {
-  int M, N, K, count, sym;
-  int a0, b0;                                 // first matrix of the batch in the operands' tensor maps
-  __half* C;
-  const __half* R;                            // null, or laid out like C
-  long long c_stride;
-  int ldc;
+  OrthoClass cls[NS_CLASSES];
+  int total, M, sym;                          // tiles in all
+  const __half* R;                            // null, or [matrices, M] rows of pitch ldr
+  long long r_stride;
+  int ldr;
   float alpha, beta, gamma;
   int* status;
 };
+struct OrthoMaps {
+  CUtensorMap a[NS_CLASSES], b[NS_CLASSES], c[NS_CLASSES];
+};
 
-constexpr int OG_TILE = 128, OG_BK = 64, OG_STAGES = 6, OG_THREADS = 192;
-constexpr int OG_OPERAND = OG_TILE * OG_BK * 2;
+constexpr int OG_BK = 64, OG_STAGES = 5, OG_EPI_WARPS = 8, OG_THREADS = 64 + 32 * OG_EPI_WARPS;
+constexpr int OG_OPERAND = 128 * OG_BK * 2;   // of one CTA, single or in a pair
 constexpr int OG_STAGE = 2 * OG_OPERAND;
-constexpr int OG_SMEM = OG_STAGES * OG_STAGE + 256 + 1024;
+constexpr int OG_PIECE = 32 * 32 * 2;         // a 32 x 32 piece of C; two and their mirror images per epilogue warp
+constexpr int OG_OUT = OG_STAGES * OG_STAGE + 256;
+constexpr int OG_SMEM = (OG_OUT + 1023) / 1024 * 1024 + OG_EPI_WARPS * 4 * OG_PIECE + 1024;
+static_assert(OG_SMEM <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
@@ -328,6 +368,12 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
           smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* smem_src, int c0, int c1, int c2) {   // no group yet
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 __host__ __device__ constexpr uint32_t make_idesc_fp16(int M, int N, int b_mn) {      // as make_idesc_bf16, formats 0 = fp16
   return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
@@ -347,9 +393,17 @@ __device__ __forceinline__ bool own_poll(uint64_t* bar, uint32_t parity, int* st
   return false;
 }
 
-// Tile `t` of one matrix: row by row, or the t-th on and below the diagonal.
-__device__ __forceinline__ void ortho_tile(int t, int sym, int n_tiles, int& ti, int& tj) {
-  if (!sym) {
+// Tile `t` of the launch: class, matrix in it, and the tile's place, row by row or on and below the diagonal.
+template <int TILE>
+__device__ __forceinline__ void ortho_tile(const OrthoGemm& p, int t, int& cls, int& mat, int& ti, int& tj) {
+  const int n0 = p.cls[0].tiles * p.cls[0].count;
+  cls = t >= n0;
+  t -= cls ? n0 : 0;
+  const int per = cls ? p.cls[1].tiles : p.cls[0].tiles;
+  mat = t / per;
+  t -= mat * per;
+  if (!p.sym) {
+    const int n_tiles = ((cls ? p.cls[1].N : p.cls[0].N) + TILE - 1) / TILE;
     ti = t / n_tiles;
     tj = t - ti * n_tiles;
     return;
@@ -360,57 +414,87 @@ __device__ __forceinline__ void ortho_tile(int t, int sym, int n_tiles, int& ti,
   tj = t - ti * (ti + 1) / 2;
 }
 
-// One thread's row of a tile: NCOL accumulator columns from `taddr` on are columns col0 .. of row `row`.
+// A warp's 32 rows (from row0 on) of NCOL accumulator columns from `taddr` on, which are columns col0 .. of matrix `mat` of C.
+// A piece's row of 64 bytes is swizzled by 16-byte chunks (64-byte swizzle of the tensor maps); in the mirror image lane l holds
+// rows l & ~1 and l | 1 of column 2 j + (l & 1).
 template <int NCOL>
-__device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, uint32_t taddr, int mat, int row, int col0, bool keep,
-                                               bool mirror) {
-  const long long at = mat * p.c_stride;
-  __half* C = p.C + at;
-  const __half* R = p.R ? p.R + at : nullptr;
+__device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtensorMap* cmap, uint8_t* stage, uint32_t taddr, int mat,
+                                               int r_mat, int row0, int col0, int N, bool keep, bool mirror, int lane,
+                                               int& pieces) {
+  const int row = row0 + lane;
+  const __half* R = p.R && row < p.M ? p.R + r_mat * p.r_stride + static_cast<long long>(row) * p.ldr : nullptr;
+  uint4 r[4] = {};
+  auto fetch = [&](int col) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const uint4*>(R + col + 8 * j);
+  };
+  if (R && col0 < p.ldr) fetch(col0);
 #pragma unroll 1
-  for (int c = 0; c < NCOL; c += 32) {
+  for (int c = 0; c < NCOL && col0 + c < N; c += 32) {
     const int col = col0 + c;
-    if (col >= p.ldc) break;
     uint32_t v[32];
     tmem_ld32(taddr + c, v);
     tmem_wait_ld();
-    if (!keep || row >= p.M) continue;
     float f[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
     if (R) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 w = *reinterpret_cast<const uint4*>(R + static_cast<long long>(row) * p.ldc + col + 8 * j);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 r2 = __half22float2(*reinterpret_cast<const __half2*>(&ww[i]));
+          const float2 r2 = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
           f[8 * j + 2 * i] += p.beta * r2.x;
           f[8 * j + 2 * i + 1] += p.beta * r2.y;
         }
       }
+      if (c + 32 < NCOL && col + 32 < p.ldr) fetch(col + 32);
     }
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (row == col + j) f[j] += p.gamma;
-    __half2 h[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-    uint4* dst = reinterpret_cast<uint4*>(C + static_cast<long long>(row) * p.ldc + col);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dst[j] = reinterpret_cast<uint4*>(h)[j];
-    if (p.sym && mirror) {                 // the mirror image: for one column after the other, 32 rows side by side
+    if (p.gamma != 0.f) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (col + j < p.N) C[static_cast<long long>(col + j) * p.ldc + row] = j & 1 ? __high2half(h[j / 2]) : __low2half(h[j / 2]);
+        if (row == col + j) f[j] += p.gamma;
     }
+    uint32_t h[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const __half2 x = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+      h[j] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    uint8_t* piece = stage + (pieces & 1) * 2 * OG_PIECE;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the piece before the last has left
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(piece + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+    if (mirror) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, h[j], 1);
+        const uint32_t t = lane & 1 ? __byte_perm(other, h[j], 0x7632) : __byte_perm(h[j], other, 0x5410);
+        const int rr = 2 * j + (lane & 1);
+        *reinterpret_cast<uint32_t*>(piece + OG_PIECE + rr * 64 + (((lane >> 3) ^ (j & 3)) << 4) + (lane & 6) * 2) = t;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (keep && row0 < p.M) {
+        tma_store_3d(cmap, piece, col, row0, mat);
+        if (mirror) tma_store_3d(cmap, piece + OG_PIECE, row0, col, mat);
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    __syncwarp();
+    ++pieces;
   }
 }
 
 template <int B_MN>
-__global__ void __launch_bounds__(OG_THREADS, 1)
-ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const OrthoGemm p) {
+__global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p) {
+  constexpr int TILE = 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + OG_STAGES * OG_STAGE);
@@ -419,25 +503,19 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   uint64_t* tempty_bar = tfull_bar + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m_tiles = (p.M + OG_TILE - 1) / OG_TILE, n_tiles = (p.N + OG_TILE - 1) / OG_TILE;
-  const int per_matrix = p.sym ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles;
-  const int total = per_matrix * p.count;
-  const int kb_total = (p.K + OG_BK - 1) / OG_BK;
   if (threadIdx.x == 0) {
-    prefetch_tmap(&tmap_a);
-    prefetch_tmap(&tmap_b);
     for (int s = 0; s < OG_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 4);
+      mbar_init(&tempty_bar[a], OG_EPI_WARPS);
     }
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * OG_TILE);
+    tmem_alloc(tmem_slot, 2 * TILE);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -451,10 +529,12 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const int mat = tile / per_matrix;
-        int ti, tj;
-        ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
+      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x) {
+        int cls, mat, ti, tj;
+        ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+        const CUtensorMap *ta = cls ? &maps.a[1] : &maps.a[0], *tb = cls ? &maps.b[1] : &maps.b[0];
+        const int ma = mat + (cls ? p.cls[1].a0 : p.cls[0].a0), mb = mat + (cls ? p.cls[1].b0 : p.cls[0].b0);
+        const int kb_total = ((cls ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
         for (int kb = 0; kb < kb_total; ++kb) {
           if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
           uint8_t* sa = smem + stage * OG_STAGE;
@@ -462,36 +542,32 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           mbar_expect_tx(&full_bar[stage], OG_STAGE);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            tma_load_3d(sa + j * 8192, &tmap_a, &full_bar[stage], kb * OG_BK, ti * OG_TILE + j * 64, p.a0 + mat);
+            tma_load_3d(sa + j * 8192, ta, &full_bar[stage], kb * OG_BK, ti * TILE + j * 64, ma);
             if (B_MN)
-              tma_load_3d(sb + j * 8192, &tmap_b, &full_bar[stage], tj * OG_TILE + j * 64, kb * OG_BK, p.b0 + mat);
+              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], tj * TILE + j * 64, kb * OG_BK, mb);
             else
-              tma_load_3d(sb + j * 8192, &tmap_b, &full_bar[stage], kb * OG_BK, tj * OG_TILE + j * 64, p.b0 + mat);
+              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], kb * OG_BK, tj * TILE + j * 64, mb);
           }
           if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      // every stage filled has been consumed, or at least arrived, before the CTA leaves
-      for (int s = 0; s < OG_STAGES; ++s) {
-        if (ok) {
-          if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) break;
-          if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
-        } else {
-          if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
-          if (!own_wait(&full_bar[stage], phase, nullptr, 0)) break;
-        }
+      // tiles that the issuer did not take (a stage never filled counts as there)
+      for (int s = 0; s < OG_STAGES && !ok; ++s) {
+        if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
+        if (!mbar_wait(&full_bar[stage], phase, nullptr, 0)) break;
       }
     }
   } else if (warp == 1) {
     if (elect_one_sync()) {
-      constexpr uint32_t idesc = make_idesc_fp16(OG_TILE, OG_TILE, B_MN);
+      constexpr uint32_t idesc = make_idesc_fp16(TILE, TILE, B_MN);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x) {
+        const int kb_total = ((tile >= p.cls[0].tiles * p.cls[0].count ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
         if (!own_wait(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
-        const uint32_t tmem_acc = tmem_base + acc * OG_TILE;
+        const uint32_t tmem_acc = tmem_base + acc * TILE;
         for (int kb = 0; kb < kb_total; ++kb) {
           if (!own_wait(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
@@ -510,73 +586,63 @@ ortho_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       }
       // the last products have completed before the tensor memory goes back (a stage never filled counts as done)
       if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
-      own_wait(&empty_bar[stage], phase, nullptr, 0);
+      mbar_wait(&empty_bar[stage], phase, nullptr, 0);
     }
   } else {
-    const int q = warp & 3;
-    int acc = 0;
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    uint8_t* out = smem + (OG_OUT + 1023) / 1024 * 1024 + (warp - 2) * 4 * OG_PIECE;
+    int acc = 0, pieces = 0;
     uint32_t acc_phase = 0;
     const bool keep = !failed(p.status);
-    for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-      const int mat = tile / per_matrix;
-      int ti, tj;
-      ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
+    for (int tile = blockIdx.x; tile < p.total; tile += gridDim.x) {
+      int cls, mat, ti, tj;
+      ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
       if (!__all_sync(0xffffffffu, own_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
-      const int row = ti * OG_TILE + q * 32 + lane;
-      const uint32_t taddr = tmem_base + acc * OG_TILE + (static_cast<uint32_t>(q * 32) << 16);
-      ortho_epilogue<OG_TILE>(p, taddr, mat, row, tj * OG_TILE, keep, ti != tj);
+      ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
+                               tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
+                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), mat, ti * TILE + q * 32, tj * TILE + part * (TILE / 2),
+                               cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[acc]);
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, 2 * OG_TILE);
+  if (warp == 1) tmem_dealloc(tmem_base, 2 * TILE);
 }
-
-// The same on CTA pairs: a cluster of two computes a 256 x 256 tile, each CTA staging its 128 rows of A and half of B's columns
-// (csrc/gemm2.cu has the scheme). Per product a third less shared memory and L2 traffic than a 128 x 128 tile needs half of.
-constexpr int OP_BM = 128, OP_BN = 256, OP_STAGES = 6;
-constexpr int OP_OPERAND = 128 * OG_BK * 2;
-constexpr int OP_STAGE = 2 * OP_OPERAND;
-constexpr int OP_SMEM = OP_STAGES * OP_STAGE + 256 + 1024;
 
 template <int B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(OG_THREADS, 1)
-ortho_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const OrthoGemm p) {
+ortho_gemm_pair_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p) {
+  constexpr int TILE = 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + OP_STAGES * OP_STAGE);      // the leader's: both CTAs' bytes
-  uint64_t* empty_bar = full_bar + OP_STAGES;
-  uint64_t* tfull_bar = empty_bar + OP_STAGES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + OG_STAGES * OG_STAGE);      // the leader's: both CTAs' bytes
+  uint64_t* empty_bar = full_bar + OG_STAGES;
+  uint64_t* tfull_bar = empty_bar + OG_STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;                                               // the leader's: both CTAs' warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = cluster_ctarank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
-  const int m_tiles = (p.M + 2 * OP_BM - 1) / (2 * OP_BM), n_tiles = (p.N + OP_BN - 1) / OP_BN;
-  const int per_matrix = p.sym ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles;
-  const int total = per_matrix * p.count;
-  const int kb_total = (p.K + OG_BK - 1) / OG_BK;
   if (threadIdx.x == 0) {
-    prefetch_tmap(&tmap_a);
-    prefetch_tmap(&tmap_b);
-    for (int s = 0; s < OP_STAGES; ++s) {
+    for (int s = 0; s < OG_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 8);
+      mbar_init(&tempty_bar[a], 2 * OG_EPI_WARPS);
     }
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc2(tmem_slot, 2 * OP_BN);
+    tmem_alloc2(tmem_slot, 2 * TILE);
     tmem_relinquish2();
   }
   tc_fence_before();
@@ -591,90 +657,95 @@ ortho_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = cluster; tile < total && ok; tile += clusters) {
-        const int mat = tile / per_matrix;
-        int ti, tj;
-        ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
-        const int m0 = ti * 2 * OP_BM + crank * OP_BM, n0 = tj * OP_BN + crank * (OP_BN / 2);
+      for (int tile = cluster; tile < p.total && ok; tile += clusters) {
+        int cls, mat, ti, tj;
+        ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+        const CUtensorMap *ta = cls ? &maps.a[1] : &maps.a[0], *tb = cls ? &maps.b[1] : &maps.b[0];
+        const int ma = mat + (cls ? p.cls[1].a0 : p.cls[0].a0), mb = mat + (cls ? p.cls[1].b0 : p.cls[0].b0);
+        const int kb_total = ((cls ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
+        const int m0 = ti * TILE + crank * 128, n0 = tj * TILE + crank * 128;
         for (int kb = 0; kb < kb_total; ++kb) {
           if (!own_poll(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
-          uint8_t* sa = smem + stage * OP_STAGE;
-          uint8_t* sb = sa + OP_OPERAND;
-          if (crank == 0) mbar_expect_tx(&full_bar[stage], 2 * OP_STAGE);
+          uint8_t* sa = smem + stage * OG_STAGE;
+          uint8_t* sb = sa + OG_OPERAND;
+          if (crank == 0) mbar_expect_tx(&full_bar[stage], 2 * OG_STAGE);
           const uint32_t fb = map_to_cta(smem_u32(&full_bar[stage]), 0);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            tma_load_3d_pair(sa + j * 8192, &tmap_a, fb, kb * OG_BK, m0 + j * 64, p.a0 + mat);
+            tma_load_3d_pair(sa + j * 8192, ta, fb, kb * OG_BK, m0 + j * 64, ma);
             if (B_MN)
-              tma_load_3d_pair(sb + j * 8192, &tmap_b, fb, n0 + j * 64, kb * OG_BK, p.b0 + mat);
+              tma_load_3d_pair(sb + j * 8192, tb, fb, n0 + j * 64, kb * OG_BK, mb);
             else
-              tma_load_3d_pair(sb + j * 8192, &tmap_b, fb, kb * OG_BK, n0 + j * 64, p.b0 + mat);
+              tma_load_3d_pair(sb + j * 8192, tb, fb, kb * OG_BK, n0 + j * 64, mb);
           }
-          if (++stage == OP_STAGES) { stage = 0; phase ^= 1; }
+          if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         }
       }
       // tiles that the issuer did not take, of both CTAs (a stage never filled counts as there)
-      for (int s = 0; s < OP_STAGES && !ok && crank == 0; ++s) {
-        if (--stage < 0) { stage = OP_STAGES - 1; phase ^= 1; }
-        if (!own_poll(&full_bar[stage], phase, nullptr, 0)) break;
+      for (int s = 0; s < OG_STAGES && !ok && crank == 0; ++s) {
+        if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
+        if (!mbar_wait_poll(&full_bar[stage], phase, nullptr, 0)) break;
       }
     }
   } else if (warp == 1) {
     if (crank == 0 && elect_one_sync()) {
-      constexpr uint32_t idesc = make_idesc_fp16(2 * OP_BM, OP_BN, B_MN);
+      constexpr uint32_t idesc = make_idesc_fp16(TILE, TILE, B_MN);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = cluster; tile < total && ok; tile += clusters) {
+      for (int tile = cluster; tile < p.total && ok; tile += clusters) {
+        const int kb_total = ((tile >= p.cls[0].tiles * p.cls[0].count ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
         if (!own_poll(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
-        const uint32_t tmem_acc = tmem_base + acc * OP_BN;
+        const uint32_t tmem_acc = tmem_base + acc * TILE;
         for (int kb = 0; kb < kb_total; ++kb) {
           if (!own_poll(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * OP_STAGE), sb = sa + OP_OPERAND;
+          const uint32_t sa = smem_u32(smem + stage * OG_STAGE), sb = sa + OG_OPERAND;
 #pragma unroll
           for (int kk = 0; kk < OG_BK / 16; ++kk)
             umma2_ss(tmem_acc, make_smem_desc(sa + kk * 32, 0, 1024),
                      B_MN ? make_smem_desc(sb + kk * 2048, 8192, 1024) : make_smem_desc(sb + kk * 32, 0, 1024), idesc,
                      kb > 0 || kk > 0);
           tc_commit2_mc(&empty_bar[stage], 0x3);
-          if (++stage == OP_STAGES) { stage = 0; phase ^= 1; }
+          if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
         tc_commit2_mc(&tfull_bar[acc], 0x3);
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
       // the last products have completed before the CTAs leave
-      if (--stage < 0) { stage = OP_STAGES - 1; phase ^= 1; }
-      own_poll(&empty_bar[stage], phase, nullptr, 0);
+      if (--stage < 0) { stage = OG_STAGES - 1; phase ^= 1; }
+      mbar_wait_poll(&empty_bar[stage], phase, nullptr, 0);
     }
   } else {
-    const int q = warp & 3;
-    int acc = 0;
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    uint8_t* out = smem + (OG_OUT + 1023) / 1024 * 1024 + (warp - 2) * 4 * OG_PIECE;
+    int acc = 0, pieces = 0;
     uint32_t acc_phase = 0;
     const bool keep = !failed(p.status);
     const uint32_t leader_tempty = map_to_cta(smem_u32(&tempty_bar[0]), 0);
-    for (int tile = cluster; tile < total; tile += clusters) {
-      const int mat = tile / per_matrix;
-      int ti, tj;
-      ortho_tile(tile - mat * per_matrix, p.sym, n_tiles, ti, tj);
+    for (int tile = cluster; tile < p.total; tile += clusters) {
+      int cls, mat, ti, tj;
+      ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
       if (!__all_sync(0xffffffffu, own_poll(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
-      const int row = ti * 2 * OP_BM + crank * OP_BM + q * 32 + lane;
-      ortho_epilogue<OP_BN>(p, tmem_base + acc * OP_BN + (static_cast<uint32_t>(q * 32) << 16), mat, row, tj * OP_BN, keep,
-                            ti != tj);
+      ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
+                               tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
+                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), mat, ti * TILE + crank * 128 + q * 32,
+                               tj * TILE + part * (TILE / 2), cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(leader_tempty + acc * 8);
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc2(tmem_base, 2 * OP_BN);
+  if (warp == 1) tmem_dealloc2(tmem_base, 2 * TILE);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -703,102 +774,180 @@ Groups groups_of(int d, int K, int steps) {
 }
 int buffers_of(const Groups& g) { return g.size[0] == 1 ? 2 : 4; }
 
-enum Factor { F_S, F_P0, F_T, F_P1 };    // where the [d, d] factors of a batch are
+enum Factor { F_S, F_P0, F_T, F_P1 };         // where the [d, d] factors of a batch are
+
+// Workspace of a batch: partial sums, both X of every class, the factors.
+struct Layout {
+  int d, count, classes, K[NS_CLASSES], members[NS_CLASSES], group_class[NS_GROUPS], group_first[NS_GROUPS];
+  Groups steps;
+  long long x_at[NS_CLASSES], s_at, bytes;
+  long long x_stride(int c) const { return static_cast<long long>(d) * pitch(K[c]); }
+  long long s_stride() const { return static_cast<long long>(d) * pitch(d); }
+  int fill(const AerisOrtho& a);
+};
+int Layout::fill(const AerisOrtho& a) {
+  if (a.groups < 1 || a.groups > NS_GROUPS || a.steps < 1 || a.steps > 20) return -1;
+  d = count = classes = 0;
+  for (int i = 0; i < a.groups; ++i) {
+    const AerisOrthoGroup& g = a.group[i];
+    if (g.rows < 1 || g.cols < 1 || g.count < 1 || g.count > (1 << 20) || g.ld < g.cols) return -2;
+    const int shorter = g.rows < g.cols ? g.rows : g.cols, longer = g.rows < g.cols ? g.cols : g.rows;
+    if (i && shorter != d) return -3;
+    d = shorter;
+    int c = 0;
+    while (c < classes && K[c] != longer) ++c;
+    if (c == NS_CLASSES) return -4;
+    if (c == classes) K[classes] = longer, members[classes++] = 0;
+    group_class[i] = c;
+    group_first[i] = members[c];
+    members[c] += g.count;
+    count += g.count;
+  }
+  if (classes == 2 && K[0] < K[1]) {          // the longer tiles first: they leave the shorter tail
+    int t = K[0];
+    K[0] = K[1], K[1] = t, t = members[0], members[0] = members[1], members[1] = t;
+    for (int i = 0; i < a.groups; ++i) group_class[i] ^= 1;
+  }
+  steps = groups_of(d, K[0], a.steps);
+  bytes = (static_cast<long long>(count) * NS_PARTS * 8 + 1023) / 1024 * 1024;
+  for (int c = 0; c < classes; ++c) {
+    x_at[c] = bytes;
+    bytes += (2ll * members[c] * x_stride(c) * 2 + 1023) / 1024 * 1024;
+  }
+  s_at = bytes;
+  bytes += static_cast<long long>(buffers_of(steps)) * count * s_stride() * 2;
+  return 0;
+}
 
 struct Products {
-  CUtensorMap x, s;                           // 2 * count matrices X, and all factors
-  __half *X, *S;
-  int count, d, K;
+  const Layout& l;
+  __half* S;
+  __half* X[NS_CLASSES];
+  CUtensorMap load_x[NS_CLASSES], store_x[NS_CLASSES], load_s, store_s;
   int* status;
   cudaStream_t stream;
   int launches = 0, rc = 0;
 
-  long long x_stride() const { return static_cast<long long>(d) * pitch(K); }
-  long long s_stride() const { return static_cast<long long>(d) * pitch(d); }
-  __half* at(int f) const { return S + f * count * s_stride(); }
-
-  template <int B_MN>
-  void launch(const CUtensorMap& a, const CUtensorMap& b, OrthoGemm p) {
+  Products(const Layout& layout, char* work, int* status_, cudaStream_t stream_) : l(layout), status(status_), stream(stream_) {
+    S = reinterpret_cast<__half*>(work + l.s_at);
+    const uint64_t factors = static_cast<uint64_t>(buffers_of(l.steps)) * l.count;
+    rc = make_tmap_3d_fp16(&load_s, S, l.d, l.d, factors, pitch(l.d), 64, 64);
+    if (!rc) rc = make_tmap_3d_fp16(&store_s, S, l.d, l.d, factors, pitch(l.d), 32, 32);
+    for (int c = 0; c < l.classes; ++c) {
+      X[c] = reinterpret_cast<__half*>(work + l.x_at[c]);
+      if (!rc) rc = make_tmap_3d_fp16(&load_x[c], X[c], l.K[c], l.d, 2ull * l.members[c], pitch(l.K[c]), 64, 64);
+      if (!rc) rc = make_tmap_3d_fp16(&store_x[c], X[c], l.K[c], l.d, 2ull * l.members[c], pitch(l.K[c]), 32, 32);
+    }
+  }
+  template <int B_MN> void launch(const OrthoMaps& maps, OrthoGemm& p) {
     if (rc) return;
     static bool configured = false;
     if (!configured) {
       if (cudaFuncSetAttribute(ortho_gemm_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
-          cudaFuncSetAttribute(ortho_gemm_pair_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OP_SMEM) != cudaSuccess) {
+          cudaFuncSetAttribute(ortho_gemm_pair_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess) {
         rc = -20;
         return;
       }
       configured = true;
     }
-    p.count = count;
+    p.M = l.d;
     p.status = status;
-    auto tiles_of = [&](int tile) {
-      const long long m = (p.M + tile - 1) / tile, n = (p.N + tile - 1) / tile;
-      return (p.sym ? m * (m + 1) / 2 : m * n) * count;
+    const int sms = num_sms(), pairs = sms / 2;
+    auto tiles = [&](int c, int tile) {
+      const long long m = (p.M + tile - 1) / tile, n = (p.cls[c].N + tile - 1) / tile;
+      return p.sym ? m * (m + 1) / 2 : m * n;
     };
-    const long long small = tiles_of(OG_TILE), large = tiles_of(2 * OG_TILE);
-    if (small > 0x7fffffff) {
+    // The work of the busiest unit in blocks of 64 of the reduction, each tile with a fixed cost, twice as long for a pair's tile.
+    auto cost = [&](int tile, int units) {
+      long long total = 0, blocks = 0;
+      for (int c = 0; c < NS_CLASSES; ++c) {
+        const long long n = tiles(c, tile) * p.cls[c].count;
+        total += n;
+        blocks += n * ((p.cls[c].K + OG_BK - 1) / OG_BK);
+      }
+      const long long rounds = (total + units - 1) / units;
+      return static_cast<double>(rounds) * (static_cast<double>(blocks) / total + TILE_COST);
+    };
+    const bool pair = PAIR_COST * cost(256, pairs) < cost(128, sms);
+    const int tile = pair ? 256 : 128, units = pair ? pairs : sms;
+    long long total = 0;
+    for (int c = 0; c < NS_CLASSES; ++c) total += tiles(c, tile) * p.cls[c].count;
+    if (total > 0x7fffffff) {
       rc = -5;
       return;
     }
-    // rounds of tiles; a pair's tile has twice the work per multiprocessor of a single one's and takes about as long
-    const int sms = num_sms(), pairs = sms / 2;
-    if ((large + pairs - 1) / pairs <= (small + sms - 1) / sms)
-      rc = launch_chained(ortho_gemm_pair_kernel<B_MN>, 2 * static_cast<int>(large < pairs ? large : pairs), OG_THREADS, OP_SMEM,
-                          stream, a, b, p);
-    else
-      rc = launch_chained(ortho_gemm_kernel<B_MN>, static_cast<int>(small < sms ? small : sms), OG_THREADS, OG_SMEM, stream, a, b,
-                          p);
+    for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles(c, tile));
+    p.total = static_cast<int>(total);
+    const int grid = (p.total < units ? p.total : units) * (pair ? 2 : 1);
+    rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : ortho_gemm_kernel<B_MN>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
     ++launches;
   }
-  void product(int out, int i, int j) {       // factor `out` = (factor i) (factor j)
+  static constexpr double TILE_COST = 6, PAIR_COST = 1.6;
+
+  OrthoGemm empty() const {
     OrthoGemm p{};
-    p.M = p.N = p.K = d;
-    p.sym = 1;
-    p.a0 = i * count;
-    p.b0 = j * count;
-    p.C = at(out);
-    p.c_stride = s_stride();
-    p.ldc = pitch(d);
+    for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].N = p.cls[c].K = 1;      // a class without matrices
     p.alpha = 1.f / NS_SCALE;
-    launch<0>(s, s, p);
+    return p;
+  }
+  OrthoMaps square() const {
+    OrthoMaps m;
+    m.a[0] = m.a[1] = m.b[0] = m.b[1] = load_s;
+    m.c[0] = m.c[1] = store_s;
+    return m;
+  }
+  OrthoGemm factors(int out, int i, int j) const {
+    OrthoGemm p = empty();
+    p.sym = 1;
+    p.cls[0].count = l.count;
+    p.cls[0].N = p.cls[0].K = l.d;
+    p.cls[0].a0 = i * l.count;
+    p.cls[0].b0 = j * l.count;
+    p.cls[0].c0 = out * l.count;
+    return p;
+  }
+  void product(int out, int i, int j) {       // factor `out` = (factor i) (factor j)
+    OrthoGemm p = factors(out, i, j);
+    launch<0>(square(), p);
   }
   void polynomial(int out) {                  // factor `out` = a I + b S + c S^2
-    OrthoGemm p{};
-    p.M = p.N = p.K = d;
-    p.sym = 1;
-    p.a0 = p.b0 = F_S * count;
-    p.C = at(out);
-    p.R = at(F_S);
-    p.c_stride = s_stride();
-    p.ldc = pitch(d);
+    OrthoGemm p = factors(out, F_S, F_S);
+    p.R = S + F_S * l.count * l.s_stride();
+    p.r_stride = l.s_stride();
+    p.ldr = pitch(l.d);
     p.alpha = NS_C / NS_SCALE;
     p.beta = NS_B;
     p.gamma = NS_A * NS_SCALE;
-    launch<0>(s, s, p);
+    launch<0>(square(), p);
   }
   void gram(int from) {                       // S = X X^T
-    OrthoGemm p{};
-    p.M = p.N = d;
-    p.K = K;
+    OrthoGemm p = empty();
+    OrthoMaps m = square();
     p.sym = 1;
-    p.a0 = p.b0 = from * count;
-    p.C = at(F_S);
-    p.c_stride = s_stride();
-    p.ldc = pitch(d);
-    p.alpha = 1.f / NS_SCALE;
-    launch<0>(x, x, p);
+    for (int c = 0, first = 0; c < l.classes; first += l.members[c++]) {
+      m.a[c] = m.b[c] = load_x[c];
+      p.cls[c].count = l.members[c];
+      p.cls[c].N = l.d;
+      p.cls[c].K = l.K[c];
+      p.cls[c].a0 = p.cls[c].b0 = from * l.members[c];
+      p.cls[c].c0 = F_S * l.count + first;
+    }
+    launch<0>(m, p);
   }
   void update(int from, int by) {             // the other X = factor `by` X
-    OrthoGemm p{};
-    p.M = p.K = d;
-    p.N = K;
-    p.a0 = by * count;
-    p.b0 = from * count;
-    p.C = X + (1 - from) * count * x_stride();
-    p.c_stride = x_stride();
-    p.ldc = pitch(K);
-    p.alpha = 1.f / NS_SCALE;
-    launch<1>(s, x, p);
+    OrthoGemm p = empty();
+    OrthoMaps m = square();
+    for (int c = 0, first = 0; c < l.classes; first += l.members[c++]) {
+      m.b[c] = load_x[c];
+      m.c[c] = store_x[c];
+      p.cls[c].count = l.members[c];
+      p.cls[c].N = l.K[c];
+      p.cls[c].K = l.d;
+      p.cls[c].a0 = by * l.count + first;
+      p.cls[c].b0 = from * l.members[c];
+      p.cls[c].c0 = (1 - from) * l.members[c];
+    }
+    launch<1>(m, p);
   }
   void group(int from, int steps) {           // one or two steps on X number `from`, into the other one
     gram(from);
@@ -817,77 +966,75 @@ struct Products {
 
 using namespace aeris;
 
-extern "C" int aeris_ortho_buffers(int d, int K, int steps) {
-  return d <= 0 || K < d || steps < 1 || steps > 20 ? -1 : buffers_of(groups_of(d, K, steps));
+extern "C" long long aeris_ortho_work_bytes(const AerisOrtho* a) {
+  Layout l;
+  const int rc = l.fill(*a);
+  return rc ? rc : l.bytes;
 }
 
-extern "C" int aeris_ortho_updates(int d, int K, int steps) {
-  return d <= 0 || K < d || steps < 1 || steps > 20 ? -1 : groups_of(d, K, steps).n;
-}
-
-extern "C" int aeris_ortho_in(const AerisOrthoIn* a, void* stream_) {
+extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
+  const AerisOrtho& a = *p;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const bool step = a->grad != nullptr;
-  if (a->count <= 0 || a->count > 65535 || a->rows <= 0 || a->cols <= 0 || a->ld < a->cols || !a->X || !a->partial) return -1;
-  if (step ? !a->momentum || !a->offsets || a->ld != a->cols : !a->x) return -2;
-  if (a->offsets && (!a->status || a->numel <= 0)) return -3;
-  const long long n = static_cast<long long>(a->rows) * a->cols;
-  const long long want = (n + 4095) / 4096;
-  const int parts = static_cast<int>(want < NS_PARTS ? want : NS_PARTS);
-  const long long tiles = static_cast<long long>((a->rows + 63) / 64) * ((a->cols + 63) / 64);
-  if (tiles > 0x7fffffff) return -5;
-  const int aligned = on_grid(step ? a->grad : a->x, !step && a->bf16 ? 8 : 16) && on_grid(a->momentum, 16);
-  const MatrixAt m = {reinterpret_cast<const long long*>(a->offsets), a->stride, a->numel, a->rows, a->cols, a->ld, a->behind,
-                      aligned, a->status};
-  const OrthoInput in = {a->x, a->bf16, a->grad, a->momentum, a->norm_sq, a->beta, a->grad_scale, a->max_norm, a->nesterov,
-                         a->zero_grad};
-  const bool upright = a->rows > a->cols;
-  const int d = upright ? a->cols : a->rows, ldx = pitch(upright ? a->rows : a->cols);
-  const long long x_stride = static_cast<long long>(d) * ldx;
-  __half* X = reinterpret_cast<__half*>(a->X);
-  const int rc = launch_chained(step ? ortho_squares_kernel<true> : ortho_squares_kernel<false>, dim3(parts, a->count), 256, 0,
-                                stream, m, in, a->partial);
+  Layout l;
+  if (const int rc = l.fill(a)) return rc;
+  const bool step = a.grad != nullptr;
+  if (step ? !a.momentum || !a.master : !a.x || !a.out) return -6;
+  if (!a.work || !on_grid(a.work, 1024) || a.work_bytes < l.bytes || !a.status) return -7;
+  char* work = reinterpret_cast<char*>(a.work);
+  OrthoGroups in{}, out{};
+  in.n = out.n = a.groups;
+  in.numel = out.numel = a.numel;
+  in.status = out.status = a.status;
+  in.aligned = on_grid(step ? a.grad : a.x, !step && a.bf16 ? 8 : 16) && on_grid(a.momentum, 16);
+  out.aligned = on_grid(a.out, 8) && on_grid(a.master, 16) && on_grid(a.ema, 16) && on_grid(a.weights, 8);
+  long long first = 0, pack_blocks[NS_GROUPS], square_blocks[NS_GROUPS];
+  for (int i = 0; i < a.groups; ++i) {
+    const AerisOrthoGroup& g = a.group[i];
+    if (step ? !g.offsets || g.ld != g.cols : g.ld_out < g.cols) return -8;
+    if (g.offsets && a.numel <= 0) return -9;
+    const int c = l.group_class[i];
+    const long long n = static_cast<long long>(g.rows) * g.cols, want = (n + 4095) / 4096;
+    OrthoGroup& o = in.g[i];
+    o.offsets = reinterpret_cast<const long long*>(g.offsets);
+    o.stride = g.stride;
+    o.x_stride = l.x_stride(c);
+    o.x = reinterpret_cast<__half*>(work + l.x_at[c]) + l.group_first[i] * o.x_stride;
+    o.parts = static_cast<int>(want < NS_PARTS ? want : NS_PARTS);
+    o.partial = reinterpret_cast<double*>(work) + first * NS_PARTS;
+    first += g.count;
+    o.rows = g.rows;
+    o.cols = g.cols;
+    o.ld = g.ld;
+    o.ldx = pitch(l.K[c]);
+    o.behind = g.behind;
+    o.count = g.count;
+    o.rate = g.rate;
+    square_blocks[i] = o.parts;
+    pack_blocks[i] = static_cast<long long>((g.rows + 63) / 64) * ((g.cols + 63) / 64);
+    if (pack_blocks[i] * g.count > 0x3fffffff) return -5;
+    out.g[i] = o;
+    out.g[i].blocks = static_cast<int>(pack_blocks[i]);
+    if (!step) out.g[i].stride = g.out_stride, out.g[i].ld = g.ld_out;
+    if (l.steps.n & 1) out.g[i].x += l.members[c] * o.x_stride;
+  }
+  Products run(l, work, a.status, stream);
+  if (run.rc) return run.rc;
+  auto blocks = [&](const OrthoGroups& g) {
+    long long n = 0;
+    for (int i = 0; i < g.n; ++i) n += static_cast<long long>(g.g[i].count) * g.g[i].blocks;
+    return static_cast<unsigned>(n);
+  };
+  const OrthoInput input = {a.x, a.bf16, a.grad, a.momentum, a.norm_sq, a.beta, a.grad_scale, a.max_norm, a.nesterov, a.zero_grad};
+  for (int i = 0; i < a.groups; ++i) in.g[i].blocks = static_cast<int>(square_blocks[i]);
+  int rc = launch_chained(step ? ortho_squares_kernel<true> : ortho_squares_kernel<false>, blocks(in), 256, 0, stream, in, input);
   if (rc) return rc;
-  auto pack = step ? (upright ? ortho_pack_kernel<true, true> : ortho_pack_kernel<true, false>)
-                   : (upright ? ortho_pack_kernel<false, true> : ortho_pack_kernel<false, false>);
-  return launch_chained(pack, dim3(static_cast<unsigned>(tiles), a->count), 256, 0, stream, m, in,
-                        static_cast<const double*>(a->partial), parts, a->eps, X, x_stride, ldx);
-}
-
-extern "C" int aeris_ortho_iterate(void* X, void* S, int count, int d, int K, int steps, int* status, void* stream) {
-  if (!X || !S || !status || count <= 0 || d <= 0 || K < d || steps < 1 || steps > 20) return -1;
-  const Groups groups = groups_of(d, K, steps);
-  Products p;
-  p.X = reinterpret_cast<__half*>(X);
-  p.S = reinterpret_cast<__half*>(S);
-  p.count = count;
-  p.d = d;
-  p.K = K;
-  p.status = status;
-  p.stream = reinterpret_cast<cudaStream_t>(stream);
-  if (const int r = make_tmap_3d_fp16(&p.x, X, K, d, 2ull * count, pitch(K), 64)) return r;
-  if (const int r = make_tmap_3d_fp16(&p.s, S, d, d, static_cast<uint64_t>(buffers_of(groups)) * count, pitch(d), 64)) return r;
-  for (int k = 0; k < groups.n; ++k) p.group(k & 1, groups.size[k]);
-  return p.rc ? p.rc : p.launches;
-}
-
-extern "C" int aeris_ortho_out(const AerisOrthoOut* a, void* stream_) {
-  const bool step = a->master != nullptr;
-  if (a->count <= 0 || a->count > 65535 || a->rows <= 0 || a->cols <= 0 || a->ld < a->cols || !a->X || !a->status) return -1;
-  if (step ? !a->offsets || a->ld != a->cols : !a->out) return -2;
-  if (a->offsets && a->numel <= 0) return -3;
-  const long long tiles = static_cast<long long>((a->rows + 63) / 64) * ((a->cols + 63) / 64);
-  if (tiles > 0x7fffffff) return -5;
-  const int aligned = on_grid(a->out, 8) && on_grid(a->master, 16) && on_grid(a->ema, 16) && on_grid(a->weights, 8);
-  const MatrixAt m = {reinterpret_cast<const long long*>(a->offsets), a->stride, a->numel, a->rows, a->cols, a->ld, a->behind,
-                      aligned, a->status};
-  const OrthoOutput o = {reinterpret_cast<__nv_bfloat16*>(a->out), a->master, a->ema, reinterpret_cast<__nv_bfloat16*>(a->weights),
-                         a->decay, a->rate, a->ema_beta};
-  const bool upright = a->rows > a->cols;
-  const int d = upright ? a->cols : a->rows, ldx = pitch(upright ? a->rows : a->cols);
-  auto kern = step ? (upright ? ortho_finish_kernel<true, true> : ortho_finish_kernel<true, false>)
-                   : (upright ? ortho_finish_kernel<false, true> : ortho_finish_kernel<false, false>);
-  return launch_chained(kern, dim3(static_cast<unsigned>(tiles), a->count), 256, 0, reinterpret_cast<cudaStream_t>(stream_), m, o,
-                        reinterpret_cast<const __half*>(a->X), static_cast<long long>(d) * ldx, ldx,
-                        static_cast<const int*>(a->status));
+  for (int i = 0; i < a.groups; ++i) in.g[i].blocks = static_cast<int>(pack_blocks[i]);
+  rc = launch_chained(step ? ortho_pack_kernel<true> : ortho_pack_kernel<false>, blocks(in), 256, 0, stream, in, input, a.eps);
+  if (rc) return rc;
+  for (int k = 0; k < l.steps.n; ++k) run.group(k & 1, l.steps.size[k]);
+  if (run.rc) return run.rc;
+  const OrthoOutput output = {reinterpret_cast<__nv_bfloat16*>(a.out), a.master, a.ema, reinterpret_cast<__nv_bfloat16*>(a.weights),
+                              a.decay, a.ema_beta};
+  rc = launch_chained(step ? ortho_finish_kernel<true> : ortho_finish_kernel<false>, blocks(out), 256, 0, stream, out, output);
+  return rc ? rc : run.launches + 3;
 }

@@ -16,63 +16,40 @@ from . import lib as _l
 
 _P, _I, _F, _LL, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_double
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-MAX_COUNT = 65535            # matrices per launch: one layer of the grid each
-PARTS = 128                  # partial sums of squares per matrix
-# Workspace of one batch; what does not fit goes in several.
-WORKSPACE_BYTES = 1 << 30
+MAX_GROUPS, MAX_LENGTHS = 4, 2       # shapes of a batch, and longer sides among them
+MAX_COUNT = 1 << 16                  # matrices of a group
+WORKSPACE_BYTES = 1 << 30            # of one batch; what does not fit goes in several
 
 
-class _In(ctypes.Structure):
-    """Mirror of ``AerisOrthoIn`` (csrc/api.h)."""
-    _fields_ = ([(n, _P) for n in ("x", "grad", "momentum", "norm_sq", "offsets", "X", "partial", "status")] + [("eps", _D)]
-                + [(n, _LL) for n in ("stride", "numel")]
-                + [(n, _I) for n in ("rows", "cols", "ld", "count", "behind", "bf16", "nesterov", "zero_grad")]
-                + [(n, _F) for n in ("beta", "grad_scale", "max_norm")])
+class _Group(ctypes.Structure):
+    """Mirror of ``AerisOrthoGroup`` (csrc/api.h)."""
+    _fields_ = [("offsets", _P), ("stride", _LL), ("out_stride", _LL)] + [(n, _I) for n in ("rows", "cols", "ld", "ld_out", "count",
+                                                                                           "behind")] + [("rate", _F)]
 
 
-class _Out(ctypes.Structure):
-    """Mirror of ``AerisOrthoOut`` (csrc/api.h)."""
-    _fields_ = ([(n, _P) for n in ("X", "out", "master", "ema", "weights", "offsets", "status")]
-                + [(n, _LL) for n in ("stride", "numel")] + [(n, _I) for n in ("rows", "cols", "ld", "count", "behind")]
-                + [(n, _F) for n in ("decay", "rate", "ema_beta")])
+class _Args(ctypes.Structure):
+    """Mirror of ``AerisOrtho`` (csrc/api.h)."""
+    _fields_ = ([("group", _Group * MAX_GROUPS)]
+                + [(n, _P) for n in ("x", "out", "grad", "momentum", "master", "ema", "weights", "norm_sq", "work", "status")]
+                + [("eps", _D), ("numel", _LL), ("work_bytes", _LL)]
+                + [(n, _I) for n in ("groups", "steps", "bf16", "nesterov", "zero_grad")]
+                + [(n, _F) for n in ("beta", "grad_scale", "max_norm", "decay", "ema_beta")])
 
 
-def _pitch(n: int) -> int:
-    return -(-n // 64) * 64
+def _bytes_per_matrix(d: int, k: int) -> int:
+    """Workspace of one matrix, at most: two X, four square factors, partial sums."""
+    return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 1024
 
 
-class _Batch:
-    """Workspaces of ``count`` matrices of shorter side ``d`` and longer side ``k``, and the products on them."""
-
-    def __init__(self, count: int, d: int, k: int, steps: int, device):
-        self.count, self.d, self.k, self.steps = count, d, k, steps
-        self.x_size, self.half = d * _pitch(k), count * d * _pitch(k)
-        s = _l.lib().aeris_ortho_buffers(d, k, steps) * count * d * _pitch(d)
-        self.x = torch.empty(2 * self.half, dtype=torch.float16, device=device)
-        self.s = torch.empty(s, dtype=torch.float16, device=device)
-        self.partial = torch.empty(count * PARTS, dtype=torch.float64, device=device)
-
-    @staticmethod
-    def most(d: int, k: int, steps: int) -> int:
-        """Matrices of one batch."""
-        per = 2 * (2 * d * _pitch(k) + _l.lib().aeris_ortho_buffers(d, k, steps) * d * _pitch(d))
-        return max(1, min(MAX_COUNT, WORKSPACE_BYTES // per))
-
-    def load(self, first: int, a: _In) -> None:
-        a.X, a.partial = self.x.data_ptr() + 2 * first * self.x_size, self.partial.data_ptr()
-        _l.check(_l.lib().aeris_ortho_in(ctypes.byref(a), _l.stream_ptr()), "aeris_ortho_in", kernels=2)
-
-    def iterate(self) -> None:
-        """Leaves the result in ``self.result``."""
-        lib = _l.lib()
-        rc = lib.aeris_ortho_iterate(_l.ptr(self.x), _l.ptr(self.s), self.count, self.d, self.k, self.steps,
-                                     _l.ptr(_l.status_word()), _l.stream_ptr())
-        _l.check(min(rc, 0), "aeris_ortho_iterate", kernels=max(rc, 0))
-        self.result = self.x.data_ptr() + 2 * self.half * (lib.aeris_ortho_updates(self.d, self.k, self.steps) & 1)
-
-    def store(self, first: int, a: _Out) -> None:
-        a.X = self.result + 2 * first * self.x_size
-        _l.check(_l.lib().aeris_ortho_out(ctypes.byref(a), _l.stream_ptr()), "aeris_ortho_out")
+def _run(a: _Args, device) -> None:
+    lib = _l.lib()
+    lib.aeris_ortho_work_bytes.restype = _LL
+    a.work_bytes = lib.aeris_ortho_work_bytes(ctypes.byref(a))
+    _l.check(min(a.work_bytes, 0), "aeris_ortho_work_bytes", kernels=0)
+    work = torch.empty(a.work_bytes + 1024, dtype=torch.uint8, device=device)
+    a.work = -(-work.data_ptr() // 1024) * 1024
+    rc = lib.aeris_orthogonalise(ctypes.byref(a), _l.stream_ptr())
+    _l.check(min(rc, 0), "aeris_orthogonalise", kernels=max(rc, 0))
 
 
 def _as_batch(t: torch.Tensor) -> torch.Tensor:
@@ -115,19 +92,15 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, eps: float = 1e-7, out: to
     if not _pitched(xs):
         xs = xs.contiguous()
     count, rows, cols = xs.shape
-    d, k = min(rows, cols), max(rows, cols)
+    most = max(1, min(MAX_COUNT, WORKSPACE_BYTES // _bytes_per_matrix(min(rows, cols), max(rows, cols))))
     with _l.on_device(x.device):
         status = _l.status_word().data_ptr()
-        most = _Batch.most(d, k, steps)
         for i in range(0, count, most):
-            n = min(most, count - i)
-            b = _Batch(n, d, k, steps, x.device)
-            a = _In(x=xs.data_ptr() + i * xs.stride(0) * xs.element_size(), bf16=xs.dtype == torch.bfloat16, stride=xs.stride(0),
-                    rows=rows, cols=cols, ld=_row_pitch(xs), count=n, eps=eps, status=status)
-            b.load(0, a)
-            b.iterate()
-            b.store(0, _Out(out=os.data_ptr() + i * os.stride(0) * 2, stride=os.stride(0), rows=rows, cols=cols,
-                            ld=_row_pitch(os), count=n, status=status))
+            a = _Args(x=xs.data_ptr() + i * xs.stride(0) * xs.element_size(), out=os.data_ptr() + i * os.stride(0) * 2, groups=1,
+                      bf16=xs.dtype == torch.bfloat16, eps=eps, steps=steps, status=status)
+            a.group[0] = _Group(stride=xs.stride(0), out_stride=os.stride(0), rows=rows, cols=cols, ld=_row_pitch(xs),
+                                ld_out=_row_pitch(os), count=min(most, count - i))
+            _run(a, x.device)
     return out
 
 
@@ -138,31 +111,33 @@ def _check_flat(name: str, t: torch.Tensor, like: torch.Tensor, dtype: torch.dty
         raise ValueError(f"{name} does not start on a 16-byte boundary")
 
 
-def _step_batches(d, k, parts, master, grad, momentum, weights, ema, norm_sq, status, steps, settings, rates) -> None:
-    """All matrices of sides ``d`` and ``k``, upright and wide ones in the same products, as many at a time as fit a batch."""
-    todo = [(rows, cols, off.data_ptr(), 0, off.numel()) for rows, cols, off in parts]
-    left, most = sum(n for *_, n in todo), _Batch.most(d, k, steps)
-    batch, taken = None, []
-    while left:
-        if batch is None:
-            batch, room = _Batch(min(most, left), d, k, steps, master.device), min(most, left)
-            first, taken = 0, []
-        rows, cols, table, start, n = todo.pop(0)
-        m = min(n, room)
-        at = dict(offsets=table + 8 * start, behind=start > 0, numel=master.numel(), rows=rows, cols=cols, ld=cols, count=m,
-                  status=status)
-        batch.load(first, _In(grad=grad.data_ptr(), momentum=momentum.data_ptr(),
-                              norm_sq=0 if norm_sq is None else norm_sq.data_ptr(), **at, **settings))
-        taken.append((first, at))
-        first, room, left = first + m, room - m, left - m
-        if m < n:
-            todo.insert(0, (rows, cols, table, start + m, n - m))
-        if not room:
-            batch.iterate()
-            for i, where in taken:
-                batch.store(i, _Out(master=master.data_ptr(), weights=0 if weights is None else weights.data_ptr(),
-                                    ema=0 if ema is None else ema.data_ptr(), **where, **rates))
-            batch = None
+def _batches(groups):
+    """Cuts groups (rows, cols, address of the offsets, how many) into batches: lists of (rows, cols, address, how many, whether
+    an entry of the same table lies before it) with one shorter side, at most MAX_LENGTHS longer ones, MAX_GROUPS parts and
+    WORKSPACE_BYTES. Shapes with one shorter side share the launches of their square factors."""
+    by_side: dict[int, list] = {}
+    for g in groups:
+        by_side.setdefault(min(g[:2]), []).append(g)
+    for d, todo in by_side.items():
+        batch, lengths, room = [], set(), WORKSPACE_BYTES
+        todo = [(*g, False) for g in todo][::-1]
+        while todo:
+            rows, cols, table, n, behind = todo.pop()
+            k = max(rows, cols)
+            per = _bytes_per_matrix(d, k)
+            m = min(n, MAX_COUNT, max(room // per, 0 if batch else 1))
+            if m == 0 or len(batch) == MAX_GROUPS or (k not in lengths and len(lengths) == MAX_LENGTHS):
+                yield batch
+                batch, lengths, room = [], set(), WORKSPACE_BYTES
+                todo.append((rows, cols, table, n, behind))
+                continue
+            batch.append((rows, cols, table, m, behind))
+            lengths.add(k)
+            room -= m * per
+            if m < n:
+                todo.append((rows, cols, table + 8 * m, n - m, True))
+        if batch:
+            yield batch
 
 
 def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, weights: torch.Tensor | None,
@@ -188,7 +163,7 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
             _check_flat(name, t, master, dt)
     if norm_sq is not None and (norm_sq.numel() != 1 or norm_sq.dtype != torch.float64 or norm_sq.device != master.device):
         raise ValueError(f"norm_sq: one fp64 value on {master.device}, got {norm_sq.dtype} {tuple(norm_sq.shape)}")
-    batches: dict[tuple[int, int], list] = {}
+    todo = []
     for rows, cols, offsets in groups:
         if rows < 1 or cols < 1 or offsets.dim() != 1 or offsets.dtype != torch.int64 or offsets.device != master.device \
                 or not offsets.is_contiguous():
@@ -197,11 +172,17 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
         if rows * cols * offsets.numel() > master.numel():
             raise ValueError(f"{offsets.numel()} matrices of {rows} x {cols} do not fit {master.numel()} elements")
         if offsets.numel():
-            batches.setdefault((min(rows, cols), max(rows, cols)), []).append((rows, cols, offsets))
+            todo.append((rows, cols, offsets.data_ptr(), offsets.numel()))
     _l.require_cuda(master)
     with _l.on_device(master.device):
-        status = _l.status_word().data_ptr()
-        for (d, k), parts in batches.items():
-            _step_batches(d, k, parts, master, grad, momentum, weights, ema, norm_sq, status, steps,
-                          dict(beta=beta, nesterov=nesterov, zero_grad=zero_grad, grad_scale=grad_scale, max_norm=max_norm, eps=eps),
-                          dict(decay=1.0 - lr * weight_decay, rate=lr * scale * math.sqrt(k), ema_beta=ema_beta))
+        a = _Args(grad=grad.data_ptr(), momentum=momentum.data_ptr(), master=master.data_ptr(), numel=master.numel(),
+                  weights=0 if weights is None else weights.data_ptr(), ema=0 if ema is None else ema.data_ptr(),
+                  norm_sq=0 if norm_sq is None else norm_sq.data_ptr(), status=_l.status_word().data_ptr(), eps=eps, steps=steps,
+                  nesterov=nesterov, zero_grad=zero_grad, beta=beta, grad_scale=grad_scale, max_norm=max_norm,
+                  decay=1.0 - lr * weight_decay, ema_beta=ema_beta)
+        for batch in _batches(todo):
+            a.groups = len(batch)
+            for i, (rows, cols, table, n, behind) in enumerate(batch):
+                a.group[i] = _Group(offsets=table, rows=rows, cols=cols, ld=cols, count=n, behind=behind,
+                                    rate=lr * scale * math.sqrt(max(rows, cols)))
+            _run(a, master.device)
