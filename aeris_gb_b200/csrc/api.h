@@ -194,7 +194,7 @@ typedef struct AerisQkNorm {
   const float *cos, *sin;           // [L, rot / 2], or null with rot = 0
   const void* pos;                  // table row of every row (int32 or int64), null: row mod L. Outside [0, L): recorded in
                                     // the status word, the row's results are not written
-  float *dwq, *dwk, *sums;          // backward: [d] each; scratch [sum_rows, 2, d]
+  float *dwq, *dwk, *sums;          // backward: [d] each; scratch [sum_rows, d]
   int* status;
   long long rows;
   int L, heads, kv_heads, d, rot, f32, w_bf16, pos64, add_dw, sum_rows;   // add_dw: dwq, dwk are added to

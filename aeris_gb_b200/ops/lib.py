@@ -53,9 +53,12 @@ def require_cuda(t: torch.Tensor) -> None:
         raise ValueError(f"the kernels take tensors on a GPU, got one on {t.device}")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
-    """Context in which ``device`` is the current one; 2 us where it is not already."""
-    return contextlib.nullcontext() if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+    """Context in which ``device`` is the current one."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _STATUS: dict[int, torch.Tensor] = {}

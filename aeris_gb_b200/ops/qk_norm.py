@@ -9,87 +9,103 @@ angles of every position, row r of a window-major stream is at position r mod L 
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 import torch
 
 from . import lib as _l
 
-_P, _I, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 MAX_HEAD_DIM = 256
+MAX_ROWS = 2 ** 31 - 2 ** 21
+# AerisQkNorm (csrc/api.h), field by field: packing 39 values takes 0.4 us, filling a ctypes.Structure with them 12.
+_RECORD = struct.Struct("Pqq" * 6 + "9P" + "q" + "10i" + "f" + "0q")
+_FLOATS = (torch.bfloat16, torch.float32)
+_NOWHERE = (0, 0, 0)
 
 
-class _Heads(ctypes.Structure):
-    """Mirror of ``AerisHeads`` (csrc/api.h)."""
-    _fields_ = [("ptr", _P), ("row", _LL), ("head", _LL)]
+def _heads(t: torch.Tensor) -> tuple[int, int, int]:
+    row, head, _ = t.stride()
+    return t.data_ptr(), row, head
 
 
-class _Args(ctypes.Structure):
-    """Mirror of ``AerisQkNorm`` (csrc/api.h)."""
-    _fields_ = ([(n, _Heads) for n in ("q", "k", "dq", "dk", "q_out", "k_out")]
-                + [(n, _P) for n in ("wq", "wk", "cos", "sin", "pos", "dwq", "dwk", "sums", "status")] + [("rows", _LL)]
-                + [(n, _I) for n in ("L", "heads", "kv_heads", "d", "rot", "f32", "w_bf16", "pos64", "add_dw", "sum_rows")]
-                + [("eps", ctypes.c_float)])
+def _like(t: torch.Tensor, shape, dtype, device) -> bool:
+    return t.shape == shape and t.dtype is dtype and t.device == device and t.stride(2) == 1
 
 
-def _heads(t: torch.Tensor) -> _Heads:
-    return _Heads(t.data_ptr(), t.stride(0), t.stride(1))
-
-
-def _check_rows(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device or (t.stride(2) != 1 and t.shape[2] > 1):
-        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}, not "
-                         f"{tuple(like.shape)} {like.dtype} on {like.device} with channels side by side")
-
-
-def _writable(name: str, t: torch.Tensor) -> None:
-    """Refuses results of which two elements share an address (expanded rows or heads): several warps would write them."""
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two elements of ``t`` share an address (expanded rows or heads would be written by several warps)."""
     (rows, heads, d), (row, head, _) = t.shape, t.stride()
-    if t.numel() == 0:
-        return
-    by_row = (heads == 1 or head >= d) and (rows == 1 or row >= (heads - 1) * head + d)
-    by_head = (rows == 1 or row >= d) and (heads == 1 or head >= (rows - 1) * row + d)
-    if not (by_row or by_head):
-        raise ValueError(f"{name}: elements of {tuple(t.shape)} with strides {t.stride()} share addresses")
+    return (((heads == 1 or head >= d) and (rows == 1 or row >= (heads - 1) * head + d))
+            or ((rows == 1 or row >= d) and (heads == 1 or head >= (rows - 1) * row + d)) or t.numel() == 0)
 
 
-def _prepare(q, k, wq, wk, cos, sin, eps, positions, out) -> _Args:
-    """Checks that the kernels do not make, and the arguments that both directions share."""
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"q [rows, heads, d] and k [rows, kv_heads, d], got {tuple(q.shape)} and {tuple(k.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"q and k are bf16 or fp32, got {q.dtype}")
-    rows, heads, d = q.shape
-    if not (0 < d <= MAX_HEAD_DIM and d % 2 == 0) or heads < 1 or k.shape[1] < 1:
-        raise ValueError(f"{heads} and {k.shape[1]} heads of {d} channels: heads of an even width up to {MAX_HEAD_DIM} are taken")
-    _check_rows("q", q, q)
-    _check_rows("k", k, k)
-    if k.dtype != q.dtype or k.device != q.device:
-        raise ValueError(f"k: {k.dtype} on {k.device}, q is {q.dtype} on {q.device}")
-    for name, w in (("wq", wq), ("wk", wk)):
-        if w.shape != (d,) or w.dtype not in (torch.bfloat16, torch.float32) or w.dtype != wq.dtype or w.device != q.device \
-                or not w.is_contiguous():
-            raise ValueError(f"{name}: bf16 or fp32 [{d}] on {q.device}, both alike, got {tuple(w.shape)} {w.dtype} on {w.device}")
-    if (cos is None) != (sin is None) or (positions is not None and cos is None):
-        raise ValueError("cos and sin come together, positions only with them")
-    a = _Args(rows=rows, heads=heads, kv_heads=k.shape[1], d=d, f32=q.dtype == torch.float32, w_bf16=wq.dtype == torch.bfloat16,
-              eps=eps, q=_heads(q), k=_heads(k), wq=wq.data_ptr(), wk=wk.data_ptr())
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dim() != 2 or t.shape != cos.shape or t.dtype != torch.float32 or t.device != q.device or not t.is_contiguous():
-                raise ValueError(f"{name}: contiguous fp32 [L, rot / 2] on {q.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        if not 0 <= 2 * cos.shape[1] <= d or (cos.shape[0] < 1 and rows):
-            raise ValueError(f"angles {tuple(cos.shape)} for heads of {d} channels")
-        a.L, a.rot, a.cos, a.sin = cos.shape[0], 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr()
-        if positions is not None:
-            if positions.shape != (rows,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device \
-                    or not positions.is_contiguous():
-                raise ValueError(f"positions: contiguous int32 or int64 [{rows}] on {q.device}, got {tuple(positions.shape)} "
-                                 f"{positions.dtype} on {positions.device}")
-            a.pos, a.pos64 = positions.data_ptr(), positions.dtype == torch.int64
-    for name, t, like in out:
-        _check_rows(name, t, like)
-        _writable(name, t)
-    return a
+def _text(t) -> str:
+    return f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+
+
+def _check(q, k, wq, wk, cos, sin, positions, rows_like_q, rows_like_k, results, dw=()) -> tuple[int, ...]:
+    """Refuses what the kernels cannot take; returns (rows, heads, kv_heads, d, table length, rotated channels)."""
+    qs, ks, dt, dev = q.shape, k.shape, q.dtype, q.device
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or dt not in _FLOATS:
+        raise ValueError(f"q [rows, heads, d] and k [rows, kv_heads, d] in bf16 or fp32, got {_text(q)} and {_text(k)}")
+    rows, heads, d = qs
+    if rows > MAX_ROWS:
+        raise ValueError(f"{rows} rows: at most {MAX_ROWS} are taken")
+    if not 0 < d <= MAX_HEAD_DIM or d % 2 or heads < 1 or ks[1] < 1:
+        raise ValueError(f"{heads} and {ks[1]} heads of {d} channels: heads of an even width up to {MAX_HEAD_DIM} are taken")
+    if not (q.stride(2) == 1 == k.stride(2)) or k.dtype is not dt or k.device != dev:
+        raise ValueError(f"q and k: one type, one device, channels side by side, got {_text(q)} and {_text(k)}")
+    for shape, tensors in ((qs, rows_like_q), (ks, rows_like_k)):
+        for t in tensors:
+            if t is not None and not _like(t, shape, dt, dev):
+                raise ValueError(f"{dt} {tuple(shape)} on {dev} with channels side by side, got {_text(t)}")
+    for t in results:
+        if t is not None and not _apart(t):
+            raise ValueError(f"elements of a result share addresses: {_text(t)}")
+    w_dt, one = wq.dtype, (d,)
+    if not (wq.shape == one == wk.shape and w_dt in _FLOATS and w_dt is wk.dtype and wq.device == dev == wk.device
+            and wq.is_contiguous() and wk.is_contiguous()):
+        raise ValueError(f"weights: bf16 or fp32 [{d}] on {dev}, both alike, got {_text(wq)} and {_text(wk)}")
+    for t in dw:
+        if t.shape != (d,) or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"gradients of the weights: contiguous fp32 [{d}] on {dev}, got {_text(t)}")
+    if cos is None or sin is None:
+        if cos is not None or sin is not None or positions is not None:
+            raise ValueError("cos and sin come together, positions only with them")
+        return rows, heads, ks[1], d, 0, 0
+    table = cos.shape
+    if not (len(table) == 2 and sin.shape == table and cos.dtype is torch.float32 is sin.dtype and cos.device == dev == sin.device
+            and cos.is_contiguous() and sin.is_contiguous() and 2 * table[1] <= d and (table[0] > 0 or not rows)):
+        raise ValueError(f"angles: contiguous fp32 [L, at most {d // 2}] on {dev}, got {_text(cos)} and {_text(sin)}")
+    if positions is not None and not (positions.shape == (rows,) and positions.dtype in (torch.int32, torch.int64)
+                                      and positions.device == dev and positions.is_contiguous()):
+        raise ValueError(f"positions: contiguous int32 or int64 [{rows}] on {dev}, got {_text(positions)}")
+    return rows, heads, ks[1], d, table[0], 2 * table[1]
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    f = getattr(_l.lib(), name)
+    f.argtypes = (ctypes.c_char_p, ctypes.c_void_p)
+    return f
+
+
+@functools.lru_cache(maxsize=None)
+def _multiprocessors(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def _record(sizes, q, k, dq, dk, q_out, k_out, wq, wk, cos, sin, positions, dwq, dwk, sums, add, eps) -> bytes:
+    rows, heads, kv_heads, d, length, rot = sizes
+    return _RECORD.pack(*_heads(q), *_heads(k), *(_heads(dq) if dq is not None else _NOWHERE),
+                        *(_heads(dk) if dk is not None else _NOWHERE), *_heads(q_out), *_heads(k_out), wq.data_ptr(), wk.data_ptr(),
+                        cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0,
+                        positions.data_ptr() if positions is not None else 0, dwq.data_ptr() if dwq is not None else 0,
+                        dwk.data_ptr() if dwk is not None else 0, sums.data_ptr() if sums is not None else 0,
+                        _l.status_word().data_ptr(), rows, length, heads, kv_heads, d, rot, q.dtype is torch.float32,
+                        wq.dtype is torch.bfloat16, positions is not None and positions.dtype is torch.int64, add,
+                        sums.shape[0] if sums is not None else 0, eps)
 
 
 def qk_norm_fwd(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: torch.Tensor | None = None,
@@ -99,15 +115,16 @@ def qk_norm_fwd(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Te
     a fused qkv matrix): normed by head with the weights ``wq``, ``wk`` [d] and, with ``cos`` / ``sin``, turned. ``positions``
     [rows] int32 or int64: the table row of every row; one outside the table sets the status word and its row is not written.
     ``q_out``, ``k_out``: where to put the results, memory of their own or ``q`` and ``k`` themselves."""
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
-    a = _prepare(q, k, wq, wk, cos, sin, eps, positions, (("q_out", q_out, q), ("k_out", k_out, k)))
-    a.q_out, a.k_out = _heads(q_out), _heads(k_out)
+    sizes = _check(q, k, wq, wk, cos, sin, positions, (q_out,), (k_out,), (q_out, k_out))
     _l.require_cuda(q)
-    if a.rows:
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if sizes[0]:
         with _l.on_device(q.device):
-            a.status = _l.status_word().data_ptr()
-            _l.check(_l.lib().aeris_qk_norm_fwd(ctypes.byref(a), _l.stream_ptr()), "aeris_qk_norm_fwd")
+            a = _record(sizes, q, k, None, None, q_out, k_out, wq, wk, cos, sin, positions, None, None, None, False, eps)
+            _l.check(_entry("aeris_qk_norm_fwd")(a, _l.raw_stream()), "aeris_qk_norm_fwd")
     return q_out, k_out
 
 
@@ -118,28 +135,22 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
     """Gradients of :func:`qk_norm_fwd` for ``dq``, ``dk`` with respect to its results; ``q``, ``k`` are its inputs. Returns
     (gradients of q and k, which may overwrite ``dq`` and ``dk``, and fp32 gradients of the weights). ``dwq``, ``dwk`` [d] fp32
     are added to where given. The same bits on every run."""
-    dq_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq_out is None else dq_out
-    dk_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk_out is None else dk_out
-    a = _prepare(q, k, wq, wk, cos, sin, eps, positions, (("dq_out", dq_out, q), ("dk_out", dk_out, k)))
-    _check_rows("dq", dq, q)
-    _check_rows("dk", dk, k)
-    if (dwq is None) != (dwk is None):
+    add = dwq is not None
+    if add != (dwk is not None):
         raise ValueError("dwq and dwk come together")
-    a.add_dw = dwq is not None
-    for name, t in (("dwq", dwq), ("dwk", dwk)):
-        if t is not None and (t.shape != wq.shape or t.dtype != torch.float32 or t.device != q.device or not t.is_contiguous()):
-            raise ValueError(f"{name}: contiguous fp32 [{a.d}] on {q.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    sizes = _check(q, k, wq, wk, cos, sin, positions, (dq, dq_out), (dk, dk_out), (dq_out, dk_out), (dwq, dwk) if add else ())
     _l.require_cuda(q)
-    if not a.rows:
-        return dq_out, dk_out, *(torch.zeros(a.d, dtype=torch.float32, device=q.device) if t is None else t for t in (dwq, dwk))
-    if dwq is None:
-        dwq, dwk = torch.empty((2, a.d), dtype=torch.float32, device=q.device).unbind(0)
-    with _l.on_device(q.device):
-        sums = torch.empty((4 * torch.cuda.get_device_properties(q.device).multi_processor_count, 2, a.d), dtype=torch.float32,
-                           device=q.device)
-        a.dq, a.dk, a.q_out, a.k_out = _heads(dq), _heads(dk), _heads(dq_out), _heads(dk_out)
-        a.dwq, a.dwk, a.sums, a.sum_rows = dwq.data_ptr(), dwk.data_ptr(), sums.data_ptr(), sums.shape[0]
-        a.status = _l.status_word().data_ptr()
-        rc = _l.lib().aeris_qk_norm_bwd(ctypes.byref(a), _l.stream_ptr())
-        _l.check(min(rc, 0), "aeris_qk_norm_bwd", kernels=max(rc, 0))
+    if dq_out is None:
+        dq_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if dk_out is None:
+        dk_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if not add:
+        make = torch.empty_like if sizes[0] else torch.zeros_like
+        dwq, dwk = make(wq, dtype=torch.float32), make(wk, dtype=torch.float32)
+    if sizes[0]:
+        with _l.on_device(q.device):
+            sums = q.new_empty((4 * _multiprocessors(q.get_device()), sizes[3]), dtype=torch.float32)
+            a = _record(sizes, q, k, dq, dk, dq_out, dk_out, wq, wk, cos, sin, positions, dwq, dwk, sums, add, eps)
+            rc = _entry("aeris_qk_norm_bwd")(a, _l.raw_stream())
+            _l.check(min(rc, 0), "aeris_qk_norm_bwd", kernels=max(rc, 0))
     return dq_out, dk_out, dwq, dwk
