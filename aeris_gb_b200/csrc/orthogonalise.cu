@@ -748,6 +748,201 @@ ortho_gemm_pair_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p
   if (warp == 1) tmem_dealloc2(tmem_base, 2 * TILE);
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// Everything for one matrix in one CTA and one launch, where X fits next to its factors: d <= 128, K <= 384. Bound by latency:
+// three products a step whose operands never leave shared memory (X in blocks of 64 columns of 128 swizzled rows, which serve
+// as the K-major operands of X X^T and as the MN-major one of P X), accumulators in tensor memory, a barrier or two between.
+// Eight matrices of 64 x 64: 64 us by the launches above, 33 of them on the host, 20 by this one.
+constexpr int OS_MAX_D = 128, OS_MAX_K = 384, OS_THREADS = 256;
+constexpr int OS_BLOCK = 128 * 128;           // 64 columns of 128 rows, in bytes
+constexpr int OS_S = (OS_MAX_K / 64) * OS_BLOCK, OS_P = OS_S + 2 * OS_BLOCK, OS_BARS = OS_P + 2 * OS_BLOCK;
+constexpr int OS_SMEM = OS_BARS + 256 + 1024;
+
+__device__ __forceinline__ uint32_t os_at(int row, int col) {         // byte offset of an element of X, S or P
+  return (col >> 6) * OS_BLOCK + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+// 32 values of one row from column `col` (a multiple of 32) on, scaled and rounded
+__device__ __forceinline__ void os_put(uint8_t* to, int row, int col, const float (&f)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __floats2half2_rn(f[8 * i + 2 * j], f[8 * i + 2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(to + os_at(row, col + 8 * i)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <bool STEP>
+__global__ void __launch_bounds__(OS_THREADS, 1)
+ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b, const OrthoOutput o, double eps, int steps) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + OS_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+  double* red = reinterpret_cast<double*>(bar + 4);
+  int* gave_up = reinterpret_cast<int*>(bar + 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    fence_barrier_init();
+    *gave_up = 0;
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  chain_point();
+
+  const OrthoPlace p = ortho_place(a);
+  const OrthoGroup& m = a.g[p.group];
+  const bool upright = m.rows > m.cols;
+  const int d = upright ? m.cols : m.rows, K = upright ? m.rows : m.cols, n = m.rows * m.cols;
+  const int blocks = (K + 63) / 64;
+  for (int i = threadIdx.x; i < blocks * OS_BLOCK / 16; i += OS_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  const float gs = STEP ? step_scale(in) : 0.f;
+  double sum = 0;
+  if (p.found) {
+    for (int v = threadIdx.x; v < n; v += OS_THREADS) {
+      const long long e = m.ld == m.cols ? p.at + v : p.at + static_cast<long long>(v / m.cols) * m.ld + v % m.cols;
+      float u;
+      if (STEP) {
+        const float g = clean(in.grad[e] * gs), mom = in.beta * in.momentum[e] + (1.f - in.beta) * g;
+        in.momentum[e] = mom;
+        u = in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom;
+      } else {
+        u = in_value(in, e);
+      }
+      sum += static_cast<double>(u) * u;
+    }
+  }
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int i = 0; i < OS_THREADS / 32; ++i) sum += red[i];
+  const double norm = sqrt(sum);
+  const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
+  if (p.found) {                              // each thread reads what it has written
+    for (int v = threadIdx.x; v < n; v += OS_THREADS) {
+      const int r = v / m.cols, c = v - r * m.cols;
+      const long long e = p.at + static_cast<long long>(r) * m.ld + c;
+      float u;
+      if (STEP) {
+        const float g = clean(in.grad[e] * gs), mom = in.momentum[e];
+        u = in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom;
+        if (in.zero_grad) in.grad[e] = 0.f;
+      } else {
+        u = in_value(in, e);
+      }
+      *reinterpret_cast<__half*>(smem + (upright ? os_at(c, r) : os_at(r, c))) = __float2half_rn(scale * u);
+    }
+  }
+
+  const int q = warp & 3, part = warp >> 2, row = q * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16, t_s = tmem + OS_MAX_K;
+  const uint32_t x_at = smem_u32(smem), s_at = smem_u32(smem + OS_S), p_at = smem_u32(smem + OS_P);
+  const int wide = d > 64 ? 128 : 64;         // columns of the square factors
+  uint32_t phase = 0;
+  // all threads: what they wrote to shared memory is there for the products, which thread 0 issues and all wait for
+  auto products = [&](auto issue) {
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      issue();
+      tc_commit(bar);
+    }
+    if (!own_wait(bar, phase, a.status, ERR_TIMEOUT_TMEM_FULL)) *gave_up = 1;
+    phase ^= 1;
+    tc_fence_after();
+  };
+  for (int step = 0; step < steps; ++step) {
+    products([&] {
+      for (int k = 0; k < blocks * 4; ++k) {
+        const uint64_t desc = make_smem_desc(x_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024);
+        umma_ss(t_s, desc, desc, make_idesc_fp16(128, wide, 0), k > 0);
+      }
+    });
+    float s[64];
+    const int mine = wide / 2, c0 = part * mine;         // this warp's columns of the factors
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= mine) break;
+      uint32_t v[32];
+      tmem_ld32(t_s + lanes + c0 + 32 * h, v);
+      tmem_wait_ld();
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j)           // b S takes S as it is in c S^2: near 1 most of a rounding cancels between the two
+        f[j] = s[32 * h + j] = __half2float(__float2half_rn(__uint_as_float(v[j]) * (1.f / NS_SCALE)));
+      os_put(smem + OS_S, row, c0 + 32 * h, f);
+    }
+    products([&] {
+      for (int k = 0; k < wide / 16; ++k) {
+        const uint64_t desc = make_smem_desc(s_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024);
+        umma_ss(t_s, desc, desc, make_idesc_fp16(128, wide, 0), k > 0);
+      }
+    });
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= mine) break;
+      uint32_t v[32];
+      tmem_ld32(t_s + lanes + c0 + 32 * h, v);
+      tmem_wait_ld();
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        f[j] = NS_C / NS_SCALE * __uint_as_float(v[j]) + NS_B * s[32 * h + j] + (row == c0 + 32 * h + j ? NS_A * NS_SCALE : 0.f);
+      os_put(smem + OS_P, row, c0 + 32 * h, f);
+    }
+    products([&] {
+      for (int c = 0; c < blocks * 64; c += 256) {
+        const int cols = min(256, blocks * 64 - c);
+        for (int k = 0; k < wide / 16; ++k)
+          umma_ss(tmem + c, make_smem_desc(p_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024),
+                  make_smem_desc(x_at + (c >> 6) * OS_BLOCK + k * 2048, OS_BLOCK, 1024), make_idesc_fp16(128, cols, 1), k > 0);
+      }
+    });
+    for (int c = part * 32; c < blocks * 64; c += 64) {
+      uint32_t v[32];
+      tmem_ld32(tmem + lanes + c, v);
+      tmem_wait_ld();
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * (1.f / NS_SCALE);
+      os_put(smem, row, c, f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+  const OrthoGroup& t = b.g[p.group];
+  if (!p.found || *gave_up || failed(a.status)) return;
+  const long long out_at = t.offsets ? p.at : p.matrix * t.stride;
+  for (int v = threadIdx.x; v < n; v += OS_THREADS) {
+    const int r = v / m.cols, c = v - r * m.cols;
+    const float x = __half2float(*reinterpret_cast<const __half*>(smem + (upright ? os_at(c, r) : os_at(r, c)))) * (1.f / NS_SCALE);
+    const long long e = out_at + static_cast<long long>(r) * t.ld + c;
+    if (!STEP) {
+      o.out[e] = __float2bfloat16_rn(x);
+      continue;
+    }
+    const float w = o.master[e] * o.decay - m.rate * x;
+    o.master[e] = w;
+    if (o.weights) o.weights[e] = __float2bfloat16_rn(w);
+    if (o.ema && o.ema_beta >= 0.f) o.ema[e] = w + o.ema_beta * (o.ema[e] - w);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 namespace {
 
@@ -757,19 +952,19 @@ bool on_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 // How the steps are grouped. One step by itself is a Gram matrix of X, its square and an update of X: in units of d^3, with
 // symmetric products at half and r = K / d, 3 r + 1. Two steps can share the update: the Gram matrix alone goes on (S <- P S P
 // with P = a I + b S + c S^2, all symmetric and commuting) and X is multiplied by the product of both P at the end: 3 r + 5
-// instead of 6 r + 2, the less for every oblong matrix. Groups of three would cost 3 r + 9, but a Gram matrix's rounding error
-// (2^-12 of its norm) grows by a^2 a step in directions that hold little of the norm, and is not small against them any more:
-// error on 127 x 640 gradients with half as much noise as signal 6e-4 by single steps and in groups (2, 2, 1), 1.8e-3 in (3, 2); on
-// 320 x 2000 5.5e-4, 6.5e-4, 9e-4; a group of five diverges. Below GROUP_FROM rows single steps: the products are shorter than
-// their launches, of which groups have two more, and a handful of rows does not average the roundings (5 x 9: up to three times
-// the error of single steps).
+// instead of 6 r + 2, the less for every oblong matrix. But a Gram matrix's rounding error (2^-12 of its norm) grows by a^2 a step
+// in directions that hold little of the norm, and is not small against them any more. So pairs of steps alternate with single
+// ones: error on 333 x 1001 gradients with half as much noise as signal 1.13e-3 by single steps, 1.09e-3 as 2, 1, 2, 1.49e-3 as
+// 2, 2, 1, 1.8e-3 as 3, 2; on 127 x 640 6e-4, 6e-4, 6e-4, 1.8e-3; a group of five diverges. Below GROUP_FROM rows single steps:
+// the products are shorter than their launches, of which groups have two more, and a handful of rows does not average the
+// roundings (5 x 9: up to three times the error of single steps).
 constexpr int GROUP_FROM = 256;
 struct Groups {
   int n, size[20];
 };
 Groups groups_of(int d, int K, int steps) {
   Groups g = {0, {}};
-  for (int left = steps, most = K > d && d >= GROUP_FROM ? 2 : 1; left > 0; left -= g.size[g.n++]) g.size[g.n] = left < most ? left : most;
+  for (int left = steps; left > 0; left -= g.size[g.n++]) g.size[g.n] = K > d && d >= GROUP_FROM && left > 1 && g.n % 2 == 0 ? 2 : 1;
   return g;
 }
 int buffers_of(const Groups& g) { return g.size[0] == 1 ? 2 : 4; }
@@ -785,6 +980,7 @@ struct Layout {
   long long s_stride() const { return static_cast<long long>(d) * pitch(d); }
   int fill(const AerisOrtho& a);
 };
+bool small(const Layout& l) { return l.d <= OS_MAX_D && l.K[0] <= OS_MAX_K; }
 int Layout::fill(const AerisOrtho& a) {
   if (a.groups < 1 || a.groups > NS_GROUPS || a.steps < 1 || a.steps > 20) return -1;
   d = count = classes = 0;
@@ -808,6 +1004,8 @@ int Layout::fill(const AerisOrtho& a) {
     K[0] = K[1], K[1] = t, t = members[0], members[0] = members[1], members[1] = t;
     for (int i = 0; i < a.groups; ++i) group_class[i] ^= 1;
   }
+  bytes = 0;
+  if (small(*this)) return 0;                 // everything in shared memory
   steps = groups_of(d, K[0], a.steps);
   bytes = (static_cast<long long>(count) * NS_PARTS * 8 + 1023) / 1024 * 1024;
   for (int c = 0; c < classes; ++c) {
@@ -979,7 +1177,7 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   if (const int rc = l.fill(a)) return rc;
   const bool step = a.grad != nullptr;
   if (step ? !a.momentum || !a.master : !a.x || !a.out) return -6;
-  if (!a.work || !on_grid(a.work, 1024) || a.work_bytes < l.bytes || !a.status) return -7;
+  if (!a.status || (l.bytes && (!a.work || !on_grid(a.work, 1024) || a.work_bytes < l.bytes))) return -7;
   char* work = reinterpret_cast<char*>(a.work);
   OrthoGroups in{}, out{};
   in.n = out.n = a.groups;
@@ -1015,16 +1213,31 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
     out.g[i] = o;
     out.g[i].blocks = static_cast<int>(pack_blocks[i]);
     if (!step) out.g[i].stride = g.out_stride, out.g[i].ld = g.ld_out;
-    if (l.steps.n & 1) out.g[i].x += l.members[c] * o.x_stride;
+    if (l.bytes && (l.steps.n & 1)) out.g[i].x += l.members[c] * o.x_stride;
   }
-  Products run(l, work, a.status, stream);
-  if (run.rc) return run.rc;
   auto blocks = [&](const OrthoGroups& g) {
     long long n = 0;
     for (int i = 0; i < g.n; ++i) n += static_cast<long long>(g.g[i].count) * g.g[i].blocks;
     return static_cast<unsigned>(n);
   };
   const OrthoInput input = {a.x, a.bf16, a.grad, a.momentum, a.norm_sq, a.beta, a.grad_scale, a.max_norm, a.nesterov, a.zero_grad};
+  const OrthoOutput output = {reinterpret_cast<__nv_bfloat16*>(a.out), a.master, a.ema, reinterpret_cast<__nv_bfloat16*>(a.weights),
+                              a.decay, a.ema_beta};
+  if (small(l)) {
+    static bool configured = false;
+    if (!configured) {
+      if (cudaFuncSetAttribute(ortho_small_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OS_SMEM) != cudaSuccess ||
+          cudaFuncSetAttribute(ortho_small_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OS_SMEM) != cudaSuccess)
+        return -20;
+      configured = true;
+    }
+    for (int i = 0; i < a.groups; ++i) in.g[i].blocks = 1;
+    const int rc = launch_chained(step ? ortho_small_kernel<true> : ortho_small_kernel<false>, blocks(in), OS_THREADS, OS_SMEM, stream,
+                                  in, input, out, output, a.eps, a.steps);
+    return rc ? rc : 1;
+  }
+  Products run(l, work, a.status, stream);
+  if (run.rc) return run.rc;
   for (int i = 0; i < a.groups; ++i) in.g[i].blocks = static_cast<int>(square_blocks[i]);
   int rc = launch_chained(step ? ortho_squares_kernel<true> : ortho_squares_kernel<false>, blocks(in), 256, 0, stream, in, input);
   if (rc) return rc;
@@ -1033,8 +1246,6 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   if (rc) return rc;
   for (int k = 0; k < l.steps.n; ++k) run.group(k & 1, l.steps.size[k]);
   if (run.rc) return run.rc;
-  const OrthoOutput output = {reinterpret_cast<__nv_bfloat16*>(a.out), a.master, a.ema, reinterpret_cast<__nv_bfloat16*>(a.weights),
-                              a.decay, a.ema_beta};
   rc = launch_chained(step ? ortho_finish_kernel<true> : ortho_finish_kernel<false>, blocks(out), 256, 0, stream, out, output);
   return rc ? rc : run.launches + 3;
 }

@@ -46,8 +46,9 @@ def _run(a: _Args, device) -> None:
     lib.aeris_ortho_work_bytes.restype = _LL
     a.work_bytes = lib.aeris_ortho_work_bytes(ctypes.byref(a))
     _l.check(min(a.work_bytes, 0), "aeris_ortho_work_bytes", kernels=0)
-    work = torch.empty(a.work_bytes + 1024, dtype=torch.uint8, device=device)
-    a.work = -(-work.data_ptr() // 1024) * 1024
+    if a.work_bytes:
+        work = torch.empty(a.work_bytes + 1024, dtype=torch.uint8, device=device)
+        a.work = -(-work.data_ptr() // 1024) * 1024
     rc = lib.aeris_orthogonalise(ctypes.byref(a), _l.stream_ptr())
     _l.check(min(rc, 0), "aeris_orthogonalise", kernels=max(rc, 0))
 
