@@ -23,7 +23,7 @@ namespace aeris {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float NS_SCALE = 512.f;             // stored = NS_SCALE * value, for X and for the [d, d] factors
 
-constexpr int NS_PARTS = 128;                 // blocks per matrix that its squares are summed in, at most
+constexpr int NS_PARTS = 1024;                // blocks per matrix that its squares are summed in, at most
 constexpr int NS_GROUPS = ORTHO_GROUPS, NS_CLASSES = 2;
 
 // ------------------------------------------------------------------------------------------------ in and out
@@ -103,9 +103,25 @@ __device__ __forceinline__ float4 in_value4(const OrthoInput& in, long long e) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Sums of squares of one matrix, NS_PARTS at most, in 64 bits (squares of any fp32 values add up without overflow). An
+// Sums of squares of one matrix, NS_PARTS at most, as good as in 64 bits (any fp32 values' squares add up without overflow). An
 // optimizer's momentum is brought up to date on the way: M = beta M + (1 - beta) g; what is summed is M, or beta M + (1 -
 // beta) g with nesterov.
+// The squares of a few vectors: in 32 bits where they neither overflow nor vanish there, which a sum between the bounds says (each
+// term lost below has 2^-60 of it at most), for conversions to 64 bits and products in them are an eighth as fast.
+template <int U> __device__ __forceinline__ double squares_of(const float4 (&u)[U]) {
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < U; ++k) s += u[k].x * u[k].x + u[k].y * u[k].y + (u[k].z * u[k].z + u[k].w * u[k].w);
+  if (s > 1e-20f && s < 1e37f) return s;
+  double d = 0;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    d += static_cast<double>(u[k].x) * u[k].x + static_cast<double>(u[k].y) * u[k].y;
+    d += static_cast<double>(u[k].z) * u[k].z + static_cast<double>(u[k].w) * u[k].w;
+  }
+  return d;
+}
+
 template <bool STEP>
 __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a, const OrthoInput in) {
   chain_point();
@@ -124,19 +140,27 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a,
     const long long step = m.blocks * 256ll, first = p.block * 256ll + threadIdx.x;
     if (p.four) {
       const int per_row = m.cols / 4;
-      for (long long v = first; v < n / 4; v += step) {
-        const long long e = flat ? p.at + 4 * v : p.at + v / per_row * m.ld + 4 * (v % per_row);
-        float4 u;
-        if (STEP) {
-          const float4 g = *reinterpret_cast<const float4*>(in.grad + e);
-          float4 mo = *reinterpret_cast<const float4*>(in.momentum + e);
-          u = make_float4(value(g.x, mo.x), value(g.y, mo.y), value(g.z, mo.z), value(g.w, mo.w));
-          *reinterpret_cast<float4*>(in.momentum + e) = mo;
-        } else {
-          u = in_value4(in, e);
+      auto at = [&](long long v) { return flat ? p.at + 4 * v : p.at + v / per_row * m.ld + 4 * (v % per_row); };
+      constexpr int U = STEP ? 2 : 4;         // vectors under way per thread
+      for (long long v = first; v < n / 4; v += U * step) {
+        float4 u[U], mo[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          u[k] = mo[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (v + k * step >= n / 4) continue;
+          const long long e = at(v + k * step);
+          u[k] = STEP ? *reinterpret_cast<const float4*>(in.grad + e) : in_value4(in, e);
+          if (STEP) mo[k] = *reinterpret_cast<const float4*>(in.momentum + e);
         }
-        sum += static_cast<double>(u.x) * u.x + static_cast<double>(u.y) * u.y;
-        sum += static_cast<double>(u.z) * u.z + static_cast<double>(u.w) * u.w;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (STEP) {
+            float4 &x = u[k], &y = mo[k];
+            x = make_float4(value(x.x, y.x), value(x.y, y.y), value(x.z, y.z), value(x.w, y.w));
+            if (v + k * step < n / 4) *reinterpret_cast<float4*>(in.momentum + at(v + k * step)) = y;
+          }
+        }
+        sum += squares_of(u);
       }
     } else {
       for (long long v = first; v < n; v += step) {
@@ -168,20 +192,21 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a,
 template <bool STEP>
 __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, const OrthoInput in, double eps) {
   __shared__ float tile[64][65];
-  __shared__ float s_scale;
+  __shared__ double red[8];
   chain_point();
   const OrthoPlace p = ortho_place(a);
   const OrthoGroup& m = a.g[p.group];
   if (!p.found) return;
-  if (threadIdx.x < 32) {
-    double sum = 0;
-    for (int i = threadIdx.x; i < m.parts; i += 32) sum += m.partial[p.matrix * static_cast<long long>(m.parts) + i];
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double norm = sqrt(sum);
-    if (threadIdx.x == 0) s_scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
-  }
+  double sum = 0;
+  for (int i = threadIdx.x; i < m.parts; i += 256) sum += m.partial[p.matrix * static_cast<long long>(m.parts) + i];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
   __syncthreads();
-  const float scale = s_scale, gs = STEP ? step_scale(in) : 0.f;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += red[i];
+  const double norm = sqrt(sum);
+  const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps)), gs = STEP ? step_scale(in) : 0.f;
   const int tiles_c = (m.cols + 63) / 64;
   const int r0 = p.block / tiles_c * 64, c0 = p.block % tiles_c * 64;
   const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
@@ -1191,13 +1216,15 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
     if (step ? !g.offsets || g.ld != g.cols : g.ld_out < g.cols) return -8;
     if (g.offsets && a.numel <= 0) return -9;
     const int c = l.group_class[i];
-    const long long n = static_cast<long long>(g.rows) * g.cols, want = (n + 4095) / 4096;
+    const long long n = static_cast<long long>(g.rows) * g.cols, want = (n + 8191) / 8192;
     OrthoGroup& o = in.g[i];
     o.offsets = reinterpret_cast<const long long*>(g.offsets);
     o.stride = g.stride;
     o.x_stride = l.x_stride(c);
     o.x = reinterpret_cast<__half*>(work + l.x_at[c]) + l.group_first[i] * o.x_stride;
-    o.parts = static_cast<int>(want < NS_PARTS ? want : NS_PARTS);
+    // one round of blocks over all matrices (four fit an SM), or so many rounds that the last one does not count
+    const long long share = 4ll * num_sms() / l.count, most = share < 128 ? 128 : share < NS_PARTS ? share : NS_PARTS;
+    o.parts = static_cast<int>(want < most ? want : most);
     o.partial = reinterpret_cast<double*>(work) + first * NS_PARTS;
     first += g.count;
     o.rows = g.rows;

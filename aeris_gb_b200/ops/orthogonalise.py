@@ -38,7 +38,7 @@ class _Args(ctypes.Structure):
 
 def _bytes_per_matrix(d: int, k: int) -> int:
     """Workspace of one matrix, at most: two X, four square factors, partial sums."""
-    return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 1024
+    return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 8192
 
 
 def _run(a: _Args, device) -> None:
