@@ -163,17 +163,28 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a,
         sum += squares_of(u);
       }
     } else {
-      for (long long v = first; v < n; v += step) {
-        const long long e = flat ? p.at + v : p.at + v / m.cols * m.ld + v % m.cols;
-        float u;
-        if (STEP) {
-          float mo = in.momentum[e];
-          u = value(in.grad[e], mo);
-          in.momentum[e] = mo;
-        } else {
-          u = in_value(in, e);
+      auto at = [&](long long v) { return flat ? p.at + v : p.at + v / m.cols * m.ld + v % m.cols; };
+      constexpr int U = 8;
+      for (long long v = first; v < n; v += U * step) {
+        float u[U], mo[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          u[k] = mo[k] = 0.f;
+          if (v + k * step >= n) continue;
+          const long long e = at(v + k * step);
+          u[k] = STEP ? in.grad[e] : in_value(in, e);
+          if (STEP) mo[k] = in.momentum[e];
         }
-        sum += static_cast<double>(u) * u;
+        float4 q[U / 4];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (STEP) {
+            u[k] = value(u[k], mo[k]);
+            if (v + k * step < n) in.momentum[at(v + k * step)] = mo[k];
+          }
+          reinterpret_cast<float*>(&q[k / 4])[k % 4] = u[k];
+        }
+        sum += squares_of(q);
       }
     }
   }
@@ -442,20 +453,30 @@ __device__ __forceinline__ void ortho_tile(const OrthoGemm& p, int t, int& cls, 
 // A warp's 32 rows (from row0 on) of NCOL accumulator columns from `taddr` on, which are columns col0 .. of matrix `mat` of C.
 // A piece's row of 64 bytes is swizzled by 16-byte chunks (64-byte swizzle of the tensor maps); in the mirror image lane l holds
 // rows l & ~1 and l | 1 of column 2 j + (l & 1).
+// `R`: this lane's row of R or null, `r` 64 values of it: two pieces are requested before the accumulator is waited for, the
+// others while the one before them is worked on (d = 333: 7.3 us a launch with each requested when it is needed, 6.2).
+struct Addend {
+  const __half* R;
+  uint4 r[2][4];
+  int ld;
+  __device__ void fetch(int col, int slot) {
+    if (R && col < ld) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[slot][j] = *reinterpret_cast<const uint4*>(R + col + 8 * j);
+    }
+  }
+  __device__ Addend(const OrthoGemm& p, int mat, int row, int col0) : R(nullptr), r{}, ld(p.ldr) {
+    if (p.R && row < p.M) R = p.R + mat * p.r_stride + static_cast<long long>(row) * p.ldr;
+    fetch(col0, 0);
+    fetch(col0 + 32, 1);
+  }
+};
 template <int NCOL>
 __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtensorMap* cmap, uint8_t* stage, uint32_t taddr, int mat,
-                                               int r_mat, int row0, int col0, int N, bool keep, bool mirror, int lane,
+                                               Addend& add, int row0, int col0, int N, bool keep, bool mirror, int lane,
                                                int& pieces) {
   const int row = row0 + lane;
-  const __half* R = p.R && row < p.M ? p.R + r_mat * p.r_stride + static_cast<long long>(row) * p.ldr : nullptr;
-  uint4 r[4] = {};
-  auto fetch = [&](int col) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const uint4*>(R + col + 8 * j);
-  };
-  if (R && col0 < p.ldr) fetch(col0);
-#pragma unroll 1
-  for (int c = 0; c < NCOL && col0 + c < N; c += 32) {
+  auto piece_of = [&](int c, uint4 (&r)[4]) {
     const int col = col0 + c;
     uint32_t v[32];
     tmem_ld32(taddr + c, v);
@@ -463,7 +484,7 @@ __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtenso
     float f[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
-    if (R) {
+    if (add.R) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
@@ -474,7 +495,6 @@ __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtenso
           f[8 * j + 2 * i + 1] += p.beta * r2.y;
         }
       }
-      if (c + 32 < NCOL && col + 32 < p.ldr) fetch(col + 32);
     }
     if (p.gamma != 0.f) {
 #pragma unroll
@@ -514,6 +534,14 @@ __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtenso
     }
     __syncwarp();
     ++pieces;
+  };
+#pragma unroll 1
+  for (int c = 0; c < NCOL && col0 + c < N; c += 64) {
+    piece_of(c, add.r[0]);
+    if (c + 64 < NCOL) add.fetch(col0 + c + 64, 0);
+    if (col0 + c + 32 >= N) break;
+    piece_of(c + 32, add.r[1]);
+    if (c + 64 < NCOL) add.fetch(col0 + c + 96, 1);
   }
 }
 
@@ -528,6 +556,13 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
   uint64_t* tempty_bar = tfull_bar + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 32) {
+    for (int c = 0; c < (p.cls[1].count ? 2 : 1); ++c) {
+      prefetch_tmap(&maps.a[c]);
+      prefetch_tmap(&maps.b[c]);
+      prefetch_tmap(&maps.c[c]);
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < OG_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -622,11 +657,12 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
     for (int tile = blockIdx.x; tile < p.total; tile += gridDim.x) {
       int cls, mat, ti, tj;
       ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+      Addend add(p, mat, ti * TILE + q * 32 + lane, tj * TILE + part * (TILE / 2));
       if (!__all_sync(0xffffffffu, own_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
       ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
                                tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
-                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), mat, ti * TILE + q * 32, tj * TILE + part * (TILE / 2),
+                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), add, ti * TILE + q * 32, tj * TILE + part * (TILE / 2),
                                cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
       tc_fence_before();
       __syncwarp();
@@ -655,6 +691,13 @@ ortho_gemm_pair_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = cluster_ctarank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  if (threadIdx.x == 32) {
+    for (int c = 0; c < (p.cls[1].count ? 2 : 1); ++c) {
+      prefetch_tmap(&maps.a[c]);
+      prefetch_tmap(&maps.b[c]);
+      prefetch_tmap(&maps.c[c]);
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < OG_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -753,11 +796,12 @@ ortho_gemm_pair_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p
     for (int tile = cluster; tile < p.total; tile += clusters) {
       int cls, mat, ti, tj;
       ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+      Addend add(p, mat, ti * TILE + crank * 128 + q * 32 + lane, tj * TILE + part * (TILE / 2));
       if (!__all_sync(0xffffffffu, own_poll(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
       ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
                                tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
-                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), mat, ti * TILE + crank * 128 + q * 32,
+                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), add, ti * TILE + crank * 128 + q * 32,
                                tj * TILE + part * (TILE / 2), cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
       tc_fence_before();
       __syncwarp();
@@ -1080,18 +1124,19 @@ struct Products {
       const long long m = (p.M + tile - 1) / tile, n = (p.cls[c].N + tile - 1) / tile;
       return p.sym ? m * (m + 1) / 2 : m * n;
     };
-    // The work of the busiest unit in blocks of 64 of the reduction, each tile with a fixed cost, twice as long for a pair's tile.
-    auto cost = [&](int tile, int units) {
+    // us of a launch: a start and an end, and for every round of tiles a fixed part and one per block of 64 of the reduction (the
+    // mean over both classes). Measured, single / pair: 10 x 333 rows and columns over 384 8.2 / 11.0, 8 x (512 x 2048 over 512)
+    // 15.6 / 14.9, 6 x (1024 x 4096 over 1024) 53.7 / 43.5, 16 x 1536 over 1536 68.7 / 58.3, 2 x 1536 over 4096 37.1 / 31.0.
+    auto cost = [&](int tile, int units, double ends, double round, double block) {
       long long total = 0, blocks = 0;
       for (int c = 0; c < NS_CLASSES; ++c) {
         const long long n = tiles(c, tile) * p.cls[c].count;
         total += n;
         blocks += n * ((p.cls[c].K + OG_BK - 1) / OG_BK);
       }
-      const long long rounds = (total + units - 1) / units;
-      return static_cast<double>(rounds) * (static_cast<double>(blocks) / total + TILE_COST);
+      return ends + static_cast<double>((total + units - 1) / units) * (round + block * blocks / total);
     };
-    const bool pair = PAIR_COST * cost(256, pairs) < cost(128, sms);
+    const bool pair = cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
     const int tile = pair ? 256 : 128, units = pair ? pairs : sms;
     long long total = 0;
     for (int c = 0; c < NS_CLASSES; ++c) total += tiles(c, tile) * p.cls[c].count;
@@ -1105,8 +1150,6 @@ struct Products {
     rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : ortho_gemm_kernel<B_MN>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
     ++launches;
   }
-  static constexpr double TILE_COST = 6, PAIR_COST = 1.6;
-
   OrthoGemm empty() const {
     OrthoGemm p{};
     for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].N = p.cls[c].K = 1;      // a class without matrices
