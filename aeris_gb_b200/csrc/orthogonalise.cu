@@ -376,10 +376,14 @@ __global__ void __launch_bounds__(256) ortho_finish_kernel(const OrthoGroups a, 
 struct OrthoClass {
   int tiles, count, N, K;                     // tiles per matrix
   int a0, b0, c0;                             // first matrix of the class in the tensor maps of A, B and C
+  // `splits` > 1 (128 x 128 tiles): so many CTAs share a tile's reduction and leave their sums in `partial`, one behind the other.
+  // `low` > 0: A comes in two parts, and the reduction goes over B's rows with both, the second one `low` matrices on
+  int splits, low;
 };
 struct OrthoGemm {
   OrthoClass cls[NS_CLASSES];
   int total, M, sym;                          // tiles in all
+  float* partial;                             // splits: [matrix, tile, split, 128, 128]
   const __half* R;                            // null, or [matrices, M] rows of pitch ldr
   long long r_stride;
   int ldr;
@@ -545,6 +549,34 @@ __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtenso
   }
 }
 
+// The tile that unit `unit` of a launch of single CTAs works on, and its blocks of the reduction.
+__device__ __forceinline__ int ortho_blocks(const OrthoGemm& p, int unit, int& kb0, int& kb1) {
+  const int splits = p.cls[0].splits, n0 = p.cls[0].tiles * p.cls[0].count;
+  const int tile = splits > 1 ? unit / splits : unit;
+  const bool second = tile >= n0;
+  const int blocks = ((second ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK * ((second ? p.cls[1].low : p.cls[0].low) ? 2 : 1);
+  kb0 = 0;
+  kb1 = blocks;
+  if (splits > 1) {
+    const int each = (blocks + splits - 1) / splits;
+    kb0 = (unit - tile * splits) * each;
+    kb1 = min(blocks, kb0 + each);
+  }
+  return tile;
+}
+// 32-bit sums of a lane's row
+template <int NCOL> __device__ __forceinline__ void ortho_partial(float* to, uint32_t taddr) {
+#pragma unroll 1
+  for (int c = 0; c < NCOL; c += 32) {
+    uint32_t v[32];
+    tmem_ld32(taddr + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint4*>(to + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+
 template <int B_MN>
 __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p) {
   constexpr int TILE = 128;
@@ -589,24 +621,25 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x) {
-        int cls, mat, ti, tj;
-        ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+      for (int unit = blockIdx.x; unit < p.total && ok; unit += gridDim.x) {
+        int cls, mat, ti, tj, kb0, kb1;
+        ortho_tile<TILE>(p, ortho_blocks(p, unit, kb0, kb1), cls, mat, ti, tj);
         const CUtensorMap *ta = cls ? &maps.a[1] : &maps.a[0], *tb = cls ? &maps.b[1] : &maps.b[0];
         const int ma = mat + (cls ? p.cls[1].a0 : p.cls[0].a0), mb = mat + (cls ? p.cls[1].b0 : p.cls[0].b0);
-        const int kb_total = ((cls ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
-        for (int kb = 0; kb < kb_total; ++kb) {
+        const int low_from = p.cls[0].low ? (p.cls[0].K + OG_BK - 1) / OG_BK : kb1, low = cls ? p.cls[1].low : p.cls[0].low;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const int k = (kb < low_from ? kb : kb - low_from) * OG_BK, ma_now = ma + (kb < low_from ? 0 : low);
           if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
           uint8_t* sa = smem + stage * OG_STAGE;
           uint8_t* sb = sa + OG_OPERAND;
           mbar_expect_tx(&full_bar[stage], OG_STAGE);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            tma_load_3d(sa + j * 8192, ta, &full_bar[stage], kb * OG_BK, ti * TILE + j * 64, ma);
+            tma_load_3d(sa + j * 8192, ta, &full_bar[stage], k, ti * TILE + j * 64, ma_now);
             if (B_MN)
-              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], tj * TILE + j * 64, kb * OG_BK, mb);
+              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], tj * TILE + j * 64, k, mb);
             else
-              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], kb * OG_BK, tj * TILE + j * 64, mb);
+              tma_load_3d(sb + j * 8192, tb, &full_bar[stage], k, tj * TILE + j * 64, mb);
           }
           if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         }
@@ -623,12 +656,13 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < p.total && ok; tile += gridDim.x) {
-        const int kb_total = ((tile >= p.cls[0].tiles * p.cls[0].count ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
+      for (int unit = blockIdx.x; unit < p.total && ok; unit += gridDim.x) {
+        int kb0, kb1;
+        ortho_blocks(p, unit, kb0, kb1);
         if (!own_wait(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
         const uint32_t tmem_acc = tmem_base + acc * TILE;
-        for (int kb = 0; kb < kb_total; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!own_wait(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * OG_STAGE), sb = sa + OG_OPERAND;
@@ -636,7 +670,7 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
           for (int kk = 0; kk < OG_BK / 16; ++kk)
             umma_ss(tmem_acc, make_smem_desc(sa + kk * 32, 0, 1024),
                     B_MN ? make_smem_desc(sb + kk * 2048, 8192, 1024) : make_smem_desc(sb + kk * 32, 0, 1024), idesc,
-                    kb > 0 || kk > 0);
+                    kb > kb0 || kk > 0);
           tc_commit(&empty_bar[stage]);
           if (++stage == OG_STAGES) { stage = 0; phase ^= 1; }
         }
@@ -654,16 +688,20 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
     int acc = 0, pieces = 0;
     uint32_t acc_phase = 0;
     const bool keep = !failed(p.status);
-    for (int tile = blockIdx.x; tile < p.total; tile += gridDim.x) {
-      int cls, mat, ti, tj;
-      ortho_tile<TILE>(p, tile, cls, mat, ti, tj);
+    for (int unit = blockIdx.x; unit < p.total; unit += gridDim.x) {
+      int cls, mat, ti, tj, kb0, kb1;
+      ortho_tile<TILE>(p, ortho_blocks(p, unit, kb0, kb1), cls, mat, ti, tj);
       Addend add(p, mat, ti * TILE + q * 32 + lane, tj * TILE + part * (TILE / 2));
       if (!__all_sync(0xffffffffu, own_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
-      ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
-                               tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
-                               mat + (cls ? p.cls[1].c0 : p.cls[0].c0), add, ti * TILE + q * 32, tj * TILE + part * (TILE / 2),
-                               cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
+      if (p.partial)
+        ortho_partial<TILE / 2>(p.partial + static_cast<long long>(unit) * (TILE * TILE) + (q * 32 + lane) * TILE + part * (TILE / 2),
+                                tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16));
+      else
+        ortho_epilogue<TILE / 2>(p, cls ? &maps.c[1] : &maps.c[0], out,
+                                 tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16),
+                                 mat + (cls ? p.cls[1].c0 : p.cls[0].c0), add, ti * TILE + q * 32, tj * TILE + part * (TILE / 2),
+                                 cls ? p.cls[1].N : p.cls[0].N, keep, p.sym && ti != tj, lane, pieces);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[acc]);
@@ -872,25 +910,37 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   const OrthoPlace p = ortho_place(a);
   const OrthoGroup& m = a.g[p.group];
   const bool upright = m.rows > m.cols;
-  const int d = upright ? m.cols : m.rows, K = upright ? m.rows : m.cols, n = m.rows * m.cols;
+  const int d = upright ? m.cols : m.rows, K = upright ? m.rows : m.cols;
   const int blocks = (K + 63) / 64;
   for (int i = threadIdx.x; i < blocks * OS_BLOCK / 16; i += OS_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   const float gs = STEP ? step_scale(in) : 0.f;
   double sum = 0;
-  if (p.found) {
-    for (int v = threadIdx.x; v < n; v += OS_THREADS) {
-      const long long e = m.ld == m.cols ? p.at + v : p.at + static_cast<long long>(v / m.cols) * m.ld + v % m.cols;
-      float u;
+  // a warp takes a row at a time, a lane up to U of its elements 32 apart
+  constexpr int U = 4;
+  auto rows = [&](int ld, long long at, auto work) {
+    for (int r = warp; r < m.rows; r += OS_THREADS / 32)
+      for (int c = lane; c < m.cols; c += 32 * U) work(r, c, at + static_cast<long long>(r) * ld + c, min(U, (m.cols - c + 31) / 32));
+  };
+  if (p.found)
+    rows(m.ld, p.at, [&](int, int, long long e, int k_end) {
+      float x[U] = {}, y[U] = {};
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (k < k_end) {
+          x[k] = STEP ? in.grad[e + 32 * k] : in_value(in, e + 32 * k);
+          if (STEP) y[k] = in.momentum[e + 32 * k];
+        }
       if (STEP) {
-        const float g = clean(in.grad[e] * gs), mom = in.beta * in.momentum[e] + (1.f - in.beta) * g;
-        in.momentum[e] = mom;
-        u = in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom;
-      } else {
-        u = in_value(in, e);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const float g = clean(x[k] * gs), mom = in.beta * y[k] + (1.f - in.beta) * g;
+          if (k < k_end) in.momentum[e + 32 * k] = mom;
+          x[k] = k >= k_end ? 0.f : in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom;
+        }
       }
-      sum += static_cast<double>(u) * u;
-    }
-  }
+      const float4 u[1] = {make_float4(x[0], x[1], x[2], x[3])};
+      sum += squares_of(u);
+    });
   for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
   if (lane == 0) red[warp] = sum;
   __syncthreads();
@@ -898,46 +948,56 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   for (int i = 0; i < OS_THREADS / 32; ++i) sum += red[i];
   const double norm = sqrt(sum);
   const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
-  if (p.found) {                              // each thread reads what it has written
-    for (int v = threadIdx.x; v < n; v += OS_THREADS) {
-      const int r = v / m.cols, c = v - r * m.cols;
-      const long long e = p.at + static_cast<long long>(r) * m.ld + c;
-      float u;
-      if (STEP) {
-        const float g = clean(in.grad[e] * gs), mom = in.momentum[e];
-        u = in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom;
-        if (in.zero_grad) in.grad[e] = 0.f;
-      } else {
-        u = in_value(in, e);
-      }
-      *reinterpret_cast<__half*>(smem + (upright ? os_at(c, r) : os_at(r, c))) = __float2half_rn(scale * u);
-    }
-  }
+  if (p.found)                                // each thread reads what it has written
+    rows(m.ld, p.at, [&](int r, int c, long long e, int k_end) {
+      float x[U], y[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (k < k_end) {
+          x[k] = STEP ? in.grad[e + 32 * k] : in_value(in, e + 32 * k);
+          if (STEP) y[k] = in.momentum[e + 32 * k];
+        }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (k < k_end) {
+          float u = x[k];
+          if (STEP) {
+            const float g = clean(x[k] * gs);
+            u = in.nesterov ? in.beta * y[k] + (1.f - in.beta) * g : y[k];
+            if (in.zero_grad) in.grad[e + 32 * k] = 0.f;
+          }
+          const int col = c + 32 * k;
+          *reinterpret_cast<__half*>(smem + (upright ? os_at(col, r) : os_at(r, col))) = __float2half_rn(scale * u);
+        }
+    });
 
   const int q = warp & 3, part = warp >> 2, row = q * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16, t_s = tmem + OS_MAX_K;
   const uint32_t x_at = smem_u32(smem), s_at = smem_u32(smem + OS_S), p_at = smem_u32(smem + OS_P);
   const int wide = d > 64 ? 128 : 64;         // columns of the square factors
   uint32_t phase = 0;
-  // all threads: what they wrote to shared memory is there for the products, which thread 0 issues and all wait for
+  bool ok = true;
+  const uint32_t lead = lane == 0;
+  // all threads: what they wrote to shared memory is there for the products, which warp 0 issues and all wait for
   auto products = [&](auto issue) {
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
       tc_fence_after();
       issue();
-      tc_commit(bar);
+      tc_commit_warp(lead, smem_u32(bar));
     }
-    if (!own_wait(bar, phase, a.status, ERR_TIMEOUT_TMEM_FULL)) *gave_up = 1;
+    ok = ok && mbar_wait_warp(bar, phase, a.status, ERR_TIMEOUT_TMEM_FULL);
+    if (!ok) *gave_up = 1;
     phase ^= 1;
     tc_fence_after();
   };
   for (int step = 0; step < steps; ++step) {
     products([&] {
-      for (int k = 0; k < blocks * 4; ++k) {
-        const uint64_t desc = make_smem_desc(x_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024);
-        umma_ss(t_s, desc, desc, make_idesc_fp16(128, wide, 0), k > 0);
+      for (int k = 0; k < blocks; ++k) {
+        const uint32_t lo = smem_desc_lo(x_at + k * OS_BLOCK, 0);
+        umma_ss4_warp<2, 2>(lead, t_s, lo, lo, make_idesc_fp16(128, wide, 0), k > 0);
       }
     });
     float s[64];
@@ -955,9 +1015,9 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
       os_put(smem + OS_S, row, c0 + 32 * h, f);
     }
     products([&] {
-      for (int k = 0; k < wide / 16; ++k) {
-        const uint64_t desc = make_smem_desc(s_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024);
-        umma_ss(t_s, desc, desc, make_idesc_fp16(128, wide, 0), k > 0);
+      for (int k = 0; k < wide / 64; ++k) {
+        const uint32_t lo = smem_desc_lo(s_at + k * OS_BLOCK, 0);
+        umma_ss4_warp<2, 2>(lead, t_s, lo, lo, make_idesc_fp16(128, wide, 0), k > 0);
       }
     });
 #pragma unroll
@@ -975,9 +1035,9 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
     products([&] {
       for (int c = 0; c < blocks * 64; c += 256) {
         const int cols = min(256, blocks * 64 - c);
-        for (int k = 0; k < wide / 16; ++k)
-          umma_ss(tmem + c, make_smem_desc(p_at + (k >> 2) * OS_BLOCK + (k & 3) * 32, 0, 1024),
-                  make_smem_desc(x_at + (c >> 6) * OS_BLOCK + k * 2048, OS_BLOCK, 1024), make_idesc_fp16(128, cols, 1), k > 0);
+        for (int k = 0; k < wide / 64; ++k)
+          umma_ss4_warp<2, 128>(lead, tmem + c, smem_desc_lo(p_at + k * OS_BLOCK, 0),
+                                smem_desc_lo(x_at + (c >> 6) * OS_BLOCK + k * 8192, OS_BLOCK), make_idesc_fp16(128, cols, 1), k > 0);
       }
     });
     for (int c = part * 32; c < blocks * 64; c += 64) {
@@ -997,18 +1057,205 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   const OrthoGroup& t = b.g[p.group];
   if (!p.found || *gave_up || failed(a.status)) return;
   const long long out_at = t.offsets ? p.at : p.matrix * t.stride;
-  for (int v = threadIdx.x; v < n; v += OS_THREADS) {
-    const int r = v / m.cols, c = v - r * m.cols;
-    const float x = __half2float(*reinterpret_cast<const __half*>(smem + (upright ? os_at(c, r) : os_at(r, c)))) * (1.f / NS_SCALE);
-    const long long e = out_at + static_cast<long long>(r) * t.ld + c;
-    if (!STEP) {
-      o.out[e] = __float2bfloat16_rn(x);
-      continue;
+  rows(t.ld, out_at, [&](int r, int c, long long e, int k_end) {
+    float w[U], ema[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (STEP && k < k_end) {
+        w[k] = o.master[e + 32 * k];
+        if (o.ema && o.ema_beta >= 0.f) ema[k] = o.ema[e + 32 * k];
+      }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (k < k_end) {
+        const int col = c + 32 * k;
+        const float x = __half2float(*reinterpret_cast<const __half*>(smem + (upright ? os_at(col, r) : os_at(r, col)))) * (1.f / NS_SCALE);
+        if (!STEP) {
+          o.out[e + 32 * k] = __float2bfloat16_rn(x);
+          continue;
+        }
+        const float now = w[k] * o.decay - m.rate * x;
+        o.master[e + 32 * k] = now;
+        if (o.weights) o.weights[e + 32 * k] = __float2bfloat16_rn(now);
+        if (o.ema && o.ema_beta >= 0.f) o.ema[e + 32 * k] = now + o.ema_beta * (ema[k] - now);
+      }
+  });
+}
+
+// ------------------------------------------------------------------------------------------------ few rows, long ones
+// d <= 128 and longer rows: all steps on the Gram matrix alone, one CTA a matrix, and X is read twice instead of ten times. What
+// keeps groups of steps from being longer than two elsewhere, the Gram matrix's rounding, is answered by precision here: sums of
+// X X^T stay in 32 bits, and the [d, d] factors are kept as two fp16 numbers (22 bits), which a product takes as three. Their
+// product Q is applied in both parts too: its entries reach a^5, and rounded to 11 bits they would leave 0.1 of a large direction.
+constexpr float NS_Q_SCALE = 64.f;
+constexpr int OL_MAX_STEPS = 5;               // a^5 times the scale is inside fp16's range
+constexpr int OL_S = 0, OL_P = 4 * OS_BLOCK, OL_Q = 8 * OS_BLOCK, OL_BARS = 12 * OS_BLOCK;      // hi, then lo
+constexpr int OL_SMEM = OL_BARS + 256 + 1024;
+constexpr int OL_MAX_SPLITS = 12;
+
+__device__ __forceinline__ void split_half(const float (&f)[32], float (&lo)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) lo[j] = f[j] - __half2float(__float2half_rn(f[j]));
+}
+__device__ __forceinline__ void os_put2(uint8_t* to, int row, int col, const float (&f)[32]) {
+  float lo[32];
+  split_half(f, lo);
+  os_put(to, row, col, f);
+  os_put(to + 2 * OS_BLOCK, row, col, lo);
+}
+
+// `partial`: [matrix, split, 128, 128] sums of X X^T; Q: [2, count] matrices of d rows of pitch ld (hi, lo).
+__global__ void __launch_bounds__(OS_THREADS, 1)
+ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* __restrict__ Q, int count, int d, int ld, int steps,
+                        int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + OL_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  chain_point();
+
+  const int q = warp & 3, part = warp >> 2, row = q * 32 + lane;
+  const int wide = d > 64 ? 128 : 64, mine = wide / 2, c0 = part * mine;
+  const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+  uint8_t *S = smem + OL_S, *P = smem + OL_P, *QQ = smem + OL_Q;
+  uint32_t phase = 0;
+  auto begin = [&] {
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  const uint32_t lead = lane == 0;
+  auto product = [&](uint32_t to, const uint8_t* a, const uint8_t* b) {        // warp 0; small terms first
+    const uint32_t a_hi = smem_desc_lo(smem_u32(a), 0), b_hi = smem_desc_lo(smem_u32(b), 0);
+    constexpr uint32_t BLOCK = OS_BLOCK / 16, LO = 2 * BLOCK;
+    const uint32_t idesc = make_idesc_fp16(128, wide, 0);
+    for (int k = 0; k < wide / 64; ++k) umma_ss4_warp<2, 2>(lead, tmem + to, a_hi + LO + k * BLOCK, b_hi + k * BLOCK, idesc, k > 0);
+    for (int k = 0; k < wide / 64; ++k) umma_ss4_warp<2, 2>(lead, tmem + to, a_hi + k * BLOCK, b_hi + LO + k * BLOCK, idesc, 1);
+    for (int k = 0; k < wide / 64; ++k) umma_ss4_warp<2, 2>(lead, tmem + to, a_hi + k * BLOCK, b_hi + k * BLOCK, idesc, 1);
+  };
+  bool ok = true;
+  auto finish = [&] {
+    if (warp == 0) tc_commit_warp(lead, smem_u32(bar));
+    ok = ok && mbar_wait_warp(bar, phase, status, ERR_TIMEOUT_TMEM_FULL);
+    phase ^= 1;
+    tc_fence_after();
+  };
+  // the sums, side by side through the (still free) place of Q, whose 16-byte chunks are swizzled by row
+  float4* sums = reinterpret_cast<float4*>(QQ);
+  const float4* from = reinterpret_cast<const float4*>(partial) + static_cast<long long>(blockIdx.x) * splits * (128 * 32);
+  for (int i = threadIdx.x; i < wide * (wide / 4); i += OS_THREADS) {
+    const int r = i / (wide / 4), c = i % (wide / 4);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 y = from[k * (128 * 32) + r * 32 + c];
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    const float w = o.master[e] * o.decay - m.rate * x;
-    o.master[e] = w;
-    if (o.weights) o.weights[e] = __float2bfloat16_rn(w);
-    if (o.ema && o.ema_beta >= 0.f) o.ema[e] = w + o.ema_beta * (o.ema[e] - w);
+    sums[r * 32 + (c ^ (r & 7))] = x;
+  }
+  __syncthreads();
+  float s[64];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (32 * h >= mine) break;
+    float f[32];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 x = row < wide ? sums[row * 32 + (((c0 + 32 * h) / 4 + j) ^ (row & 7))] : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[4 * j] = x.x; f[4 * j + 1] = x.y; f[4 * j + 2] = x.z; f[4 * j + 3] = x.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[32 * h + j] = f[j] *= 1.f / NS_SCALE;
+    os_put2(S, row, c0 + 32 * h, f);
+  }
+  __syncthreads();                            // all sums are taken before Q comes
+  // this lane's columns c0 + 32 h .. of an accumulator, times alpha
+  auto take = [&](uint32_t from, int h, float alpha, float (&f)[32]) {
+    uint32_t v[32];
+    tmem_ld32(tmem + from + lanes + c0 + 32 * h, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = alpha * __uint_as_float(v[j]);
+  };
+  for (int step = 0; step < steps; ++step) {
+    const bool last = step + 1 == steps;
+    begin();
+    if (warp == 0) product(0, S, S);
+    finish();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= mine) break;
+      float f[32];
+      take(0, h, NS_C / NS_SCALE, f);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] += NS_B * s[32 * h + j] + (row == c0 + 32 * h + j ? NS_A * NS_SCALE : 0.f);
+      os_put2(P, row, c0 + 32 * h, f);
+      if (step == 0) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] *= NS_Q_SCALE / NS_SCALE;
+        os_put2(QQ, row, c0 + 32 * h, f);
+      }
+    }
+    if (step || !last) {
+      begin();
+      if (warp == 0) {
+        if (step) product(128, P, QQ);
+        if (!last) product(0, P, S);
+      }
+      finish();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= mine) break;
+      float f[32];
+      if (step) {
+        take(128, h, 1.f / NS_SCALE, f);
+        os_put2(QQ, row, c0 + 32 * h, f);
+      }
+      if (!last) {
+        take(0, h, 1.f / NS_SCALE, f);
+        os_put2(S, row, c0 + 32 * h, f);      // P S takes the place of S
+      }
+    }
+    if (last) break;
+    begin();
+    if (warp == 0) product(0, S, P);
+    finish();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= mine) break;
+      float f[32];
+      take(0, h, 1.f / NS_SCALE, f);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s[32 * h + j] = f[j];
+      os_put2(S, row, c0 + 32 * h, f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 256);
+  __half* to = Q + static_cast<long long>(blockIdx.x) * d * ld;
+  const long long low = static_cast<long long>(count) * d * ld;
+  for (int i = threadIdx.x; i < d * (wide / 8); i += OS_THREADS) {
+    const int r = i / (wide / 8), c = i % (wide / 8) * 8;
+    if (c >= ld) continue;
+    *reinterpret_cast<uint4*>(to + r * ld + c) = *reinterpret_cast<const uint4*>(QQ + os_at(r, c));
+    *reinterpret_cast<uint4*>(to + low + r * ld + c) = *reinterpret_cast<const uint4*>(QQ + 2 * OS_BLOCK + os_at(r, c));
   }
 }
 
@@ -1044,12 +1291,21 @@ enum Factor { F_S, F_P0, F_T, F_P1 };         // where the [d, d] factors of a b
 struct Layout {
   int d, count, classes, K[NS_CLASSES], members[NS_CLASSES], group_class[NS_GROUPS], group_first[NS_GROUPS];
   Groups steps;
-  long long x_at[NS_CLASSES], s_at, bytes;
+  bool few;                                   // all steps on the Gram matrix
+  long long x_at[NS_CLASSES], s_at, partial_at, bytes;
   long long x_stride(int c) const { return static_cast<long long>(d) * pitch(K[c]); }
   long long s_stride() const { return static_cast<long long>(d) * pitch(d); }
   int fill(const AerisOrtho& a);
 };
 bool small(const Layout& l) { return l.d <= OS_MAX_D && l.K[0] <= OS_MAX_K; }
+// CTAs that share one matrix's X X^T where rows are few: eight blocks of 64 each, up to OL_MAX_SPLITS. By the length alone, so that
+// a matrix has the same bits in every batch.
+int splits_of(const Layout& l, int c) {
+  const int blocks = (l.K[c] + OG_BK - 1) / OG_BK, s = blocks / 8 < OL_MAX_SPLITS ? blocks / 8 : OL_MAX_SPLITS;
+  if (s < 2) return 1;
+  const int each = (blocks + s - 1) / s;
+  return (blocks + each - 1) / each;          // none of them empty
+}
 int Layout::fill(const AerisOrtho& a) {
   if (a.groups < 1 || a.groups > NS_GROUPS || a.steps < 1 || a.steps > 20) return -1;
   d = count = classes = 0;
@@ -1074,7 +1330,9 @@ int Layout::fill(const AerisOrtho& a) {
     for (int i = 0; i < a.groups; ++i) group_class[i] ^= 1;
   }
   bytes = 0;
+  few = false;
   if (small(*this)) return 0;                 // everything in shared memory
+  few = d <= OS_MAX_D && a.steps <= OL_MAX_STEPS;
   steps = groups_of(d, K[0], a.steps);
   bytes = (static_cast<long long>(count) * NS_PARTS * 8 + 1023) / 1024 * 1024;
   for (int c = 0; c < classes; ++c) {
@@ -1082,7 +1340,12 @@ int Layout::fill(const AerisOrtho& a) {
     bytes += (2ll * members[c] * x_stride(c) * 2 + 1023) / 1024 * 1024;
   }
   s_at = bytes;
-  bytes += static_cast<long long>(buffers_of(steps)) * count * s_stride() * 2;
+  bytes += (static_cast<long long>(few ? 2 : buffers_of(steps)) * count * s_stride() * 2 + 1023) / 1024 * 1024;
+  partial_at = bytes;
+  if (few) {
+    if (classes > 1) return -10;
+    bytes += static_cast<long long>(splits_of(*this, 0)) * count * (128 * 128 * 4);
+  }
   return 0;
 }
 
@@ -1097,7 +1360,7 @@ struct Products {
 
   Products(const Layout& layout, char* work, int* status_, cudaStream_t stream_) : l(layout), status(status_), stream(stream_) {
     S = reinterpret_cast<__half*>(work + l.s_at);
-    const uint64_t factors = static_cast<uint64_t>(buffers_of(l.steps)) * l.count;
+    const uint64_t factors = static_cast<uint64_t>(l.few ? 2 : buffers_of(l.steps)) * l.count;
     rc = make_tmap_3d_fp16(&load_s, S, l.d, l.d, factors, pitch(l.d), 64, 64);
     if (!rc) rc = make_tmap_3d_fp16(&store_s, S, l.d, l.d, factors, pitch(l.d), 32, 32);
     for (int c = 0; c < l.classes; ++c) {
@@ -1136,7 +1399,7 @@ struct Products {
       }
       return ends + static_cast<double>((total + units - 1) / units) * (round + block * blocks / total);
     };
-    const bool pair = cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
+    const bool pair = p.partial == nullptr && p.cls[0].low == 0 && cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
     const int tile = pair ? 256 : 128, units = pair ? pairs : sms;
     long long total = 0;
     for (int c = 0; c < NS_CLASSES; ++c) total += tiles(c, tile) * p.cls[c].count;
@@ -1145,7 +1408,7 @@ struct Products {
       return;
     }
     for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles(c, tile));
-    p.total = static_cast<int>(total);
+    p.total = static_cast<int>(total) * (p.cls[0].splits > 1 ? p.cls[0].splits : 1);
     const int grid = (p.total < units ? p.total : units) * (pair ? 2 : 1);
     rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : ortho_gemm_kernel<B_MN>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
     ++launches;
@@ -1215,6 +1478,42 @@ struct Products {
     }
     launch<1>(m, p);
   }
+  // all steps on X number 0, into the other one
+  void few(float* partial, int splits, int steps) {
+    OrthoGemm g = empty();
+    OrthoMaps m = square();
+    g.sym = 1;
+    m.a[0] = m.b[0] = load_x[0];
+    g.cls[0].count = l.count;
+    g.cls[0].N = l.d;
+    g.cls[0].K = l.K[0];
+    g.cls[0].splits = splits;
+    g.partial = partial;
+    launch<0>(m, g);
+    if (rc) return;
+    static bool configured = false;
+    if (!configured) {
+      if (cudaFuncSetAttribute(ortho_polynomial_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OL_SMEM) != cudaSuccess) {
+        rc = -20;
+        return;
+      }
+      configured = true;
+    }
+    rc = launch_chained(ortho_polynomial_kernel, l.count, OS_THREADS, OL_SMEM, stream, static_cast<const float*>(partial), splits, S,
+                        l.count, l.d, pitch(l.d), steps, status);
+    ++launches;
+    OrthoGemm u = empty();
+    m = square();
+    m.b[0] = load_x[0];
+    m.c[0] = store_x[0];
+    u.cls[0].count = l.count;
+    u.cls[0].N = l.K[0];
+    u.cls[0].K = l.d;
+    u.cls[0].low = l.count;
+    u.cls[0].c0 = l.count;
+    u.alpha = 1.f / NS_Q_SCALE;
+    launch<1>(m, u);
+  }
   void group(int from, int steps) {           // one or two steps on X number `from`, into the other one
     gram(from);
     polynomial(F_P0);
@@ -1283,7 +1582,7 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
     out.g[i] = o;
     out.g[i].blocks = static_cast<int>(pack_blocks[i]);
     if (!step) out.g[i].stride = g.out_stride, out.g[i].ld = g.ld_out;
-    if (l.bytes && (l.steps.n & 1)) out.g[i].x += l.members[c] * o.x_stride;
+    if (l.bytes && (l.few || (l.steps.n & 1))) out.g[i].x += l.members[c] * o.x_stride;
   }
   auto blocks = [&](const OrthoGroups& g) {
     long long n = 0;
@@ -1314,7 +1613,10 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   for (int i = 0; i < a.groups; ++i) in.g[i].blocks = static_cast<int>(pack_blocks[i]);
   rc = launch_chained(step ? ortho_pack_kernel<true> : ortho_pack_kernel<false>, blocks(in), 256, 0, stream, in, input, a.eps);
   if (rc) return rc;
-  for (int k = 0; k < l.steps.n; ++k) run.group(k & 1, l.steps.size[k]);
+  if (l.few)
+    run.few(reinterpret_cast<float*>(work + l.partial_at), splits_of(l, 0), a.steps);
+  else
+    for (int k = 0; k < l.steps.n; ++k) run.group(k & 1, l.steps.size[k]);
   if (run.rc) return run.rc;
   rc = launch_chained(step ? ortho_finish_kernel<true> : ortho_finish_kernel<false>, blocks(out), 256, 0, stream, out, output);
   return rc ? rc : run.launches + 3;

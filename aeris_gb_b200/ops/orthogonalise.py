@@ -18,6 +18,7 @@ _P, _I, _F, _LL, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_lo
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_GROUPS, MAX_LENGTHS = 4, 2       # shapes of a batch, and longer sides among them
 MAX_COUNT = 1 << 16                  # matrices of a group
+FEW_ROWS, SHORT_ROWS = 128, 384      # up to so many rows (d) matrices with rows longer than that have a batch for each length
 WORKSPACE_BYTES = 1 << 30            # of one batch; what does not fit goes in several
 
 
@@ -37,8 +38,9 @@ class _Args(ctypes.Structure):
 
 
 def _bytes_per_matrix(d: int, k: int) -> int:
-    """Workspace of one matrix, at most: two X, four square factors, partial sums."""
-    return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 8192
+    """Workspace of one matrix, about: two X, four square factors, partial sums."""
+    few = min(16, max(1, k // 512)) * 65536 if d <= FEW_ROWS and k > SHORT_ROWS else 0
+    return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 8192 + few
 
 
 def _run(a: _Args, device) -> None:
@@ -116,10 +118,11 @@ def _batches(groups):
     """Cuts groups (rows, cols, address of the offsets, how many) into batches: lists of (rows, cols, address, how many, whether
     an entry of the same table lies before it) with one shorter side, at most MAX_LENGTHS longer ones, MAX_GROUPS parts and
     WORKSPACE_BYTES. Shapes with one shorter side share the launches of their square factors."""
-    by_side: dict[int, list] = {}
+    by_side: dict[tuple[int, int], list] = {}
     for g in groups:
-        by_side.setdefault(min(g[:2]), []).append(g)
-    for d, todo in by_side.items():
+        d, k = min(g[:2]), max(g[:2])
+        by_side.setdefault((d, k if d <= FEW_ROWS and k > SHORT_ROWS else 0), []).append(g)
+    for (d, _), todo in by_side.items():
         batch, lengths, room = [], set(), WORKSPACE_BYTES
         todo = [(*g, False) for g in todo][::-1]
         while todo:

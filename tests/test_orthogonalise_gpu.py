@@ -65,7 +65,8 @@ def gradient(*shape, noise=0.5, seed=0):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (200, 3), (31, 33), (63, 65), (64, 64), (65, 64), (128, 128), (128, 129), (129, 127),
-          (127, 640), (192, 192), (256, 256), (257, 300), (300, 257), (384, 1024), (1001, 333), (320, 2000), (515, 515), (768, 640)]
+          (127, 640), (192, 192), (256, 256), (257, 300), (300, 257), (384, 1024), (1001, 333), (320, 2000), (515, 515), (768, 640),
+          (1, 385), (2, 5000), (64, 4000), (65, 700), (100, 13001), (128, 8192), (5000, 96), (150, 9000)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
@@ -76,7 +77,8 @@ def test_one_matrix(shape, dt):
 
 
 @pytest.mark.parametrize("count,rows,cols", [(3, 5, 9), (2, 64, 64), (40, 64, 64), (7, 100, 60), (3, 130, 260), (300, 16, 16),
-                                             (5, 333, 200), (2, 512, 1536), (9, 384, 384)])
+                                             (5, 333, 200), (2, 512, 1536), (9, 384, 384),
+                                             (3, 40, 6000), (200, 128, 400), (160, 9, 1000), (3, 1200, 100)])
 def test_batches_equal_single_matrices(count, rows, cols):
     x = gradient(count, rows, cols)
     got = OR.orthogonalise(x)
@@ -92,7 +94,7 @@ def test_steps(steps, shape):
     close(OR.orthogonalise(x, steps=steps), *model(x, steps))
 
 
-@pytest.mark.parametrize("shape", [(200, 200), (150, 600)])
+@pytest.mark.parametrize("shape", [(200, 200), (150, 600), (100, 900), (60, 90)])
 @pytest.mark.parametrize("noise", [0.0, 0.1, 10.0])
 def test_spectra(shape, noise):
     x = gradient(*shape, noise=noise)
@@ -102,8 +104,9 @@ def test_spectra(shape, noise):
 def test_low_rank():
     g = torch.Generator(device=DEV).manual_seed(3)
     for rank in (1, 4):
-        x = torch.randn(160, rank, generator=g, device=DEV) @ torch.randn(rank, 300, generator=g, device=DEV)
-        close(OR.orthogonalise(x), *model(x))
+        for rows, cols in ((160, 300), (60, 2000), (100, 200)):
+            x = torch.randn(rows, rank, generator=g, device=DEV) @ torch.randn(rank, cols, generator=g, device=DEV)
+            close(OR.orthogonalise(x), *model(x))
 
 
 def test_singular_values_end_around_one():
@@ -260,6 +263,7 @@ def check(groups, at, b, kw, zero_grad, spread=True):
 
 
 @pytest.mark.parametrize("shapes", [[(1, 1, 1)], [(64, 64, 5)], [(48, 96, 2), (96, 48, 3)], [(33, 57, 3), (57, 33, 2), (20, 20, 4)],
+                                    [(30, 500, 3), (500, 30, 2), (30, 700, 1), (40, 30, 2), (600, 30, 1)],
                                     [(130, 70, 1), (128, 300, 2)]])
 @pytest.mark.parametrize("gap", [0, 1, 16])
 def test_step(shapes, gap):
