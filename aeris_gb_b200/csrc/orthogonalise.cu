@@ -549,12 +549,16 @@ __device__ __forceinline__ void ortho_epilogue(const OrthoGemm& p, const CUtenso
   }
 }
 
-// The tile that unit `unit` of a launch of single CTAs works on, and its blocks of the reduction.
-__device__ __forceinline__ int ortho_blocks(const OrthoGemm& p, int unit, int& kb0, int& kb1) {
-  const int splits = p.cls[0].splits, n0 = p.cls[0].tiles * p.cls[0].count;
+// The tile that unit `unit` of a launch of single CTAs works on, and its blocks of the reduction. PARTS: `splits` or `low` are set.
+template <bool PARTS> __device__ __forceinline__ int ortho_blocks(const OrthoGemm& p, int unit, int& kb0, int& kb1) {
+  if (!PARTS) {
+    kb0 = 0;
+    kb1 = ((unit >= p.cls[0].tiles * p.cls[0].count ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK;
+    return unit;
+  }
+  const int splits = p.cls[0].splits;
   const int tile = splits > 1 ? unit / splits : unit;
-  const bool second = tile >= n0;
-  const int blocks = ((second ? p.cls[1].K : p.cls[0].K) + OG_BK - 1) / OG_BK * ((second ? p.cls[1].low : p.cls[0].low) ? 2 : 1);
+  const int blocks = (p.cls[0].K + OG_BK - 1) / OG_BK * (p.cls[0].low ? 2 : 1);         // one class
   kb0 = 0;
   kb1 = blocks;
   if (splits > 1) {
@@ -577,7 +581,7 @@ template <int NCOL> __device__ __forceinline__ void ortho_partial(float* to, uin
   }
 }
 
-template <int B_MN>
+template <int B_MN, bool PARTS>
 __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p) {
   constexpr int TILE = 128;
   extern __shared__ uint8_t smem_raw[];
@@ -623,10 +627,10 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.total && ok; unit += gridDim.x) {
         int cls, mat, ti, tj, kb0, kb1;
-        ortho_tile<TILE>(p, ortho_blocks(p, unit, kb0, kb1), cls, mat, ti, tj);
+        ortho_tile<TILE>(p, ortho_blocks<PARTS>(p, unit, kb0, kb1), cls, mat, ti, tj);
         const CUtensorMap *ta = cls ? &maps.a[1] : &maps.a[0], *tb = cls ? &maps.b[1] : &maps.b[0];
         const int ma = mat + (cls ? p.cls[1].a0 : p.cls[0].a0), mb = mat + (cls ? p.cls[1].b0 : p.cls[0].b0);
-        const int low_from = p.cls[0].low ? (p.cls[0].K + OG_BK - 1) / OG_BK : kb1, low = cls ? p.cls[1].low : p.cls[0].low;
+        const int low_from = PARTS && p.cls[0].low ? (p.cls[0].K + OG_BK - 1) / OG_BK : kb1, low = PARTS ? p.cls[0].low : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           const int k = (kb < low_from ? kb : kb - low_from) * OG_BK, ma_now = ma + (kb < low_from ? 0 : low);
           if (!own_wait(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
@@ -658,7 +662,7 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
       bool ok = true;
       for (int unit = blockIdx.x; unit < p.total && ok; unit += gridDim.x) {
         int kb0, kb1;
-        ortho_blocks(p, unit, kb0, kb1);
+        ortho_blocks<PARTS>(p, unit, kb0, kb1);
         if (!own_wait(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
         const uint32_t tmem_acc = tmem_base + acc * TILE;
@@ -690,11 +694,11 @@ __global__ void __launch_bounds__(OG_THREADS, 1) ortho_gemm_kernel(const __grid_
     const bool keep = !failed(p.status);
     for (int unit = blockIdx.x; unit < p.total; unit += gridDim.x) {
       int cls, mat, ti, tj, kb0, kb1;
-      ortho_tile<TILE>(p, ortho_blocks(p, unit, kb0, kb1), cls, mat, ti, tj);
+      ortho_tile<TILE>(p, ortho_blocks<PARTS>(p, unit, kb0, kb1), cls, mat, ti, tj);
       Addend add(p, mat, ti * TILE + q * 32 + lane, tj * TILE + part * (TILE / 2));
       if (!__all_sync(0xffffffffu, own_wait(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
-      if (p.partial)
+      if (PARTS && p.partial)
         ortho_partial<TILE / 2>(p.partial + static_cast<long long>(unit) * (TILE * TILE) + (q * 32 + lane) * TILE + part * (TILE / 2),
                                 tmem_base + acc * TILE + part * (TILE / 2) + (static_cast<uint32_t>(q * 32) << 16));
       else
@@ -853,6 +857,39 @@ ortho_gemm_pair_kernel(const __grid_constant__ OrthoMaps maps, const OrthoGemm p
   cluster_sync_all();
   tc_fence_after();
   if (warp == 1) tmem_dealloc2(tmem_base, 2 * TILE);
+}
+
+// S from the sums that several CTAs left for each tile on and below the diagonal, added up in order: 16 rows of a tile per block.
+__global__ void __launch_bounds__(256) ortho_reduce_kernel(const float* __restrict__ partial, int splits, int tiles, int d,
+                                                           __half* __restrict__ S, long long stride, int ld, float alpha) {
+  chain_point();
+  const int strip = blockIdx.x & 7, unit = blockIdx.x >> 3, mat = unit / tiles;
+  OrthoGemm place{};
+  place.sym = 1;
+  place.cls[0].tiles = tiles;
+  place.cls[0].count = mat + 1;
+  int cls, m, ti, tj;
+  ortho_tile<128>(place, unit, cls, m, ti, tj);
+  const int r = strip * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 8;
+  const float4* from = reinterpret_cast<const float4*>(partial + static_cast<long long>(unit) * splits * (128 * 128) + r * 128 + c);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    const float4 a = from[k * (128 * 32)], b = from[k * (128 * 32) + 1];
+    x.x += a.x; x.y += a.y; x.z += a.z; x.w += a.w;
+    y.x += b.x; y.y += b.y; y.z += b.z; y.w += b.w;
+  }
+  const int row = ti * 128 + r, col = tj * 128 + c;
+  if (row >= d || col >= ld) return;
+  const __half2 h[4] = {__floats2half2_rn(alpha * x.x, alpha * x.y), __floats2half2_rn(alpha * x.z, alpha * x.w),
+                        __floats2half2_rn(alpha * y.x, alpha * y.y), __floats2half2_rn(alpha * y.z, alpha * y.w)};
+  S += mat * stride;
+  *reinterpret_cast<uint4*>(S + static_cast<long long>(row) * ld + col) = *reinterpret_cast<const uint4*>(h);
+  if (ti != tj) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j < d) S[static_cast<long long>(col + j) * ld + row] = j & 1 ? __high2half(h[j / 2]) : __low2half(h[j / 2]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -1306,6 +1343,19 @@ int splits_of(const Layout& l, int c) {
   const int each = (blocks + s - 1) / s;
   return (blocks + each - 1) / each;          // none of them empty
 }
+// The same for X X^T of longer sides whose tiles leave most of the GPU idle: seven 151 x 4472 have 21 tiles of 70 blocks, 16 us by
+// themselves and 4 in parts, plus 4 for adding those up. 1: in one piece.
+int gram_splits(const Layout& l) {
+  if (l.few || l.classes > 1) return 1;
+  const int m = (l.d + 127) / 128, blocks = (l.K[0] + OG_BK - 1) / OG_BK;
+  const long long units = static_cast<long long>(m) * (m + 1) / 2 * l.count;
+  if (2 * units > num_sms()) return 1;
+  int s = num_sms() / static_cast<int>(units);
+  if (s > blocks / 6) s = blocks / 6;
+  if (s < 2) return 1;
+  const int each = (blocks + s - 1) / s;
+  return (blocks - each) * 0.235 > 6 ? (blocks + each - 1) / each : 1;
+}
 int Layout::fill(const AerisOrtho& a) {
   if (a.groups < 1 || a.groups > NS_GROUPS || a.steps < 1 || a.steps > 20) return -1;
   d = count = classes = 0;
@@ -1345,6 +1395,9 @@ int Layout::fill(const AerisOrtho& a) {
   if (few) {
     if (classes > 1) return -10;
     bytes += static_cast<long long>(splits_of(*this, 0)) * count * (128 * 128 * 4);
+  } else if (const int splits = gram_splits(*this); splits > 1) {
+    const int m = (d + 127) / 128;
+    bytes += static_cast<long long>(splits) * count * (m * (m + 1) / 2) * (128 * 128 * 4);
   }
   return 0;
 }
@@ -1352,6 +1405,7 @@ int Layout::fill(const AerisOrtho& a) {
 struct Products {
   const Layout& l;
   __half* S;
+  float* partial;
   __half* X[NS_CLASSES];
   CUtensorMap load_x[NS_CLASSES], store_x[NS_CLASSES], load_s, store_s;
   int* status;
@@ -1360,6 +1414,7 @@ struct Products {
 
   Products(const Layout& layout, char* work, int* status_, cudaStream_t stream_) : l(layout), status(status_), stream(stream_) {
     S = reinterpret_cast<__half*>(work + l.s_at);
+    partial = reinterpret_cast<float*>(work + l.partial_at);
     const uint64_t factors = static_cast<uint64_t>(l.few ? 2 : buffers_of(l.steps)) * l.count;
     rc = make_tmap_3d_fp16(&load_s, S, l.d, l.d, factors, pitch(l.d), 64, 64);
     if (!rc) rc = make_tmap_3d_fp16(&store_s, S, l.d, l.d, factors, pitch(l.d), 32, 32);
@@ -1373,7 +1428,8 @@ struct Products {
     if (rc) return;
     static bool configured = false;
     if (!configured) {
-      if (cudaFuncSetAttribute(ortho_gemm_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
+      if (cudaFuncSetAttribute(ortho_gemm_kernel<B_MN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
+          cudaFuncSetAttribute(ortho_gemm_kernel<B_MN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
           cudaFuncSetAttribute(ortho_gemm_pair_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess) {
         rc = -20;
         return;
@@ -1399,7 +1455,8 @@ struct Products {
       }
       return ends + static_cast<double>((total + units - 1) / units) * (round + block * blocks / total);
     };
-    const bool pair = p.partial == nullptr && p.cls[0].low == 0 && cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
+    const bool parts = p.partial || p.cls[0].low;
+    const bool pair = !parts && cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
     const int tile = pair ? 256 : 128, units = pair ? pairs : sms;
     long long total = 0;
     for (int c = 0; c < NS_CLASSES; ++c) total += tiles(c, tile) * p.cls[c].count;
@@ -1410,7 +1467,7 @@ struct Products {
     for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles(c, tile));
     p.total = static_cast<int>(total) * (p.cls[0].splits > 1 ? p.cls[0].splits : 1);
     const int grid = (p.total < units ? p.total : units) * (pair ? 2 : 1);
-    rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : ortho_gemm_kernel<B_MN>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
+    rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : parts ? ortho_gemm_kernel<B_MN, true> : ortho_gemm_kernel<B_MN, false>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
     ++launches;
   }
   OrthoGemm empty() const {
@@ -1461,7 +1518,17 @@ struct Products {
       p.cls[c].a0 = p.cls[c].b0 = from * l.members[c];
       p.cls[c].c0 = F_S * l.count + first;
     }
+    const int splits = gram_splits(l);
+    if (splits > 1) {
+      p.cls[0].splits = splits;
+      p.partial = partial;
+    }
     launch<0>(m, p);
+    if (splits == 1 || rc) return;
+    const int units = p.cls[0].tiles * l.count;
+    rc = launch_chained(ortho_reduce_kernel, units * 8, 256, 0, stream, static_cast<const float*>(partial), splits, p.cls[0].tiles, l.d,
+                        at(F_S), l.s_stride(), pitch(l.d), 1.f / NS_SCALE);
+    ++launches;
   }
   void update(int from, int by) {             // the other X = factor `by` X
     OrthoGemm p = empty();
@@ -1479,7 +1546,8 @@ struct Products {
     launch<1>(m, p);
   }
   // all steps on X number 0, into the other one
-  void few(float* partial, int splits, int steps) {
+  __half* at(int f) const { return S + static_cast<long long>(f) * l.count * l.s_stride(); }
+  void few(int splits, int steps) {
     OrthoGemm g = empty();
     OrthoMaps m = square();
     g.sym = 1;
@@ -1614,7 +1682,7 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   rc = launch_chained(step ? ortho_pack_kernel<true> : ortho_pack_kernel<false>, blocks(in), 256, 0, stream, in, input, a.eps);
   if (rc) return rc;
   if (l.few)
-    run.few(reinterpret_cast<float*>(work + l.partial_at), splits_of(l, 0), a.steps);
+    run.few(splits_of(l, 0), a.steps);
   else
     for (int k = 0; k < l.steps.n; ++k) run.group(k & 1, l.steps.size[k]);
   if (run.rc) return run.rc;

@@ -66,7 +66,7 @@ def gradient(*shape, noise=0.5, seed=0):
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 2), (3, 200), (200, 3), (31, 33), (63, 65), (64, 64), (65, 64), (128, 128), (128, 129), (129, 127),
           (127, 640), (192, 192), (256, 256), (257, 300), (300, 257), (384, 1024), (1001, 333), (320, 2000), (515, 515), (768, 640),
-          (1, 385), (2, 5000), (64, 4000), (65, 700), (100, 13001), (128, 8192), (5000, 96), (150, 9000)]
+          (1, 385), (2, 5000), (64, 4000), (65, 700), (100, 13001), (128, 8192), (5000, 96), (150, 9000), (9001, 300), (512, 5000)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
