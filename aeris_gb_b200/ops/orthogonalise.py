@@ -8,33 +8,46 @@ singular vectors.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
 from . import lib as _l
 
-_P, _I, _F, _LL, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_double
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_GROUPS, MAX_LENGTHS = 4, 2       # shapes of a batch, and longer sides among them
 MAX_COUNT = 1 << 16                  # matrices of a group
 FEW_ROWS, SHORT_ROWS = 128, 384      # up to so many rows (d) matrices with rows longer than that have a batch for each length
 WORKSPACE_BYTES = 1 << 30            # of one batch; what does not fit goes in several
 
-
-class _Group(ctypes.Structure):
-    """Mirror of ``AerisOrthoGroup`` (csrc/api.h)."""
-    _fields_ = [("offsets", _P), ("stride", _LL), ("out_stride", _LL)] + [(n, _I) for n in ("rows", "cols", "ld", "ld_out", "count",
-                                                                                           "behind")] + [("rate", _F)]
+# AerisOrthoGroup and AerisOrtho (csrc/api.h), field by field
+_GROUP = struct.Struct("Pqq6if4x")
+_REST = struct.Struct("10Pdqq5i5f")
 
 
-class _Args(ctypes.Structure):
-    """Mirror of ``AerisOrtho`` (csrc/api.h)."""
-    _fields_ = ([("group", _Group * MAX_GROUPS)]
-                + [(n, _P) for n in ("x", "out", "grad", "momentum", "master", "ema", "weights", "norm_sq", "work", "status")]
-                + [("eps", _D), ("numel", _LL), ("work_bytes", _LL)]
-                + [(n, _I) for n in ("groups", "steps", "bf16", "nesterov", "zero_grad")]
-                + [(n, _F) for n in ("beta", "grad_scale", "max_norm", "decay", "ema_beta")])
+def _group(rows, cols, count, *, offsets=0, stride=0, out_stride=0, ld=0, ld_out=0, behind=False, rate=0.0) -> bytes:
+    return _GROUP.pack(offsets, stride, out_stride, rows, cols, ld or cols, ld_out, count, behind, rate)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    f = getattr(_l.lib(), name)
+    if name == "aeris_ortho_work_bytes":
+        f.argtypes, f.restype = (ctypes.c_char_p,), ctypes.c_longlong
+    else:
+        f.argtypes = (ctypes.c_char_p, ctypes.c_void_p)
+    return f
+
+
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(shapes: tuple, steps: int) -> int:
+    """Workspace of a batch of (rows, cols, how many)."""
+    rest = _REST.pack(*[0] * 10, 0.0, 0, 0, len(shapes), steps, 0, 0, 0, *[0.0] * 5)
+    n = _entry("aeris_ortho_work_bytes")(b"".join(_group(*g) for g in shapes) + bytes(_GROUP.size * (MAX_GROUPS - len(shapes))) + rest)
+    _l.check(min(n, 0), "aeris_ortho_work_bytes", kernels=0)
+    return n
 
 
 def _bytes_per_matrix(d: int, k: int) -> int:
@@ -43,15 +56,16 @@ def _bytes_per_matrix(d: int, k: int) -> int:
     return 2 * d * (2 * (-(-k // 64) * 64) + 4 * (-(-d // 64) * 64)) + 8192 + few
 
 
-def _run(a: _Args, device) -> None:
-    lib = _l.lib()
-    lib.aeris_ortho_work_bytes.restype = _LL
-    a.work_bytes = lib.aeris_ortho_work_bytes(ctypes.byref(a))
-    _l.check(min(a.work_bytes, 0), "aeris_ortho_work_bytes", kernels=0)
-    if a.work_bytes:
-        work = torch.empty(a.work_bytes + 1024, dtype=torch.uint8, device=device)
-        a.work = -(-work.data_ptr() // 1024) * 1024
-    rc = lib.aeris_orthogonalise(ctypes.byref(a), _l.stream_ptr())
+def _run(device, groups: list[bytes], shapes: tuple, *, x=0, out=0, grad=0, momentum=0, master=0, ema=0, weights=0, norm_sq=0, eps,
+         numel=0, steps, bf16=False, nesterov=False, zero_grad=False, beta=0.0, grad_scale=0.0, max_norm=0.0, decay=0.0,
+         ema_beta=-1.0) -> None:
+    n, work = _work_bytes(shapes, steps), 0
+    if n:
+        buf = torch.empty(n + 1024, dtype=torch.uint8, device=device)
+        work = -(-buf.data_ptr() // 1024) * 1024
+    rest = _REST.pack(x, out, grad, momentum, master, ema, weights, norm_sq, work, _l.status_word().data_ptr(), eps, numel, n,
+                      len(groups), steps, bf16, nesterov, zero_grad, beta, grad_scale, max_norm, decay, ema_beta)
+    rc = _entry("aeris_orthogonalise")(b"".join(groups) + bytes(_GROUP.size * (MAX_GROUPS - len(groups))) + rest, _l.raw_stream())
     _l.check(min(rc, 0), "aeris_orthogonalise", kernels=max(rc, 0))
 
 
@@ -88,22 +102,21 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, eps: float = 1e-7, out: to
                              f"{tuple(out.shape)} on {out.device} with strides {out.stride()}")
     _l.require_cuda(x)
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        out = torch.empty_like(x, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
     if x.numel() == 0:
         return out
-    xs, os = _as_batch(x.detach()), _as_batch(out)
+    xs, os = _as_batch(x), _as_batch(out)
     if not _pitched(xs):
         xs = xs.contiguous()
     count, rows, cols = xs.shape
     most = max(1, min(MAX_COUNT, WORKSPACE_BYTES // _bytes_per_matrix(min(rows, cols), max(rows, cols))))
+    stride, out_stride, ld, ld_out = xs.stride(0), os.stride(0), _row_pitch(xs), _row_pitch(os)
     with _l.on_device(x.device):
-        status = _l.status_word().data_ptr()
         for i in range(0, count, most):
-            a = _Args(x=xs.data_ptr() + i * xs.stride(0) * xs.element_size(), out=os.data_ptr() + i * os.stride(0) * 2, groups=1,
-                      bf16=xs.dtype == torch.bfloat16, eps=eps, steps=steps, status=status)
-            a.group[0] = _Group(stride=xs.stride(0), out_stride=os.stride(0), rows=rows, cols=cols, ld=_row_pitch(xs),
-                                ld_out=_row_pitch(os), count=min(most, count - i))
-            _run(a, x.device)
+            n = min(most, count - i)
+            _run(x.device, [_group(rows, cols, n, stride=stride, out_stride=out_stride, ld=ld, ld_out=ld_out)], ((rows, cols, n),),
+                 x=xs.data_ptr() + i * stride * xs.element_size(), out=os.data_ptr() + i * out_stride * 2,
+                 bf16=xs.dtype is torch.bfloat16, eps=eps, steps=steps)
     return out
 
 
@@ -179,14 +192,12 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
             todo.append((rows, cols, offsets.data_ptr(), offsets.numel()))
     _l.require_cuda(master)
     with _l.on_device(master.device):
-        a = _Args(grad=grad.data_ptr(), momentum=momentum.data_ptr(), master=master.data_ptr(), numel=master.numel(),
-                  weights=0 if weights is None else weights.data_ptr(), ema=0 if ema is None else ema.data_ptr(),
-                  norm_sq=0 if norm_sq is None else norm_sq.data_ptr(), status=_l.status_word().data_ptr(), eps=eps, steps=steps,
-                  nesterov=nesterov, zero_grad=zero_grad, beta=beta, grad_scale=grad_scale, max_norm=max_norm,
-                  decay=1.0 - lr * weight_decay, ema_beta=ema_beta)
+        common = dict(grad=grad.data_ptr(), momentum=momentum.data_ptr(), master=master.data_ptr(), numel=master.numel(),
+                      weights=0 if weights is None else weights.data_ptr(), ema=0 if ema is None else ema.data_ptr(),
+                      norm_sq=0 if norm_sq is None else norm_sq.data_ptr(), eps=eps, steps=steps, nesterov=nesterov,
+                      zero_grad=zero_grad, beta=beta, grad_scale=grad_scale, max_norm=max_norm, decay=1.0 - lr * weight_decay,
+                      ema_beta=ema_beta)
         for batch in _batches(todo):
-            a.groups = len(batch)
-            for i, (rows, cols, table, n, behind) in enumerate(batch):
-                a.group[i] = _Group(offsets=table, rows=rows, cols=cols, ld=cols, count=n, behind=behind,
-                                    rate=lr * scale * math.sqrt(max(rows, cols)))
-            _run(a, master.device)
+            _run(master.device, [_group(rows, cols, n, offsets=table, behind=behind, rate=lr * scale * math.sqrt(max(rows, cols)))
+                                 for rows, cols, table, n, behind in batch],
+                 tuple((rows, cols, n) for rows, cols, _, n, _ in batch), **common)
