@@ -72,6 +72,20 @@ __device__ __forceinline__ OrthoPlace ortho_place(const OrthoGroups& a) {
   return p;
 }
 
+// One warp: records a matrix of another group that shares elements with this one.
+__device__ __forceinline__ void ortho_apart(const OrthoGroups& a, const OrthoPlace& p) {
+  if (!a.g[p.group].offsets || !p.found) return;
+  const long long end = p.at + static_cast<long long>(a.g[p.group].rows) * a.g[p.group].cols;
+  for (int h = 0; h < a.n; ++h) {
+    const OrthoGroup& g = a.g[h];
+    if (h == p.group) continue;
+    for (int i = threadIdx.x & 31; i < g.count; i += 32) {
+      const long long at = g.offsets[g.first + i];
+      if (at < end && at + static_cast<long long>(g.rows) * g.cols > p.at) atomicCAS(a.status, 0, ERR_BOUNDS);
+    }
+  }
+}
+
 // What is orthogonalised: a tensor (fp32 or bf16), or the momentum of an optimizer.
 struct OrthoInput {
   const void* x;
@@ -128,6 +142,7 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a,
   chain_point();
   const OrthoPlace p = ortho_place(a);
   const OrthoGroup& m = a.g[p.group];
+  if (STEP && p.block == 0 && threadIdx.x < 32) ortho_apart(a, p);
   double sum = 0;
   if (p.found) {
     const float gs = STEP ? step_scale(in) : 0.f;
@@ -946,6 +961,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   chain_point();
 
   const OrthoPlace p = ortho_place(a);
+  if (STEP && warp == 1) ortho_apart(a, p);
   const OrthoGroup& m = a.g[p.group];
   const bool upright = m.rows > m.cols;
   const int d = upright ? m.cols : m.rows, K = upright ? m.rows : m.cols;
@@ -1362,9 +1378,10 @@ bool on_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 // in directions that hold little of the norm, and is not small against them any more. So pairs of steps alternate with single
 // ones: error on 333 x 1001 gradients with half as much noise as signal 1.13e-3 by single steps, 1.09e-3 as 2, 1, 2, 1.49e-3 as
 // 2, 2, 1, 1.8e-3 as 3, 2; on 127 x 640 6e-4, 6e-4, 6e-4, 1.8e-3; a group of five diverges. Below GROUP_FROM rows single steps:
-// the products are shorter than their launches, of which groups have two more, and a handful of rows does not average the
+// the products are no longer than their launches, of which groups have two more (us by single steps / in pairs: 256 x 600 94 / 101,
+// ten 333 x 1001 139 / 142, 42 of 384 x 1024 282 / 266, 30 of 500 x 1500 434 / 397), and a handful of rows does not average the
 // roundings (5 x 9: up to three times the error of single steps).
-constexpr int GROUP_FROM = 256;
+constexpr int GROUP_FROM = 384;
 struct Groups {
   int n, size[20];
 };

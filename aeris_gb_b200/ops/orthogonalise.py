@@ -169,8 +169,9 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
     ``weights`` (bf16) receives the new master, ``ema`` its running average (``ema_beta`` < 0: not), ``grad`` zeros with
     ``zero_grad``. ``norm_sq`` and ``max_norm``: clipping as in ``adamw``. ``groups``: (rows, cols, offsets) for matrices that lie
     without gaps from the element offsets on, an int64 tensor on the same device, ascending; no two matrices may overlap. One
-    that does not lie inside the buffers, or not behind the one before it, sets the status word and is left as it is; elements
-    of no matrix are not touched. ``scale`` = 0.2 gives updates the root mean square of AdamW's."""
+    that does not lie inside the buffers, or not behind the one before it, is left as it is and sets the status word, and so
+    does one that shares elements with a matrix of another group: the call has then failed (``lib.check_status`` raises), and
+    which of its other matrices have been updated is not defined. Elements of no matrix are not touched. ``scale`` = 0.2 gives updates the root mean square of AdamW's."""
     _check_steps(steps)
     if master.dim() != 1 or master.dtype != torch.float32 or not master.is_contiguous() or master.data_ptr() % 16:
         raise ValueError(f"master: contiguous fp32 [n] from a 16-byte boundary on, got {master.dtype} {tuple(master.shape)}")

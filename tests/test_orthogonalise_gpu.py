@@ -307,12 +307,54 @@ def test_offsets_outside_or_overlapping_are_reported_and_left(bad):
     seen = _l.status_word().item()
     _l.status_word().zero_()
     assert seen == 6
-    # a kernel that finds the word set keeps its results to itself: nothing half done is applied to the weights
-    whole = torch.ones(2000, dtype=torch.bool, device=DEV)
     for k in ("momentum", "grad"):
-        assert torch.equal(b[k][whole], want[k][whole]), k
-    groups, at, fresh = flat([(20, 20, 5)], gap=0)
-    assert torch.equal(b["master"], fresh["master"]) and torch.equal(b["weights"], fresh["weights"])
+        assert torch.equal(b[k], want[k]), k
+    _, _, fresh = flat([(20, 20, 5)], gap=0)
+    outside = torch.ones(2000, dtype=torch.bool, device=DEV)
+    for o in good:
+        outside[o:o + 400] = False
+    # the others of a failed call may have been updated or not
+    assert torch.equal(b["master"][outside], fresh["master"][outside]) and torch.equal(b["weights"][outside], fresh["weights"][outside])
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 30), (150, 160)])          # in one launch, in many
+def test_a_matrix_in_two_groups_is_reported(rows, cols):
+    n = rows * cols
+    for second, bad in ((n, False), (n - 1, True), (0, True)):
+        b = {k: torch.zeros(3 * n + 8, device=DEV) for k in ("master", "grad", "momentum")}
+        groups = [(rows, cols, torch.tensor([0, 2 * n + 4], device=DEV)), (cols, rows, torch.tensor([second], device=DEV))]
+        OR.orthogonal_step(b["master"], b["grad"], b["momentum"], None, None, None, groups=groups, **KW)
+        seen = _l.status_word().item()
+        _l.status_word().zero_()
+        assert seen == (6 if bad else 0)
+
+
+def test_matrices_beyond_32_bit_offsets():
+    base = torch.empty(2 ** 32 + 2 ** 20, dtype=torch.bfloat16, device=DEV)
+    for rows, cols in ((64, 80), (200, 300)):
+        x = base.as_strided((2, rows, cols), (2 ** 32, cols, 1))
+        x.copy_(gradient(2, rows, cols))
+        want = OR.orthogonalise(x.clone())
+        assert torch.equal(OR.orthogonalise(x), want)
+        OR.orthogonalise(x.clone(), out=x)
+        assert torch.equal(x, want)
+
+
+def test_two_calls_at_once():
+    """On streams of their own, without waiting for one another: neither's workspace is the other's."""
+    a, b = gradient(6, 200, 600), gradient(8, 300, 500, seed=3)
+    want = OR.orthogonalise(a), OR.orthogonalise(b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for k, (s, x) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[k].append(OR.orthogonalise(x))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(g, want[k]) for g in got[k])
 
 
 def test_batches_of_a_small_workspace_give_the_same_bits(monkeypatch):
