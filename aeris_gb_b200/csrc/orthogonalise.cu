@@ -243,13 +243,13 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
     g = clean(g * gs);
     return scale * (in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom);
   };
+  if (p.four) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int r = r0 + tr + 16 * k, c = c0 + tc;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (r < m.rows && c < m.cols) {
-      const long long e = p.at + static_cast<long long>(r) * m.ld + c;
-      if (p.four) {
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + tr + 16 * k, c = c0 + tc;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < m.rows && c < m.cols) {
+        const long long e = p.at + static_cast<long long>(r) * m.ld + c;
         if (STEP) {
           const float4 g = *reinterpret_cast<const float4*>(in.grad + e);
           const float4 mo = *reinterpret_cast<const float4*>(in.momentum + e);
@@ -259,25 +259,38 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
           const float4 u = in_value4(in, e);
           v[0] = scale * u.x; v[1] = scale * u.y; v[2] = scale * u.z; v[3] = scale * u.w;
         }
-      } else {
+      }
+      if (upright) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (c + j >= m.cols) break;
-          if (STEP) {
-            v[j] = value(in.grad[e + j], in.momentum[e + j]);
-            if (in.zero_grad) in.grad[e + j] = 0.f;
-          } else {
-            v[j] = scale * in_value(in, e + j);
-          }
-        }
+        for (int j = 0; j < 4; ++j) tile[tr + 16 * k][tc + j] = v[j];
+      } else if (r < m.rows && c < m.ldx) {
+        __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+        *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * m.ldx + c) = *reinterpret_cast<uint2*>(h);
       }
     }
-    if (upright) {
+  } else {                                    // element by element, a warp's side by side
+    const int cc = threadIdx.x & 63, c = c0 + cc;
+    const int first = threadIdx.x >> 6;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      float u[8], mo[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tile[tr + 16 * k][tc + j] = v[j];
-    } else if (r < m.rows && c < m.ldx) {
-      __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
-      *reinterpret_cast<uint2*>(X + static_cast<long long>(r) * m.ldx + c) = *reinterpret_cast<uint2*>(h);
+      for (int k = 0; k < 8; ++k) {
+        const int r = r0 + first + 32 * half + 4 * k;
+        u[k] = mo[k] = 0.f;
+        if (r >= m.rows || c >= m.cols) continue;
+        const long long e = p.at + static_cast<long long>(r) * m.ld + c;
+        u[k] = STEP ? in.grad[e] : in_value(in, e);
+        if (STEP) mo[k] = in.momentum[e];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int rr = first + 32 * half + 4 * k, r = r0 + rr;
+        const float v = STEP ? value(u[k], mo[k]) : scale * u[k];
+        if (STEP && in.zero_grad && r < m.rows && c < m.cols) in.grad[p.at + static_cast<long long>(r) * m.ld + c] = 0.f;
+        if (upright) tile[rr][cc] = v;
+        else if (r < m.rows && c < m.ldx) X[static_cast<long long>(r) * m.ldx + c] = __float2half_rn(v);
+      }
     }
   }
   if (upright) {
@@ -333,6 +346,26 @@ __global__ void __launch_bounds__(256) ortho_finish_kernel(const OrthoGroups a, 
     }
     __syncthreads();
   }
+  if (!p.four) {                              // element by element, a warp's side by side
+    const int cc = threadIdx.x & 63, c = c0 + cc;
+    if (c >= m.cols) return;
+#pragma unroll 4
+    for (int rr = threadIdx.x >> 6; rr < 64; rr += 4) {
+      const int r = r0 + rr;
+      if (r >= m.rows) break;
+      const long long e = p.at + static_cast<long long>(r) * m.ld + c;
+      const float v = (upright ? tile[rr][cc] : __half2float(X[static_cast<long long>(r) * m.ldx + c])) * (1.f / NS_SCALE);
+      if (!STEP) {
+        o.out[e] = __float2bfloat16_rn(v);
+        continue;
+      }
+      const float w = o.master[e] * o.decay - m.rate * v;
+      o.master[e] = w;
+      if (o.weights) o.weights[e] = __float2bfloat16_rn(w);
+      if (o.ema && o.ema_beta >= 0.f) o.ema[e] = w + o.ema_beta * (o.ema[e] - w);
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int r = r0 + tr + 16 * k, c = c0 + tc;
@@ -348,32 +381,19 @@ __global__ void __launch_bounds__(256) ortho_finish_kernel(const OrthoGroups a, 
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= 1.f / NS_SCALE;
     if (!STEP) {
-      if (p.four) {
-        *reinterpret_cast<uint2*>(o.out + e) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      } else {
-        for (int j = 0; j < 4 && c + j < m.cols; ++j) o.out[e + j] = __float2bfloat16_rn(v[j]);
-      }
+      *reinterpret_cast<uint2*>(o.out + e) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
       continue;
     }
-    if (p.four) {
-      const float4 p4 = *reinterpret_cast<const float4*>(o.master + e);
-      const float w[4] = {p4.x * o.decay - m.rate * v[0], p4.y * o.decay - m.rate * v[1], p4.z * o.decay - m.rate * v[2],
-                          p4.w * o.decay - m.rate * v[3]};
-      *reinterpret_cast<float4*>(o.master + e) = make_float4(w[0], w[1], w[2], w[3]);
-      if (o.weights) *reinterpret_cast<uint2*>(o.weights + e) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
-      if (o.ema && o.ema_beta >= 0.f) {
-        float4 x = *reinterpret_cast<const float4*>(o.ema + e);
-        x.x = w[0] + o.ema_beta * (x.x - w[0]); x.y = w[1] + o.ema_beta * (x.y - w[1]);
-        x.z = w[2] + o.ema_beta * (x.z - w[2]); x.w = w[3] + o.ema_beta * (x.w - w[3]);
-        *reinterpret_cast<float4*>(o.ema + e) = x;
-      }
-    } else {
-      for (int j = 0; j < 4 && c + j < m.cols; ++j) {
-        const float w = o.master[e + j] * o.decay - m.rate * v[j];
-        o.master[e + j] = w;
-        if (o.weights) o.weights[e + j] = __float2bfloat16_rn(w);
-        if (o.ema && o.ema_beta >= 0.f) o.ema[e + j] = w + o.ema_beta * (o.ema[e + j] - w);
-      }
+    const float4 p4 = *reinterpret_cast<const float4*>(o.master + e);
+    const float w[4] = {p4.x * o.decay - m.rate * v[0], p4.y * o.decay - m.rate * v[1], p4.z * o.decay - m.rate * v[2],
+                        p4.w * o.decay - m.rate * v[3]};
+    *reinterpret_cast<float4*>(o.master + e) = make_float4(w[0], w[1], w[2], w[3]);
+    if (o.weights) *reinterpret_cast<uint2*>(o.weights + e) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
+    if (o.ema && o.ema_beta >= 0.f) {
+      float4 x = *reinterpret_cast<const float4*>(o.ema + e);
+      x.x = w[0] + o.ema_beta * (x.x - w[0]); x.y = w[1] + o.ema_beta * (x.y - w[1]);
+      x.z = w[2] + o.ema_beta * (x.z - w[2]); x.w = w[3] + o.ema_beta * (x.w - w[3]);
+      *reinterpret_cast<float4*>(o.ema + e) = x;
     }
   }
 }
