@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_ring_kernel(const 
 }
 
 // dw from one row of sums per block, those of q before those of k: 32 channels of q (blockIdx.y = 0) or k per block, one warp's
-// lanes side by side, 32 warps over the rows.
+// lanes side by side, 32 warps over the rows. A weight that q and k share has one sum of both (gridDim.y = 1, no rows of k).
 __global__ void __launch_bounds__(1024) qk_norm_sums_kernel(const float* __restrict__ sums, int q_rows, int k_rows, int d, float* dwq,
                                                             float* dwk, int add) {
   __shared__ float red[32][33];
@@ -516,8 +516,9 @@ extern "C" int aeris_qk_norm_bwd(const AerisQkNorm* p, void* stream_) {
   auto kern = a.f32 ? (vec ? qk_norm_bwd_ring_kernel<float> : qk_norm_bwd_kernel<float>)
                     : (vec ? qk_norm_bwd_ring_kernel<__nv_bfloat16> : qk_norm_bwd_kernel<__nv_bfloat16>);
   if (const int rc = launch_chained(kern, c.q_blocks + c.k_blocks, QKN_THREADS, 0, stream, a, c)) return rc;
-  if (const int rc = launch_chained(qk_norm_sums_kernel, dim3((a.d + 31) / 32, 2), 1024, 0, stream, a.sums, c.q_blocks, c.k_blocks,
-                                    a.d, a.dwq, a.dwk, a.add_dw))
+  const bool shared = a.dwq == a.dwk;
+  if (const int rc = launch_chained(qk_norm_sums_kernel, dim3((a.d + 31) / 32, shared ? 1 : 2), 1024, 0, stream, a.sums,
+                                    c.q_blocks + (shared ? c.k_blocks : 0), c.k_blocks, a.d, a.dwq, a.dwk, a.add_dw))
     return rc;
   return 2;
 }

@@ -63,6 +63,8 @@ def _check(q, k, wq, wk, cos, sin, positions, rows_like_q, rows_like_k, results,
     for t in results:
         if t is not None and not _apart(t):
             raise ValueError(f"elements of a result share addresses: {_text(t)}")
+    if rows and results[0] is not None and results[1] is not None and results[0].data_ptr() == results[1].data_ptr():
+        raise ValueError("the results of q and k are the same memory")
     w_dt, one = wq.dtype, (d,)
     if not (wq.shape == one == wk.shape and w_dt in _FLOATS and w_dt is wk.dtype and wq.device == dev == wk.device
             and wq.is_contiguous() and wk.is_contiguous()):
@@ -70,6 +72,8 @@ def _check(q, k, wq, wk, cos, sin, positions, rows_like_q, rows_like_k, results,
     for t in dw:
         if t.shape != (d,) or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
             raise ValueError(f"gradients of the weights: contiguous fp32 [{d}] on {dev}, got {_text(t)}")
+    if dw and 0 < abs(dw[0].data_ptr() - dw[1].data_ptr()) < 4 * d:
+        raise ValueError("gradients of the weights that overlap are the same tensor, a weight's that q and k share")
     if cos is None or sin is None:
         if cos is not None or sin is not None or positions is not None:
             raise ValueError("cos and sin come together, positions only with them")
@@ -134,7 +138,8 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
                 dwq: torch.Tensor | None = None, dwk: torch.Tensor | None = None):
     """Gradients of :func:`qk_norm_fwd` for ``dq``, ``dk`` with respect to its results; ``q``, ``k`` are its inputs. Returns
     (gradients of q and k, which may overwrite ``dq`` and ``dk``, and fp32 gradients of the weights). ``dwq``, ``dwk`` [d] fp32
-    are added to where given. The same bits on every run."""
+    are added to where given, and may be one tensor, of a weight that q and k share. A row whose position lies outside the table
+    adds nothing, and its gradients are not written. The same bits on every run."""
     add = dwq is not None
     if add != (dwk is not None):
         raise ValueError("dwq and dwk come together")

@@ -59,9 +59,16 @@ def test_cpu_tensors_are_refused_and_not_computed_elsewhere():
         forward(args())
 
 
+def test_results_in_one_place_are_refused():
+    t = torch.empty(ROWS, H, D)
+    with pytest.raises(ValueError, match="same memory"):
+        forward(args(q_out=t, k_out=t[:, :HK]))
+
+
 @pytest.mark.parametrize("bad", [dict(dq=torch.randn(ROWS, H, D + 2)), dict(dk=torch.randn(ROWS, HK, D).bfloat16()),
                                  dict(dwq=torch.zeros(D)), dict(dwq=torch.zeros(D), dwk=torch.zeros(D + 1)),
                                  dict(dwq=torch.zeros(D), dwk=torch.zeros(D).bfloat16()),
+                                 dict(zip(("dwq", "dwk"), (lambda t: (t[:D], t[4:D + 4]))(torch.zeros(2 * D)))),
                                  dict(dq_out=torch.empty(ROWS, 1, D).expand(ROWS, H, D))])
 def test_backward_refuses(bad):
     a = args()

@@ -191,6 +191,28 @@ def test_in_place_and_into_sections(d):
     assert torch.equal(q, yq) and torch.equal(k, yk)
 
 
+@pytest.mark.parametrize("rows,d", [(1, 16), (700, 64), (33, 250)])
+def test_a_weight_that_q_and_k_share(rows, d):
+    """One tensor for both gradients: the sum of both."""
+    q, k, dq, dk, w, _, cos, sin, _, at = make(rows, 4, 2, d, d, rows, torch.bfloat16)
+    dw = torch.full((d,), 3.0, device=DEV)
+    QN.qk_norm_bwd(dq, dk, q, k, w, w, cos, sin, eps=1e-6, dwq=dw, dwk=dw)
+    _, _, eq, size_q = formula(q, w, cos, sin, at, 1e-6, dq)
+    _, _, ek, size_k = formula(k, w, cos, sin, at, 1e-6, dk)
+    close(dw, 3 + eq + ek, 3 + size_q + size_k, torch.float32, 16 + 6 * rows)
+
+
+def test_few_query_heads_beside_many_key_heads():
+    q, k, dq, dk, wq, wk, cos, sin, _, at = make(50, 1, 2001, 8, 8, 50, torch.bfloat16, layout="own")
+    yq, yk = QN.qk_norm_fwd(q, k, wq, wk, cos, sin, eps=1e-6)
+    gq, gk, gwq, gwk = QN.qk_norm_bwd(dq, dk, q, k, wq, wk, cos, sin, eps=1e-6)
+    for x, w, dy, y, dx, dw in ((q, wq, dq, yq, gq, gwq), (k, wk, dk, yk, gk, gwk)):
+        close(y, *formula(x, w, cos, sin, at, 1e-6), q.dtype)
+        ex, size, ew, wsize = formula(x, w, cos, sin, at, 1e-6, dy)
+        close(dx, ex, size, q.dtype)
+        close(dw, ew, wsize, torch.float32, 16 + x.shape[0] * x.shape[1])
+
+
 def test_no_rows():
     q, k, dq, dk, wq, wk, cos, sin, _, _ = make(0, 4, 2, 16, 16, 4, torch.bfloat16)
     before = _l.launch_count()
