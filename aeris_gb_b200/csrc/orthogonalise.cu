@@ -17,6 +17,7 @@
 #include "host.h"
 
 #include <cuda_fp16.h>
+#include <atomic>
 #include <type_traits>
 
 namespace aeris {
@@ -24,6 +25,7 @@ namespace aeris {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float NS_SCALE = 512.f;             // stored = NS_SCALE * value, for X and for the [d, d] factors
 
+constexpr int NS_MAX_SIDE = 1 << 30;          // rows or columns of a matrix
 constexpr int NS_PARTS = 1024;                // blocks per matrix that its squares are summed in, at most
 constexpr int NS_GROUPS = ORTHO_GROUPS, NS_CLASSES = 2;
 
@@ -1092,14 +1094,15 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
+    if (!ok) return;                          // with this warp's last products perhaps still under way
     if (warp == 0) {
       tc_fence_after();
       issue();
       tc_commit_warp(lead, smem_u32(bar));
     }
-    ok = ok && mbar_wait_warp(bar, phase, a.status, ERR_TIMEOUT_TMEM_FULL);
-    if (!ok) *gave_up = 1;
-    phase ^= 1;
+    ok = mbar_wait_warp(bar, phase, a.status, ERR_TIMEOUT_TMEM_FULL);
+    if (ok) phase ^= 1;
+    else *gave_up = 1;
     tc_fence_after();
   };
   for (int step = 0; step < steps; ++step) {
@@ -1159,6 +1162,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
       os_put(smem, row, c, f);
     }
   }
+  if (warp == 0 && !ok) mbar_wait_warp(bar, phase, nullptr, 0);       // the last products, before the tensor memory goes back
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1275,9 +1279,10 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
   };
   bool ok = true;
   auto finish = [&] {
+    if (!ok) return;                          // with warp 0's last products perhaps still under way
     if (warp == 0) tc_commit_warp(lead, smem_u32(bar));
-    ok = ok && mbar_wait_warp(bar, phase, status, ERR_TIMEOUT_TMEM_FULL);
-    phase ^= 1;
+    ok = mbar_wait_warp(bar, phase, status, ERR_TIMEOUT_TMEM_FULL);
+    if (ok) phase ^= 1;
     tc_fence_after();
   };
   // the sums, side by side through the (still free) place of Q, whose 16-byte chunks are swizzled by row
@@ -1320,7 +1325,7 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
   for (int step = 0; step < steps; ++step) {
     const bool last = step + 1 == steps;
     begin();
-    if (warp == 0) product(0, S, S);
+    if (warp == 0 && ok) product(0, S, S);
     finish();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -1338,7 +1343,7 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
     }
     if (step || !last) {
       begin();
-      if (warp == 0) {
+      if (warp == 0 && ok) {
         if (step) product(128, P, QQ);
         if (!last) product(0, P, S);
       }
@@ -1359,7 +1364,7 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
     }
     if (last) break;
     begin();
-    if (warp == 0) product(0, S, P);
+    if (warp == 0 && ok) product(0, S, P);
     finish();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -1371,6 +1376,7 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
       os_put2(S, row, c0 + 32 * h, f);
     }
   }
+  if (warp == 0 && !ok) mbar_wait_warp(bar, phase, nullptr, 0);       // the last products, before the tensor memory goes back
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1387,6 +1393,17 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
 
 // ------------------------------------------------------------------------------------------------ host side
 namespace {
+
+// Lets a kernel have `bytes` of shared memory, once a device.
+template <typename F> bool allow_smem(F kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 int pitch(int n) { return (n + 63) / 64 * 64; }
 bool on_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -1453,6 +1470,7 @@ int Layout::fill(const AerisOrtho& a) {
     const AerisOrthoGroup& g = a.group[i];
     if (g.rows < 1 || g.cols < 1 || g.count < 1 || g.count > (1 << 20) || g.ld < g.cols) return -2;
     const int shorter = g.rows < g.cols ? g.rows : g.cols, longer = g.rows < g.cols ? g.cols : g.rows;
+    if (longer > NS_MAX_SIDE) return -2;
     if (i && shorter != d) return -3;
     d = shorter;
     int c = 0;
@@ -1516,16 +1534,6 @@ struct Products {
   }
   template <int B_MN> void launch(const OrthoMaps& maps, OrthoGemm& p) {
     if (rc) return;
-    static bool configured = false;
-    if (!configured) {
-      if (cudaFuncSetAttribute(ortho_gemm_kernel<B_MN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
-          cudaFuncSetAttribute(ortho_gemm_kernel<B_MN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess ||
-          cudaFuncSetAttribute(ortho_gemm_pair_kernel<B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, OG_SMEM) != cudaSuccess) {
-        rc = -20;
-        return;
-      }
-      configured = true;
-    }
     p.M = l.d;
     p.status = status;
     const int sms = num_sms(), pairs = sms / 2;
@@ -1557,7 +1565,9 @@ struct Products {
     for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles(c, tile));
     p.total = static_cast<int>(total) * (p.cls[0].splits > 1 ? p.cls[0].splits : 1);
     const int grid = (p.total < units ? p.total : units) * (pair ? 2 : 1);
-    rc = launch_chained(pair ? ortho_gemm_pair_kernel<B_MN> : parts ? ortho_gemm_kernel<B_MN, true> : ortho_gemm_kernel<B_MN, false>, grid, OG_THREADS, OG_SMEM, stream, maps, p);
+    auto kern = pair ? ortho_gemm_pair_kernel<B_MN> : parts ? ortho_gemm_kernel<B_MN, true> : ortho_gemm_kernel<B_MN, false>;
+    static std::atomic<uint64_t> done[3];
+    rc = allow_smem(kern, OG_SMEM, done[pair ? 2 : parts]) ? launch_chained(kern, grid, OG_THREADS, OG_SMEM, stream, maps, p) : -20;
     ++launches;
   }
   OrthoGemm empty() const {
@@ -1649,13 +1659,10 @@ struct Products {
     g.partial = partial;
     launch<0>(m, g);
     if (rc) return;
-    static bool configured = false;
-    if (!configured) {
-      if (cudaFuncSetAttribute(ortho_polynomial_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OL_SMEM) != cudaSuccess) {
-        rc = -20;
-        return;
-      }
-      configured = true;
+    static std::atomic<uint64_t> done;
+    if (!allow_smem(ortho_polynomial_kernel, OL_SMEM, done)) {
+      rc = -20;
+      return;
     }
     rc = launch_chained(ortho_polynomial_kernel, l.count, OS_THREADS, OL_SMEM, stream, static_cast<const float*>(partial), splits, S,
                         l.count, l.d, pitch(l.d), steps, status);
@@ -1702,7 +1709,7 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   if (const int rc = l.fill(a)) return rc;
   const bool step = a.grad != nullptr;
   if (step ? !a.momentum || !a.master : !a.x || !a.out) return -6;
-  if (!a.status || (l.bytes && (!a.work || !on_grid(a.work, 1024) || a.work_bytes < l.bytes))) return -7;
+  if (!(a.eps >= 1e-30) || !a.status || (l.bytes && (!a.work || !on_grid(a.work, 1024) || a.work_bytes < l.bytes))) return -7;
   char* work = reinterpret_cast<char*>(a.work);
   OrthoGroups in{}, out{};
   in.n = out.n = a.groups;
@@ -1751,15 +1758,11 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
   const OrthoOutput output = {reinterpret_cast<__nv_bfloat16*>(a.out), a.master, a.ema, reinterpret_cast<__nv_bfloat16*>(a.weights),
                               a.decay, a.ema_beta};
   if (small(l)) {
-    static bool configured = false;
-    if (!configured) {
-      if (cudaFuncSetAttribute(ortho_small_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, OS_SMEM) != cudaSuccess ||
-          cudaFuncSetAttribute(ortho_small_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, OS_SMEM) != cudaSuccess)
-        return -20;
-      configured = true;
-    }
+    auto kern = step ? ortho_small_kernel<true> : ortho_small_kernel<false>;
+    static std::atomic<uint64_t> done[2];
+    if (!allow_smem(kern, OS_SMEM, done[step])) return -20;
     for (int i = 0; i < a.groups; ++i) in.g[i].blocks = 1;
-    const int rc = launch_chained(step ? ortho_small_kernel<true> : ortho_small_kernel<false>, blocks(in), OS_THREADS, OS_SMEM, stream,
+    const int rc = launch_chained(kern, blocks(in), OS_THREADS, OS_SMEM, stream,
                                   in, input, out, output, a.eps, a.steps);
     return rc ? rc : 1;
   }

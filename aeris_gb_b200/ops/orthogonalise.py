@@ -18,6 +18,8 @@ from . import lib as _l
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_GROUPS, MAX_LENGTHS = 4, 2       # shapes of a batch, and longer sides among them
+MAX_SIDE = 1 << 30                   # rows or columns of a matrix
+MIN_EPS = 1e-30                      # one over it, times the scale of the fp16 factors, is a 32-bit number
 MAX_COUNT = 1 << 16                  # matrices of a group
 FEW_ROWS, SHORT_ROWS = 128, 384      # up to so many rows (d) matrices with rows longer than that have a batch for each length
 WORKSPACE_BYTES = 1 << 30            # of one batch; what does not fit goes in several
@@ -75,25 +77,29 @@ def _as_batch(t: torch.Tensor) -> torch.Tensor:
 
 def _pitched(t: torch.Tensor) -> bool:
     """Whether the kernels find the elements of ``t`` [count, rows, cols]: columns side by side, rows one behind the other."""
-    return (t.stride(2) == 1 or t.shape[2] == 1) and (t.shape[1] == 1 or t.stride(1) >= t.shape[2])
+    return (t.stride(2) == 1 or t.shape[2] == 1) and (t.shape[1] == 1 or t.shape[2] <= t.stride(1) < 2 ** 31)
 
 
 def _row_pitch(t: torch.Tensor) -> int:
     return t.stride(1) if t.shape[1] > 1 else t.shape[2]
 
 
-def _check_steps(steps: int) -> None:
+def _check_steps(steps: int, eps: float) -> None:
     if not isinstance(steps, int) or not 1 <= steps <= 20:
         raise ValueError(f"1 to 20 steps are taken, got {steps!r}")
+    if not MIN_EPS <= eps < math.inf:
+        raise ValueError(f"eps from {MIN_EPS} on is taken, got {eps!r}")
 
 
 def orthogonalise(x: torch.Tensor, *, steps: int = 5, eps: float = 1e-7, out: torch.Tensor | None = None) -> torch.Tensor:
     """``x`` [rows, cols] or [count, rows, cols], fp32 or bf16, each matrix by itself; bf16 result of the same shape, ``out``
     where given (any pitch between rows; may not share memory with ``x``). A matrix of zeros stays one; one that holds a NaN or
     an infinity becomes NaN, the others of its batch do not notice."""
-    _check_steps(steps)
+    _check_steps(steps, eps)
     if x.dim() not in (2, 3) or x.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"fp32 or bf16 [rows, cols] or [count, rows, cols], got {x.dtype} {tuple(x.shape)}")
+    if max(x.shape[-2:]) > MAX_SIDE:
+        raise ValueError(f"matrices of up to {MAX_SIDE} rows and columns are taken, got {tuple(x.shape)}")
     if out is not None:
         o = _as_batch(out)
         if out.shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device or (out.numel() and not (
@@ -170,9 +176,10 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
     ``zero_grad``. ``norm_sq`` and ``max_norm``: clipping as in ``adamw``. ``groups``: (rows, cols, offsets) for matrices that lie
     without gaps from the element offsets on, an int64 tensor on the same device, ascending; no two matrices may overlap. One
     that does not lie inside the buffers, or not behind the one before it, is left as it is and sets the status word, and so
-    does one that shares elements with a matrix of another group: the call has then failed (``lib.check_status`` raises), and
-    which of its other matrices have been updated is not defined. Elements of no matrix are not touched. ``scale`` = 0.2 gives updates the root mean square of AdamW's."""
-    _check_steps(steps)
+    does one that shares elements with a matrix of another group in the same launch (one shorter side): the call has then
+    failed (``lib.check_status`` raises), and which of its other matrices have been updated is not defined. Elements of no
+    matrix are not touched. ``scale`` = 0.2 gives updates the root mean square of AdamW's."""
+    _check_steps(steps, eps)
     if master.dim() != 1 or master.dtype != torch.float32 or not master.is_contiguous() or master.data_ptr() % 16:
         raise ValueError(f"master: contiguous fp32 [n] from a 16-byte boundary on, got {master.dtype} {tuple(master.shape)}")
     for name, t, dt in (("grad", grad, torch.float32), ("momentum", momentum, torch.float32), ("weights", weights, torch.bfloat16),
@@ -183,7 +190,7 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
         raise ValueError(f"norm_sq: one fp64 value on {master.device}, got {norm_sq.dtype} {tuple(norm_sq.shape)}")
     todo = []
     for rows, cols, offsets in groups:
-        if rows < 1 or cols < 1 or offsets.dim() != 1 or offsets.dtype != torch.int64 or offsets.device != master.device \
+        if not 1 <= rows <= MAX_SIDE or not 1 <= cols <= MAX_SIDE or offsets.dim() != 1 or offsets.dtype != torch.int64 or offsets.device != master.device \
                 or not offsets.is_contiguous():
             raise ValueError(f"groups hold (rows, cols, contiguous int64 offsets on {master.device}), got ({rows}, {cols}, "
                              f"{offsets.dtype} {tuple(offsets.shape)} on {offsets.device})")

@@ -12,6 +12,8 @@ from aeris_gb_b200.ops import orthogonalise as OR
     (torch.randn(4, 4), dict(out=torch.empty(1, 4).bfloat16().expand(4, 4))),
     (torch.randn(2, 4, 4), dict(out=torch.empty(1, 4, 4).bfloat16().expand(2, 4, 4))),
     (torch.randn(4, 4), dict(out=torch.empty(4, 4).bfloat16().t())),
+    (torch.randn(4, 4), dict(eps=0.0)), (torch.randn(4, 4), dict(eps=-1e-7)), (torch.randn(4, 4), dict(eps=float("nan"))),
+    (torch.randn(1).expand(1, 2 ** 30 + 1), {}), (torch.randn(1).expand(2 ** 30 + 1, 1), {}),
     (torch.randn(4, 4), {}),                                                     # not on a GPU
 ])
 def test_orthogonalise_refuses(x, kw):
@@ -40,8 +42,17 @@ def step(**over):
     dict(groups=[(0, 4, torch.tensor([0]))]), dict(groups=[(4, 4, torch.tensor([0], dtype=torch.int32))]),
     dict(groups=[(4, 4, torch.tensor([[0]]))]), dict(groups=[(4, 4, torch.tensor([0, 1, 2, 3])[::2])]),
     dict(groups=[(4, 4, torch.tensor([0, 16, 32, 48, 64]))]), dict(groups=[(9, 9, torch.tensor([0]))]), dict(steps=0),
+    dict(eps=0.0), dict(groups=[(1, 2 ** 30 + 1, torch.tensor([], dtype=torch.int64))]),
     {},                                                                           # not on a GPU
 ])
 def test_step_refuses(bad):
     with pytest.raises(ValueError):
         step(**bad)
+
+
+@pytest.mark.parametrize("strides,shape,fine", [((32, 8, 1), (2, 4, 8), True), ((32, 7, 1), (2, 4, 8), False),
+                                                ((32, 0, 1), (2, 4, 8), False), ((32, 1, 4), (2, 4, 8), False),
+                                                ((0, 2 ** 31 - 1, 1), (2, 4, 8), True), ((0, 2 ** 31, 1), (2, 4, 8), False),
+                                                ((0, 2 ** 40, 1), (2, 1, 8), True), ((0, 9, 5), (2, 4, 1), True)])
+def test_pitches_that_the_kernels_count(strides, shape, fine):
+    assert OR._pitched(torch.empty(1, device="meta").as_strided(shape, strides)) == fine
