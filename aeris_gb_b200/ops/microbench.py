@@ -1,4 +1,5 @@
-"""Kernel micro-benchmarks: ``python -m aeris_gb_b200.ops.microbench <gemm|attn_fwd|attn_bwd|modnorm|modnorm_bwd|swiglu|adamw|embed|loss> ...``
+"""Kernel micro-benchmarks: ``python -m aeris_gb_b200.ops.microbench <gemm|attn_fwd|attn_bwd|modnorm|modnorm_bwd|qk_norm|qk_norm_bwd|
+orthogonalise|orthogonal_step|swiglu|adamw|embed|loss> ...``
 
 Times one kernel with CUDA events (3 warm-up launches, then ``--iters`` launches, inputs larger than L2) and prints
 one JSON line with achieved TFLOP/s or GB/s and, when ``MEASURED_PEAKS.json`` is present at the repository root, the
@@ -62,7 +63,8 @@ def _time(fn, iters):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "attn_fwd", "attn_bwd", "modnorm", "modnorm_bwd", "swiglu", "adamw",
+    ap.add_argument("kernel", choices=["gemm", "attn_fwd", "attn_bwd", "modnorm", "modnorm_bwd", "qk_norm", "qk_norm_bwd",
+                                       "orthogonalise", "orthogonal_step", "swiglu", "adamw",
                                        "embed", "loss", "fused_ag_gemm", "fused_rs_gemm", "fused_scatter_heads",
                                        "fused_grad_rs", "fused_shard_adamw", "fused_modnorm_gather"])
     ap.add_argument("--m", type=int, default=32768)
@@ -78,6 +80,7 @@ def main():
     ap.add_argument("--head-dim", type=int, default=64)
     ap.add_argument("--rows", type=int, default=129600)
     ap.add_argument("--dim", type=int, default=1536)
+    ap.add_argument("--count", type=int, default=1, help="orthogonalise, orthogonal_step: matrices of --m rows and --n columns")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--one-cta", action="store_true", help="force the one-CTA GEMM kernel")
     ap.add_argument("--fwd-variant", type=int, default=None,
@@ -150,6 +153,40 @@ def main():
         by = 4.0 * x.numel() * 2
         out.update(shape=[a.rows, a.dim], ms=ms, gbs=by / ms / 1e6, frac_of_peak=by / ms / 1e6 / bw_peak,
                    peak_source=src)
+    elif a.kernel in ("qk_norm", "qk_norm_bwd"):
+        from . import qk_norm as QN
+        rows, H, d = a.windows * a.tokens, a.heads, a.head_dim
+        angles = torch.randn(a.tokens, d // 2, device=dev)
+        cos, sin = angles.cos(), angles.sin()
+        q, k, dq, dk = (torch.randn(rows, H, d, device=dev).bfloat16() for _ in range(4))
+        w = torch.ones(d, device=dev).bfloat16()
+        yq, yk = torch.empty_like(q), torch.empty_like(k)
+        dw = torch.zeros(2, d, device=dev)
+        if a.kernel == "qk_norm":
+            ms = _time(lambda: QN.qk_norm_fwd(q, k, w, w, cos, sin, eps=1e-6, q_out=yq, k_out=yk), a.iters)
+        else:
+            ms = _time(lambda: QN.qk_norm_bwd(dq, dk, q, k, w, w, cos, sin, eps=1e-6, dq_out=yq, dk_out=yk, dwq=dw[0], dwk=dw[1]),
+                       a.iters)
+        by = (2.0 if a.kernel == "qk_norm" else 3.0) * 2 * q.numel() * 2
+        out.update(shape=[rows, H, d], ms=ms, gbs=by / ms / 1e6, frac_of_peak=by / ms / 1e6 / bw_peak, peak_source=src)
+    elif a.kernel in ("orthogonalise", "orthogonal_step"):
+        from . import orthogonalise as OR
+        size = a.m * a.n
+        x = torch.randn(a.count, a.m, a.n, device=dev)
+        short, ratio = min(a.m, a.n), max(a.m, a.n) / min(a.m, a.n)
+        if a.kernel == "orthogonalise":
+            y = torch.empty_like(x, dtype=torch.bfloat16)
+            ms = _time(lambda: OR.orthogonalise(x, out=y), a.iters)
+        else:
+            grad, master = x.view(-1), torch.randn(x.numel(), device=dev)
+            momentum, ema, weights = torch.zeros_like(master), master.clone(), master.bfloat16()
+            groups = [(a.m, a.n, torch.arange(a.count, device=dev) * size)]
+            ms = _time(lambda: OR.orthogonal_step(master, grad, momentum, weights, ema, None, groups=groups, lr=1e-3, beta=0.95,
+                                                  nesterov=True, weight_decay=0.1, scale=0.2, grad_scale=1.0, max_norm=0.0,
+                                                  ema_beta=0.999, zero_grad=False), a.iters)
+        # five steps by themselves, symmetric products at half: what the time is compared with, not what is computed
+        fl = 5 * (3 * ratio + 1) * a.count * float(short) ** 3
+        out.update(shape=[a.count, a.m, a.n], ms=ms, tflops=fl / ms / 1e9, frac_of_peak=fl / ms / 1e9 / tf_peak, peak_source=src)
     elif a.kernel in ("embed", "loss"):
         from ..models import layout as LY
         from . import diffusion as DF
