@@ -64,9 +64,10 @@ def on_device(device: torch.device):
 _STATUS: dict[int, torch.Tensor] = {}
 
 
-def status_word() -> torch.Tensor:
-    """Per-device int32 word that kernels set when a bounded wait runs out or a bounds check fails."""
-    dev = torch._C._cuda_getDevice()
+def status_word(device: torch.device | None = None) -> torch.Tensor:
+    """Per-device int32 word that kernels set when a bounded wait runs out or a bounds check fails; of the current device where
+    none is given."""
+    dev = torch._C._cuda_getDevice() if device is None else device.index
     if dev not in _STATUS:
         _STATUS[dev] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
     return _STATUS[dev]

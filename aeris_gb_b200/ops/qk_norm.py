@@ -21,12 +21,7 @@ MAX_ROWS = 2 ** 31 - 2 ** 21
 # AerisQkNorm (csrc/api.h), field by field: packing 39 values takes 0.4 us, filling a ctypes.Structure with them 12.
 _RECORD = struct.Struct("Pqq" * 6 + "9P" + "q" + "10i" + "f" + "0q")
 _FLOATS = (torch.bfloat16, torch.float32)
-_NOWHERE = (0, 0, 0)
-
-
-def _heads(t: torch.Tensor) -> tuple[int, int, int]:
-    row, head, _ = t.stride()
-    return t.data_ptr(), row, head
+_INTEGERS = (torch.int32, torch.int64)
 
 
 def _like(t: torch.Tensor, shape, dtype, device) -> bool:
@@ -44,8 +39,31 @@ def _text(t) -> str:
     return f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
 
 
-def _check(q, k, wq, wk, cos, sin, positions, rows_like_q, rows_like_k, results, dw=()) -> tuple[int, ...]:
-    """Refuses what the kernels cannot take; returns (rows, heads, kv_heads, d, table length, rotated channels)."""
+def _check_more(shape, dt, dev, *tensors) -> None:
+    for t in tensors:
+        if t is not None and not _like(t, shape, dt, dev):
+            raise ValueError(f"{dt} {tuple(shape)} on {dev} with channels side by side, got {_text(t)}")
+
+
+def _check_results(q_out, k_out, rows: int) -> None:
+    for t in (q_out, k_out):
+        if t is not None and not _apart(t):
+            raise ValueError(f"elements of a result share addresses: {_text(t)}")
+    if rows and q_out is not None and k_out is not None and q_out.data_ptr() == k_out.data_ptr():
+        raise ValueError("the results of q and k are the same memory")
+
+
+def _check_dw(dwq, dwk, d: int, dev) -> None:
+    for t in (dwq, dwk):
+        if t.shape != (d,) or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"gradients of the weights: contiguous fp32 [{d}] on {dev}, got {_text(t)}")
+    if 0 < abs(dwq.data_ptr() - dwk.data_ptr()) < 4 * d:
+        raise ValueError("gradients of the weights that overlap are the same tensor, a weight's that q and k share")
+
+
+def _check(q, k, wq, wk, cos, sin, positions):
+    """Refuses what the kernels cannot take of the inputs that both directions share; returns (shape of q, of k, strides of q,
+    of k, type, device, table length, rotated channels). Every attribute is asked for once: they are half of a small call."""
     qs, ks, dt, dev = q.shape, k.shape, q.dtype, q.device
     if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or dt not in _FLOATS:
         raise ValueError(f"q [rows, heads, d] and k [rows, kv_heads, d] in bf16 or fp32, got {_text(q)} and {_text(k)}")
@@ -54,38 +72,25 @@ def _check(q, k, wq, wk, cos, sin, positions, rows_like_q, rows_like_k, results,
         raise ValueError(f"{rows} rows: at most {MAX_ROWS} are taken")
     if not 0 < d <= MAX_HEAD_DIM or d % 2 or heads < 1 or ks[1] < 1:
         raise ValueError(f"{heads} and {ks[1]} heads of {d} channels: heads of an even width up to {MAX_HEAD_DIM} are taken")
-    if not (q.stride(2) == 1 == k.stride(2)) or k.dtype is not dt or k.device != dev:
+    q_at, k_at = q.stride(), k.stride()
+    if not (q_at[2] == 1 == k_at[2]) or k.dtype is not dt or k.device != dev:
         raise ValueError(f"q and k: one type, one device, channels side by side, got {_text(q)} and {_text(k)}")
-    for shape, tensors in ((qs, rows_like_q), (ks, rows_like_k)):
-        for t in tensors:
-            if t is not None and not _like(t, shape, dt, dev):
-                raise ValueError(f"{dt} {tuple(shape)} on {dev} with channels side by side, got {_text(t)}")
-    for t in results:
-        if t is not None and not _apart(t):
-            raise ValueError(f"elements of a result share addresses: {_text(t)}")
-    if rows and results[0] is not None and results[1] is not None and results[0].data_ptr() == results[1].data_ptr():
-        raise ValueError("the results of q and k are the same memory")
     w_dt, one = wq.dtype, (d,)
     if not (wq.shape == one == wk.shape and w_dt in _FLOATS and w_dt is wk.dtype and wq.device == dev == wk.device
             and wq.is_contiguous() and wk.is_contiguous()):
         raise ValueError(f"weights: bf16 or fp32 [{d}] on {dev}, both alike, got {_text(wq)} and {_text(wk)}")
-    for t in dw:
-        if t.shape != (d,) or t.dtype is not torch.float32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"gradients of the weights: contiguous fp32 [{d}] on {dev}, got {_text(t)}")
-    if dw and 0 < abs(dw[0].data_ptr() - dw[1].data_ptr()) < 4 * d:
-        raise ValueError("gradients of the weights that overlap are the same tensor, a weight's that q and k share")
     if cos is None or sin is None:
         if cos is not None or sin is not None or positions is not None:
             raise ValueError("cos and sin come together, positions only with them")
-        return rows, heads, ks[1], d, 0, 0
+        return qs, ks, q_at, k_at, dt, dev, 0, 0
     table = cos.shape
     if not (len(table) == 2 and sin.shape == table and cos.dtype is torch.float32 is sin.dtype and cos.device == dev == sin.device
             and cos.is_contiguous() and sin.is_contiguous() and 2 * table[1] <= d and (table[0] > 0 or not rows)):
         raise ValueError(f"angles: contiguous fp32 [L, at most {d // 2}] on {dev}, got {_text(cos)} and {_text(sin)}")
-    if positions is not None and not (positions.shape == (rows,) and positions.dtype in (torch.int32, torch.int64)
+    if positions is not None and not (positions.shape == (rows,) and positions.dtype in _INTEGERS
                                       and positions.device == dev and positions.is_contiguous()):
         raise ValueError(f"positions: contiguous int32 or int64 [{rows}] on {dev}, got {_text(positions)}")
-    return rows, heads, ks[1], d, table[0], 2 * table[1]
+    return qs, ks, q_at, k_at, dt, dev, table[0], 2 * table[1]
 
 
 @functools.lru_cache(maxsize=None)
@@ -100,16 +105,11 @@ def _multiprocessors(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-def _record(sizes, q, k, dq, dk, q_out, k_out, wq, wk, cos, sin, positions, dwq, dwk, sums, add, eps) -> bytes:
-    rows, heads, kv_heads, d, length, rot = sizes
-    return _RECORD.pack(*_heads(q), *_heads(k), *(_heads(dq) if dq is not None else _NOWHERE),
-                        *(_heads(dk) if dk is not None else _NOWHERE), *_heads(q_out), *_heads(k_out), wq.data_ptr(), wk.data_ptr(),
-                        cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0,
-                        positions.data_ptr() if positions is not None else 0, dwq.data_ptr() if dwq is not None else 0,
-                        dwk.data_ptr() if dwk is not None else 0, sums.data_ptr() if sums is not None else 0,
-                        _l.status_word().data_ptr(), rows, length, heads, kv_heads, d, rot, q.dtype is torch.float32,
-                        wq.dtype is torch.bfloat16, positions is not None and positions.dtype is torch.int64, add,
-                        sums.shape[0] if sums is not None else 0, eps)
+def _launch(name: str, record: bytes, dev) -> int:
+    if torch._C._cuda_getDevice() == dev.index:
+        return _entry(name)(record, _l.raw_stream())
+    with torch.cuda.device(dev):
+        return _entry(name)(record, _l.raw_stream())
 
 
 def qk_norm_fwd(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, cos: torch.Tensor | None = None,
@@ -119,16 +119,30 @@ def qk_norm_fwd(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Te
     a fused qkv matrix): normed by head with the weights ``wq``, ``wk`` [d] and, with ``cos`` / ``sin``, turned. ``positions``
     [rows] int32 or int64: the table row of every row; one outside the table sets the status word and its row is not written.
     ``q_out``, ``k_out``: where to put the results, memory of their own or ``q`` and ``k`` themselves."""
-    sizes = _check(q, k, wq, wk, cos, sin, positions, (q_out,), (k_out,), (q_out, k_out))
+    qs, ks, q_at, k_at, dt, dev, length, rot = _check(q, k, wq, wk, cos, sin, positions)
+    rows, heads, d = qs
+    if q_out is not None or k_out is not None:
+        _check_more(qs, dt, dev, q_out)
+        _check_more(ks, dt, dev, k_out)
+        _check_results(q_out, k_out, rows)
     _l.require_cuda(q)
+    q_row, q_head, k_row, k_head = heads * d, d, ks[1] * d, d
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        q_row, q_head, _ = q_out.stride()
     if k_out is None:
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    if sizes[0]:
-        with _l.on_device(q.device):
-            a = _record(sizes, q, k, None, None, q_out, k_out, wq, wk, cos, sin, positions, None, None, None, False, eps)
-            _l.check(_entry("aeris_qk_norm_fwd")(a, _l.raw_stream()), "aeris_qk_norm_fwd")
+    else:
+        k_row, k_head, _ = k_out.stride()
+    if rows:
+        record = _RECORD.pack(q.data_ptr(), q_at[0], q_at[1], k.data_ptr(), k_at[0], k_at[1], 0, 0, 0, 0, 0, 0, q_out.data_ptr(),
+                              q_row, q_head, k_out.data_ptr(), k_row, k_head, wq.data_ptr(), wk.data_ptr(),
+                              cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0,
+                              0 if positions is None else positions.data_ptr(), 0, 0, 0, _l.status_word(dev).data_ptr(), rows, length,
+                              heads, ks[1], d, rot, dt is torch.float32, wq.dtype is torch.bfloat16,
+                              positions is not None and positions.dtype is torch.int64, 0, 0, eps)
+        _l.check(_launch("aeris_qk_norm_fwd", record, dev), "aeris_qk_norm_fwd")
     return q_out, k_out
 
 
@@ -143,19 +157,34 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
     add = dwq is not None
     if add != (dwk is not None):
         raise ValueError("dwq and dwk come together")
-    sizes = _check(q, k, wq, wk, cos, sin, positions, (dq, dq_out), (dk, dk_out), (dq_out, dk_out), (dwq, dwk) if add else ())
+    qs, ks, q_at, k_at, dt, dev, length, rot = _check(q, k, wq, wk, cos, sin, positions)
+    rows, heads, d = qs
+    _check_more(qs, dt, dev, dq, dq_out)
+    _check_more(ks, dt, dev, dk, dk_out)
+    _check_results(dq_out, dk_out, rows)
+    if add:
+        _check_dw(dwq, dwk, d, dev)
     _l.require_cuda(q)
     if dq_out is None:
         dq_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if dk_out is None:
         dk_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     if not add:
-        make = torch.empty_like if sizes[0] else torch.zeros_like
+        make = torch.empty_like if rows else torch.zeros_like
         dwq, dwk = make(wq, dtype=torch.float32), make(wk, dtype=torch.float32)
-    if sizes[0]:
-        with _l.on_device(q.device):
-            sums = q.new_empty((4 * _multiprocessors(q.get_device()), sizes[3]), dtype=torch.float32)
-            a = _record(sizes, q, k, dq, dk, dq_out, dk_out, wq, wk, cos, sin, positions, dwq, dwk, sums, add, eps)
-            rc = _entry("aeris_qk_norm_bwd")(a, _l.raw_stream())
-            _l.check(min(rc, 0), "aeris_qk_norm_bwd", kernels=max(rc, 0))
+    if rows:
+        blocks = 4 * _multiprocessors(dev.index)
+        sums = torch.empty((blocks, d), dtype=torch.float32, device=dev)
+        dq_row, dq_head, _ = dq.stride()
+        dk_row, dk_head, _ = dk.stride()
+        q_row, q_head, _ = dq_out.stride()
+        k_row, k_head, _ = dk_out.stride()
+        record = _RECORD.pack(q.data_ptr(), q_at[0], q_at[1], k.data_ptr(), k_at[0], k_at[1], dq.data_ptr(), dq_row, dq_head,
+                              dk.data_ptr(), dk_row, dk_head, dq_out.data_ptr(), q_row, q_head, dk_out.data_ptr(), k_row, k_head,
+                              wq.data_ptr(), wk.data_ptr(), cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0,
+                              0 if positions is None else positions.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), sums.data_ptr(),
+                              _l.status_word(dev).data_ptr(), rows, length, heads, ks[1], d, rot, dt is torch.float32,
+                              wq.dtype is torch.bfloat16, positions is not None and positions.dtype is torch.int64, add, blocks, eps)
+        rc = _launch("aeris_qk_norm_bwd", record, dev)
+        _l.check(min(rc, 0), "aeris_qk_norm_bwd", kernels=max(rc, 0))
     return dq_out, dk_out, dwq, dwk
