@@ -107,6 +107,28 @@ CASES = [  # rows, heads, kv heads, d, rot, L, type, weights, positions, layout
     (19, 2, 2, 256, 256, 19, torch.bfloat16, None, torch.int32, "heads first"),
     (11, 2, 2, 254, 254, 11, torch.float32, None, None, "own"),
     (4099, 2, 2, 32, 32, 64, torch.bfloat16, None, None, "fused"),
+    # widths of whole fours, with every kind of rotation
+    (257, 5, 3, 20, 10, 33, torch.bfloat16, None, torch.int32, "own"),
+    (300, 9, 2, 36, 18, 100, torch.bfloat16, torch.float32, None, "fused"),
+    (101, 4, 4, 100, 50, 101, torch.bfloat16, None, None, "own"),
+    (64, 3, 3, 100, 100, 64, torch.float32, None, torch.int64, "heads first"),
+    (90, 7, 1, 12, 12, 9, torch.float32, None, None, "own"),
+    (33, 2, 2, 4, 4, 33, torch.bfloat16, None, None, "own"),
+    (120, 6, 6, 128, 60, 40, torch.bfloat16, None, None, "fused"),
+    (77, 2, 2, 252, 130, 7, torch.bfloat16, None, None, "own"),
+    (59, 3, 2, 256, 256, 59, torch.float32, None, None, "own"),
+    # groups of three, five, six, nine and ten lanes
+    (210, 11, 4, 24, 24, 70, torch.bfloat16, None, None, "own"),
+    (211, 13, 5, 40, 20, 71, torch.float32, None, torch.int32, "fused"),
+    (212, 6, 2, 48, 48, 72, torch.bfloat16, None, None, "fused"),
+    (213, 4, 3, 72, 72, 73, torch.bfloat16, None, None, "own"),
+    (214, 7, 2, 80, 80, 74, torch.float32, None, None, "heads first"),
+    # steps that take heads of several rows, up to a row that is the last of them
+    (1001, 1, 1, 8, 8, 100, torch.bfloat16, None, torch.int32, "own"),
+    (1003, 2, 1, 64, 64, 1003, torch.bfloat16, None, None, "fused"),
+    (2049, 3, 1, 24, 12, 50, torch.float32, None, torch.int64, "fused"),
+    (515, 4, 1, 16, 16, 515, torch.bfloat16, None, None, "heads first"),
+    (5, 1, 1, 2, 2, 5, torch.float32, None, None, "own"),
 ]
 
 
@@ -189,6 +211,19 @@ def test_in_place_and_into_sections(d):
         3 + gwk.abs().max())
     QN.qk_norm_fwd(q, k, wq, wk, cos, sin, eps=1e-6, q_out=q, k_out=k)
     assert torch.equal(q, yq) and torch.equal(k, yk)
+
+
+@pytest.mark.parametrize("heads,d,dt", [(5, 64, torch.bfloat16), (1, 24, torch.float32), (3, 100, torch.bfloat16), (5, 72, torch.float32)])
+def test_without_eps(heads, d, dt):
+    """Places of a step that hold no head have a root of zero, which must not reach the sums."""
+    q, k, dq, dk, wq, wk, cos, sin, _, at = make(37, heads, heads, d, d, 37, dt)
+    yq, _ = QN.qk_norm_fwd(q, k, wq, wk, cos, sin, eps=0.0)
+    close(yq, *formula(q, wq, cos, sin, at, 0.0), dt)
+    gq, _, gwq, gwk = QN.qk_norm_bwd(dq, dk, q, k, wq, wk, cos, sin, eps=0.0)
+    ex, size, ew, wsize = formula(q, wq, cos, sin, at, 0.0, dq)
+    close(gq, ex, size, dt)
+    close(gwq, ew, wsize, torch.float32, 16 + 37 * heads)
+    assert bool(gwk.isfinite().all())
 
 
 @pytest.mark.parametrize("rows,d", [(1, 16), (700, 64), (33, 250)])
