@@ -14,8 +14,8 @@
 // (200,000 rows of 8 + 2 heads of 8: 93 us a row a step, 19 so). q and k have blocks in proportion to the time of a row. Everything
 // between load and store is fp32. 64,800 rows of 24 + 24 heads of 64, bf16: forward 135 us, 5.9 TB/s (90 % of what a plain copy
 // reaches); backward 214 us, 5.6 TB/s; 28,800 rows of 40 + 40 heads of 128 backward 319 us. fp32: 5.3 to 6 TB/s both ways from 64
-// channels on. Less where lanes or steps stay empty: 3.8 to 4.8 TB/s with heads of 72 to 104, 2 to 4 with heads of 16 to 36, 1.4
-// where heads are not whole fours. One row, or one window of 900, takes the GPU 2 to 4 us, less than the host needs (12).
+// channels on. Less where lanes or steps stay empty: 3.8 to 4.8 TB/s with heads of 72 to 104, 2 to 4 with heads of 16 to 36, 0.4
+// to 1.4 where heads are not whole fours. One row, or one window of 900, takes the GPU 2 to 4 us, less than the host needs (12).
 #include "api.h"
 #include "common.cuh"
 #include "host.h"
