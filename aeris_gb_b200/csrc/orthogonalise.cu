@@ -947,7 +947,10 @@ __global__ void __launch_bounds__(256) ortho_reduce_kernel(const float* __restri
 // three products a step whose operands never leave shared memory (X in blocks of 64 columns of 128 swizzled rows, which serve
 // as the K-major operands of X X^T and as the MN-major one of P X), accumulators in tensor memory, a barrier or two between.
 // Eight matrices of 64 x 64: 64 us by the launches above, 33 of them on the host, 13 by this one.
-constexpr int OS_MAX_D = 128, OS_MAX_K = 384, OS_THREADS = 256;
+constexpr int OS_MAX_D = 128, OS_MAX_K = 384, OS_THREADS = 512;
+// Threads: a warp for 32 rows and 32 columns of a square factor, 16 warps above 64 rows and 8 up to there (eight 128 x 384 by 8 warps
+// 42.7 us, by 16 38; 64 x 64 12.2 and 13.2).
+constexpr int os_threads(int d) { return d > 64 ? OS_THREADS : OS_THREADS / 2; }
 constexpr int OS_BLOCK = 128 * 128;           // 64 columns of 128 rows, in bytes
 constexpr int OS_S = (OS_MAX_K / 64) * OS_BLOCK, OS_P = OS_S + 2 * OS_BLOCK, OS_BARS = OS_P + 2 * OS_BLOCK;
 constexpr int OS_SMEM = OS_BARS + 256 + 1024;
@@ -977,8 +980,8 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + OS_BARS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   double* red = reinterpret_cast<double*>(bar + 4);
-  int* gave_up = reinterpret_cast<int*>(bar + 16);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* gave_up = reinterpret_cast<int*>(bar + 4 + OS_THREADS / 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x;
   if (threadIdx.x == 0) {
     mbar_init(bar, 1);
     fence_barrier_init();
@@ -1000,7 +1003,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   const bool upright = m.rows > m.cols;
   const int d = upright ? m.cols : m.rows, K = upright ? m.rows : m.cols;
   const int blocks = (K + 63) / 64;
-  for (int i = threadIdx.x; i < blocks * OS_BLOCK / 16; i += OS_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < blocks * OS_BLOCK / 16; i += threads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   const float gs = STEP ? step_scale(in) : 0.f;
   double sum = 0;
   // The matrix in vectors of W = 4 elements or 1, four per thread at a time: `before` for all four (loads), then `work`, both
@@ -1008,7 +1011,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   constexpr int U = 4;
   auto walk = [&](auto width, int ld, long long at, auto before, auto work) {
     constexpr int W = decltype(width)::value;
-    const int per_row = m.cols / W, down = OS_THREADS / per_row, over = OS_THREADS - down * per_row;
+    const int per_row = m.cols / W, down = threads / per_row, over = threads - down * per_row;
     int r = threadIdx.x / per_row, c = threadIdx.x - r * per_row;
     while (r < m.rows) {
       int rr[U], cc[U];
@@ -1063,7 +1066,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   if (lane == 0) red[warp] = sum;
   __syncthreads();
   sum = 0;
-  for (int i = 0; i < OS_THREADS / 32; ++i) sum += red[i];
+  for (int i = 0; i < threads / 32; ++i) sum += red[i];
   const double norm = sqrt(sum);
   const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
   if (p.found)                                // each thread reads what it has written
@@ -1124,19 +1127,16 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
         umma_ss4_warp<2, 2>(lead, t_s, lo, lo, make_idesc_fp16(128, wide, 0), k > 0);
       }
     });
-    float s[64];
-    const int mine = wide / 2, c0 = part * mine;         // this warp's columns of the factors
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= mine) break;
+    float s[32];
+    const int c0 = part * 32;                 // this warp's columns of the factors
+    if (c0 < wide) {
       uint32_t v[32];
-      tmem_ld32(t_s + lanes + c0 + 32 * h, v);
+      tmem_ld32(t_s + lanes + c0, v);
       tmem_wait_ld();
-      float f[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j)           // b S takes S as it is in c S^2: near 1 most of a rounding cancels between the two
-        f[j] = s[32 * h + j] = __half2float(__float2half_rn(__uint_as_float(v[j]) * (1.f / NS_SCALE)));
-      os_put(smem + OS_S, row, c0 + 32 * h, f);
+        s[j] = __half2float(__float2half_rn(__uint_as_float(v[j]) * (1.f / NS_SCALE)));
+      os_put(smem + OS_S, row, c0, s);
     }
     products([&] {
       for (int k = 0; k < wide / 64; ++k) {
@@ -1144,17 +1144,15 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
         umma_ss4_warp<2, 2>(lead, t_s, lo, lo, make_idesc_fp16(128, wide, 0), k > 0);
       }
     });
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= mine) break;
+    if (c0 < wide) {
       uint32_t v[32];
-      tmem_ld32(t_s + lanes + c0 + 32 * h, v);
+      tmem_ld32(t_s + lanes + c0, v);
       tmem_wait_ld();
       float f[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        f[j] = NS_C / NS_SCALE * __uint_as_float(v[j]) + NS_B * s[32 * h + j] + (row == c0 + 32 * h + j ? NS_A * NS_SCALE : 0.f);
-      os_put(smem + OS_P, row, c0 + 32 * h, f);
+        f[j] = NS_C / NS_SCALE * __uint_as_float(v[j]) + NS_B * s[j] + (row == c0 + j ? NS_A * NS_SCALE : 0.f);
+      os_put(smem + OS_P, row, c0, f);
     }
     products([&] {
       for (int c = 0; c < blocks * 64; c += 256) {
@@ -1164,7 +1162,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
                                 smem_desc_lo(x_at + (c >> 6) * OS_BLOCK + k * 8192, OS_BLOCK), make_idesc_fp16(128, cols, 1), k > 0);
       }
     });
-    for (int c = part * 32; c < blocks * 64; c += 64) {
+    for (int c = part * 32; c < blocks * 64; c += threads / 4) {
       uint32_t v[32];
       tmem_ld32(tmem + lanes + c, v);
       tmem_wait_ld();
@@ -1229,6 +1227,8 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
 // keeps groups of steps from being longer than two elsewhere, the Gram matrix's rounding, is answered by precision here: sums of
 // X X^T stay in 32 bits, and the [d, d] factors are kept as two fp16 numbers (22 bits), which a product takes as three. Their
 // product Q is applied in both parts too: its entries reach a^5, and rounded to 11 bits they would leave 0.1 of a large direction.
+// Bound by the chain of products, three deep a step and each three times over: 128 x 4000 takes 64 us in six launches (71 with 8
+// warps here instead of 16), 64 x 4000 43.
 constexpr float NS_Q_SCALE = 64.f;
 constexpr int OL_MAX_STEPS = 5;               // a^5 times the scale is inside fp16's range
 constexpr int OL_S = 0, OL_P = 4 * OS_BLOCK, OL_Q = 8 * OS_BLOCK, OL_BARS = 12 * OS_BLOCK;      // hi, then lo
@@ -1270,7 +1270,8 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
   chain_point();
 
   const int q = warp & 3, part = warp >> 2, row = q * 32 + lane;
-  const int wide = d > 64 ? 128 : 64, mine = wide / 2, c0 = part * mine;
+  const int wide = d > 64 ? 128 : 64, c0 = part * 32;        // this warp's columns
+  const bool mine = c0 < wide;
   const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
   uint8_t *S = smem + OL_S, *P = smem + OL_P, *QQ = smem + OL_Q;
   uint32_t phase = 0;
@@ -1311,25 +1312,23 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
     sums[r * 32 + (c ^ (r & 7))] = x;
   }
   __syncthreads();
-  float s[64];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (32 * h >= mine) break;
+  float s[32];
+  if (mine) {
     float f[32];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 x = row < wide ? sums[row * 32 + (((c0 + 32 * h) / 4 + j) ^ (row & 7))] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = row < wide ? sums[row * 32 + ((c0 / 4 + j) ^ (row & 7))] : make_float4(0.f, 0.f, 0.f, 0.f);
       f[4 * j] = x.x; f[4 * j + 1] = x.y; f[4 * j + 2] = x.z; f[4 * j + 3] = x.w;
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[32 * h + j] = f[j] *= 1.f / NS_SCALE;
-    os_put2(S, row, c0 + 32 * h, f);
+    for (int j = 0; j < 32; ++j) s[j] = f[j] *= 1.f / NS_SCALE;
+    os_put2(S, row, c0, f);
   }
   __syncthreads();                            // all sums are taken before Q comes
   // this lane's columns c0 + 32 h .. of an accumulator, times alpha
-  auto take = [&](uint32_t from, int h, float alpha, float (&f)[32]) {
+  auto take = [&](uint32_t from, float alpha, float (&f)[32]) {
     uint32_t v[32];
-    tmem_ld32(tmem + from + lanes + c0 + 32 * h, v);
+    tmem_ld32(tmem + from + lanes + c0, v);
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 32; ++j) f[j] = alpha * __uint_as_float(v[j]);
@@ -1339,18 +1338,16 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
     begin();
     if (warp == 0 && ok) product(0, S, S);
     finish();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= mine) break;
+    if (mine) {
       float f[32];
-      take(0, h, NS_C / NS_SCALE, f);
+      take(0, NS_C / NS_SCALE, f);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) f[j] += NS_B * s[32 * h + j] + (row == c0 + 32 * h + j ? NS_A * NS_SCALE : 0.f);
-      os_put2(P, row, c0 + 32 * h, f);
+      for (int j = 0; j < 32; ++j) f[j] += NS_B * s[j] + (row == c0 + j ? NS_A * NS_SCALE : 0.f);
+      os_put2(P, row, c0, f);
       if (step == 0) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] *= NS_Q_SCALE / NS_SCALE;
-        os_put2(QQ, row, c0 + 32 * h, f);
+        os_put2(QQ, row, c0, f);
       }
     }
     if (step || !last) {
@@ -1361,31 +1358,27 @@ ortho_polynomial_kernel(const float* __restrict__ partial, int splits, __half* _
       }
       finish();
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= mine) break;
+    if (mine) {
       float f[32];
       if (step) {
-        take(128, h, 1.f / NS_SCALE, f);
-        os_put2(QQ, row, c0 + 32 * h, f);
+        take(128, 1.f / NS_SCALE, f);
+        os_put2(QQ, row, c0, f);
       }
       if (!last) {
-        take(0, h, 1.f / NS_SCALE, f);
-        os_put2(S, row, c0 + 32 * h, f);      // P S takes the place of S
+        take(0, 1.f / NS_SCALE, f);
+        os_put2(S, row, c0, f);      // P S takes the place of S
       }
     }
     if (last) break;
     begin();
     if (warp == 0 && ok) product(0, S, P);
     finish();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= mine) break;
+    if (mine) {
       float f[32];
-      take(0, h, 1.f / NS_SCALE, f);
+      take(0, 1.f / NS_SCALE, f);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) s[32 * h + j] = f[j];
-      os_put2(S, row, c0 + 32 * h, f);
+      for (int j = 0; j < 32; ++j) s[j] = f[j];
+      os_put2(S, row, c0, f);
     }
   }
   if (warp == 0 && !ok) mbar_wait_warp(bar, phase, nullptr, 0);       // the last products, before the tensor memory goes back
@@ -1774,7 +1767,7 @@ extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {
     static std::atomic<uint64_t> done[2];
     if (!allow_smem(kern, OS_SMEM, done[step])) return -20;
     for (int i = 0; i < a.groups; ++i) in.g[i].blocks = 1;
-    const int rc = launch_chained(kern, blocks(in), OS_THREADS, OS_SMEM, stream,
+    const int rc = launch_chained(kern, blocks(in), os_threads(l.d), OS_SMEM, stream,
                                   in, input, out, output, a.eps, a.steps);
     return rc ? rc : 1;
   }
