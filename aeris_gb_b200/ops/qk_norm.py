@@ -25,7 +25,7 @@ _INTEGERS = (torch.int32, torch.int64)
 
 
 def _like(t: torch.Tensor, shape, dtype, device) -> bool:
-    return t.shape == shape and t.dtype is dtype and t.device == device and t.stride(2) == 1
+    return t.shape == shape and t.dtype is dtype and t.device == device and (t.is_contiguous() or t.stride(2) == 1)
 
 
 def _apart(t: torch.Tensor) -> bool:
@@ -47,7 +47,7 @@ def _check_more(shape, dt, dev, *tensors) -> None:
 
 def _check_results(q_out, k_out, rows: int) -> None:
     for t in (q_out, k_out):
-        if t is not None and not _apart(t):
+        if t is not None and not t.is_contiguous() and not _apart(t):
             raise ValueError(f"elements of a result share addresses: {_text(t)}")
     if rows and q_out is not None and k_out is not None and q_out.data_ptr() == k_out.data_ptr():
         raise ValueError("the results of q and k are the same memory")
@@ -161,24 +161,28 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
     rows, heads, d = qs
     _check_more(qs, dt, dev, dq, dq_out)
     _check_more(ks, dt, dev, dk, dk_out)
-    _check_results(dq_out, dk_out, rows)
+    if dq_out is not None or dk_out is not None:
+        _check_results(dq_out, dk_out, rows)
     if add:
         _check_dw(dwq, dwk, d, dev)
     _l.require_cuda(q)
+    q_row, q_head, k_row, k_head = heads * d, d, ks[1] * d, d
     if dq_out is None:
         dq_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        q_row, q_head, _ = dq_out.stride()
     if dk_out is None:
         dk_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    else:
+        k_row, k_head, _ = dk_out.stride()
     if not add:
         make = torch.empty_like if rows else torch.zeros_like
         dwq, dwk = make(wq, dtype=torch.float32), make(wk, dtype=torch.float32)
     if rows:
         blocks = 4 * _multiprocessors(dev.index)
-        sums = torch.empty((blocks, d), dtype=torch.float32, device=dev)
+        sums = q.new_empty((blocks, d), dtype=torch.float32)
         dq_row, dq_head, _ = dq.stride()
         dk_row, dk_head, _ = dk.stride()
-        q_row, q_head, _ = dq_out.stride()
-        k_row, k_head, _ = dk_out.stride()
         record = _RECORD.pack(q.data_ptr(), q_at[0], q_at[1], k.data_ptr(), k_at[0], k_at[1], dq.data_ptr(), dq_row, dq_head,
                               dk.data_ptr(), dk_row, dk_head, dq_out.data_ptr(), q_row, q_head, dk_out.data_ptr(), k_row, k_head,
                               wq.data_ptr(), wk.data_ptr(), cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0,
