@@ -61,6 +61,11 @@ struct OrthoPlace {
   long long at;
   bool found, four;                           // four: rows are whole vectors of four
 };
+__device__ __forceinline__ long long ortho_size(const OrthoGroup& g) { return static_cast<long long>(g.rows) * g.cols; }
+// Whether a matrix at `at` lies inside the buffers. Any 64-bit offset may be asked about: nothing is added to it.
+__device__ __forceinline__ bool ortho_inside(const OrthoGroups& a, const OrthoGroup& g, long long at) {
+  return at >= 0 && at <= a.numel - ortho_size(g);
+}
 __device__ __forceinline__ OrthoPlace ortho_place(const OrthoGroups& a) {
   OrthoPlace p;
   int b = blockIdx.x;
@@ -74,25 +79,25 @@ __device__ __forceinline__ OrthoPlace ortho_place(const OrthoGroups& a) {
     p.at = p.matrix * g.stride;
   } else {
     p.at = g.offsets[p.matrix];
-    const long long size = static_cast<long long>(g.rows) * g.cols;
-    p.found = p.at >= 0 && p.at + size <= a.numel &&
-              ((p.matrix == 0 && !g.behind) || p.at >= g.offsets[p.matrix - 1] + size);
+    p.found = ortho_inside(a, g, p.at) &&
+              ((p.matrix == 0 && !g.behind) || g.offsets[p.matrix - 1] <= p.at - ortho_size(g));
     if (!p.found && threadIdx.x == 0) atomicCAS(a.status, 0, ERR_BOUNDS);
   }
   p.four = a.aligned && g.cols % 4 == 0 && g.ld % 4 == 0 && p.at % 4 == 0;
   return p;
 }
 
-// One warp: records a matrix of another group that shares elements with this one.
+// One warp: records a matrix of another group that shares elements with this one. One that lies outside is left out where its
+// own block finds that.
 __device__ __forceinline__ void ortho_apart(const OrthoGroups& a, const OrthoPlace& p) {
   if (!a.g[p.group].offsets || !p.found) return;
-  const long long end = p.at + static_cast<long long>(a.g[p.group].rows) * a.g[p.group].cols;
+  const long long end = p.at + ortho_size(a.g[p.group]);
   for (int h = 0; h < a.n; ++h) {
     const OrthoGroup& g = a.g[h];
     if (h == p.group) continue;
     for (int i = threadIdx.x & 31; i < g.count; i += 32) {
       const long long at = g.offsets[g.first + i];
-      if (at < end && at + static_cast<long long>(g.rows) * g.cols > p.at) atomicCAS(a.status, 0, ERR_BOUNDS);
+      if (ortho_inside(a, g, at) && at < end && at + ortho_size(g) > p.at) atomicCAS(a.status, 0, ERR_BOUNDS);
     }
   }
 }

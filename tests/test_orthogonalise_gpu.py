@@ -317,6 +317,32 @@ def test_offsets_outside_or_overlapping_are_reported_and_left(bad):
     assert torch.equal(b["master"][outside], fresh["master"][outside]) and torch.equal(b["weights"][outside], fresh["weights"][outside])
 
 
+@pytest.mark.parametrize("rows,cols", [(20, 30), (150, 160), (40, 700)])          # in one launch, in many, on the Gram matrix alone
+@pytest.mark.parametrize("back", [0, 1, 63, 64, "size", "behind"])
+def test_offsets_whose_ends_pass_64_bits_are_reported_and_left(rows, cols, back):
+    """A matrix that starts less than its size before 2^63, such as the largest integer for "no matrix": its end is no 64-bit
+    number."""
+    n, last = rows * cols, torch.iinfo(torch.int64).max
+    bad = last - (n if back == "size" else n + 1 if back == "behind" else back)
+    groups, at, b = flat([(rows, cols, 3)], gap=0)
+    off = torch.tensor([0, n, bad], device=DEV)
+    want = {k: v.clone() for k, v in b.items()}
+    OR.orthogonal_step(*(want[k] for k in ORDER), groups=[(rows, cols, off[:2])], **KW)
+    assert _l.status_word().item() == 0
+    for table in ([(rows, cols, off)], [(rows, cols, off[:2]), (cols, rows, off[2:])]):      # among its kind, as a group of its own
+        new = {k: v.clone() for k, v in b.items()}
+        OR.orthogonal_step(*(new[k] for k in ORDER), groups=table, **KW)
+        seen = _l.status_word().item()
+        _l.status_word().zero_()
+        assert seen == 6
+        for k in ("momentum", "grad"):
+            assert torch.equal(new[k], want[k]), k
+        for k in ("master", "weights", "ema"):               # the others of a failed call may have been updated or not
+            assert torch.equal(new[k][2 * n:], b[k][2 * n:]), k
+            for i in (slice(0, n), slice(n, 2 * n)):
+                assert torch.equal(new[k][i], b[k][i]) or torch.equal(new[k][i], want[k][i]), k
+
+
 @pytest.mark.parametrize("rows,cols", [(20, 30), (150, 160)])          # in one launch, in many
 def test_a_matrix_in_two_groups_is_reported(rows, cols):
     n = rows * cols
