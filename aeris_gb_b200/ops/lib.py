@@ -61,6 +61,57 @@ def on_device(device: torch.device):
     return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+def _pieces(t: torch.Tensor) -> tuple[int, int, list]:
+    """(first byte, bytes in one piece, [(how many, bytes apart), ..] from the inside out) of a tensor that is not empty."""
+    size = t.element_size()
+    width, dims = size, []
+    for step, n in sorted((st * size, n) for n, st in zip(t.shape, t.stride()) if n > 1 and st):
+        if not dims and step <= width:         # behind one another, or over one another
+            width += (n - 1) * step
+        elif dims and step == dims[-1][0] * dims[-1][1]:
+            dims[-1] = (dims[-1][0] * n, dims[-1][1])
+        else:
+            dims.append((n, step))
+    return t.data_ptr(), width, dims
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether ``a`` and ``b`` have a byte in common. Tensors that interleave, such as sections of one matrix's rows, do not. Exact
+    where both have one pitch at most and the same one, or the same outermost pitch; two that lie in one range of memory
+    otherwise count as sharing it."""
+    if not a.numel() or not b.numel():
+        return False
+    at, wa, da = _pieces(a)
+    to, wb, db = _pieces(b)
+    if at >= to + wb + sum((n - 1) * s for n, s in db) or to >= at + wa + sum((n - 1) * s for n, s in da):
+        return False
+    pitches = {d[-1][1] for d in (da, db) if d}
+    if len(pitches) != 1 or len(da) > 2 or len(db) > 2:
+        return True
+    pitch = pitches.pop()
+    na, nb = (d[-1][0] if d else 1 for d in (da, db))
+    (ma, sa), (mb, sb) = (d[0] if len(d) == 2 else (1, 0) for d in (da, db))
+    if sa == sb or mb == 1:
+        offsets = range((1 - mb) * sa, ma * sa, sa) if sa else (0,)
+    elif ma * mb <= 4096:
+        offsets = (i * sa - j * sb for i in range(ma) for j in range(mb))
+    else:
+        return True
+    for d in offsets:
+        # pieces r * pitch on in ``a`` and q * pitch on in ``b``, m = r - q: [d + m pitch, .. + wa) against [0, wb)
+        d += at - to
+        m = max((-wa - d) // pitch + 1, 1 - nb)
+        if m < na and d + m * pitch < wb:
+            return True
+    return False
+
+
+def same_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether every element of ``a`` lies where the same element of ``b`` does."""
+    return (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.dtype is b.dtype
+            and all(n < 2 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride())))
+
+
 _STATUS: dict[int, torch.Tensor] = {}
 
 

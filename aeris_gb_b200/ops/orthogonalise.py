@@ -106,6 +106,8 @@ def orthogonalise(x: torch.Tensor, *, steps: int = 5, eps: float = 1e-7, out: to
                 _pitched(o) and (o.shape[0] == 1 or o.stride(0) >= (o.shape[1] - 1) * _row_pitch(o) + o.shape[2]))):
             raise ValueError(f"out: bf16 {tuple(x.shape)} on {x.device} whose rows do not overlap, got {out.dtype} "
                              f"{tuple(out.shape)} on {out.device} with strides {out.stride()}")
+        if _l.share_memory(out, x):
+            raise ValueError("out shares memory with x")
     _l.require_cuda(x)
     if out is None:
         out = torch.empty_like(x, dtype=torch.bfloat16, memory_format=torch.contiguous_format)
@@ -186,6 +188,9 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
                         ("ema", ema, torch.float32)):
         if t is not None:
             _check_flat(name, t, master, dt)
+    parts = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (master, grad, momentum, weights, ema) if t is not None)
+    if any(a + n > b for (a, n), (b, _) in zip(parts, parts[1:])):
+        raise ValueError("the buffers of a step share memory")
     if norm_sq is not None and (norm_sq.numel() != 1 or norm_sq.dtype != torch.float64 or norm_sq.device != master.device):
         raise ValueError(f"norm_sq: one fp64 value on {master.device}, got {norm_sq.dtype} {tuple(norm_sq.shape)}")
     todo = []

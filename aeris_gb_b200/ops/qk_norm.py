@@ -45,12 +45,42 @@ def _check_more(shape, dt, dev, *tensors) -> None:
             raise ValueError(f"{dt} {tuple(shape)} on {dev} with channels side by side, got {_text(t)}")
 
 
-def _check_results(q_out, k_out, rows: int) -> None:
+def _share(a: tuple, b: tuple, rows: int, d: int, size: int) -> bool:
+    """:func:`.lib.share_memory` of (tensor [rows, heads, d], address, row pitch, head pitch, heads), without asking tensors again
+    where ranges of memory lie apart or rows are one piece each."""
+    t, at, row, head, heads = a
+    u, to, pitch, u_head, u_heads = b
+    if at >= to + ((rows - 1) * pitch + (u_heads - 1) * u_head + d) * size or to >= at + ((rows - 1) * row + (heads - 1) * head + d) * size:
+        return False
+    if row != pitch or row <= 0 or (head != d and heads > 1) or (u_head != d and u_heads > 1):
+        return _l.share_memory(t, u)
+    off, row = at - to, row * size
+    m = max((-heads * d * size - off) // row + 1, 1 - rows)
+    return m < rows and off + m * row < u_heads * d * size
+
+
+def _check_results(q_out, k_out, of_q: tuple, of_k: tuple, rows: int, d: int) -> None:
+    """``of_q``, ``of_k``: inputs of q's and k's kernels. Either result may take the place of one of its own. One that lies over
+    the other's, or beside an input's elements, would be written while other warps read there."""
     for t in (q_out, k_out):
         if t is not None and not t.is_contiguous() and not _apart(t):
             raise ValueError(f"elements of a result share addresses: {_text(t)}")
-    if rows and q_out is not None and k_out is not None and q_out.data_ptr() == k_out.data_ptr():
-        raise ValueError("the results of q and k are the same memory")
+    if not rows:
+        return
+    size = of_q[0].element_size()
+    places = [[(t, t.data_ptr(), *t.stride()[:2], heads) for t in ts if t is not None]
+              for heads, ts in ((of_q[0].shape[1], (q_out, *of_q)), (of_k[0].shape[1], (k_out, *of_k)))]
+    for t, mine, others in ((q_out, *places), (k_out, *places[::-1])):
+        if t is None:
+            continue
+        for b in others[-len(of_q):]:
+            if _share(mine[0], b, rows, d, size):
+                raise ValueError(f"a result of q lies over k or one of k over q: {_text(t)}, {_text(b[0])}")
+        for b in mine[1:]:
+            if t is not b[0] and _share(mine[0], b, rows, d, size) and not _l.same_memory(t, b[0]):
+                raise ValueError(f"a result lies beside its input's elements: {_text(t)}, {_text(b[0])}")
+    if q_out is not None and k_out is not None and _share(places[0][0], places[1][0], rows, d, size):
+        raise ValueError("the results of q and k are in the same memory")
 
 
 def _check_dw(dwq, dwk, d: int, dev) -> None:
@@ -118,13 +148,14 @@ def qk_norm_fwd(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor, wk: torch.Te
     """``q`` [rows, heads, d] and ``k`` [rows, kv_heads, d], bf16 or fp32, with any strides between rows and heads (sections of
     a fused qkv matrix): normed by head with the weights ``wq``, ``wk`` [d] and, with ``cos`` / ``sin``, turned. ``positions``
     [rows] int32 or int64: the table row of every row; one outside the table sets the status word and its row is not written.
-    ``q_out``, ``k_out``: where to put the results, memory of their own or ``q`` and ``k`` themselves."""
+    ``q_out``, ``k_out``: where to put the results, memory of their own or ``q`` and ``k`` themselves; results that lie over
+    anything else of them are refused."""
     qs, ks, q_at, k_at, dt, dev, length, rot = _check(q, k, wq, wk, cos, sin, positions)
     rows, heads, d = qs
     if q_out is not None or k_out is not None:
         _check_more(qs, dt, dev, q_out)
         _check_more(ks, dt, dev, k_out)
-        _check_results(q_out, k_out, rows)
+        _check_results(q_out, k_out, (q,), (k,), rows, d)
     _l.require_cuda(q)
     q_row, q_head, k_row, k_head = heads * d, d, ks[1] * d, d
     if q_out is None:
@@ -151,9 +182,9 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
                 positions: torch.Tensor | None = None, dq_out: torch.Tensor | None = None, dk_out: torch.Tensor | None = None,
                 dwq: torch.Tensor | None = None, dwk: torch.Tensor | None = None):
     """Gradients of :func:`qk_norm_fwd` for ``dq``, ``dk`` with respect to its results; ``q``, ``k`` are its inputs. Returns
-    (gradients of q and k, which may overwrite ``dq`` and ``dk``, and fp32 gradients of the weights). ``dwq``, ``dwk`` [d] fp32
-    are added to where given, and may be one tensor, of a weight that q and k share. A row whose position lies outside the table
-    adds nothing, and its gradients are not written. The same bits on every run."""
+    (gradients of q and k, which may overwrite ``dq`` and ``dk`` element by element, and fp32 gradients of the weights). ``dwq``,
+    ``dwk`` [d] fp32 are added to where given, and may be one tensor, of a weight that q and k share. A row whose position lies
+    outside the table adds nothing, and its gradients are not written. The same bits on every run."""
     add = dwq is not None
     if add != (dwk is not None):
         raise ValueError("dwq and dwk come together")
@@ -162,7 +193,7 @@ def qk_norm_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Te
     _check_more(qs, dt, dev, dq, dq_out)
     _check_more(ks, dt, dev, dk, dk_out)
     if dq_out is not None or dk_out is not None:
-        _check_results(dq_out, dk_out, rows)
+        _check_results(dq_out, dk_out, (dq, q), (dk, k), rows, d)
     if add:
         _check_dw(dwq, dwk, d, dev)
     _l.require_cuda(q)

@@ -56,3 +56,27 @@ def test_step_refuses(bad):
                                                 ((0, 2 ** 40, 1), (2, 1, 8), True), ((0, 9, 5), (2, 4, 1), True)])
 def test_pitches_that_the_kernels_count(strides, shape, fine):
     assert OR._pitched(torch.empty(1, device="meta").as_strided(shape, strides)) == fine
+
+
+def test_results_over_the_input_are_refused():
+    x = torch.randn(3, 4, 8).bfloat16()
+    wide = torch.zeros(3, 4, 16).bfloat16()
+    for inp, out, fine in ((x, x, False), (x, x.clone(), True), (x, x[:1].clone().expand(3, 4, 8), False),
+                           (wide[:, :, :8], wide[:, :, 8:], True), (wide[:, :, :8], wide[:, :, 4:12], False),
+                           (wide[:2, :, :8], wide[1:, :, :8], False), (wide[:1, :, :8], wide[1:2, :, :8], True),
+                           (torch.randn(4, 8), torch.empty(4, 8).bfloat16(), True)):
+        with pytest.raises(ValueError) as e:
+            OR.orthogonalise(inp, out=out)
+        assert ("on a GPU" in str(e.value)) == fine, e.value
+
+
+@pytest.mark.parametrize("a,b", [("master", "grad"), ("grad", "momentum"), ("master", "ema"), ("ema", "momentum")])
+@pytest.mark.parametrize("by", [0, 4, N - 4])
+def test_buffers_of_a_step_that_share_memory_are_refused(a, b, by):
+    whole = torch.zeros(2 * N)
+    with pytest.raises(ValueError, match="share memory"):
+        step(**{a: whole[:N], b: whole[by:by + N]})
+    with pytest.raises(ValueError, match="share memory"):
+        step(**{a: whole[:N], "weights": whole[by:by + N].view(torch.bfloat16)[:N]})
+    with pytest.raises(ValueError, match="on a GPU"):
+        step(**{a: whole[:N], b: whole[N:]})

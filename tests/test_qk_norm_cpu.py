@@ -86,3 +86,88 @@ def test_backward_refuses(bad):
 def test_overlap_of_results(shape, strides, fine):
     t = torch.empty(1000).as_strided(shape, strides)
     assert QN._apart(t) == fine
+
+
+def sections(pitch, q_at, k_at):
+    """q [ROWS, H, D] and k [ROWS, HK, D] out of one matrix's rows, from those elements of a row on."""
+    m = torch.zeros(ROWS, pitch)
+    return m[:, q_at:q_at + H * D].unflatten(1, (H, D)), m[:, k_at:k_at + HK * D].unflatten(1, (HK, D))
+
+
+def placements():
+    """(whether the call is taken, q, k, q_out, k_out)"""
+    q, k = torch.randn(ROWS, H, D), torch.randn(ROWS, HK, D)
+    s, t = sections((H + HK) * D, 0, H * D), sections((H + HK) * D, 0, (H - 1) * D)
+    one = torch.zeros(ROWS, 2, HK, 3, D)                  # q, k and v of every head side by side, of two groups of heads
+    first, second = one[:, 0, :, 0], one[:, 0, :, 1]
+    long = torch.randn((ROWS + 1) * H * D)
+    rows = long[:-H * D].view(ROWS, H, D)
+    back = torch.zeros(H, ROWS, D).transpose(0, 1)        # rows inside heads
+    return {
+        "sections": (True, q, k, *s),
+        "in place": (True, q, k, q, k),
+        "sections in place": (True, *s, *s),
+        "q alone in place": (True, *s, s[0], None),
+        "head by head": (True, q[:, :HK], k, first, second),
+        "head by head in place": (True, first, second, first, second),
+        "rows inside heads, in place": (True, back, k, back, k),
+        "q over k": (False, q, q[:, :HK], q, None),
+        "k over q": (False, q, k, None, q[:, :HK]),
+        "k over q's last heads": (False, q, k, None, q[:, H - HK:]),
+        "q and k changed over": (False, first, second, second, first),
+        "results over each other": (False, q, k, *t),
+        "results in one place": (False, q[:, :HK], k, first, first),
+        "a row behind the input": (False, rows, k, long[H * D:].view(ROWS, H, D), None),
+        "a channel behind the input": (False, rows, k, long[1:1 + ROWS * H * D].view(ROWS, H, D), None),
+        "over the input in another order": (False, rows, k, long[:-H * D].view(H, ROWS, D).transpose(0, 1), None),
+    }
+
+
+@pytest.mark.parametrize("what", placements())
+def test_results_over_another_one_s_elements_are_refused(what):
+    """Blocks of q and blocks of k run at the same time. What is taken here goes on to ask for a GPU."""
+    fine, q, k, q_out, k_out = placements()[what]
+    with pytest.raises(ValueError) as e:
+        forward(args(q=q, k=k, q_out=q_out, k_out=k_out))
+    assert ("on a GPU" in str(e.value)) == fine, e.value
+    a = args()
+    # the gradients of q and k over those of the results
+    with pytest.raises(ValueError) as e:
+        QN.qk_norm_bwd(q, k, torch.randn(q.shape), torch.randn(k.shape), a["wq"], a["wk"], a["cos"], a["sin"], eps=1e-6,
+                       dq_out=q_out, dk_out=k_out)
+    assert ("on a GPU" in str(e.value)) == fine, e.value
+    # and over the inputs themselves
+    with pytest.raises(ValueError) as e:
+        QN.qk_norm_bwd(torch.randn(q.shape), torch.randn(k.shape), q, k, a["wq"], a["wk"], a["cos"], a["sin"], eps=1e-6,
+                       dq_out=q_out, dk_out=k_out)
+    assert ("on a GPU" in str(e.value)) == fine, e.value
+
+
+def test_shared_memory_against_every_byte():
+    """What is said to be apart is apart; sections and whole tensors are told apart exactly."""
+    import random
+    from aeris_gb_b200.ops import lib as L
+    rnd, base = random.Random(1), torch.empty(400, dtype=torch.uint8)
+
+    def one(d, rows):
+        heads = rnd.randint(1, 3)
+        head = d * rnd.choice([1, 1, 1, 2, 0])
+        return base.as_strided((rows, heads, d), (rnd.choice([heads * head, 24, 24, d, 0]), head, 1), rnd.randint(0, 60))
+
+    def places(t):
+        (r, h, d), (a, b, _), o = t.shape, t.stride(), t.storage_offset()
+        return {o + i * a + j * b + k for i in range(r) for j in range(h) for k in range(d)}
+
+    met = exact = 0
+    for _ in range(20000):
+        d, rows = rnd.choice([2, 4, 6]), rnd.randint(1, 4)
+        a, b = one(d, rows), one(d, rows)
+        want, got = bool(places(a) & places(b)), L.share_memory(a, b)
+        met += want
+        assert got or not want
+        if rows > 1 and a.stride(0) == b.stride(0) == 24 and all(t.shape[1] == 1 or t.stride(1) == d for t in (a, b)):
+            assert got == want
+            exact += 1
+        wa, wb = ((t, t.data_ptr(), *t.stride()[:2], t.shape[1]) for t in (a, b))
+        assert QN._share(wa, wb, rows, d, 1) == got
+    assert 1000 < met < 19000 and exact > 100
