@@ -185,6 +185,31 @@ __device__ __forceinline__ int table_row(const AerisQkNorm& a, int row) {
 struct Angles {
   uint64_t c[2], s[2];                        // of pairs 0 and 1, of pairs 2 and 3
 };
+// Which of the lane's pairs are turned, a bit each.
+template <int W> __device__ __forceinline__ int turned_pairs(const AerisQkNorm& a, const Lane& l) {
+  int bits = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bits |= (pair_channel<W>(l, j) < a.rot) << j;
+  return bits;
+}
+// The pairs turned by their angles, back with BACK. A pair that is not turned has no part in it, not even times zero: an
+// infinity or NaN in one of its channels is none in the other.
+template <bool BACK> __device__ __forceinline__ void turn_pair(uint64_t& e, uint64_t& o, uint64_t c, uint64_t s, uint64_t mask) {
+  const uint64_t x = f2_mul(o & mask, s), y = f2_mul(e & mask, s);
+  e = f2_fma(e, c, BACK ? x : f2_neg(x));
+  o = f2_fma(o, c, BACK ? f2_neg(y) : y);
+}
+// TURN: how much of a head is turned, 0 nothing, 1 a part, 2 all of it. A kernel of its own for each: the branch or the masks of the
+// second cost it 6 % (24 + 24 heads of 64, 32 channels turned, bf16: forward 132 us without them, 140; by masks alone 140 too,
+// backward 200, 209, 212), and asked for in heads that are turned as a whole they cost the backward pass as much.
+template <int W, int TURN, bool BACK> __device__ __forceinline__ void turn(Eight& v, const Angles& r, int turned) {
+  if (!TURN || (TURN == 1 && W == 8 && !turned)) return;              // by eights a lane turns all its pairs or none
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    turn_pair<BACK>(v.e[k], v.o[k], r.c[k], r.s[k],
+                    TURN == 2 || W == 8 ? ~uint64_t(0)
+                                        : (turned >> (2 * k) & 1 ? 0xffffffffull : 0) | (turned >> (2 * k) & 2 ? 0xffffffff00000000ull : 0));
+}
 template <int W, bool PAIRS> __device__ __forceinline__ Angles load_angles(const AerisQkNorm& a, int row, const Lane& l) {
   const long long at = row;
   float c[4], s[4];
@@ -283,7 +308,7 @@ template <bool ODD, int N> __device__ __forceinline__ void group_sums(float (&v)
 // Blocks an SM of the forward kernel; fp32 by fours needs more registers for the heads in flight.
 template <typename T, int W> constexpr int fwd_blocks() { return W == 0 ? 2 : W == 4 && sizeof(T) == 4 ? 3 : 4; }
 
-template <typename T, int W, bool ODD>
+template <typename T, int W, bool ODD, int TURN>
 __global__ void __launch_bounds__(QKN_THREADS, fwd_blocks<T, W>()) qk_norm_fwd_kernel(const AerisQkNorm a, const QkCut cut) {
   constexpr int U = W ? 3 : 2;                // heads in flight per lane
   const Part t = Part::make<W>(a, cut);
@@ -293,6 +318,7 @@ __global__ void __launch_bounds__(QKN_THREADS, fwd_blocks<T, W>()) qk_norm_fwd_k
   const float inv_d = 1.f / a.d;
   chain_point();
   const Eight w = load_weight<W>(t.is_k ? a.wk : a.wq, a.w_bf16, t.lane);
+  const int turned = TURN == 1 ? turned_pairs<W>(a, t.lane) : 0;
   for (int row = t.row; row - t.row_sub < a.rows; row += t.stride, x_row += t.stride * in.row, y_row += t.stride * out.row) {
     const int at = table_row(a, row);         // nothing but the angles waits for it
     const int heads = row < a.rows ? t.heads : 0;
@@ -316,10 +342,10 @@ __global__ void __launch_bounds__(QKN_THREADS, fwd_blocks<T, W>()) qk_norm_fwd_k
         const uint64_t scale = f2_all(rsqrtf(sum[0] * inv_d + a.eps));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint64_t e = f2_mul(f2_mul(v.e[k], scale), w.e[k]), o = f2_mul(f2_mul(v.o[k], scale), w.o[k]);
-          v.e[k] = f2_fma(e, r.c[k], f2_neg(f2_mul(o, r.s[k])));
-          v.o[k] = f2_fma(o, r.c[k], f2_mul(e, r.s[k]));
+          v.e[k] = f2_mul(f2_mul(v.e[k], scale), w.e[k]);
+          v.o[k] = f2_mul(f2_mul(v.o[k], scale), w.o[k]);
         }
+        turn<W, TURN, false>(v, r, turned);
         HeadRaw<T, W>::store(y + u * (cut.per_step * out.head), at >= 0 && (step + u) * cut.per_step < heads, t.lane, v);
       }
       y += U * (cut.per_step * out.head);
@@ -329,20 +355,17 @@ __global__ void __launch_bounds__(QKN_THREADS, fwd_blocks<T, W>()) qk_norm_fwd_k
 
 // One head's gradient in a lane: v = x and g = dy on entry; dw is added to, g holds dx on return. Not `live`: a place without a
 // head, all zeros, whose root without eps would be infinite.
-template <bool ODD>
-__device__ __forceinline__ void head_backward(const Eight& v, Eight& g, const Eight& w, const Angles& r, Eight& dw, int i,
+template <int W, bool ODD, int TURN>
+__device__ __forceinline__ void head_backward(const Eight& v, Eight& g, const Eight& w, const Angles& r, int turned, Eight& dw, int i,
                                               const QkCut& cut, bool live, float inv_d, float eps) {
   uint64_t ss2 = 0, dot2 = 0;                 // two zeros
   Eight gw;
+  turn<W, TURN, true>(g, r, turned);
   // mean(g x r) needs no r before its sum: both sums go through the shuffles together
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const uint64_t e = f2_fma(g.e[k], r.c[k], f2_mul(g.o[k], r.s[k]));
-    const uint64_t o = f2_fma(g.o[k], r.c[k], f2_neg(f2_mul(g.e[k], r.s[k])));
-    g.e[k] = e;
-    g.o[k] = o;
-    gw.e[k] = f2_mul(e, w.e[k]);
-    gw.o[k] = f2_mul(o, w.o[k]);
+    gw.e[k] = f2_mul(g.e[k], w.e[k]);
+    gw.o[k] = f2_mul(g.o[k], w.o[k]);
     ss2 = f2_fma(v.o[k], v.o[k], f2_fma(v.e[k], v.e[k], ss2));
     dot2 = f2_fma(gw.o[k], v.o[k], f2_fma(gw.e[k], v.e[k], dot2));
   }
@@ -384,7 +407,7 @@ __device__ __forceinline__ void block_sums(float (*red)[QKN_MAX_D], const Eight&
 }
 
 // Any even width, any alignment.
-template <typename T>
+template <typename T, int TURN>
 __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_kernel(const AerisQkNorm a, const QkCut cut) {
   __shared__ float red[QKN_WARPS][QKN_MAX_D];
   const Part t = Part::make<0>(a, cut);
@@ -394,6 +417,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_kernel(const Aeris
   const float inv_d = 1.f / a.d;
   chain_point();
   const Eight w = load_weight<0>(t.is_k ? a.wk : a.wq, a.w_bf16, t.lane);
+  const int turned = TURN == 1 ? turned_pairs<0>(a, t.lane) : 0;
   Eight dw = {};
   for (int row = t.row; row < a.rows; row += t.stride, x += t.stride * in.row, dy += t.stride * grad.row, dx += t.stride * out.row) {
     const int at = table_row(a, row);
@@ -405,7 +429,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_kernel(const Aeris
       rx.load(x + step * in.head, true, t.lane);
       rg.load(dy + step * grad.head, true, t.lane);
       Eight g = rg.get();
-      head_backward<false>(rx.get(), g, w, r, dw, t.lane.i, cut, true, inv_d, a.eps);
+      head_backward<0, false, TURN>(rx.get(), g, w, r, turned, dw, t.lane.i, cut, true, inv_d, a.eps);
       HeadRaw<T, 0>::store(dx + step * out.head, true, t.lane, g);
     }
   }
@@ -416,7 +440,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_kernel(const Aeris
 // of 16 bytes that the same lane takes out again): with the loads in registers, two steps at a time, 127 registers left 16
 // warps per SM too little under way (64,800 rows, 24 + 24 heads of 64: 265 us; ring 247, with two-wide arithmetic 212 to 217;
 // three blocks an SM instead of two 217 where that took 212).
-template <typename T, int W, bool ODD>
+template <typename T, int W, bool ODD, int TURN>
 __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_ring_kernel(const AerisQkNorm a, const QkCut cut) {
   constexpr int VECS = W == 8 ? 1 : 2, BYTES = W * sizeof(T);         // copies a head and lane, and their size
   constexpr int AHEAD = VECS * BYTES == 16 ? 4 : 3;                   // stages of the ring
@@ -432,6 +456,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_ring_kernel(const 
   uint4 (*ring)[2][VECS][2 * BYTES] = sm.ring[threadIdx.x >> 5];
   chain_point();
   const Eight w = load_weight<W>(t.is_k ? a.wk : a.wq, a.w_bf16, t.lane);
+  const int turned = TURN == 1 ? turned_pairs<W>(a, t.lane) : 0;
   Eight dw = {};
   const long long in_step = cut.per_step * in.head, grad_step = cut.per_step * grad.head, out_step = cut.per_step * out.head;
   int ahead_row = t.row, ahead_step = 0;
@@ -484,7 +509,7 @@ __global__ void __launch_bounds__(QKN_THREADS, 2) qk_norm_bwd_ring_kernel(const 
       rg.load(slot + 32 * VECS * W, mine, in_ring);
       Eight g = rg.get();
       // lanes behind the head's width hold zeros and have their head's root
-      head_backward<ODD>(rx.get(), g, w, r, dw, t.lane.i, cut, mine, inv_d, a.eps);
+      head_backward<W, ODD, TURN>(rx.get(), g, w, r, turned, dw, t.lane.i, cut, mine, inv_d, a.eps);
       HeadRaw<T, W>::store(dx, mine, t.lane, g);
       from = next(from);
     }
@@ -582,7 +607,10 @@ QkCut cut_of(const AerisQkNorm& a, int width, int blocks_per_sm, double own, int
   return c;
 }
 
-template <int W> using Width = std::integral_constant<int, W>;
+template <int N> using Int = std::integral_constant<int, N>;
+template <typename F> auto by_turn(const AerisQkNorm& a, F f) {
+  return !a.rot ? f(Int<0>{}) : a.rot < a.d ? f(Int<1>{}) : f(Int<2>{});
+}
 
 int refused(const AerisQkNorm& a) {
   if (a.rows <= 0 || a.rows > 0x7fffffff - (1 << 20) || a.heads <= 0 || a.kv_heads <= 0 || a.d <= 0 || a.d % 2 || a.d > QKN_MAX_D) return -1;
@@ -602,13 +630,19 @@ extern "C" int aeris_qk_norm_fwd(const AerisQkNorm* p, void* stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const int w = width_of(a, false);
   const QkCut c = cut_of(a, w, !w ? 2 : a.f32 && w == 4 ? 3 : 4, 2, 1 << 30);
-  auto groups = [&](auto t, auto width) {
-    return odd(a.d) ? qk_norm_fwd_kernel<decltype(t), decltype(width)::value, true>
-                    : qk_norm_fwd_kernel<decltype(t), decltype(width)::value, false>;
-  };
   using bf16 = __nv_bfloat16;
-  auto kern = a.f32 ? (w == 8 ? groups(0.f, Width<8>{}) : w ? groups(0.f, Width<4>{}) : qk_norm_fwd_kernel<float, 0, false>)
-                    : (w == 8 ? groups(bf16(), Width<8>{}) : w ? groups(bf16(), Width<4>{}) : qk_norm_fwd_kernel<bf16, 0, false>);
+  auto pick = [&](auto t, auto width, auto turn) {
+    constexpr int W = decltype(width)::value, TURN = decltype(turn)::value;
+    using T = decltype(t);
+    return W && odd(a.d) ? qk_norm_fwd_kernel<T, W, W != 0, TURN> : qk_norm_fwd_kernel<T, W, false, TURN>;
+  };
+  auto by_width = [&](auto t, auto turn) {
+    return w == 8 ? pick(t, Int<8>{}, turn) : w ? pick(t, Int<4>{}, turn) : pick(t, Int<0>{}, turn);
+  };
+  auto by_type = [&](auto turn) { return a.f32 ? by_width(0.f, turn) : by_width(bf16(), turn); };
+  // Heads by eights of which nothing is turned go through the kernel with the branch: 65,000 rows of 24 + 24 heads of 64 take 127 us
+  // there and 146 without it, where all of a step's stores come at once.
+  auto kern = w == 8 && !a.rot ? by_type(Int<1>{}) : by_turn(a, by_type);
   return launch_chained(kern, c.q_blocks + c.k_blocks, QKN_THREADS, 0, stream, a, c);
 }
 
@@ -621,13 +655,17 @@ extern "C" int aeris_qk_norm_bwd(const AerisQkNorm* p, void* stream_) {
   const int w = width_of(a, true);
   const QkCut c = cut_of(a, w, 2, 1, a.sum_rows);
   if (c.q_blocks + c.k_blocks > a.sum_rows) return -5;
-  auto ring = [&](auto t, auto width) {
-    return odd(a.d) ? qk_norm_bwd_ring_kernel<decltype(t), decltype(width)::value, true>
-                    : qk_norm_bwd_ring_kernel<decltype(t), decltype(width)::value, false>;
-  };
   using bf16 = __nv_bfloat16;
-  auto kern = a.f32 ? (w ? ring(0.f, Width<4>{}) : qk_norm_bwd_kernel<float>)
-                    : (w == 8 ? ring(bf16(), Width<8>{}) : w ? ring(bf16(), Width<4>{}) : qk_norm_bwd_kernel<bf16>);
+  auto ring = [&](auto t, auto width, auto turn) {
+    constexpr int W = decltype(width)::value, TURN = decltype(turn)::value;
+    using T = decltype(t);
+    return odd(a.d) ? qk_norm_bwd_ring_kernel<T, W, true, TURN> : qk_norm_bwd_ring_kernel<T, W, false, TURN>;
+  };
+  auto kern = by_turn(a, [&](auto turn) {
+    constexpr int TURN = decltype(turn)::value;
+    return a.f32 ? (w ? ring(0.f, Int<4>{}, turn) : qk_norm_bwd_kernel<float, TURN>)
+                 : (w == 8 ? ring(bf16(), Int<8>{}, turn) : w ? ring(bf16(), Int<4>{}, turn) : qk_norm_bwd_kernel<bf16, TURN>);
+  });
   if (const int rc = launch_chained(kern, c.q_blocks + c.k_blocks, QKN_THREADS, 0, stream, a, c)) return rc;
   const bool shared = a.dwq == a.dwk;
   if (const int rc = launch_chained(qk_norm_sums_kernel, dim3((a.d + 31) / 32, shared ? 1 : 2), 1024, 0, stream, a.sums,

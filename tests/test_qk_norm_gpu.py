@@ -191,6 +191,39 @@ def test_one_row_of_nan_stays_one_row(dt):
     assert torch.equal(got, want)
 
 
+def same_or_close(got, want, size, dt, roundings=16):
+    """:func:`close` where ``want`` is a number; elsewhere the same infinity, or no number in both."""
+    ok = want.isfinite() & size.isfinite()
+    got = got.double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[want.isinf()], want[want.isinf()])
+    close(got[ok], want[ok], size[ok], dt, roundings)
+
+
+@pytest.mark.parametrize("d,rot,dt", [(64, 32, torch.bfloat16), (64, 0, torch.bfloat16), (72, 40, torch.bfloat16), (36, 18, torch.bfloat16),
+                                      (100, 50, torch.bfloat16), (80, 78, torch.bfloat16), (254, 100, torch.bfloat16),
+                                      (64, 32, torch.float32), (36, 18, torch.float32), (20, 2, torch.float32), (30, 14, torch.float32)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_a_channel_that_is_not_turned_leaves_its_neighbour_alone(d, rot, dt, value):
+    """Infinities and NaN in the weights, in q and in the results' gradient, in channels behind the turned ones."""
+    rows = 9
+    q, k, dq, dk, wq, wk, cos, sin, _, at = make(rows, 3, 2, d, rot, rows, dt, layout="own")
+    for what in ("weight", "q", "dq"):
+        for c in {rot, rot + 1, d - 1}:
+            x, w, dy = q.clone(), wq.clone(), dq.clone()
+            if what == "weight":
+                w[c] = value
+            else:
+                (x if what == "q" else dy)[4, 1, c] = value
+            y, _ = QN.qk_norm_fwd(x, k, w, wk, cos, sin, eps=1e-6)
+            same_or_close(y, *formula(x, w, cos, sin, at, 1e-6), dt)
+            if what == "q":                      # the root is zero or no number: nothing of this head's gradient is left
+                continue
+            dx, _, dw, _ = QN.qk_norm_bwd(dy, dk, x, k, w, wk, cos, sin, eps=1e-6)
+            ex, size, ew, wsize = formula(x, w, cos, sin, at, 1e-6, dy)
+            same_or_close(dx, ex, size, dt)
+            same_or_close(dw, ew, wsize, torch.float32, 16 + 3 * rows)
+
+
 @pytest.mark.parametrize("d", [64, 36])
 def test_in_place_and_into_sections(d):
     """Results over the inputs, and into sections of one matrix whose rest is left as it was."""
