@@ -114,13 +114,17 @@ def _read_optim_state(osd: dict, names: list[str]) -> tuple[int, dict, dict]:
     return step, m, v
 
 
-def check_methods(opt, exp_avg: dict, exp_avg_sq: dict) -> None:
+def _momentum_only(opt) -> set[str]:
+    return opt.momentum_only() if hasattr(opt, "momentum_only") else set()
+
+
+def check_methods(opt, momentum_only, exp_avg_sq) -> None:
     """Raises before anything is touched where the state is not of ``opt``'s kind: matrices with orthogonalised updates have a
-    momentum alone, without second moments AdamW would divide by nothing, and its first moments have another scale."""
-    alone = opt.momentum_only() if hasattr(opt, "momentum_only") else set()
-    for n in exp_avg:
-        if (n in exp_avg_sq) == (n in alone):
-            raise ValueError(f"optimizer state of {n} was written with another method than {opt.cfg.method!r}")
+    momentum alone (``momentum_only``: those that the state was written with), without second moments AdamW would divide by
+    nothing, and its first moments have another scale."""
+    alone = _momentum_only(opt)
+    for n in sorted((set(momentum_only) - alone) | (alone & set(exp_avg_sq))):
+        raise ValueError(f"optimizer state of {n} was written with another method than {opt.cfg.method!r}")
 
 
 def _stage_param_names(module) -> dict[int, list[str]]:
@@ -191,7 +195,7 @@ def load_stage_checkpoint(directory: str | None, module, opt, device) -> bool:
     if not directory:
         return False
     loaded = {}
-    names = _stage_param_names(module)
+    names, alone = _stage_param_names(module), _momentum_only(opt)
     model_sd, master, ema, m, v = {}, {}, {}, {}, {}
     step = 0
     for stage in _stage_ids(module):
@@ -203,6 +207,8 @@ def load_stage_checkpoint(directory: str | None, module, opt, device) -> bool:
                     if not (abs(now.get(k, float("nan")) - val) <= 1e-9 * max(1.0, abs(val))):
                         raise ValueError(f"checkpoint payload damaged: {k}")
             st_step, st_m, st_v = _read_optim_state(ck["optimizer_state_dict"], names.get(stage, []))
+            if st_m and not st_v and not alone:
+                raise ValueError("optimizer_state_dict holds no second moments")
             for k, t in ck["model_state_dict"].items():
                 model_sd[_key_for(module, stage, k)] = t
             for k, t in ck["main_model_state_dict"].items():
@@ -220,7 +226,7 @@ def load_stage_checkpoint(directory: str | None, module, opt, device) -> bool:
             logging.getLogger(__name__).warning("checkpoint of stage %d in %s not loaded: %s", stage, directory, e)
             return False
     first = next(iter(loaded.values()))
-    check_methods(opt, m, v)
+    check_methods(opt, set(m) - set(v), v)
     # parameters are views of the optimizer's flat buffers, so loading the masters refreshes the model copies too;
     # buffers and frozen parameters come from the model state dict
     own = module.state_dict()

@@ -298,18 +298,22 @@ class FlatOptimizer:
         return self._named_views("ema")
 
     def state_dict(self) -> dict:
+        alone = sorted(self.momentum_only())
         return {"step": self.step_count, "cur_nimg": self.cur_nimg,
                 "exp_avg": {k: v.clone() for k, v in self._named_views("m").items()},
-                "exp_avg_sq": {k: v.clone() for k, v in self._named_views("v").items()}}
+                "exp_avg_sq": {k: v.clone() for k, v in self._named_views("v").items()},
+                **({"momentum_only": alone} if alone else {})}
 
     def momentum_only(self) -> set[str]:
         """Parameters whose state is a momentum without second moments."""
         return {n for s in self.segments if s.groups is not None for n in s.names}
 
     def load_state_dict(self, sd: dict, master: dict | None = None, ema: dict | None = None):
+        """What ``sd`` (moments as ``None`` or of some parameters alone too), ``master`` and ``ema`` hold; the rest is left as it is.
+        A state of another method (``momentum_only``) is refused."""
         from .checkpoint import check_methods
-        check_methods(self, {n: t for s in self.segments for n in s.names if (t := sd["exp_avg"].get(n)) is not None},
-                      sd["exp_avg_sq"])
+        mine = {n for s in self.segments for n in s.names}
+        check_methods(self, mine & set(sd.get("momentum_only", ())), sd["exp_avg_sq"] or ())
         self.step_count, self.cur_nimg = sd["step"], sd["cur_nimg"]
         for which, src in (("m", sd["exp_avg"]), ("v", sd["exp_avg_sq"]), ("master", master), ("ema", ema)):
             if src is None:

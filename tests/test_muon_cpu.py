@@ -137,6 +137,53 @@ def test_state_goes_through_a_checkpoint_and_other_methods_are_refused(tmp_path)
         opt2.load_state_dict(adam.state_dict())
 
 
+@pytest.mark.parametrize("method", ["adamw", "muon"])
+def test_states_in_part_are_loaded_in_part(method):
+    """Moments that are not there are left as they are; a momentum without second moments is refused by AdamW alone."""
+    m, other = model(), model(seed=3)
+    opt, src = optim(m, method=method), optim(other, method=method)
+    for s in src.segments:
+        s.m.normal_()
+        if s.v is not None:
+            s.v.uniform_()
+    src.step_count, src.cur_nimg = 3, 7
+    sd = src.state_dict()
+    clone = lambda: {k: {n: t.clone() for n, t in opt._named_views(k).items()} for k in "mv"}  # noqa: E731
+    for first, second in ((None, None), (None, sd["exp_avg_sq"]), (sd["exp_avg"], None), (sd["exp_avg"], {}),
+                          ({}, sd["exp_avg_sq"]), (dict(list(sd["exp_avg"].items())[:2]), sd["exp_avg_sq"])):
+        before = clone()
+        opt.load_state_dict({**sd, "exp_avg": first, "exp_avg_sq": second})
+        after = clone()
+        for k, given in (("m", first), ("v", second)):
+            for n, t in after[k].items():
+                assert torch.equal(t, (given if given and n in given else before[k])[n]), (k, n)
+        assert (opt.step_count, opt.cur_nimg) == (3, 7)
+        for s in opt.segments:
+            s.m.zero_()
+
+
+def test_a_momentum_alone_is_refused_by_adamw_and_untouched():
+    muon, adam = optim(model()), optim(model(), method="adamw")
+    muon.step_count = 5
+    for s in muon.segments:
+        s.m.normal_()
+    with pytest.raises(ValueError, match="another method"):
+        adam.load_state_dict(muon.state_dict())
+    assert adam.step_count == 0 and all(float(s.m.abs().max()) == 0 for s in adam.segments)
+
+
+def test_a_file_without_any_second_moments_is_not_loaded(tmp_path):
+    m = model()
+    opt = optim(m, method="adamw")
+    path, = CK.save_stage_checkpoint(str(tmp_path), m, opt)[:1]
+    file = torch.load(path, weights_only=True)
+    for st in file["optimizer_state_dict"]["state"].values():
+        del st["exp_avg_sq"]
+    file.pop("integrity")
+    torch.save(file, path)
+    assert CK.load_stage_checkpoint(str(tmp_path), m, opt, "cpu") is False
+
+
 def test_unknown_method_and_optimizers_that_cut_matrices():
     with pytest.raises(ValueError, match="method"):
         optim(model(), method="sgd")
