@@ -132,7 +132,9 @@ def compose(config_name: str = "train", overrides: list[str] | None = None, conf
     """Hydra-style composition: ``<root>/<config_name>.yaml`` with a ``defaults`` list of ``group: option`` entries
     (each merged under the group key unless the file starts with ``# @package _global_``; experiment files are
     global, as the reference intends: the keys its code reads are top-level), then dotted overrides. An override
-    ``group=option`` for a defaults group re-selects the option (``experiment=benchmark``)."""
+    ``group=option`` for a defaults group re-selects the option (``experiment=benchmark``). Of an option selected that way
+    ``_target_`` stands against an experiment's section of that group, whose other keys (learning rate, decay) come later
+    than the option's as they do without a selection."""
     root = Path(config_root or CONFIG_ROOT)
     overrides = list(overrides or [])
     main = _load_yaml(root / f"{config_name}.yaml")
@@ -145,6 +147,7 @@ def compose(config_name: str = "train", overrides: list[str] | None = None, conf
             group_sel[k] = v
             overrides.remove(ov)
     cfg: dict = {}
+    targets: dict = {}
     self_merged = False
     for entry in defaults:
         if entry == "_self_":
@@ -159,6 +162,8 @@ def compose(config_name: str = "train", overrides: list[str] | None = None, conf
         nested = body.pop("defaults", None) or []
         m = re.match(r"\s*#\s*@package\s+(\S+)", text)
         package = m.group(1) if m else group
+        if group in group_sel and package == group and "_target_" in body:
+            targets[group] = body["_target_"]
         # a group file may list siblings of its own group that it builds on (`defaults: [defaults]` in
         # configs/data/era5-aurora.yaml): they are merged first, into the same package
         for sib in nested:
@@ -172,6 +177,8 @@ def compose(config_name: str = "train", overrides: list[str] | None = None, conf
             _merge(cfg.setdefault(package, {}), body)
     if not self_merged:
         _merge(cfg, main)
+    for group, target in targets.items():
+        cfg[group]["_target_"] = target
     out = Config(cfg)
     for ov in overrides:
         k, _, v = ov.partition("=")

@@ -217,3 +217,35 @@ def test_configuration():
     assert C.optim_config(plain).method == "adamw" and not C.model_config(plain).qk_norm
     group = C.compose("train", ["optimizer=muon", "experiment=b200_wp_inference"])
     assert C.optim_config(group).method in ("muon", "adamw")       # an experiment's own optimizer section comes later
+
+
+def experiments():
+    return sorted(p.stem for p in (C.CONFIG_ROOT / "experiment").glob("*.yaml"))
+
+
+@pytest.mark.parametrize("experiment", experiments())
+def test_the_group_selects_the_method_with_every_experiment(experiment):
+    """Whose other optimizer keys stand."""
+    plain = C.optim_config(C.compose("train", [f"experiment={experiment}"]))
+    group = C.optim_config(C.compose("train", ["optimizer=muon", f"experiment={experiment}"]))
+    assert plain.method == "adamw" and group.method == "muon"
+    assert (group.lr, group.betas, group.weight_decay, group.eps) == (plain.lr, plain.betas, plain.weight_decay, plain.eps)
+    assert (group.muon_beta, group.muon_nesterov, group.muon_steps, group.muon_scale) == (0.95, True, 5, 0.2)
+    back = C.compose("train", ["optimizer=muon", f"experiment={experiment}", "optimizer._target_=torch.optim.AdamW"])
+    assert C.optim_config(back).method == "adamw"                  # a key on the command line comes last
+    assert C.optim_config(C.compose("train", ["optimizer=muon"])).method == "muon"
+    assert C.optim_config(C.compose("train", ["optimizer=adamw", f"experiment={experiment}"])) == plain
+
+
+def test_a_selected_target_stands_against_an_experiment_of_another(tmp_path):
+    for group in ("optimizer", "experiment"):
+        (tmp_path / group).mkdir()
+    (tmp_path / "train.yaml").write_text("defaults:\n  - _self_\n  - optimizer: a\n  - experiment: x\n")
+    (tmp_path / "optimizer" / "a.yaml").write_text("_target_: A\nlr: 1.0\nown: 2\n")
+    (tmp_path / "optimizer" / "b.yaml").write_text("lr: 3.0\n")
+    (tmp_path / "experiment" / "x.yaml").write_text("# @package _global_\noptimizer:\n  _target_: X\n  lr: 5.0\n")
+    section = lambda *o: C.compose("train", list(o), tmp_path).optimizer.to_dict()  # noqa: E731
+    assert section() == {"_target_": "X", "lr": 5.0, "own": 2}
+    assert section("optimizer=a") == {"_target_": "A", "lr": 5.0, "own": 2}
+    assert section("optimizer=b") == {"_target_": "X", "lr": 5.0}
+    assert section("optimizer=a", "optimizer._target_=Y")["_target_"] == "Y"
