@@ -249,3 +249,13 @@ def test_a_selected_target_stands_against_an_experiment_of_another(tmp_path):
     assert section("optimizer=a") == {"_target_": "A", "lr": 5.0, "own": 2}
     assert section("optimizer=b") == {"_target_": "X", "lr": 5.0}
     assert section("optimizer=a", "optimizer._target_=Y")["_target_"] == "Y"
+
+
+@pytest.mark.parametrize("key", ["ns_coefficients=[3.4445,-4.775,2.0315]", "adjust_lr_fn=match_rms_adamw", "adjust_lr_fn=original",
+                                 "momentun=0.9"])
+def test_keys_that_the_orthogonalised_updates_do_not_take_are_refused(key):
+    name = key.partition("=")[0]
+    cfg = C.compose("train", ["experiment=tiny_cpu", "optimizer=muon", f"+optimizer.{key}"])
+    with pytest.raises(ValueError, match=f"optimizer.{name}"):
+        C.optim_config(cfg)
+    C.optim_config(C.compose("train", ["experiment=tiny_cpu", f"+optimizer.{key}"]))       # AdamW's sections as before
