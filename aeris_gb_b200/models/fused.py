@@ -173,15 +173,15 @@ KEPT = ("h1", "qkv", "o", "lse", "x1", "h2", "act", "u")
 KEPT_QK = (*KEPT, "qk")      # with norms of q and k: both as they were before
 
 
-def _qk_shape(T: int, HD: int):
-    return {"qk": ((T, 2 * HD), torch.bfloat16)}
+def _qk_shape(T: int, HD: int, qk: bool):
+    return {"qk": ((T, 2 * HD), torch.bfloat16)} if qk else {}
 
 
-def _kept_shapes(T: int, D: int, HD: int, heads: int, F: int) -> dict[str, tuple[tuple[int, ...], torch.dtype]]:
-    """What a block keeps for its backward pass: every internal the recompute would produce again."""
+def _kept_shapes(T: int, D: int, HD: int, heads: int, F: int, qk: bool = False) -> dict[str, tuple[tuple[int, ...], torch.dtype]]:
+    """What a block keeps for its backward pass: every internal the recompute would produce again. ``qk``: with norms of q and k."""
     bf = torch.bfloat16
     return {"h1": ((T, D), bf), "qkv": ((T, 3 * HD), bf), "o": ((T, HD), bf), "lse": ((T * heads,), torch.float32),
-            "x1": ((T, D), bf), "h2": ((T, D), bf), "act": ((T, F), bf), "u": ((T, 2 * F), bf)}
+            "x1": ((T, D), bf), "h2": ((T, D), bf), "act": ((T, F), bf), "u": ((T, 2 * F), bf), **_qk_shape(T, HD, qk)}
 
 
 class FreshKept(dict):
@@ -213,18 +213,18 @@ def _whole_kept(kept: dict[str, torch.Tensor], shapes, device) -> dict[str, torc
     return out
 
 
-def kept_bytes(T: int, D: int, HD: int, heads: int, F: int) -> int:
+def kept_bytes(T: int, D: int, HD: int, heads: int, F: int, qk: bool = False) -> int:
     """Bytes of :func:`_kept_shapes`, in closed form: every pass over a block asks for them."""
-    return T * (2 * (3 * D + 4 * HD + 3 * F) + 4 * heads)
+    return T * (2 * (3 * D + (6 if qk else 4) * HD + 3 * F) + 4 * heads)
 
 
-def _chunk_shapes(rows: int, D: int, HD: int, heads: int, F: int, tpn: int = 1):
+def _chunk_shapes(rows: int, D: int, HD: int, heads: int, F: int, tpn: int = 1, qk: bool = False):
     """Chunk workspaces of a forward pass that keeps nothing, and of the recompute (``h2`` in the forward pass is ``h``).
-    ``tpn``: ranks whose rows a tensor-parallel MLP gathers."""
+    ``tpn``: ranks whose rows a tensor-parallel MLP gathers; ``qk``: as :func:`_kept_shapes`."""
     bf = torch.bfloat16
     return {"h": ((rows, D), bf), "qkv": ((rows, 3 * HD), bf), "o": ((rows, HD), bf),
             "lse": ((rows * heads,), torch.float32), "x1": ((rows, D), bf), "h2": ((rows, D), bf),
-            "act": ((rows * tpn, F), bf)}
+            "act": ((rows * tpn, F), bf), **_qk_shape(rows, HD, qk)}
 
 
 def _grad_shapes(rows: int, D: int, HD: int, heads: int, F: int, tpn: int = 1):
@@ -257,7 +257,7 @@ def plan_kept_blocks(meta: BlockMeta, batch: int, D: int, F: int, n_blocks: int,
     they do not count as free."""
     HD = meta.heads * meta.head_dim
     T = batch * meta.n_win_per_sample * meta.L
-    per_block = kept_bytes(T, D, HD, meta.heads, F) + (4 * T * HD if meta.qk_norm else 0)
+    per_block = kept_bytes(T, D, HD, meta.heads, F, meta.qk_norm)
     step = chunk_step(meta, D, F)
     rows = step * meta.L
     fwd_rows = max(nw for _, _, nw, _ in _forward_spans(meta, batch, step, D, F, False)) * meta.L
@@ -270,7 +270,7 @@ def plan_kept_blocks(meta: BlockMeta, batch: int, D: int, F: int, n_blocks: int,
     if n_blocks * per_block + (n_blocks + 2) * stream + grads <= reserved - allocated:
         return n_blocks
     # a margin of two streams, and the workspaces of the blocks that recompute
-    base = (n_blocks + 4) * stream + grads + _WS.missing(_chunk_shapes(fwd_rows, D, HD, meta.heads, F), device)
+    base = (n_blocks + 4) * stream + grads + _WS.missing(_chunk_shapes(fwd_rows, D, HD, meta.heads, F, 1, meta.qk_norm), device)
     free = max(0, reserved - allocated - fragments) + torch.cuda.mem_get_info(device)[0]
     return n_kept(n_blocks, per_block, base, free)
 
@@ -284,7 +284,7 @@ def chunk_step(meta: BlockMeta, D: int, F: int) -> int:
     gigabyte saves no memory worth having and costs launches that the GPU finishes faster than they are issued (32
     windows of 64 tokens at dim 128 in chunks of 8: 1,582 launches per step for 7 ms of device time). With
     ``min_chunk_bytes = 0`` the bound is ``chunk_windows`` itself."""
-    floor = meta.chunk_floor // (kept_bytes(1, D, meta.heads * meta.head_dim, meta.heads, F) * meta.L)
+    floor = meta.chunk_floor // (kept_bytes(1, D, meta.heads * meta.head_dim, meta.heads, F, meta.qk_norm) * meta.L)
     step = min(max(meta.chunk_windows, floor), meta.n_win_per_sample, MAX_CHUNK_WINDOWS)
     if step < 1:
         raise ValueError(f"chunks of {step} windows: chunk_windows {meta.chunk_windows} with min_chunk_bytes "
@@ -303,7 +303,7 @@ def _forward_spans(meta: BlockMeta, B: int, step: int, D: int, F: int, kept: boo
     chunk each run in one launch per kernel (their modulation vectors are picked by row), when their internals are kept
     anyway or take less than the smallest chunk; the exchanges of the parallel paths work on one sample at a time."""
     if (B > 1 and step == meta.n_win_per_sample and meta.sp is None and meta.tp is None
-            and (kept or kept_bytes(B * step * meta.L, D, meta.heads * meta.head_dim, meta.heads, F) <= meta.chunk_floor)
+            and (kept or kept_bytes(B * step * meta.L, D, meta.heads * meta.head_dim, meta.heads, F, meta.qk_norm) <= meta.chunk_floor)
             and B * step <= MAX_CHUNK_WINDOWS):
         return [(0, 0, B * step, B)]
     return [(b, w0, nw, 1) for b in range(B) for w0, nw in _chunks(meta, step)]
@@ -417,9 +417,7 @@ def block_forward(x: torch.Tensor, mod: torch.Tensor, meta: BlockMeta, wn1, wqkv
     if kept is None:
         cmax = max(nw for _, _, nw, _ in spans) * meta.L
         tpn = meta.tp.tp if meta.tp is not None else 1   # gathered rows x local features: the same element count
-        shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn)
-        if qk is not None:
-            shapes.update(_qk_shape(cmax, HD))
+        shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn, meta.qk_norm)
         get = ws.whole if native else ws.get
         chunk_bufs = {k: get(k, *sh, dev) for k, sh in shapes.items() if k != "h2"}
         chunk_bufs["h1"] = chunk_bufs["h2"] = chunk_bufs.pop("h")
@@ -490,14 +488,10 @@ def block_backward(x: torch.Tensor, mod: torch.Tensor, dy: torch.Tensor, meta: B
         NB.refuse_misfits(meta, x, mod, weights, dx, grads)
     get = ws.whole if native else ws.get
     if kept is not None:
-        if qk is not None:
-            kept = _whole_kept(kept, {**_kept_shapes(T, D, HD, meta.heads, F), **_qk_shape(T, HD)}, dev)
-        elif not _all_whole(kept, T, D, HD, meta.heads, F, x.get_device()):
-            kept = _whole_kept(kept, _kept_shapes(T, D, HD, meta.heads, F), dev)
+        if qk is not None or not _all_whole(kept, T, D, HD, meta.heads, F, x.get_device()):
+            kept = _whole_kept(kept, _kept_shapes(T, D, HD, meta.heads, F, meta.qk_norm), dev)
     else:
-        shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn)
-        if qk is not None:
-            shapes.update(_qk_shape(cmax, HD))
+        shapes = _chunk_shapes(cmax, D, HD, meta.heads, F, tpn, meta.qk_norm)
         chunk_bufs = {k: get(k, *sh, dev) for k, sh in shapes.items()}
         chunk_bufs["h1"], act_b = chunk_bufs.pop("h"), chunk_bufs["act"]
     work = {k: get(k, *sh, dev) for k, sh in _grad_shapes(cmax, D, HD, meta.heads, F, tpn).items()}
@@ -651,9 +645,7 @@ class FusedBlock(torch.autograd.Function):
         kept = None
         if meta.keep and any(ctx.needs_input_grad):        # a frozen block has no backward pass to keep anything for
             shapes = _kept_shapes(regroup[0].numel() if regroup is not None else x.shape[0], x.shape[1],
-                                  meta.heads * meta.head_dim, meta.heads, w2.shape[1])
-            if qk:
-                shapes = {**shapes, **_qk_shape(shapes["qkv"][0][0], meta.heads * meta.head_dim)}
+                                  meta.heads * meta.head_dim, meta.heads, w2.shape[1], meta.qk_norm)
             try:
                 kept = FreshKept({k: torch.empty(shape, dtype=dt, device=x.device) for k, (shape, dt) in shapes.items()})
             except torch.OutOfMemoryError:

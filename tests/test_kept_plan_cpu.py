@@ -214,6 +214,59 @@ def test_the_plan_counts_the_workspaces_that_the_passes_use(monkeypatch):
     assert sum(asked.values()) <= empty.missing(shapes, "cpu")
 
 
+# ------------------------------------------------------------------------------------------------ norms of q and k
+NORMED = fused.BlockMeta(32, 900, 12, 64, E.MODE_MOD_THEN_NORM, 1e-6, 64, qk_norm=True)
+
+
+def test_norms_of_q_and_k_keep_both_as_they_were():
+    shapes = fused._kept_shapes(1000, 1536, 1280, 20, 4104, True)
+    assert set(shapes) == set(fused.KEPT_QK) and shapes["qk"] == ((1000, 2 * 1280), torch.bfloat16)
+    assert fused.kept_bytes(1000, 1536, 1280, 20, 4104, True) == sum(math.prod(sh) * dt.itemsize for sh, dt in shapes.values())
+
+
+def test_chunks_with_norms_stay_below_the_floor_too():
+    """1536 wide, 24 heads, 900 tokens: 12 windows take 499 MB (46,176 bytes a row) without the raw q and k and 565 with them, 512 MiB are 537."""
+    for qk, want in ((False, 12), (True, 11)):
+        meta = fused.BlockMeta(288, 900, 24, 64, E.MODE_MOD_THEN_NORM, 1e-6, 4, qk_norm=qk)
+        assert fused.chunk_step(meta, 1536, 4096) == want
+        bytes_of = lambda n: fused.kept_bytes(n * 900, 1536, 1536, 24, 4096, qk)  # noqa: E731
+        assert bytes_of(want) <= fused.MIN_CHUNK_BYTES < bytes_of(want + 1)
+
+
+def test_the_plan_counts_the_raw_q_and_k_of_blocks_that_recompute(monkeypatch):
+    need, raw = BLOCKS * fused.kept_bytes(ROWS, D, D, 12, FF, True), 32 * 900 * 2 * D * 2
+    base = PEAK + 2 * STREAM + GRADS + CHUNK + raw
+    for more, want in ((0, 3), (-1, 2)):               # half of the rest holds three of six blocks to the byte
+        _Memory(monkeypatch, driver=base + need + more)
+        assert _plan(NORMED) == want
+
+
+def test_the_passes_with_norms_use_the_workspaces_that_the_plan_counts(monkeypatch):
+    asked = {}
+
+    class Spy(fused.Workspace):
+        def get(self, name, shape, dtype, device, zero=False):
+            asked[name] = max(asked.get(name, 0), math.prod(shape) * dtype.itemsize)
+            return super().get(name, shape, dtype, device, zero)
+
+    monkeypatch.setattr(fused, "_WS", Spy())
+    for mod, names in ((fused.E, ("modnorm_fwd", "modnorm_bwd", "scale_rows", "gate_grad_finalize")), (fused.G, ("gemm",)),
+                       (fused.A, ("attn_fwd", "attn_bwd")), (fused.QN, ("qk_norm_fwd", "qk_norm_bwd"))):
+        for n in names:
+            monkeypatch.setattr(mod, n, lambda *a, **k: None)
+    meta = fused.BlockMeta(4, 16, 2, 8, E.MODE_MOD_THEN_NORM, 1e-6, 64, qk_norm=True)
+    bf = torch.bfloat16
+    ws = [torch.zeros(s, dtype=bf) for s in ((16,), (48, 16), (16, 16), (16,), (64, 16), (16, 32))]
+    qk = tuple(torch.ones(8, dtype=bf) for _ in range(2))
+    x, mod = torch.zeros(2 * 64, 16, dtype=bf), torch.zeros(2, 96)
+    fused.block_forward(x, mod, meta, *ws, qk=qk)
+    grads = {k: torch.zeros(w.shape) for k, w in zip(("n1", "to_qkv", "wo", "n2", "w1", "w2", "qn", "kn"), (*ws, *qk))}
+    fused.block_backward(x, mod, x.clone(), meta, *ws, grads, qk=qk)
+    shapes = {**fused._chunk_shapes(128, 16, 16, 2, 32, 1, True), **fused._grad_shapes(64, 16, 16, 2, 32)}
+    assert asked["qk"] == 128 * 32 * 2 and set(asked) == set(shapes)
+    assert sum(asked.values()) <= fused.Workspace().missing(shapes, "cpu")
+
+
 def _slices(tiles, kb, units=74, most=64, want=0):
     from aeris_gb_b200.ops import lib as L
     return L.lib().aeris_choose_k_splits(tiles, kb, units, most, want)
