@@ -228,6 +228,13 @@ typedef struct AerisOrtho {
   int groups, steps, bf16, nesterov, zero_grad; // 1 to 20 steps
   float beta, grad_scale, max_norm, decay, ema_beta;
 } AerisOrtho;
+// How a batch goes on this device, by its groups and steps, or a negative code: everything in one launch, all steps on the Gram
+// matrix, or launch by launch with these, where "pairs" are products by CTA pairs.
+enum {
+  ORTHO_ROUTE_ONE_LAUNCH = 1, ORTHO_ROUTE_GRAM_ALONE = 2, ORTHO_ROUTE_TWO_STEPS = 4, ORTHO_ROUTE_GRAM_PARTS = 8,
+  ORTHO_ROUTE_GRAM_PAIRS = 16, ORTHO_ROUTE_FACTOR_PAIRS = 32, ORTHO_ROUTE_UPDATE_PAIRS = 64
+};
+int aeris_ortho_route(const AerisOrtho* a);
 long long aeris_ortho_work_bytes(const AerisOrtho* a);          // of its groups and steps, or a negative code
 int aeris_orthogonalise(const AerisOrtho* a, void* stream);     // the number of kernels launched, or a negative code
 

@@ -1520,6 +1520,54 @@ int Layout::fill(const AerisOrtho& a) {
   return 0;
 }
 
+// The products of a batch by their sizes: S = X X^T, factor times factor, factor times X.
+OrthoGemm empty_gemm() {
+  OrthoGemm p{};
+  for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].N = p.cls[c].K = 1;        // a class without matrices
+  p.alpha = 1.f / NS_SCALE;
+  return p;
+}
+OrthoGemm gram_gemm(const Layout& l) {
+  OrthoGemm p = empty_gemm();
+  p.sym = 1;
+  p.M = l.d;
+  for (int c = 0; c < l.classes; ++c) p.cls[c].count = l.members[c], p.cls[c].N = l.d, p.cls[c].K = l.K[c];
+  return p;
+}
+OrthoGemm factor_gemm(const Layout& l) {
+  OrthoGemm p = empty_gemm();
+  p.sym = 1;
+  p.M = l.d;
+  p.cls[0].count = l.count;
+  p.cls[0].N = p.cls[0].K = l.d;
+  return p;
+}
+OrthoGemm update_gemm(const Layout& l) {
+  OrthoGemm p = empty_gemm();
+  p.M = l.d;
+  for (int c = 0; c < l.classes; ++c) p.cls[c].count = l.members[c], p.cls[c].N = l.K[c], p.cls[c].K = l.d;
+  return p;
+}
+long long tiles_of(const OrthoGemm& p, int c, int tile) {
+  const long long m = (p.M + tile - 1) / tile, n = (p.cls[c].N + tile - 1) / tile;
+  return p.sym ? m * (m + 1) / 2 : m * n;
+}
+// us of a launch: a start and an end, and for every round of tiles a fixed part and one per block of 64 of the reduction (the
+// mean over both classes). Measured, single / pair: 10 x 333 rows and columns over 384 8.2 / 11.0, 8 x (512 x 2048 over 512)
+// 15.6 / 14.9, 6 x (1024 x 4096 over 1024) 53.7 / 43.5, 16 x 1536 over 1536 68.7 / 58.3, 2 x 1536 over 4096 37.1 / 31.0.
+double cost_of(const OrthoGemm& p, int tile, int units, double ends, double round, double block) {
+  long long total = 0, blocks = 0;
+  for (int c = 0; c < NS_CLASSES; ++c) {
+    const long long n = tiles_of(p, c, tile) * p.cls[c].count;
+    total += n;
+    blocks += n * ((p.cls[c].K + OG_BK - 1) / OG_BK);
+  }
+  return ends + static_cast<double>((total + units - 1) / units) * (round + block * blocks / total);
+}
+bool takes_pairs(const OrthoGemm& p) {
+  return cost_of(p, 256, num_sms() / 2, 7, 1.6, 0.36) < cost_of(p, 128, num_sms(), 4.5, 1.3, 0.235);
+}
+
 struct Products {
   const Layout& l;
   __half* S;
@@ -1544,47 +1592,23 @@ struct Products {
   }
   template <int B_MN> void launch(const OrthoMaps& maps, OrthoGemm& p) {
     if (rc) return;
-    p.M = l.d;
     p.status = status;
-    const int sms = num_sms(), pairs = sms / 2;
-    auto tiles = [&](int c, int tile) {
-      const long long m = (p.M + tile - 1) / tile, n = (p.cls[c].N + tile - 1) / tile;
-      return p.sym ? m * (m + 1) / 2 : m * n;
-    };
-    // us of a launch: a start and an end, and for every round of tiles a fixed part and one per block of 64 of the reduction (the
-    // mean over both classes). Measured, single / pair: 10 x 333 rows and columns over 384 8.2 / 11.0, 8 x (512 x 2048 over 512)
-    // 15.6 / 14.9, 6 x (1024 x 4096 over 1024) 53.7 / 43.5, 16 x 1536 over 1536 68.7 / 58.3, 2 x 1536 over 4096 37.1 / 31.0.
-    auto cost = [&](int tile, int units, double ends, double round, double block) {
-      long long total = 0, blocks = 0;
-      for (int c = 0; c < NS_CLASSES; ++c) {
-        const long long n = tiles(c, tile) * p.cls[c].count;
-        total += n;
-        blocks += n * ((p.cls[c].K + OG_BK - 1) / OG_BK);
-      }
-      return ends + static_cast<double>((total + units - 1) / units) * (round + block * blocks / total);
-    };
     const bool parts = p.partial || p.cls[0].low;
-    const bool pair = !parts && cost(256, pairs, 7, 1.6, 0.36) < cost(128, sms, 4.5, 1.3, 0.235);
-    const int tile = pair ? 256 : 128, units = pair ? pairs : sms;
+    const bool pair = !parts && takes_pairs(p);
+    const int tile = pair ? 256 : 128, units = pair ? num_sms() / 2 : num_sms();
     long long total = 0;
-    for (int c = 0; c < NS_CLASSES; ++c) total += tiles(c, tile) * p.cls[c].count;
+    for (int c = 0; c < NS_CLASSES; ++c) total += tiles_of(p, c, tile) * p.cls[c].count;
     if (total > 0x7fffffff) {
       rc = -5;
       return;
     }
-    for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles(c, tile));
+    for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].tiles = static_cast<int>(tiles_of(p, c, tile));
     p.total = static_cast<int>(total) * (p.cls[0].splits > 1 ? p.cls[0].splits : 1);
     const int grid = (p.total < units ? p.total : units) * (pair ? 2 : 1);
     auto kern = pair ? ortho_gemm_pair_kernel<B_MN> : parts ? ortho_gemm_kernel<B_MN, true> : ortho_gemm_kernel<B_MN, false>;
     static std::atomic<uint64_t> done[3];
     rc = allow_smem(kern, OG_SMEM, done[pair ? 2 : parts]) ? launch_chained(kern, grid, OG_THREADS, OG_SMEM, stream, maps, p) : -20;
     ++launches;
-  }
-  OrthoGemm empty() const {
-    OrthoGemm p{};
-    for (int c = 0; c < NS_CLASSES; ++c) p.cls[c].N = p.cls[c].K = 1;      // a class without matrices
-    p.alpha = 1.f / NS_SCALE;
-    return p;
   }
   OrthoMaps square() const {
     OrthoMaps m;
@@ -1593,10 +1617,7 @@ struct Products {
     return m;
   }
   OrthoGemm factors(int out, int i, int j) const {
-    OrthoGemm p = empty();
-    p.sym = 1;
-    p.cls[0].count = l.count;
-    p.cls[0].N = p.cls[0].K = l.d;
+    OrthoGemm p = factor_gemm(l);
     p.cls[0].a0 = i * l.count;
     p.cls[0].b0 = j * l.count;
     p.cls[0].c0 = out * l.count;
@@ -1617,14 +1638,10 @@ struct Products {
     launch<0>(square(), p);
   }
   void gram(int from) {                       // S = X X^T
-    OrthoGemm p = empty();
+    OrthoGemm p = gram_gemm(l);
     OrthoMaps m = square();
-    p.sym = 1;
     for (int c = 0, first = 0; c < l.classes; first += l.members[c++]) {
       m.a[c] = m.b[c] = load_x[c];
-      p.cls[c].count = l.members[c];
-      p.cls[c].N = l.d;
-      p.cls[c].K = l.K[c];
       p.cls[c].a0 = p.cls[c].b0 = from * l.members[c];
       p.cls[c].c0 = F_S * l.count + first;
     }
@@ -1641,14 +1658,11 @@ struct Products {
     ++launches;
   }
   void update(int from, int by) {             // the other X = factor `by` X
-    OrthoGemm p = empty();
+    OrthoGemm p = update_gemm(l);
     OrthoMaps m = square();
     for (int c = 0, first = 0; c < l.classes; first += l.members[c++]) {
       m.b[c] = load_x[c];
       m.c[c] = store_x[c];
-      p.cls[c].count = l.members[c];
-      p.cls[c].N = l.K[c];
-      p.cls[c].K = l.d;
       p.cls[c].a0 = by * l.count + first;
       p.cls[c].b0 = from * l.members[c];
       p.cls[c].c0 = (1 - from) * l.members[c];
@@ -1658,13 +1672,9 @@ struct Products {
   // all steps on X number 0, into the other one
   __half* at(int f) const { return S + static_cast<long long>(f) * l.count * l.s_stride(); }
   void few(int splits, int steps) {
-    OrthoGemm g = empty();
+    OrthoGemm g = gram_gemm(l);
     OrthoMaps m = square();
-    g.sym = 1;
     m.a[0] = m.b[0] = load_x[0];
-    g.cls[0].count = l.count;
-    g.cls[0].N = l.d;
-    g.cls[0].K = l.K[0];
     g.cls[0].splits = splits;
     g.partial = partial;
     launch<0>(m, g);
@@ -1677,13 +1687,10 @@ struct Products {
     rc = launch_chained(ortho_polynomial_kernel, l.count, OS_THREADS, OL_SMEM, stream, static_cast<const float*>(partial), splits, S,
                         l.count, l.d, pitch(l.d), steps, status);
     ++launches;
-    OrthoGemm u = empty();
+    OrthoGemm u = update_gemm(l);
     m = square();
     m.b[0] = load_x[0];
     m.c[0] = store_x[0];
-    u.cls[0].count = l.count;
-    u.cls[0].N = l.K[0];
-    u.cls[0].K = l.d;
     u.cls[0].low = l.count;
     u.cls[0].c0 = l.count;
     u.alpha = 1.f / NS_Q_SCALE;
@@ -1710,6 +1717,17 @@ extern "C" long long aeris_ortho_work_bytes(const AerisOrtho* a) {
   Layout l;
   const int rc = l.fill(*a);
   return rc ? rc : l.bytes;
+}
+
+extern "C" int aeris_ortho_route(const AerisOrtho* a) {
+  Layout l;
+  if (const int rc = l.fill(*a)) return rc;
+  if (small(l)) return ORTHO_ROUTE_ONE_LAUNCH;
+  if (l.few) return ORTHO_ROUTE_GRAM_ALONE;
+  const bool parts = gram_splits(l) > 1;
+  return (l.steps.size[0] == 2 ? ORTHO_ROUTE_TWO_STEPS : 0) | (parts ? ORTHO_ROUTE_GRAM_PARTS : 0) |
+         (!parts && takes_pairs(gram_gemm(l)) ? ORTHO_ROUTE_GRAM_PAIRS : 0) |
+         (takes_pairs(factor_gemm(l)) ? ORTHO_ROUTE_FACTOR_PAIRS : 0) | (takes_pairs(update_gemm(l)) ? ORTHO_ROUTE_UPDATE_PAIRS : 0);
 }
 
 extern "C" int aeris_orthogonalise(const AerisOrtho* p, void* stream_) {

@@ -38,6 +38,8 @@ def _entry(name: str):
     f = getattr(_l.lib(), name)
     if name == "aeris_ortho_work_bytes":
         f.argtypes, f.restype = (ctypes.c_char_p,), ctypes.c_longlong
+    elif name == "aeris_ortho_route":
+        f.argtypes = (ctypes.c_char_p,)
     else:
         f.argtypes = (ctypes.c_char_p, ctypes.c_void_p)
     return f
@@ -46,10 +48,24 @@ def _entry(name: str):
 @functools.lru_cache(maxsize=4096)
 def _work_bytes(shapes: tuple, steps: int) -> int:
     """Workspace of a batch of (rows, cols, how many)."""
-    rest = _REST.pack(*[0] * 10, 0.0, 0, 0, len(shapes), steps, 0, 0, 0, *[0.0] * 5)
-    n = _entry("aeris_ortho_work_bytes")(b"".join(_group(*g) for g in shapes) + bytes(_GROUP.size * (MAX_GROUPS - len(shapes))) + rest)
+    n = _entry("aeris_ortho_work_bytes")(_shapes_alone(shapes, steps))
     _l.check(min(n, 0), "aeris_ortho_work_bytes", kernels=0)
     return n
+
+
+def _shapes_alone(shapes: tuple, steps: int) -> bytes:
+    rest = _REST.pack(*[0] * 10, 0.0, 0, 0, len(shapes), steps, 0, 0, 0, *[0.0] * 5)
+    return b"".join(_group(*g) for g in shapes) + bytes(_GROUP.size * (MAX_GROUPS - len(shapes))) + rest
+
+
+_ROUTES = ("one launch", "gram alone", "two steps", "gram parts", "gram pairs", "factor pairs", "update pairs")
+
+
+def route(shapes, steps: int = 5) -> set[str]:
+    """How a batch of (rows, cols, how many) with one shorter side goes on the current device (``ORTHO_ROUTE_``* of csrc/api.h)."""
+    rc = _entry("aeris_ortho_route")(_shapes_alone(tuple(shapes), steps))
+    _l.check(min(rc, 0), "aeris_ortho_route", kernels=0)
+    return {name for i, name in enumerate(_ROUTES) if rc >> i & 1}
 
 
 def _bytes_per_matrix(d: int, k: int) -> int:
