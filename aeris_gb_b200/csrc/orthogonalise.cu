@@ -230,6 +230,17 @@ __global__ void __launch_bounds__(256) ortho_squares_kernel(const OrthoGroups a,
   }
 }
 
+// What an element u is multiplied by for X, as scale (pre u): one factor alone would be below fp32's normal range, and zero, where
+// the norm is beyond 2^135, which elements within it reach. A norm that is no number stays one.
+struct NormScale {
+  float pre, scale;
+  __device__ __forceinline__ NormScale(double norm, double eps) {
+    pre = norm > 1e30 ? 0x1p-64f : 1.f;
+    scale = static_cast<float>(NS_SCALE / ((norm > eps || norm != norm ? norm : eps) * pre));
+  }
+  __device__ __forceinline__ float operator()(float u) const { return scale * (pre * u); }
+};
+
 // Normed, scaled and rounded to fp16 into X [d, K], through shared memory where the matrix is upright: one 64 x 64 tile per
 // block. An optimizer's value is computed again from gradient and momentum, which were read a moment before. Bound by memory
 // like the pass before it: 113 million elements of a step, 14 bytes each, 188 us.
@@ -250,7 +261,8 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += red[i];
   const double norm = sqrt(sum);
-  const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps)), gs = STEP ? step_scale(in) : 0.f;
+  const NormScale scale(norm, eps);
+  const float gs = STEP ? step_scale(in) : 0.f;
   const int tiles_c = (m.cols + 63) / 64;
   const int r0 = p.block / tiles_c * 64, c0 = p.block % tiles_c * 64;
   const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
@@ -258,7 +270,7 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
   const bool upright = m.rows > m.cols;
   auto value = [&](float g, float mom) {
     g = clean(g * gs);
-    return scale * (in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom);
+    return scale(in.nesterov ? in.beta * mom + (1.f - in.beta) * g : mom);
   };
   if (p.four) {
 #pragma unroll
@@ -274,7 +286,7 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
           if (in.zero_grad) *reinterpret_cast<float4*>(in.grad + e) = make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
           const float4 u = in_value4(in, e);
-          v[0] = scale * u.x; v[1] = scale * u.y; v[2] = scale * u.z; v[3] = scale * u.w;
+          v[0] = scale(u.x); v[1] = scale(u.y); v[2] = scale(u.z); v[3] = scale(u.w);
         }
       }
       if (upright) {
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(256) ortho_pack_kernel(const OrthoGroups a, co
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int rr = first + 32 * half + 4 * k, r = r0 + rr;
-        const float v = STEP ? value(u[k], mo[k]) : scale * u[k];
+        const float v = STEP ? value(u[k], mo[k]) : scale(u[k]);
         if (STEP && in.zero_grad && r < m.rows && c < m.cols) in.grad[p.at + static_cast<long long>(r) * m.ld + c] = 0.f;
         if (upright) tile[rr][cc] = v;
         else if (r < m.rows && c < m.ldx) X[static_cast<long long>(r) * m.ldx + c] = __float2half_rn(v);
@@ -1073,7 +1085,7 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
   sum = 0;
   for (int i = 0; i < threads / 32; ++i) sum += red[i];
   const double norm = sqrt(sum);
-  const float scale = static_cast<float>(NS_SCALE / (norm > eps || norm != norm ? norm : eps));
+  const NormScale scale(norm, eps);
   if (p.found)                                // each thread reads what it has written
     at_width(p.four, [&](auto width) {
       constexpr int W = decltype(width)::value;
@@ -1092,12 +1104,12 @@ ortho_small_kernel(const OrthoGroups a, const OrthoInput in, const OrthoGroups b
           }
         }
         if (W == 4 && !upright) {
-          const __half2 h[2] = {__floats2half2_rn(scale * u[0], scale * u[1]), __floats2half2_rn(scale * u[2], scale * u[3])};
+          const __half2 h[2] = {__floats2half2_rn(scale(u[0]), scale(u[1])), __floats2half2_rn(scale(u[2]), scale(u[3]))};
           *reinterpret_cast<uint2*>(smem + os_at(r, c)) = *reinterpret_cast<const uint2*>(h);
         } else {
 #pragma unroll
           for (int j = 0; j < W; ++j)
-            *reinterpret_cast<__half*>(smem + (upright ? os_at(c + j, r) : os_at(r, c + j))) = __float2half_rn(scale * u[j]);
+            *reinterpret_cast<__half*>(smem + (upright ? os_at(c + j, r) : os_at(r, c + j))) = __float2half_rn(scale(u[j]));
         }
       });
     });

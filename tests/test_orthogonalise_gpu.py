@@ -162,6 +162,18 @@ def test_scale_of_the_input_does_not_matter(power):
     assert torch.equal(OR.orthogonalise(x * 2.0 ** power, eps=1e-30), OR.orthogonalise(x))
 
 
+@pytest.mark.parametrize("shape", [(128, 384), (300, 400), (400, 300), (100, 2000), (33, 1001), (301, 403)], ids=str)
+def test_norms_beyond_fp32(shape):
+    """Elements up to fp32's largest, whose squares add up to more than it holds: 512 over the norm is below the normal range."""
+    x = gradient(*shape).sign() * 2.0 ** 127
+    x *= 1 + 0.9 * torch.rand(shape, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    assert bool(x.isfinite().all()) and 512 / x.double().norm() < torch.finfo(torch.float32).tiny
+    assert torch.equal(OR.orthogonalise(x), OR.orthogonalise(x * 2.0 ** -100))
+    low = x.bfloat16()
+    assert torch.equal(OR.orthogonalise(low), OR.orthogonalise(low * 2.0 ** -100))
+    assert OR.orthogonalise(x).abs().max() > 0
+
+
 def test_small_norms_are_not_raised():
     x = gradient(60, 60)
     x *= 1e-9 / x.norm()
