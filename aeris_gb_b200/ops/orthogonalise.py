@@ -204,8 +204,10 @@ def orthogonal_step(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Te
                         ("ema", ema, torch.float32)):
         if t is not None:
             _check_flat(name, t, master, dt)
-    parts = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (master, grad, momentum, weights, ema) if t is not None)
-    if any(a + n > b for (a, n), (b, _) in zip(parts, parts[1:])):
+    at = sorted([t.data_ptr() for t in (master, grad, momentum, ema) if t is not None])
+    size = 4 * master.numel()
+    if any(b - a < size for a, b in zip(at, at[1:])) or weights is not None and any(
+            -size < a - weights.data_ptr() < size // 2 for a in at):
         raise ValueError("the buffers of a step share memory")
     if norm_sq is not None and (norm_sq.numel() != 1 or norm_sq.dtype != torch.float64 or norm_sq.device != master.device):
         raise ValueError(f"norm_sq: one fp64 value on {master.device}, got {norm_sq.dtype} {tuple(norm_sq.shape)}")
