@@ -7,7 +7,8 @@
 // 1.21, |S| <= 1.46, |a I + b S + c S^2| <= a), so a constant scale of 512 keeps all of them inside fp16's range, and eight
 // times finer rounding matters: a rounding of the first steps is amplified like the small singular values, by up to a^5 = 485.
 // Error of the result (2-norm) against 64 bits on 768 x 2048 gradients with as much, a tenth and no white noise on a spectrum
-// falling like 1 / i: 1.0e-3, 2.5e-3, 4.9e-3; with bf16 operands 9.3e-3, 2.0e-2, 3.9e-2.
+// falling like 1 / i: 1.0e-3, 2.5e-3, 4.9e-3; with bf16 operands 9.3e-3, 2.0e-2, 3.9e-2. Empty directions raise roundings by as much:
+// a 400 x 900 matrix of rank 1, 4, 60 ends 0.026, 0.011, 0.009 of its 2-norm off (bf16 0.31, 0.11, 0.10).
 //
 // An optimizer's master moves by learning rate times the result, so the results' error is 3e-6 of the master a step; to halve it,
 // nearly every factor would need more bits (two fp16 parts, three times the products): left at fp16 by choice.
@@ -17,9 +18,11 @@
 //
 // Four routes by size: one launch where everything fits one CTA's shared memory (ortho_small_kernel), all steps on the Gram
 // matrix where rows are few and long (ortho_polynomial_kernel), else a launch per product, step by step or in pairs of steps
-// (groups_of). What bounds them: latency, then the start and end of launches (4.5 us each where products are short), and from
-// about 1000 rows on the tensor cores under the power cap (a step of 16 matrices of 1536 x 1536 and 12 of 1536 x 4096: products
-// 2.9 ms of 3.75, 2.2 where each is timed by itself).
+// (groups_of). The same call gives the same bits; other matrices in a batch may change the last ones of a matrix, by groups_of,
+// gram_splits and the number of blocks that sum its squares. What bounds them: latency, then the start and end of launches (4.5 us
+// each where products are short), and from about 1000 rows on the tensor cores under the power cap (a step of 16 matrices of 1536 x
+// 1536 and 12 of 1536 x 4096: products 2.9 ms of 3.75, 0.92 PFLOP/s, 2.2 where each is timed by itself; one 5120 x 13696 0.98 to 1.06
+// of the 1.41 that a GEMM holds).
 #include "api.h"
 #include "cluster.cuh"
 #include "common.cuh"
@@ -1439,7 +1442,8 @@ bool on_grid(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 // 2, 2, 1, 1.8e-3 as 3, 2; on 127 x 640 6e-4, 6e-4, 6e-4, 1.8e-3; a group of five diverges. Below GROUP_FROM rows single steps:
 // the products are no longer than their launches, of which groups have two more (us by single steps / in pairs: 256 x 600 94 / 101,
 // ten 333 x 1001 139 / 142, 42 of 384 x 1024 282 / 266, 30 of 500 x 1500 434 / 397), and a handful of rows does not average the
-// roundings (5 x 9: up to three times the error of single steps).
+// roundings (5 x 9: up to three times the error of single steps). K is the longest side of the batch: square matrices beside oblong
+// ones go in pairs with them, which costs them nothing (4 d^3 a step either way).
 constexpr int GROUP_FROM = 384;
 struct Groups {
   int n, size[20];
@@ -1464,8 +1468,8 @@ struct Layout {
   int fill(const AerisOrtho& a);
 };
 bool small(const Layout& l) { return l.d <= OS_MAX_D && l.K[0] <= OS_MAX_K; }
-// CTAs that share one matrix's X X^T where rows are few: eight blocks of 64 each, up to OL_MAX_SPLITS. By the length alone, so that
-// a matrix has the same bits in every batch.
+// CTAs that share one matrix's X X^T where rows are few: eight blocks of 64 each, up to OL_MAX_SPLITS. By the length alone: with few
+// rows a matrix has the same bits in every batch.
 int splits_of(const Layout& l, int c) {
   const int blocks = (l.K[c] + OG_BK - 1) / OG_BK, s = blocks / 8 < OL_MAX_SPLITS ? blocks / 8 : OL_MAX_SPLITS;
   if (s < 2) return 1;
@@ -1473,7 +1477,8 @@ int splits_of(const Layout& l, int c) {
   return (blocks + each - 1) / each;          // none of them empty
 }
 // The same for X X^T of longer sides whose tiles leave most of the GPU idle: seven 151 x 4472 have 21 tiles of 70 blocks, 16 us by
-// themselves and 4 in parts, plus 4 for adding those up. 1: in one piece.
+// themselves and 4 in parts, plus 4 for adding those up. 1: in one piece. By how many matrices there are too: a sum's order, and with it
+// its last bits, is another alone and among seven.
 int gram_splits(const Layout& l) {
   if (l.few || l.classes > 1) return 1;
   const int m = (l.d + 127) / 128, blocks = (l.K[0] + OG_BK - 1) / OG_BK;

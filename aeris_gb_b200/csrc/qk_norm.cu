@@ -14,8 +14,10 @@
 // (200,000 rows of 8 + 2 heads of 8: 93 us a row a step, 19 so). q and k have blocks in proportion to the time of a row. Everything
 // between load and store is fp32. 64,800 rows of 24 + 24 heads of 64, bf16: forward 135 us, 5.9 TB/s (90 % of what a plain copy
 // reaches); backward 214 us, 5.6 TB/s; 28,800 rows of 40 + 40 heads of 128 backward 319 us. fp32: 5.3 to 6 TB/s both ways from 64
-// channels on. Less where lanes or steps stay empty: 3.8 to 4.8 TB/s with heads of 72 to 104, 2 to 4 with heads of 16 to 36, 0.4
-// to 1.4 where heads are not whole fours. One row, or one window of 900, takes the GPU 2 to 4 us, less than the host needs (12).
+// channels on. bf16 less where lanes or steps stay empty, 3.8 to 4.8 TB/s with heads of 72 to 104, 2 to 4 with heads of 16 to 36, and
+// where a row has few heads, for a forward warp has the loads of one row under way (8 + 2 heads of 64: 4.1, stalls on loads first, 62 %
+// of the issue slots taken, 41 % of DRAM); 0.4 to 1.4 where heads are not whole fours. One row, or one window of 900, takes the GPU 2 to
+// 4 us, less than the host needs (12).
 #include "api.h"
 #include "common.cuh"
 #include "host.h"
@@ -551,7 +553,7 @@ bool angles_in_vectors(const AerisQkNorm& a) {
 }
 // Channels that load side by side, see Lane. fp32 backward goes by four: a group's two loads are a piece each then, where halves of
 // 32 bytes come twice through L2 (copies pass L1 by; 65,000 rows of 12 + 12 heads of 64 by eight 307 us, by four 210). Forward
-// L1 has the second half, and by eight is the faster (12,345 rows of 10 + 2 heads of 72: 22.6 us, by four 24.9).
+// L1 has the second half, and by eight is the faster (12,345 rows of 10 + 2 heads of 72, 40 channels turned: 23.5 us, by four 27.8).
 int width_of(const AerisQkNorm& a, bool grad) {
   const int size = a.f32 ? 4 : 2;
   auto all = [&](int w) {

@@ -281,8 +281,9 @@ def optim_config(cfg: Config):
     if family not in ("AdamW", "Adam", "Muon"):
         raise ValueError(f"optimizer._target_ = {target}: the fused updates implement Adam / AdamW and Muon")
     if family == "Muon" and (other := sorted(set(o) - MUON_KEYS)):
-        raise ValueError(f"optimizer.{other[0]}: torch.optim.Muon is taken with {', '.join(sorted(MUON_KEYS))} here. The coefficients of its "
-                         "iteration are (3.4445, -4.7750, 2.0315) and its updates are scaled by update_scale * sqrt(max(rows, columns))")
+        raise ValueError(f"optimizer.{other[0]}: torch.optim.Muon is taken with {', '.join(sorted(MUON_KEYS))} here. The "
+                         "coefficients of its iteration are (3.4445, -4.7750, 2.0315), and its updates are scaled by "
+                         "update_scale * sqrt(max(rows, columns))")
     if target.endswith(".Adam") and float(o.weight_decay) != 0.0:
         # torch.optim.Adam adds weight_decay * w to the gradient (L2); the fused kernels decay the weights directly
         warnings.warn("optimizer._target_ is torch.optim.Adam with a non-zero weight_decay: the decoupled (AdamW) "
