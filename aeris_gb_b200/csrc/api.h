@@ -238,6 +238,81 @@ int aeris_ortho_route(const AerisOrtho* a);
 long long aeris_ortho_work_bytes(const AerisOrtho* a);          // of its groups and steps, or a negative code
 int aeris_orthogonalise(const AerisOrtho* a, void* stream);     // the number of kernels launched, or a negative code
 
+// Layer norm (csrc/layer_norm.cu; mirrored in ops/layer_norm.py). Pitches in elements; columns lie side by side. Forward: y and
+// stats (mean, 1 / sqrt(var + eps)) of x. Backward: y receives the gradient of x, dw and db (both or neither is null only with
+// the other's flag) the column sums. y may be x or dy itself.
+typedef struct AerisLayerNorm {
+  const void *x, *dy;
+  void* y;
+  const void *w, *b;                // [cols], bf16 or fp32 both; null: ones, zeros
+  float *stats;                     // [rows, 2]
+  float *dw, *db, *work;            // [cols] each, null: not wanted; work: [slices, 2, cols]
+  long long rows, ld_x, ld_dy, ld_y;
+  int cols, f32, w_f32, add, slices;            // f32: type of x, dy, y; add: dw, db are added to
+  float eps;
+} AerisLayerNorm;
+// Both return the number of kernels launched, or a negative code.
+int aeris_layer_norm_fwd(const AerisLayerNorm* a, void* stream);
+int aeris_layer_norm_bwd(const AerisLayerNorm* a, void* stream);
+
+// Linear layer (csrc/linear.cu; mirrored in ops/linear.py): y = resid + act(x w^T + bias) with x [rows, inner], w [cols, inner],
+// bf16. Pitches in elements; those of x and w are multiples of 8 and their bases on 16-byte boundaries, the others' are free.
+enum { LIN_ACT_NONE = 0, LIN_ACT_RELU = 1, LIN_ACT_SILU = 2, LIN_ACT_GELU = 3, LIN_ACT_GELU_TANH = 4 };
+typedef struct AerisLinear {
+  const void *x, *w, *bias;         // bias [cols], fp32 or bf16, or null
+  const void* resid;                // [rows, cols] or null
+  void *y, *z;                      // z: null, or receives x w^T + bias
+  long long ld_x, ld_w, ld_resid, ld_y, ld_z;
+  int rows, inner, cols, act, bias_bf16;
+  int* status;
+} AerisLinear;
+int aeris_linear_fwd(const AerisLinear* a, void* stream);
+// dz = dy act'(z) and its column sums. dz: null where it is not wanted; db [cols] fp32 or null, added to with `add`; work:
+// [slices, cols] where db is wanted.
+typedef struct AerisLinearDz {
+  const void *dy, *z;
+  void* dz;
+  float *db, *work;
+  long long ld_dy, ld_z, ld_dz;
+  int rows, cols, act, add, slices;
+} AerisLinearDz;
+int aeris_linear_dz(const AerisLinearDz* a, void* stream);
+// dx = dz w and dw = dz^T x, each where its result is given. dz, w and x as x and w above. dw: bf16, or fp32 that is added to
+// (dw_f32). work: aeris_linear_work_bytes for the sums of slices of the rows (0: none needed).
+typedef struct AerisLinearGrad {
+  const void *dz, *w, *x;
+  void *dx, *dw;
+  float* work;
+  long long ld_dz, ld_w, ld_x, ld_dx, ld_dw, work_bytes;
+  int rows, inner, cols, dw_f32;
+  int* status;
+} AerisLinearGrad;
+long long aeris_linear_work_bytes(int rows, int inner, int cols, int dw_f32);
+int aeris_linear_grad(const AerisLinearGrad* a, void* stream);  // all three: the number of kernels launched, or a negative code
+
+// Window attention with a learned bias by relative position (csrc/position_bias.cu; mirrored in ops/position_bias.py). Windows of
+// high x wide tokens in rows; the relative position of query i and key j is (y_i - y_j + high - 1) (2 wide - 1) + x_i - x_j + wide - 1,
+// its bucket buckets[that] (null: itself), its bias table[bucket, head]. Entries of -1e30 and less hide the pairs of their bucket.
+typedef struct AerisBiasedAttn {
+  const void* qkv;                  // [n_win * high * wide, 3 * heads * head_dim] bf16, (q|k|v, head, channel)
+  void* o;                          // [n_win * high * wide, heads * head_dim]
+  float* lse;                       // [n_win, heads, high * wide], log2; +infinity where a query sees nothing
+  const void *table, *buckets;      // [table_rows, heads] fp32 or bf16; int32 or int64, outside [0, table_rows): recorded in the
+                                    // status word, the pairs hidden
+  const void* d_o;                  // backward: pitch of o
+  void* dqkv;
+  float* dtable;                    // [table_rows, heads], added to with `add`; null: not wanted
+  void* work;                       // aeris_biased_attn_work_bytes, from a 256-byte boundary on
+  int* status;
+  long long ld_qkv, ld_o, ld_dqkv, work_bytes;
+  int n_win, high, wide, heads, head_dim, table_rows, table_bf16, buckets64, add;
+  float scale;
+} AerisBiasedAttn;
+long long aeris_biased_attn_work_bytes(int n_win, int high, int wide, int heads, int head_dim, int backward, int with_table);
+// Both return the number of kernels launched, or a negative code.
+int aeris_biased_attn_fwd(const AerisBiasedAttn* a, void* stream);
+int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
