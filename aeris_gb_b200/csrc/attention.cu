@@ -19,6 +19,14 @@ namespace aeris {
 constexpr int ATT_THREADS = 192;
 constexpr int TILE = 128;
 
+// Bias of the scores by relative position: that of query i and key j of head h is table[h * size + zero + at[i] - at[j]], in log2
+// units (position_bias.cu). -infinity hides the pair. `at` goes on to the next multiple of 128 behind the window's end.
+struct PairBias {
+  const float* table;
+  const int* at;
+  int size, zero;
+};
+
 struct AttnFwdParams {
   __nv_bfloat16* O;
   int ldo;
@@ -31,6 +39,7 @@ struct AttnFwdParams {
   // is stored at row win * push_n_local + grow % push_n_local, column push_col0 + head * d of that rank's buffer.
   void* o_peers[8];
   int push_n_local, push_ld, push_col0;
+  PairBias bias;               // kernels with BIAS
 };
 
 // Byte offset of 16-byte vector `v` (0..7) of row `r` inside a [rows x 64] bf16 tile stored with the 128-byte swizzle.
@@ -165,7 +174,10 @@ template <int DCH, int MODE> struct AttnFwdRing {
 // product with both operands in shared memory reads 6 KB for 32 cycles of math, more than the 128 B/cycle the shared
 // memory delivers, so the kernel with P in shared memory (16 KB written and 16 KB read back per tile, on top of
 // Q, K and V) is bound by shared-memory bandwidth rather than by the tensor or the exp unit.
-template <int DCH, int POLY, int MODE>
+// BIAS: scores are biased by relative position (PairBias) on their way out of TMEM. The table of a head is read through L1, whose
+// lanes ask for neighbouring entries (their rows are neighbours); a column's place is the same for all lanes. A row that
+// sees no key has a sum of zero: zeros, and +infinity for its lse, which makes exp(score - lse) zero in the backward pass.
+template <int DCH, int POLY, int MODE, bool BIAS = false>
 __global__ void __launch_bounds__(ATT_THREADS, AttnFwdRing<DCH, MODE>::MIN_CTAS)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const AttnFwdParams p) {
@@ -325,13 +337,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const float sl2 = p.scale_log2;
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
+    [[maybe_unused]] const float* bias = nullptr;       // of this row: bias[-at[j]]
+    if constexpr (BIAS) bias = p.bias.table + static_cast<size_t>(head) * p.bias.size + p.bias.zero + p.bias.at[min(grow, N - 1)];
     // Raises the reference maximum to m_new: rescales the TMEM accumulator (once P V of the previous tile is done) and l.
     auto rescale = [&](int j, float m_new, bool& waited) -> bool {
       if (j > 0) {
         if (!mbar_wait(pv_done, (j - 1) & 1, p.status, ERR_TIMEOUT_ATTN)) return false;
         waited = true;
         tc_fence_after();
-        const float alpha = fast_exp2(m_ref - m_new);
+        const float alpha = BIAS && m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
         rescale_tmem_rows(tO + lane_addr, HD, alpha);
         tc_fence_before();
         l *= alpha;
@@ -366,6 +380,21 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (lane == 0) mbar_arrive(s_free);
         }
         if (warp_valid) {
+          if constexpr (BIAS) {
+            const int4* at = reinterpret_cast<const int4*>(p.bias.at + j * KVT);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int4 a = at[i], b = at[8 + i];
+              v0[4 * i] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i]), sl2, bias[-a.x]));
+              v0[4 * i + 1] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i + 1]), sl2, bias[-a.y]));
+              v0[4 * i + 2] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i + 2]), sl2, bias[-a.z]));
+              v0[4 * i + 3] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i + 3]), sl2, bias[-a.w]));
+              v1[4 * i] = __float_as_uint(fmaf(__uint_as_float(v1[4 * i]), sl2, bias[-b.x]));
+              v1[4 * i + 1] = __float_as_uint(fmaf(__uint_as_float(v1[4 * i + 1]), sl2, bias[-b.y]));
+              v1[4 * i + 2] = __float_as_uint(fmaf(__uint_as_float(v1[4 * i + 2]), sl2, bias[-b.z]));
+              v1[4 * i + 3] = __float_as_uint(fmaf(__uint_as_float(v1[4 * i + 3]), sl2, bias[-b.w]));
+            }
+          }
           // four independent chains of eight 3-input maxima instead of one chain of thirty-two
           float mxc[4];
 #pragma unroll
@@ -378,13 +407,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               mxc[c] = max3(mxc[c], __uint_as_float(v0[4 * i + c]), __uint_as_float(v1[4 * i + c]));
           }
           const float mx = fmaxf(max3(mxc[0], mxc[1], mxc[2]), mxc[3]);
-          const float m_new = fmaxf(m_ref, mx * sl2);
+          const float m_new = fmaxf(m_ref, BIAS ? mx : mx * sl2);
           if (__any_sync(0xffffffffu, m_new - m_ref > RESCALE_LOG2)) {
             if (!rescale(j, m_new, waited)) { ok = false; break; }
           }
           ATTN_STAMP(3);
           uint32_t pk[32];
-          if constexpr (POLY >= 0) {
+          if constexpr (BIAS) {
+            const float m = m_ref == -INFINITY ? 0.f : m_ref;
+            float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const uint32_t a = i < 16 ? v0[2 * i] : v1[2 * i - 32], b = i < 16 ? v0[2 * i + 1] : v1[2 * i - 31];
+              const float p0 = fast_exp2(__uint_as_float(a) - m), p1 = fast_exp2(__uint_as_float(b) - m);
+              rs[(2 * i) & 3] += p0;
+              rs[(2 * i + 1) & 3] += p1;
+              pk[i] = pack_bf16x2(p0, p1);
+            }
+            l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+          } else if constexpr (POLY >= 0) {
             l += softmax_row64<POLY>(v0, v1, sl2, m_ref, pk);
           } else {
             float rs[4] = {0.f, 0.f, 0.f, 0.f};
@@ -427,10 +468,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tmem_ld16(tSj + lane_addr + c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c + i < rem) mx = fmaxf(mx, __uint_as_float(v[i]));
+            for (int i = 0; i < 16; ++i) {
+              float s = __uint_as_float(v[i]);
+              if constexpr (BIAS) s = fmaf(s, sl2, bias[-p.bias.at[j * KVT + c + i]]);
+              if (c + i < rem) mx = fmaxf(mx, s);
+            }
           }
-          const float m_new = fmaxf(m_ref, mx * sl2);
+          const float m_new = fmaxf(m_ref, BIAS ? mx : mx * sl2);
           if (__any_sync(0xffffffffu, m_new - m_ref > RESCALE_LOG2)) {
             if (!rescale(j, m_new, waited)) { ok = false; break; }
           }
@@ -438,6 +482,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (j > 0 && !waited && !mbar_wait(pv_done, (j - 1) & 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
           }
           float rs = 0.f;
+          [[maybe_unused]] const float m = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll 1
           for (int c = 0; c < n_last; c += 16) {
             uint32_t v[16], pk[8];
@@ -445,8 +490,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              float p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, -m_ref));
-              float p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -m_ref));
+              float p0, p1;
+              if constexpr (BIAS) {
+                const int* at = p.bias.at + j * KVT + c + 2 * i;
+                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, bias[-at[0]]) - m);
+                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, bias[-at[1]]) - m);
+              } else {
+                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, -m_ref));
+                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -m_ref));
+              }
               if (c + 2 * i >= rem) p0 = 0.f;
               if (c + 2 * i + 1 >= rem) p1 = 0.f;
               rs += p0 + p1;
@@ -482,7 +534,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         !noted(&s_failed[q])) {
       tc_fence_after();
       {
-        const float inv = 1.f / l;
+        const float inv = BIAS && l == 0.f ? 0.f : 1.f / l;
         const size_t trow = static_cast<size_t>(win) * N + grow;
         __nv_bfloat16* dst = (p.O && grow < N) ? p.O + trow * p.ldo + head * p.d : nullptr;
         __nv_bfloat16* pdst = nullptr;
@@ -510,7 +562,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (pdst && live) *reinterpret_cast<uint4*>(pdst + c + 8 * g) = u;
           }
         }
-        if (p.lse && grow < N) p.lse[(static_cast<size_t>(win) * p.H + head) * N + grow] = m_ref + log2f(l);
+        if (p.lse && grow < N)
+          p.lse[(static_cast<size_t>(win) * p.H + head) * N + grow] = BIAS && l == 0.f ? INFINITY : m_ref + log2f(l);
       }
     }
   }
@@ -522,13 +575,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
 static int g_fwd_smem_pad = 0;   // extra dynamic shared memory per CTA: lowers the number of CTAs per SM (measurements)
 
-template <int DCH, int POLY, int MODE>
+template <int DCH, int POLY, int MODE, bool BIAS = false>
 static int launch_attn_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                            const AttnFwdParams& p, cudaStream_t stream) {
   constexpr int SMEM = DCH * 16384 + (AttnFwdRing<DCH, MODE>::NSK + AttnFwdRing<DCH, MODE>::NSV) * DCH * 8192 +
                        (MODE != 0 ? 0 : 16384) + 256;
   static int configured = -1;
-  auto kern = attn_fwd_kernel<DCH, POLY, MODE>;
+  auto kern = attn_fwd_kernel<DCH, POLY, MODE, BIAS>;
   const int smem = SMEM + g_fwd_smem_pad;
   if (configured != smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -20;
@@ -680,6 +733,26 @@ static int attn_fwd_impl(const void* q, int ldq, int q_col0, const void* k, int 
   return poly ? launch_attn_fwd<1, 2, 0>(tq, tk, tv, p, stream) : launch_attn_fwd<1, -1, 0>(tq, tk, tv, p, stream);
 }
 
+int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int N, int H, int head_dim, float scale,
+                           const float* table, const int* at, int size, int zero, int* status, void* stream_) {
+  if (head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
+  if (n_win <= 0 || N <= 0 || H <= 0 || n_win > 65535 || H > 65535) return -2;
+  if (!o || !whole_vectors(o, ldo)) return -4;
+  AttnFwdParams p{};
+  p.O = reinterpret_cast<__nv_bfloat16*>(o); p.ldo = ldo; p.lse = lse; p.N = N; p.H = H; p.n_win = n_win; p.d = head_dim;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  p.bias = {table, at, size, zero};
+  const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(qkv);
+  CUtensorMap tq, tk, tv;
+  int r;
+  if ((r = make_tmap_heads_bf16(&tq, b, head_dim, H, N, n_win, ld, TILE))) return r;
+  if ((r = make_tmap_heads_bf16(&tk, b + H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
+  if ((r = make_tmap_heads_bf16(&tv, b + 2 * H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  return head_dim > 64 ? launch_attn_fwd<2, -1, 1, true>(tq, tk, tv, p, stream)
+                       : launch_attn_fwd<1, -1, 1, true>(tq, tk, tv, p, stream);
+}
+
 // Whether the backward kernels can count their items, and a CTA the tiles it streams past them, in 32 bits.
 extern "C" int aeris_attn_bwd_countable(int n_win, int N, int H, int head_dim, int sms) {
   const int bt = head_dim <= 64 ? BwdCfg<1, false>::BT : BwdCfg<2, false>::BT;
@@ -692,7 +765,16 @@ extern "C" int aeris_attn_bwd_countable(int n_win, int N, int H, int head_dim, i
 static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v_col0, const void* o, const void* d_o,
                          int ldo, const float* lse, float* delta, void* dqkv, int ldg, int n_win, int N, int H,
                          int head_dim, float scale, int* status, void* stream_, const void* const* dq_peers, int sp,
-                         int push_n_local, int push_ld, int push_sec_w, int push_col0);
+                         int push_n_local, int push_ld, int push_sec_w, int push_col0, const PairBias* bias = nullptr,
+                         float* rest = nullptr);
+
+int aeris::attn_bwd_biased(const void* qkv, int ldq, const void* o, const void* d_o, int ldo, const float* lse, float* delta, float* rest,
+                           void* dqkv, int ldg, int n_win, int N, int H, int head_dim, float scale, const float* table,
+                           const int* at, int size, int zero, int* status, void* stream_) {
+  const PairBias bias{table, at, size, zero};
+  return attn_bwd_impl(qkv, ldq, 0, H * head_dim, 2 * H * head_dim, o, d_o, ldo, lse, delta, dqkv, ldg, n_win, N, H, head_dim, scale,
+                       status, stream_, nullptr, 0, 0, 0, 0, 0, &bias, rest);
+}
 
 extern "C" int aeris_attn_bwd(const void* qkv, int ldq, int q_col0, int k_col0, int v_col0, const void* o,
                               const void* d_o, int ldo, const float* lse, float* delta, void* dqkv, int ldg,
@@ -716,7 +798,7 @@ extern "C" int aeris_attn_bwd_push(const void* qkv, int ld, int H_local, const v
 static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v_col0, const void* o, const void* d_o,
                          int ldo, const float* lse, float* delta, void* dqkv, int ldg, int n_win, int N, int H,
                          int head_dim, float scale, int* status, void* stream_, const void* const* dq_peers, int sp,
-                         int push_n_local, int push_ld, int push_sec_w, int push_col0) {
+                         int push_n_local, int push_ld, int push_sec_w, int push_col0, const PairBias* bias, float* rest) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
   if (n_win <= 0 || N <= 0 || H <= 0 || n_win > 65535 || H > 65535) return -2;
@@ -749,6 +831,12 @@ static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v
     const int cols[3] = {q_col0, k_col0, v_col0};
     for (int i = 0; i < 3; ++i)
       if ((r = make_tmap_heads32_bf16(&out[i], g + cols[i], head_dim, H, N, n_win, ldg, 32))) return r;
+  }
+  if (bias) {
+    p.bias = *bias;
+    p.rest = rest;
+    return head_dim <= 64 ? launch_attn_bwd<1, true>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
+                          : launch_attn_bwd<2, true>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
   }
   return head_dim <= 64 ? launch_attn_bwd<1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
                         : launch_attn_bwd<2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);

@@ -45,6 +45,9 @@ struct AttnBwdParams {
   // row win * push_n_local + grow % push_n_local, column section * push_sec_w + push_col0 + head * d.
   void* dq_peers[8];
   int push_n_local, push_ld, push_sec_w, push_col0;
+  // kernels with BIAS: `rest` [4][n_win*H*N] receives, from the dQ kernel, four parts of what rows of dS add up to
+  PairBias bias;
+  float* rest;
 };
 
 __device__ __forceinline__ __nv_bfloat16* bwd_dst(const AttnBwdParams& p, int win, int grow, int head, int section,
@@ -170,7 +173,10 @@ __device__ __forceinline__ BwdItem bwd_item(int it, int n_row_tiles, int H) {
   return b;
 }
 
-template <int DCH, bool DKV>
+// BIAS: scores are biased by relative position (PairBias). A row of dS = P (dP - delta) adds up to nothing but for what rounding O
+// to bf16 costs delta (3e-4 of |dO| |O|); the dQ kernel records what it adds up to, which makes delta exact for the kernels that
+// follow: sums of dS over windows, which the bias's gradient is made of, would show it.
+template <int DCH, bool DKV, bool BIAS = false>
 __global__ void __launch_bounds__(BwdCfg<DCH, DKV>::THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant__ CUtensorMap tm_i1,
                 const __grid_constant__ CUtensorMap tm_r0, const __grid_constant__ CUtensorMap tm_r1,
@@ -621,6 +627,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
         if (lane == 0) mbar_arrive(&bar->stat_empty[sb.i]);
         sb.next(R::NSB);
         const uint64_t nl = f2_pack(nlse, nlse), nd = f2_pack(ndelta, ndelta);
+        [[maybe_unused]] const float* bias = nullptr;      // of this row: bias[-at[j]]
+        [[maybe_unused]] uint64_t left = 0;                // what the row's dS add up to
+        [[maybe_unused]] size_t rest_at = 0;
+        [[maybe_unused]] bool rest_in = false;
+        if constexpr (BIAS) {
+          const BwdItem w = bwd_item(it, row_tiles, p.H);
+          const int grow = w.tile * TILE + row;
+          rest_in = grow < N;
+          rest_at = ((static_cast<size_t>(ch * R::WPC + wg % R::WPC) * p.n_win + w.win) * p.H + w.head) * N + grow;
+          bias = p.bias.table + static_cast<size_t>(w.head) * p.bias.size + p.bias.zero + p.bias.at[min(grow, N - 1)];
+        }
         for (; j < n_str; j += NCH, ph ^= 1) {
           if (!wait(&bar->s_full[ch], ph)) { ok = false; break; }
           if (j < nfull) {
@@ -630,7 +647,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
 #pragma unroll
             for (int i = 0; i < CPT; i += 2) {
               float t0, t1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(pr[i]), __uint_as_float(pr[i + 1])), sl, nl), t0, t1);
+              const uint64_t s2 = f2_pack(__uint_as_float(pr[i]), __uint_as_float(pr[i + 1]));
+              if constexpr (BIAS) {
+                const int2 a = *reinterpret_cast<const int2*>(p.bias.at + j * BT + c0 + i);
+                f2_unpack(f2_add(f2_fma(s2, sl, f2_pack(bias[-a.x], bias[-a.y])), nl), t0, t1);
+              } else {
+                f2_unpack(f2_fma(s2, sl, nl), t0, t1);
+              }
               pr[i] = __float_as_uint(fast_exp2(t0));           // in place: ahead of the wait
               pr[i + 1] = __float_as_uint(fast_exp2(t1));
             }
@@ -644,7 +667,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
               for (int i = 0; i < 8; ++i) {
                 const uint64_t df = f2_add(f2_pack(__uint_as_float(dv[2 * i]), __uint_as_float(dv[2 * i + 1])), nd);
                 const uint64_t p2 = f2_pack(__uint_as_float(pr[c + 2 * i]), __uint_as_float(pr[c + 2 * i + 1]));
-                pk[i] = f2_to_bf16x2(f2_mul(p2, df));
+                const uint64_t ds = f2_mul(p2, df);
+                if constexpr (BIAS) left = f2_add(left, ds);
+                pk[i] = f2_to_bf16x2(ds);
               }
               // 16 columns become 8 words at column c / 2 <= c: only columns that were read are overwritten
               tmem_st8(tD + (c >> 1), pk);
@@ -660,12 +685,20 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, nlse));
-                const float p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, nlse));
+                float p0, p1;
+                if constexpr (BIAS) {
+                  const int* at = p.bias.at + j * BT + c0 + c + 2 * i;
+                  p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, bias[-at[0]]) + nlse);
+                  p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, bias[-at[1]]) + nlse);
+                } else {
+                  p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, nlse));
+                  p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, nlse));
+                }
                 float d0 = p0 * (__uint_as_float(dv[2 * i]) + ndelta);
                 float d1 = p1 * (__uint_as_float(dv[2 * i + 1]) + ndelta);
                 if (c0 + c + 2 * i >= rem) d0 = 0.f;
                 if (c0 + c + 2 * i + 1 >= rem) d1 = 0.f;
+                if constexpr (BIAS) left = f2_add(left, f2_pack(d0, d1));
                 pk[i] = pack_bf16x2(d0, d1);
               }
               tmem_st8(tD + (c >> 1), pk);
@@ -675,15 +708,26 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
           tmem_wait_st();
           tell(&bar->ds_full[ch]);
         }
+        if constexpr (BIAS) {
+          float a, b;
+          f2_unpack(left, a, b);
+          if (ok && rest_in) p.rest[rest_at] = a + b;
+        }
         j -= n_str;                      // the stream of tiles runs on into the next item
       }
     } else {
       const uint64_t nsl = f2_pack(-p.scale_log2, -p.scale_log2);
       // Columns past the window's end have zero Q and dO rows and zero statistics (P = 1, dS = 0): they add nothing. Rows
       // past its end may hold anything: they are not stored.
-      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l) -> uint32_t {
+      [[maybe_unused]] const float* bias = nullptr;         // of this row's key: bias[at[i]]
+      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l, [[maybe_unused]] const int* at) -> uint32_t {
         float t0, t1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), nsl, l), t0, t1);     // -(log2 P)
+        uint64_t x = f2_fma(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), nsl, l);             // -(log2 P)
+        if constexpr (BIAS) {
+          const int2 a = *reinterpret_cast<const int2*>(at);
+          x = f2_sub(x, f2_pack(bias[a.x], bias[a.y]));
+        }
+        f2_unpack(x, t0, t1);
         t0 = fast_exp2(-t0);
         t1 = fast_exp2(-t1);
         s0 = __float_as_uint(t0);
@@ -696,6 +740,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       };
       int st = ch;
       for (int it = 0; it < n_items && ok; ++it) {
+        if constexpr (BIAS) {
+          const BwdItem w = bwd_item(it, row_tiles, p.H);
+          bias = p.bias.table + static_cast<size_t>(w.head) * p.bias.size + p.bias.zero - p.bias.at[min(w.tile * TILE + row, N - 1)];
+        }
         for (; j < n_str; j += NCH, ph ^= 1, st = st + NCH >= NST ? st + NCH - NST : st + NCH) {
           if (!wait(&bar->s_full[ch], ph)) { ok = false; break; }
           const ulonglong2* ls = reinterpret_cast<const ulonglong2*>(s_stat + st * 2 * BT + c0);
@@ -709,8 +757,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const ulonglong2 l = ls[c / 4 + i];
-                pp[2 * i] = probs(pr[c + 4 * i], pr[c + 4 * i + 1], l.x);
-                pp[2 * i + 1] = probs(pr[c + 4 * i + 2], pr[c + 4 * i + 3], l.y);
+                const int* at = BIAS ? p.bias.at + j * BT + c0 + c + 4 * i : nullptr;
+                pp[2 * i] = probs(pr[c + 4 * i], pr[c + 4 * i + 1], l.x, at);
+                pp[2 * i + 1] = probs(pr[c + 4 * i + 2], pr[c + 4 * i + 3], l.y, at + 2);
               }
               tmem_st8(tS + (c >> 1), pp);
             }
@@ -741,8 +790,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const ulonglong2 l = ls[c / 4 + i], de = ds[c / 4 + i];
-                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x);
-                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y);
+                const int* at = BIAS ? p.bias.at + j * BT + c0 + c + 4 * i : nullptr;
+                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x, at);
+                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y, at + 2);
                 dd[2 * i] = grad(sv[4 * i], sv[4 * i + 1], dv[4 * i], dv[4 * i + 1], de.x);
                 dd[2 * i + 1] = grad(sv[4 * i + 2], sv[4 * i + 3], dv[4 * i + 2], dv[4 * i + 3], de.y);
               }
@@ -765,15 +815,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
   if (warp == R::W_A) tmem_dealloc(tmem_base, 512);
 }
 
-template <int DCH>
+// What the rows of dS added up to joins delta (see BIAS above): the four parts in their order.
+static __global__ void __launch_bounds__(256) attn_delta_rest_kernel(float* delta, const float* rest, long long n) {
+  chain_point();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x)
+    delta[i] += (rest[i] + rest[n + i]) + (rest[2 * n + i] + rest[3 * n + i]);
+}
+
+template <int DCH, bool BIAS = false>
 static int launch_attn_bwd(const CUtensorMap& tq128, const CUtensorMap& tk64, const CUtensorMap& tv64,
                            const CUtensorMap& tdo128, const CUtensorMap& tq64, const CUtensorMap& tk128,
                            const CUtensorMap& tv128, const CUtensorMap& tdo64, const CUtensorMap (&out)[3],
                            const AttnBwdParams& p, cudaStream_t stream) {
   using R1 = BwdCfg<DCH, false>;
   using R2 = BwdCfg<DCH, true>;
-  auto k1 = attn_bwd_kernel<DCH, false>;
-  auto k2 = attn_bwd_kernel<DCH, true>;
+  auto k1 = attn_bwd_kernel<DCH, false, BIAS>;
+  auto k2 = attn_bwd_kernel<DCH, true, BIAS>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, R1::SMEM) != cudaSuccess) return -20;
@@ -786,6 +843,12 @@ static int launch_attn_bwd(const CUtensorMap& tq128, const CUtensorMap& tk64, co
   }
   const int n = (p.N + TILE - 1) / TILE * p.H * p.n_win, grid = n < num_sms() ? n : num_sms();
   if (launch_chained(k1, grid, R1::THREADS, R1::SMEM, stream, tq128, tdo128, tk64, tv64, out[0], out[0], p, n)) return -21;
+  if constexpr (BIAS) {
+    const long long rows = static_cast<long long>(p.n_win) * p.H * p.N, blocks = (rows + 255) / 256, most = 8ll * num_sms();
+    if (launch_chained(attn_delta_rest_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, p.delta,
+                       static_cast<const float*>(p.rest), rows))
+      return -21;
+  }
   return launch_chained(k2, grid, R2::THREADS, R2::SMEM, stream, tk128, tv128, tq64, tdo64, out[1], out[2], p, n) ? -22 : 0;
 }
 
