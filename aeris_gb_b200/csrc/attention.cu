@@ -20,7 +20,7 @@ constexpr int ATT_THREADS = 192;
 constexpr int TILE = 128;
 
 // Bias of the scores by relative position: that of query i and key j of head h is table[h * size + zero + at[i] - at[j]], in log2
-// units (position_bias.cu). -infinity hides the pair. `at` goes on to the next multiple of 128 behind the window's end.
+// units (position_bias.cu, which lays it out so that 32 queries next to one another are in 32 banks of shared memory); `size` is a multiple of 4. -infinity hides the pair. `at` goes on to the next multiple of 128 behind the window's end.
 struct PairBias {
   const float* table;
   const int* at;
@@ -580,13 +580,12 @@ static int launch_attn_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const C
                            const AttnFwdParams& p, cudaStream_t stream) {
   constexpr int SMEM = DCH * 16384 + (AttnFwdRing<DCH, MODE>::NSK + AttnFwdRing<DCH, MODE>::NSV) * DCH * 8192 +
                        (MODE != 0 ? 0 : 16384) + 256;
-  static int configured = -1;
+  static std::atomic<uint64_t> done{0};
   auto kern = attn_fwd_kernel<DCH, POLY, MODE, BIAS>;
   const int smem = SMEM + g_fwd_smem_pad;
-  if (configured != smem) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -20;
-    configured = smem;
-  }
+  if (g_fwd_smem_pad) done.store(0);        // a measurement: asked for anew
+  if (!allow_smem_once(kern, smem, done)) return -20;
+  if (g_fwd_smem_pad) done.store(0);
   dim3 grid((p.N + TILE - 1) / TILE, p.H, p.n_win);
   return launch_chained(kern, grid, ATT_THREADS, smem, stream, tq, tk, tv, p);
 }
@@ -749,6 +748,13 @@ int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse
   if ((r = make_tmap_heads_bf16(&tk, b + H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
   if ((r = make_tmap_heads_bf16(&tv, b + 2 * H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const int room = 4 * size + (N + 127) / 128 * 512;
+  if (head_dim <= 64 && N > 2 * TILE && room <= AttnQuad<2>::TABLE) {
+    CUtensorMap to;
+    if ((r = make_tmap_heads32_bf16(&to, o, head_dim, H, N, n_win, ldo, 32))) return r;
+    return room <= AttnQuad<1>::TABLE ? launch_attn_fwd_quad<1>(tq, tk, tv, to, p, stream)
+                                      : launch_attn_fwd_quad<2>(tq, tk, tv, to, p, stream);
+  }
   return head_dim > 64 ? launch_attn_fwd<2, -1, 1, true>(tq, tk, tv, p, stream)
                        : launch_attn_fwd<1, -1, 1, true>(tq, tk, tv, p, stream);
 }
@@ -835,8 +841,14 @@ static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v
   if (bias) {
     p.bias = *bias;
     p.rest = rest;
-    return head_dim <= 64 ? launch_attn_bwd<1, true>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
-                          : launch_attn_bwd<2, true>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
+    const int room = 4 * p.bias.size + (N + 127) / 128 * 512;
+    if (head_dim <= 64)
+      return room <= BwdCfg<1, false, 1>::TABLE && room <= BwdCfg<1, true, 1>::TABLE
+                 ? launch_attn_bwd<1, 1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
+                 : launch_attn_bwd<1, 2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
+    return room <= BwdCfg<2, false, 1>::TABLE && room <= BwdCfg<2, true, 1>::TABLE
+               ? launch_attn_bwd<2, 1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
+               : launch_attn_bwd<2, 2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
   }
   return head_dim <= 64 ? launch_attn_bwd<1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
                         : launch_attn_bwd<2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);

@@ -63,13 +63,15 @@ __device__ __forceinline__ __nv_bfloat16* bwd_dst(const AttnBwdParams& p, int wi
 
 // Shared memory (227 KB) and the 512 TMEM columns set the numbers: the chains' S and dP + the accumulators (HD columns for
 // dQ, twice while there is room; HD each for dK and dV).
-template <int DCH, bool DKV> struct BwdCfg {
+// BIASED: 0, or scores are biased by relative position (PairBias): from a copy of the head's table in shared memory, for which a
+// stage of the ring makes room (1), or where it does not fit from memory through L1 (2).
+template <int DCH, bool DKV, int BIASED = 0> struct BwdCfg {
   static constexpr int HD = 64 * DCH;
   static constexpr int BT = (DCH == 1) ? 96 : 64;         // rows of a streamed tile
   static constexpr int NCH = 2;                           // chains
   static constexpr int WPC = 2;                           // warpgroups of math warps per chain, side by side
   static constexpr int CPT = BT / WPC;                    // columns of a tile per math thread
-  static constexpr int NST = (DCH == 1) ? 5 : 4;          // ring of streamed tiles
+  static constexpr int NST = ((DCH == 1) ? 5 : 4) - (BIASED == 1);     // ring of streamed tiles
   static constexpr int NB = (DCH == 1) ? 2 : 1;           // buffers for an item's own operands
   // dQ: dO rows for delta come from an item's own operand where its buffers are loaded early enough, O rows from memory
   static constexpr bool DO_SMEM = !DKV && NB > 1;
@@ -82,6 +84,7 @@ template <int DCH, bool DKV> struct BwdCfg {
   static constexpr int OUT_BYTES = 4 * 4096;              // two buffers of 32 rows x 32 columns per epilogue warp
   static constexpr int STAT = DKV ? NST * 2 * BT : NSB * 2 * TILE;
   static constexpr int SMEM = NB * 2 * OP + NST * STAGE + OUT_BYTES + STAT * 4 + 512;
+  static constexpr int TABLE = BIASED == 1 ? 227 * 1024 - SMEM : 0;     // room for a table and the places
   // warps: epilogue; math from 4 on; loads, the two issuers, one without work
   static constexpr int W_EPI = 0, W_MATH = 4, W_LOAD = 4 + 4 * NCH * WPC, W_A = W_LOAD + 1, W_B = W_LOAD + 2;
   static constexpr int THREADS = 32 * (W_LOAD + 4);
@@ -105,6 +108,7 @@ struct BwdBars {
   uint64_t a_full, a_empty; // dV
   uint64_t b_full[2], b_empty[2];
   uint64_t stat_full[4], stat_empty[4];
+  uint64_t bias_full, bias_empty;   // a head's table is there; no math warp needs it any more
 };
 static_assert(sizeof(BwdBars) + 8 + 4 * 4 <= 512, "barriers");
 
@@ -176,13 +180,24 @@ __device__ __forceinline__ BwdItem bwd_item(int it, int n_row_tiles, int H) {
 // BIAS: scores are biased by relative position (PairBias). A row of dS = P (dP - delta) adds up to nothing but for what rounding O
 // to bf16 costs delta (3e-4 of |dO| |O|); the dQ kernel records what it adds up to, which makes delta exact for the kernels that
 // follow: sums of dS over windows, which the bias's gradient is made of, would show it.
-template <int DCH, bool DKV, bool BIAS = false>
+// Items go by head and window then, and every CTA has a run of them: it loads one table or two.
+__device__ __forceinline__ BwdItem bwd_bias_item(int idx, int n_row_tiles, int n_win) {
+  const int hw = idx / n_row_tiles;
+  BwdItem b;
+  b.tile = idx - hw * n_row_tiles;
+  b.head = hw / n_win;
+  b.win = hw - b.head * n_win;
+  return b;
+}
+
+template <int DCH, bool DKV, int BIASED = 0>
 __global__ void __launch_bounds__(BwdCfg<DCH, DKV>::THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant__ CUtensorMap tm_i1,
                 const __grid_constant__ CUtensorMap tm_r0, const __grid_constant__ CUtensorMap tm_r1,
                 const __grid_constant__ CUtensorMap tm_out_b, const __grid_constant__ CUtensorMap tm_out_a,
                 const AttnBwdParams p, const int n_items_total) {
-  using R = BwdCfg<DCH, DKV>;
+  using R = BwdCfg<DCH, DKV, BIASED>;
+  constexpr bool BIAS = BIASED != 0;
   constexpr int HD = R::HD, BT = R::BT, NCH = R::NCH, NST = R::NST, NB = R::NB, CPT = R::CPT;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* s_i0 = smem;                          // [NB]
@@ -195,6 +210,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_failed = s_abort + 1;      // [4] see note_failure
+  [[maybe_unused]] float* s_table = reinterpret_cast<float*>(smem + R::SMEM);      // [p.bias.size], then places
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int N = p.N;
@@ -203,8 +219,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
   const int n_last = rem ? ((rem + 15) & ~15) : BT;       // columns of the products with the last one
   const int row_tiles = (N + TILE - 1) / TILE;
   const int n_ctas = static_cast<int>(gridDim.x);
-  const int n_items = (n_items_total - static_cast<int>(blockIdx.x) + n_ctas - 1) / n_ctas;
+  int n_items = (n_items_total - static_cast<int>(blockIdx.x) + n_ctas - 1) / n_ctas;
+  [[maybe_unused]] int item0 = 0;
+  if constexpr (BIAS) {
+    item0 = static_cast<int>(static_cast<long long>(n_items_total) * blockIdx.x / n_ctas);
+    n_items = static_cast<int>(static_cast<long long>(n_items_total) * (blockIdx.x + 1) / n_ctas) - item0;
+  }
   const int total = n_items * n_str;
+  auto item_at = [&](int it) -> BwdItem {
+    if constexpr (BIAS) return bwd_bias_item(item0 + it, row_tiles, p.n_win);
+    else return bwd_item(it, row_tiles, p.H);
+  };
 
   if (threadIdx.x == 0) {
     int ab = (p.status && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
@@ -228,6 +253,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
     }
     mbar_init(&bar->a_full, 1); mbar_init(&bar->a_empty, 4);
     for (int i = 0; i < R::NACC; ++i) { mbar_init(&bar->b_full[i], 1); mbar_init(&bar->b_empty[i], 4); }
+    if constexpr (BIASED == 1) { mbar_init(&bar->bias_full, 1); mbar_init(&bar->bias_empty, 4 * NCH * R::WPC); }
     for (int i = 0; i < R::NSB; ++i) { mbar_init(&bar->stat_full[i], 4); mbar_init(&bar->stat_empty[i], 4 * NCH * R::WPC); }
     fence_barrier_init();
   }
@@ -249,7 +275,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       };
       Slot is;
       auto load_item = [&](int it) -> bool {
-        const BwdItem w = bwd_item(it, row_tiles, p.H);
+        const BwdItem w = item_at(it);
         if (!wait(&bar->i0_empty[is.i], is.ph ^ 1)) return false;
         if (lane == 0) {
           mbar_expect_tx(&bar->i0_full[is.i], R::OP);
@@ -274,8 +300,26 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       for (int i = 0; i < (AHEAD ? AHEAD : 1) && i < n_items && ok; ++i) ok = load_item(i);
       const int j_item = min(AHEAD ? 2 : NCH - 1, n_str - 1);
       Slot rs;
+      [[maybe_unused]] int head = -1;
+      [[maybe_unused]] uint32_t bias_ph = 0;
       for (int it = 0; it < n_items && ok; ++it) {
-        const BwdItem w = bwd_item(it, row_tiles, p.H);
+        const BwdItem w = item_at(it);
+        if constexpr (BIASED == 1) {
+          // the table of a head, once the math warps are through with the one before; with the first the tokens' places
+          if (w.head != head) {
+            if (head >= 0) {
+              if (!wait(&bar->bias_empty, bias_ph)) { ok = false; break; }
+              bias_ph ^= 1;
+            }
+            if (lane == 0) {
+              const uint32_t bytes = p.bias.size * 4, at_bytes = head < 0 ? (N + 127) / 128 * 512 : 0;
+              mbar_expect_tx(&bar->bias_full, bytes + at_bytes);
+              bulk_load(s_table, p.bias.table + static_cast<size_t>(w.head) * p.bias.size, bytes, &bar->bias_full);
+              if (at_bytes) bulk_load(s_table + p.bias.size, p.bias.at, at_bytes, &bar->bias_full);
+            }
+            head = w.head;
+          }
+        }
         const size_t sbase = (static_cast<size_t>(w.win) * p.H + w.head) * N;
         for (int j = 0; j < n_str; ++j) {
           if (!wait(&bar->r_empty[rs.i], rs.ph ^ 1)) { ok = false; break; }
@@ -461,7 +505,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       constexpr int UN = R::DO_SMEM ? 8 : 2;           // loads in flight
       const int sub = lane % LPR, r0 = lane / LPR;
       if (!mbar_wait_warp(&bar->stat_empty[sb.i], sb.ph ^ 1, p.status, ERR_TIMEOUT_ATTN)) return false;
-      const BwdItem w = bwd_item(it, row_tiles, p.H);
+      const BwdItem w = item_at(it);
       float* st = s_stat + sb.i * 2 * TILE;
       const size_t sbase = (static_cast<size_t>(w.win) * p.H + w.head) * N + w.tile * TILE;
       const int live = N - w.tile * TILE;            // rows of this tile inside the window
@@ -557,7 +601,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
     };
     // O and dO rows of an item on their way to L2 (short windows: 200 x 225, 12 x 128 0.532 -> 0.478 ms)
     auto prefetch = [&](int it) {
-      const BwdItem w = bwd_item(it, row_tiles, p.H);
+      const BwdItem w = item_at(it);
       const int r = w.tile * TILE + q * 32 + lane;
       if (r < N) {
         const size_t o = (static_cast<size_t>(w.win) * N + r) * p.ldo + w.head * p.d;
@@ -578,7 +622,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
         if (it + AHEAD + 1 < n_items) prefetch(it + AHEAD + 1);
       if constexpr (!DKV)
         if (it + AHEAD < n_items && !statistics(it + AHEAD)) { ok = false; break; }
-      const BwdItem w = bwd_item(it, row_tiles, p.H);
+      const BwdItem w = item_at(it);
       if constexpr (DKV) {
         if (!mbar_wait_warp(&bar->a_full, it & 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
         tc_fence_after();
@@ -611,6 +655,33 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
+    // The bias of an item: entry tab[mine + at[..]] or tab[mine - at[..]] of the table, `tab` and `at` in shared memory or not.
+    const float* tab = nullptr;
+    const int* at = nullptr;
+    int mine = 0;
+    [[maybe_unused]] int head = -1;
+    [[maybe_unused]] uint32_t bias_ph = 0;
+    [[maybe_unused]] auto bias_of = [&](const BwdItem& w) -> bool {
+      if constexpr (BIASED == 1) {
+        if (w.head != head) {       // this warp is through with the table before
+          if (head >= 0) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->bias_empty);
+          }
+          head = w.head;
+          if (!mbar_wait_warp(&bar->bias_full, bias_ph, p.status, ERR_TIMEOUT_ATTN)) return false;
+          bias_ph ^= 1;
+        }
+        tab = s_table;
+        at = reinterpret_cast<const int*>(s_table + p.bias.size);
+      } else {
+        tab = p.bias.table + static_cast<size_t>(w.head) * p.bias.size;
+        at = p.bias.at;
+      }
+      const int place = at[min(w.tile * TILE + row, N - 1)];
+      mine = DKV ? p.bias.zero - place : p.bias.zero + place;
+      return true;
+    };
     // CPT columns to registers
     auto load = [&](uint32_t t, uint32_t (&v)[CPT]) {
 #pragma unroll
@@ -627,16 +698,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
         if (lane == 0) mbar_arrive(&bar->stat_empty[sb.i]);
         sb.next(R::NSB);
         const uint64_t nl = f2_pack(nlse, nlse), nd = f2_pack(ndelta, ndelta);
-        [[maybe_unused]] const float* bias = nullptr;      // of this row: bias[-at[j]]
         [[maybe_unused]] uint64_t left = 0;                // what the row's dS add up to
         [[maybe_unused]] size_t rest_at = 0;
         [[maybe_unused]] bool rest_in = false;
         if constexpr (BIAS) {
-          const BwdItem w = bwd_item(it, row_tiles, p.H);
+          const BwdItem w = item_at(it);
           const int grow = w.tile * TILE + row;
           rest_in = grow < N;
           rest_at = ((static_cast<size_t>(ch * R::WPC + wg % R::WPC) * p.n_win + w.win) * p.H + w.head) * N + grow;
-          bias = p.bias.table + static_cast<size_t>(w.head) * p.bias.size + p.bias.zero + p.bias.at[min(grow, N - 1)];
+          if (!bias_of(w)) { ok = false; break; }
         }
         for (; j < n_str; j += NCH, ph ^= 1) {
           if (!wait(&bar->s_full[ch], ph)) { ok = false; break; }
@@ -649,8 +719,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
               float t0, t1;
               const uint64_t s2 = f2_pack(__uint_as_float(pr[i]), __uint_as_float(pr[i + 1]));
               if constexpr (BIAS) {
-                const int2 a = *reinterpret_cast<const int2*>(p.bias.at + j * BT + c0 + i);
-                f2_unpack(f2_add(f2_fma(s2, sl, f2_pack(bias[-a.x], bias[-a.y])), nl), t0, t1);
+                const int2 a = *reinterpret_cast<const int2*>(at + j * BT + c0 + i);
+                f2_unpack(f2_add(f2_fma(s2, sl, f2_pack(tab[mine - a.x], tab[mine - a.y])), nl), t0, t1);
               } else {
                 f2_unpack(f2_fma(s2, sl, nl), t0, t1);
               }
@@ -687,9 +757,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
               for (int i = 0; i < 8; ++i) {
                 float p0, p1;
                 if constexpr (BIAS) {
-                  const int* at = p.bias.at + j * BT + c0 + c + 2 * i;
-                  p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, bias[-at[0]]) + nlse);
-                  p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, bias[-at[1]]) + nlse);
+                  const int* a = at + j * BT + c0 + c + 2 * i;
+                  p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, tab[mine - a[0]]) + nlse);
+                  p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, tab[mine - a[1]]) + nlse);
                 } else {
                   p0 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, nlse));
                   p1 = mufu_exp2(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, nlse));
@@ -719,14 +789,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       const uint64_t nsl = f2_pack(-p.scale_log2, -p.scale_log2);
       // Columns past the window's end have zero Q and dO rows and zero statistics (P = 1, dS = 0): they add nothing. Rows
       // past its end may hold anything: they are not stored.
-      [[maybe_unused]] const float* bias = nullptr;         // of this row's key: bias[at[i]]
-      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l, [[maybe_unused]] const int* at) -> uint32_t {
+      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l, [[maybe_unused]] int a0, [[maybe_unused]] int a1) -> uint32_t {
         float t0, t1;
         uint64_t x = f2_fma(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), nsl, l);             // -(log2 P)
-        if constexpr (BIAS) {
-          const int2 a = *reinterpret_cast<const int2*>(at);
-          x = f2_sub(x, f2_pack(bias[a.x], bias[a.y]));
-        }
+        if constexpr (BIAS) x = f2_sub(x, f2_pack(tab[mine + a0], tab[mine + a1]));
         f2_unpack(x, t0, t1);
         t0 = fast_exp2(-t0);
         t1 = fast_exp2(-t1);
@@ -741,8 +807,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       int st = ch;
       for (int it = 0; it < n_items && ok; ++it) {
         if constexpr (BIAS) {
-          const BwdItem w = bwd_item(it, row_tiles, p.H);
-          bias = p.bias.table + static_cast<size_t>(w.head) * p.bias.size + p.bias.zero - p.bias.at[min(w.tile * TILE + row, N - 1)];
+          if (!bias_of(item_at(it))) { ok = false; break; }
         }
         for (; j < n_str; j += NCH, ph ^= 1, st = st + NCH >= NST ? st + NCH - NST : st + NCH) {
           if (!wait(&bar->s_full[ch], ph)) { ok = false; break; }
@@ -757,9 +822,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const ulonglong2 l = ls[c / 4 + i];
-                const int* at = BIAS ? p.bias.at + j * BT + c0 + c + 4 * i : nullptr;
-                pp[2 * i] = probs(pr[c + 4 * i], pr[c + 4 * i + 1], l.x, at);
-                pp[2 * i + 1] = probs(pr[c + 4 * i + 2], pr[c + 4 * i + 3], l.y, at + 2);
+                int4 a = {};
+                if constexpr (BIAS) a = *reinterpret_cast<const int4*>(at + j * BT + c0 + c + 4 * i);
+                pp[2 * i] = probs(pr[c + 4 * i], pr[c + 4 * i + 1], l.x, a.x, a.y);
+                pp[2 * i + 1] = probs(pr[c + 4 * i + 2], pr[c + 4 * i + 3], l.y, a.z, a.w);
               }
               tmem_st8(tS + (c >> 1), pp);
             }
@@ -790,9 +856,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const ulonglong2 l = ls[c / 4 + i], de = ds[c / 4 + i];
-                const int* at = BIAS ? p.bias.at + j * BT + c0 + c + 4 * i : nullptr;
-                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x, at);
-                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y, at + 2);
+                int4 a = {};
+                if constexpr (BIAS) a = *reinterpret_cast<const int4*>(at + j * BT + c0 + c + 4 * i);
+                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x, a.x, a.y);
+                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y, a.z, a.w);
                 dd[2 * i] = grad(sv[4 * i], sv[4 * i + 1], dv[4 * i], dv[4 * i + 1], de.x);
                 dd[2 * i + 1] = grad(sv[4 * i + 2], sv[4 * i + 3], dv[4 * i + 2], dv[4 * i + 3], de.y);
               }
@@ -822,34 +889,35 @@ static __global__ void __launch_bounds__(256) attn_delta_rest_kernel(float* delt
     delta[i] += (rest[i] + rest[n + i]) + (rest[2 * n + i] + rest[3 * n + i]);
 }
 
-template <int DCH, bool BIAS = false>
+template <int DCH, int BIASED = 0>
 static int launch_attn_bwd(const CUtensorMap& tq128, const CUtensorMap& tk64, const CUtensorMap& tv64,
                            const CUtensorMap& tdo128, const CUtensorMap& tq64, const CUtensorMap& tk128,
                            const CUtensorMap& tv128, const CUtensorMap& tdo64, const CUtensorMap (&out)[3],
                            const AttnBwdParams& p, cudaStream_t stream) {
-  using R1 = BwdCfg<DCH, false>;
-  using R2 = BwdCfg<DCH, true>;
-  auto k1 = attn_bwd_kernel<DCH, false, BIAS>;
-  auto k2 = attn_bwd_kernel<DCH, true, BIAS>;
-  static bool configured = false;
-  if (!configured) {
-    if (cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, R1::SMEM) != cudaSuccess) return -20;
-    if (cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize, R2::SMEM) != cudaSuccess) return -20;
-    // warpgroups that ask for more registers than the launch holds would wait for ever
-    cudaFuncAttributes f1, f2;
-    if (cudaFuncGetAttributes(&f1, k1) != cudaSuccess || cudaFuncGetAttributes(&f2, k2) != cudaSuccess) return -20;
-    if (f1.numRegs * R1::THREADS < R1::REGS || f2.numRegs * R2::THREADS < R2::REGS) return -24;
-    configured = true;
-  }
+  using R1 = BwdCfg<DCH, false, BIASED>;
+  using R2 = BwdCfg<DCH, true, BIASED>;
+  constexpr int SMEM1 = R1::SMEM + R1::TABLE, SMEM2 = R2::SMEM + R2::TABLE;
+  auto k1 = attn_bwd_kernel<DCH, false, BIASED>;
+  auto k2 = attn_bwd_kernel<DCH, true, BIASED>;
+  static std::atomic<uint64_t> done{0};
+  if (!once_a_device(done, [&] {
+        // warpgroups that ask for more registers than the launch holds would wait for ever
+        cudaFuncAttributes f1, f2;
+        return cudaFuncSetAttribute(k1, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM1) == cudaSuccess &&
+               cudaFuncSetAttribute(k2, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM2) == cudaSuccess &&
+               cudaFuncGetAttributes(&f1, k1) == cudaSuccess && cudaFuncGetAttributes(&f2, k2) == cudaSuccess &&
+               f1.numRegs * R1::THREADS >= R1::REGS && f2.numRegs * R2::THREADS >= R2::REGS;
+      }))
+    return -20;
   const int n = (p.N + TILE - 1) / TILE * p.H * p.n_win, grid = n < num_sms() ? n : num_sms();
-  if (launch_chained(k1, grid, R1::THREADS, R1::SMEM, stream, tq128, tdo128, tk64, tv64, out[0], out[0], p, n)) return -21;
-  if constexpr (BIAS) {
+  if (launch_chained(k1, grid, R1::THREADS, SMEM1, stream, tq128, tdo128, tk64, tv64, out[0], out[0], p, n)) return -21;
+  if constexpr (BIASED != 0) {
     const long long rows = static_cast<long long>(p.n_win) * p.H * p.N, blocks = (rows + 255) / 256, most = 8ll * num_sms();
     if (launch_chained(attn_delta_rest_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, p.delta,
                        static_cast<const float*>(p.rest), rows))
       return -21;
   }
-  return launch_chained(k2, grid, R2::THREADS, R2::SMEM, stream, tk128, tv128, tq64, tdo64, out[1], out[2], p, n) ? -22 : 0;
+  return launch_chained(k2, grid, R2::THREADS, SMEM2, stream, tk128, tv128, tq64, tdo64, out[1], out[2], p, n) ? -22 : 0;
 }
 
 }  // namespace aeris

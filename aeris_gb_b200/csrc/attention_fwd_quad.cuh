@@ -17,13 +17,16 @@
 
 namespace aeris {
 
-struct AttnQuad {
+// BIASED: 0, or scores are biased by relative position (PairBias) from a copy of the head's table in shared memory, for which a
+// stage of the ring makes room (1: 18 KB of table and places) or the second buffers of the query tiles (2: 66 KB).
+template <int BIASED> struct AttnQuad {
   static constexpr int NC = 4;                              // chains
-  static constexpr int NBQ = 2;                             // buffers per chain for its query tile
-  static constexpr int NST = 4;                             // ring of K | V tiles
+  static constexpr int NBQ = BIASED == 2 ? 1 : 2;           // buffers per chain for its query tile
+  static constexpr int NST = BIASED == 1 ? 3 : 4;           // ring of K | V tiles
   static constexpr int Q_BYTES = 16384, HALF = KVT * 128, STAGE = 2 * HALF;
   static constexpr int OUT_BYTES = 2048;                    // per softmax warp: 32 rows x 32 columns
   static constexpr int SMEM = NC * NBQ * Q_BYTES + NST * STAGE + 4 * NC * OUT_BYTES + 512;
+  static constexpr int TABLE = BIASED ? 227 * 1024 - SMEM : 0;     // room for a table and the places
   // tensor memory, per chain: scores, over them P, then O
   static constexpr int COLS = 128, COL_O = 64;
   // warps: softmax, four per chain; loads; an issuer for two chains each; one without work
@@ -32,7 +35,7 @@ struct AttnQuad {
   static constexpr int REGS_SOFTMAX = 104, REGS_REST = 64;
   static constexpr int REGS = 32 * (4 * NC * REGS_SOFTMAX + 4 * REGS_REST);
 };
-static_assert(AttnQuad::SMEM <= 227 * 1024, "shared memory");
+static_assert(AttnQuad<0>::SMEM <= 227 * 1024, "shared memory");
 
 struct QuadBars {
   uint64_t q_full[4][2], q_empty[4][2];
@@ -40,15 +43,28 @@ struct QuadBars {
   uint64_t s_full[4];                   // the chain's scores are in tensor memory
   uint64_t p_full[4];                   // its probabilities have taken their place
   uint64_t o_full[4];                   // the last P V of an item has completed
+  uint64_t bias_full, bias_empty;       // a head's table is there; no softmax warp needs it any more
 };
 static_assert(sizeof(QuadBars) + 8 + 4 * 16 <= 512, "barriers");
 
-__global__ void __launch_bounds__(AttnQuad::THREADS, 1)
+// Items with a bias: the windows of a head one behind the other and a run of them for each CTA, so that it loads one table or two.
+__device__ __forceinline__ PairItem bias_item(int idx, int n_groups, int n_win) {
+  const int hw = idx / n_groups;
+  PairItem b;
+  b.pair = idx - hw * n_groups;
+  b.head = hw / n_win;
+  b.win = hw - b.head * n_win;
+  return b;
+}
+
+template <int BIASED>
+__global__ void __launch_bounds__(AttnQuad<BIASED>::THREADS, 1)
 attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                      const AttnFwdParams p, const int n_items_total) {
-  using R = AttnQuad;
+  using R = AttnQuad<BIASED>;
   constexpr int NC = R::NC, NBQ = R::NBQ, NST = R::NST;
+  constexpr bool BIAS = BIASED != 0;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                               // [chains][NBQ]
   uint8_t* sT = sQ + NC * NBQ * R::Q_BYTES;         // [NST] K | V
@@ -57,6 +73,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_failed = s_abort + 1;      // [16] see note_failure
+  [[maybe_unused]] const float* s_table = reinterpret_cast<const float*>(smem + R::SMEM);      // [p.bias.size], then places
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int N = p.N;
@@ -66,8 +83,17 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   // an item: up to four query tiles of one (window, head); see pair_item
   const int q_tiles = (N + TILE - 1) / TILE, n_groups = (q_tiles + NC - 1) / NC;
   const int n_ctas = static_cast<int>(gridDim.x);
-  const int n_items = (n_items_total - static_cast<int>(blockIdx.x) + n_ctas - 1) / n_ctas;
+  int n_items = (n_items_total - static_cast<int>(blockIdx.x) + n_ctas - 1) / n_ctas;
+  [[maybe_unused]] int item0 = 0;
+  if constexpr (BIAS) {
+    item0 = static_cast<int>(static_cast<long long>(n_items_total) * blockIdx.x / n_ctas);
+    n_items = static_cast<int>(static_cast<long long>(n_items_total) * (blockIdx.x + 1) / n_ctas) - item0;
+  }
   const int total = n_items * nkv;
+  auto item_at = [&](int it) -> PairItem {
+    if constexpr (BIAS) return bias_item(item0 + it, n_groups, p.n_win);
+    else return pair_item(it, n_groups, p.H);
+  };
 
   if (threadIdx.x == 0) {
     int ab = (p.status && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
@@ -83,6 +109,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&bar->s_full[c], 1); mbar_init(&bar->p_full[c], 4); mbar_init(&bar->o_full[c], 1);
     }
     for (int i = 0; i < NST; ++i) { mbar_init(&bar->t_full[i], 1); mbar_init(&bar->t_empty[i], 2); }
+    if constexpr (BIAS) { mbar_init(&bar->bias_full, 1); mbar_init(&bar->bias_empty, 4 * NC); }
     fence_barrier_init();
   }
   if (warp == R::W_LOAD) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
@@ -98,7 +125,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       // ---------------------------------------------------------- TMA producer
       Slot qs[NC];
       auto load_q = [&](int it) -> bool {
-        const PairItem w = pair_item(it, n_groups, p.H);
+        const PairItem w = item_at(it);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int qt = NC * w.pair + c;
@@ -113,10 +140,29 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         return true;
       };
+      // The table of a head, once the softmax warps are through with the one before; with the first the tokens' places.
+      [[maybe_unused]] int head = -1;
+      [[maybe_unused]] uint32_t bias_ph = 0;
+      [[maybe_unused]] auto load_table = [&](const PairItem& w) -> bool {
+        if (w.head == head) return true;
+        if (head >= 0) {
+          if (!mbar_wait_warp(&bar->bias_empty, bias_ph, p.status, ERR_TIMEOUT_ATTN)) return false;
+          bias_ph ^= 1;
+        }
+        if (lane == 0) {
+          const uint32_t bytes = p.bias.size * 4, at_bytes = head < 0 ? (N + 127) / 128 * 512 : 0;
+          mbar_expect_tx(&bar->bias_full, bytes + at_bytes);
+          bulk_load(smem + R::SMEM, p.bias.table + static_cast<size_t>(w.head) * p.bias.size, bytes, &bar->bias_full);
+          if (at_bytes) bulk_load(smem + R::SMEM + bytes, p.bias.at, at_bytes, &bar->bias_full);
+        }
+        head = w.head;
+        return true;
+      };
       bool ok = load_q(0);
       Slot ts;
       for (int it = 0; it < n_items && ok; ++it) {
-        const PairItem w = pair_item(it, n_groups, p.H);
+        const PairItem w = item_at(it);
+        if constexpr (BIAS) ok = load_table(w);
         for (int j = 0; j < nkv && ok; ++j) {
           ok = mbar_wait_warp(&bar->t_empty[ts.i], ts.ph ^ 1, p.status, ERR_TIMEOUT_ATTN);
           if (ok && lane == 0) {
@@ -127,8 +173,8 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             tma_load_4d(d + R::HALF, &tm_v, full, 0, w.head, j * KVT, w.win);
           }
           ts.next(NST);
-          // the query tiles of the next item, early in this one
-          if (ok && j == min(2, nkv - 1) && it + 1 < n_items) ok = load_q(it + 1);
+          // the query tiles of the next item, early in this one; with one buffer behind this one's last tile
+          if (ok && j == (NBQ == 1 ? nkv - 1 : min(2, nkv - 1)) && it + 1 < n_items) ok = load_q(it + 1);
         }
       }
     } else if (warp < R::W_ISSUE + 2) {
@@ -144,7 +190,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       constexpr uint32_t B_TEMPTY = offsetof(QuadBars, t_empty) - offsetof(QuadBars, t_full),
                          B_QEMPTY = offsetof(QuadBars, q_empty) - offsetof(QuadBars, q_full),
                          B_OFULL = offsetof(QuadBars, o_full) - offsetof(QuadBars, s_full);
-      auto chains = [&](int it) { return min(NC, q_tiles - NC * pair_item(it, n_groups, p.H).pair) - c0; };
+      auto chains = [&](int it) { return min(NC, q_tiles - NC * item_at(it).pair) - c0; };
       Slot qs[2];                       // query buffers of the two chains
       uint32_t p_ph[2] = {};
       // S = Q K^T of ring slot `slot` for chain u
@@ -219,7 +265,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     // through shared memory.
     auto epilogue = [&](const PairItem& w) {
       const int tile_row = (NC * w.pair + c) * TILE + q * 32, grow = tile_row + lane;
-      const float inv = 1.f / l;
+      const float inv = BIAS && l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* pdst = nullptr;
       if (p.push_n_local > 0 && grow < N) {
         const int owner = grow / p.push_n_local;
@@ -250,16 +296,17 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (lane == 0 && p.O) tma_store_4d(&tm_o, stage, col, w.head, tile_row, w.win);
         __syncwarp();
       }
-      if (p.lse && grow < N) p.lse[(static_cast<size_t>(w.win) * p.H + w.head) * N + grow] = m_ref + log2f(l);
+      if (p.lse && grow < N)
+        p.lse[(static_cast<size_t>(w.win) * p.H + w.head) * N + grow] = BIAS && l == 0.f ? INFINITY : m_ref + log2f(l);
       __syncwarp();
     };
     // The reference maximum is raised when a row's maximum grows by more than 2^8; these scores were issued behind the P V
     // of the tile before, so the accumulator is up to date.
     auto raise = [&](int j, float mx) {
-      const float m_new = fmaxf(m_ref, mx * sl2);
+      const float m_new = fmaxf(m_ref, BIAS ? mx : mx * sl2);
       if (__any_sync(0xffffffffu, m_new - m_ref > RESCALE_LOG2)) {
         if (j > 0) {
-          const float alpha = fast_exp2(m_ref - m_new);
+          const float alpha = BIAS && m_new == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
           rescale_tmem_rows(tO, 64, alpha);
           l *= alpha;
         }
@@ -268,11 +315,28 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     };
     bool pending = false;               // `prev` has rows that are still in tensor memory
     PairItem prev{0, 0, 0};
+    [[maybe_unused]] int head = -1;
+    [[maybe_unused]] uint32_t bias_ph = 0;
+    [[maybe_unused]] const int* s_at = reinterpret_cast<const int*>(s_table + p.bias.size);
     for (int it = 0; it < n_items && ok; ++it) {
-      const PairItem w = pair_item(it, n_groups, p.H);
+      const PairItem w = item_at(it);
+      if constexpr (BIAS) {
+        if (w.head != head) {       // the warp is through with the table before
+          if (head >= 0) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->bias_empty);
+          }
+          head = w.head;
+          ok = mbar_wait_warp(&bar->bias_full, bias_ph, p.status, ERR_TIMEOUT_ATTN);
+          if (!ok) break;
+          bias_ph ^= 1;
+        }
+      }
       const int qt = NC * w.pair + c;
       if (qt >= q_tiles) continue;
       const bool rows = qt * TILE + q * 32 < N;
+      [[maybe_unused]] int mine = 0;          // entry of this row's query and a key at place 0
+      if constexpr (BIAS) mine = p.bias.zero + s_at[min(qt * TILE + q * 32 + lane, N - 1)];
       for (int j = 0; j < nkv; ++j) {
         ok = mbar_wait_warp(&bar->s_full[c], s_ph, p.status, ERR_TIMEOUT_ATTN);
         if (!ok) break;
@@ -292,6 +356,23 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           tmem_ld32(tS, v[0]);
           tmem_ld32(tS + 32, v[1]);
           tmem_wait_ld();
+          if constexpr (BIAS) {
+            const int4* at = reinterpret_cast<const int4*>(s_at + j * KVT);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int4 a = at[i];
+              uint32_t* x = &v[i >> 3][4 * (i & 7)];
+              float b0, b1, b2, b3;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(x[0]), __uint_as_float(x[1])), sl,
+                               f2_pack(s_table[mine - a.x], s_table[mine - a.y])), b0, b1);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2]), __uint_as_float(x[3])), sl,
+                               f2_pack(s_table[mine - a.z], s_table[mine - a.w])), b2, b3);
+              x[0] = __float_as_uint(b0);
+              x[1] = __float_as_uint(b1);
+              x[2] = __float_as_uint(b2);
+              x[3] = __float_as_uint(b3);
+            }
+          }
           float mx[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(v[0][k]), __uint_as_float(v[1][k]));
@@ -301,10 +382,11 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(v[0][i + k]), __uint_as_float(v[1][i + k]));
           }
           raise(j, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]));
-          const uint64_t nm = f2_pack(-m_ref, -m_ref);
+          const float m_now = BIAS && m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t nm = f2_pack(-m_now, -m_now), su = BIAS ? f2_pack(1.f, 1.f) : sl;
           HalfSum sum;
-          softmax_chunk<false>(v[0], sl, nm, sum, tS);          // over columns that have been read
-          softmax_chunk<false>(v[1], sl, nm, sum, tS + 16);
+          softmax_chunk<false>(v[0], su, nm, sum, tS);          // over columns that have been read
+          softmax_chunk<false>(v[1], su, nm, sum, tS + 16);
           l += sum.total(false);
           tmem_wait_st();
         } else {
@@ -316,11 +398,15 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             tmem_ld16(tS + k, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (k + i < rem) mx = fmaxf(mx, __uint_as_float(v[i]));
+            for (int i = 0; i < 16; ++i) {
+              float s = __uint_as_float(v[i]);
+              if constexpr (BIAS) s = fmaf(s, sl2, s_table[mine - s_at[j * KVT + k + i]]);
+              if (k + i < rem) mx = fmaxf(mx, s);
+            }
           }
           raise(j, mx);
           float rs = 0.f;
+          [[maybe_unused]] const float m_now = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll 1
           for (int k = 0; k < n_last; k += 16) {
             uint32_t v[16], pk[8];
@@ -328,8 +414,15 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              float p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, -m_ref));
-              float p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -m_ref));
+              float p0, p1;
+              if constexpr (BIAS) {
+                const int* at = s_at + j * KVT + k + 2 * i;
+                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, s_table[mine - at[0]]) - m_now);
+                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, s_table[mine - at[1]]) - m_now);
+              } else {
+                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, -m_ref));
+                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -m_ref));
+              }
               if (k + 2 * i >= rem) p0 = 0.f;
               if (k + 2 * i + 1 >= rem) p1 = 0.f;
               rs += p0 + p1;
@@ -359,25 +452,25 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (warp == R::W_LOAD) tmem_dealloc(tmem_base, 512);
 }
 
+template <int BIASED = 0>
 static int launch_attn_fwd_quad(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                 const CUtensorMap& to, const AttnFwdParams& p, cudaStream_t stream) {
-  using R = AttnQuad;
-  static bool configured = false;
-  if (!configured) {
-    if (cudaFuncSetAttribute(attn_fwd_quad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM) != cudaSuccess)
-      return -20;
-    // warpgroups that ask for more registers than the launch holds would wait for ever
-    cudaFuncAttributes f;
-    if (cudaFuncGetAttributes(&f, attn_fwd_quad_kernel) != cudaSuccess) return -20;
-    if (f.numRegs * R::THREADS < R::REGS) return -24;
-    configured = true;
-  }
+  using R = AttnQuad<BIASED>;
+  static std::atomic<uint64_t> done{0};
+  auto kern = attn_fwd_quad_kernel<BIASED>;
+  if (!once_a_device(done, [&] {
+        // warpgroups that ask for more registers than the launch holds would wait for ever
+        cudaFuncAttributes f;
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM + R::TABLE) == cudaSuccess &&
+               cudaFuncGetAttributes(&f, kern) == cudaSuccess && f.numRegs * R::THREADS >= R::REGS;
+      }))
+    return -20;
   const int groups = ((p.N + TILE - 1) / TILE + R::NC - 1) / R::NC;
   const long long items = static_cast<long long>(groups) * p.H * p.n_win;
   const int nkv = (p.N + KVT - 1) / KVT;
   if (items > 0x3fffffff || items * nkv > 0x3fffffffll * num_sms()) return -23;
   const int n = static_cast<int>(items), grid = n < num_sms() ? n : num_sms();
-  return launch_chained(attn_fwd_quad_kernel, grid, R::THREADS, R::SMEM, stream, tq, tk, tv, to, p, n);
+  return launch_chained(kern, grid, R::THREADS, R::SMEM + R::TABLE, stream, tq, tk, tv, to, p, n);
 }
 
 }  // namespace aeris

@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #ifndef AERIS_WAIT_TIMEOUT_NS
 #define AERIS_WAIT_TIMEOUT_NS 2000000000ull  // 2 s per wait, far above any legitimate tile time
 #endif
@@ -195,6 +197,12 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
+// Untiled copy into shared memory: both addresses on 16-byte boundaries, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1,
                                             int c2, int c3) {
   asm volatile(
@@ -265,6 +273,22 @@ template <typename... P, typename... A>
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
   return cudaGetLastError() == cudaSuccess ? 0 : -21;
+}
+
+// What has to be done once for a kernel on every device, such as allowing it its shared memory: `done` has a bit for each.
+template <typename F> static inline bool once_a_device(std::atomic<uint64_t>& done, F&& f) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (!f()) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+template <typename K> static inline bool allow_smem_once(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  return once_a_device(done, [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  });
 }
 
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {  // whole warp

@@ -364,8 +364,8 @@ template <int BN, int A_MN, int B_MN>
 int launch_lin(const void* A, long long lda, const void* B, long long ldb, LinParams p, cudaStream_t stream) {
   using S = LinSmem<BN>;
   auto kern = lin_kernel<BN, A_MN, B_MN>;
-  // asked for on every launch, for the attribute belongs to the device at hand
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL) != cudaSuccess) return -20;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem_once(kern, S::TOTAL, done)) return -20;
   CUtensorMap ta, tb, ty, tz;
   int r;
   if (!whole_rows(A, lda) || !whole_rows(B, ldb)) return -11;

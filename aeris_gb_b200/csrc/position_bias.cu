@@ -4,14 +4,14 @@
 //   s_ij = scale q_i k_j + table[bucket(pos_i - pos_j), head], p = softmax_j(s), o = p v
 //   ds = p (dp - delta), dp = dO v^T, delta = rowsum(p dp);  dtable[b, head] = sum of ds over windows and the pairs of bucket b
 //
-// The bias of a pair is a function of the difference of two tokens' places: with at(t) = y (2 wide - 1) + x it is entry
+// The bias of a pair is a function of the difference of two tokens' places: with at(t) = y pitch + x it is entry
 // at(i) - at(j) + at(last) of a table by relative position, which is all that the attention kernels read: one table of
-// (2 high - 1)(2 wide - 1) floats for a head, whatever the buckets, in log2 units, instead of an N x N matrix.
+// (2 high - 1) rows of `pitch` floats for a head, whatever the buckets, in log2 units, instead of an N x N matrix. The pitch is the
+// least from 2 wide - 1 on that is `wide` more than a multiple of 32: from one token to the next `at` then grows by one
+// modulo 32 even where a row of the window ends, and 32 queries read 32 banks of shared memory.
 #include "common.cuh"
 #include "api.h"
 #include "host.h"
-
-#include <atomic>
 
 namespace aeris {
 
@@ -21,59 +21,82 @@ constexpr float HIDDEN = -1e30f;
 constexpr int PB_TILE = 128;
 
 struct Place {
-  int n, off;         // tokens of a window, relative positions
+  int n;              // tokens of a window
+  int pitch, zero;    // of the table's rows; entry of a token and itself
+  int size;           // floats from one head's table to the next: whole vectors
   int at_words;       // `at`, up to the next multiple of 128 behind the window's end
 };
 Place place_of(int high, int wide) {
   Place p;
   p.n = high * wide;
-  p.off = (2 * high - 1) * (2 * wide - 1);
+  p.pitch = wide + (wide - 1 + 31) / 32 * 32;
+  p.zero = (high - 1) * p.pitch + wide - 1;
+  p.size = ((2 * high - 1) * p.pitch + 3) / 4 * 4;
   p.at_words = (p.n + 127) / 128 * 128;
   return p;
 }
 
-// The table by relative position [heads, off] in log2 units, and the places of the tokens.
-__global__ void __launch_bounds__(256) bias_expand_kernel(const AerisBiasedAttn a, float* out, int* at, int n, int off, int at_words) {
+// The tables by relative position [heads, size] in log2 units, and the places of the tokens.
+__global__ void __launch_bounds__(256) bias_expand_kernel(const AerisBiasedAttn a, float* out, int* at, const Place pl) {
   chain_point();
   const int i = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
-  if (i < off) {
-    long long b = i;
-    if (a.buckets)
-      b = a.buckets64 ? static_cast<const long long*>(a.buckets)[i] : static_cast<const int*>(a.buckets)[i];
-    float v = -INFINITY;
-    if (b >= 0 && b < a.table_rows) {
-      const long long k = b * a.heads + head;
-      v = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[k]) : static_cast<const float*>(a.table)[k];
-      v = v <= HIDDEN ? -INFINITY : v * 1.4426950408889634f;
-    } else if (a.status) {
-      atomicCAS(a.status, 0, ERR_BOUNDS);
+  if (i < pl.size) {
+    const int r = i / pl.pitch, c = i - r * pl.pitch;
+    float v = 0.f;                // between the rows: not read
+    if (r < 2 * a.high - 1 && c < 2 * a.wide - 1) {
+      const int k = r * (2 * a.wide - 1) + c;
+      long long b = k;
+      if (a.buckets)
+        b = a.buckets64 ? static_cast<const long long*>(a.buckets)[k] : static_cast<const int*>(a.buckets)[k];
+      if (b >= 0 && b < a.table_rows) {
+        const long long e = b * a.heads + head;
+        v = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e]) : static_cast<const float*>(a.table)[e];
+        v = v <= HIDDEN ? -INFINITY : v * 1.4426950408889634f;
+      } else {
+        v = -INFINITY;
+        if (a.status) atomicCAS(a.status, 0, ERR_BOUNDS);
+      }
     }
-    out[static_cast<long long>(head) * off + i] = v;
+    out[static_cast<long long>(head) * pl.size + i] = v;
   }
-  if (head == 0 && i < at_words) {
-    const int t = i < n ? i : n - 1, y = t / a.wide;
-    at[i] = y * (2 * a.wide - 1) + t - y * a.wide;
+  if (head == 0 && i < pl.at_words) {
+    const int t = i < pl.n ? i : pl.n - 1, y = t / a.wide;
+    at[i] = y * pl.pitch + t - y * a.wide;
   }
 }
 
 // ------------------------------------------------------------------------------------------ sums of dS over windows
-// One CTA = a 128 x TK tile of (query, key) of one head. It goes over its windows: S = Q K^T and dP = dO V^T into TMEM, two
-// buffers in turn, and adds p (dp - delta) to sums that stay in registers; the bias of its pairs stays there too. No atomics: slices of
-// the windows have sums of their own, which bias_sums_kernel adds in their order.
+// A tile is 128 queries x TK keys of one head, taken through all windows: S = Q K^T and dP = dO V^T of one window and the next
+// into TMEM in turn, while p (dp - delta) of the one before is added up in registers. CTAs take whole tiles in rounds, all of them
+// window after window at the same time, so that tiles of a head find their operands in L2 (runs of tiles that start in
+// different windows, 128 x 256: 1.19 ms where rounds took 0.88). The windows of the tiles that are left for the last round are one sequence
+// of steps, of which every CTA takes a run: no atomics, and no round of a few tiles. A tile whose last window is in a CTA's run is
+// written to its place, what goes on in the next CTA's to `extra`, which bias_join_kernel adds.
+//
+// With p = 2^(c s + b - lse) the bias b of a pair is the same for all windows: 2^(c s - lse) (dp - delta) is added up and the sum
+// multiplied by 2^b at the end, where every pair of a warp's is visible and |b| is at most 64; else b is added to every score.
+//
+// What bounds it is the operands' way from L2, 64 KB a window: loads and products alone take 0.62 of the 0.75 ms (72 windows of 30 x 30, 24
+// heads of 64), 11 TB/s; the exponentials of a window take 1,024 cycles. Tiles of 128 x 256 read 48 KB for 128 x 128, but two
+// windows' operands fill the shared memory then: 0.69 ms of loads alone, 0.88 in all.
 template <int DCH> struct BgCfg {
   static constexpr int TK = DCH == 1 ? 128 : 64, CPT = TK / 4;
-  static constexpr int QB = DCH * 16384, KB = DCH * TK * 128, STAGE = 2 * QB + 2 * KB, NST = DCH == 1 ? 3 : 2;
-  static constexpr int MATH = 16, THREADS = 64 + 32 * MATH;
-  static constexpr int TMEM = 4 * TK, SMEM = NST * STAGE + 256 + 1024;
+  static constexpr int QB = DCH * 16384, KB = DCH * TK * 128;
+  static constexpr int NST = DCH == 1 ? 3 : 2, STAGE = 2 * QB + 2 * KB;      // ring of Q | dO | K | V
+  // warps: math, loads, products, two without work; registers: together what 640 threads are launched with (96 each)
+  static constexpr int MATH = 16, W_LOAD = MATH, W_MMA = MATH + 1, THREADS = 32 * (MATH + 4);
+  static constexpr int REGS_MATH = 104, REGS_REST = 64, REGS = 32 * (MATH * REGS_MATH + 4 * REGS_REST);
+  static constexpr int BARS = NST * STAGE, TMEM = 4 * TK, SMEM = BARS + 256 + 1024;
+  static constexpr int TILE_FLOATS = PB_TILE * TK;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct BgParams {
   const float *lse, *delta, *table;
   const int* at;
-  float* part;                // [splits, heads at hand, n, ld]
+  float *part, *extra;        // [heads at hand, n, ld]; [CTAs, 128, TK]
   long long ld;
-  int n, heads, n_win, off, zero, head0, n_heads, splits;
+  int n, heads, n_win, size, zero, head0, n_heads;
   float scale_log2;
   int* status;
 };
@@ -84,15 +107,59 @@ __device__ __forceinline__ float bg_exp2(float x) {
   return y;
 }
 
+struct BgTile {
+  int head, ti, tj;           // head: of those at hand
+};
+__device__ __forceinline__ BgTile bg_tile(long long t, int n, int tk) {
+  const int nj = (n + tk - 1) / tk, ni = (n + PB_TILE - 1) / PB_TILE;
+  BgTile b;
+  b.tj = static_cast<int>(t % nj);
+  const long long r = t / nj;
+  b.ti = static_cast<int>(r % ni);
+  b.head = static_cast<int>(r / ni);
+  return b;
+}
+// First step of CTA b of g, of `steps` in all.
+__host__ __device__ __forceinline__ long long bg_first(long long steps, int b, int g) { return steps * b / g; }
+
+// What a CTA does, piece by piece: windows [w0, w1) of tile t.
+struct BgWork {
+  long long t, u, u1, last_round;
+  int w0, w1, n_win;
+  __device__ __forceinline__ BgWork(long long tiles, int n_win_) : n_win(n_win_) {
+    last_round = tiles / gridDim.x * gridDim.x;
+    t = static_cast<long long>(blockIdx.x) - gridDim.x;
+    const long long steps = (tiles - last_round) * n_win;
+    u = bg_first(steps, blockIdx.x, gridDim.x);
+    u1 = bg_first(steps, blockIdx.x + 1, gridDim.x);
+  }
+  __device__ __forceinline__ bool next() {
+    if (t + gridDim.x < last_round) {
+      t += gridDim.x;
+      w0 = 0;
+      w1 = n_win;
+      return true;
+    }
+    if (u >= u1) return false;
+    const long long r = u / n_win;
+    t = last_round + r;
+    w0 = static_cast<int>(u - r * n_win);
+    w1 = static_cast<int>(min(static_cast<long long>(n_win), w0 + u1 - u));
+    u += w1 - w0;
+    return true;
+  }
+};
+
 template <int DCH>
 __global__ void __launch_bounds__(BgCfg<DCH>::THREADS, 1)
 bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-                 const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BgParams p) {
+                 const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BgParams p,
+                 const long long tiles) {
   using C = BgCfg<DCH>;
   constexpr int TK = C::TK, CPT = C::CPT, NST = C::NST;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + NST * C::STAGE);     // [NST]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);     // [NST]
   uint64_t* empty = full + NST;
   uint64_t* s_full = empty + NST;       // [2]
   uint64_t* s_empty = s_full + 2;       // [2]
@@ -104,144 +171,217 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     __syncthreads();
     if (s_abort) { chain_point(); return; }
   }
-  const int ti = blockIdx.x, tj = blockIdx.y, split = blockIdx.z / p.n_heads, hl = blockIdx.z - split * p.n_heads;
-  const int head = p.head0 + hl, per = (p.n_win + p.splits - 1) / p.splits;
-  const int w0 = split * per, w1 = min(p.n_win, w0 + per);
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q); prefetch_tmap(&tm_do); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v);
     for (int i = 0; i < NST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], C::MATH); }
     fence_barrier_init();
   }
-  if (warp == 1) { tmem_alloc(tmem_slot, C::TMEM); tmem_relinquish(); }
+  if (warp == C::W_MMA) { tmem_alloc(tmem_slot, C::TMEM); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   chain_point();
 
-  if (warp == 0) {
+  if (warp >= C::MATH) regs_dec<C::REGS_REST>();
+  if (warp == C::W_LOAD) {
     if (elect_one_sync()) {
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int w = w0; w < w1; ++w) {
-        if (!mbar_wait(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
-        uint8_t* s = smem + st * C::STAGE;
-        mbar_expect_tx(&full[st], C::STAGE);
+      for (BgWork k(tiles, p.n_win); ok && k.next();) {
+        const BgTile b = bg_tile(k.t, p.n, TK);
+        const int head = p.head0 + b.head;
+        for (int w = k.w0; w < k.w1; ++w) {
+          if (!mbar_wait_poll(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
+          uint8_t* s = smem + st * C::STAGE;
+          mbar_expect_tx(&full[st], C::STAGE);
 #pragma unroll
-        for (int c = 0; c < DCH; ++c) {
-          tma_load_4d(s + c * 16384, &tm_q, &full[st], c * 64, head, ti * PB_TILE, w);
-          tma_load_4d(s + 2 * C::QB + c * (TK * 128), &tm_k, &full[st], c * 64, head, tj * TK, w);
-          tma_load_4d(s + C::QB + c * 16384, &tm_do, &full[st], c * 64, head, ti * PB_TILE, w);
-          tma_load_4d(s + 2 * C::QB + C::KB + c * (TK * 128), &tm_v, &full[st], c * 64, head, tj * TK, w);
+          for (int c = 0; c < DCH; ++c) {
+            tma_load_4d(s + c * 16384, &tm_q, &full[st], c * 64, head, b.ti * PB_TILE, w);
+            tma_load_4d(s + 2 * C::QB + c * (TK * 128), &tm_k, &full[st], c * 64, head, b.tj * TK, w);
+            tma_load_4d(s + C::QB + c * 16384, &tm_do, &full[st], c * 64, head, b.ti * PB_TILE, w);
+            tma_load_4d(s + 2 * C::QB + C::KB + c * (TK * 128), &tm_v, &full[st], c * 64, head, b.tj * TK, w);
+          }
+          if (++st == NST) { st = 0; ph ^= 1; }
         }
-        if (++st == NST) { st = 0; ph ^= 1; }
       }
       for (int i = 0; i < NST && ok; ++i) {      // every stage has been released: no copy is under way at exit
-        ok = mbar_wait(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN);
+        ok = mbar_wait_poll(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN);
         if (++st == NST) { st = 0; ph ^= 1; }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == C::W_MMA) {
     if (elect_one_sync()) {
       constexpr uint32_t idesc = make_idesc_bf16(PB_TILE, TK, 0, 0);
       int st = 0, buf = 0;
-      uint32_t ph = 0, bph = 0;
-      for (int w = w0; w < w1; ++w) {
-        if (!mbar_wait(&s_empty[buf], bph ^ 1, p.status, ERR_TIMEOUT_ATTN)) break;
-        if (!mbar_wait(&full[st], ph, p.status, ERR_TIMEOUT_ATTN)) break;
-        tc_fence_after();
-        const uint32_t s = smem_u32(smem + st * C::STAGE), t = tmem_base + buf * 2 * TK;
+      uint32_t ph = 0, b_ph = 0;
+      bool ok = true;
+      for (BgWork k(tiles, p.n_win); ok && k.next();) {
+        for (int w = k.w0; w < k.w1; ++w) {
+          ok = mbar_wait_poll(&s_empty[buf], b_ph ^ 1, p.status, ERR_TIMEOUT_ATTN) &&
+               mbar_wait_poll(&full[st], ph, p.status, ERR_TIMEOUT_ATTN);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t s = smem_u32(smem + st * C::STAGE), d = tmem_base + buf * 2 * TK;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int kk = 0; kk < 4 * DCH; ++kk)
-            umma_ss(t + m * TK, make_smem_desc(s + m * C::QB + (kk >> 2) * 16384 + (kk & 3) * 32, 0, 1024),
-                    make_smem_desc(s + 2 * C::QB + m * C::KB + (kk >> 2) * (TK * 128) + (kk & 3) * 32, 0, 1024), idesc, kk > 0);
-        tc_commit(&empty[st]);
-        tc_commit(&s_full[buf]);
-        if (++st == NST) { st = 0; ph ^= 1; }
-        if (++buf == 2) { buf = 0; bph ^= 1; }
+            for (int kk = 0; kk < 4 * DCH; ++kk)
+              umma_ss(d + m * TK, make_smem_desc(s + m * C::QB + (kk >> 2) * 16384 + (kk & 3) * 32, 0, 1024),
+                      make_smem_desc(s + 2 * C::QB + m * C::KB + (kk >> 2) * (TK * 128) + (kk & 3) * 32, 0, 1024), idesc, kk > 0);
+          tc_commit(&empty[st]);
+          tc_commit(&s_full[buf]);
+          if (++st == NST) { st = 0; ph ^= 1; }
+          if (++buf == 2) { buf = 0; b_ph ^= 1; }
+        }
       }
     }
-  } else {
-    const int q = warp & 3, g = (warp - 2) >> 2;
-    const int row = ti * PB_TILE + q * 32 + lane, col = tj * TK + g * CPT;      // of this thread's sums
-    const bool in = row < p.n;
+  } else if (warp < C::MATH) {
+    regs_inc<C::REGS_MATH>();
+    const int q = warp & 3, g = warp >> 2;
     const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + g * CPT;
-    float bias[CPT], sum[CPT];
-    {
-      const float* b = p.table + static_cast<long long>(head) * p.off + p.zero + p.at[in ? row : p.n - 1];
-#pragma unroll
-      for (int i = 0; i < CPT; ++i) {
-        bias[i] = col + i < p.n ? b[-p.at[col + i]] : -INFINITY;
-        sum[i] = 0.f;
-      }
-    }
-    const long long base = static_cast<long long>(head) * p.n + (in ? row : 0), step = static_cast<long long>(p.heads) * p.n;
+    const uint64_t sl = f2_pack(p.scale_log2, p.scale_log2);
+    const long long stat_step = static_cast<long long>(p.heads) * p.n;
     int buf = 0;
-    uint32_t bph = 0;
+    uint32_t b_ph = 0;
     bool ok = true;
-    float lse = w0 < w1 ? p.lse[base + w0 * step] : 0.f, delta = w0 < w1 ? p.delta[base + w0 * step] : 0.f;
-    for (int w = w0; w < w1; ++w) {
-      const float l = lse, d = delta;
-      if (w + 1 < w1) {
-        lse = p.lse[base + (w + 1) * step];
-        delta = p.delta[base + (w + 1) * step];
-      }
-      if (!mbar_wait_warp(&s_full[buf], bph, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
-      tc_fence_after();
+    for (BgWork work(tiles, p.n_win); ok && work.next();) {
+      const int w1 = work.w1;
+      int w = work.w0;
+      const BgTile b = bg_tile(work.t, p.n, TK);
+      const int row0 = b.ti * PB_TILE + q * 32, row = row0 + lane, col = b.tj * TK + g * CPT;
+      const bool in = row < p.n, has = row0 < p.n && col < p.n;       // has: some of this warp's pairs are in the window
+      const float* bias = p.table + static_cast<long long>(p.head0 + b.head) * p.size + p.zero + p.at[in ? row : p.n - 1];    // bias[-at[j]]
+      uint64_t sum[CPT / 2];
+      bool near = true;
 #pragma unroll
-      for (int c = 0; c < CPT; c += 16) {
-        uint32_t s[16], dp[16];
-        tmem_ld16(t0 + buf * 2 * TK + c, s);
-        tmem_ld16(t0 + buf * 2 * TK + TK + c, dp);
-        tmem_wait_ld();
-        if (c + 16 == CPT) {
-          tc_fence_before();
+      for (int i = 0; i < CPT / 2; ++i) sum[i] = 0ull;
+      if (has)
+#pragma unroll 4
+        for (int i = 0; i < CPT; ++i) near = near && fabsf(bias[-p.at[min(col + i, p.n - 1)]]) <= 64.f;       // no NaN either
+      near = __all_sync(0xffffffffu, near);
+      const long long stat = static_cast<long long>(p.head0 + b.head) * p.n + (in ? row : p.n - 1);
+      float lse = p.lse[stat + w * stat_step], delta = p.delta[stat + w * stat_step];
+      // 16 columns from column c on
+      auto add = [&](const uint32_t (&s)[16], const uint32_t (&dp)[16], uint64_t nl, uint64_t nd, int c, bool with_bias) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          uint64_t e = f2_fma(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sl, nl);
+          if (with_bias) {          // the places go on behind the window's end
+            const int2 a = *reinterpret_cast<const int2*>(p.at + col + c + i);
+            e = f2_add(e, f2_pack(bias[-a.x], bias[-a.y]));
+          }
+          float e0, e1;
+          f2_unpack(e, e0, e1);
+          const uint64_t d = f2_add(f2_pack(__uint_as_float(dp[i]), __uint_as_float(dp[i + 1])), nd);
+          const int k = (c + i) / 2;
+          sum[k] = f2_fma(f2_pack(bg_exp2(e0), bg_exp2(e1)), d, sum[k]);
+        }
+      };
+      for (; w < w1; ++w) {
+        const uint64_t nl = f2_pack(-lse, -lse), nd = f2_pack(-delta, -delta);
+        if (w + 1 < w1) {
+          lse = p.lse[stat + (w + 1) * stat_step];
+          delta = p.delta[stat + (w + 1) * stat_step];
+        }
+        ok = mbar_wait_warp(&s_full[buf], b_ph, p.status, ERR_TIMEOUT_ATTN);
+        if (!ok) break;
+        tc_fence_after();
+        if (has) {
+          const uint32_t tS = t0 + buf * 2 * TK, tD = tS + TK;
+#pragma unroll
+          for (int c = 0; c < CPT; c += 16) {
+            uint32_t s[16], dp[16];
+            tmem_ld16(tS + c, s);
+            tmem_ld16(tD + c, dp);
+            tmem_wait_ld();
+            if (c + 16 == CPT) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_empty[buf]);
+            }
+            if (near) add(s, dp, nl, nd, c, false);
+            else if (col + c < p.n) add(s, dp, nl, nd, c, true);
+          }
+        } else {
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[buf]);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = bg_exp2(fmaf(__uint_as_float(s[i]), p.scale_log2, bias[c + i]) - l);
-          sum[c + i] = fmaf(e, __uint_as_float(dp[i]) - d, sum[c + i]);
-        }
+        if (++buf == 2) { buf = 0; b_ph ^= 1; }
       }
-      if (++buf == 2) { buf = 0; bph ^= 1; }
-    }
-    if (ok && in && !failed(p.status)) {
-      float* dst = p.part + ((static_cast<long long>(split) * p.n_heads + hl) * p.n + row) * p.ld + col;       // ld a multiple of 4
+      if (!ok || failed(p.status)) break;
+      float* dst = w1 == p.n_win ? p.part + (static_cast<long long>(b.head) * p.n + row) * p.ld + col       // ld a multiple of 4
+                                 : p.extra + static_cast<long long>(blockIdx.x) * C::TILE_FLOATS + (q * 32 + lane) * TK + g * CPT;
+      if (has && in)
 #pragma unroll
-      for (int i = 0; i < CPT; i += 4)
-        if (col + i < p.n) *reinterpret_cast<float4*>(dst + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+        for (int i = 0; i < CPT; i += 4)
+          if (col + i < p.n) {
+            float v[4];
+            f2_unpack(sum[i / 2], v[0], v[1]);
+            f2_unpack(sum[i / 2 + 1], v[2], v[3]);
+            if (near) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] *= bg_exp2(bias[-p.at[min(col + i + k, p.n - 1)]]);
+            }
+            *reinterpret_cast<float4*>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
+          }
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, C::TMEM);
+  if (warp == C::W_MMA) tmem_dealloc(tmem_base, C::TMEM);
+}
+
+// Tiles that several CTAs took part in: what those before the last one left in `extra`, in their order. Block (x, y): the
+// tile that CTA x of the sums left unfinished, if x is the first one that did; rows y, y + 32, .. of it.
+__global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, long long tiles, int g, int tk) {
+  chain_point();
+  const int b0 = blockIdx.x;
+  const long long last_round = tiles / g * g, steps = (tiles - last_round) * p.n_win;
+  const long long first = bg_first(steps, b0, g), end = bg_first(steps, b0 + 1, g), t = (end - 1) / p.n_win;
+  // it ends in the middle of tile t, unless an earlier CTA that does has its turn with the tile, or it has no steps
+  if (first == end || end % p.n_win == 0 || first > t * p.n_win) return;
+  const BgTile b = bg_tile(last_round + t, p.n, tk);
+  const int cols = min(tk, p.n - b.tj * tk), vecs = (cols + 3) / 4;
+  int b1 = b0 + 1;        // CTAs b0 .. b1 - 1 left it unfinished
+  while (bg_first(steps, b1 + 1, g) < (t + 1) * p.n_win) ++b1;
+  for (int r = blockIdx.y; r < PB_TILE && b.ti * PB_TILE + r < p.n; r += gridDim.y)
+    for (int v = threadIdx.x; v < vecs; v += 256) {
+      float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
+      float4 s = *dst;
+      for (int i = b0; i < b1; ++i) {
+        if (bg_first(steps, i, g) == bg_first(steps, i + 1, g)) continue;
+        const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(i) * PB_TILE + r) * tk) + v);
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      }
+      *dst = s;
+    }
 }
 
 // Sums of the pairs of one relative position: a block has 32 positions of one difference in y (a lane each), its warps
 // share the queries. Lanes read neighbouring keys of one query: 128 bytes a load.
-__global__ void __launch_bounds__(256) bias_sums_kernel(const float* part, long long ld, int splits, int n_heads, int head0, int high,
-                                                        int wide, float* out, int heads, int add) {
+__global__ void __launch_bounds__(256) bias_sums_kernel(const float* part, long long ld, int head0, int high, int wide, float* out,
+                                                        int heads, int add) {
   __shared__ float part_sum[8][32];
   chain_point();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int dy = static_cast<int>(blockIdx.x) - (high - 1), k = blockIdx.y * 32 + lane, dx = k - (wide - 1), hl = blockIdx.z;
-  const int n = high * wide, y0 = max(0, dy), y1 = min(high, high + dy), rows = (y1 - y0) * wide;
+  const int n = high * wide, y0 = max(0, dy), y1 = min(high, high + dy);
+  const int nx = min(8, wide), ny = 8 / nx;         // warps along x, y
+  const long long down = static_cast<long long>(wide) * (ld + 1) * ny;
   float s = 0.f;
-  for (int sp = 0; sp < splits; ++sp) {
-    const float* src = part + (static_cast<long long>(sp) * n_heads + hl) * n * ld;
-#pragma unroll 4
-    for (int r = warp; r < rows; r += 8) {
-      const int y = y0 + r / wide, xi = r % wide, xj = xi - dx;
-      if (xj >= 0 && xj < wide) s += src[static_cast<long long>(y * wide + xi) * ld + (y - dy) * wide + xj];
+  if (warp < nx * ny)
+    for (int xi = warp % nx; xi < wide; xi += nx) {
+      const int xj = xi - dx, y = y0 + warp / nx;
+      if (xj >= 0 && xj < wide) {
+        const float* src = part + (static_cast<long long>(hl) * n + y * wide + xi) * ld + (y - dy) * wide + xj;
+#pragma unroll 8
+        for (int r = y; r < y1; r += ny, src += down) s += *src;
+      }
     }
-  }
   part_sum[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && k < 2 * wide - 1) {
@@ -280,58 +420,46 @@ __global__ void __launch_bounds__(256) bias_zero_kernel(float* p, long long n) {
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) p[i] = 0.f;
 }
 
-// Lets a kernel have `bytes` of shared memory, once a device.
-template <typename F> bool allow_smem(F kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-
 constexpr long long PART_BYTES = 256ll << 20;
 
-// How the sums of dS are taken: slices of the windows, heads at a time (their matrices take at most 256 MB, or are one head's).
+// How the sums of dS are taken: heads at a time (their matrices take at most 256 MB, or are one head's).
 struct SumsPlan {
-  int splits, heads;
-  long long ld, bytes;
+  int heads, ctas;
+  long long ld, part, extra;      // bytes
 };
 SumsPlan plan_sums(int n_win, int n, int heads, int head_dim) {
   SumsPlan s;
-  s.ld = (n + 3) / 4 * 4;
   const int tk = head_dim <= 64 ? BgCfg<1>::TK : BgCfg<2>::TK;
-  const long long tiles = static_cast<long long>((n + PB_TILE - 1) / PB_TILE) * ((n + tk - 1) / tk) * heads;
-  // a slice costs as much as four windows to start and to add up
-  auto cost = [&](long long k) { return (tiles * k + num_sms() - 1) / num_sms() * ((n_win + k - 1) / k + 4); };
-  s.splits = 1;
-  for (int k = 2; k <= n_win && k <= 64; ++k)
-    if (cost(k) < cost(s.splits)) s.splits = k;
-  const long long one = 4ll * s.splits * n * s.ld;
+  s.ld = (n + 3) / 4 * 4;
+  const long long one = 4ll * n * s.ld, tiles = static_cast<long long>((n + PB_TILE - 1) / PB_TILE) * ((n + tk - 1) / tk);
   s.heads = static_cast<int>(PART_BYTES / one);
   if (s.heads < 1) s.heads = 1;
   if (s.heads > heads) s.heads = heads;
-  while (s.heads > 1 && static_cast<long long>(s.heads) * s.splits > 65535) --s.heads;
-  s.bytes = one * s.heads;
+  // runs of four steps at least: a run costs about as much to start and to write
+  const long long most = (tiles * s.heads * n_win + 3) / 4;
+  s.ctas = most < num_sms() ? static_cast<int>(most) : num_sms();
+  s.part = one * s.heads;
+  s.extra = 4ll * s.ctas * PB_TILE * tk;
   return s;
 }
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
 
 struct Work {
-  long long table, at, delta, rest, by_position, part, total;
+  long long table, at, delta, rest, by_position, part, extra, total;
 };
 Work work_of(int n_win, int high, int wide, int heads, int head_dim, bool backward, bool with_table) {
   const Place p = place_of(high, wide);
   Work w{};
   const long long stats = 4ll * n_win * heads * p.n;
-  w.at = up(4ll * heads * p.off);
+  w.at = up(4ll * heads * p.size);
   w.delta = w.at + up(4ll * p.at_words);
   w.rest = w.delta + (backward ? up(stats) : 0);
   w.by_position = w.rest + (backward ? up(4 * stats) : 0);
-  w.part = w.by_position + (backward && with_table ? up(4ll * heads * p.off) : 0);
-  w.total = w.part + (backward && with_table ? up(plan_sums(n_win, p.n, heads, head_dim).bytes) : 0);
+  w.part = w.by_position + (backward && with_table ? up(4ll * heads * (2 * high - 1) * (2 * wide - 1)) : 0);
+  const SumsPlan s = plan_sums(n_win, p.n, heads, head_dim);
+  w.extra = w.part + (backward && with_table ? up(s.part) : 0);
+  w.total = w.extra + (backward && with_table ? up(s.extra) : 0);
   return w;
 }
 
@@ -343,15 +471,23 @@ bool fits(const AerisBiasedAttn* a) {
 }
 
 int expand(const AerisBiasedAttn* a, const Place& p, float* table, int* at, cudaStream_t stream) {
-  const int most = p.off > p.at_words ? p.off : p.at_words;
-  return launch_chained(bias_expand_kernel, dim3((most + 255) / 256, a->heads), 256, 0, stream, *a, table, at, p.n, p.off, p.at_words);
+  const int most = p.size > p.at_words ? p.size : p.at_words;
+  return launch_chained(bias_expand_kernel, dim3((most + 255) / 256, a->heads), 256, 0, stream, *a, table, at, p);
 }
 
 template <int DCH>
-int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, dim3 grid, cudaStream_t stream) {
+int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, long long tiles, int ctas, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  if (!allow_smem(bias_grad_kernel<DCH>, BgCfg<DCH>::SMEM, done)) return -20;
-  return launch_chained(bias_grad_kernel<DCH>, grid, BgCfg<DCH>::THREADS, BgCfg<DCH>::SMEM, stream, m[0], m[1], m[2], m[3], p);
+  using C = BgCfg<DCH>;
+  if (!once_a_device(done, [&] {
+        // warpgroups that ask for more registers than the launch holds would wait for ever
+        cudaFuncAttributes f;
+        return cudaFuncSetAttribute(bias_grad_kernel<DCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) == cudaSuccess &&
+               cudaFuncGetAttributes(&f, bias_grad_kernel<DCH>) == cudaSuccess && f.numRegs * C::THREADS >= C::REGS;
+      }))
+    return -20;
+  const int r = launch_chained(bias_grad_kernel<DCH>, ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, tiles);
+  return r ? r : launch_chained(bias_join_kernel, dim3(ctas, 32), 256, 0, stream, p, tiles, ctas, C::TK);
 }
 
 }  // namespace
@@ -377,7 +513,7 @@ extern "C" int aeris_biased_attn_fwd(const AerisBiasedAttn* a, void* stream_) {
   int r = expand(a, p, table, at, stream);
   if (r) return r;
   r = attn_fwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, static_cast<int>(a->ld_o), a->lse, a->n_win, p.n, a->heads, a->head_dim,
-                      a->scale, table, at, p.off, p.off / 2, a->status, stream);
+                      a->scale, table, at, p.size, p.zero, a->status, stream);
   return r ? r - 100 : 2;
 }
 
@@ -396,7 +532,7 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   if (r) return r;
   r = attn_bwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, a->d_o, static_cast<int>(a->ld_o), a->lse, delta,
                       reinterpret_cast<float*>(work + w.rest), a->dqkv, static_cast<int>(a->ld_dqkv), a->n_win, p.n, a->heads,
-                      a->head_dim, a->scale, table, at, p.off, p.off / 2, a->status, stream);
+                      a->head_dim, a->scale, table, at, p.size, p.zero, a->status, stream);
   if (r) return r - 100;
   int count = 4;
   if (!sums) return count;
@@ -416,24 +552,26 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
     if ((r = make_tmap_heads_bf16(&m[i], ops[i].base, a->head_dim, a->heads, p.n, a->n_win, ops[i].ld, ops[i].rows))) return r - 200;
   const SumsPlan s = plan_sums(a->n_win, p.n, a->heads, a->head_dim);
   BgParams g{};
-  g.lse = a->lse; g.delta = delta; g.table = table; g.at = at; g.part = reinterpret_cast<float*>(work + w.part); g.ld = s.ld;
-  g.n = p.n; g.heads = a->heads; g.n_win = a->n_win; g.off = p.off; g.zero = p.off / 2; g.splits = s.splits;
+  g.lse = a->lse; g.delta = delta; g.table = table; g.at = at; g.part = reinterpret_cast<float*>(work + w.part);
+  g.extra = reinterpret_cast<float*>(work + w.extra); g.ld = s.ld;
+  g.n = p.n; g.heads = a->heads; g.n_win = a->n_win; g.size = p.size; g.zero = p.zero;
   g.scale_log2 = a->scale * 1.4426950408889634f; g.status = a->status;
   float* by_position = a->buckets ? reinterpret_cast<float*>(work + w.by_position) : a->dtable;
   for (int h0 = 0; h0 < a->heads; h0 += s.heads) {
     g.head0 = h0;
     g.n_heads = a->heads - h0 < s.heads ? a->heads - h0 : s.heads;
-    const dim3 grid((p.n + PB_TILE - 1) / PB_TILE, (p.n + tk - 1) / tk, s.splits * g.n_heads);
-    if ((r = dch == 1 ? launch_bias_grad<1>(m, g, grid, stream) : launch_bias_grad<2>(m, g, grid, stream))) return r - 300;
+    const long long tiles = static_cast<long long>((p.n + PB_TILE - 1) / PB_TILE) * ((p.n + tk - 1) / tk) * g.n_heads;
+    const long long steps = tiles * a->n_win;
+    const int ctas = steps < s.ctas ? static_cast<int>(steps) : s.ctas;
+    if ((r = dch == 1 ? launch_bias_grad<1>(m, g, tiles, ctas, stream) : launch_bias_grad<2>(m, g, tiles, ctas, stream))) return r - 300;
     r = launch_chained(bias_sums_kernel, dim3(2 * a->high - 1, (2 * a->wide - 1 + 31) / 32, g.n_heads), 256, 0, stream,
-                       static_cast<const float*>(g.part), s.ld, s.splits, g.n_heads, h0, a->high, a->wide, by_position, a->heads,
-                       a->buckets ? 0 : a->add);
+                       static_cast<const float*>(g.part), s.ld, h0, a->high, a->wide, by_position, a->heads, a->buckets ? 0 : a->add);
     if (r) return r - 400;
-    count += 2;
+    count += 3;
   }
   if (a->buckets) {
     r = launch_chained(bias_buckets_kernel, dim3(a->table_rows, (a->heads + 31) / 32), 256, 0, stream, *a,
-                       static_cast<const float*>(by_position), p.off);
+                       static_cast<const float*>(by_position), (2 * a->high - 1) * (2 * a->wide - 1));
     if (r) return r - 500;
     ++count;
   }
