@@ -41,7 +41,7 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return warp_sum(v);
 }
 
-// Any width: a block per row, which it reads three times.
+// Any width (what layer_norm_fast.cuh does not hold in registers): a block per row, which it reads three times.
 template <typename T>
 __global__ void __launch_bounds__(LN_THREADS) ln_fwd_any_kernel(const AerisLayerNorm a) {
   __shared__ float part[32];
@@ -121,24 +121,24 @@ __global__ void __launch_bounds__(LN_THREADS) ln_sums_any_kernel(const AerisLaye
   }
 }
 
-// dw, db from the slices' sums: a warp per 32 columns and eight slices at a time.
-__global__ void __launch_bounds__(LN_THREADS) ln_join_kernel(const AerisLayerNorm a) {
-  __shared__ float part[8][32];
+// dw, db from the slices' sums: 32 columns by 32 warps, which share the slices.
+__global__ void __launch_bounds__(1024) ln_join_kernel(const AerisLayerNorm a, int slices) {
+  __shared__ float part[32][33];
   chain_point();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane, which = blockIdx.y;
   float* out = which ? a.db : a.dw;
+  if (!out) return;
   float s = 0.f;
-  if (c < a.cols && out)
-    for (int i = warp; i < a.slices; i += 8) s += a.work[(static_cast<long long>(i) * 2 + which) * a.cols + c];
-  part[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0 && c < a.cols && out) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += part[i][lane];
-    out[c] = a.add ? out[c] + s : s;
+  if (c < a.cols) {
+#pragma unroll 4
+    for (int i = warp; i < slices; i += 32) s += a.work[(static_cast<long long>(i) * 2 + which) * a.cols + c];
   }
+  part[lane][warp] = s;
+  __syncthreads();
+  s = warp_sum(part[warp][lane]);         // the warps' sums of column `warp`
+  const int col = blockIdx.x * 32 + warp;
+  if (lane == 0 && col < a.cols) out[col] = a.add ? out[col] + s : s;
 }
 
 bool ln_fits(const AerisLayerNorm* a) {
@@ -149,14 +149,18 @@ bool ln_fits(const AerisLayerNorm* a) {
 
 }  // namespace aeris
 
+#include "layer_norm_fast.cuh"
+
 using namespace aeris;
 
 extern "C" int aeris_layer_norm_fwd(const AerisLayerNorm* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!ln_fits(a)) return -1;
+  int r = a->f32 ? ln_fwd_fast<float>(*a, stream) : ln_fwd_fast<__nv_bfloat16>(*a, stream);
+  if (r <= 0) return r ? r : 1;
   const dim3 grid(static_cast<unsigned>(a->rows));
-  const int r = a->f32 ? launch_chained(ln_fwd_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
-                       : launch_chained(ln_fwd_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);
+  r = a->f32 ? launch_chained(ln_fwd_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
+             : launch_chained(ln_fwd_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);
   return r ? r : 1;
 }
 
@@ -164,19 +168,26 @@ extern "C" int aeris_layer_norm_bwd(const AerisLayerNorm* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!ln_fits(a) || !a->dy || a->ld_dy < 0) return -1;
   const bool sums = a->dw || a->db;
-  if (sums && (!a->work || a->slices <= 0 || a->slices > 65535)) return -2;
-  int n = 0, r = 0;
-  if (sums) {     // first: the gradient of x may take the place of x or dy
+  if (sums != (a->work != nullptr) || (sums && (a->slices <= 0 || a->slices > 65535))) return -2;
+  int n = 1, slices = a->slices;
+  int r = a->f32 ? ln_bwd_fast<float>(*a, stream, slices) : ln_bwd_fast<__nv_bfloat16>(*a, stream, slices);
+  if (r < 0) return r;
+  const bool fast = r == 0;
+  if (!fast && sums) {     // first: the gradient of x may take the place of x or dy
     const dim3 grid((a->cols + LN_COLS - 1) / LN_COLS, a->slices);
     r = a->f32 ? launch_chained(ln_sums_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
                : launch_chained(ln_sums_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);
     if (r) return r;
-    r = launch_chained(ln_join_kernel, dim3((a->cols + 31) / 32, 2), LN_THREADS, 0, stream, *a);
-    if (r) return r;
-    n += 2;
+    ++n;
   }
+  if (sums) {
+    r = launch_chained(ln_join_kernel, dim3((a->cols + 31) / 32, 2), 1024, 0, stream, *a, slices);
+    if (r) return r;
+    ++n;
+  }
+  if (fast) return n;
   const dim3 grid(static_cast<unsigned>(a->rows));
   r = a->f32 ? launch_chained(ln_bwd_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
              : launch_chained(ln_bwd_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);
-  return r ? r : n + 1;
+  return r ? r : n;
 }

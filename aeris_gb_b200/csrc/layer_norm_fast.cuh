@@ -1,0 +1,527 @@
+// Layer norm of rows that lie in registers. Included by layer_norm.cu.
+//
+// Memory is the floor: a row is read once (forward) or with its gradient once (backward) and written once. Rows are taken in
+// vectors of 16 bytes where they start on 16-byte boundaries and consist of whole ones, else element by element; a lane has up to NV of them. Narrow
+// rows share a warp (a group of lanes each), rows up to 32 NV vectors take a warp, wider ones a block of up to 1,024 threads.
+#pragma once
+
+namespace aeris {
+
+namespace {
+
+// One vector of a row: W elements, as pairs of fp32.
+template <typename T> struct RowVec;
+template <> struct RowVec<__nv_bfloat16> {
+  uint4 r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(uint64_t (&f)[4]) const {
+    f[0] = f2_from_bf16x2(r.x); f[1] = f2_from_bf16x2(r.y); f[2] = f2_from_bf16x2(r.z); f[3] = f2_from_bf16x2(r.w);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const uint64_t (&f)[4]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(f2_to_bf16x2(f[0]), f2_to_bf16x2(f[1]), f2_to_bf16x2(f[2]), f2_to_bf16x2(f[3]));
+  }
+};
+template <> struct RowVec<float> {
+  ulonglong2 r;
+  __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const ulonglong2*>(p); }
+  __device__ __forceinline__ void get(uint64_t (&f)[2]) const { f[0] = r.x; f[1] = r.y; }
+  static __device__ __forceinline__ void store(float* p, const uint64_t (&f)[2]) {
+    *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(f[0], f[1]);
+  }
+};
+
+// W elements of the weight or the bias from column c on.
+template <int W>
+__device__ __forceinline__ void load_weights(const void* w, int f32, int c, uint64_t (&f)[W / 2]) {
+  if (f32) {
+    const ulonglong2* p = reinterpret_cast<const ulonglong2*>(static_cast<const float*>(w) + c);
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const ulonglong2 v = p[i];
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  } else if constexpr (W == 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + c);
+    f[0] = f2_from_bf16x2(v.x); f[1] = f2_from_bf16x2(v.y); f[2] = f2_from_bf16x2(v.z); f[3] = f2_from_bf16x2(v.w);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + c);
+    f[0] = f2_from_bf16x2(v.x); f[1] = f2_from_bf16x2(v.y);
+  }
+}
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+__device__ __forceinline__ uint64_t f2_both(float v) { return f2_pack(v, v); }
+
+struct LnCut {
+  int group;        // lanes of a row (a power of two up to 32), or 0: the block
+  int rows;         // rows of a block at a time
+};
+
+// Sum over the lanes of a row, in each of them. `part`: 32 words for every value that is summed at once (block only).
+template <bool BLOCK, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], int group, float* part) {
+  if constexpr (!BLOCK) {
+    for (int o = group >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+    __syncthreads();        // the words may still be read from the sum before
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) part[k * 32 + (threadIdx.x >> 5)] = v[k];
+    __syncthreads();
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? part[k * 32 + lane] : 0.f);
+  }
+}
+
+// A row per group of lanes (BLOCK = false: 8 warps) or per block. Lane l has vectors l, l + lanes, .. Issue slots bound it beside
+// memory (62 % of them, 64,800 rows of 1536, bf16: 80 us, 5.0 TB/s): arithmetic is two-wide, the differences from the mean take the
+// row's place, and rows are whole vectors (with the differences taken twice and a last vector that may be cut off, whose
+// predicated code is issued for all of them, 89 us). Tried: rows through a ring of bulk copies 140, a block per row 133,
+// four blocks an SM (64 registers, spilled) 103.
+template <typename T, int W, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_kernel(const AerisLayerNorm a, const LnCut cut) {
+  __shared__ float part[BLOCK ? 32 : 1];
+  constexpr int P = W / 2;
+  chain_point();
+  const int lanes = BLOCK ? blockDim.x : cut.group, lane = BLOCK ? threadIdx.x : threadIdx.x & (cut.group - 1);
+  const long long row = BLOCK ? blockIdx.x : static_cast<long long>(blockIdx.x) * cut.rows + threadIdx.x / cut.group;
+  const bool live = row < a.rows;       // lanes of rows that there are not stay for the sums of their warp
+  const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x;
+  uint64_t v[NV][P];
+  {
+    RowVec<T> raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * lanes + lane) * W;
+      if (c < a.cols) raw[i].load(x + c);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * lanes + lane) * W < a.cols) {
+        raw[i].get(v[i]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[i][k] = 0ull;
+      }
+    }
+  }
+  constexpr bool EARLY = BLOCK && NV == 1;        // weight and bias are asked for with the row
+  uint64_t we[P], be[P];
+  if constexpr (EARLY) {
+    const int c = lane * W;
+    if (a.w && c < a.cols) load_weights<W>(a.w, a.w_f32, c, we);
+    if (a.b && c < a.cols) load_weights<W>(a.b, a.w_f32, c, be);
+  }
+  const float inv = 1.f / static_cast<float>(a.cols);
+  uint64_t t = 0ull;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < P; ++k) t = f2_add(t, v[i][k]);
+  float s[1] = {f2_sum(t)};
+  row_sums<BLOCK, 1>(s, cut.group, part);
+  const float mean = s[0] * inv;
+  const uint64_t m = f2_both(mean);
+  t = 0ull;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i * lanes + lane) * W < a.cols) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        v[i][k] = f2_sub(v[i][k], m);
+        t = f2_fma(v[i][k], v[i][k], t);
+      }
+    }
+  }
+  s[0] = f2_sum(t);
+  row_sums<BLOCK, 1>(s, cut.group, part);
+  const float rstd = 1.f / sqrtf(s[0] * inv + a.eps);
+  if (!live) return;
+  const uint64_t r = f2_both(rstd);
+  T* y = static_cast<T*>(a.y) + row * a.ld_y;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * lanes + lane) * W;
+    if (c < a.cols) {
+      uint64_t w[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[i][k] = f2_mul(v[i][k], r);
+      if (a.w) {
+        if constexpr (!EARLY) load_weights<W>(a.w, a.w_f32, c, w);
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[i][k] = f2_mul(v[i][k], EARLY ? we[k] : w[k]);
+      }
+      if (a.b) {
+        if constexpr (!EARLY) load_weights<W>(a.b, a.w_f32, c, w);
+#pragma unroll
+        for (int k = 0; k < P; ++k) v[i][k] = f2_add(v[i][k], EARLY ? be[k] : w[k]);
+      }
+      RowVec<T>::store(y + c, v[i]);
+    }
+  }
+  if (lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, rstd);
+}
+
+// The same element by element, for rows that start anywhere.
+template <typename T, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_one_kernel(const AerisLayerNorm a, const LnCut cut) {
+  __shared__ float part[BLOCK ? 32 : 1];
+  chain_point();
+  const int lanes = BLOCK ? blockDim.x : cut.group, lane = BLOCK ? threadIdx.x : threadIdx.x & (cut.group - 1);
+  const long long row = BLOCK ? blockIdx.x : static_cast<long long>(blockIdx.x) * cut.rows + threadIdx.x / cut.group;
+  const bool live = row < a.rows;
+  const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ld_x;
+  float v[NV], s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = i * lanes + lane < a.cols ? ld_f(x + i * lanes + lane) : 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) s[0] += v[i];
+  const float inv = 1.f / static_cast<float>(a.cols);
+  row_sums<BLOCK, 1>(s, cut.group, part);
+  const float mean = s[0] * inv;
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * lanes + lane < a.cols) {
+      v[i] -= mean;
+      s[0] = fmaf(v[i], v[i], s[0]);
+    }
+  row_sums<BLOCK, 1>(s, cut.group, part);
+  const float rstd = 1.f / sqrtf(s[0] * inv + a.eps);
+  if (!live) return;
+  T* y = static_cast<T*>(a.y) + row * a.ld_y;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * lanes + lane;
+    if (c < a.cols) {
+      float f = v[i] * rstd;
+      if (a.w) f *= weight_at(a.w, a.w_f32, c);
+      if (a.b) f += weight_at(a.b, a.w_f32, c);
+      st_f(y + c, f);
+    }
+  }
+  if (lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, rstd);
+}
+
+// The groups' column sums, one after the other so that the order of additions is fixed, and the block's slice of `work`.
+template <typename F>
+__device__ __forceinline__ void join_groups(const AerisLayerNorm& a, float* joined, int group, int groups, F&& each) {
+  for (int t = 0; t < groups; ++t) {
+    if (group == t)
+      each([&](int c, float dw, float db) {
+        joined[c] = t ? joined[c] + dw : dw;
+        joined[a.cols + c] = t ? joined[a.cols + c] + db : db;
+      });
+    __syncthreads();
+  }
+  float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+  for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) out[c] = joined[c];
+}
+
+// Gradients. A thread keeps its columns for all rows that it sees (NV vectors), and their sums of dy xhat and dy in registers; R
+// rows are taken at a time, so that their loads and the latencies of their sums are shared. MIN: blocks that an SM is to hold.
+// 64,800 rows of 1536, bf16: 132 us, 4.5 TB/s, and 5 for the slices' join; with two blocks an SM 153; the next rows asked for
+// a round ahead 135 (R = 2); a warp per row and its sums in 170 registers 360.
+template <typename T, int W, int NV, int R, bool BLOCK, int THREADS, int MIN>
+__global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNorm a, const LnCut cut) {
+  __shared__ float part[BLOCK ? 64 * R : 1];
+  extern __shared__ float joined[];         // BLOCK = false: [2, cols]
+  constexpr int P = W / 2;
+  constexpr bool KEEP = NV == 1;            // the weight stays in registers
+  chain_point();
+  const int lanes = BLOCK ? blockDim.x : cut.group, lane = BLOCK ? threadIdx.x : threadIdx.x & (cut.group - 1);
+  const int group = BLOCK ? 0 : threadIdx.x / cut.group, groups = BLOCK ? 1 : cut.rows;
+  const float inv = 1.f / static_cast<float>(a.cols);
+  uint64_t dw[NV][P], db[NV][P], w[P];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < P; ++k) dw[i][k] = db[i][k] = 0ull;
+#pragma unroll
+  for (int k = 0; k < P; ++k) w[k] = f2_both(1.f);
+  auto weights = [&](int c) {
+    if (a.w && c < a.cols) load_weights<W>(a.w, a.w_f32, c, w);
+  };
+  if (KEEP) weights(lane * W);
+  // a block's rows: R times `groups` of them, one of each R for every group
+  for (long long r0 = static_cast<long long>(blockIdx.x) * groups * R; r0 < a.rows; r0 += static_cast<long long>(gridDim.x) * groups * R) {
+    RowVec<T> x[R][NV], g[R][NV];
+    float2 st[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = r0 + r * groups + group;
+      const bool live = row < a.rows;
+      st[r] = live ? *reinterpret_cast<const float2*>(a.stats + 2 * row) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * lanes + lane) * W;
+        if (live && c < a.cols) {
+          x[r][i].load(static_cast<const T*>(a.x) + row * a.ld_x + c);
+          g[r][i].load(static_cast<const T*>(a.dy) + row * a.ld_dy + c);
+        }
+      }
+    }
+    float s[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = r0 + r * groups + group < a.rows;
+      const uint64_t m = f2_both(st[r].x), rs = f2_both(st[r].y);
+      uint64_t s1 = 0ull, s2 = 0ull;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * lanes + lane) * W;
+        if (live && c < a.cols) {
+          uint64_t fx[P], fg[P];
+          if (!KEEP) weights(c);
+          x[r][i].get(fx);
+          g[r][i].get(fg);
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            const uint64_t xhat = f2_mul(f2_sub(fx[k], m), rs), gw = f2_mul(fg[k], w[k]);
+            dw[i][k] = f2_fma(fg[k], xhat, dw[i][k]);
+            db[i][k] = f2_add(db[i][k], fg[k]);
+            s1 = f2_add(s1, gw);
+            s2 = f2_fma(gw, xhat, s2);
+          }
+        }
+      }
+      s[2 * r] = f2_sum(s1);
+      s[2 * r + 1] = f2_sum(s2);
+    }
+    row_sums<BLOCK, 2 * R>(s, cut.group, part);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = r0 + r * groups + group;
+      if (row < a.rows) {
+        const uint64_t m = f2_both(st[r].x), rs = f2_both(st[r].y), m1 = f2_both(s[2 * r] * inv), m2 = f2_both(-s[2 * r + 1] * inv);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * lanes + lane) * W;
+          if (c < a.cols) {
+            uint64_t fx[P], fg[P];
+            if (!KEEP) weights(c);
+            x[r][i].get(fx);
+            g[r][i].get(fg);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+              const uint64_t xhat = f2_mul(f2_sub(fx[k], m), rs), gw = f2_mul(fg[k], w[k]);
+              fg[k] = f2_mul(rs, f2_fma(xhat, m2, f2_sub(gw, m1)));
+            }
+            RowVec<T>::store(static_cast<T*>(a.y) + row * a.ld_y + c, fg);
+          }
+        }
+      }
+    }
+  }
+  if (!a.work) return;
+  auto each = [&](auto&& put) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int c = (i * lanes + lane) * W + 2 * k;
+        float w0, w1, b0, b1;
+        f2_unpack(dw[i][k], w0, w1);
+        f2_unpack(db[i][k], b0, b1);
+        if (c < a.cols) put(c, w0, b0);
+        if (c + 1 < a.cols) put(c + 1, w1, b1);
+      }
+  };
+  if constexpr (BLOCK) {
+    float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+    each([&](int c, float dw_, float db_) {
+      out[c] = dw_;
+      out[a.cols + c] = db_;
+    });
+  } else {
+    join_groups(a, joined, group, groups, each);
+  }
+}
+
+// The same element by element, for rows that start anywhere.
+template <typename T, int NV, int R, bool BLOCK, int THREADS, int MIN>
+__global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLayerNorm a, const LnCut cut) {
+  __shared__ float part[BLOCK ? 64 * R : 1];
+  extern __shared__ float joined[];
+  chain_point();
+  const int lanes = BLOCK ? blockDim.x : cut.group, lane = BLOCK ? threadIdx.x : threadIdx.x & (cut.group - 1);
+  const int group = BLOCK ? 0 : threadIdx.x / cut.group, groups = BLOCK ? 1 : cut.rows;
+  const float inv = 1.f / static_cast<float>(a.cols);
+  float dw[NV], db[NV], w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * lanes + lane;
+    dw[i] = db[i] = 0.f;
+    w[i] = c >= a.cols ? 0.f : a.w ? weight_at(a.w, a.w_f32, c) : 1.f;
+  }
+  for (long long r0 = static_cast<long long>(blockIdx.x) * groups * R; r0 < a.rows; r0 += static_cast<long long>(gridDim.x) * groups * R) {
+    T x[R][NV], g[R][NV];
+    float2 st[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = r0 + r * groups + group;
+      const bool live = row < a.rows;
+      st[r] = live ? *reinterpret_cast<const float2*>(a.stats + 2 * row) : make_float2(0.f, 0.f);
+      const T *px = static_cast<const T*>(a.x) + row * a.ld_x + lane, *pg = static_cast<const T*>(a.dy) + row * a.ld_dy + lane;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = live && i * lanes + lane < a.cols;
+        x[r][i] = in ? px[i * lanes] : T(0.f);
+        g[r][i] = in ? pg[i * lanes] : T(0.f);
+      }
+    }
+    float s[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[2 * r] = s[2 * r + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        // zeros of dy behind the row's end add nothing; the statistics there are finite
+        const float xhat = (ld_f(&x[r][i]) - st[r].x) * st[r].y, fg = ld_f(&g[r][i]), gw = fg * w[i];
+        dw[i] = fmaf(fg, xhat, dw[i]);
+        db[i] += fg;
+        s[2 * r] += gw;
+        s[2 * r + 1] = fmaf(gw, xhat, s[2 * r + 1]);
+      }
+    }
+    row_sums<BLOCK, 2 * R>(s, cut.group, part);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = r0 + r * groups + group;
+      if (row < a.rows) {
+        const float m1 = s[2 * r] * inv, m2 = s[2 * r + 1] * inv;
+        T* dx = static_cast<T*>(a.y) + row * a.ld_y + lane;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * lanes + lane < a.cols) {
+            const float xhat = (ld_f(&x[r][i]) - st[r].x) * st[r].y;
+            st_f(dx + i * lanes, st[r].y * (fmaf(ld_f(&g[r][i]), w[i], -m1) - xhat * m2));
+          }
+      }
+    }
+  }
+  if (!a.work) return;
+  auto each = [&](auto&& put) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * lanes + lane;
+      if (c < a.cols) put(c, dw[i], db[i]);
+    }
+  };
+  if constexpr (BLOCK) {
+    float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+    each([&](int c, float dw_, float db_) {
+      out[c] = dw_;
+      out[a.cols + c] = db_;
+    });
+  } else {
+    join_groups(a, joined, group, groups, each);
+  }
+}
+
+bool ln_aligned(const void* p, long long ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+
+template <typename T, int W, int NV, bool BLOCK>
+int launch_ln_fwd(const AerisLayerNorm& a, LnCut cut, int threads, cudaStream_t stream) {
+  const long long blocks = BLOCK ? a.rows : (a.rows + cut.rows - 1) / cut.rows;
+  if constexpr (W > 1)
+    return launch_chained(ln_fwd_kernel<T, W, NV, BLOCK>, static_cast<unsigned>(blocks), threads, 0, stream, a, cut);
+  else
+    return launch_chained(ln_fwd_one_kernel<T, NV, BLOCK>, static_cast<unsigned>(blocks), threads, 0, stream, a, cut);
+}
+
+// The cut of rows of `vecs` vectors into lanes: groups of a warp as far as `most` vectors a lane go.
+LnCut ln_cut(int vecs) {
+  LnCut c;
+  c.group = 1;
+  while (c.group < vecs && c.group < 32) c.group *= 2;
+  c.rows = 256 / c.group;
+  return c;
+}
+int ln_threads(int vecs, int nv) { return ((vecs + nv - 1) / nv + 31) / 32 * 32; }
+
+// Forward. Returns 1 where no kernel takes the width.
+template <typename T>
+int ln_fwd_fast(const AerisLayerNorm& a, cudaStream_t stream) {
+  constexpr int S = sizeof(T), W = 16 / S;
+  if (a.cols % W == 0 && ln_aligned(a.x, a.ld_x, S) && ln_aligned(a.y, a.ld_y, S) && ln_aligned(a.w, 0, S) && ln_aligned(a.b, 0, S)) {
+    const int vecs = a.cols / W, nv = (vecs + 31) / 32;
+    const LnCut cut = ln_cut(vecs);
+    // few rows: a block each, as long as that makes the chain of a row's steps shorter
+    if (nv > 2 && a.rows <= 2 * num_sms() && vecs <= 1024) return launch_ln_fwd<T, W, 1, true>(a, cut, ln_threads(vecs, 1), stream);
+    if (nv <= 1) return launch_ln_fwd<T, W, 1, false>(a, cut, 256, stream);
+    if (nv <= 2) return launch_ln_fwd<T, W, 2, false>(a, cut, 256, stream);
+    if (nv <= 4) return launch_ln_fwd<T, W, 4, false>(a, cut, 256, stream);
+    if (nv <= 6) return launch_ln_fwd<T, W, 6, false>(a, cut, 256, stream);
+    if (nv <= 8) return launch_ln_fwd<T, W, 8, false>(a, cut, 256, stream);
+    if (vecs <= 2048) return launch_ln_fwd<T, W, 2, true>(a, cut, ln_threads(vecs, 2), stream);
+    if (vecs <= 4096) return launch_ln_fwd<T, W, 4, true>(a, cut, ln_threads(vecs, 4), stream);
+    return 1;
+  }
+  const int nv = (a.cols + 31) / 32;
+  const LnCut cut = ln_cut(a.cols);
+  if (nv <= 1) return launch_ln_fwd<T, 1, 1, false>(a, cut, 256, stream);
+  if (nv <= 2) return launch_ln_fwd<T, 1, 2, false>(a, cut, 256, stream);
+  if (nv <= 4) return launch_ln_fwd<T, 1, 4, false>(a, cut, 256, stream);
+  if (nv <= 8) return launch_ln_fwd<T, 1, 8, false>(a, cut, 256, stream);
+  if (nv <= 16) return launch_ln_fwd<T, 1, 16, false>(a, cut, 256, stream);
+  if (a.cols <= 8192) return launch_ln_fwd<T, 1, 8, true>(a, cut, ln_threads(a.cols, 8), stream);
+  if (a.cols <= 16384) return launch_ln_fwd<T, 1, 16, true>(a, cut, ln_threads(a.cols, 16), stream);
+  return 1;
+}
+
+// `slices`: receives how many slices of column sums were written.
+template <typename T, int W, int NV, int R, bool BLOCK, int THREADS, int MIN>
+int launch_ln_bwd(const AerisLayerNorm& a, LnCut cut, int threads, cudaStream_t stream, int& slices) {
+  const int at_once = (BLOCK ? 1 : cut.rows) * R;       // rows of a block
+  const long long need = (a.rows + at_once - 1) / at_once;
+  // as many blocks as the SMs hold (MIN, more of narrower ones)
+  long long blocks = static_cast<long long>(num_sms()) * (MIN * THREADS / threads);
+  if (blocks > need) blocks = need;
+  if (a.work && blocks > a.slices) blocks = a.slices;
+  slices = static_cast<int>(blocks);
+  const int smem = !BLOCK && a.work ? 2 * a.cols * 4 : 0;
+  if constexpr (W > 1)
+    return launch_chained(ln_bwd_kernel<T, W, NV, R, BLOCK, THREADS, MIN>, slices, threads, smem, stream, a, cut);
+  else
+    return launch_chained(ln_bwd_one_kernel<T, NV, R, BLOCK, THREADS, MIN>, slices, threads, smem, stream, a, cut);
+}
+template <typename T>
+int ln_bwd_fast(const AerisLayerNorm& a, cudaStream_t stream, int& slices) {
+  constexpr int S = sizeof(T), W = 16 / S;
+  if (a.cols % W == 0 && ln_aligned(a.x, a.ld_x, S) && ln_aligned(a.y, a.ld_y, S) && ln_aligned(a.dy, a.ld_dy, S) && ln_aligned(a.w, 0, S)) {
+    const int vecs = a.cols / W;
+    const LnCut cut = ln_cut(vecs);
+    if (vecs <= 32) return launch_ln_bwd<T, W, 1, 4, false, 256, 2>(a, cut, 256, stream, slices);
+    if (vecs <= 64) return launch_ln_bwd<T, W, 2, 2, false, 256, 2>(a, cut, 256, stream, slices);
+    if (vecs <= 192) return launch_ln_bwd<T, W, 1, 4, true, 192, 3>(a, cut, ln_threads(vecs, 1), stream, slices);
+    if (vecs <= 256) return launch_ln_bwd<T, W, 1, 4, true, 256, 2>(a, cut, ln_threads(vecs, 1), stream, slices);
+    if (vecs <= 512) return launch_ln_bwd<T, W, 1, 4, true, 512, 1>(a, cut, ln_threads(vecs, 1), stream, slices);
+    if (vecs <= 1024) return launch_ln_bwd<T, W, 2, 2, true, 512, 1>(a, cut, ln_threads(vecs, 2), stream, slices);
+    if (vecs <= 2048) return launch_ln_bwd<T, W, 4, 1, true, 512, 1>(a, cut, ln_threads(vecs, 4), stream, slices);
+    return 1;
+  }
+  const LnCut cut = ln_cut(a.cols);
+  if (a.cols <= 32) return launch_ln_bwd<T, 1, 1, 4, false, 256, 3>(a, cut, 256, stream, slices);
+  if (a.cols <= 128) return launch_ln_bwd<T, 1, 4, 4, false, 256, 2>(a, cut, 256, stream, slices);
+  if (a.cols <= 512) return launch_ln_bwd<T, 1, 4, 4, true, 128, 5>(a, cut, ln_threads(a.cols, 4), stream, slices);
+  if (a.cols <= 1024) return launch_ln_bwd<T, 1, 4, 4, true, 256, 2>(a, cut, ln_threads(a.cols, 4), stream, slices);
+  if (a.cols <= 4096) return launch_ln_bwd<T, 1, 8, 2, true, 512, 1>(a, cut, ln_threads(a.cols, 8), stream, slices);
+  if (a.cols <= 8192) return launch_ln_bwd<T, 1, 16, 1, true, 512, 1>(a, cut, ln_threads(a.cols, 16), stream, slices);
+  return 1;
+}
+
+}  // namespace
+
+}  // namespace aeris

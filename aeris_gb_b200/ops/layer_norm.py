@@ -116,7 +116,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
     """Gradients of :func:`layer_norm_fwd` for ``dy`` with respect to its rows; ``x`` and ``stats`` are its input and its second
     result. Returns (gradient of x in x's type, fp32 gradient of the weight or None without one, fp32 gradient of the bias or None
     with ``bias=False``). ``dx`` may be ``dy`` or ``x`` itself; ``dw``, ``db`` [cols] fp32 are added to where given. The same
-    bits on every run."""
+    bits on every run; tensors whose rows start elsewhere may be added up in another order."""
     rows, cols, pitch, dt, dev = _check(x, weight, None)
     pitch_dy = _like(dy, x.shape, dt, dev, "dy")
     if not (stats.shape == (rows, 2) and stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous()):
@@ -148,7 +148,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
         slices = 0
         work = None
         if dw is not None or db is not None:
-            slices = slices_for(rows, cols, _multiprocessors(dev.index))
+            slices = slices_for(rows, _multiprocessors(dev.index))
             work = x.new_empty((slices, 2, cols), dtype=torch.float32)
         _launch("aeris_layer_norm_bwd", _RECORD.pack(
             x.data_ptr(), dy.data_ptr(), dx.data_ptr(), 0 if weight is None else weight.data_ptr(), 0, stats.data_ptr(),
@@ -158,6 +158,6 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
     return dx, dw, db
 
 
-def slices_for(rows: int, cols: int, multiprocessors: int) -> int:
-    """Slices of the rows whose column sums are taken apart: about eight blocks of 64 columns on every multiprocessor."""
-    return max(1, min(8 * multiprocessors * 64 // cols + 1, -(-rows // 16), 4096))
+def slices_for(rows: int, multiprocessors: int) -> int:
+    """Slices of the rows whose column sums may be taken apart: four blocks on every multiprocessor, four rows each."""
+    return max(1, min(4 * multiprocessors, -(-rows // 4)))
