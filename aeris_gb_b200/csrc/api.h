@@ -256,39 +256,35 @@ int aeris_layer_norm_fwd(const AerisLayerNorm* a, void* stream);
 int aeris_layer_norm_bwd(const AerisLayerNorm* a, void* stream);
 
 // Linear layer (csrc/linear.cu; mirrored in ops/linear.py): y = resid + act(x w^T + bias) with x [rows, inner], w [cols, inner],
-// bf16. Pitches in elements; those of x and w are multiples of 8 and their bases on 16-byte boundaries, the others' are free.
+// bf16. Pitches in elements; rows may start anywhere.
 enum { LIN_ACT_NONE = 0, LIN_ACT_RELU = 1, LIN_ACT_SILU = 2, LIN_ACT_GELU = 3, LIN_ACT_GELU_TANH = 4 };
 typedef struct AerisLinear {
   const void *x, *w, *bias;         // bias [cols], fp32 or bf16, or null
   const void* resid;                // [rows, cols] or null
   void *y, *z;                      // z: null, or receives x w^T + bias
-  long long ld_x, ld_w, ld_resid, ld_y, ld_z;
+  void* work;                       // aeris_linear_fwd_bytes (may be none), from a 256-byte boundary on
+  int* status;
+  long long ld_x, ld_w, ld_resid, ld_y, ld_z, work_bytes;
   int rows, inner, cols, act, bias_bf16;
-  int* status;
 } AerisLinear;
-int aeris_linear_fwd(const AerisLinear* a, void* stream);
-// dz = dy act'(z) and its column sums. dz: null where it is not wanted; db [cols] fp32 or null, added to with `add`; work:
-// [slices, cols] where db is wanted.
-typedef struct AerisLinearDz {
-  const void *dy, *z;
-  void* dz;
-  float *db, *work;
-  long long ld_dy, ld_z, ld_dz;
-  int rows, cols, act, add, slices;
-} AerisLinearDz;
-int aeris_linear_dz(const AerisLinearDz* a, void* stream);
-// dx = dz w and dw = dz^T x, each where its result is given. dz, w and x as x and w above. dw: bf16, or fp32 that is added to
-// (dw_f32). work: aeris_linear_work_bytes for the sums of slices of the rows (0: none needed).
+// dz = dy act'(z), db = its column sums, dx = dz w, dw = dz^T x, each where its result is given. dw: bf16, or fp32 that is added to
+// (dw_f32); db: fp32, added to with `add_db`.
 typedef struct AerisLinearGrad {
-  const void *dz, *w, *x;
+  const void *dy, *x, *w, *z;       // z: null where act is LIN_ACT_NONE
   void *dx, *dw;
-  float* work;
-  long long ld_dz, ld_w, ld_x, ld_dx, ld_dw, work_bytes;
-  int rows, inner, cols, dw_f32;
+  float* db;
+  void* work;                       // aeris_linear_bwd_bytes, from a 256-byte boundary on
   int* status;
+  long long ld_dy, ld_x, ld_w, ld_z, ld_dx, ld_dw, work_bytes;
+  int rows, inner, cols, act, dw_f32, add_db;
 } AerisLinearGrad;
-long long aeris_linear_work_bytes(int rows, int inner, int cols, int dw_f32);
-int aeris_linear_grad(const AerisLinearGrad* a, void* stream);  // all three: the number of kernels launched, or a negative code
+// Bytes of the workspace: copies of operands whose rows do not start on 16-byte boundaries (pad_*), dz (own_dz: with an activation,
+// or for a dy of such rows), sums of slices of the rows.
+long long aeris_linear_fwd_bytes(int rows, int inner, int cols, int pad_x, int pad_w);
+long long aeris_linear_bwd_bytes(int rows, int inner, int cols, int own_dz, int pad_x, int pad_w, int dx, int dw, int db, int dw_f32);
+// Both return the number of kernels launched, or a negative code.
+int aeris_linear_fwd(const AerisLinear* a, void* stream);
+int aeris_linear_bwd(const AerisLinearGrad* a, void* stream);
 
 // Window attention with a learned bias by relative position (csrc/position_bias.cu; mirrored in ops/position_bias.py). Windows of
 // high x wide tokens in rows; the relative position of query i and key j is (y_i - y_j + high - 1) (2 wide - 1) + x_i - x_j + wide - 1,

@@ -8,8 +8,8 @@
 // bias, activation and residual are applied to the accumulators, which are rounded once.
 #include "common.cuh"
 #include "api.h"
+#include "cluster.cuh"
 #include "host.h"
-#include "gemm_epilogue.cuh"
 
 namespace aeris {
 
@@ -33,8 +33,20 @@ struct LinParams {
   int* status;
 };
 
-// Gaussian distribution function. erff is CUDA's; near -infinity the sum cancels to an absolute error of 6e-8.
-__device__ __forceinline__ float gauss_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f); }
+// exp(-z^2 / 2) and the Gaussian distribution function of z: erfc by the rational approximation in 1 / (1 + p x) times exp(-x^2)
+// of Abramowitz and Stegun, 7.1.26, whose absolute error is below 1.5e-7. Next to CUDA's erff it takes half the instructions,
+// shares its exponential with the derivative and does not cancel far below zero.
+__device__ __forceinline__ void gauss(float z, float& e, float& cdf) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = 1.f / fmaf(0.3275911f, x, 1.f);
+  e = __expf(-x * x);
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * (p * t) * e;
+  cdf = z < 0.f ? tail : 1.f - tail;
+}
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
 
 // gelu_tanh by 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), which keeps the relative precision of small results.
@@ -42,7 +54,7 @@ __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
     case LIN_ACT_RELU: return z < 0.f ? 0.f : z;      // a NaN stays
     case LIN_ACT_SILU: return z * sigmoid(z);
-    case LIN_ACT_GELU: return z * gauss_cdf(z);
+    case LIN_ACT_GELU: { float e, c; gauss(z, e, c); return z * c; }
     case LIN_ACT_GELU_TANH: return z * sigmoid(z * fmaf(z * z, 0.07135481282f, 1.59576912161f));
     default: return z;
   }
@@ -51,7 +63,7 @@ __device__ __forceinline__ float act_grad(float z, int act) {
   switch (act) {
     case LIN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case LIN_ACT_SILU: { const float s = sigmoid(z); return s * fmaf(z, 1.f - s, 1.f); }
-    case LIN_ACT_GELU: return fmaf(z * 0.39894228040143268f, __expf(-0.5f * z * z), gauss_cdf(z));
+    case LIN_ACT_GELU: { float e, c; gauss(z, e, c); return fmaf(z * 0.39894228040143268f, e, c); }
     case LIN_ACT_GELU_TANH: {
       z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;      // 1 and 0 long before; the square of a large one would be infinite
       const float s = sigmoid(z * fmaf(z * z, 0.07135481282f, 1.59576912161f));
@@ -358,7 +370,189 @@ lin_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUt
   if (warp == 1) tmem_dealloc(tmem_base, S::TMEM);
 }
 
+// 256 x 256 tiles by CTA pairs (a cluster of two), which share the operands' reads from L2 and from shared memory: each CTA loads
+// its 128 rows of A and half of B's tile, the leader issues products of both (tcgen05.mma.cta_group::2), each CTA writes its
+// rows. Roles and barriers as in gemm2.cu. EW: epilogue warps, eight (two for 32 rows) for the price of one of the ring's stages
+// where results leave in bf16: us, four / eight, 64800 x 1536 -> 4096 plain 543 / 522, GELU 641 / 576, with z 696 / 631, residual 739 /
+// 604, 28800 x 768 -> 2048 105 / 80, 152 / 116, 162 / 122, 175 / 117. 64,800 x 1536 -> 4096 with GELU and z, 631 us, are 1.29
+// PFLOP/s, of the 1.40 that a product holds under the power cap.
+constexpr int LIN2_BN = 256, LIN2_STAGE = 32768;
+template <int EW> struct Lin2Smem {
+  static constexpr int STAGES = EW == 8 ? 5 : 6;
+  static constexpr int BARS = STAGES * LIN2_STAGE, OUT = BARS + 1024, TOTAL = OUT + EW * 8192 + 1024;
+  static constexpr int THREADS = 64 + 32 * EW;
+  static_assert(TOTAL <= 227 * 1024, "shared memory");
+};
+
+template <int A_MN, int B_MN, int EW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Lin2Smem<EW>::THREADS, 1)
+lin2_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+            const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z, const LinParams p) {
+  using S = Lin2Smem<EW>;
+  constexpr int STAGES = S::STAGES, GROUP_M = 8;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::BARS);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;           // [2]
+  uint64_t* tempty_bar = tfull_bar + 2;               // [2], in the leader: an arrival per epilogue warp of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+  const int m_tiles = (p.M + 255) / 256, n_tiles = (p.N + LIN2_BN - 1) / LIN2_BN;
+  const int kb_total = (p.K + LIN_BK - 1) / LIN_BK, kb_per_split = (kb_total + p.k_splits - 1) / p.k_splits;
+  const int mn_tiles = m_tiles * n_tiles, total_tiles = mn_tiles * p.k_splits;
+  // eight rows of tiles at a time: what the pairs at work read of A and B stays in L2
+  auto tile_at = [&](int tile, int& split, int& tm, int& tn) {
+    split = tile / mn_tiles;
+    const int mn = tile - split * mn_tiles, g = mn / (GROUP_M * n_tiles), in = mn - g * GROUP_M * n_tiles;
+    const int gm = min(GROUP_M, m_tiles - g * GROUP_M);
+    tn = in / gm;
+    tm = g * GROUP_M + in - tn * gm;
+  };
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], 2 * EW); }
+    fence_barrier_init();
+  }
+  if (warp == 1) { tmem_alloc2(tmem_slot, 2 * LIN2_BN); tmem_relinquish2(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();       // both CTAs' barriers are initialised and tensor memory is allocated before anyone signals
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_point();
+
+  if (warp == 0) {
+    if (elect_one_sync()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < total_tiles && ok; tile += n_clusters) {
+        int split, tm, tn;
+        tile_at(tile, split, tm, tn);
+        const int kb0 = split * kb_per_split, kb1 = min(kb_total, kb0 + kb_per_split), m0 = tm * 256 + crank * 128;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_poll(&empty_bar[stage], phase ^ 1, p.status, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
+          uint8_t* sa = smem + stage * LIN2_STAGE;
+          uint8_t* sb = sa + 16384;
+          if (crank == 0) mbar_expect_tx(&full_bar[stage], 2 * LIN2_STAGE);       // both CTAs' copies
+          const uint32_t fb = map_to_cta(smem_u32(&full_bar[stage]), 0);
+          if constexpr (A_MN == 0) {
+            tma_load_2d_pair(sa, &tm_a, fb, kb * LIN_BK, m0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) tma_load_2d_pair(sa + j * 8192, &tm_a, fb, m0 + j * 64, kb * LIN_BK);
+          }
+          const int n0 = tn * LIN2_BN + crank * 128;
+          if constexpr (B_MN == 0) {
+            tma_load_2d_pair(sb, &tm_b, fb, kb * LIN_BK, n0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) tma_load_2d_pair(sb + j * 8192, &tm_b, fb, n0 + j * 64, kb * LIN_BK);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // after a time-out: the tiles that the issuer did not take, of both CTAs (a stage never filled counts as there)
+      for (int s = 0; s < STAGES && !ok && crank == 0; ++s) {
+        if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+        if (!mbar_wait_poll(&full_bar[stage], phase, nullptr, 0)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (crank == 0 && elect_one_sync()) {
+      constexpr uint32_t idesc = make_idesc_bf16(256, LIN2_BN, A_MN, B_MN);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < total_tiles && ok; tile += n_clusters) {
+        const int split = tile / mn_tiles;
+        const int kb0 = split * kb_per_split, kb1 = min(kb_total, kb0 + kb_per_split);
+        if (!mbar_wait_poll(&tempty_bar[acc], acc_phase ^ 1, p.status, ERR_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t tmem_acc = tmem_base + acc * LIN2_BN;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_poll(&full_bar[stage], phase, p.status, ERR_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * LIN2_STAGE), sb = sa + 16384;
+#pragma unroll
+          for (int kk = 0; kk < LIN_BK / 16; ++kk) {
+            const uint64_t ad = A_MN ? make_smem_desc(sa + kk * 2048, 8192, 1024) : make_smem_desc(sa + kk * 32, 0, 1024);
+            const uint64_t bd = B_MN ? make_smem_desc(sb + kk * 2048, 8192, 1024) : make_smem_desc(sb + kk * 32, 0, 1024);
+            umma2_ss(tmem_acc, ad, bd, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit2_mc(&empty_bar[stage], 0x3);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tc_commit2_mc(&tfull_bar[acc], 0x3);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      // the last products have completed: an epilogue that gave up has not waited for them
+      if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+      mbar_wait_poll(&empty_bar[stage], phase, nullptr, 0);
+    }
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const bool keep = !failed(p.status);       // see note_failure
+    const uint32_t leader_tempty = map_to_cta(smem_u32(&tempty_bar[0]), 0);
+    LinOut out{smem + S::OUT + (part * 4 + q) * 8192, lane};
+    for (int tile = cluster; tile < total_tiles; tile += n_clusters) {
+      int split, tm, tn;
+      tile_at(tile, split, tm, tn);
+      if (!__all_sync(0xffffffffu, mbar_wait_poll(&tfull_bar[acc], acc_phase, p.status, ERR_TIMEOUT_TMEM_FULL))) break;
+      tc_fence_after();
+      const int row = tm * 256 + crank * 128 + q * 32 + lane;
+      const uint32_t taddr = tmem_base + acc * LIN2_BN + (static_cast<uint32_t>(q * 32) << 16);
+      constexpr int COLS = LIN2_BN / (EW / 4);
+      if (keep)
+        lin_epilogue_row(p, taddr, row, row < p.M, tn * LIN2_BN, part * COLS, (part + 1) * COLS, split,
+                         split * kb_per_split >= kb_total, out, p.c_map ? &tm_y : nullptr, p.z_map ? &tm_z : nullptr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(leader_tempty + acc * 8);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    out.drain();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();       // nobody leaves while the pair may still touch its shared memory or tensor memory
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc2(tmem_base, 2 * LIN2_BN);
+}
+
 bool whole_rows(const void* base, long long ld) { return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ld % 8 == 0; }
+
+struct LinMaps {
+  CUtensorMap a, b, y, z;
+};
+// Tensor maps of a product whose tiles take `rows_a` rows of A and `rows_b` of B at a time; decides how results leave.
+template <int A_MN, int B_MN>
+int lin_maps(LinMaps& m, const void* A, long long lda, const void* B, long long ldb, LinParams& p, int rows_a, int rows_b) {
+  int r;
+  if (!whole_rows(A, lda) || !whole_rows(B, ldb)) return -11;
+  if ((r = A_MN ? make_tmap_2d_bf16(&m.a, A, p.M, p.K, lda, 64, LIN_BK) : make_tmap_2d_bf16(&m.a, A, p.K, p.M, lda, LIN_BK, rows_a)))
+    return r;
+  if ((r = B_MN ? make_tmap_2d_bf16(&m.b, B, p.N, p.K, ldb, 64, LIN_BK) : make_tmap_2d_bf16(&m.b, B, p.K, p.N, ldb, LIN_BK, rows_b)))
+    return r - 100;
+  m.y = m.z = m.a;         // not stored through where rows go element by element
+  p.c_map = p.mode == LIN_OUT && whole_rows(p.C, p.ldc);
+  p.z_map = p.mode == LIN_OUT && p.Z && whole_rows(p.Z, p.ldz);
+  p.r_vec = p.resid && whole_rows(p.resid, p.ldr);
+  if (p.c_map && (r = make_tmap_2d_sw64_bf16(&m.y, p.C, p.N, p.M, p.ldc, 32, 32))) return r - 200;
+  if (p.z_map && (r = make_tmap_2d_sw64_bf16(&m.z, p.Z, p.N, p.M, p.ldz, 32, 32))) return r - 300;
+  return 0;
+}
+
+long long lin_tiles(int M, int N, int bm, int bn) { return static_cast<long long>((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 
 template <int BN, int A_MN, int B_MN>
 int launch_lin(const void* A, long long lda, const void* B, long long ldb, LinParams p, cudaStream_t stream) {
@@ -366,36 +560,152 @@ int launch_lin(const void* A, long long lda, const void* B, long long ldb, LinPa
   auto kern = lin_kernel<BN, A_MN, B_MN>;
   static std::atomic<uint64_t> done{0};
   if (!allow_smem_once(kern, S::TOTAL, done)) return -20;
-  CUtensorMap ta, tb, ty, tz;
-  int r;
-  if (!whole_rows(A, lda) || !whole_rows(B, ldb)) return -11;
-  if ((r = A_MN ? make_tmap_2d_bf16(&ta, A, p.M, p.K, lda, 64, LIN_BK) : make_tmap_2d_bf16(&ta, A, p.K, p.M, lda, LIN_BK, LIN_BM)))
-    return r;
-  if ((r = B_MN ? make_tmap_2d_bf16(&tb, B, p.N, p.K, ldb, 64, LIN_BK) : make_tmap_2d_bf16(&tb, B, p.K, p.N, ldb, LIN_BK, BN)))
-    return r - 100;
-  ty = tz = ta;         // not stored through where rows go element by element
-  p.c_map = p.mode == LIN_OUT && whole_rows(p.C, p.ldc);
-  p.z_map = p.mode == LIN_OUT && p.Z && whole_rows(p.Z, p.ldz);
-  p.r_vec = p.resid && whole_rows(p.resid, p.ldr);
-  if (p.c_map && (r = make_tmap_2d_sw64_bf16(&ty, p.C, p.N, p.M, p.ldc, 32, 32))) return r - 200;
-  if (p.z_map && (r = make_tmap_2d_sw64_bf16(&tz, p.Z, p.N, p.M, p.ldz, 32, 32))) return r - 300;
-  const long long tiles = static_cast<long long>((p.M + LIN_BM - 1) / LIN_BM) * ((p.N + BN - 1) / BN) * p.k_splits;
+  LinMaps m;
+  const int r = lin_maps<A_MN, B_MN>(m, A, lda, B, ldb, p, LIN_BM, BN);
+  if (r) return r;
+  const long long tiles = lin_tiles(p.M, p.N, LIN_BM, BN) * p.k_splits;
   if (tiles > 0x3fffffff) return -2;
   const int grid = tiles < num_sms() ? static_cast<int>(tiles) : num_sms();
-  return launch_chained(kern, grid, LIN_THREADS, S::TOTAL, stream, ta, tb, ty, tz, p);
+  return launch_chained(kern, grid, LIN_THREADS, S::TOTAL, stream, m.a, m.b, m.y, m.z, p);
 }
 
-long long lin_tiles(int M, int N, int bn) { return static_cast<long long>((M + LIN_BM - 1) / LIN_BM) * ((N + bn - 1) / bn); }
+template <int A_MN, int B_MN, int EW>
+int launch_lin2(const void* A, long long lda, const void* B, long long ldb, LinParams p, cudaStream_t stream) {
+  using S = Lin2Smem<EW>;
+  auto kern = lin2_kernel<A_MN, B_MN, EW>;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem_once(kern, S::TOTAL, done)) return -20;
+  LinMaps m;
+  const int r = lin_maps<A_MN, B_MN>(m, A, lda, B, ldb, p, 128, 128);
+  if (r) return r;
+  const long long tiles = lin_tiles(p.M, p.N, 256, LIN2_BN) * p.k_splits;
+  if (tiles > 0x1fffffff) return -2;
+  // as many pairs as the device holds at once (a group of SMs with an odd number of them has one left over)
+  static std::atomic<int> held{0};
+  int pairs = held.load(std::memory_order_relaxed);
+  if (!pairs) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(num_sms() / 2 * 2);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::TOTAL;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {2, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs <= 0) pairs = num_sms() / 2;
+    held.store(pairs, std::memory_order_relaxed);
+  }
+  const int clusters = tiles < pairs ? static_cast<int>(tiles) : pairs;
+  return launch_chained(kern, 2 * clusters, S::THREADS, S::TOTAL, stream, m.a, m.b, m.y, m.z, p);
+}
 
-// Width of the tiles: the widest of which there is one for every multiprocessor, else narrow ones.
+// Few rows: a warp per two columns, whose weights it reads once while x lies in shared memory. The tensor core's tiles are 128 rows
+// high whatever there is of them; one row of 1536 -> 4096 takes them 9.7 us, this kernel 3.6, which is the weights' way from L2 (3.5 TB/s).
+constexpr int ROWS_MAX = 8, ROWS_COLS = 2, ROWS_WARPS = 8;
+template <int M>
+__global__ void __launch_bounds__(32 * ROWS_WARPS) lin_rows_kernel(const LinParams p, const __nv_bfloat16* x, long long lda,
+                                                                   const __nv_bfloat16* w, long long ldb) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint4* sx = reinterpret_cast<uint4*>(smem_raw);       // [M][vecs], zeros behind the row's end
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, vecs = (p.K + 7) / 8, whole = p.K / 8;
+  chain_point();
+  const int col0 = (blockIdx.x * ROWS_WARPS + warp) * ROWS_COLS;
+  auto vec_of = [&](const __nv_bfloat16* row, int v) -> uint4 {
+    if (v < whole) return reinterpret_cast<const uint4*>(row)[v];
+    unsigned short e[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (8 * v + i < p.K) e[i] = reinterpret_cast<const unsigned short*>(row)[8 * v + i];
+    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+  };
+  for (int i = threadIdx.x; i < M * vecs; i += 32 * ROWS_WARPS) {
+    const int m = i / vecs;
+    sx[i] = vec_of(x + m * lda, i - m * vecs);
+  }
+  __syncthreads();
+  if (col0 >= p.N) return;
+  const __nv_bfloat16* w0 = w + col0 * ldb;
+  const __nv_bfloat16* w1 = w + min(col0 + 1, p.N - 1) * ldb;
+  uint64_t acc[M][ROWS_COLS];
+#pragma unroll
+  for (int m = 0; m < M; ++m) acc[m][0] = acc[m][1] = 0ull;
+#pragma unroll 4
+  for (int v = lane; v < vecs; v += 32) {
+    const uint4 a = vec_of(w0, v), b = vec_of(w1, v);
+    const uint64_t fa[4] = {f2_from_bf16x2(a.x), f2_from_bf16x2(a.y), f2_from_bf16x2(a.z), f2_from_bf16x2(a.w)};
+    const uint64_t fb[4] = {f2_from_bf16x2(b.x), f2_from_bf16x2(b.y), f2_from_bf16x2(b.z), f2_from_bf16x2(b.w)};
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const uint4 c = sx[m * vecs + v];
+      const uint64_t fx[4] = {f2_from_bf16x2(c.x), f2_from_bf16x2(c.y), f2_from_bf16x2(c.z), f2_from_bf16x2(c.w)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[m][0] = f2_fma(fx[i], fa[i], acc[m][0]);
+        acc[m][1] = f2_fma(fx[i], fb[i], acc[m][1]);
+      }
+    }
+  }
+  float mine = 0.f;         // lane 2 m + c: row m, column c
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < ROWS_COLS; ++c) {
+      float lo, hi;
+      f2_unpack(acc[m][c], lo, hi);
+      float s = lo + hi;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 2 * m + c) mine = s;
+    }
+  const int m = lane >> 1, col = col0 + (lane & 1);
+  if (m >= M || col >= p.N) return;
+  if (p.bias)
+    mine += p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]) : static_cast<const float*>(p.bias)[col];
+  if (p.Z) p.Z[m * p.ldz + col] = __float2bfloat16_rn(mine);
+  float v = act_of(mine, p.act);
+  if (p.resid) v += __bfloat162float(p.resid[m * p.ldr + col]);
+  p.C[m * p.ldc + col] = __float2bfloat16_rn(v);
+}
+
+template <int M = 1>
+int launch_rows(const LinParams& p, const void* x, long long ldx, const void* w, long long ldw, cudaStream_t stream) {
+  if constexpr (M < ROWS_MAX) {
+    if (p.M > M) return launch_rows<M + 1>(p, x, ldx, w, ldw, stream);
+  }
+  const int per = ROWS_WARPS * ROWS_COLS;
+  return launch_chained(lin_rows_kernel<M>, (p.N + per - 1) / per, 32 * ROWS_WARPS, M * ((p.K + 7) / 8) * 16, stream, p,
+                        static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(w), ldw);
+}
+
+// Which kernel takes a product: the one whose rounds of tiles are over first by the cycles that a block of 64 of the reduction
+// takes (fitted to what they measured, us, CTA pairs / single CTAs 256 / 128 / 64 / 32 wide, forward: 64 x 1536 -> 4096 14.8 / 14.2 /
+// 9.2 / 7.4 / 6.9, 900 x 768 -> 768 10.0 / 11.3 / 7.4 / 5.8 / 6.8, 3600 x 512 -> 512 9.2 / 10.3 / 7.0 / 7.1 / 8.5, 12150 x 1152 ->
+// 1152 34.3 / 34.3 / 30.3 / 40.4 / 69.5, 28800 x 768 -> 2048 76 / 85 / 90 / 112 / 196, 64800 x 1536 -> 1536 213 / 235 / 269 / 374 /
+// 691; of these the rule loses 13 % at 12150 x 1152 and nothing elsewhere).
+constexpr int LIN_PAIR = 0;
+long long lin_cost(const LinParams& p, int bn, int splits) {
+  const int kb = (p.K + LIN_BK - 1) / LIN_BK, units = bn == LIN_PAIR ? num_sms() / 2 : num_sms();
+  const long long tiles = (bn == LIN_PAIR ? lin_tiles(p.M, p.N, 256, 256) : lin_tiles(p.M, p.N, 128, bn)) * splits;
+  const int per = bn == LIN_PAIR ? 530 : bn == 256 ? 640 : bn == 128 ? 400 : bn == 64 ? 260 : 230;
+  return (tiles + units - 1) / units * ((kb + splits - 1) / splits) * per + 4000;
+}
+
 template <int A_MN, int B_MN>
 int launch_product(const void* A, long long lda, const void* B, long long ldb, const LinParams& p, cudaStream_t stream) {
-  if (lin_tiles(p.M, p.N, 256) * p.k_splits >= num_sms()) return launch_lin<256, A_MN, B_MN>(A, lda, B, ldb, p, stream);
-  if (lin_tiles(p.M, p.N, 128) * p.k_splits >= num_sms()) return launch_lin<128, A_MN, B_MN>(A, lda, B, ldb, p, stream);
-  if constexpr (!B_MN) {
-    if (lin_tiles(p.M, p.N, 64) * p.k_splits < num_sms()) return launch_lin<32, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+  int best = LIN_PAIR;
+  for (int bn : {256, 128, 64, 32})
+    if ((bn > 32 || !B_MN) && lin_cost(p, bn, p.k_splits) < lin_cost(p, best, p.k_splits)) best = bn;
+  switch (best) {
+    case 256: return launch_lin<256, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+    case 128: return launch_lin<128, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+    case 64: return launch_lin<64, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+    case 32:
+      if constexpr (!B_MN) return launch_lin<32, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+      break;
+    default: break;
   }
-  return launch_lin<64, A_MN, B_MN>(A, lda, B, ldb, p, stream);
+  return launch_lin2<A_MN, B_MN, A_MN ? 4 : 8>(A, lda, B, ldb, p, stream);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients' own passes
@@ -403,45 +713,61 @@ constexpr int DZ_THREADS = 256, DZ_COLS = 64;
 
 __device__ __forceinline__ float bf(unsigned short u) { return __uint_as_float(static_cast<uint32_t>(u) << 16); }
 
+struct DzParams {
+  const void *dy, *z;
+  void* dz;
+  float* work;              // [gridDim.y, cols], or null
+  long long ld_dy, ld_z, ld_dz;
+  int rows, cols;
+};
 // dz = dy act'(z) and the column sums of one slice of the rows. A thread takes V columns (one 16-byte vector, or one column
 // where rows start anywhere) of every R-th row of its slice; a block 64 columns.
-template <int V>
-__global__ void __launch_bounds__(DZ_THREADS) lin_dz_kernel(const AerisLinearDz a) {
-  constexpr int CT = DZ_COLS / V, R = DZ_THREADS / CT;
+template <int V, int ACT>
+__global__ void __launch_bounds__(DZ_THREADS) lin_dz_kernel(const DzParams a) {
+  constexpr int CT = DZ_COLS / V, R = DZ_THREADS / CT, U = 4;      // rows asked for at a time
   __shared__ float part[R][DZ_COLS];
   chain_point();
   const int c0 = threadIdx.x % CT * V, col = blockIdx.x * DZ_COLS + c0, r0 = threadIdx.x / CT;
   float s[V] = {};
   if (col < a.cols) {
-    for (long long row = static_cast<long long>(blockIdx.y) * R + r0; row < a.rows; row += static_cast<long long>(gridDim.y) * R) {
-      const unsigned short* dy = static_cast<const unsigned short*>(a.dy) + row * a.ld_dy + col;
-      const unsigned short* z = a.z ? static_cast<const unsigned short*>(a.z) + row * a.ld_z + col : nullptr;
-      unsigned short d[V], zz[V];
-      if constexpr (V == 8) {
-        *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(dy);
-        if (z) *reinterpret_cast<uint4*>(zz) = *reinterpret_cast<const uint4*>(z);
-      } else {
-        d[0] = *dy;
-        if (z) zz[0] = *z;
-      }
-      float g[V];
+    const long long step = static_cast<long long>(gridDim.y) * R;
+    for (long long row = static_cast<long long>(blockIdx.y) * R + r0; row < a.rows; row += U * step) {
+      unsigned short d[U][V], z[U][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        // a product by itself, so that the sums are the same bits whether dz is written or not
-        g[i] = z ? __fmul_rn(bf(d[i]), act_grad(bf(zz[i]), a.act)) : bf(d[i]);
-        s[i] += g[i];
-      }
-      if (a.dz) {
-        __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(a.dz) + row * a.ld_dz + col;
-        if constexpr (V == 8)
-          *reinterpret_cast<uint4*>(dz) = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]),
-                                                     pack_bf16x2(g[6], g[7]));
-        else
-          *dz = __float2bfloat16_rn(g[0]);
-      }
+      for (int u = 0; u < U; ++u)
+        if (row + u * step < a.rows) {
+          const unsigned short* pd = static_cast<const unsigned short*>(a.dy) + (row + u * step) * a.ld_dy + col;
+          const unsigned short* pz = static_cast<const unsigned short*>(a.z) + (row + u * step) * a.ld_z + col;
+          if constexpr (V == 8) {
+            *reinterpret_cast<uint4*>(d[u]) = *reinterpret_cast<const uint4*>(pd);
+            if (ACT != LIN_ACT_NONE) *reinterpret_cast<uint4*>(z[u]) = *reinterpret_cast<const uint4*>(pz);
+          } else {
+            d[u][0] = *pd;
+            if (ACT != LIN_ACT_NONE) z[u][0] = *pz;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (row + u * step < a.rows) {
+          float g[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            // a product by itself, so that the sums are the same bits whether dz is written or not
+            g[i] = ACT != LIN_ACT_NONE ? __fmul_rn(bf(d[u][i]), act_grad(bf(z[u][i]), ACT)) : bf(d[u][i]);
+            s[i] += g[i];
+          }
+          if (a.dz) {
+            __nv_bfloat16* dz = static_cast<__nv_bfloat16*>(a.dz) + (row + u * step) * a.ld_dz + col;
+            if constexpr (V == 8)
+              *reinterpret_cast<uint4*>(dz) = make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]),
+                                                         pack_bf16x2(g[6], g[7]));
+            else
+              *dz = __float2bfloat16_rn(g[0]);
+          }
+        }
     }
   }
-  if (!a.db) return;
+  if (!a.work) return;
 #pragma unroll
   for (int i = 0; i < V; ++i) part[r0][c0 + i] = s[i];
   __syncthreads();
@@ -449,6 +775,33 @@ __global__ void __launch_bounds__(DZ_THREADS) lin_dz_kernel(const AerisLinearDz 
     float t = 0.f;
     for (int r = 0; r < R; ++r) t += part[r][threadIdx.x];
     a.work[static_cast<long long>(blockIdx.y) * a.cols + blockIdx.x * DZ_COLS + threadIdx.x] = t;
+  }
+}
+
+template <int V>
+int launch_dz(const DzParams& a, int act, dim3 grid, cudaStream_t stream) {
+  switch (act) {
+    case LIN_ACT_RELU: return launch_chained(lin_dz_kernel<V, LIN_ACT_RELU>, grid, DZ_THREADS, 0, stream, a);
+    case LIN_ACT_SILU: return launch_chained(lin_dz_kernel<V, LIN_ACT_SILU>, grid, DZ_THREADS, 0, stream, a);
+    case LIN_ACT_GELU: return launch_chained(lin_dz_kernel<V, LIN_ACT_GELU>, grid, DZ_THREADS, 0, stream, a);
+    case LIN_ACT_GELU_TANH: return launch_chained(lin_dz_kernel<V, LIN_ACT_GELU_TANH>, grid, DZ_THREADS, 0, stream, a);
+    default: return launch_chained(lin_dz_kernel<V, LIN_ACT_NONE>, grid, DZ_THREADS, 0, stream, a);
+  }
+}
+
+// Rows that start on 16-byte boundaries, for tiled loads: dst [rows, (cols + 7) / 8 * 8] of src, zeros behind the rows' ends.
+__global__ void __launch_bounds__(DZ_THREADS) lin_pad_kernel(const unsigned short* src, long long ld, uint4* dst, int rows, int cols) {
+  chain_point();
+  const int vecs = (cols + 7) / 8;
+  const long long n = static_cast<long long>(rows) * vecs;
+  for (long long i = static_cast<long long>(blockIdx.x) * DZ_THREADS + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * DZ_THREADS) {
+    const long long row = i / vecs;
+    const int c = static_cast<int>(i - row * vecs) * 8;
+    const unsigned short* s = src + row * ld + c;
+    unsigned short e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = c + k < cols ? s[k] : static_cast<unsigned short>(0);
+    dst[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
   }
 }
 
@@ -504,16 +857,21 @@ __global__ void __launch_bounds__(DZ_THREADS) lin_join_dw_kernel(const float* pa
   }
 }
 
-// Slices of the reduction over the rows of dw: enough tiles for every multiprocessor, rounds x (k-blocks of a slice + 10 for its
-// start and its sums); at most 8192 rows a slice, for the tensor core truncates at every addition and the error of a sum grows
-// with its length (9e-10 of it per row).
+// Slices of the reduction over the rows of dw, of which each costs its start and its sums' way through memory as well; at most 8192
+// rows a slice, for the tensor core truncates at every addition and the error of a sum grows with its length (9e-10 of it per
+// row).
 int dw_slices(int rows, int inner, int cols) {
-  const int kb = (rows + LIN_BK - 1) / LIN_BK;
-  const long long tiles = lin_tiles(cols, inner, 256);
-  int best = (kb + 127) / 128;
-  auto cost = [&](int s) { return ((tiles * s + num_sms() - 1) / num_sms()) * ((kb + s - 1) / s + 10); };
-  for (int s = best + 1; s <= 64 && kb / s >= 4; ++s)
-    if (cost(s) < cost(best)) best = s;
+  LinParams p{};
+  p.M = cols; p.N = inner; p.K = rows;
+  const int kb = (rows + LIN_BK - 1) / LIN_BK, least = (kb + 127) / 128;
+  const double sums = 8.0 * cols * inner / 3000;      // cycles to write and read one slice's, 3 KB a cycle
+  int best = least;
+  double cost = 1e30;
+  for (int s = least; s <= 64 && (s == least || kb / s >= 4); ++s)
+    for (int bn : {LIN_PAIR, 256, 128, 64}) {
+      const double c = static_cast<double>(lin_cost(p, bn, s)) + (s > 1 ? s * sums + 4000 : 0);
+      if (c < cost) { cost = c; best = s; }
+    }
   return best;
 }
 
@@ -523,74 +881,150 @@ int dw_slices(int rows, int inner, int cols) {
 
 using namespace aeris;
 
+namespace {
+
+long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
+long long padded(int cols) { return (static_cast<long long>(cols) + 7) / 8 * 8; }
+// A single row has no pitch of its own: one that tensor maps take.
+long long pitch(long long ld, int rows, int cols) { return rows == 1 ? padded(cols) : ld; }
+int blocks_for(long long threads) {
+  const long long b = (threads + DZ_THREADS - 1) / DZ_THREADS, most = 16ll * num_sms();
+  return static_cast<int>(b < most ? b : most);
+}
+// Whether tiled loads take the rows where they are.
+bool tiled(const void* p, long long ld, int rows, int cols) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || (ld % 8 == 0 && ld >= cols));
+}
+// An operand of a product: where it is, or its copy at `at` of the workspace, which then goes on behind it.
+struct Operand {
+  const void* p;
+  long long ld;
+};
+int operand(Operand& o, const void* p, long long ld, int rows, int cols, uint8_t* work, long long& at, int& kernels, cudaStream_t stream) {
+  if (tiled(p, ld, rows, cols)) {
+    o = {p, pitch(ld, rows, cols)};
+    return 0;
+  }
+  o = {work + at, padded(cols)};
+  at += up(2 * padded(cols) * rows);
+  ++kernels;
+  return launch_chained(lin_pad_kernel, blocks_for(padded(cols) / 8 * rows), DZ_THREADS, 0, stream, static_cast<const unsigned short*>(p),
+                        ld, reinterpret_cast<uint4*>(work + at - up(2 * padded(cols) * rows)), rows, cols);
+}
+
+// Slices of the rows whose column sums are taken apart: about eight blocks of 64 columns on every multiprocessor.
+int db_slices(int rows, int cols) {
+  const long long most = 8ll * num_sms() * DZ_COLS / cols + 1, need = (rows + 31ll) / 32;
+  return static_cast<int>(most < need ? (most < 4096 ? most : 4096) : (need < 4096 ? need : 4096));
+}
+long long dw_bytes(int rows, int inner, int cols, bool f32) {
+  const int s = dw_slices(rows, inner, cols);
+  return s > 1 || f32 ? 4ll * s * cols * ((inner + 3) / 4 * 4) : 0;
+}
+
+}  // namespace
+
+extern "C" long long aeris_linear_fwd_bytes(int rows, int inner, int cols, int pad_x, int pad_w) {
+  if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
+  return (pad_x ? up(2 * padded(inner) * rows) : 0) + (pad_w ? up(2 * padded(inner) * cols) : 0);
+}
+
 extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
-  if (a->rows <= 0 || a->inner <= 0 || a->cols <= 0 || !a->y || a->act < 0 || a->act > LIN_ACT_GELU_TANH) return -1;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (a->rows <= 0 || a->inner <= 0 || a->cols <= 0 || !a->x || !a->w || !a->y || a->act < 0 || a->act > LIN_ACT_GELU_TANH) return -1;
+  const bool pad_x = !tiled(a->x, a->ld_x, a->rows, a->inner), pad_w = !tiled(a->w, a->ld_w, a->cols, a->inner);
+  if (a->work_bytes < aeris_linear_fwd_bytes(a->rows, a->inner, a->cols, pad_x, pad_w)) return -2;
   LinParams p{};
   p.M = a->rows; p.N = a->cols; p.K = a->inner; p.act = a->act; p.mode = LIN_OUT; p.k_splits = 1; p.bias_bf16 = a->bias_bf16;
-  p.C = static_cast<__nv_bfloat16*>(a->y); p.ldc = a->ld_y; p.bias = a->bias;
-  p.resid = static_cast<const __nv_bfloat16*>(a->resid); p.ldr = a->ld_resid;
-  p.Z = static_cast<__nv_bfloat16*>(a->z); p.ldz = a->ld_z; p.status = a->status;
-  const int r = launch_product<0, 0>(a->x, a->ld_x, a->w, a->ld_w, p, static_cast<cudaStream_t>(stream_));
-  return r ? r : 1;
+  p.C = static_cast<__nv_bfloat16*>(a->y); p.ldc = pitch(a->ld_y, a->rows, a->cols); p.bias = a->bias;
+  p.resid = static_cast<const __nv_bfloat16*>(a->resid); p.ldr = pitch(a->ld_resid, a->rows, a->cols);
+  p.Z = static_cast<__nv_bfloat16*>(a->z); p.ldz = pitch(a->ld_z, a->rows, a->cols); p.status = a->status;
+  uint8_t* work = static_cast<uint8_t*>(a->work);
+  long long at = 0;
+  int n = 1, r;
+  Operand x, w;
+  if ((r = operand(x, a->x, a->ld_x, a->rows, a->inner, work, at, n, stream))) return r;
+  if ((r = operand(w, a->w, a->ld_w, a->cols, a->inner, work, at, n, stream))) return r;
+  // x of few rows lies in shared memory, at most 48 KB of it
+  if (a->rows <= ROWS_MAX && a->rows * padded(a->inner) * 2 <= 48 * 1024) r = launch_rows(p, x.p, x.ld, w.p, w.ld, stream);
+  else r = launch_product<0, 0>(x.p, x.ld, w.p, w.ld, p, stream);
+  return r ? r : n;
 }
 
-extern "C" int aeris_linear_dz(const AerisLinearDz* a, void* stream_) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (a->rows <= 0 || a->cols <= 0 || !a->dy || (!a->dz && !a->db) || a->slices <= 0 || a->slices > 65535) return -1;
-  if (a->db && !a->work) return -2;
-  const bool vec = a->cols % 8 == 0 && whole_rows(a->dy, a->ld_dy) && (!a->z || whole_rows(a->z, a->ld_z)) &&
-                   (!a->dz || whole_rows(a->dz, a->ld_dz));
-  const dim3 grid((a->cols + DZ_COLS - 1) / DZ_COLS, a->slices);
-  int r = vec ? launch_chained(lin_dz_kernel<8>, grid, DZ_THREADS, 0, stream, *a)
-              : launch_chained(lin_dz_kernel<1>, grid, DZ_THREADS, 0, stream, *a);
-  if (r) return r;
-  if (!a->db) return 1;
-  r = launch_chained(lin_join_sums_kernel, (a->cols + 31) / 32, DZ_THREADS, 0, stream, static_cast<const float*>(a->work), a->db,
-                     a->slices, a->cols, a->add);
-  return r ? r : 2;
-}
-
-extern "C" long long aeris_linear_work_bytes(int rows, int inner, int cols, int dw_f32) {
+extern "C" long long aeris_linear_bwd_bytes(int rows, int inner, int cols, int own_dz, int pad_x, int pad_w, int dx, int dw, int db,
+                                            int dw_f32) {
   if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
-  const int s = dw_slices(rows, inner, cols);
-  return s > 1 || dw_f32 ? 4ll * s * cols * ((inner + 3) / 4 * 4) : 0;
+  long long n = db ? up(4ll * db_slices(rows, cols) * cols) : 0;
+  if (own_dz && (dx || dw)) n += up(2 * padded(cols) * rows);
+  if (dx && pad_w) n += up(2 * padded(inner) * cols);
+  if (dw) n += (pad_x ? up(2 * padded(inner) * rows) : 0) + up(dw_bytes(rows, inner, cols, dw_f32));
+  return n;
 }
 
-extern "C" int aeris_linear_grad(const AerisLinearGrad* a, void* stream_) {
+extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (a->rows <= 0 || a->inner <= 0 || a->cols <= 0 || (!a->dx && !a->dw)) return -1;
+  const int rows = a->rows, inner = a->inner, cols = a->cols;
+  if (rows <= 0 || inner <= 0 || cols <= 0 || !a->dy || a->act < 0 || a->act > LIN_ACT_GELU_TANH) return -1;
+  if ((a->act != LIN_ACT_NONE) != (a->z != nullptr)) return -1;
+  const bool products = a->dx || a->dw, own_dz = products && (a->z || !tiled(a->dy, a->ld_dy, rows, cols));
+  if (a->work_bytes < aeris_linear_bwd_bytes(rows, inner, cols, own_dz, !tiled(a->x, a->ld_x, rows, inner), !tiled(a->w, a->ld_w, cols, inner),
+                                             a->dx != nullptr, a->dw != nullptr, a->db != nullptr, a->dw_f32))
+    return -2;
+  uint8_t* work = static_cast<uint8_t*>(a->work);
+  long long at = 0;
   int n = 0, r;
-  if (a->dx) {        // [rows, inner] = dz [rows, cols] w [cols, inner]
-    LinParams p{};
-    p.M = a->rows; p.N = a->inner; p.K = a->cols; p.mode = LIN_OUT; p.k_splits = 1;
-    p.C = static_cast<__nv_bfloat16*>(a->dx); p.ldc = a->ld_dx; p.status = a->status;
-    if ((r = launch_product<0, 1>(a->dz, a->ld_dz, a->w, a->ld_w, p, stream))) return r;
-    ++n;
-  }
-  if (a->dw) {        // [cols, inner] = dz^T x
-    LinParams p{};
-    p.M = a->cols; p.N = a->inner; p.K = a->rows; p.status = a->status;
-    p.k_splits = dw_slices(a->rows, a->inner, a->cols);
-    const bool direct = p.k_splits == 1 && !a->dw_f32;
-    p.mode = direct ? LIN_OUT : LIN_PART;
-    if (direct) {
-      p.C = static_cast<__nv_bfloat16*>(a->dw); p.ldc = a->ld_dw;
-    } else {
-      if (!a->work || a->work_bytes < aeris_linear_work_bytes(a->rows, a->inner, a->cols, a->dw_f32)) return -3;
-      p.part = a->work; p.ld_part = (a->inner + 3) / 4 * 4;
+  Operand dz{a->dy, pitch(a->ld_dy, rows, cols)};
+  if (own_dz || a->db) {
+    DzParams d{a->dy, a->z, nullptr, nullptr, a->ld_dy, a->ld_z, padded(cols), rows, cols};
+    const int slices = db_slices(rows, cols);
+    if (a->db) {
+      d.work = reinterpret_cast<float*>(work + at);
+      at += up(4ll * slices * cols);
     }
-    if ((r = launch_product<1, 1>(a->dz, a->ld_dz, a->x, a->ld_x, p, stream))) return r - 1000;
+    if (own_dz) {
+      d.dz = work + at;
+      dz = {d.dz, padded(cols)};
+      at += up(2 * padded(cols) * rows);
+    }
+    const bool vec = cols % 8 == 0 && whole_rows(d.dy, d.ld_dy) && (!d.z || whole_rows(d.z, d.ld_z));
+    const dim3 grid((cols + DZ_COLS - 1) / DZ_COLS, slices);
+    if ((r = vec ? launch_dz<8>(d, a->act, grid, stream) : launch_dz<1>(d, a->act, grid, stream))) return r;
     ++n;
-    if (!direct) {
-      const long long vecs = static_cast<long long>(a->cols) * ((a->inner + 3) / 4);
-      const long long blocks = (vecs + DZ_THREADS - 1) / DZ_THREADS;
-      const int vec = (reinterpret_cast<uintptr_t>(a->dw) & 7) == 0 && a->ld_dw % 4 == 0;
-      r = launch_chained(lin_join_dw_kernel, static_cast<unsigned>(blocks < 16 * num_sms() ? blocks : 16 * num_sms()), DZ_THREADS, 0,
-                         stream, static_cast<const float*>(a->work), a->dw, a->ld_dw, a->dw_f32, vec, p.k_splits, a->cols, a->inner,
-                         p.ld_part);
-      if (r) return r - 2000;
+    if (a->db) {
+      r = launch_chained(lin_join_sums_kernel, (cols + 31) / 32, DZ_THREADS, 0, stream, static_cast<const float*>(d.work), a->db, slices, cols,
+                         a->add_db);
+      if (r) return r;
       ++n;
     }
   }
-  return n;
+  if (a->dx) {        // [rows, inner] = dz [rows, cols] w [cols, inner]
+    Operand w;
+    if ((r = operand(w, a->w, a->ld_w, cols, inner, work, at, n, stream))) return r;
+    LinParams p{};
+    p.M = rows; p.N = inner; p.K = cols; p.mode = LIN_OUT; p.k_splits = 1;
+    p.C = static_cast<__nv_bfloat16*>(a->dx); p.ldc = pitch(a->ld_dx, rows, inner); p.status = a->status;
+    if ((r = launch_product<0, 1>(dz.p, dz.ld, w.p, w.ld, p, stream))) return r;
+    ++n;
+  }
+  if (!a->dw) return n;
+  // [cols, inner] = dz^T x
+  Operand x;
+  if ((r = operand(x, a->x, a->ld_x, rows, inner, work, at, n, stream))) return r;
+  LinParams p{};
+  p.M = cols; p.N = inner; p.K = rows; p.status = a->status;
+  p.k_splits = dw_slices(rows, inner, cols);
+  const bool direct = p.k_splits == 1 && !a->dw_f32;
+  p.mode = direct ? LIN_OUT : LIN_PART;
+  if (direct) {
+    p.C = static_cast<__nv_bfloat16*>(a->dw); p.ldc = pitch(a->ld_dw, cols, inner);
+  } else {
+    p.part = reinterpret_cast<float*>(work + at); p.ld_part = (inner + 3) / 4 * 4;
+  }
+  if ((r = launch_product<1, 1>(dz.p, dz.ld, x.p, x.ld, p, stream))) return r - 1000;
+  ++n;
+  if (direct) return n;
+  const int vec = (reinterpret_cast<uintptr_t>(a->dw) & 7) == 0 && a->ld_dw % 4 == 0;
+  r = launch_chained(lin_join_dw_kernel, blocks_for(static_cast<long long>(cols) * ((inner + 3) / 4)), DZ_THREADS, 0, stream,
+                     static_cast<const float*>(p.part), a->dw, a->ld_dw, a->dw_f32, vec, p.k_splits, cols, inner, p.ld_part);
+  return r ? r - 2000 : n + 1;
 }

@@ -18,10 +18,9 @@ from . import lib as _l
 ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")
 _ACT = {name: i for i, name in enumerate(ACTIVATIONS)}
 MOST = 2 ** 31 - 2 ** 12         # rows, columns
-# AerisLinear, AerisLinearDz, AerisLinearGrad (csrc/api.h), field by field
-_FORWARD = struct.Struct("6P5q5iP")
-_DZ = struct.Struct("5P3q5i0q")
-_GRAD = struct.Struct("6P6q4iP")
+# AerisLinear, AerisLinearGrad (csrc/api.h), field by field
+_FORWARD = struct.Struct("8P6q5i0q")
+_GRAD = struct.Struct("9P7q6i0q")
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
@@ -30,26 +29,25 @@ def _text(t) -> str:
 
 
 @functools.lru_cache(maxsize=None)
-def _entry(name: str, *types):
+def _entry(name: str, sizes: int = 0):
     f = getattr(_l.lib(), name)
-    f.argtypes = types or (ctypes.c_char_p, ctypes.c_void_p)
-    f.restype = ctypes.c_longlong if types else ctypes.c_int
+    f.argtypes = (ctypes.c_int,) * sizes or (ctypes.c_char_p, ctypes.c_void_p)
+    f.restype = ctypes.c_longlong if sizes else ctypes.c_int
     return f
 
 
-@functools.lru_cache(maxsize=None)
-def _multiprocessors(device: int) -> int:
-    return torch.cuda.get_device_properties(device).multi_processor_count
+@functools.lru_cache(maxsize=1024)
+def _bytes(name: str, *sizes: int) -> int:
+    return _entry(name, len(sizes))(*sizes)
 
 
-def _launch(name: str, record: bytes) -> None:
-    rc = _entry(name)(record, _l.raw_stream())
+def _launch(name: str, record: bytes, dev) -> None:
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = _entry(name)(record, _l.raw_stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = _entry(name)(record, _l.raw_stream())
     _l.check(min(rc, 0), name, kernels=max(rc, 0))
-
-
-@functools.lru_cache(maxsize=256)
-def _work_bytes(rows: int, inner: int, cols: int, f32: bool) -> int:
-    return _entry("aeris_linear_work_bytes", *[ctypes.c_int] * 4)(rows, inner, cols, f32)
 
 
 def _matrix(t, shape, dev, what: str, dtypes=(_BF16,)) -> None:
@@ -86,22 +84,10 @@ def _act_code(act: str) -> int:
     return _ACT[act]
 
 
-def _tiled(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy whose rows start on 16-byte boundaries, as tiled loads need it."""
+def _padded(t: torch.Tensor) -> bool:
+    """Whether a product takes a copy of ``t`` whose rows start on 16-byte boundaries, as tiled loads need it."""
     rows, cols = t.shape
-    if t.data_ptr() % 16 == 0 and (t.stride(0) % 8 == 0 and t.stride(0) >= cols or rows == 1):
-        return t
-    return _padded(t).copy_(t)
-
-
-def _padded(t: torch.Tensor) -> torch.Tensor:
-    return t.new_empty((t.shape[0], -(-t.shape[1] // 8) * 8))[:, :t.shape[1]]
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Elements between rows; of a single row any valid one."""
-    rows, cols = t.shape
-    return t.stride(0) if rows > 1 else -(-max(cols, 1) // 8) * 8
+    return t.data_ptr() % 16 != 0 or (rows > 1 and (t.stride(0) % 8 != 0 or t.stride(0) < cols))
 
 
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, act: str = "none",
@@ -127,18 +113,21 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     if z is not None:
         _result(z, (rows, cols), dev, "z", x, w, bias, resid)
     _l.require_cuda(x)
-    with _l.on_device(dev):
-        if out is None:
-            out = x.new_empty((rows, cols))
-        if keep and z is None:
-            z = x.new_empty((rows, cols))
-        if rows:
-            xt, wt = _tiled(x), _tiled(w)
-            _launch("aeris_linear_fwd", _FORWARD.pack(
-                xt.data_ptr(), wt.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if resid is None else resid.data_ptr(),
-                out.data_ptr(), z.data_ptr() if keep else 0, _pitch(xt), _pitch(wt), 0 if resid is None else _pitch(resid),
-                _pitch(out), _pitch(z) if keep else 0, rows, inner, cols, code, bias is not None and bias.dtype is _BF16,
-                _l.status_word(dev).data_ptr()))
+    if out is None:
+        out = x.new_empty((rows, cols))
+    if keep and z is None:
+        z = x.new_empty((rows, cols))
+    if rows:
+        work, n = None, 0
+        pad = _padded(x), _padded(w)
+        if pad[0] or pad[1]:
+            n = _bytes("aeris_linear_fwd_bytes", rows, inner, cols, *pad)
+            work = x.new_empty(n, dtype=torch.uint8)
+        _launch("aeris_linear_fwd", _FORWARD.pack(
+            x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if resid is None else resid.data_ptr(),
+            out.data_ptr(), z.data_ptr() if keep else 0, 0 if work is None else work.data_ptr(), _l.status_word(dev).data_ptr(),
+            x.stride(0), w.stride(0), 0 if resid is None else resid.stride(0), out.stride(0), z.stride(0) if keep else 0, n,
+            rows, inner, cols, code, bias is not None and bias.dtype is _BF16), dev)
     return out, z
 
 
@@ -172,38 +161,21 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, z: torch.Tens
         if any(t is not None and _l.share_memory(db, t) for t in (dy, x, w, z)):
             raise ValueError("db lies over an input")
     _l.require_cuda(x)
-    with _l.on_device(dev):
-        add_db = db is not None
-        if need_dx and dx is None:
-            dx = x.new_empty((rows, inner))
-        if bias and db is None:
-            db = (x.new_empty if rows else x.new_zeros)((cols,), dtype=_F32)
-        dw_f32 = dw is not None
-        if need_dw and dw is None:
-            dw = (x.new_empty if rows else x.new_zeros)((cols, inner))
-        if rows and (need_dx or need_dw or bias):
-            dz = _tiled(dy) if z is None and (need_dx or need_dw) else None
-            own = z is not None and (need_dx or need_dw)
-            if own:
-                dz = _padded(dy)
-            if own or bias:
-                slices = slices_for(rows, cols, _multiprocessors(dev.index))
-                work = x.new_empty((slices, cols), dtype=_F32) if bias else None
-                _launch("aeris_linear_dz", _DZ.pack(
-                    dy.data_ptr(), 0 if z is None else z.data_ptr(), dz.data_ptr() if own else 0, db.data_ptr() if bias else 0,
-                    work.data_ptr() if bias else 0, _pitch(dy), 0 if z is None else _pitch(z), _pitch(dz) if own else 0,
-                    rows, cols, code, add_db, slices))
-            if need_dx or need_dw:
-                n = _work_bytes(rows, inner, cols, dw_f32) if need_dw else 0
-                work = x.new_empty(n // 4, dtype=_F32) if n else None
-                wt, xt = _tiled(w) if need_dx else w, _tiled(x) if need_dw else x
-                _launch("aeris_linear_grad", _GRAD.pack(
-                    dz.data_ptr(), wt.data_ptr(), xt.data_ptr(), dx.data_ptr() if need_dx else 0, dw.data_ptr() if need_dw else 0,
-                    work.data_ptr() if n else 0, _pitch(dz), _pitch(wt), _pitch(xt), _pitch(dx) if need_dx else 0,
-                    _pitch(dw) if need_dw else 0, n, rows, inner, cols, dw_f32, _l.status_word(dev).data_ptr()))
+    add_db, dw_f32 = db is not None, dw is not None
+    make = x.new_empty if rows else x.new_zeros
+    if need_dx and dx is None:
+        dx = make((rows, inner))
+    if need_dw and dw is None:
+        dw = make((cols, inner))
+    if bias and db is None:
+        db = make((cols,), dtype=_F32)
+    if rows and (need_dx or need_dw or bias):
+        n = _bytes("aeris_linear_bwd_bytes", rows, inner, cols, z is not None or _padded(dy), _padded(x), _padded(w), need_dx, need_dw,
+                   bias, dw_f32)
+        work = x.new_empty(n, dtype=torch.uint8) if n else None
+        _launch("aeris_linear_bwd", _GRAD.pack(
+            dy.data_ptr(), x.data_ptr(), w.data_ptr(), 0 if z is None else z.data_ptr(), dx.data_ptr() if need_dx else 0,
+            dw.data_ptr() if need_dw else 0, db.data_ptr() if bias else 0, 0 if work is None else work.data_ptr(),
+            _l.status_word(dev).data_ptr(), dy.stride(0), x.stride(0), w.stride(0), 0 if z is None else z.stride(0),
+            dx.stride(0) if need_dx else 0, dw.stride(0) if need_dw else 0, n, rows, inner, cols, code, dw_f32, add_db), dev)
     return dx, dw, db
-
-
-def slices_for(rows: int, cols: int, multiprocessors: int) -> int:
-    """Slices of the rows whose column sums are taken apart: about eight blocks of 64 columns on every multiprocessor."""
-    return max(1, min(8 * multiprocessors * 64 // cols + 1, -(-rows // 32), 4096))

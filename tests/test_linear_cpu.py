@@ -91,7 +91,3 @@ def test_cpu_tensors_are_refused_and_not_computed_elsewhere():
     with pytest.raises(ValueError, match="GPU"):
         backward()
 
-
-def test_slices_cover_the_rows():
-    for rows, cols in ((1, 1), (64800, 4096), (2 ** 31 - 2 ** 12, 1)):
-        assert 1 <= LI.slices_for(rows, cols, 148) <= min(4096, -(-rows // 32))

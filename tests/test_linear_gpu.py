@@ -96,7 +96,8 @@ def laid_out(t, layout):
     return wide[:, at:at + cols]
 
 
-SIZES = [(1, 1, 1), (1, 64, 64), (1, 1536, 4096), (2, 3, 5), (7, 8, 16), (17, 100, 31), (33, 333, 777), (64, 64, 32), (100, 40, 130), (127, 65, 129),
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 1536, 4096), (2, 3, 5), (3, 1000, 70), (4, 300, 1), (5, 2000, 33), (6, 48, 500), (7, 8, 16), (8, 512, 333),
+         (8, 5120, 40), (9, 256, 256), (17, 100, 31), (33, 333, 777), (64, 64, 32), (100, 40, 130), (127, 65, 129),
          (128, 128, 128), (129, 256, 33), (200, 520, 256), (256, 512, 512), (300, 1000, 264), (513, 96, 1000), (1000, 777, 320),
          (2500, 128, 640), (5000, 48, 200)]
 
@@ -132,6 +133,17 @@ def test_layouts_of_inputs_and_results(rows, inner, cols, layout):
     dx, dw2, db2 = LI.linear_bwd(dy, x, w, z, act="silu", dx=place, dw=dw, db=db)
     assert dx is place and dw2 is dw and db2 is db
     backward_check(dy, x, w, z, "silu", dx, dw, db, base=2.0)
+
+
+def test_a_single_row_without_a_pitch():
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x, w, r = rnd(g, 72).to(BF).expand(1, 72), rnd(g, 72).to(BF).expand(1, 72), rnd(g, 1).to(BF).expand(1, 1)
+    y, z = LI.linear_fwd(x, w, resid=r, keep=True, act="silu", out=torch.empty(1, device=DEV, dtype=BF).expand(1, 1))
+    forward_check(x, w, None, "silu", r, y, z)
+    backward_check(r, x, w, z, "silu", *LI.linear_bwd(r, x, w, z, act="silu", dx=torch.empty(72, device=DEV, dtype=BF).expand(1, 72)))
+    many = rnd(g, 40, 72).to(BF)
+    y, z = LI.linear_fwd(many, w, keep=True)
+    forward_check(many, w, None, "none", None, y, z)
 
 
 def test_columns_beside_a_result_stay():
