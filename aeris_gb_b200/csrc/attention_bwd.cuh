@@ -692,6 +692,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       const uint64_t sl = f2_pack(p.scale_log2, p.scale_log2);
       Slot sb;
       for (int it = 0; it < n_items && ok; ++it) {
+        // first of all: the loads of this item wait for every warp to leave the last head's table, and its statistics come only
+        // after products of earlier items that are issued behind those loads
+        if constexpr (BIAS) {
+          if (!bias_of(item_at(it))) { ok = false; break; }
+        }
         if (!mbar_wait_warp(&bar->stat_full[sb.i], sb.ph, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
         const float nlse = -s_stat[sb.i * 2 * TILE + row], ndelta = -s_stat[sb.i * 2 * TILE + TILE + row];
         __syncwarp();
@@ -706,7 +711,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
           const int grow = w.tile * TILE + row;
           rest_in = grow < N;
           rest_at = ((static_cast<size_t>(ch * R::WPC + wg % R::WPC) * p.n_win + w.win) * p.H + w.head) * N + grow;
-          if (!bias_of(w)) { ok = false; break; }
         }
         for (; j < n_str; j += NCH, ph ^= 1) {
           if (!wait(&bar->s_full[ch], ph)) { ok = false; break; }

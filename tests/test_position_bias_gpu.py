@@ -266,6 +266,15 @@ def test_many_windows_and_many_heads():
     run_both(*make(1, (40, 40), 30, 16, g), 1, (40, 40), 30, 16)
 
 
+@pytest.mark.parametrize("n_win,window,heads,d", [(40, (8, 8), 24, 64), (30, (8, 8), 24, 128), (60, (3, 3), 40, 16), (20, (12, 12), 24, 32),
+                                                  (20, (9, 11), 24, 72), (25, (16, 20), 9, 64), (30, (13, 20), 10, 128), (10, (30, 30), 5, 64),
+                                                  (2, (8, 8), 300, 64), (1, (16, 17), 200, 32), (1, (20, 13), 160, 128), (6, (40, 40), 7, 64)])
+def test_several_heads_in_the_run_of_a_block(n_win, window, heads, d):
+    """More items than multiprocessors: blocks go from the table of one head to that of the next."""
+    g = torch.Generator(device=DEV).manual_seed(n_win)
+    run_both(*make(n_win, window, heads, d, g), n_win, window, heads, d)
+
+
 def test_same_bits_captured_and_on_another_stream():
     g = torch.Generator(device=DEV).manual_seed(8)
     qkv, table, buckets, d_o = make(20, (9, 16), 4, 64, g, 50)
