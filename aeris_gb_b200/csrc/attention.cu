@@ -24,8 +24,22 @@ constexpr int TILE = 128;
 struct PairBias {
   const float* table;
   const int* at;
-  int size, zero;
+  int size, zero;             // zero: also the place of the last token
+  int whole;                  // kernels that stay with a head: shared memory has room for its whole table, not only for a slice
 };
+// The entries that queries at places a0 .. a1 and all keys have, or keys at places a0 .. a1 and all queries: a slice of whole vectors.
+struct BiasSlice {
+  int first, n;
+};
+__host__ __device__ __forceinline__ BiasSlice bias_of_queries(int zero, int a0, int a1) {
+  const int lo = a0 & ~3;
+  return {lo, (zero + a1 - lo + 4) & ~3};
+}
+__host__ __device__ __forceinline__ BiasSlice bias_of_keys(int zero, int a0, int a1) {
+  const int lo = (zero - a1) & ~3;
+  return {lo, (2 * zero - a0 - lo + 4) & ~3};
+}
+__device__ __forceinline__ int place_words(int N) { return (N + 127) / 128 * 128; }
 
 struct AttnFwdParams {
   __nv_bfloat16* O;
@@ -174,10 +188,11 @@ template <int DCH, int MODE> struct AttnFwdRing {
 // product with both operands in shared memory reads 6 KB for 32 cycles of math, more than the 128 B/cycle the shared
 // memory delivers, so the kernel with P in shared memory (16 KB written and 16 KB read back per tile, on top of
 // Q, K and V) is bound by shared-memory bandwidth rather than by the tensor or the exp unit.
-// BIAS: scores are biased by relative position (PairBias) on their way out of TMEM. The table of a head is read through L1, whose
-// lanes ask for neighbouring entries (their rows are neighbours); a column's place is the same for all lanes. A row that
-// sees no key has a sum of zero: zeros, and +infinity for its lse, which makes exp(score - lse) zero in the backward pass.
-template <int DCH, int POLY, int MODE, bool BIAS = false>
+// BIASED: scores are biased by relative position (PairBias) on their way out of TMEM, from the tile's slice of the head's table in
+// shared memory (1) or, where that has no room for it and the tokens' places, through L1 (2). Lanes ask for neighbouring
+// entries, their rows being neighbours; a column's place is the same for all lanes. A row that sees no key has a sum of zero:
+// zeros, and +infinity for its lse, which makes exp(score - lse) zero in the backward pass.
+template <int DCH, int POLY, int MODE, int BIASED = 0>
 __global__ void __launch_bounds__(ATT_THREADS, AttnFwdRing<DCH, MODE>::MIN_CTAS)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const AttnFwdParams p) {
@@ -188,6 +203,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // the V tile of the same step, so its successor is requested that much earlier and the load latency hides behind
   // the softmax of the tiles in between.
   constexpr bool PTMEM = MODE != 0;
+  constexpr bool BIAS = BIASED != 0;
   constexpr int NSK = AttnFwdRing<DCH, MODE>::NSK, NSV = AttnFwdRing<DCH, MODE>::NSV;
   constexpr int P_BYTES = PTMEM ? 0 : 16384;   // [128 x 64] bf16
   constexpr int TMEM_COLS = (DCH == 1) ? 128 : 256;
@@ -206,6 +222,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* s_free = bars + 18;    // every softmax warp has read them into registers
   uint64_t* p_full = bars + 19;    // probabilities of tile j are in shared memory
   uint64_t* pv_done = bars + 20;   // P V of tile j has completed (P buffer reusable, accumulator up to date)
+  [[maybe_unused]] uint64_t* bias_full = bars + 25;      // places and table slice, behind the barriers
+  [[maybe_unused]] int* s_at = reinterpret_cast<int*>(bars + 32);
   static_assert(NSK <= 4 && NSV <= 4, "barrier slots");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
@@ -235,6 +253,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // would run a tile ahead of the others and its arrivals would complete a phase that belongs to the slower warps
     const int n_valid_warps = min(4, (N - qt * TILE + 31) / 32);
     mbar_init(s_full, 1); mbar_init(s_free, n_valid_warps); mbar_init(p_full, n_valid_warps); mbar_init(pv_done, 1);
+    if constexpr (BIASED == 1) mbar_init(bias_full, 1);
     fence_barrier_init();
   }
   if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
@@ -252,6 +271,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < DCH; ++c)
         tma_load_4d(sQ + c * 16384, &tm_q, q_full, c * 64, head, qt * TILE, win);
+      if constexpr (BIASED == 1) {
+        const BiasSlice b = bias_of_queries(p.bias.zero, p.bias.at[qt * TILE], p.bias.at[min(qt * TILE + TILE, N) - 1]);
+        const uint32_t words = place_words(N);
+        mbar_expect_tx(bias_full, 4 * (words + b.n));
+        bulk_load(s_at, p.bias.at, 4 * words, bias_full);
+        bulk_load(s_at + words, p.bias.table + static_cast<size_t>(head) * p.bias.size + b.first, 4 * b.n, bias_full);
+      }
       // K_i, then V_{i-1}: the order in which their slots come free (K_i after Q K^T of tile i - NSK, V_{i-1} after P V
       // of tile i - 1 - NSV, which completes later), so no wait holds up a load whose slot is already free
       for (int i = 0; i <= nkv; ++i) {
@@ -338,7 +364,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
     [[maybe_unused]] const float* bias = nullptr;       // of this row: bias[-at[j]]
-    if constexpr (BIAS) bias = p.bias.table + static_cast<size_t>(head) * p.bias.size + p.bias.zero + p.bias.at[min(grow, N - 1)];
+    [[maybe_unused]] const int* at = p.bias.at;
+    if constexpr (BIASED == 1) {
+      ok = !warp_valid || mbar_wait(bias_full, 0, p.status, ERR_TIMEOUT_ATTN);
+      at = s_at;
+      bias = reinterpret_cast<const float*>(s_at + place_words(N)) - (p.bias.at[qt * TILE] & ~3) + p.bias.zero + p.bias.at[min(grow, N - 1)];
+    } else if constexpr (BIASED == 2) {
+      bias = p.bias.table + static_cast<size_t>(head) * p.bias.size + p.bias.zero + at[min(grow, N - 1)];
+    }
     // Raises the reference maximum to m_new: rescales the TMEM accumulator (once P V of the previous tile is done) and l.
     auto rescale = [&](int j, float m_new, bool& waited) -> bool {
       if (j > 0) {
@@ -381,10 +414,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         if (warp_valid) {
           if constexpr (BIAS) {
-            const int4* at = reinterpret_cast<const int4*>(p.bias.at + j * KVT);
+            const int4* places = reinterpret_cast<const int4*>(at + j * KVT);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int4 a = at[i], b = at[8 + i];
+              const int4 a = places[i], b = places[8 + i];
               v0[4 * i] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i]), sl2, bias[-a.x]));
               v0[4 * i + 1] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i + 1]), sl2, bias[-a.y]));
               v0[4 * i + 2] = __float_as_uint(fmaf(__uint_as_float(v0[4 * i + 2]), sl2, bias[-a.z]));
@@ -470,7 +503,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float s = __uint_as_float(v[i]);
-              if constexpr (BIAS) s = fmaf(s, sl2, bias[-p.bias.at[j * KVT + c + i]]);
+              if constexpr (BIAS) s = fmaf(s, sl2, bias[-at[j * KVT + c + i]]);
               if (c + i < rem) mx = fmaxf(mx, s);
             }
           }
@@ -492,9 +525,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             for (int i = 0; i < 8; ++i) {
               float p0, p1;
               if constexpr (BIAS) {
-                const int* at = p.bias.at + j * KVT + c + 2 * i;
-                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, bias[-at[0]]) - m);
-                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, bias[-at[1]]) - m);
+                const int* a = at + j * KVT + c + 2 * i;
+                p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, bias[-a[0]]) - m);
+                p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, bias[-a[1]]) - m);
               } else {
                 p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), sl2, -m_ref));
                 p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -m_ref));
@@ -575,13 +608,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
 static int g_fwd_smem_pad = 0;   // extra dynamic shared memory per CTA: lowers the number of CTAs per SM (measurements)
 
-template <int DCH, int POLY, int MODE, bool BIAS = false>
+template <int DCH, int POLY, int MODE, int BIASED = 0>
 static int launch_attn_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                           const AttnFwdParams& p, cudaStream_t stream) {
+                           const AttnFwdParams& p, cudaStream_t stream, int bias_bytes = 0) {
   constexpr int SMEM = DCH * 16384 + (AttnFwdRing<DCH, MODE>::NSK + AttnFwdRing<DCH, MODE>::NSV) * DCH * 8192 +
                        (MODE != 0 ? 0 : 16384) + 256;
   static std::atomic<uint64_t> done{0};
-  auto kern = attn_fwd_kernel<DCH, POLY, MODE, BIAS>;
+  auto kern = attn_fwd_kernel<DCH, POLY, MODE, BIASED>;
+  if constexpr (BIASED == 1) {
+    if (SMEM + bias_bytes > 227 * 1024 || !allow_smem_once(kern, 227 * 1024, done)) return -20;
+    return launch_chained(kern, dim3((p.N + TILE - 1) / TILE, p.H, p.n_win), ATT_THREADS, SMEM + bias_bytes, stream, tq, tk, tv, p);
+  }
   const int smem = SMEM + g_fwd_smem_pad;
   if (g_fwd_smem_pad) done.store(0);        // a measurement: asked for anew
   if (!allow_smem_once(kern, smem, done)) return -20;
@@ -732,15 +769,30 @@ static int attn_fwd_impl(const void* q, int ldq, int q_col0, const void* k, int 
   return poly ? launch_attn_fwd<1, 2, 0>(tq, tk, tv, p, stream) : launch_attn_fwd<1, -1, 0>(tq, tk, tv, p, stream);
 }
 
+// Floats of the largest slice that `rows` neighbouring tokens need of a head's table (as many as keys need for as many).
+template <typename F>
+static int slice_of_rows(F&& at_of, int N, int zero, int rows) {
+  int most = 0;
+  for (int r = 0; r < N; r += rows) {
+    const int a0 = at_of(r), a1 = at_of(r + rows < N ? r + rows - 1 : N - 1);
+    const int q = bias_of_queries(zero, a0, a1).n, k = bias_of_keys(zero, a0, a1).n;
+    most = most > q ? most : q;
+    most = most > k ? most : k;
+  }
+  return most;
+}
+
 int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int N, int H, int head_dim, float scale,
-                           const float* table, const int* at, int size, int zero, int* status, void* stream_) {
+                           const float* table, const int* at, int wide, int pitch, int size, int* status, void* stream_) {
+  auto at_of = [&](int t) { return t / wide * pitch + t % wide; };
+  const int zero = at_of(N - 1);
   if (head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
   if (n_win <= 0 || N <= 0 || H <= 0 || n_win > 65535 || H > 65535) return -2;
   if (!o || !whole_vectors(o, ldo)) return -4;
   AttnFwdParams p{};
   p.O = reinterpret_cast<__nv_bfloat16*>(o); p.ldo = ldo; p.lse = lse; p.N = N; p.H = H; p.n_win = n_win; p.d = head_dim;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
-  p.bias = {table, at, size, zero};
+  p.bias = {table, at, size, zero, 1};
   const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(qkv);
   CUtensorMap tq, tk, tv;
   int r;
@@ -748,15 +800,22 @@ int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse
   if ((r = make_tmap_heads_bf16(&tk, b + H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
   if ((r = make_tmap_heads_bf16(&tv, b + 2 * H * head_dim, head_dim, H, N, n_win, ld, KVT))) return r;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const int room = 4 * size + (N + 127) / 128 * 512;
-  if (head_dim <= 64 && N > 2 * TILE && room <= AttnQuad<2>::TABLE) {
-    CUtensorMap to;
-    if ((r = make_tmap_heads32_bf16(&to, o, head_dim, H, N, n_win, ldo, 32))) return r;
-    return room <= AttnQuad<1>::TABLE ? launch_attn_fwd_quad<1>(tq, tk, tv, to, p, stream)
-                                      : launch_attn_fwd_quad<2>(tq, tk, tv, to, p, stream);
+  const int places = (N + 127) / 128 * 512;
+  // Four query tiles at a time where a window has three; the whole table or what four tiles need of it beside the places.
+  if (head_dim <= 64 && N > 2 * TILE) {
+    const int whole = 4 * size + places, slice = 4 * slice_of_rows(at_of, N, zero, 4 * TILE) + places;
+    p.bias.whole = whole <= AttnQuad<2>::TABLE;
+    if (slice <= AttnQuad<2>::TABLE) {
+      CUtensorMap to;
+      if ((r = make_tmap_heads32_bf16(&to, o, head_dim, H, N, n_win, ldo, 32))) return r;
+      return whole <= AttnQuad<1>::TABLE ? launch_attn_fwd_quad<1>(tq, tk, tv, to, p, stream)
+                                         : launch_attn_fwd_quad<2>(tq, tk, tv, to, p, stream);
+    }
   }
-  return head_dim > 64 ? launch_attn_fwd<2, -1, 1, true>(tq, tk, tv, p, stream)
-                       : launch_attn_fwd<1, -1, 1, true>(tq, tk, tv, p, stream);
+  const int bytes = 4 * slice_of_rows(at_of, N, zero, TILE) + places;
+  if (head_dim > 64)
+    return bytes <= 120 * 1024 ? launch_attn_fwd<2, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<2, -1, 1, 2>(tq, tk, tv, p, stream);
+  return bytes <= 120 * 1024 ? launch_attn_fwd<1, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<1, -1, 1, 2>(tq, tk, tv, p, stream);
 }
 
 // Whether the backward kernels can count their items, and a CTA the tiles it streams past them, in 32 bits.
@@ -774,10 +833,20 @@ static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v
                          int push_n_local, int push_ld, int push_sec_w, int push_col0, const PairBias* bias = nullptr,
                          float* rest = nullptr);
 
+static int bias_room(int head_dim) {
+  const int a = head_dim <= 64 ? BwdCfg<1, false, 1>::TABLE : BwdCfg<2, false, 1>::TABLE;
+  const int b = head_dim <= 64 ? BwdCfg<1, true, 1>::TABLE : BwdCfg<2, true, 1>::TABLE;
+  return a < b ? a : b;
+}
+
 int aeris::attn_bwd_biased(const void* qkv, int ldq, const void* o, const void* d_o, int ldo, const float* lse, float* delta, float* rest,
                            void* dqkv, int ldg, int n_win, int N, int H, int head_dim, float scale, const float* table,
-                           const int* at, int size, int zero, int* status, void* stream_) {
-  const PairBias bias{table, at, size, zero};
+                           const int* at, int wide, int pitch, int size, int* status, void* stream_) {
+  auto at_of = [&](int t) { return t / wide * pitch + t % wide; };
+  const int zero = at_of(N - 1), places = (N + 127) / 128 * 512, room = bias_room(head_dim);
+  // the whole table, or what a tile needs of it, beside the places; or neither (-1)
+  const int whole = 4 * size + places <= room ? 1 : 4 * slice_of_rows(at_of, N, zero, TILE) + places <= room ? 0 : -1;
+  const PairBias bias{table, at, size, zero, whole};
   return attn_bwd_impl(qkv, ldq, 0, H * head_dim, 2 * H * head_dim, o, d_o, ldo, lse, delta, dqkv, ldg, n_win, N, H, head_dim, scale,
                        status, stream_, nullptr, 0, 0, 0, 0, 0, &bias, rest);
 }
@@ -841,12 +910,10 @@ static int attn_bwd_impl(const void* qkv, int ldq, int q_col0, int k_col0, int v
   if (bias) {
     p.bias = *bias;
     p.rest = rest;
-    const int room = 4 * p.bias.size + (N + 127) / 128 * 512;
     if (head_dim <= 64)
-      return room <= BwdCfg<1, false, 1>::TABLE && room <= BwdCfg<1, true, 1>::TABLE
-                 ? launch_attn_bwd<1, 1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
-                 : launch_attn_bwd<1, 2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
-    return room <= BwdCfg<2, false, 1>::TABLE && room <= BwdCfg<2, true, 1>::TABLE
+      return bias->whole >= 0 ? launch_attn_bwd<1, 1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
+                              : launch_attn_bwd<1, 2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
+    return bias->whole >= 0
                ? launch_attn_bwd<2, 1>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream)
                : launch_attn_bwd<2, 2>(q128, k64, v64, d128, q64, k128, v128, d64, out, p, stream);
   }

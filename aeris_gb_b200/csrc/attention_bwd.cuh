@@ -210,7 +210,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_failed = s_abort + 1;      // [4] see note_failure
-  [[maybe_unused]] float* s_table = reinterpret_cast<float*>(smem + R::SMEM);      // [p.bias.size], then places
+  [[maybe_unused]] int* s_at = reinterpret_cast<int*>(smem + R::SMEM);      // places, then the table or a slice of it
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int N = p.N;
@@ -226,6 +226,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
     n_items = static_cast<int>(static_cast<long long>(n_items_total) * (blockIdx.x + 1) / n_ctas) - item0;
   }
   const int total = n_items * n_str;
+  // what an item needs of its head's table
+  [[maybe_unused]] auto bias_slice = [&](const BwdItem& w) -> BiasSlice {
+    if (p.bias.whole > 0) return {0, p.bias.size};
+    const int a0 = p.bias.at[w.tile * TILE], a1 = p.bias.at[min(w.tile * TILE + TILE, N) - 1];
+    return DKV ? bias_of_keys(p.bias.zero, a0, a1) : bias_of_queries(p.bias.zero, a0, a1);
+  };
   auto item_at = [&](int it) -> BwdItem {
     if constexpr (BIAS) return bwd_bias_item(item0 + it, row_tiles, p.n_win);
     else return bwd_item(it, row_tiles, p.H);
@@ -306,16 +312,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
         const BwdItem w = item_at(it);
         if constexpr (BIASED == 1) {
           // the table of a head, once the math warps are through with the one before; with the first the tokens' places
-          if (w.head != head) {
+          if (w.head != head || !p.bias.whole) {
             if (head >= 0) {
               if (!wait(&bar->bias_empty, bias_ph)) { ok = false; break; }
               bias_ph ^= 1;
             }
             if (lane == 0) {
-              const uint32_t bytes = p.bias.size * 4, at_bytes = head < 0 ? (N + 127) / 128 * 512 : 0;
-              mbar_expect_tx(&bar->bias_full, bytes + at_bytes);
-              bulk_load(s_table, p.bias.table + static_cast<size_t>(w.head) * p.bias.size, bytes, &bar->bias_full);
-              if (at_bytes) bulk_load(s_table + p.bias.size, p.bias.at, at_bytes, &bar->bias_full);
+              const uint32_t words = place_words(N), b = head < 0 ? 4 * words : 0;
+              const BiasSlice s = bias_slice(w);
+              mbar_expect_tx(&bar->bias_full, 4 * s.n + b);
+              if (b) bulk_load(s_at, p.bias.at, b, &bar->bias_full);
+              bulk_load(s_at + words, p.bias.table + static_cast<size_t>(w.head) * p.bias.size + s.first, 4 * s.n, &bar->bias_full);
             }
             head = w.head;
           }
@@ -663,7 +670,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
     [[maybe_unused]] uint32_t bias_ph = 0;
     [[maybe_unused]] auto bias_of = [&](const BwdItem& w) -> bool {
       if constexpr (BIASED == 1) {
-        if (w.head != head) {       // this warp is through with the table before
+        if (w.head != head || !p.bias.whole) {       // this warp is through with the table before
           if (head >= 0) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->bias_empty);
@@ -672,14 +679,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
           if (!mbar_wait_warp(&bar->bias_full, bias_ph, p.status, ERR_TIMEOUT_ATTN)) return false;
           bias_ph ^= 1;
         }
-        tab = s_table;
-        at = reinterpret_cast<const int*>(s_table + p.bias.size);
+        at = s_at;
+        tab = reinterpret_cast<const float*>(s_at + place_words(N));
       } else {
         tab = p.bias.table + static_cast<size_t>(w.head) * p.bias.size;
         at = p.bias.at;
       }
       const int place = at[min(w.tile * TILE + row, N - 1)];
-      mine = DKV ? p.bias.zero - place : p.bias.zero + place;
+      mine = (DKV ? p.bias.zero - place : p.bias.zero + place) - (BIASED == 1 ? bias_slice(w).first : 0);
       return true;
     };
     // CPT columns to registers

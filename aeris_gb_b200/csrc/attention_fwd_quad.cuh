@@ -73,7 +73,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_failed = s_abort + 1;      // [16] see note_failure
-  [[maybe_unused]] const float* s_table = reinterpret_cast<const float*>(smem + R::SMEM);      // [p.bias.size], then places
+  [[maybe_unused]] const int* s_at = reinterpret_cast<const int*>(smem + R::SMEM);      // places, then the table or a slice of it
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int N = p.N;
@@ -90,6 +90,12 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     n_items = static_cast<int>(static_cast<long long>(n_items_total) * (blockIdx.x + 1) / n_ctas) - item0;
   }
   const int total = n_items * nkv;
+  // what an item needs of its head's table
+  [[maybe_unused]] auto bias_slice = [&](const PairItem& w) -> BiasSlice {
+    if (p.bias.whole) return {0, p.bias.size};
+    const int r0 = w.pair * NC * TILE;
+    return bias_of_queries(p.bias.zero, p.bias.at[r0], p.bias.at[min(r0 + NC * TILE, N) - 1]);
+  };
   auto item_at = [&](int it) -> PairItem {
     if constexpr (BIAS) return bias_item(item0 + it, n_groups, p.n_win);
     else return pair_item(it, n_groups, p.H);
@@ -144,16 +150,17 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       [[maybe_unused]] int head = -1;
       [[maybe_unused]] uint32_t bias_ph = 0;
       [[maybe_unused]] auto load_table = [&](const PairItem& w) -> bool {
-        if (w.head == head) return true;
+        if (w.head == head && p.bias.whole) return true;
         if (head >= 0) {
           if (!mbar_wait_warp(&bar->bias_empty, bias_ph, p.status, ERR_TIMEOUT_ATTN)) return false;
           bias_ph ^= 1;
         }
         if (lane == 0) {
-          const uint32_t bytes = p.bias.size * 4, at_bytes = head < 0 ? (N + 127) / 128 * 512 : 0;
-          mbar_expect_tx(&bar->bias_full, bytes + at_bytes);
-          bulk_load(smem + R::SMEM, p.bias.table + static_cast<size_t>(w.head) * p.bias.size, bytes, &bar->bias_full);
-          if (at_bytes) bulk_load(smem + R::SMEM + bytes, p.bias.at, at_bytes, &bar->bias_full);
+          const uint32_t at_bytes = 4 * place_words(N), b = head < 0 ? at_bytes : 0;
+          const BiasSlice s = bias_slice(w);
+          mbar_expect_tx(&bar->bias_full, 4 * s.n + b);
+          if (b) bulk_load(smem + R::SMEM, p.bias.at, b, &bar->bias_full);
+          bulk_load(smem + R::SMEM + at_bytes, p.bias.table + static_cast<size_t>(w.head) * p.bias.size + s.first, 4 * s.n, &bar->bias_full);
         }
         head = w.head;
         return true;
@@ -317,11 +324,11 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     PairItem prev{0, 0, 0};
     [[maybe_unused]] int head = -1;
     [[maybe_unused]] uint32_t bias_ph = 0;
-    [[maybe_unused]] const int* s_at = reinterpret_cast<const int*>(s_table + p.bias.size);
+    [[maybe_unused]] const float* s_table = reinterpret_cast<const float*>(s_at + place_words(N));
     for (int it = 0; it < n_items && ok; ++it) {
       const PairItem w = item_at(it);
       if constexpr (BIAS) {
-        if (w.head != head) {       // the warp is through with the table before
+        if (w.head != head || !p.bias.whole) {       // the warp is through with the table before
           if (head >= 0) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->bias_empty);
@@ -336,7 +343,7 @@ attn_fwd_quad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if (qt >= q_tiles) continue;
       const bool rows = qt * TILE + q * 32 < N;
       [[maybe_unused]] int mine = 0;          // entry of this row's query and a key at place 0
-      if constexpr (BIAS) mine = p.bias.zero + s_at[min(qt * TILE + q * 32 + lane, N - 1)];
+      if constexpr (BIAS) mine = p.bias.zero + s_at[min(qt * TILE + q * 32 + lane, N - 1)] - bias_slice(w).first;
       for (int j = 0; j < nkv; ++j) {
         ok = mbar_wait_warp(&bar->s_full[c], s_ph, p.status, ERR_TIMEOUT_ATTN);
         if (!ok) break;

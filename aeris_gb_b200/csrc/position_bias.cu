@@ -513,7 +513,7 @@ extern "C" int aeris_biased_attn_fwd(const AerisBiasedAttn* a, void* stream_) {
   int r = expand(a, p, table, at, stream);
   if (r) return r;
   r = attn_fwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, static_cast<int>(a->ld_o), a->lse, a->n_win, p.n, a->heads, a->head_dim,
-                      a->scale, table, at, p.size, p.zero, a->status, stream);
+                      a->scale, table, at, a->wide, p.pitch, p.size, a->status, stream);
   return r ? r - 100 : 2;
 }
 
@@ -532,7 +532,7 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   if (r) return r;
   r = attn_bwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, a->d_o, static_cast<int>(a->ld_o), a->lse, delta,
                       reinterpret_cast<float*>(work + w.rest), a->dqkv, static_cast<int>(a->ld_dqkv), a->n_win, p.n, a->heads,
-                      a->head_dim, a->scale, table, at, p.size, p.zero, a->status, stream);
+                      a->head_dim, a->scale, table, at, a->wide, p.pitch, p.size, a->status, stream);
   if (r) return r - 100;
   int count = 4;
   if (!sums) return count;
