@@ -298,7 +298,7 @@ typedef struct AerisBiasedAttn {
   const void* d_o;                  // backward: pitch of o
   void* dqkv;
   float* dtable;                    // [table_rows, heads], added to with `add`; null: not wanted
-  void* work;                       // aeris_biased_attn_work_bytes, from a 256-byte boundary on
+  void* work;                       // aeris_biased_attn_work_bytes (may be none), from a 256-byte boundary on
   int* status;
   long long ld_qkv, ld_o, ld_dqkv, work_bytes;
   int n_win, high, wide, heads, head_dim, table_rows, table_bf16, buckets64, add;

@@ -13,6 +13,7 @@
 #include "common.cuh"
 #include "api.h"
 #include "host.h"
+#include "position_bias.cuh"
 
 namespace aeris {
 
@@ -54,6 +55,7 @@ struct AttnFwdParams {
   void* o_peers[8];
   int push_n_local, push_ld, push_col0;
   PairBias bias;               // kernels with BIAS
+  BiasSource source;
 };
 
 // Byte offset of 16-byte vector `v` (0..7) of row `r` inside a [rows x 64] bf16 tile stored with the 128-byte swizzle.
@@ -189,7 +191,8 @@ template <int DCH, int MODE> struct AttnFwdRing {
 // memory delivers, so the kernel with P in shared memory (16 KB written and 16 KB read back per tile, on top of
 // Q, K and V) is bound by shared-memory bandwidth rather than by the tensor or the exp unit.
 // BIASED: scores are biased by relative position (PairBias) on their way out of TMEM, from the tile's slice of the head's table in
-// shared memory (1) or, where that has no room for it and the tokens' places, through L1 (2). Lanes ask for neighbouring
+// shared memory, copied (1) or, where that saves a launch more than it costs, made from the learned table (3); or, where there is
+// no room for it and the tokens' places, through L1 (2). Lanes ask for neighbouring
 // entries, their rows being neighbours; a column's place is the same for all lanes. A row that sees no key has a sum of zero:
 // zeros, and +infinity for its lse, which makes exp(score - lse) zero in the backward pass.
 template <int DCH, int POLY, int MODE, int BIASED = 0>
@@ -262,6 +265,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   chain_point();
+  if constexpr (BIASED == 3) {
+    const BiasSource& s = p.source;
+    const BiasSlice b = bias_of_queries(p.bias.zero, s.at(qt * TILE), s.at(min(qt * TILE + TILE, N) - 1));
+    const int words = place_words(N);
+    for (int i = threadIdx.x; i < words; i += ATT_THREADS) s_at[i] = s.at(min(i, N - 1));
+    for (int i = threadIdx.x; i < b.n; i += ATT_THREADS) reinterpret_cast<float*>(s_at + words)[i] = s.entry(b.first + i, head);
+    __syncthreads();
+  }
   const uint32_t tS = tmem_base;          // S : 64 columns
   const uint32_t tO = tmem_base + 64;     // O : HD columns, accumulated over all tiles
 
@@ -365,10 +376,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     bool ok = true;
     [[maybe_unused]] const float* bias = nullptr;       // of this row: bias[-at[j]]
     [[maybe_unused]] const int* at = p.bias.at;
-    if constexpr (BIASED == 1) {
-      ok = !warp_valid || mbar_wait(bias_full, 0, p.status, ERR_TIMEOUT_ATTN);
+    if constexpr (BIASED == 1 || BIASED == 3) {
+      if constexpr (BIASED == 1) ok = !warp_valid || mbar_wait(bias_full, 0, p.status, ERR_TIMEOUT_ATTN);
       at = s_at;
-      bias = reinterpret_cast<const float*>(s_at + place_words(N)) - (p.bias.at[qt * TILE] & ~3) + p.bias.zero + p.bias.at[min(grow, N - 1)];
+      if (ok)
+        bias = reinterpret_cast<const float*>(s_at + place_words(N)) - (s_at[qt * TILE] & ~3) + p.bias.zero + s_at[min(grow, N - 1)];
     } else if constexpr (BIASED == 2) {
       bias = p.bias.table + static_cast<size_t>(head) * p.bias.size + p.bias.zero + at[min(grow, N - 1)];
     }
@@ -615,7 +627,7 @@ static int launch_attn_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const C
                        (MODE != 0 ? 0 : 16384) + 256;
   static std::atomic<uint64_t> done{0};
   auto kern = attn_fwd_kernel<DCH, POLY, MODE, BIASED>;
-  if constexpr (BIASED == 1) {
+  if constexpr (BIASED == 1 || BIASED == 3) {
     if (SMEM + bias_bytes > 227 * 1024 || !allow_smem_once(kern, 227 * 1024, done)) return -20;
     return launch_chained(kern, dim3((p.N + TILE - 1) / TILE, p.H, p.n_win), ATT_THREADS, SMEM + bias_bytes, stream, tq, tk, tv, p);
   }
@@ -782,17 +794,29 @@ static int slice_of_rows(F&& at_of, int N, int zero, int rows) {
   return most;
 }
 
-int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int N, int H, int head_dim, float scale,
-                           const float* table, const int* at, int wide, int pitch, int size, int* status, void* stream_) {
-  auto at_of = [&](int t) { return t / wide * pitch + t % wide; };
-  const int zero = at_of(N - 1);
+constexpr int SLICE_BYTES = 120 * 1024;      // the most that a tile's slice and the places may take beside the operands
+
+// Whether the forward pass makes its tables from the learned one: in the kernels of one query tile, where that comes to fewer reads than a
+// launch of its own is worth (2 us; 16 windows of 8 x 8, 2 heads: 5.5 -> @ us).
+bool aeris::biased_fwd_reads_source(int n_win, int H, int head_dim, const BiasSource& s) {
+  const int N = s.high * s.wide, zero = s.at(N - 1);
+  if (head_dim <= 64 && N > 2 * TILE) return false;
+  const long long slice = slice_of_rows([&](int t) { return s.at(t); }, N, zero, TILE), tiles = (N + TILE - 1) / TILE;
+  return 4 * slice + (N + 127) / 128 * 512 <= SLICE_BYTES && slice * tiles * H * n_win <= 2 << 20;
+}
+
+int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int H, int head_dim, float scale,
+                           const BiasSource& source, const float* table, const int* at, int size, void* stream_) {
+  auto at_of = [&](int t) { return source.at(t); };
+  const int N = source.high * source.wide, zero = at_of(N - 1);
   if (head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
   if (n_win <= 0 || N <= 0 || H <= 0 || n_win > 65535 || H > 65535) return -2;
   if (!o || !whole_vectors(o, ldo)) return -4;
   AttnFwdParams p{};
   p.O = reinterpret_cast<__nv_bfloat16*>(o); p.ldo = ldo; p.lse = lse; p.N = N; p.H = H; p.n_win = n_win; p.d = head_dim;
-  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = source.status;
   p.bias = {table, at, size, zero, 1};
+  p.source = source;
   const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(qkv);
   CUtensorMap tq, tk, tv;
   int r;
@@ -802,7 +826,7 @@ int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   const int places = (N + 127) / 128 * 512;
   // Four query tiles at a time where a window has three; the whole table or what four tiles need of it beside the places.
-  if (head_dim <= 64 && N > 2 * TILE) {
+  if (table && head_dim <= 64 && N > 2 * TILE) {
     const int whole = 4 * size + places, slice = 4 * slice_of_rows(at_of, N, zero, 4 * TILE) + places;
     p.bias.whole = whole <= AttnQuad<2>::TABLE;
     if (slice <= AttnQuad<2>::TABLE) {
@@ -813,9 +837,13 @@ int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse
     }
   }
   const int bytes = 4 * slice_of_rows(at_of, N, zero, TILE) + places;
+  if (!table) {
+    if (bytes > SLICE_BYTES) return -5;
+    return head_dim > 64 ? launch_attn_fwd<2, -1, 1, 3>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<1, -1, 1, 3>(tq, tk, tv, p, stream, bytes);
+  }
   if (head_dim > 64)
-    return bytes <= 120 * 1024 ? launch_attn_fwd<2, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<2, -1, 1, 2>(tq, tk, tv, p, stream);
-  return bytes <= 120 * 1024 ? launch_attn_fwd<1, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<1, -1, 1, 2>(tq, tk, tv, p, stream);
+    return bytes <= SLICE_BYTES ? launch_attn_fwd<2, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<2, -1, 1, 2>(tq, tk, tv, p, stream);
+  return bytes <= SLICE_BYTES ? launch_attn_fwd<1, -1, 1, 1>(tq, tk, tv, p, stream, bytes) : launch_attn_fwd<1, -1, 1, 2>(tq, tk, tv, p, stream);
 }
 
 // Whether the backward kernels can count their items, and a CTA the tiles it streams past them, in 32 bits.
@@ -840,15 +868,15 @@ static int bias_room(int head_dim) {
 }
 
 int aeris::attn_bwd_biased(const void* qkv, int ldq, const void* o, const void* d_o, int ldo, const float* lse, float* delta, float* rest,
-                           void* dqkv, int ldg, int n_win, int N, int H, int head_dim, float scale, const float* table,
-                           const int* at, int wide, int pitch, int size, int* status, void* stream_) {
-  auto at_of = [&](int t) { return t / wide * pitch + t % wide; };
-  const int zero = at_of(N - 1), places = (N + 127) / 128 * 512, room = bias_room(head_dim);
+                           void* dqkv, int ldg, int n_win, int H, int head_dim, float scale, const BiasSource& source,
+                           const float* table, const int* at, int size, void* stream_) {
+  auto at_of = [&](int t) { return source.at(t); };
+  const int N = source.high * source.wide, zero = at_of(N - 1), places = (N + 127) / 128 * 512, room = bias_room(head_dim);
   // the whole table, or what a tile needs of it, beside the places; or neither (-1)
   const int whole = 4 * size + places <= room ? 1 : 4 * slice_of_rows(at_of, N, zero, TILE) + places <= room ? 0 : -1;
   const PairBias bias{table, at, size, zero, whole};
   return attn_bwd_impl(qkv, ldq, 0, H * head_dim, 2 * H * head_dim, o, d_o, ldo, lse, delta, dqkv, ldg, n_win, N, H, head_dim, scale,
-                       status, stream_, nullptr, 0, 0, 0, 0, 0, &bias, rest);
+                       source.status, stream_, nullptr, 0, 0, 0, 0, 0, &bias, rest);
 }
 
 extern "C" int aeris_attn_bwd(const void* qkv, int ldq, int q_col0, int k_col0, int v_col0, const void* o,

@@ -27,12 +27,4 @@ int choose_k_splits(int tiles, int kb_total, int units, int most, int want);
 int gemm_one_cta(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc, int a_mn, int b_mn,
                  int epi, const void* resid, int ldr, const float* gate, int rows_per_gate, int ld_gate, void* aux,
                  int ld_aux, int swiglu_f, int k_splits, int bn, int* status, void* stream);
-// Window attention with scores biased by relative position (attention.cu): fused qkv rows as aeris_attn_fwd and _bwd, q in the first
-// columns; table, at, size: PairBias there, for windows of rows of `wide` tokens in a table of rows of `pitch`. delta, rest: scratch of one and four floats per (window, head, token);
-// delta holds dO . O afterwards, exact but for fp32 roundings.
-int attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int N, int H, int head_dim, float scale,
-                    const float* table, const int* at, int wide, int pitch, int size, int* status, void* stream);
-int attn_bwd_biased(const void* qkv, int ldq, const void* o, const void* d_o, int ldo, const float* lse, float* delta, float* rest,
-                    void* dqkv, int ldg, int n_win, int N, int H, int head_dim, float scale, const float* table, const int* at,
-                    int wide, int pitch, int size, int* status, void* stream);
 }  // namespace aeris

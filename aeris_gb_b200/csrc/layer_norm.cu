@@ -168,19 +168,20 @@ extern "C" int aeris_layer_norm_bwd(const AerisLayerNorm* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!ln_fits(a) || !a->dy || a->ld_dy < 0) return -1;
   const bool sums = a->dw || a->db;
-  if (sums != (a->work != nullptr) || (sums && (a->slices <= 0 || a->slices > 65535))) return -2;
+  if (sums && (a->slices <= 0 || a->slices > 65535 || (a->slices > 1) != (a->work != nullptr))) return -2;
   int n = 1, slices = a->slices;
   int r = a->f32 ? ln_bwd_fast<float>(*a, stream, slices) : ln_bwd_fast<__nv_bfloat16>(*a, stream, slices);
   if (r < 0) return r;
   const bool fast = r == 0;
   if (!fast && sums) {     // first: the gradient of x may take the place of x or dy
+    if (!a->work) return -3;
     const dim3 grid((a->cols + LN_COLS - 1) / LN_COLS, a->slices);
     r = a->f32 ? launch_chained(ln_sums_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
                : launch_chained(ln_sums_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);
     if (r) return r;
     ++n;
   }
-  if (sums) {
+  if (sums && a->work) {
     r = launch_chained(ln_join_kernel, dim3((a->cols + 31) / 32, 2), 1024, 0, stream, *a, slices);
     if (r) return r;
     ++n;

@@ -212,6 +212,12 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) ln_fwd_one_kernel(const Ae
   if (lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mean, rstd);
 }
 
+// The column sums of the only block.
+__device__ __forceinline__ void column_sums(const AerisLayerNorm& a, int c, float dw, float db) {
+  if (a.dw) a.dw[c] = a.add ? a.dw[c] + dw : dw;
+  if (a.db) a.db[c] = a.add ? a.db[c] + db : db;
+}
+
 // The groups' column sums, one after the other so that the order of additions is fixed, and the block's slice of `work`.
 template <typename F>
 __device__ __forceinline__ void join_groups(const AerisLayerNorm& a, float* joined, int group, int groups, F&& each) {
@@ -222,6 +228,10 @@ __device__ __forceinline__ void join_groups(const AerisLayerNorm& a, float* join
         joined[a.cols + c] = t ? joined[a.cols + c] + db : db;
       });
     __syncthreads();
+  }
+  if (!a.work) {
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) column_sums(a, c, joined[c], joined[a.cols + c]);
+    return;
   }
   float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
   for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) out[c] = joined[c];
@@ -322,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNo
       }
     }
   }
-  if (!a.work) return;
+  if (!a.dw && !a.db) return;
   auto each = [&](auto&& put) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -339,8 +349,12 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNo
   if constexpr (BLOCK) {
     float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
     each([&](int c, float dw_, float db_) {
-      out[c] = dw_;
-      out[a.cols + c] = db_;
+      if (!a.work) {
+        column_sums(a, c, dw_, db_);
+      } else {
+        out[c] = dw_;
+        out[a.cols + c] = db_;
+      }
     });
   } else {
     join_groups(a, joined, group, groups, each);
@@ -409,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLay
       }
     }
   }
-  if (!a.work) return;
+  if (!a.dw && !a.db) return;
   auto each = [&](auto&& put) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -420,8 +434,12 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLay
   if constexpr (BLOCK) {
     float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
     each([&](int c, float dw_, float db_) {
-      out[c] = dw_;
-      out[a.cols + c] = db_;
+      if (!a.work) {
+        column_sums(a, c, dw_, db_);
+      } else {
+        out[c] = dw_;
+        out[a.cols + c] = db_;
+      }
     });
   } else {
     join_groups(a, joined, group, groups, each);
@@ -489,9 +507,10 @@ int launch_ln_bwd(const AerisLayerNorm& a, LnCut cut, int threads, cudaStream_t 
   // as many blocks as the SMs hold (MIN, more of narrower ones)
   long long blocks = static_cast<long long>(num_sms()) * (MIN * THREADS / threads);
   if (blocks > need) blocks = need;
-  if (a.work && blocks > a.slices) blocks = a.slices;
+  const bool sums = a.dw || a.db;
+  if (sums && blocks > a.slices) blocks = a.slices;
   slices = static_cast<int>(blocks);
-  const int smem = !BLOCK && a.work ? 2 * a.cols * 4 : 0;
+  const int smem = !BLOCK && sums ? 2 * a.cols * 4 : 0;
   if constexpr (W > 1)
     return launch_chained(ln_bwd_kernel<T, W, NV, R, BLOCK, THREADS, MIN>, slices, threads, smem, stream, a, cut);
   else

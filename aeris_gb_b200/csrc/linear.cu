@@ -716,7 +716,8 @@ __device__ __forceinline__ float bf(unsigned short u) { return __uint_as_float(s
 struct DzParams {
   const void *dy, *z;
   void* dz;
-  float* work;              // [gridDim.y, cols], or null
+  float* sums;              // [gridDim.y, cols], or null
+  int add;                  // one slice: whether sums is added to
   long long ld_dy, ld_z, ld_dz;
   int rows, cols;
 };
@@ -768,14 +769,15 @@ __global__ void __launch_bounds__(DZ_THREADS, ACT == LIN_ACT_NONE ? 5 : 3) lin_d
         }
     }
   }
-  if (!a.work) return;
+  if (!a.sums) return;
 #pragma unroll
   for (int i = 0; i < V; ++i) part[r0][c0 + i] = s[i];
   __syncthreads();
   if (threadIdx.x < DZ_COLS && blockIdx.x * DZ_COLS + threadIdx.x < a.cols) {
     float t = 0.f;
     for (int r = 0; r < R; ++r) t += part[r][threadIdx.x];
-    a.work[static_cast<long long>(blockIdx.y) * a.cols + blockIdx.x * DZ_COLS + threadIdx.x] = t;
+    float* out = a.sums + static_cast<long long>(blockIdx.y) * a.cols + blockIdx.x * DZ_COLS + threadIdx.x;
+    *out = a.add ? *out + t : t;
   }
 }
 
@@ -915,6 +917,7 @@ int operand(Operand& o, const void* p, long long ld, int rows, int cols, uint8_t
 
 // Slices of the rows whose column sums are taken apart: about sixteen blocks of 64 columns on every multiprocessor.
 int db_slices(int rows, int cols) {
+  if (rows <= (cols % 8 ? 32 : 256)) return 1;        // over before a second launch would begin
   const long long most = 16ll * num_sms() * DZ_COLS / cols + 1, need = (rows + 31ll) / 32;
   return static_cast<int>(most < need ? (most < 4096 ? most : 4096) : (need < 4096 ? need : 4096));
 }
@@ -955,7 +958,8 @@ extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
 extern "C" long long aeris_linear_bwd_bytes(int rows, int inner, int cols, int own_dz, int pad_x, int pad_w, int dx, int dw, int db,
                                             int dw_f32) {
   if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
-  long long n = db ? up(4ll * db_slices(rows, cols) * cols) : 0;
+  const int slices = db_slices(rows, cols);
+  long long n = db && slices > 1 ? up(4ll * slices * cols) : 0;
   if (own_dz && (dx || dw)) n += up(2 * padded(cols) * rows);
   if (dx && pad_w) n += up(2 * padded(inner) * cols);
   if (dw) n += (pad_x ? up(2 * padded(inner) * rows) : 0) + up(dw_bytes(rows, inner, cols, dw_f32));
@@ -976,10 +980,13 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   int n = 0, r;
   Operand dz{a->dy, pitch(a->ld_dy, rows, cols)};
   if (own_dz || a->db) {
-    DzParams d{a->dy, a->z, nullptr, nullptr, a->ld_dy, a->ld_z, padded(cols), rows, cols};
+    DzParams d{a->dy, a->z, nullptr, nullptr, 0, a->ld_dy, a->ld_z, padded(cols), rows, cols};
     const int slices = db_slices(rows, cols);
-    if (a->db) {
-      d.work = reinterpret_cast<float*>(work + at);
+    if (a->db && slices == 1) {
+      d.sums = a->db;
+      d.add = a->add_db;
+    } else if (a->db) {
+      d.sums = reinterpret_cast<float*>(work + at);
       at += up(4ll * slices * cols);
     }
     if (own_dz) {
@@ -991,8 +998,8 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
     const dim3 grid((cols + DZ_COLS - 1) / DZ_COLS, slices);
     if ((r = vec ? launch_dz<8>(d, a->act, grid, stream) : launch_dz<1>(d, a->act, grid, stream))) return r;
     ++n;
-    if (a->db) {
-      r = launch_chained(lin_join_sums_kernel, (cols + 31) / 32, DZ_THREADS, 0, stream, static_cast<const float*>(d.work), a->db, slices, cols,
+    if (a->db && slices > 1) {
+      r = launch_chained(lin_join_sums_kernel, (cols + 31) / 32, DZ_THREADS, 0, stream, static_cast<const float*>(d.sums), a->db, slices, cols,
                          a->add_db);
       if (r) return r;
       ++n;

@@ -12,12 +12,12 @@
 #include "common.cuh"
 #include "api.h"
 #include "host.h"
+#include "position_bias.cuh"
 
 namespace aeris {
 
 namespace {
 
-constexpr float HIDDEN = -1e30f;
 constexpr int PB_TILE = 128;
 
 struct Place {
@@ -35,34 +35,16 @@ Place place_of(int high, int wide) {
   p.at_words = (p.n + 127) / 128 * 128;
   return p;
 }
+BiasSource source_of(const AerisBiasedAttn* a, const Place& p) {
+  return {a->table, a->buckets, a->table_rows, a->heads, a->high, a->wide, p.pitch, a->table_bf16, a->buckets64, a->status};
+}
 
 // The tables by relative position [heads, size] in log2 units, and the places of the tokens.
-__global__ void __launch_bounds__(256) bias_expand_kernel(const AerisBiasedAttn a, float* out, int* at, const Place pl) {
+__global__ void __launch_bounds__(256) bias_expand_kernel(const BiasSource s, float* out, int* at, const Place pl) {
   chain_point();
   const int i = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
-  if (i < pl.size) {
-    const int r = i / pl.pitch, c = i - r * pl.pitch;
-    float v = 0.f;                // between the rows: not read
-    if (r < 2 * a.high - 1 && c < 2 * a.wide - 1) {
-      const int k = r * (2 * a.wide - 1) + c;
-      long long b = k;
-      if (a.buckets)
-        b = a.buckets64 ? static_cast<const long long*>(a.buckets)[k] : static_cast<const int*>(a.buckets)[k];
-      if (b >= 0 && b < a.table_rows) {
-        const long long e = b * a.heads + head;
-        v = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e]) : static_cast<const float*>(a.table)[e];
-        v = v <= HIDDEN ? -INFINITY : v * 1.4426950408889634f;
-      } else {
-        v = -INFINITY;
-        if (a.status) atomicCAS(a.status, 0, ERR_BOUNDS);
-      }
-    }
-    out[static_cast<long long>(head) * pl.size + i] = v;
-  }
-  if (head == 0 && i < pl.at_words) {
-    const int t = i < pl.n ? i : pl.n - 1, y = t / a.wide;
-    at[i] = y * pl.pitch + t - y * a.wide;
-  }
+  if (i < pl.size) out[static_cast<long long>(head) * pl.size + i] = s.entry(i, head);
+  if (head == 0 && i < pl.at_words) at[i] = s.at(i < pl.n ? i : pl.n - 1);
 }
 
 // ------------------------------------------------------------------------------------------ sums of dS over windows
@@ -466,13 +448,13 @@ Work work_of(int n_win, int high, int wide, int heads, int head_dim, bool backwa
 bool fits(const AerisBiasedAttn* a) {
   return a->n_win > 0 && a->high > 0 && a->wide > 0 && a->heads > 0 && a->head_dim > 0 && a->n_win <= 65535 && a->heads <= 65535 &&
          a->high <= 32768 && a->wide <= 32768 && static_cast<long long>(a->high) * a->wide <= 32768 && a->table && a->table_rows > 0 &&
-         a->work && (reinterpret_cast<uintptr_t>(a->work) & 255) == 0 && a->ld_qkv <= 0x7fffffff && a->ld_o <= 0x7fffffff &&
+         (reinterpret_cast<uintptr_t>(a->work) & 255) == 0 && a->ld_qkv <= 0x7fffffff && a->ld_o <= 0x7fffffff &&
          a->ld_dqkv <= 0x7fffffff;
 }
 
-int expand(const AerisBiasedAttn* a, const Place& p, float* table, int* at, cudaStream_t stream) {
+int expand(const BiasSource& s, const Place& p, float* table, int* at, cudaStream_t stream) {
   const int most = p.size > p.at_words ? p.size : p.at_words;
-  return launch_chained(bias_expand_kernel, dim3((most + 255) / 256, a->heads), 256, 0, stream, *a, table, at, p);
+  return launch_chained(bias_expand_kernel, dim3((most + 255) / 256, s.heads), 256, 0, stream, s, table, at, p);
 }
 
 template <int DCH>
@@ -498,22 +480,33 @@ using namespace aeris;
 
 extern "C" long long aeris_biased_attn_work_bytes(int n_win, int high, int wide, int heads, int head_dim, int backward, int with_table) {
   if (n_win <= 0 || high <= 0 || wide <= 0 || heads <= 0 || head_dim <= 0 || static_cast<long long>(high) * wide > 32768) return -1;
+  if (!backward) {
+    BiasSource s{};
+    s.high = high; s.wide = wide; s.pitch = place_of(high, wide).pitch;
+    if (biased_fwd_reads_source(n_win, heads, head_dim, s)) return 0;
+  }
   return work_of(n_win, high, wide, heads, head_dim, backward, with_table).total;
 }
 
 extern "C" int aeris_biased_attn_fwd(const AerisBiasedAttn* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!fits(a)) return -1;
-  const Work w = work_of(a->n_win, a->high, a->wide, a->heads, a->head_dim, false, false);
-  if (a->work_bytes < w.total) return -2;
   const Place p = place_of(a->high, a->wide);
+  const BiasSource source = source_of(a, p);
+  if (biased_fwd_reads_source(a->n_win, a->heads, a->head_dim, source)) {
+    const int r = attn_fwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, static_cast<int>(a->ld_o), a->lse, a->n_win, a->heads,
+                                  a->head_dim, a->scale, source, nullptr, nullptr, p.size, stream);
+    return r ? r - 100 : 1;
+  }
+  const Work w = work_of(a->n_win, a->high, a->wide, a->heads, a->head_dim, false, false);
+  if (!a->work || a->work_bytes < w.total) return -2;
   uint8_t* work = static_cast<uint8_t*>(a->work);
   float* table = reinterpret_cast<float*>(work + w.table);
   int* at = reinterpret_cast<int*>(work + w.at);
-  int r = expand(a, p, table, at, stream);
+  int r = expand(source, p, table, at, stream);
   if (r) return r;
-  r = attn_fwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, static_cast<int>(a->ld_o), a->lse, a->n_win, p.n, a->heads, a->head_dim,
-                      a->scale, table, at, a->wide, p.pitch, p.size, a->status, stream);
+  r = attn_fwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, static_cast<int>(a->ld_o), a->lse, a->n_win, a->heads, a->head_dim,
+                      a->scale, source, table, at, p.size, stream);
   return r ? r - 100 : 2;
 }
 
@@ -522,17 +515,18 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   if (!fits(a) || !a->d_o || !a->dqkv || !a->lse) return -1;
   const bool sums = a->dtable != nullptr;
   const Work w = work_of(a->n_win, a->high, a->wide, a->heads, a->head_dim, true, sums);
-  if (a->work_bytes < w.total) return -2;
+  if (!a->work || a->work_bytes < w.total) return -2;
   const Place p = place_of(a->high, a->wide);
+  const BiasSource source = source_of(a, p);
   uint8_t* work = static_cast<uint8_t*>(a->work);
   float* table = reinterpret_cast<float*>(work + w.table);
   int* at = reinterpret_cast<int*>(work + w.at);
   float* delta = reinterpret_cast<float*>(work + w.delta);
-  int r = expand(a, p, table, at, stream);
+  int r = expand(source, p, table, at, stream);
   if (r) return r;
   r = attn_bwd_biased(a->qkv, static_cast<int>(a->ld_qkv), a->o, a->d_o, static_cast<int>(a->ld_o), a->lse, delta,
-                      reinterpret_cast<float*>(work + w.rest), a->dqkv, static_cast<int>(a->ld_dqkv), a->n_win, p.n, a->heads,
-                      a->head_dim, a->scale, table, at, a->wide, p.pitch, p.size, a->status, stream);
+                      reinterpret_cast<float*>(work + w.rest), a->dqkv, static_cast<int>(a->ld_dqkv), a->n_win, a->heads,
+                      a->head_dim, a->scale, source, table, at, p.size, stream);
   if (r) return r - 100;
   int count = 4;
   if (!sums) return count;

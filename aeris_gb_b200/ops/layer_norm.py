@@ -38,44 +38,50 @@ def _multiprocessors(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-def _launch(name: str, record: bytes, dev) -> None:
-    if torch._C._cuda_getDevice() == dev.index:
+def _launch(name: str, record: bytes, index: int) -> None:
+    if torch._C._cuda_getDevice() == index:
         rc = _entry(name)(record, _l.raw_stream())
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = _entry(name)(record, _l.raw_stream())
     _l.check(min(rc, 0), name, kernels=max(rc, 0))
 
 
+def _vector(t, cols: int, index: int) -> bool:
+    return t.shape == (cols,) and t.dtype in _FLOATS and t.get_device() == index and t.is_contiguous()
+
+
 def _check(x, w, b):
-    """Refuses what the kernels cannot take of the inputs that both directions share; returns (shape, pitch, type, device)."""
-    shape, dt, dev = x.shape, x.dtype, x.device
-    if len(shape) != 2 or dt not in _FLOATS:
+    """Refuses what the kernels cannot take of the inputs that both directions share; returns (rows, cols, pitch, type, device index).
+    Every attribute is asked for once: they are half of a small call."""
+    dt, index = x.dtype, x.get_device()
+    if x.ndim != 2 or dt not in _FLOATS:
         raise ValueError(f"x [rows, cols] in bf16 or fp32, got {_text(x)}")
-    rows, cols = shape
+    rows, cols = x.shape
     if rows > MAX_ROWS or not 0 < cols <= MAX_COLS:
         raise ValueError(f"{rows} rows of {cols} columns: at most {MAX_ROWS} of 1 to {MAX_COLS} are taken")
     pitch, one = x.stride()
-    if (one != 1 and cols > 1) or pitch < 0:
+    if one != 1 and cols > 1:
         raise ValueError(f"columns lie side by side, got {_text(x)}")
-    for t in (w, b):
-        if t is not None and not (t.shape == (cols,) and t.dtype in _FLOATS and t.device == dev and t.is_contiguous()):
-            raise ValueError(f"weight and bias: bf16 or fp32 [{cols}] on {dev}, got {_text(t)}")
+    if w is not None and not _vector(w, cols, index) or b is not None and not _vector(b, cols, index):
+        raise ValueError(f"weight and bias: contiguous bf16 or fp32 [{cols}] on {x.device}, got {_text(w)} and {_text(b)}")
     if w is not None and b is not None and w.dtype is not b.dtype:
         raise ValueError(f"weight and bias are of one type, got {w.dtype} and {b.dtype}")
-    return rows, cols, pitch, dt, dev
+    return rows, cols, pitch, dt, index
 
 
-def _like(t, shape, dt, dev, what: str) -> int:
+def _like(t, shape, dt, index, what: str) -> int:
     """Pitch of a second matrix of the same form."""
-    if not (t.shape == shape and t.dtype is dt and t.device == dev and (t.stride(1) == 1 or shape[1] == 1) and t.stride(0) >= 0):
-        raise ValueError(f"{what}: {dt} {tuple(shape)} on {dev} with columns side by side, got {_text(t)}")
-    return t.stride(0)
+    if t.shape == shape and t.dtype is dt and t.get_device() == index:
+        pitch, one = t.stride()
+        if one == 1 or shape[1] == 1:
+            return pitch
+    raise ValueError(f"{what}: {dt} {tuple(shape)} on the device of x with columns side by side, got {_text(t)}")
 
 
-def _result(t, shape, dt, dev, what: str, *inputs) -> int:
+def _result(t, shape, dt, index, what: str, *inputs) -> int:
     """Pitch of a matrix that is written: rows apart, and in the place of an input only element by element."""
-    pitch = _like(t, shape, dt, dev, what)
+    pitch = _like(t, shape, dt, index, what)
     if shape[0] > 1 and pitch < shape[1]:
         raise ValueError(f"{what}: rows lie over one another, got {_text(t)}")
     for i in inputs:
@@ -89,25 +95,29 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     """``x`` [rows, cols] bf16 or fp32, rows of any pitch (a section of a wider matrix). Returns (normed rows in x's type, fp32
     [rows, 2]: mean and 1 / sqrt(var + eps) of every row, which :func:`layer_norm_bwd` takes). ``weight``, ``bias`` [cols] bf16 or
     fp32, each may be missing. ``out`` may be ``x`` itself."""
-    rows, cols, pitch, dt, dev = _check(x, weight, bias)
+    rows, cols, pitch, dt, index = _check(x, weight, bias)
     if out is not None:
-        pitch_out = _result(out, x.shape, dt, dev, "out", x, weight, bias)
+        pitch_out = _result(out, x.shape, dt, index, "out", x, weight, bias)
     if stats is not None:
-        if not (stats.shape == (rows, 2) and stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous()):
-            raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {dev}, got {_text(stats)}")
+        if not _stats(stats, rows, index):
+            raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {x.device}, got {_text(stats)}")
         if any(t is not None and _l.share_memory(stats, t) for t in (x, weight, bias, out)):
             raise ValueError("stats lie over another tensor of the call")
     _l.require_cuda(x)
     if out is None:
-        out, pitch_out = x.new_empty((rows, cols)), cols
+        out, pitch_out = (torch.empty_like(x) if pitch == cols else x.new_empty((rows, cols))), cols
     if stats is None:
         stats = x.new_empty((rows, 2), dtype=torch.float32)
     if rows:
         w_f32 = (weight if weight is not None else bias if bias is not None else x).dtype is torch.float32
         _launch("aeris_layer_norm_fwd", _RECORD.pack(
             x.data_ptr(), 0, out.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            stats.data_ptr(), 0, 0, 0, rows, pitch, 0, max(pitch_out, cols), cols, dt is torch.float32, w_f32, 0, 0, eps), dev)
+            stats.data_ptr(), 0, 0, 0, rows, pitch, 0, max(pitch_out, cols), cols, dt is torch.float32, w_f32, 0, 0, eps), index)
     return out, stats
+
+
+def _stats(t, rows: int, index: int) -> bool:
+    return t.shape == (rows, 2) and t.dtype is torch.float32 and t.get_device() == index and t.is_contiguous()
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: torch.Tensor | None = None, *,
@@ -117,47 +127,54 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
     result. Returns (gradient of x in x's type, fp32 gradient of the weight or None without one, fp32 gradient of the bias or None
     with ``bias=False``). ``dx`` may be ``dy`` or ``x`` itself; ``dw``, ``db`` [cols] fp32 are added to where given. The same
     bits on every run; tensors whose rows start elsewhere may be added up in another order."""
-    rows, cols, pitch, dt, dev = _check(x, weight, None)
-    pitch_dy = _like(dy, x.shape, dt, dev, "dy")
-    if not (stats.shape == (rows, 2) and stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous()):
-        raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {dev}, got {_text(stats)}")
-    if weight is None and dw is not None or not bias and db is not None:
-        raise ValueError("a gradient to add to without the parameter")
+    rows, cols, pitch, dt, index = _check(x, weight, None)
+    shape = x.shape
+    pitch_dy = _like(dy, shape, dt, index, "dy")
+    if not _stats(stats, rows, index):
+        raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {x.device}, got {_text(stats)}")
     add = dw is not None or db is not None
-    if add and ((weight is not None) != (dw is not None) or bias != (db is not None)):
-        raise ValueError("dw and db come together")
-    for t in (dw, db):
-        if t is not None and not (t.shape == (cols,) and t.dtype is torch.float32 and t.device == dev and t.is_contiguous()):
-            raise ValueError(f"dw and db: contiguous fp32 [{cols}] on {dev}, got {_text(t)}")
-    if add and dw is not None and db is not None and _l.share_memory(dw, db):
-        raise ValueError("dw and db are in the same memory")
+    if add:
+        if weight is None and dw is not None or not bias and db is not None:
+            raise ValueError("a gradient to add to without the parameter")
+        if (weight is not None) != (dw is not None) or bias != (db is not None):
+            raise ValueError("dw and db come together")
+        for t in (dw, db):
+            if t is not None and not (_vector(t, cols, index) and t.dtype is torch.float32):
+                raise ValueError(f"dw and db: contiguous fp32 [{cols}] on {x.device}, got {_text(t)}")
+        if dw is not None and db is not None and _l.share_memory(dw, db):
+            raise ValueError("dw and db are in the same memory")
+        if any(_l.share_memory(t, u) for t in (dw, db) if t is not None for u in (dy, x, stats, weight) if u is not None):
+            raise ValueError("dw or db lies over an input")
     if dx is not None:
-        pitch_dx = _result(dx, x.shape, dt, dev, "dx", dy, x)
+        pitch_dx = _result(dx, shape, dt, index, "dx", dy, x)
         if any(t is not None and _l.share_memory(dx, t) for t in (stats, weight, dw, db)):
             raise ValueError("dx lies over another tensor of the call")
-    if add and any(_l.share_memory(t, u) for t in (dw, db) if t is not None for u in (dy, x, stats, weight) if u is not None):
-        raise ValueError("dw or db lies over an input")
     _l.require_cuda(x)
     if dx is None:
-        dx, pitch_dx = x.new_empty((rows, cols)), cols
+        dx, pitch_dx = (torch.empty_like(x) if pitch == cols else x.new_empty((rows, cols))), cols
     if not add:
         make = x.new_empty if rows else x.new_zeros
-        dw = make((cols,), dtype=torch.float32) if weight is not None else None
-        db = make((cols,), dtype=torch.float32) if bias else None
+        if weight is not None:
+            dw = make((cols,), dtype=torch.float32)
+        if bias:
+            db = make((cols,), dtype=torch.float32)
     if rows:
-        slices = 0
-        work = None
+        slices, work = 0, None
         if dw is not None or db is not None:
-            slices = slices_for(rows, _multiprocessors(dev.index))
-            work = x.new_empty((slices, 2, cols), dtype=torch.float32)
+            slices = slices_for(rows, cols, _multiprocessors(index))
+            if slices > 1:
+                work = x.new_empty((slices, 2, cols), dtype=torch.float32)
         _launch("aeris_layer_norm_bwd", _RECORD.pack(
             x.data_ptr(), dy.data_ptr(), dx.data_ptr(), 0 if weight is None else weight.data_ptr(), 0, stats.data_ptr(),
             0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), 0 if work is None else work.data_ptr(),
             rows, pitch, pitch_dy, max(pitch_dx, cols), cols, dt is torch.float32, weight is not None and weight.dtype is torch.float32,
-            add, slices, 0.0), dev)
+            add, slices, 0.0), index)
     return dx, dw, db
 
 
-def slices_for(rows: int, multiprocessors: int) -> int:
-    """Slices of the rows whose column sums may be taken apart: four blocks on every multiprocessor, four rows each."""
-    return max(1, min(4 * multiprocessors, -(-rows // 4)))
+def slices_for(rows: int, cols: int, multiprocessors: int) -> int:
+    """Slices of the rows whose column sums may be taken apart: four blocks on every multiprocessor, four rows each. One for what a
+    single block is through with before a second launch would begin (221 x 35, bf16: @ us a call for @)."""
+    if rows * cols <= 2 ** 14 and cols <= 4096:
+        return 1
+    return max(2, min(4 * multiprocessors, -(-rows // 4)))

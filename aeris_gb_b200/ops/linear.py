@@ -22,6 +22,7 @@ MOST = 2 ** 31 - 2 ** 12         # rows, columns
 _FORWARD = struct.Struct("8P6q5i0q")
 _GRAD = struct.Struct("9P7q6i0q")
 _BF16, _F32 = torch.bfloat16, torch.float32
+_BIAS = (_F32, _BF16)
 
 
 def _text(t) -> str:
@@ -41,53 +42,57 @@ def _bytes(name: str, *sizes: int) -> int:
     return _entry(name, len(sizes))(*sizes)
 
 
-def _launch(name: str, record: bytes, dev) -> None:
-    if torch._C._cuda_getDevice() == dev.index:
+def _launch(name: str, record: bytes, index: int) -> None:
+    if torch._C._cuda_getDevice() == index:
         rc = _entry(name)(record, _l.raw_stream())
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = _entry(name)(record, _l.raw_stream())
     _l.check(min(rc, 0), name, kernels=max(rc, 0))
 
 
-def _matrix(t, shape, dev, what: str, dtypes=(_BF16,)) -> None:
-    if not (t.dim() == 2 and t.shape == shape and t.dtype in dtypes and t.device == dev):
-        raise ValueError(f"{what}: {dtypes[0]} {tuple(shape)} on {dev}, got {_text(t)}")
-    if (t.stride(1) != 1 and shape[1] > 1) or t.stride(0) < 0:
-        raise ValueError(f"{what}: columns lie side by side, got {_text(t)}")
+def _matrix(t, shape, index: int, what: str, dtype=_BF16) -> int:
+    """Pitch of a matrix of the given shape. Every attribute is asked for once: they are half of a small call."""
+    if t.shape == shape and t.dtype is dtype and t.get_device() == index and t.ndim == 2:
+        pitch, one = t.stride()
+        if one == 1 or shape[1] == 1:
+            return pitch
+    raise ValueError(f"{what}: {dtype} {tuple(shape)} on one device with the others, columns side by side, got {_text(t)}")
 
 
-def _result(t, shape, dev, what: str, *others, dtypes=(_BF16,), inside=None) -> None:
+def _result(t, shape, index: int, what: str, *others, dtype=_BF16, inside=None) -> int:
     """``inside``: the one input that the result may take the place of, element by element."""
-    _matrix(t, shape, dev, what, dtypes)
-    if shape[0] > 1 and t.stride(0) < shape[1]:
+    pitch = _matrix(t, shape, index, what, dtype)
+    if shape[0] > 1 and pitch < shape[1]:
         raise ValueError(f"{what}: rows lie over one another, got {_text(t)}")
     for o in others:
         if o is not None and _l.share_memory(t, o) and not (o is inside and _l.same_memory(t, o)):
             raise ValueError(f"{what} lies over another tensor of the call: {_text(t)}, {_text(o)}")
+    return pitch
 
 
 def _check(x, w):
-    if x.dim() != 2 or w.dim() != 2 or x.dtype is not _BF16:
+    """(rows, inner, columns, pitches of x and w, device index)"""
+    if x.ndim != 2 or w.ndim != 2 or x.dtype is not _BF16:
         raise ValueError(f"x [rows, inner] and w [cols, inner] in bf16, got {_text(x)} and {_text(w)}")
-    (rows, inner), cols, dev = x.shape, w.shape[0], x.device
-    if max(rows, inner, cols) > MOST or inner < 1 or cols < 1:
-        raise ValueError(f"x {tuple(x.shape)}, w {tuple(w.shape)}: 1 to {MOST} of each (rows: none, too)")
-    _matrix(x, (rows, inner), dev, "x")
-    _matrix(w, (cols, inner), dev, "w")
-    return rows, inner, cols, dev
+    shape, other, index = x.shape, w.shape, x.get_device()
+    rows, inner = shape
+    cols, _ = other
+    if not (rows <= MOST and 0 < inner <= MOST and 0 < cols <= MOST):
+        raise ValueError(f"x {tuple(shape)}, w {tuple(other)}: 1 to {MOST} of each (rows: none, too)")
+    return rows, inner, cols, _matrix(x, shape, index, "x"), _matrix(w, (cols, inner), index, "w"), index
 
 
 def _act_code(act: str) -> int:
-    if act not in _ACT:
+    code = _ACT.get(act)
+    if code is None:
         raise ValueError(f"act is one of {', '.join(ACTIVATIONS)}, got {act!r}")
-    return _ACT[act]
+    return code
 
 
-def _padded(t: torch.Tensor) -> bool:
-    """Whether a product takes a copy of ``t`` whose rows start on 16-byte boundaries, as tiled loads need it."""
-    rows, cols = t.shape
-    return t.data_ptr() % 16 != 0 or (rows > 1 and (t.stride(0) % 8 != 0 or t.stride(0) < cols))
+def _padded(at: int, rows: int, cols: int, pitch: int) -> bool:
+    """Whether a product takes a copy of a matrix whose rows start on 16-byte boundaries, as tiled loads need it."""
+    return at % 16 != 0 or (rows > 1 and (pitch % 8 != 0 or pitch < cols))
 
 
 def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, *, act: str = "none",
@@ -100,34 +105,35 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
 
     Any sizes and pitches. Rows that start on 16-byte boundaries are fastest: others of ``x`` and ``w`` are copied first, others of
     the results are written element by element."""
-    rows, inner, cols, dev = _check(x, w)
+    rows, inner, cols, x_pitch, w_pitch, index = _check(x, w)
     code = _act_code(act)
-    if bias is not None and not (bias.shape == (cols,) and bias.dtype in (_F32, _BF16) and bias.device == dev and bias.is_contiguous()):
-        raise ValueError(f"bias: contiguous fp32 or bf16 [{cols}] on {dev}, got {_text(bias)}")
-    if resid is not None:
-        _matrix(resid, (rows, cols), dev, "resid")
+    shape = (rows, cols)
+    if bias is not None and not (bias.shape == (cols,) and bias.dtype in _BIAS and bias.get_device() == index and bias.is_contiguous()):
+        raise ValueError(f"bias: contiguous fp32 or bf16 [{cols}] on {x.device}, got {_text(bias)}")
+    r_pitch = 0 if resid is None else _matrix(resid, shape, index, "resid")
     if z is not None and not keep:
         raise ValueError("z is written with keep=True")
+    y_pitch = z_pitch = cols
     if out is not None:
-        _result(out, (rows, cols), dev, "out", x, w, bias, resid, z, inside=resid)
+        y_pitch = _result(out, shape, index, "out", x, w, bias, resid, z, inside=resid)
     if z is not None:
-        _result(z, (rows, cols), dev, "z", x, w, bias, resid)
+        z_pitch = _result(z, shape, index, "z", x, w, bias, resid)
     _l.require_cuda(x)
     if out is None:
-        out = x.new_empty((rows, cols))
+        out = x.new_empty(shape)
     if keep and z is None:
-        z = x.new_empty((rows, cols))
+        z = x.new_empty(shape)
     if rows:
-        work, n = None, 0
-        pad = _padded(x), _padded(w)
+        at, w_at, work, n = x.data_ptr(), w.data_ptr(), 0, 0
+        pad = _padded(at, rows, inner, x_pitch), _padded(w_at, cols, inner, w_pitch)
         if pad[0] or pad[1]:
             n = _bytes("aeris_linear_fwd_bytes", rows, inner, cols, *pad)
-            work = x.new_empty(n, dtype=torch.uint8)
+            buffer = x.new_empty(n, dtype=torch.uint8)
+            work = buffer.data_ptr()
         _launch("aeris_linear_fwd", _FORWARD.pack(
-            x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if resid is None else resid.data_ptr(),
-            out.data_ptr(), z.data_ptr() if keep else 0, 0 if work is None else work.data_ptr(), _l.status_word(dev).data_ptr(),
-            x.stride(0), w.stride(0), 0 if resid is None else resid.stride(0), out.stride(0), z.stride(0) if keep else 0, n,
-            rows, inner, cols, code, bias is not None and bias.dtype is _BF16), dev)
+            at, w_at, 0 if bias is None else bias.data_ptr(), 0 if resid is None else resid.data_ptr(), out.data_ptr(),
+            z.data_ptr() if keep else 0, work, _l.status_word(x.device).data_ptr(), x_pitch, w_pitch, r_pitch, y_pitch, z_pitch, n,
+            rows, inner, cols, code, bias is not None and bias.dtype is _BF16), index)
     return out, z
 
 
@@ -140,28 +146,35 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, z: torch.Tens
     fp32, are added to where given. The same bits on every run.
 
     The gradient of z is rounded to bf16 for both products; ``db`` sums it before."""
-    rows, inner, cols, dev = _check(x, w)
+    rows, inner, cols, x_pitch, w_pitch, index = _check(x, w)
     code = _act_code(act)
-    _matrix(dy, (rows, cols), dev, "dy")
-    if act != "none":
+    shape = (rows, cols)
+    dy_pitch = _matrix(dy, shape, index, "dy")
+    z_pitch = 0
+    if code:
         if z is None:
             raise ValueError(f"act={act!r}: the backward pass takes z, the values before the activation")
-        _matrix(z, (rows, cols), dev, "z")
+        z_pitch = _matrix(z, shape, index, "z")
     else:
         z = None
-    if dx is not None and not need_dx or dw is not None and not need_dw or db is not None and not bias:
-        raise ValueError("a place for a gradient that is not wanted")
+    dx_pitch = dw_pitch = inner
+    add_db, dw_f32 = db is not None, dw is not None
     if dx is not None:
-        _result(dx, (rows, inner), dev, "dx", dy, x, w, z, dw, db)
-    if dw is not None:
-        _result(dw, (cols, inner), dev, "dw", dy, x, w, z, db, dtypes=(_F32,))
-    if db is not None:
-        if not (db.shape == (cols,) and db.dtype is _F32 and db.device == dev and db.is_contiguous()):
-            raise ValueError(f"db: contiguous fp32 [{cols}] on {dev}, got {_text(db)}")
+        if not need_dx:
+            raise ValueError("a place for a gradient that is not wanted")
+        dx_pitch = _result(dx, (rows, inner), index, "dx", dy, x, w, z, dw, db)
+    if dw_f32:
+        if not need_dw:
+            raise ValueError("a place for a gradient that is not wanted")
+        dw_pitch = _result(dw, (cols, inner), index, "dw", dy, x, w, z, db, dtype=_F32)
+    if add_db:
+        if not bias:
+            raise ValueError("a place for a gradient that is not wanted")
+        if not (db.shape == (cols,) and db.dtype is _F32 and db.get_device() == index and db.is_contiguous()):
+            raise ValueError(f"db: contiguous fp32 [{cols}] on {x.device}, got {_text(db)}")
         if any(t is not None and _l.share_memory(db, t) for t in (dy, x, w, z)):
             raise ValueError("db lies over an input")
     _l.require_cuda(x)
-    add_db, dw_f32 = db is not None, dw is not None
     make = x.new_empty if rows else x.new_zeros
     if need_dx and dx is None:
         dx = make((rows, inner))
@@ -170,12 +183,14 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, z: torch.Tens
     if bias and db is None:
         db = make((cols,), dtype=_F32)
     if rows and (need_dx or need_dw or bias):
-        n = _bytes("aeris_linear_bwd_bytes", rows, inner, cols, z is not None or _padded(dy), _padded(x), _padded(w), need_dx, need_dw,
-                   bias, dw_f32)
-        work = x.new_empty(n, dtype=torch.uint8) if n else None
+        dy_at, x_at, w_at, work = dy.data_ptr(), x.data_ptr(), w.data_ptr(), 0
+        n = _bytes("aeris_linear_bwd_bytes", rows, inner, cols, code != 0 or _padded(dy_at, rows, cols, dy_pitch),
+                   _padded(x_at, rows, inner, x_pitch), _padded(w_at, cols, inner, w_pitch), need_dx, need_dw, bias, dw_f32)
+        if n:
+            buffer = x.new_empty(n, dtype=torch.uint8)
+            work = buffer.data_ptr()
         _launch("aeris_linear_bwd", _GRAD.pack(
-            dy.data_ptr(), x.data_ptr(), w.data_ptr(), 0 if z is None else z.data_ptr(), dx.data_ptr() if need_dx else 0,
-            dw.data_ptr() if need_dw else 0, db.data_ptr() if bias else 0, 0 if work is None else work.data_ptr(),
-            _l.status_word(dev).data_ptr(), dy.stride(0), x.stride(0), w.stride(0), 0 if z is None else z.stride(0),
-            dx.stride(0) if need_dx else 0, dw.stride(0) if need_dw else 0, n, rows, inner, cols, code, dw_f32, add_db), dev)
+            dy_at, x_at, w_at, 0 if z is None else z.data_ptr(), dx.data_ptr() if need_dx else 0, dw.data_ptr() if need_dw else 0,
+            db.data_ptr() if bias else 0, work, _l.status_word(x.device).data_ptr(), dy_pitch, x_pitch, w_pitch, z_pitch, dx_pitch,
+            dw_pitch, n, rows, inner, cols, code, dw_f32, add_db), index)
     return dx, dw, db

@@ -23,6 +23,7 @@ HIDDEN = -1e30              # table entries that are no larger hide the pairs of
 # AerisBiasedAttn (csrc/api.h), field by field
 _RECORD = struct.Struct("10P4q9if0q")
 _BF16, _F32 = torch.bfloat16, torch.float32
+_TABLES, _INTEGERS = (_F32, _BF16), (torch.int32, torch.int64)
 
 
 def _text(t) -> str:
@@ -49,42 +50,48 @@ def relative_positions(window: tuple[int, int]) -> int:
     return (2 * high - 1) * (2 * wide - 1)
 
 
-def _rows(t, shape, dev, what: str, dt=_BF16) -> None:
-    if not (t.dim() == 2 and t.shape == shape and t.dtype is dt and t.device == dev and t.stride(1) == 1
-            and (shape[0] < 2 or t.stride(0) >= shape[1])):
-        raise ValueError(f"{what}: {dt} {tuple(shape)} on {dev} with columns side by side and rows apart, got {_text(t)}")
+def _rows(t, shape, index: int, what: str) -> int:
+    """Pitch of rows of bf16. Every attribute is asked for once: they are half of a small call."""
+    if t.shape == shape and t.dtype is _BF16 and t.get_device() == index and t.ndim == 2:
+        pitch, one = t.stride()
+        if one == 1 and (pitch >= shape[1] or shape[0] < 2):
+            return pitch if shape[0] > 1 else shape[1]
+    raise ValueError(f"{what}: {_BF16} {tuple(shape)} on one device with the others, columns side by side and rows apart, got {_text(t)}")
 
 
 def _check(qkv, n_win, window, heads, d, table, buckets, scale):
-    """Refuses what the kernels cannot take of the inputs that both directions share; returns (high, wide, tokens, scale, device)."""
+    """Refuses what the kernels cannot take of the inputs that both directions share; returns (high, wide, tokens of a window, pitch
+    of qkv, scale, device index)."""
     if len(window) != 2:
         raise ValueError(f"window: (high, wide), got {window!r}")
     high, wide = window
-    n, dev = high * wide, qkv.device
+    n, index = high * wide, qkv.get_device()
     if high < 1 or wide < 1 or n > MAX_TOKENS:
         raise ValueError(f"windows of {high} x {wide} tokens: at least one a side, at most {MAX_TOKENS} in all")
     if not (0 <= n_win <= 65535 and 0 < heads <= 65535 and 0 < d <= 128):
         raise ValueError(f"{n_win} windows, {heads} heads of {d} channels: up to 65535, 65535 and 128 are taken")
-    _rows(qkv, (n_win * n, 3 * heads * d), dev, "qkv")
-    off = relative_positions(window)
-    if not (table.dim() == 2 and table.shape[1] == heads and table.shape[0] > 0 and table.dtype in (_F32, _BF16)
-            and table.device == dev and table.is_contiguous() and table.numel() < 2 ** 31):
-        raise ValueError(f"table: contiguous fp32 or bf16 [rows, {heads}] on {dev}, got {_text(table)}")
+    pitch = _rows(qkv, (n_win * n, 3 * heads * d), index, "qkv")
+    off = (2 * high - 1) * (2 * wide - 1)
+    if not (table.ndim == 2 and table.dtype in _TABLES and table.get_device() == index and table.is_contiguous()):
+        raise ValueError(f"table: contiguous fp32 or bf16 [rows, {heads}] on {qkv.device}, got {_text(table)}")
+    rows, columns = table.shape
+    if columns != heads or not 0 < rows * heads < 2 ** 31:
+        raise ValueError(f"table: [rows, {heads}], got {_text(table)}")
     if buckets is None:
-        if table.shape[0] != off:
+        if rows != off:
             raise ValueError(f"without buckets the table has a row for each of the {off} relative positions, got {_text(table)}")
-    elif not (buckets.shape == (off,) and buckets.dtype in (torch.int32, torch.int64) and buckets.device == dev
-              and buckets.is_contiguous()):
-        raise ValueError(f"buckets: contiguous int32 or int64 [{off}] on {dev}, got {_text(buckets)}")
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(scale):
+    elif not (buckets.shape == (off,) and buckets.dtype in _INTEGERS and buckets.get_device() == index and buckets.is_contiguous()):
+        raise ValueError(f"buckets: contiguous int32 or int64 [{off}] on {qkv.device}, got {_text(buckets)}")
+    if scale is None:
+        scale = d ** -0.5
+    elif not math.isfinite(scale):
         raise ValueError(f"scale {scale}")
-    return high, wide, n, scale, dev
+    return high, wide, n, pitch, scale, index
 
 
-def _stats(t, shape, dev, what: str) -> None:
-    if not (t.shape == shape and t.dtype is _F32 and t.device == dev and t.is_contiguous()):
-        raise ValueError(f"{what}: contiguous fp32 {tuple(shape)} on {dev}, got {_text(t)}")
+def _stats(t, shape, index: int, what: str) -> None:
+    if not (t.shape == shape and t.dtype is _F32 and t.get_device() == index and t.is_contiguous()):
+        raise ValueError(f"{what}: contiguous fp32 {tuple(shape)} on one device with the others, got {_text(t)}")
 
 
 def _apart(t, others, what: str) -> None:
@@ -93,12 +100,13 @@ def _apart(t, others, what: str) -> None:
             raise ValueError(f"{what} lies over another tensor of the call: {_text(t)}, {_text(o)}")
 
 
-def _record(qkv, o, lse, table, buckets, d_o, dqkv, dtable, work, n_win, high, wide, heads, d, scale, add, dev) -> bytes:
-    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    pitch = lambda t: 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
-    return _RECORD.pack(at(qkv), at(o), at(lse), at(table), at(buckets), at(d_o), at(dqkv), at(dtable), at(work),
-                        _l.status_word(dev).data_ptr(), pitch(qkv), pitch(o), pitch(dqkv), work.numel(), n_win, high, wide, heads, d,
-                        table.shape[0], table.dtype is _BF16, buckets is not None and buckets.dtype is torch.int64, add, scale)
+def _launch(name: str, record: bytes, index: int) -> None:
+    if torch._C._cuda_getDevice() == index:
+        rc = _entry(name)(record, _l.raw_stream())
+    else:
+        with torch.cuda.device(index):
+            rc = _entry(name)(record, _l.raw_stream())
+    _l.check(min(rc, 0), name, kernels=max(rc, 0))
 
 
 def biased_attn_fwd(qkv: torch.Tensor, n_win: int, window: tuple[int, int], heads: int, d: int, table: torch.Tensor,
@@ -114,30 +122,38 @@ def biased_attn_fwd(qkv: torch.Tensor, n_win: int, window: tuple[int, int], head
 
     Returns ``(o [n_win * high * wide, heads * d] bf16, lse [n_win, heads, high * wide] fp32 in the log2 domain, +infinity where a
     query sees nothing)``."""
-    high, wide, n, scale, dev = _check(qkv, n_win, window, heads, d, table, buckets, scale)
+    high, wide, n, pitch, scale, index = _check(qkv, n_win, window, heads, d, table, buckets, scale)
+    tokens, inner = n_win * n, heads * d
+    o_pitch = inner
     if out is not None:
-        _rows(out, (n_win * n, heads * d), dev, "out")
+        o_pitch = _rows(out, (tokens, inner), index, "out")
         _apart(out, (qkv, table, buckets, lse), "out")
     if lse is not None:
-        _stats(lse, (n_win, heads, n), dev, "lse")
+        _stats(lse, (n_win, heads, n), index, "lse")
         _apart(lse, (qkv, table, buckets), "lse")
     _l.require_cuda(qkv)
-    with _l.on_device(dev):
-        if lse is None:
-            lse = qkv.new_empty((n_win, heads, n), dtype=_F32)
-        dp = d if d % 8 == 0 and _a._whole_vectors(qkv) and _a._whole_vectors(out) else -(-d // 8) * 8
-        tiled = dp == d and _a._whole_vectors(qkv) and _a._whole_vectors(out)
-        rows = qkv if tiled else _a._pad_heads(qkv, 3, heads, d, dp)
-        o = out if tiled and out is not None else qkv.new_empty((n_win * n, heads * dp))
-        if n_win:
-            work = qkv.new_empty(_work_bytes(n_win, high, wide, heads, dp, False, False), dtype=torch.uint8)
-            rc = _entry("aeris_biased_attn_fwd")(_record(rows, o, lse, table, buckets, None, None, None, work, n_win, high, wide, heads,
-                                                         dp, scale, 0, dev), _l.raw_stream())
-            _l.check(min(rc, 0), "aeris_biased_attn_fwd", kernels=max(rc, 0))
-        if not tiled:
-            o = _a._unpad_heads(o, 1, heads, d, dp)
-            if out is not None:
-                o = out.copy_(o)
+    if lse is None:
+        lse = qkv.new_empty((n_win, heads, n), dtype=_F32)
+    # heads and rows of whole 16-byte vectors; others run as zero-padded copies
+    tiled = (d | pitch | o_pitch) % 8 == 0 and qkv.data_ptr() % 16 == 0 and (out is None or out.data_ptr() % 16 == 0)
+    rows, dp = qkv, d
+    if not tiled:
+        dp = -(-d // 8) * 8
+        rows, pitch, o_pitch = _a._pad_heads(qkv, 3, heads, d, dp), 3 * heads * dp, heads * dp
+    o = out if tiled and out is not None else qkv.new_empty((tokens, heads * dp))
+    if n_win:
+        work, size = 0, _work_bytes(n_win, high, wide, heads, dp, False, False)
+        if size:
+            buffer = qkv.new_empty(size, dtype=torch.uint8)
+            work = buffer.data_ptr()
+        _launch("aeris_biased_attn_fwd", _RECORD.pack(
+            rows.data_ptr(), o.data_ptr(), lse.data_ptr(), table.data_ptr(), 0 if buckets is None else buckets.data_ptr(), 0, 0, 0, work,
+            _l.status_word(qkv.device).data_ptr(), pitch, o_pitch, 0, size, n_win, high, wide, heads, dp, table.shape[0],
+            table.dtype is _BF16, buckets is not None and buckets.dtype is torch.int64, 0, scale), index)
+    if not tiled:
+        o = _a._unpad_heads(o, 1, heads, d, dp)
+        if out is not None:
+            o = out.copy_(o)
     return o, lse
 
 
@@ -148,39 +164,43 @@ def biased_attn_bwd(d_o: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, lse: 
     """Gradients of :func:`biased_attn_fwd` for ``d_o`` with respect to its first result; ``o``, ``lse`` are its results. Returns
     (gradient of qkv, in its layout; fp32 gradient of the table [rows, heads], or None without ``need_dtable``). ``dqkv``: where to
     put it; ``dtable`` fp32 is added to where given. Rows that hide their pairs get zero. The same bits on every run."""
-    high, wide, n, scale, dev = _check(qkv, n_win, window, heads, d, table, buckets, scale)
-    _rows(o, (n_win * n, heads * d), dev, "o")
-    _rows(d_o, (n_win * n, heads * d), dev, "d_o")
-    _stats(lse, (n_win, heads, n), dev, "lse")
+    high, wide, n, pitch, scale, index = _check(qkv, n_win, window, heads, d, table, buckets, scale)
+    tokens, inner = n_win * n, heads * d
+    o_pitch, do_pitch = _rows(o, (tokens, inner), index, "o"), _rows(d_o, (tokens, inner), index, "d_o")
+    _stats(lse, (n_win, heads, n), index, "lse")
+    g_pitch = 3 * inner
     if dqkv is not None:
-        _rows(dqkv, tuple(qkv.shape), dev, "dqkv")
+        g_pitch = _rows(dqkv, (tokens, 3 * inner), index, "dqkv")
         _apart(dqkv, (qkv, o, d_o, lse, table, buckets, dtable), "dqkv")
-    if dtable is not None:
+    add = dtable is not None
+    if add:
         if not need_dtable:
             raise ValueError("a place for a gradient that is not wanted")
-        _stats(dtable, tuple(table.shape), dev, "dtable")
+        _stats(dtable, table.shape, index, "dtable")
         _apart(dtable, (qkv, o, d_o, lse, table, buckets), "dtable")
     _l.require_cuda(qkv)
-    with _l.on_device(dev):
-        add = dtable is not None
-        if need_dtable and dtable is None:
-            dtable = (qkv.new_empty if n_win else qkv.new_zeros)(table.shape, dtype=_F32)
-        tiled = d % 8 == 0 and all(map(_a._whole_vectors, (qkv, o, d_o, dqkv)))
+    if need_dtable and not add:
+        dtable = (qkv.new_empty if n_win else qkv.new_zeros)(table.shape, dtype=_F32)
+    tiled = ((d | pitch | o_pitch | do_pitch | g_pitch) % 8 == 0 and qkv.data_ptr() % 16 == 0 and o.data_ptr() % 16 == 0
+             and d_o.data_ptr() % 16 == 0 and (dqkv is None or dqkv.data_ptr() % 16 == 0))
+    rows, of, do, dp = qkv, o, d_o, d
+    if not tiled:
         dp = -(-d // 8) * 8
-        if tiled:
-            rows, of, do = qkv, o, d_o
-            if of.stride(0) != do.stride(0) and n_win * n > 1:
-                of, do = of.contiguous(), do.contiguous()
-        else:
-            rows, of, do = _a._pad_heads(qkv, 3, heads, d, dp), _a._pad_heads(o, 1, heads, d, dp), _a._pad_heads(d_o, 1, heads, d, dp)
-        g = dqkv if tiled and dqkv is not None else qkv.new_empty((n_win * n, 3 * heads * dp))
-        if n_win:
-            work = qkv.new_empty(_work_bytes(n_win, high, wide, heads, dp, True, need_dtable), dtype=torch.uint8)
-            rc = _entry("aeris_biased_attn_bwd")(_record(rows, of, lse, table, buckets, do, g, dtable, work, n_win, high, wide, heads,
-                                                         dp, scale, add, dev), _l.raw_stream())
-            _l.check(min(rc, 0), "aeris_biased_attn_bwd", kernels=max(rc, 0))
-        if not tiled:
-            g = _a._unpad_heads(g, 3, heads, d, dp)
-            if dqkv is not None:
-                g = dqkv.copy_(g)
+        rows, of, do = (_a._pad_heads(t, k, heads, d, dp) for t, k in ((qkv, 3), (o, 1), (d_o, 1)))
+        pitch, o_pitch, g_pitch = 3 * heads * dp, heads * dp, 3 * heads * dp
+    elif o_pitch != do_pitch:
+        of, do, o_pitch = o.contiguous(), d_o.contiguous(), inner
+    g = dqkv if tiled and dqkv is not None else qkv.new_empty((tokens, 3 * heads * dp))
+    if n_win:
+        size = _work_bytes(n_win, high, wide, heads, dp, True, need_dtable)
+        work = qkv.new_empty(size, dtype=torch.uint8)
+        _launch("aeris_biased_attn_bwd", _RECORD.pack(
+            rows.data_ptr(), of.data_ptr(), lse.data_ptr(), table.data_ptr(), 0 if buckets is None else buckets.data_ptr(), do.data_ptr(),
+            g.data_ptr(), dtable.data_ptr() if need_dtable else 0, work.data_ptr(), _l.status_word(qkv.device).data_ptr(), pitch,
+            o_pitch, g_pitch, size, n_win, high, wide, heads, dp, table.shape[0], table.dtype is _BF16,
+            buckets is not None and buckets.dtype is torch.int64, add, scale), index)
+    if not tiled:
+        g = _a._unpad_heads(g, 3, heads, d, dp)
+        if dqkv is not None:
+            g = dqkv.copy_(g)
     return g, dtable

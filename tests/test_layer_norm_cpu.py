@@ -82,6 +82,6 @@ def test_cpu_tensors_are_refused_and_not_computed_elsewhere():
 
 
 def test_slices_cover_the_rows_and_the_machine():
-    for rows in (1, 5, 64800, 2 ** 31 - 1):
-        s = LN.slices_for(rows, 148)
-        assert 1 <= s <= min(65535, rows)
+    for rows, cols in ((1, 1), (5, 20000), (64800, 1536), (2 ** 31 - 1, 1)):
+        s = LN.slices_for(rows, cols, 148)
+        assert s <= 65535 and (s == 1) == (rows * cols <= 2 ** 14 and cols <= 4096)
