@@ -797,12 +797,13 @@ static int slice_of_rows(F&& at_of, int N, int zero, int rows) {
 constexpr int SLICE_BYTES = 120 * 1024;      // the most that a tile's slice and the places may take beside the operands
 
 // Whether the forward pass makes its tables from the learned one: in the kernels of one query tile, where that comes to fewer reads than a
-// launch of its own is worth (2 us; 16 windows of 8 x 8, 2 heads: 5.5 -> @ us).
+// launch of its own is worth: that takes the host 3 us (16 windows of 8 x 8, 2 heads: 20.1 -> 12.2 us a call), the GPU 0.2; made by
+// every block, 275,000 entries cost it 3 us, two million 18.
 bool aeris::biased_fwd_reads_source(int n_win, int H, int head_dim, const BiasSource& s) {
   const int N = s.high * s.wide, zero = s.at(N - 1);
   if (head_dim <= 64 && N > 2 * TILE) return false;
   const long long slice = slice_of_rows([&](int t) { return s.at(t); }, N, zero, TILE), tiles = (N + TILE - 1) / TILE;
-  return 4 * slice + (N + 127) / 128 * 512 <= SLICE_BYTES && slice * tiles * H * n_win <= 2 << 20;
+  return 4 * slice + (N + 127) / 128 * 512 <= SLICE_BYTES && slice * tiles * H * n_win <= 1 << 17;
 }
 
 int aeris::attn_fwd_biased(const void* qkv, int ld, void* o, int ldo, float* lse, int n_win, int H, int head_dim, float scale,

@@ -808,6 +808,82 @@ __global__ void __launch_bounds__(DZ_THREADS) lin_pad_kernel(const unsigned shor
   }
 }
 
+// Small layers without the tensor core, any pitch, in one launch: G neighbouring lanes per result, which share its sum. The
+// gradients make dz anew for every result that needs it.
+constexpr long long SMALL_FWD = 1 << 23, SMALL_BWD = 1 << 18;       // rows x inner x columns, see small_fwd and small_bwd
+
+template <typename F>
+__device__ __forceinline__ float group_sum(int n, int g, int lane, F&& term) {
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = lane; k < n; k += g) s += term(k);
+  for (int o = g >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+__global__ void __launch_bounds__(DZ_THREADS) lin_small_fwd_kernel(const LinParams p, const unsigned short* x, long long ldx,
+                                                                   const unsigned short* w, long long ldw, int g) {
+  chain_point();
+  const long long n = static_cast<long long>(p.M) * p.N;
+  const int lane = threadIdx.x % g, per = DZ_THREADS / g;
+  for (long long base = static_cast<long long>(blockIdx.x) * per; base < n; base += static_cast<long long>(gridDim.x) * per) {
+    const long long i = base + threadIdx.x / g, j = i < n ? i : n - 1;      // lanes of results that there are not stay for the sums
+    const int row = static_cast<int>(j / p.N), col = static_cast<int>(j - static_cast<long long>(row) * p.N);
+    const unsigned short *px = x + row * ldx, *pw = w + col * ldw;
+    float z = group_sum(p.K, g, lane, [&](int k) { return bf(px[k]) * bf(pw[k]); });
+    if (lane || i >= n) continue;
+    if (p.bias)
+      z += p.bias_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]) : static_cast<const float*>(p.bias)[col];
+    if (p.Z) p.Z[row * p.ldz + col] = __float2bfloat16_rn(z);
+    float v = act_of(z, p.act);
+    if (p.resid) v += __bfloat162float(p.resid[row * p.ldr + col]);
+    p.C[row * p.ldc + col] = __float2bfloat16_rn(v);
+  }
+}
+
+__global__ void __launch_bounds__(DZ_THREADS) lin_small_bwd_kernel(const AerisLinearGrad a, int g) {
+  chain_point();
+  const unsigned short *dy = static_cast<const unsigned short*>(a.dy), *zz = static_cast<const unsigned short*>(a.z),
+                       *x = static_cast<const unsigned short*>(a.x), *w = static_cast<const unsigned short*>(a.w);
+  auto dz = [&](int r, int c) {
+    const float d = bf(dy[r * a.ld_dy + c]);
+    return zz ? d * act_grad(bf(zz[r * a.ld_z + c]), a.act) : d;
+  };
+  const long long n_dx = a.dx ? static_cast<long long>(a.rows) * a.inner : 0, n_dw = a.dw ? static_cast<long long>(a.cols) * a.inner : 0;
+  const long long n = n_dx + n_dw + (a.db ? a.cols : 0);
+  const int lane = threadIdx.x % g, per = DZ_THREADS / g;
+  for (long long base = static_cast<long long>(blockIdx.x) * per; base < n; base += static_cast<long long>(gridDim.x) * per) {
+    long long i = base + threadIdx.x / g;
+    const bool live = i < n && lane == 0;
+    // a warp's lanes may be at results of two kinds: each group loops by itself, all of them meet at the sums
+    float s = 0.f;
+    if (i < n_dx) {
+      const int r = static_cast<int>(i / a.inner), k = static_cast<int>(i - static_cast<long long>(r) * a.inner);
+      for (int c = lane; c < a.cols; c += g) s = fmaf(dz(r, c), bf(w[c * a.ld_w + k]), s);
+    } else if (i < n_dx + n_dw) {
+      const int c = static_cast<int>((i - n_dx) / a.inner), k = static_cast<int>(i - n_dx - static_cast<long long>(c) * a.inner);
+      for (int r = lane; r < a.rows; r += g) s = fmaf(dz(r, c), bf(x[r * a.ld_x + k]), s);
+    } else if (i < n) {
+      for (int r = lane; r < a.rows; r += g) s += dz(r, static_cast<int>(i - n_dx - n_dw));
+    }
+    __syncwarp();
+    for (int o = g >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (!live) continue;
+    if (i < n_dx) {
+      const long long r = i / a.inner;
+      static_cast<__nv_bfloat16*>(a.dx)[r * a.ld_dx + i - r * a.inner] = __float2bfloat16_rn(s);
+    } else if (i < n_dx + n_dw) {
+      i -= n_dx;
+      const long long c = i / a.inner, at = c * a.ld_dw + i - c * a.inner;
+      if (a.dw_f32) static_cast<float*>(a.dw)[at] += s;
+      else static_cast<__nv_bfloat16*>(a.dw)[at] = __float2bfloat16_rn(s);
+    } else {
+      float* out = a.db + i - n_dx - n_dw;
+      *out = a.add_db ? *out + s : s;
+    }
+  }
+}
+
 // Sums of the slices, in their order: out[c] (+)= sum_s work[s][c].
 __global__ void __launch_bounds__(DZ_THREADS) lin_join_sums_kernel(const float* work, float* out, int slices, int cols, int add) {
   __shared__ float part[8][32];
@@ -928,8 +1004,26 @@ long long dw_bytes(int rows, int inner, int cols, bool f32) {
 
 }  // namespace
 
+namespace {
+
+// Whether a layer goes without the tensor core: forward where operands would have to be copied first, backward where five launches
+// would cost more than the work. us a call, before / so: forward 10 x 3685 -> 100 17.9 / @, backward 369 x 4 -> 2 27.5 / @.
+bool small_fwd(int rows, int inner, int cols, bool pad) {
+  return pad && static_cast<double>(rows) * inner * cols <= SMALL_FWD;
+}
+bool small_bwd(int rows, int inner, int cols) { return static_cast<double>(rows) * inner * cols <= SMALL_BWD; }
+// Lanes that share a sum of n terms: four terms each at least, at most a warp.
+int lanes_for(int n) {
+  int g = 1;
+  while (g < 32 && 8 * g <= n) g *= 2;
+  return g;
+}
+
+}  // namespace
+
 extern "C" long long aeris_linear_fwd_bytes(int rows, int inner, int cols, int pad_x, int pad_w) {
   if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
+  if (small_fwd(rows, inner, cols, pad_x || pad_w)) return 0;
   return (pad_x ? up(2 * padded(inner) * rows) : 0) + (pad_w ? up(2 * padded(inner) * cols) : 0);
 }
 
@@ -943,9 +1037,15 @@ extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
   p.C = static_cast<__nv_bfloat16*>(a->y); p.ldc = pitch(a->ld_y, a->rows, a->cols); p.bias = a->bias;
   p.resid = static_cast<const __nv_bfloat16*>(a->resid); p.ldr = pitch(a->ld_resid, a->rows, a->cols);
   p.Z = static_cast<__nv_bfloat16*>(a->z); p.ldz = pitch(a->ld_z, a->rows, a->cols); p.status = a->status;
+  int n = 1, r;
+  if (small_fwd(a->rows, a->inner, a->cols, pad_x || pad_w)) {
+    const int g = lanes_for(a->inner);
+    r = launch_chained(lin_small_fwd_kernel, blocks_for(static_cast<long long>(a->rows) * a->cols * g), DZ_THREADS, 0, stream, p,
+                       static_cast<const unsigned short*>(a->x), a->ld_x, static_cast<const unsigned short*>(a->w), a->ld_w, g);
+    return r ? r : 1;
+  }
   uint8_t* work = static_cast<uint8_t*>(a->work);
   long long at = 0;
-  int n = 1, r;
   Operand x, w;
   if ((r = operand(x, a->x, a->ld_x, a->rows, a->inner, work, at, n, stream))) return r;
   if ((r = operand(w, a->w, a->ld_w, a->cols, a->inner, work, at, n, stream))) return r;
@@ -958,6 +1058,7 @@ extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
 extern "C" long long aeris_linear_bwd_bytes(int rows, int inner, int cols, int own_dz, int pad_x, int pad_w, int dx, int dw, int db,
                                             int dw_f32) {
   if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
+  if (small_bwd(rows, inner, cols)) return 0;
   const int slices = db_slices(rows, cols);
   long long n = db && slices > 1 ? up(4ll * slices * cols) : 0;
   if (own_dz && (dx || dw)) n += up(2 * padded(cols) * rows);
@@ -975,9 +1076,15 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   if (a->work_bytes < aeris_linear_bwd_bytes(rows, inner, cols, own_dz, !tiled(a->x, a->ld_x, rows, inner), !tiled(a->w, a->ld_w, cols, inner),
                                              a->dx != nullptr, a->dw != nullptr, a->db != nullptr, a->dw_f32))
     return -2;
+  int n = 0, r;
+  if (small_bwd(rows, inner, cols)) {
+    const long long results = (a->dx ? static_cast<long long>(rows) * inner : 0) + (a->dw ? static_cast<long long>(cols) * inner : 0) + cols;
+    const int g = lanes_for(rows > cols ? rows : cols);
+    r = launch_chained(lin_small_bwd_kernel, blocks_for(results * g), DZ_THREADS, 0, stream, *a, g);
+    return r ? r : 1;
+  }
   uint8_t* work = static_cast<uint8_t*>(a->work);
   long long at = 0;
-  int n = 0, r;
   Operand dz{a->dy, pitch(a->ld_dy, rows, cols)};
   if (own_dz || a->db) {
     DzParams d{a->dy, a->z, nullptr, nullptr, 0, a->ld_dy, a->ld_z, padded(cols), rows, cols};

@@ -92,41 +92,45 @@ __device__ __forceinline__ float bg_exp2(float x) {
 struct BgTile {
   int head, ti, tj;           // head: of those at hand
 };
-__device__ __forceinline__ BgTile bg_tile(long long t, int n, int tk) {
+__device__ __forceinline__ BgTile bg_tile(int t, int n, int tk) {
   const int nj = (n + tk - 1) / tk, ni = (n + PB_TILE - 1) / PB_TILE;
   BgTile b;
-  b.tj = static_cast<int>(t % nj);
-  const long long r = t / nj;
-  b.ti = static_cast<int>(r % ni);
-  b.head = static_cast<int>(r / ni);
+  const int r = t / nj;
+  b.tj = t - r * nj;
+  b.head = r / ni;
+  b.ti = r - b.head * ni;
   return b;
 }
-// First step of CTA b of g, of `steps` in all.
-__host__ __device__ __forceinline__ long long bg_first(long long steps, int b, int g) { return steps * b / g; }
-
+// Who takes what: CTAs take `rounds` rounds of whole tiles, and the first `runs` of them runs of the steps (tile, window) that are left, as
+// long as one another. runs = 0: what is left are whole tiles, one for a CTA.
+struct BgPlan {
+  int tiles, ctas, rounds, steps, runs;
+  __host__ __device__ __forceinline__ int first(int b) const { return static_cast<int>(static_cast<long long>(steps) * b / runs); }
+};
 // What a CTA does, piece by piece: windows [w0, w1) of tile t.
 struct BgWork {
-  long long t, u, u1, last_round;
-  int w0, w1, n_win;
-  __device__ __forceinline__ BgWork(long long tiles, int n_win_) : n_win(n_win_) {
-    last_round = tiles / gridDim.x * gridDim.x;
-    t = static_cast<long long>(blockIdx.x) - gridDim.x;
-    const long long steps = (tiles - last_round) * n_win;
-    u = bg_first(steps, blockIdx.x, gridDim.x);
-    u1 = bg_first(steps, blockIdx.x + 1, gridDim.x);
+  const BgPlan& p;
+  int n_win, round = 0, u = 0, u1 = 0, t = 0, w0 = 0, w1 = 0;
+  __device__ __forceinline__ BgWork(const BgPlan& plan, int n_win_) : p(plan), n_win(n_win_) {
+    if (static_cast<int>(blockIdx.x) < p.runs) {
+      u = p.first(blockIdx.x);
+      u1 = p.first(blockIdx.x + 1);
+    }
   }
   __device__ __forceinline__ bool next() {
-    if (t + gridDim.x < last_round) {
-      t += gridDim.x;
+    const int whole = round * p.ctas + blockIdx.x;
+    if (round < p.rounds || (!p.runs && whole < p.tiles)) {
+      ++round;
+      t = whole;
       w0 = 0;
       w1 = n_win;
       return true;
     }
     if (u >= u1) return false;
-    const long long r = u / n_win;
-    t = last_round + r;
-    w0 = static_cast<int>(u - r * n_win);
-    w1 = static_cast<int>(min(static_cast<long long>(n_win), w0 + u1 - u));
+    const int r = u / n_win;
+    t = p.rounds * p.ctas + r;
+    w0 = u - r * n_win;
+    w1 = min(n_win, w0 + u1 - u);
     u += w1 - w0;
     return true;
   }
@@ -136,7 +140,7 @@ template <int DCH>
 __global__ void __launch_bounds__(BgCfg<DCH>::THREADS, 1)
 bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BgParams p,
-                 const long long tiles) {
+                 const BgPlan plan) {
   using C = BgCfg<DCH>;
   constexpr int TK = C::TK, CPT = C::CPT, NST = C::NST;
   extern __shared__ uint8_t smem_raw[];
@@ -172,7 +176,7 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (BgWork k(tiles, p.n_win); ok && k.next();) {
+      for (BgWork k(plan, p.n_win); ok && k.next();) {
         const BgTile b = bg_tile(k.t, p.n, TK);
         const int head = p.head0 + b.head;
         for (int w = k.w0; w < k.w1; ++w) {
@@ -200,7 +204,7 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       int st = 0, buf = 0;
       uint32_t ph = 0, b_ph = 0;
       bool ok = true;
-      for (BgWork k(tiles, p.n_win); ok && k.next();) {
+      for (BgWork k(plan, p.n_win); ok && k.next();) {
         for (int w = k.w0; w < k.w1; ++w) {
           ok = mbar_wait_poll(&s_empty[buf], b_ph ^ 1, p.status, ERR_TIMEOUT_ATTN) &&
                mbar_wait_poll(&full[st], ph, p.status, ERR_TIMEOUT_ATTN);
@@ -229,7 +233,7 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     int buf = 0;
     uint32_t b_ph = 0;
     bool ok = true;
-    for (BgWork work(tiles, p.n_win); ok && work.next();) {
+    for (BgWork work(plan, p.n_win); ok && work.next();) {
       const int w1 = work.w1;
       int w = work.w0;
       const BgTile b = bg_tile(work.t, p.n, TK);
@@ -319,28 +323,27 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
 // Tiles that several CTAs took part in: what those before the last one left in `extra`, in their order. Block (x, y): the
 // tile that CTA x of the sums left unfinished, if x is the first one that did; rows y, y + 32, .. of it.
-__global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, long long tiles, int g, int tk) {
+__global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, const BgPlan plan, int tk) {
   chain_point();
-  const int b0 = blockIdx.x;
-  const long long last_round = tiles / g * g, steps = (tiles - last_round) * p.n_win;
-  const long long first = bg_first(steps, b0, g), end = bg_first(steps, b0 + 1, g), t = (end - 1) / p.n_win;
-  // it ends in the middle of tile t, unless an earlier CTA that does has its turn with the tile, or it has no steps
-  if (first == end || end % p.n_win == 0 || first > t * p.n_win) return;
-  const BgTile b = bg_tile(last_round + t, p.n, tk);
+  const int b0 = blockIdx.x, first = plan.first(b0), end = plan.first(b0 + 1), t = (end - 1) / p.n_win;
+  // it ends in the middle of tile t, unless an earlier CTA that does has its turn with the tile
+  if (end % p.n_win == 0 || first > t * p.n_win) return;
+  const BgTile b = bg_tile(plan.rounds * plan.ctas + t, p.n, tk);
   const int cols = min(tk, p.n - b.tj * tk), vecs = (cols + 3) / 4;
   int b1 = b0 + 1;        // CTAs b0 .. b1 - 1 left it unfinished
-  while (bg_first(steps, b1 + 1, g) < (t + 1) * p.n_win) ++b1;
-  for (int r = blockIdx.y; r < PB_TILE && b.ti * PB_TILE + r < p.n; r += gridDim.y)
-    for (int v = threadIdx.x; v < vecs; v += 256) {
-      float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
-      float4 s = *dst;
-      for (int i = b0; i < b1; ++i) {
-        if (bg_first(steps, i, g) == bg_first(steps, i + 1, g)) continue;
-        const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(i) * PB_TILE + r) * tk) + v);
-        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
-      }
-      *dst = s;
+  while (plan.first(b1 + 1) < (t + 1) * p.n_win) ++b1;
+  for (int i = threadIdx.x; i < 4 * vecs; i += 256) {       // four rows at a time
+    const int r = blockIdx.y + gridDim.y * (i / vecs), v = i % vecs;
+    if (b.ti * PB_TILE + r >= p.n) continue;
+    float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
+    float4 s = *dst;
+#pragma unroll 4
+    for (int k = b0; k < b1; ++k) {
+      const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(k) * PB_TILE + r) * tk) + v);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
+    *dst = s;
+  }
 }
 
 // Sums of the pairs of one relative position: a block has 32 positions of one difference in y (a lane each), its warps
@@ -417,12 +420,29 @@ SumsPlan plan_sums(int n_win, int n, int heads, int head_dim) {
   s.heads = static_cast<int>(PART_BYTES / one);
   if (s.heads < 1) s.heads = 1;
   if (s.heads > heads) s.heads = heads;
-  // runs of four steps at least: a run costs about as much to start and to write
-  const long long most = (tiles * s.heads * n_win + 3) / 4;
-  s.ctas = most < num_sms() ? static_cast<int>(most) : num_sms();
+  // tiles and steps are counted in 32 bits
+  while (s.heads > 1 && tiles * s.heads * n_win > 0x3fffffff) s.heads /= 2;
+  s.ctas = num_sms();
   s.part = one * s.heads;
   s.extra = 4ll * s.ctas * PB_TILE * tk;
   return s;
+}
+
+// Runs of four steps at least, for a run costs about as much to start and to join; where tiles have few windows none.
+BgPlan plan_tiles(int tiles, int n_win) {
+  BgPlan p{};
+  p.tiles = tiles;
+  const bool split = n_win > 16;
+  const long long steps = static_cast<long long>(tiles) * n_win;
+  p.ctas = split && tiles < num_sms() ? static_cast<int>((steps + 3) / 4 < num_sms() ? (steps + 3) / 4 : num_sms())
+                                      : (tiles < num_sms() ? tiles : num_sms());
+  p.rounds = tiles / p.ctas;
+  const int left = tiles - p.rounds * p.ctas;
+  if (split && left) {
+    p.steps = left * n_win;
+    p.runs = p.steps < p.ctas ? p.steps : p.ctas;
+  }
+  return p;
 }
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
@@ -458,7 +478,7 @@ int expand(const BiasSource& s, const Place& p, float* table, int* at, cudaStrea
 }
 
 template <int DCH>
-int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, long long tiles, int ctas, cudaStream_t stream) {
+int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, const BgPlan& plan, cudaStream_t stream, int& kernels) {
   static std::atomic<uint64_t> done{0};
   using C = BgCfg<DCH>;
   if (!once_a_device(done, [&] {
@@ -468,8 +488,11 @@ int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, long long til
                cudaFuncGetAttributes(&f, bias_grad_kernel<DCH>) == cudaSuccess && f.numRegs * C::THREADS >= C::REGS;
       }))
     return -20;
-  const int r = launch_chained(bias_grad_kernel<DCH>, ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, tiles);
-  return r ? r : launch_chained(bias_join_kernel, dim3(ctas, 32), 256, 0, stream, p, tiles, ctas, C::TK);
+  const int r = launch_chained(bias_grad_kernel<DCH>, plan.ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, plan);
+  ++kernels;
+  if (r || !plan.runs) return r;
+  ++kernels;
+  return launch_chained(bias_join_kernel, dim3(plan.runs, PB_TILE / 4), 256, 0, stream, p, plan, C::TK);
 }
 
 }  // namespace
@@ -554,14 +577,12 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   for (int h0 = 0; h0 < a->heads; h0 += s.heads) {
     g.head0 = h0;
     g.n_heads = a->heads - h0 < s.heads ? a->heads - h0 : s.heads;
-    const long long tiles = static_cast<long long>((p.n + PB_TILE - 1) / PB_TILE) * ((p.n + tk - 1) / tk) * g.n_heads;
-    const long long steps = tiles * a->n_win;
-    const int ctas = steps < s.ctas ? static_cast<int>(steps) : s.ctas;
-    if ((r = dch == 1 ? launch_bias_grad<1>(m, g, tiles, ctas, stream) : launch_bias_grad<2>(m, g, tiles, ctas, stream))) return r - 300;
+    const BgPlan plan = plan_tiles((p.n + PB_TILE - 1) / PB_TILE * ((p.n + tk - 1) / tk) * g.n_heads, a->n_win);
+    if ((r = dch == 1 ? launch_bias_grad<1>(m, g, plan, stream, count) : launch_bias_grad<2>(m, g, plan, stream, count))) return r - 300;
     r = launch_chained(bias_sums_kernel, dim3(2 * a->high - 1, (2 * a->wide - 1 + 31) / 32, g.n_heads), 256, 0, stream,
                        static_cast<const float*>(g.part), s.ld, h0, a->high, a->wide, by_position, a->heads, a->buckets ? 0 : a->add);
     if (r) return r - 400;
-    count += 3;
+    ++count;
   }
   if (a->buckets) {
     r = launch_chained(bias_buckets_kernel, dim3(a->table_rows, (a->heads + 31) / 32), 256, 0, stream, *a,
