@@ -134,14 +134,19 @@ struct LinOut {
   }
 };
 
-// The first `n` of 32 bf16 columns of one row, element by element: rows that start anywhere.
-__device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (&o)[16], int n) {
+// 32 rows x 32 columns of a warp to rows that start anywhere, through its staging: a lane per column, so that a store is 64 bytes of
+// one row (a lane per row, column by column: 1111 x 777 -> 333 15.3 us, so 8.5). `rows`, `cols`: how many there are.
+__device__ __forceinline__ void store_anywhere(uint8_t* stage, int lane, const uint32_t (&o)[16], __nv_bfloat16* dst, long long ld, int rows,
+                                               int cols) {
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < n) {
-      const uint32_t h = i & 1 ? o[i / 2] >> 16 : o[i / 2] & 0xffffu;
-      reinterpret_cast<unsigned short*>(dst)[i] = static_cast<unsigned short>(h);
-    }
+  for (int i = 0; i < 16; ++i) *reinterpret_cast<uint32_t*>(stage + lane * 68 + 4 * i) = o[i];       // rows of 68 bytes: 17 banks apart
+  __syncwarp();
+  if (lane < cols)
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r)
+      reinterpret_cast<unsigned short*>(dst)[r * ld + lane] = *reinterpret_cast<const unsigned short*>(stage + r * 68 + 2 * lane);
+  __syncwarp();
 }
 
 // One thread = one accumulator row; columns [c_lo, c_hi) of the tile whose first column is col0 and lies at `taddr`.
@@ -191,7 +196,7 @@ __device__ __forceinline__ void lin_epilogue_row(const LinParams& p, uint32_t ta
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
       if (mz) out.put(1, o);
-      else if (row_ok) store_row32(p.Z + static_cast<long long>(row) * p.ldz + col0 + c, o, n);
+      else store_anywhere(out.stage + 4096, out.lane, o, p.Z + (row - out.lane) * p.ldz + col0 + c, p.ldz, min(32, p.M - row + out.lane), n);
     }
     switch (p.act) {
       case LIN_ACT_RELU: act32<LIN_ACT_RELU>(v); break;
@@ -219,7 +224,7 @@ __device__ __forceinline__ void lin_epilogue_row(const LinParams& p, uint32_t ta
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
     if (my) out.put(0, o);
-    else if (row_ok) store_row32(p.C + static_cast<long long>(row) * p.ldc + col0 + c, o, n);
+    else store_anywhere(out.stage, out.lane, o, p.C + (row - out.lane) * p.ldc + col0 + c, p.ldc, min(32, p.M - row + out.lane), n);
     if (my || mz) out.send(my, mz, col0 + c, row - out.lane, p.M);
   }
 }
@@ -792,19 +797,30 @@ int launch_dz(const DzParams& a, int act, dim3 grid, cudaStream_t stream) {
   }
 }
 
-// Rows that start on 16-byte boundaries, for tiled loads: dst [rows, (cols + 7) / 8 * 8] of src, zeros behind the rows' ends.
-__global__ void __launch_bounds__(DZ_THREADS) lin_pad_kernel(const unsigned short* src, long long ld, uint4* dst, int rows, int cols) {
+// Rows that start on 16-byte boundaries, for tiled loads: dst [rows, (cols + 7) / 8 * 8] of src, zeros behind the rows' ends. One or two
+// matrices a launch.
+struct PadJob {
+  const unsigned short* src;
+  uint4* dst;
+  long long ld;
+  int rows, cols;
+};
+struct PadJobs {
+  PadJob job[2];
+};
+__global__ void __launch_bounds__(DZ_THREADS) lin_pad_kernel(const PadJobs jobs) {
   chain_point();
-  const int vecs = (cols + 7) / 8;
-  const long long n = static_cast<long long>(rows) * vecs;
+  const PadJob j = jobs.job[blockIdx.y];
+  const int vecs = (j.cols + 7) / 8;
+  const long long n = static_cast<long long>(j.rows) * vecs;
   for (long long i = static_cast<long long>(blockIdx.x) * DZ_THREADS + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * DZ_THREADS) {
     const long long row = i / vecs;
     const int c = static_cast<int>(i - row * vecs) * 8;
-    const unsigned short* s = src + row * ld + c;
+    const unsigned short* s = j.src + row * j.ld + c;
     unsigned short e[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = c + k < cols ? s[k] : static_cast<unsigned short>(0);
-    dst[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    for (int k = 0; k < 8; ++k) e[k] = c + k < j.cols ? s[k] : static_cast<unsigned short>(0);
+    j.dst[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
   }
 }
 
@@ -974,22 +990,33 @@ int blocks_for(long long threads) {
 bool tiled(const void* p, long long ld, int rows, int cols) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || (ld % 8 == 0 && ld >= cols));
 }
-// An operand of a product: where it is, or its copy at `at` of the workspace, which then goes on behind it.
+// Operands of products: where they are, or copies in the workspace, which go on behind one another and are made in one launch.
 struct Operand {
   const void* p;
   long long ld;
 };
-int operand(Operand& o, const void* p, long long ld, int rows, int cols, uint8_t* work, long long& at, int& kernels, cudaStream_t stream) {
-  if (tiled(p, ld, rows, cols)) {
-    o = {p, pitch(ld, rows, cols)};
-    return 0;
+struct Operands {
+  uint8_t* work;
+  long long at = 0;
+  PadJobs jobs{};
+  int n = 0;
+  long long most = 0;
+
+  Operand add(const void* p, long long ld, int rows, int cols) {
+    if (tiled(p, ld, rows, cols)) return {p, pitch(ld, rows, cols)};
+    uint8_t* copy = work + at;
+    at += up(2 * padded(cols) * rows);
+    jobs.job[n++] = {static_cast<const unsigned short*>(p), reinterpret_cast<uint4*>(copy), ld, rows, cols};
+    const long long vecs = padded(cols) / 8 * rows;
+    most = most > vecs ? most : vecs;
+    return {copy, padded(cols)};
   }
-  o = {work + at, padded(cols)};
-  at += up(2 * padded(cols) * rows);
-  ++kernels;
-  return launch_chained(lin_pad_kernel, blocks_for(padded(cols) / 8 * rows), DZ_THREADS, 0, stream, static_cast<const unsigned short*>(p),
-                        ld, reinterpret_cast<uint4*>(work + at - up(2 * padded(cols) * rows)), rows, cols);
-}
+  int launch(int& kernels, cudaStream_t stream) {
+    if (!n) return 0;
+    ++kernels;
+    return launch_chained(lin_pad_kernel, dim3(blocks_for(most), n), DZ_THREADS, 0, stream, jobs);
+  }
+};
 
 // Slices of the rows whose column sums are taken apart: about sixteen blocks of 64 columns on every multiprocessor.
 int db_slices(int rows, int cols) {
@@ -1007,7 +1034,7 @@ long long dw_bytes(int rows, int inner, int cols, bool f32) {
 namespace {
 
 // Whether a layer goes without the tensor core: forward where operands would have to be copied first, backward where five launches
-// would cost more than the work. us a call, before / so: forward 10 x 3685 -> 100 17.9 / @, backward 369 x 4 -> 2 27.5 / @.
+// would cost more than the work. us a call, before / so: forward 10 x 3685 -> 100 17.9 / 13.4, backward 369 x 4 -> 2 27.5 / 14.5.
 bool small_fwd(int rows, int inner, int cols, bool pad) {
   return pad && static_cast<double>(rows) * inner * cols <= SMALL_FWD;
 }
@@ -1044,11 +1071,9 @@ extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
                        static_cast<const unsigned short*>(a->x), a->ld_x, static_cast<const unsigned short*>(a->w), a->ld_w, g);
     return r ? r : 1;
   }
-  uint8_t* work = static_cast<uint8_t*>(a->work);
-  long long at = 0;
-  Operand x, w;
-  if ((r = operand(x, a->x, a->ld_x, a->rows, a->inner, work, at, n, stream))) return r;
-  if ((r = operand(w, a->w, a->ld_w, a->cols, a->inner, work, at, n, stream))) return r;
+  Operands operands{static_cast<uint8_t*>(a->work)};
+  const Operand x = operands.add(a->x, a->ld_x, a->rows, a->inner), w = operands.add(a->w, a->ld_w, a->cols, a->inner);
+  if ((r = operands.launch(n, stream))) return r;
   // x of few rows lies in shared memory, at most 48 KB of it
   if (a->rows <= ROWS_MAX && a->rows * padded(a->inner) * 2 <= 48 * 1024) r = launch_rows(p, x.p, x.ld, w.p, w.ld, stream);
   else r = launch_product<0, 0>(x.p, x.ld, w.p, w.ld, p, stream);
@@ -1112,9 +1137,12 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
       ++n;
     }
   }
+  Operands operands{work, at};
+  Operand w{}, x{};
+  if (a->dx) w = operands.add(a->w, a->ld_w, cols, inner);
+  if (a->dw) x = operands.add(a->x, a->ld_x, rows, inner);
+  if ((r = operands.launch(n, stream))) return r;
   if (a->dx) {        // [rows, inner] = dz [rows, cols] w [cols, inner]
-    Operand w;
-    if ((r = operand(w, a->w, a->ld_w, cols, inner, work, at, n, stream))) return r;
     LinParams p{};
     p.M = rows; p.N = inner; p.K = cols; p.mode = LIN_OUT; p.k_splits = 1;
     p.C = static_cast<__nv_bfloat16*>(a->dx); p.ldc = pitch(a->ld_dx, rows, inner); p.status = a->status;
@@ -1123,8 +1151,6 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   }
   if (!a->dw) return n;
   // [cols, inner] = dz^T x
-  Operand x;
-  if ((r = operand(x, a->x, a->ld_x, rows, inner, work, at, n, stream))) return r;
   LinParams p{};
   p.M = cols; p.N = inner; p.K = rows; p.status = a->status;
   p.k_splits = dw_slices(rows, inner, cols);
@@ -1133,7 +1159,7 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   if (direct) {
     p.C = static_cast<__nv_bfloat16*>(a->dw); p.ldc = pitch(a->ld_dw, cols, inner);
   } else {
-    p.part = reinterpret_cast<float*>(work + at); p.ld_part = (inner + 3) / 4 * 4;
+    p.part = reinterpret_cast<float*>(work + operands.at); p.ld_part = (inner + 3) / 4 * 4;
   }
   if ((r = launch_product<1, 1>(dz.p, dz.ld, x.p, x.ld, p, stream))) return r - 1000;
   ++n;
