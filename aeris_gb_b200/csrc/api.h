@@ -247,6 +247,7 @@ typedef struct AerisLayerNorm {
   const void *w, *b;                // [cols], bf16 or fp32 both; null: ones, zeros
   float *stats;                     // [rows, 2]
   float *dw, *db, *work;            // [cols] each, null: not wanted; work: [slices, 2, cols]
+  int* status;
   long long rows, ld_x, ld_dy, ld_y;
   int cols, f32, w_f32, add, slices;            // f32: type of x, dy, y; add: dw, db are added to
   float eps;

@@ -1,8 +1,8 @@
 // Layer norm of rows that lie in registers. Included by layer_norm.cu.
 //
 // Memory is the floor: a row is read once (forward) or with its gradient once (backward) and written once. Rows are taken in
-// vectors of 16 bytes where they start on 16-byte boundaries and consist of whole ones, else element by element; a lane has up to NV of them. Narrow
-// rows share a warp (a group of lanes each), rows up to 32 NV vectors take a warp, wider ones a block of up to 1,024 threads.
+// vectors of 16 bytes where they start on 16-byte boundaries and consist of whole ones, else element by element; a lane has up to
+// NV of them. Narrow rows share a warp (a group of lanes each), rows up to 32 NV vectors take a warp, wider ones a block of up to 1,024 threads.
 #pragma once
 
 namespace aeris {
@@ -446,6 +446,263 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLay
   }
 }
 
+// Many rows that start anywhere: a block per R rows, which come through a ring of bulk copies some rounds ahead, in the granules of 16
+// bytes that hold them (a granule with one byte of an allocation lies in it as a whole). A thread has columns threadIdx,
+// threadIdx + TH, .. of all rows; weights and column sums stay in registers. More rows a round hide the
+// block's sums, fewer leave registers (gradients of rows of 3,411 bf16: two rows a round 158 us, with spills, one 123). What bounds it
+// is issue slots: an element at a time, of two bytes. Forward and gradients, in us, against lanes that read memory themselves:
+// 19,366 x 3,411 bf16 88 and 123 (222 and 224), 50,000 x 1,001 bf16 78 and 99 (128 and 157), 20,000 x 333 fp32 17 and 23 (26 and 26),
+// 1,200 x 1,001 bf16 5.3 and 6.2 (6.2 and 7.7).
+struct OddRing {
+  uint64_t* bars;
+  uint8_t* mem;
+  int stages, bytes;            // bytes of a row's place
+  static __device__ __forceinline__ uint32_t granules(const void* row, int size) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+    return static_cast<uint32_t>(((at + size + 15) & ~uintptr_t(15)) - (at & ~uintptr_t(15)));
+  }
+  static __device__ __forceinline__ void request(uint8_t* dst, const void* row, int size, uint64_t* bar) {
+    bulk_load(dst, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15)), granules(row, size), bar);
+  }
+};
+// A wait gave up: the rounds that were asked for from (st, ph) on are let in (bounded) before the block's memory is another's.
+__device__ __forceinline__ void odd_drain(uint64_t* bars, int stages, int st, uint32_t ph, long long r0, long long step, const AerisLayerNorm& a) {
+  for (int i = 0; i < stages && r0 < a.rows; ++i, r0 += step) {
+    if (threadIdx.x < 32) mbar_wait_warp(bars + st, ph, a.status, ERR_TIMEOUT_FULL);
+    if (++st == stages) { st = 0; ph ^= 1; }
+  }
+}
+// Sums over the block in every thread; false where a thread of it says so.
+template <int K>
+__device__ __forceinline__ bool odd_sums(float (&v)[K], bool ok, float* part) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  // everyone has taken the words of the sums before, and its elements of this round's rows
+  if (!__syncthreads_and(ok)) return false;
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) part[k * 32 + (threadIdx.x >> 5)] = v[k];
+  __syncthreads();
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? part[k * 32 + lane] : 0.f);
+  return true;
+}
+
+template <typename T, int NV, int R, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) ln_fwd_odd_kernel(const AerisLayerNorm a, const int stages, const int bytes) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float part[32 * R];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  uint8_t* mem = smem + 64;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  chain_point();
+  const int size = a.cols * static_cast<int>(sizeof(T));
+  const T* x0 = static_cast<const T*>(a.x);
+  const long long step = static_cast<long long>(gridDim.x) * R;
+  auto request = [&](long long r0, int st) {
+    if (threadIdx.x != 0 || r0 >= a.rows) return;
+    uint32_t all = 0;
+    for (int r = 0; r < R && r0 + r < a.rows; ++r) all += OddRing::granules(x0 + (r0 + r) * a.ld_x, size);
+    mbar_expect_tx(bars + st, all);
+    for (int r = 0; r < R && r0 + r < a.rows; ++r)
+      OddRing::request(mem + (st * R + r) * bytes, x0 + (r0 + r) * a.ld_x, size, bars + st);
+  };
+  long long r0 = static_cast<long long>(blockIdx.x) * R;
+  for (int i = 0; i < stages; ++i) request(r0 + i * step, i);
+  float w[NV], b[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * TH + threadIdx.x;
+    w[i] = c < a.cols && a.w ? weight_at(a.w, a.w_f32, c) : 1.f;
+    b[i] = c < a.cols && a.b ? weight_at(a.b, a.w_f32, c) : 0.f;
+  }
+  const float inv = 1.f / static_cast<float>(a.cols);
+  uint32_t ph = 0;
+  for (int st = 0; r0 < a.rows; r0 += step) {
+    const bool ok = mbar_wait_warp(bars + st, ph, a.status, ERR_TIMEOUT_FULL);
+    float v[R][NV], s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const T* x = reinterpret_cast<const T*>(mem + (st * R + r) * bytes + (reinterpret_cast<uintptr_t>(x0 + (r0 + r) * a.ld_x) & 15));
+      s[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TH + threadIdx.x;
+        v[r][i] = c < a.cols && r0 + r < a.rows ? ld_f(x + c) : 0.f;
+        s[r] += v[r][i];
+      }
+    }
+    if (!odd_sums(s, ok, part)) {
+      odd_drain(bars, stages, st, ph, r0, step, a);
+      return;
+    }
+    request(r0 + stages * step, st);
+    if (++st == stages) { st = 0; ph ^= 1; }
+    float mean[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = s[r] * inv;
+      s[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        v[r][i] -= mean[r];
+        if (i * TH + static_cast<int>(threadIdx.x) < a.cols) s[r] = fmaf(v[r][i], v[r][i], s[r]);
+      }
+    }
+    odd_sums(s, true, part);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r0 + r >= a.rows) continue;
+      const float rstd = 1.f / sqrtf(s[r] * inv + a.eps);
+      T* y = static_cast<T*>(a.y) + (r0 + r) * a.ld_y;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TH + threadIdx.x;
+        if (c < a.cols) st_f(y + c, fmaf(v[r][i] * rstd, w[i], b[i]));
+      }
+      if (threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + 2 * (r0 + r)) = make_float2(mean[r], rstd);
+    }
+  }
+}
+
+template <typename T, int NV, int R, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) ln_bwd_odd_kernel(const AerisLayerNorm a, const int stages, const int bytes) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float part[64 * R];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  uint8_t* mem = smem + 64;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  chain_point();
+  const int size = a.cols * static_cast<int>(sizeof(T));
+  const T *x0 = static_cast<const T*>(a.x), *g0 = static_cast<const T*>(a.dy);
+  const long long step = static_cast<long long>(gridDim.x) * R;
+  auto request = [&](long long r0, int st) {
+    if (threadIdx.x != 0 || r0 >= a.rows) return;
+    uint32_t all = 0;
+    for (int r = 0; r < R && r0 + r < a.rows; ++r)
+      all += OddRing::granules(x0 + (r0 + r) * a.ld_x, size) + OddRing::granules(g0 + (r0 + r) * a.ld_dy, size);
+    mbar_expect_tx(bars + st, all);
+    for (int r = 0; r < R && r0 + r < a.rows; ++r) {
+      uint8_t* dst = mem + (st * R + r) * 2 * bytes;
+      OddRing::request(dst, x0 + (r0 + r) * a.ld_x, size, bars + st);
+      OddRing::request(dst + bytes, g0 + (r0 + r) * a.ld_dy, size, bars + st);
+    }
+  };
+  long long r0 = static_cast<long long>(blockIdx.x) * R;
+  for (int i = 0; i < stages; ++i) request(r0 + i * step, i);
+  float w[NV], dw[NV], db[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * TH + threadIdx.x;
+    w[i] = c < a.cols && a.w ? weight_at(a.w, a.w_f32, c) : 1.f;
+    dw[i] = db[i] = 0.f;
+  }
+  const float inv = 1.f / static_cast<float>(a.cols);
+  uint32_t ph = 0;
+  for (int st = 0; r0 < a.rows; r0 += step) {
+    const bool ok = mbar_wait_warp(bars + st, ph, a.status, ERR_TIMEOUT_FULL);
+    float v[R][NV], g[R][NV], s[2 * R];       // v: xhat
+    float rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool live = r0 + r < a.rows;
+      const float2 t = live ? *reinterpret_cast<const float2*>(a.stats + 2 * (r0 + r)) : make_float2(0.f, 0.f);
+      const uint8_t* at = mem + (st * R + r) * 2 * bytes;
+      const T* x = reinterpret_cast<const T*>(at + (reinterpret_cast<uintptr_t>(x0 + (r0 + r) * a.ld_x) & 15));
+      const T* dy = reinterpret_cast<const T*>(at + bytes + (reinterpret_cast<uintptr_t>(g0 + (r0 + r) * a.ld_dy) & 15));
+      rstd[r] = t.y;
+      s[2 * r] = s[2 * r + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TH + threadIdx.x;
+        const bool in = c < a.cols && live;
+        v[r][i] = in ? (ld_f(x + c) - t.x) * t.y : 0.f;
+        const float d = in ? ld_f(dy + c) : 0.f;
+        dw[i] = fmaf(d, v[r][i], dw[i]);
+        db[i] += d;
+        g[r][i] = d * w[i];
+        s[2 * r] += g[r][i];
+        s[2 * r + 1] = fmaf(g[r][i], v[r][i], s[2 * r + 1]);
+      }
+    }
+    if (!odd_sums(s, ok, part)) {
+      odd_drain(bars, stages, st, ph, r0, step, a);
+      return;
+    }
+    request(r0 + stages * step, st);
+    if (++st == stages) { st = 0; ph ^= 1; }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r0 + r >= a.rows) continue;
+      const float m1 = s[2 * r] * inv, m2 = s[2 * r + 1] * inv;
+      T* dx = static_cast<T*>(a.y) + (r0 + r) * a.ld_y;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = i * TH + threadIdx.x;
+        if (c < a.cols) st_f(dx + c, rstd[r] * (g[r][i] - m1 - v[r][i] * m2));
+      }
+    }
+  }
+  if (!a.work) return;
+  float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = i * TH + threadIdx.x;
+    if (c < a.cols) {
+      out[c] = dw[i];
+      out[a.cols + c] = db[i];
+    }
+  }
+}
+
+// `slices`: null forward; backward it receives how many slices of column sums were written. Returns 1 where the ring would have one
+// stage alone.
+template <typename T, int NV, int RF, int RB, int TH>
+int launch_ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
+  constexpr int PER_SM = 1024 / TH;
+  const int R = slices ? RB : RF;
+  const int bytes = (a.cols * static_cast<int>(sizeof(T)) + 30) / 16 * 16, row = slices ? 2 * bytes : bytes;
+  int stages = (200 * 1024 / PER_SM - 1024) / (R * row);
+  if (stages < 2) return 1;
+  if (stages > 6) stages = 6;
+  const long long need = (a.rows + R - 1) / R;
+  long long blocks = static_cast<long long>(num_sms()) * PER_SM;
+  if (blocks > need) blocks = need;
+  if (slices && a.work && blocks > a.slices) blocks = a.slices;
+  const int smem = 64 + stages * R * row;
+  if (slices) {
+    static std::atomic<uint64_t> done{0};
+    if (!allow_smem_once(ln_bwd_odd_kernel<T, NV, RB, TH>, 200 * 1024, done)) return -20;
+    *slices = static_cast<int>(blocks);
+    return launch_chained(ln_bwd_odd_kernel<T, NV, RB, TH>, static_cast<unsigned>(blocks), TH, smem, stream, a, stages, bytes);
+  }
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem_once(ln_fwd_odd_kernel<T, NV, RF, TH>, 200 * 1024, done)) return -20;
+  return launch_chained(ln_fwd_odd_kernel<T, NV, RF, TH>, static_cast<unsigned>(blocks), TH, smem, stream, a, stages, bytes);
+}
+// Where rows are many enough for rounds that follow one another; others, and the widest, go straight from memory.
+template <typename T>
+int ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
+  if (a.rows < 8 * num_sms() || a.cols <= 96 || a.cols > 8192) return 1;
+  int r = 1;
+  if (a.cols <= 256) r = launch_ln_odd<T, 4, 4, 2, 64>(a, stream, slices);
+  else if (a.cols <= 512) r = launch_ln_odd<T, 4, 4, 2, 128>(a, stream, slices);
+  else if (a.cols <= 1024) r = launch_ln_odd<T, 4, 4, 2, 256>(a, stream, slices);
+  else if (a.cols <= 2048) r = launch_ln_odd<T, 4, 4, 2, 512>(a, stream, slices);
+  else if (a.cols <= 4096) r = launch_ln_odd<T, 8, 2, 1, 512>(a, stream, slices);
+  if (r == 1 && a.cols > 2048) r = a.cols <= 4096 ? launch_ln_odd<T, 8, 1, 1, 512>(a, stream, slices) : launch_ln_odd<T, 8, 1, 1, 1024>(a, stream, slices);
+  return r;
+}
+
 bool ln_aligned(const void* p, long long ld, int size) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
 }
@@ -487,6 +744,8 @@ int ln_fwd_fast(const AerisLayerNorm& a, cudaStream_t stream) {
     if (vecs <= 4096) return launch_ln_fwd<T, W, 4, true>(a, cut, ln_threads(vecs, 4), stream);
     return 1;
   }
+  const int odd = ln_odd<T>(a, stream, nullptr);
+  if (odd <= 0) return odd;
   const int nv = (a.cols + 31) / 32;
   const LnCut cut = ln_cut(a.cols);
   if (nv <= 1) return launch_ln_fwd<T, 1, 1, false>(a, cut, 256, stream);
@@ -530,6 +789,10 @@ int ln_bwd_fast(const AerisLayerNorm& a, cudaStream_t stream, int& slices) {
     if (vecs <= 1024) return launch_ln_bwd<T, W, 2, 2, true, 512, 1>(a, cut, ln_threads(vecs, 2), stream, slices);
     if (vecs <= 2048) return launch_ln_bwd<T, W, 4, 1, true, 512, 1>(a, cut, ln_threads(vecs, 4), stream, slices);
     return 1;
+  }
+  if ((!a.dw && !a.db) || a.work) {
+    const int odd = ln_odd<T>(a, stream, &slices);
+    if (odd <= 0) return odd;
   }
   const LnCut cut = ln_cut(a.cols);
   if (a.cols <= 32) return launch_ln_bwd<T, 1, 1, 4, false, 256, 3>(a, cut, 256, stream, slices);
