@@ -275,6 +275,26 @@ template <typename... P, typename... A>
   return cudaGetLastError() == cudaSuccess ? 0 : -21;
 }
 
+// The same for one cluster of CTAs.
+template <typename... P, typename... A>
+[[nodiscard]] static inline int launch_chained_cluster(void (*kern)(P...), unsigned ctas, int threads, size_t smem,
+                                                       cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {ctas, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  return cudaGetLastError() == cudaSuccess ? 0 : -21;
+}
+
 // What has to be done once for a kernel on every device, such as allowing it its shared memory: `done` has a bit for each.
 template <typename F> static inline bool once_a_device(std::atomic<uint64_t>& done, F&& f) {
   int dev = 0;

@@ -9,6 +9,7 @@
 #include "common.cuh"
 #include "api.h"
 #include "host.h"
+#include "cluster.cuh"
 
 namespace aeris {
 
@@ -169,12 +170,12 @@ extern "C" int aeris_layer_norm_bwd(const AerisLayerNorm* a, void* stream_) {
   if (!ln_fits(a) || !a->dy || a->ld_dy < 0) return -1;
   const bool sums = a->dw || a->db;
   if (sums && (a->slices <= 0 || a->slices > 65535 || (a->slices > 1) != (a->work != nullptr))) return -2;
+  if (sums && !a->work && a->cols > 4096) return -3;       // a CTA's column sums are in shared memory
   int n = 1, slices = a->slices;
   int r = a->f32 ? ln_bwd_fast<float>(*a, stream, slices) : ln_bwd_fast<__nv_bfloat16>(*a, stream, slices);
   if (r < 0) return r;
   const bool fast = r == 0;
   if (!fast && sums) {     // first: the gradient of x may take the place of x or dy
-    if (!a->work) return -3;
     const dim3 grid((a->cols + LN_COLS - 1) / LN_COLS, a->slices);
     r = a->f32 ? launch_chained(ln_sums_any_kernel<float>, grid, LN_THREADS, 0, stream, *a)
                : launch_chained(ln_sums_any_kernel<__nv_bfloat16>, grid, LN_THREADS, 0, stream, *a);

@@ -321,28 +321,42 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   if (warp == C::W_MMA) tmem_dealloc(tmem_base, C::TMEM);
 }
 
-// Tiles that several CTAs took part in: what those before the last one left in `extra`, in their order. Block (x, y): the
-// tile that CTA x of the sums left unfinished, if x is the first one that did; rows y, y + 32, .. of it.
+// Tiles that several CTAs took part in: what those before the last one left in `extra`, in their order, eight sequences of them beside one
+// another. Block (t, y): rows y, y + gridDim.y, .. of the t-th tile of the runs.
 __global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, const BgPlan plan, int tk) {
+  __shared__ float4 part[8][32];
   chain_point();
-  const int b0 = blockIdx.x, first = plan.first(b0), end = plan.first(b0 + 1), t = (end - 1) / p.n_win;
-  // it ends in the middle of tile t, unless an earlier CTA that does has its turn with the tile
-  if (end % p.n_win == 0 || first > t * p.n_win) return;
-  const BgTile b = bg_tile(plan.rounds * plan.ctas + t, p.n, tk);
-  const int cols = min(tk, p.n - b.tj * tk), vecs = (cols + 3) / 4;
-  int b1 = b0 + 1;        // CTAs b0 .. b1 - 1 left it unfinished
-  while (plan.first(b1 + 1) < (t + 1) * p.n_win) ++b1;
-  for (int i = threadIdx.x; i < 4 * vecs; i += 256) {       // four rows at a time
-    const int r = blockIdx.y + gridDim.y * (i / vecs), v = i % vecs;
-    if (b.ti * PB_TILE + r >= p.n) continue;
-    float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
-    float4 s = *dst;
+  const int u0 = blockIdx.x * p.n_win, u1 = u0 + p.n_win, v = threadIdx.x & 31, k = threadIdx.x >> 5;
+  int b0 = static_cast<int>(static_cast<long long>(u0) * plan.runs / plan.steps), b1;      // those with its first and its last step
+  while (plan.first(b0 + 1) <= u0) ++b0;
+  while (plan.first(b0) > u0) --b0;
+  b1 = static_cast<int>(static_cast<long long>(u1 - 1) * plan.runs / plan.steps);
+  while (plan.first(b1 + 1) < u1) ++b1;
+  while (plan.first(b1) >= u1) --b1;
+  if (b0 == b1) return;
+  const BgTile b = bg_tile(plan.rounds * plan.ctas + blockIdx.x, p.n, tk);
+  const bool in = v < (min(tk, p.n - b.tj * tk) + 3) / 4;
+  for (int r = blockIdx.y; r < min(PB_TILE, p.n - b.ti * PB_TILE); r += gridDim.y) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in)
 #pragma unroll 4
-    for (int k = b0; k < b1; ++k) {
-      const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(k) * PB_TILE + r) * tk) + v);
-      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      for (int i = b0 + k; i < b1; i += 8) {
+        const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(i) * PB_TILE + r) * tk) + v);
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      }
+    part[k][v] = s;
+    __syncthreads();
+    if (k == 0 && in) {
+      float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
+      s = *dst;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 x = part[i][v];
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+      }
+      *dst = s;
     }
-    *dst = s;
+    __syncthreads();
   }
 }
 
@@ -492,7 +506,8 @@ int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, const BgPlan&
   ++kernels;
   if (r || !plan.runs) return r;
   ++kernels;
-  return launch_chained(bias_join_kernel, dim3(plan.runs, PB_TILE / 4), 256, 0, stream, p, plan, C::TK);
+  const int tiles = plan.tiles - plan.rounds * plan.ctas;
+  return launch_chained(bias_join_kernel, dim3(tiles, tiles < 32 ? PB_TILE : PB_TILE / 4), 256, 0, stream, p, plan, C::TK);
 }
 
 }  // namespace

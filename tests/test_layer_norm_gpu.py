@@ -105,6 +105,14 @@ def test_many_rows(rows, cols, layout, dt):
     test_both_directions(rows, cols, layout, dt)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["whole", "odd pitch", "odd start"])
+@pytest.mark.parametrize("rows,cols", [(1200, 3411), (1300, 5003), (1190, 8191), (400, 9001), (200, 16383), (330, 12544), (123, 290), (31, 4001),
+                                       (33, 3968), (16, 8192), (2000, 65), (4096, 32)])
+def test_wide_rows_and_clusters(rows, cols, layout, dt):
+    test_both_directions(rows, cols, layout, dt)
+
+
 @pytest.mark.parametrize("rows,cols", [(65, 512), (40, 333), (77, 1536), (5, 8191), (900, 48), (2500, 640), (2400, 333)])
 @pytest.mark.parametrize("parts", ["none", "weight", "bias", "fp32"])
 def test_weight_and_bias_may_be_missing_or_in_fp32(rows, cols, parts):

@@ -275,6 +275,12 @@ def test_several_heads_in_the_run_of_a_block(n_win, window, heads, d):
     run_both(*make(n_win, window, heads, d, g), n_win, window, heads, d)
 
 
+@pytest.mark.parametrize("n_win,window,heads,d", [(700, (17, 4), 1, 72), (900, (3, 20), 1, 64), (149, (8, 16), 2, 32), (40, (12, 12), 17, 64)])
+def test_few_tiles_of_many_windows(n_win, window, heads, d):
+    g = torch.Generator(device=DEV).manual_seed(n_win)
+    run_both(*make(n_win, window, heads, d, g), n_win, window, heads, d)
+
+
 def test_same_bits_captured_and_on_another_stream():
     g = torch.Generator(device=DEV).manual_seed(8)
     qkv, table, buckets, d_o = make(20, (9, 16), 4, 64, g, 50)
