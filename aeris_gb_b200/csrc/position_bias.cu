@@ -414,10 +414,15 @@ __global__ void __launch_bounds__(256) bias_buckets_kernel(const AerisBiasedAttn
   }
 }
 
-__global__ void __launch_bounds__(256) bias_zero_kernel(float* p, long long n) {
-  chain_point();
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) p[i] = 0.f;
-}
+}  // namespace
+
+}  // namespace aeris
+
+#include "position_bias_small.cuh"
+
+namespace aeris {
+
+namespace {
 
 constexpr long long PART_BYTES = 256ll << 20;
 
@@ -460,6 +465,26 @@ BgPlan plan_tiles(int tiles, int n_win) {
 }
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
+
+// Windows that position_bias_small.cuh takes; what it needs: sums by relative position of every run of windows, and where there are
+// buckets those of all runs.
+bool small(int high, int wide) { return static_cast<long long>(high) * wide <= SMALL_TOKENS; }
+long long small_part(int n_win, int high, int wide, int heads, int head_dim) {
+  return up(4ll * small_runs(n_win, high * wide, heads, head_dim, true) * heads * (2 * high - 1) * (2 * wide - 1));
+}
+SmallParams small_params(const AerisBiasedAttn* a, bool backward) {
+  SmallParams p{};
+  p.qkv = static_cast<const __nv_bfloat16*>(a->qkv); p.d_o = static_cast<const __nv_bfloat16*>(a->d_o);
+  p.o = static_cast<__nv_bfloat16*>(a->o); p.dqkv = static_cast<__nv_bfloat16*>(a->dqkv); p.lse = a->lse;
+  p.ld = a->ld_qkv; p.ldo = a->ld_o; p.ldg = a->ld_dqkv;
+  p.n_win = a->n_win; p.n = a->high * a->wide; p.d = a->head_dim; p.scale = a->scale;
+  p.runs = small_runs(a->n_win, p.n, a->heads, a->head_dim, backward);
+  Place dense{};
+  dense.pitch = 2 * a->wide - 1;
+  p.source = source_of(a, dense);
+  return p;
+}
+bool whole_rows(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
 struct Work {
   long long table, at, delta, rest, by_position, part, extra, total;
@@ -518,6 +543,10 @@ using namespace aeris;
 
 extern "C" long long aeris_biased_attn_work_bytes(int n_win, int high, int wide, int heads, int head_dim, int backward, int with_table) {
   if (n_win <= 0 || high <= 0 || wide <= 0 || heads <= 0 || head_dim <= 0 || static_cast<long long>(high) * wide > 32768) return -1;
+  if (small(high, wide)) {
+    if (!backward || !with_table) return 0;
+    return small_part(n_win, high, wide, heads, head_dim) + up(4ll * heads * (2 * high - 1) * (2 * wide - 1));
+  }
   if (!backward) {
     BiasSource s{};
     s.high = high; s.wide = wide; s.pitch = place_of(high, wide).pitch;
@@ -529,6 +558,11 @@ extern "C" long long aeris_biased_attn_work_bytes(int n_win, int high, int wide,
 extern "C" int aeris_biased_attn_fwd(const AerisBiasedAttn* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!fits(a)) return -1;
+  if (small(a->high, a->wide)) {
+    if (a->head_dim > 128 || a->head_dim % 8 || !whole_rows(a->qkv, a->ld_qkv) || !whole_rows(a->o, a->ld_o) || !a->lse) return -3;
+    const int r = launch_small(small_params(a, false), false, stream);
+    return r ? r : 1;
+  }
   const Place p = place_of(a->high, a->wide);
   const BiasSource source = source_of(a, p);
   if (biased_fwd_reads_source(a->n_win, a->heads, a->head_dim, source)) {
@@ -552,6 +586,25 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (!fits(a) || !a->d_o || !a->dqkv || !a->lse) return -1;
   const bool sums = a->dtable != nullptr;
+  if (small(a->high, a->wide)) {
+    const int size = (2 * a->high - 1) * (2 * a->wide - 1) * a->heads;
+    const long long part = small_part(a->n_win, a->high, a->wide, a->heads, a->head_dim);
+    if (a->head_dim > 128 || a->head_dim % 8 || !whole_rows(a->qkv, a->ld_qkv) || !whole_rows(a->d_o, a->ld_o) ||
+        !whole_rows(a->dqkv, a->ld_dqkv))
+      return -3;
+    if (sums && (!a->work || a->work_bytes < part + up(4ll * size))) return -2;
+    SmallParams s = small_params(a, true);
+    if (sums) s.part = static_cast<float*>(a->work);
+    int r = launch_small(s, true, stream);
+    if (r || !sums) return r ? r : 1;
+    float* out = a->buckets ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->work) + part) : a->dtable;
+    r = launch_chained(small_join_kernel, (size + 31) / 32, 256, 0, stream, static_cast<const float*>(s.part), out, s.runs, size,
+                       a->buckets ? 0 : a->add);
+    if (r || !a->buckets) return r ? r - 100 : 2;
+    r = launch_chained(bias_buckets_kernel, dim3(a->table_rows, (a->heads + 31) / 32), 256, 0, stream, *a, static_cast<const float*>(out),
+                       (2 * a->high - 1) * (2 * a->wide - 1));
+    return r ? r - 500 : 3;
+  }
   const Work w = work_of(a->n_win, a->high, a->wide, a->heads, a->head_dim, true, sums);
   if (!a->work || a->work_bytes < w.total) return -2;
   const Place p = place_of(a->high, a->wide);
@@ -568,12 +621,6 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   if (r) return r - 100;
   int count = 4;
   if (!sums) return count;
-  if (p.n == 1) {       // one token sees itself whatever the bias
-    if (a->add) return count;
-    const long long cells = static_cast<long long>(a->table_rows) * a->heads, blocks = (cells + 255) / 256;
-    r = launch_chained(bias_zero_kernel, static_cast<unsigned>(blocks < 1024 ? blocks : 1024), 256, 0, stream, a->dtable, cells);
-    return r ? r : count + 1;
-  }
   const int dch = a->head_dim <= 64 ? 1 : 2, tk = dch == 1 ? BgCfg<1>::TK : BgCfg<2>::TK, hd = a->heads * a->head_dim;
   const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a->qkv);
   CUtensorMap m[4];

@@ -193,10 +193,10 @@ def biased_attn_bwd(d_o: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, lse: 
     g = dqkv if tiled and dqkv is not None else qkv.new_empty((tokens, 3 * heads * dp))
     if n_win:
         size = _work_bytes(n_win, high, wide, heads, dp, True, need_dtable)
-        work = qkv.new_empty(size, dtype=torch.uint8)
+        work = qkv.new_empty(size, dtype=torch.uint8) if size else None
         _launch("aeris_biased_attn_bwd", _RECORD.pack(
             rows.data_ptr(), of.data_ptr(), lse.data_ptr(), table.data_ptr(), 0 if buckets is None else buckets.data_ptr(), do.data_ptr(),
-            g.data_ptr(), dtable.data_ptr() if need_dtable else 0, work.data_ptr(), _l.status_word(qkv.device).data_ptr(), pitch,
+            g.data_ptr(), dtable.data_ptr() if need_dtable else 0, work.data_ptr() if size else 0, _l.status_word(qkv.device).data_ptr(), pitch,
             o_pitch, g_pitch, size, n_win, high, wide, heads, dp, table.shape[0], table.dtype is _BF16,
             buckets is not None and buckets.dtype is torch.int64, add, scale), index)
     if not tiled:
