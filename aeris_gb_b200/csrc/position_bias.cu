@@ -12,6 +12,7 @@
 #include "common.cuh"
 #include "api.h"
 #include "host.h"
+#include "cluster.cuh"
 #include "position_bias.cuh"
 
 namespace aeris {
@@ -92,8 +93,8 @@ __device__ __forceinline__ float bg_exp2(float x) {
 struct BgTile {
   int head, ti, tj;           // head: of those at hand
 };
-__device__ __forceinline__ BgTile bg_tile(int t, int n, int tk) {
-  const int nj = (n + tk - 1) / tk, ni = (n + PB_TILE - 1) / PB_TILE;
+__device__ __forceinline__ BgTile bg_tile(int t, int n, int tm, int tk) {      // tiles of tm queries x tk keys
+  const int nj = (n + tk - 1) / tk, ni = (n + tm - 1) / tm;
   BgTile b;
   const int r = t / nj;
   b.tj = t - r * nj;
@@ -110,15 +111,15 @@ struct BgPlan {
 // What a CTA does, piece by piece: windows [w0, w1) of tile t.
 struct BgWork {
   const BgPlan& p;
-  int n_win, round = 0, u = 0, u1 = 0, t = 0, w0 = 0, w1 = 0;
-  __device__ __forceinline__ BgWork(const BgPlan& plan, int n_win_) : p(plan), n_win(n_win_) {
-    if (static_cast<int>(blockIdx.x) < p.runs) {
-      u = p.first(blockIdx.x);
-      u1 = p.first(blockIdx.x + 1);
+  int n_win, cta, round = 0, u = 0, u1 = 0, t = 0, w0 = 0, w1 = 0;
+  __device__ __forceinline__ BgWork(const BgPlan& plan, int n_win_, int cta_) : p(plan), n_win(n_win_), cta(cta_) {
+    if (cta < p.runs) {
+      u = p.first(cta);
+      u1 = p.first(cta + 1);
     }
   }
   __device__ __forceinline__ bool next() {
-    const int whole = round * p.ctas + blockIdx.x;
+    const int whole = round * p.ctas + cta;
     if (round < p.rounds || (!p.runs && whole < p.tiles)) {
       ++round;
       t = whole;
@@ -176,8 +177,8 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (BgWork k(plan, p.n_win); ok && k.next();) {
-        const BgTile b = bg_tile(k.t, p.n, TK);
+      for (BgWork k(plan, p.n_win, blockIdx.x); ok && k.next();) {
+        const BgTile b = bg_tile(k.t, p.n, PB_TILE, TK);
         const int head = p.head0 + b.head;
         for (int w = k.w0; w < k.w1; ++w) {
           if (!mbar_wait_poll(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
@@ -204,7 +205,7 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       int st = 0, buf = 0;
       uint32_t ph = 0, b_ph = 0;
       bool ok = true;
-      for (BgWork k(plan, p.n_win); ok && k.next();) {
+      for (BgWork k(plan, p.n_win, blockIdx.x); ok && k.next();) {
         for (int w = k.w0; w < k.w1; ++w) {
           ok = mbar_wait_poll(&s_empty[buf], b_ph ^ 1, p.status, ERR_TIMEOUT_ATTN) &&
                mbar_wait_poll(&full[st], ph, p.status, ERR_TIMEOUT_ATTN);
@@ -233,10 +234,10 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     int buf = 0;
     uint32_t b_ph = 0;
     bool ok = true;
-    for (BgWork work(plan, p.n_win); ok && work.next();) {
+    for (BgWork work(plan, p.n_win, blockIdx.x); ok && work.next();) {
       const int w1 = work.w1;
       int w = work.w0;
-      const BgTile b = bg_tile(work.t, p.n, TK);
+      const BgTile b = bg_tile(work.t, p.n, PB_TILE, TK);
       const int row0 = b.ti * PB_TILE + q * 32, row = row0 + lane, col = b.tj * TK + g * CPT;
       const bool in = row < p.n, has = row0 < p.n && col < p.n;       // has: some of this warp's pairs are in the window
       const float* bias = p.table + static_cast<long long>(p.head0 + b.head) * p.size + p.zero + p.at[in ? row : p.n - 1];    // bias[-at[j]]
@@ -321,9 +322,210 @@ bias_grad_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   if (warp == C::W_MMA) tmem_dealloc(tmem_base, C::TMEM);
 }
 
+// The same for more than 64 channels and 128 tokens, by pairs of CTAs (tcgen05.mma.cta_group::2): a tile is 256 queries, 128 of each
+// CTA, x 128 keys, of which a CTA brings in half. A CTA then reads 96 KB from L2 for 128 x 128 pairs where one alone reads 192. 30 windows
+// of 30 x 30, 24 heads of 128: 612 -> 456 us. With 64 channels (256 x 256, sums of 256 keys a row) the exponentials and the hand-over between
+// CTAs take what the reads gave: 72 windows, 24 heads 777 us for 755, 100 windows of 16 x 16, 8 heads 206 for 188 (whole backward pass).
+struct Bg2Cfg {
+  static constexpr int TK = 128, CPT = 32, DCH = 2, QB = DCH * 16384, KB = DCH * 8192, NST = 2, STAGE = 2 * QB + 2 * KB;
+  // warps and registers as above
+  static constexpr int MATH = 16, W_LOAD = MATH, W_MMA = MATH + 1, THREADS = 32 * (MATH + 4);
+  static constexpr int REGS_MATH = 104, REGS_REST = 64, REGS = 32 * (MATH * REGS_MATH + 4 * REGS_REST);
+  static constexpr int BARS = NST * STAGE, SMEM = BARS + 256 + 1024, TILE_FLOATS = 2 * PB_TILE * TK;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Bg2Cfg::THREADS, 1)
+bias_grad2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BgParams p,
+                  const BgPlan plan) {
+  using C = Bg2Cfg;
+  constexpr int TK = C::TK, NST = C::NST, DCH = C::DCH, CPT = C::CPT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);     // [NST], of the leader: both CTAs' copies
+  uint64_t* empty = full + NST;
+  uint64_t* s_full = empty + NST;       // [2]
+  uint64_t* s_empty = s_full + 2;       // [2], of the leader: an arrival per warp of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank()), pair = blockIdx.x >> 1;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_q); prefetch_tmap(&tm_do); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v);
+    for (int i = 0; i < NST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 2 * C::MATH); }
+    fence_barrier_init();
+  }
+  if (warp == C::W_MMA) { tmem_alloc2(tmem_slot, 512); tmem_relinquish2(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();       // both CTAs' barriers are initialised and tensor memory is allocated before anyone signals
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_point();
+
+  if (warp >= C::MATH) regs_dec<C::REGS_REST>();
+  if (warp == C::W_LOAD) {
+    if (elect_one_sync()) {
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (BgWork k(plan, p.n_win, pair); ok && k.next();) {
+        const BgTile b = bg_tile(k.t, p.n, 2 * PB_TILE, TK);
+        const int head = p.head0 + b.head, row0 = (2 * b.ti + rank) * PB_TILE, col0 = b.tj * TK + rank * 64;
+        for (int w = k.w0; w < k.w1; ++w) {
+          if (!mbar_wait_poll(&empty[st], ph ^ 1, p.status, ERR_TIMEOUT_ATTN)) { ok = false; break; }
+          uint8_t* s = smem + st * C::STAGE;
+          if (rank == 0) mbar_expect_tx(&full[st], 2 * C::STAGE);
+          const uint32_t fb = map_to_cta(smem_u32(&full[st]), 0);
+#pragma unroll
+          for (int c = 0; c < DCH; ++c) {
+            tma_load_4d_pair(s + c * 16384, &tm_q, fb, c * 64, head, row0, w);
+            tma_load_4d_pair(s + 2 * C::QB + c * 8192, &tm_k, fb, c * 64, head, col0, w);
+            tma_load_4d_pair(s + C::QB + c * 16384, &tm_do, fb, c * 64, head, row0, w);
+            tma_load_4d_pair(s + 2 * C::QB + C::KB + c * 8192, &tm_v, fb, c * 64, head, col0, w);
+          }
+          if (++st == NST) { st = 0; ph ^= 1; }
+        }
+      }
+      // after a time-out: the tiles that the issuer did not take, of both CTAs (a stage never filled counts as there)
+      for (int s = 0; s < NST && !ok && rank == 0; ++s) {
+        if (--st < 0) { st = NST - 1; ph ^= 1; }
+        if (!mbar_wait_poll(&full[st], ph, nullptr, 0)) break;
+      }
+    }
+  } else if (warp == C::W_MMA) {
+    if (rank == 0 && elect_one_sync()) {
+      constexpr uint32_t idesc = make_idesc_bf16(2 * PB_TILE, TK, 0, 0);
+      int st = 0, buf = 0;
+      uint32_t ph = 0, b_ph = 0;
+      bool ok = true, any = false;
+      for (BgWork k(plan, p.n_win, pair); ok && k.next();) {
+        for (int w = k.w0; w < k.w1; ++w) {
+          ok = mbar_wait_poll(&s_empty[buf], b_ph ^ 1, p.status, ERR_TIMEOUT_ATTN) &&
+               mbar_wait_poll(&full[st], ph, p.status, ERR_TIMEOUT_ATTN);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t s = smem_u32(smem + st * C::STAGE), d = tmem_base + buf * 2 * TK;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kk = 0; kk < 4 * DCH; ++kk)
+              umma2_ss(d + m * TK, make_smem_desc(s + m * C::QB + (kk >> 2) * 16384 + (kk & 3) * 32, 0, 1024),
+                       make_smem_desc(s + 2 * C::QB + m * C::KB + (kk >> 2) * 8192 + (kk & 3) * 32, 0, 1024), idesc, kk > 0);
+          tc_commit2_mc(&empty[st], 0x3);
+          tc_commit2_mc(&s_full[buf], 0x3);
+          any = true;
+          if (++st == NST) { st = 0; ph ^= 1; }
+          if (++buf == 2) { buf = 0; b_ph ^= 1; }
+        }
+      }
+      // the last products have completed, whether those who wait for them gave up or not
+      if (any) {
+        if (--st < 0) { st = NST - 1; ph ^= 1; }
+        mbar_wait_poll(&empty[st], ph, nullptr, 0);
+      }
+    }
+  } else if (warp < C::MATH) {
+    regs_inc<C::REGS_MATH>();
+    const int q = warp & 3, g = warp >> 2;
+    const uint32_t t0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + g * CPT;
+    const uint64_t sl = f2_pack(p.scale_log2, p.scale_log2);
+    const long long stat_step = static_cast<long long>(p.heads) * p.n;
+    int buf = 0;
+    uint32_t b_ph = 0;
+    bool ok = true;
+    for (BgWork work(plan, p.n_win, pair); ok && work.next();) {
+      const int w1 = work.w1;
+      int w = work.w0;
+      const BgTile b = bg_tile(work.t, p.n, 2 * PB_TILE, TK);
+      const int row0 = (2 * b.ti + rank) * PB_TILE + q * 32, row = row0 + lane, col = b.tj * TK + g * CPT;
+      const bool in = row < p.n, has = row0 < p.n && col < p.n;
+      const float* bias = p.table + static_cast<long long>(p.head0 + b.head) * p.size + p.zero + p.at[in ? row : p.n - 1];    // bias[-at[j]]
+      uint64_t sum[CPT / 2];
+      bool near = true;
+#pragma unroll
+      for (int i = 0; i < CPT / 2; ++i) sum[i] = 0ull;
+      if (has)
+#pragma unroll 4
+        for (int i = 0; i < CPT; ++i) near = near && fabsf(bias[-p.at[min(col + i, p.n - 1)]]) <= 64.f;       // no NaN either
+      near = __all_sync(0xffffffffu, near);
+      const long long stat = static_cast<long long>(p.head0 + b.head) * p.n + (in ? row : p.n - 1);
+      float lse = p.lse[stat + w * stat_step], delta = p.delta[stat + w * stat_step];
+      // 16 columns from column c on; one branch for all of them keeps their exponentials together
+      auto add = [&](const uint32_t (&s)[16], const uint32_t (&dp)[16], uint64_t nl, uint64_t nd, int c, bool with_bias) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          uint64_t e = f2_fma(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sl, nl);
+          if (with_bias) {          // the places go on behind the window's end
+            const int2 a = *reinterpret_cast<const int2*>(p.at + col + c + i);
+            e = f2_add(e, f2_pack(bias[-a.x], bias[-a.y]));
+          }
+          float e0, e1;
+          f2_unpack(e, e0, e1);
+          const uint64_t d = f2_add(f2_pack(__uint_as_float(dp[i]), __uint_as_float(dp[i + 1])), nd);
+          sum[(c + i) / 2] = f2_fma(f2_pack(bg_exp2(e0), bg_exp2(e1)), d, sum[(c + i) / 2]);
+        }
+      };
+      for (; w < w1; ++w) {
+        const uint64_t nl = f2_pack(-lse, -lse), nd = f2_pack(-delta, -delta);
+        if (w + 1 < w1) {
+          lse = p.lse[stat + (w + 1) * stat_step];
+          delta = p.delta[stat + (w + 1) * stat_step];
+        }
+        ok = mbar_wait_warp(&s_full[buf], b_ph, p.status, ERR_TIMEOUT_ATTN);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t tS = t0 + buf * 2 * TK, tD = tS + TK, freed = map_to_cta(smem_u32(&s_empty[buf]), 0);
+        if (has) {
+#pragma unroll
+          for (int c = 0; c < CPT; c += 16) {
+            uint32_t s[16], dp[16];
+            tmem_ld16(tS + c, s);
+            tmem_ld16(tD + c, dp);
+            tmem_wait_ld();
+            if (c + 16 == CPT) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_remote_relaxed(freed);
+            }
+            if (near) add(s, dp, nl, nd, c, false);
+            else if (col + c < p.n) add(s, dp, nl, nd, c, true);
+          }
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote_relaxed(freed);
+        }
+        if (++buf == 2) { buf = 0; b_ph ^= 1; }
+      }
+      if (!ok || failed(p.status)) break;
+      float* dst = w1 == p.n_win ? p.part + (static_cast<long long>(b.head) * p.n + row) * p.ld + col       // ld a multiple of 4
+                                 : p.extra + static_cast<long long>(pair) * C::TILE_FLOATS + (rank * PB_TILE + q * 32 + lane) * TK + g * CPT;
+      if (has && in)
+#pragma unroll
+        for (int i = 0; i < CPT; i += 4)
+          if (col + i < p.n) {
+            float v[4];
+            f2_unpack(sum[i / 2], v[0], v[1]);
+            f2_unpack(sum[i / 2 + 1], v[2], v[3]);
+            if (near) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] *= bg_exp2(bias[-p.at[min(col + i + k, p.n - 1)]]);
+            }
+            *reinterpret_cast<float4*>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();       // nobody leaves while the pair may still touch its shared memory or tensor memory
+  tc_fence_after();
+  if (warp == C::W_MMA) tmem_dealloc2(tmem_base, 512);
+}
+
 // Tiles that several CTAs took part in: what those before the last one left in `extra`, in their order, eight sequences of them beside one
-// another. Block (t, y): rows y, y + gridDim.y, .. of the t-th tile of the runs.
-__global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, const BgPlan plan, int tk) {
+// another. Block (t, y): parts y, y + gridDim.y, .. (32 vectors of a row each) of the t-th tile of the runs.
+__global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, const BgPlan plan, int tm, int tk) {
   __shared__ float4 part[8][32];
   chain_point();
   const int u0 = blockIdx.x * p.n_win, u1 = u0 + p.n_win, v = threadIdx.x & 31, k = threadIdx.x >> 5;
@@ -334,20 +536,22 @@ __global__ void __launch_bounds__(256) bias_join_kernel(const BgParams p, const 
   while (plan.first(b1 + 1) < u1) ++b1;
   while (plan.first(b1) >= u1) --b1;
   if (b0 == b1) return;
-  const BgTile b = bg_tile(plan.rounds * plan.ctas + blockIdx.x, p.n, tk);
-  const bool in = v < (min(tk, p.n - b.tj * tk) + 3) / 4;
-  for (int r = blockIdx.y; r < min(PB_TILE, p.n - b.ti * PB_TILE); r += gridDim.y) {
+  const BgTile b = bg_tile(plan.rounds * plan.ctas + blockIdx.x, p.n, tm, tk);
+  const int vecs = (min(tk, p.n - b.tj * tk) + 3) / 4, groups = (vecs + 31) / 32, rows = min(tm, p.n - b.ti * tm);
+  for (int item = blockIdx.y; item < rows * groups; item += gridDim.y) {
+    const int r = item / groups, c = (item - r * groups) * 32 + v;
+    const bool in = c < vecs;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (in)
 #pragma unroll 4
       for (int i = b0 + k; i < b1; i += 8) {
-        const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(i) * PB_TILE + r) * tk) + v);
+        const float4 x = *(reinterpret_cast<const float4*>(p.extra + (static_cast<long long>(i) * tm + r) * tk) + c);
         s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
       }
     part[k][v] = s;
     __syncthreads();
     if (k == 0 && in) {
-      float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * PB_TILE + r) * p.ld + b.tj * tk) + v;
+      float4* dst = reinterpret_cast<float4*>(p.part + (static_cast<long long>(b.head) * p.n + b.ti * tm + r) * p.ld + b.tj * tk) + c;
       s = *dst;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -428,33 +632,34 @@ constexpr long long PART_BYTES = 256ll << 20;
 
 // How the sums of dS are taken: heads at a time (their matrices take at most 256 MB, or are one head's).
 struct SumsPlan {
-  int heads, ctas;
+  int heads, tm, tk;
+  bool pairs;
   long long ld, part, extra;      // bytes
 };
 SumsPlan plan_sums(int n_win, int n, int heads, int head_dim) {
   SumsPlan s;
-  const int tk = head_dim <= 64 ? BgCfg<1>::TK : BgCfg<2>::TK;
+  s.pairs = n > PB_TILE && head_dim > 64;      // see Bg2Cfg
+  s.tm = s.pairs ? 2 * PB_TILE : PB_TILE;
+  s.tk = s.pairs ? Bg2Cfg::TK : head_dim <= 64 ? BgCfg<1>::TK : BgCfg<2>::TK;
   s.ld = (n + 3) / 4 * 4;
-  const long long one = 4ll * n * s.ld, tiles = static_cast<long long>((n + PB_TILE - 1) / PB_TILE) * ((n + tk - 1) / tk);
+  const long long one = 4ll * n * s.ld, tiles = static_cast<long long>((n + s.tm - 1) / s.tm) * ((n + s.tk - 1) / s.tk);
   s.heads = static_cast<int>(PART_BYTES / one);
   if (s.heads < 1) s.heads = 1;
   if (s.heads > heads) s.heads = heads;
   // tiles and steps are counted in 32 bits
   while (s.heads > 1 && tiles * s.heads * n_win > 0x3fffffff) s.heads /= 2;
-  s.ctas = num_sms();
   s.part = one * s.heads;
-  s.extra = 4ll * s.ctas * PB_TILE * tk;
+  s.extra = 4ll * num_sms() * PB_TILE * s.tk;
   return s;
 }
 
 // Runs of four steps at least, for a run costs about as much to start and to join; where tiles have few windows none.
-BgPlan plan_tiles(int tiles, int n_win) {
+BgPlan plan_tiles(int tiles, int n_win, int units) {
   BgPlan p{};
   p.tiles = tiles;
   const bool split = n_win > 16;
   const long long steps = static_cast<long long>(tiles) * n_win;
-  p.ctas = split && tiles < num_sms() ? static_cast<int>((steps + 3) / 4 < num_sms() ? (steps + 3) / 4 : num_sms())
-                                      : (tiles < num_sms() ? tiles : num_sms());
+  p.ctas = split && tiles < units ? static_cast<int>((steps + 3) / 4 < units ? (steps + 3) / 4 : units) : (tiles < units ? tiles : units);
   p.rounds = tiles / p.ctas;
   const int left = tiles - p.rounds * p.ctas;
   if (split && left) {
@@ -527,12 +732,41 @@ int launch_bias_grad(const CUtensorMap (&m)[4], const BgParams& p, const BgPlan&
                cudaFuncGetAttributes(&f, bias_grad_kernel<DCH>) == cudaSuccess && f.numRegs * C::THREADS >= C::REGS;
       }))
     return -20;
-  const int r = launch_chained(bias_grad_kernel<DCH>, plan.ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, plan);
   ++kernels;
-  if (r || !plan.runs) return r;
+  return launch_chained(bias_grad_kernel<DCH>, plan.ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, plan);
+}
+// As many pairs as the device holds at once (a group of SMs with an odd number of them has one left over).
+int pairs_held() {
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> held{0};
+  using C = Bg2Cfg;
+  if (!once_a_device(done, [&] {        // see launch_bias_grad
+        cudaFuncAttributes f;
+        return cudaFuncSetAttribute(bias_grad2_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) == cudaSuccess &&
+               cudaFuncGetAttributes(&f, bias_grad2_kernel) == cudaSuccess && f.numRegs * C::THREADS >= C::REGS;
+      }))
+    return 0;
+  int pairs = held.load(std::memory_order_relaxed);
+  if (!pairs) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(num_sms() / 2 * 2);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {2, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&pairs, bias_grad2_kernel, &cfg) != cudaSuccess || pairs <= 0 || pairs > num_sms() / 2)
+      pairs = num_sms() / 2;
+    held.store(pairs, std::memory_order_relaxed);
+  }
+  return pairs;
+}
+int launch_bias_grad2(const CUtensorMap (&m)[4], const BgParams& p, const BgPlan& plan, cudaStream_t stream, int& kernels) {
+  using C = Bg2Cfg;
   ++kernels;
-  const int tiles = plan.tiles - plan.rounds * plan.ctas;
-  return launch_chained(bias_join_kernel, dim3(tiles, tiles < 32 ? PB_TILE : PB_TILE / 4), 256, 0, stream, p, plan, C::TK);
+  return launch_chained(bias_grad2_kernel, 2 * plan.ctas, C::THREADS, C::SMEM, stream, m[0], m[1], m[2], m[3], p, plan);
 }
 
 }  // namespace
@@ -621,15 +855,17 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   if (r) return r - 100;
   int count = 4;
   if (!sums) return count;
-  const int dch = a->head_dim <= 64 ? 1 : 2, tk = dch == 1 ? BgCfg<1>::TK : BgCfg<2>::TK, hd = a->heads * a->head_dim;
+  const int dch = a->head_dim <= 64 ? 1 : 2, hd = a->heads * a->head_dim;
+  const SumsPlan s = plan_sums(a->n_win, p.n, a->heads, a->head_dim);
+  const uint32_t keys = s.pairs ? 64 : s.tk;        // rows of K and V at a time
+  const int units = s.pairs ? pairs_held() : num_sms();
+  if (!units) return -20;
   const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(a->qkv);
   CUtensorMap m[4];
   const struct { const void* base; long long ld; uint32_t rows; } ops[4] = {
-      {b, a->ld_qkv, PB_TILE}, {a->d_o, a->ld_o, PB_TILE}, {b + hd, a->ld_qkv, static_cast<uint32_t>(tk)},
-      {b + 2 * hd, a->ld_qkv, static_cast<uint32_t>(tk)}};
+      {b, a->ld_qkv, PB_TILE}, {a->d_o, a->ld_o, PB_TILE}, {b + hd, a->ld_qkv, keys}, {b + 2 * hd, a->ld_qkv, keys}};
   for (int i = 0; i < 4; ++i)
     if ((r = make_tmap_heads_bf16(&m[i], ops[i].base, a->head_dim, a->heads, p.n, a->n_win, ops[i].ld, ops[i].rows))) return r - 200;
-  const SumsPlan s = plan_sums(a->n_win, p.n, a->heads, a->head_dim);
   BgParams g{};
   g.lse = a->lse; g.delta = delta; g.table = table; g.at = at; g.part = reinterpret_cast<float*>(work + w.part);
   g.extra = reinterpret_cast<float*>(work + w.extra); g.ld = s.ld;
@@ -639,8 +875,15 @@ extern "C" int aeris_biased_attn_bwd(const AerisBiasedAttn* a, void* stream_) {
   for (int h0 = 0; h0 < a->heads; h0 += s.heads) {
     g.head0 = h0;
     g.n_heads = a->heads - h0 < s.heads ? a->heads - h0 : s.heads;
-    const BgPlan plan = plan_tiles((p.n + PB_TILE - 1) / PB_TILE * ((p.n + tk - 1) / tk) * g.n_heads, a->n_win);
-    if ((r = dch == 1 ? launch_bias_grad<1>(m, g, plan, stream, count) : launch_bias_grad<2>(m, g, plan, stream, count))) return r - 300;
+    const BgPlan plan = plan_tiles((p.n + s.tm - 1) / s.tm * ((p.n + s.tk - 1) / s.tk) * g.n_heads, a->n_win, units);
+    r = s.pairs ? launch_bias_grad2(m, g, plan, stream, count)
+                : (dch == 1 ? launch_bias_grad<1>(m, g, plan, stream, count) : launch_bias_grad<2>(m, g, plan, stream, count));
+    if (r) return r - 300;
+    if (plan.runs) {
+      const int tiles = plan.tiles - plan.rounds * plan.ctas;
+      if ((r = launch_chained(bias_join_kernel, dim3(tiles, tiles < 32 ? 128 : 32), 256, 0, stream, g, plan, s.tm, s.tk))) return r - 300;
+      ++count;
+    }
     r = launch_chained(bias_sums_kernel, dim3(2 * a->high - 1, (2 * a->wide - 1 + 31) / 32, g.n_heads), 256, 0, stream,
                        static_cast<const float*>(g.part), s.ld, h0, a->high, a->wide, by_position, a->heads, a->buckets ? 0 : a->add);
     if (r) return r - 400;

@@ -7,11 +7,11 @@
 // shared memory. Backward everything comes from one pass: delta is the row sum of p dp (o is not read), dS is added up over the
 // CTA's windows in registers, and only its sums by relative position leave the CTA.
 //
-// What bounds it is latency: a CTA waits for a window, works on it and waits for the next, with others of the SM in between. us in a graph
-// against the kernels of large windows, forward / backward with the table's gradient: 2,000 windows of 4 x 4, 16 heads of 64, 56 / 136
-// (256 / 1,393; their bytes take 40 / 80); 500 of 6 x 5, 8 heads of 64, 19 / 40 (35 / 214); 1,000 of 8 x 8, 4 heads of 32, 30 / 58 (39 / 205); 1,440
-// of 17 x 4, one head of 72, 24 / 67 (31 / 176); 500 of 9 x 10, 4 heads of 64, 38 / 130 (34 / 148); 500 of 9 x 8, 4 heads of 128,
-// 56 / 190 (50 / 241). Backward, eight sixteens of queries would not have their scores, dP and sums in registers.
+// What bounds it is latency: a CTA waits for a window, works on it and waits for the next, with others of the SM in between. us in a
+// graph against the kernels of large windows, forward / backward with the table's gradient: 2,000 windows of 4 x 4, 16 heads of 64,
+// 56 / 136 (256 / 1,393; their bytes take 40 / 80); 500 of 6 x 5, 8 heads of 64, 19 / 40 (35 / 214); 1,000 of 8 x 8, 4 heads of 32,
+// 30 / 58 (39 / 205); 1,440 of 17 x 4, one head of 72, 24 / 67 (31 / 176); 500 of 9 x 10, 4 heads of 64, 38 / 130 (34 / 148); 500 of
+// 9 x 8, 4 heads of 128, 56 / 190 (50 / 241). Backward, eight sixteens of queries would not have scores, dP and sums in registers.
 #pragma once
 
 namespace aeris {
@@ -61,7 +61,8 @@ __device__ __forceinline__ float quad_max(float v) {
 template <int NT> struct SmallCfg {
   static constexpr int GROUPS = NT == 1 ? 4 : NT == 2 ? 2 : 1, THREADS = GROUPS * NT * 32, ROWS = 16 * NT;
   // CTAs on an SM, as far as registers go
-  static constexpr int HELD_FWD = NT == 1 ? 10 : NT == 2 ? 8 : NT == 3 ? 7 : NT == 4 ? 6 : NT == 5 ? 4 : 3, HELD_BWD = NT == 1 ? 7 : NT == 4 ? 3 : NT == 5 ? 2 : NT == 6 ? 1 : 5;
+  static constexpr int HELD_FWD = NT == 1 ? 10 : NT == 2 ? 8 : NT == 3 ? 7 : NT == 4 ? 6 : NT == 5 ? 4 : 3;
+  static constexpr int HELD_BWD = NT == 1 ? 7 : NT <= 3 ? 5 : NT == 4 ? 3 : NT == 5 ? 2 : 1;
   static constexpr int P_PITCH = ROWS * 2 + 16;      // odd in 16-byte units, as the operands' pitch: eight rows are in different banks
   static __host__ __device__ __forceinline__ int pitch(int d) { return (d + 15) / 16 * 32 + 16; }
   // a group's: operands of one or two windows, and backward P and dS

@@ -275,7 +275,9 @@ def test_several_heads_in_the_run_of_a_block(n_win, window, heads, d):
     run_both(*make(n_win, window, heads, d, g), n_win, window, heads, d)
 
 
-@pytest.mark.parametrize("n_win,window,heads,d", [(700, (17, 4), 1, 72), (900, (3, 20), 1, 64), (149, (8, 16), 2, 32), (40, (12, 12), 17, 64)])
+@pytest.mark.parametrize("n_win,window,heads,d", [(700, (17, 4), 1, 72), (900, (3, 20), 1, 64), (149, (8, 16), 2, 32), (40, (12, 12), 17, 64),
+                                                  (40, (10, 13), 3, 128), (90, (12, 17), 1, 96), (20, (16, 16), 9, 72), (19, (1, 257), 5, 128),
+                                                  (17, (20, 20), 33, 80)])
 def test_few_tiles_of_many_windows(n_win, window, heads, d):
     g = torch.Generator(device=DEV).manual_seed(n_win)
     run_both(*make(n_win, window, heads, d, g), n_win, window, heads, d)
