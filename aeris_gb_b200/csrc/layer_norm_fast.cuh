@@ -238,7 +238,7 @@ __device__ __forceinline__ void cluster_sums(const AerisLayerNorm& a, const floa
 
 // The warps' column sums (of each warp's first group, which has those of the others), one after the other so that the order of
 // additions is fixed, and the block's slice of `work`.
-template <typename F>
+template <bool FEW, typename F>
 __device__ __forceinline__ void join_warps(const AerisLayerNorm& a, float* joined, int lanes, F&& each) {
   const int warp = threadIdx.x >> 5;
   const bool first = static_cast<int>(threadIdx.x & 31) < lanes;
@@ -250,20 +250,17 @@ __device__ __forceinline__ void join_warps(const AerisLayerNorm& a, float* joine
       });
     __syncthreads();
   }
-  if (!a.work) {
-    if (gridDim.x > 1) return cluster_sums(a, joined);
-    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) column_sums(a, c, joined[c], joined[a.cols + c]);
-    return;
-  }
+  if constexpr (FEW) return cluster_sums(a, joined);
   float* out = a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
   for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) out[c] = joined[c];
 }
 
 // Gradients. A thread keeps its columns for all rows that it sees (NV vectors), and their sums of dy xhat and dy in registers; R
 // rows are taken at a time, so that their loads and the latencies of their sums are shared. MIN: blocks that an SM is to hold.
+// FEW: the grid is a cluster that joins its sums, in code of its own (as a branch it cost many rows 133 -> 163 us).
 // 64,800 rows of 1536, bf16: 132 us, 4.5 TB/s, and 5 for the slices' join; with two blocks an SM 153; the next rows asked for
 // a round ahead 135 (R = 2); a warp per row and its sums in 170 registers 360.
-template <typename T, int W, int NV, int R, bool BLOCK, int THREADS, int MIN>
+template <typename T, int W, int NV, int R, bool BLOCK, int THREADS, int MIN, bool FEW>
 __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNorm a, const LnCut cut) {
   __shared__ float part[BLOCK ? 64 * R : 1];
   extern __shared__ float joined[];         // [2, cols] of a cluster's CTA, and where BLOCK = false
@@ -369,17 +366,12 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNo
       }
   };
   if constexpr (BLOCK) {
-    const bool alone = !a.work && gridDim.x == 1;
-    float* out = a.work ? a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols : joined;
+    float* out = FEW ? joined : a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
     each([&](int c, float dw_, float db_) {
-      if (alone) {
-        column_sums(a, c, dw_, db_);
-      } else {
-        out[c] = dw_;
-        out[a.cols + c] = db_;
-      }
+      out[c] = dw_;
+      out[a.cols + c] = db_;
     });
-    if (!a.work && !alone) cluster_sums(a, joined);
+    if constexpr (FEW) cluster_sums(a, joined);
   } else {
     for (int o = lanes; o < 32; o <<= 1)
 #pragma unroll
@@ -389,12 +381,12 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_kernel(const AerisLayerNo
           dw[i][k] = f2_add(dw[i][k], __shfl_xor_sync(0xffffffffu, dw[i][k], o));
           db[i][k] = f2_add(db[i][k], __shfl_xor_sync(0xffffffffu, db[i][k], o));
         }
-    join_warps(a, joined, lanes, each);
+    join_warps<FEW>(a, joined, lanes, each);
   }
 }
 
 // The same element by element, for rows that start anywhere.
-template <typename T, int NV, int R, bool BLOCK, int THREADS, int MIN>
+template <typename T, int NV, int R, bool BLOCK, int THREADS, int MIN, bool FEW>
 __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLayerNorm a, const LnCut cut) {
   __shared__ float part[BLOCK ? 64 * R : 1];
   extern __shared__ float joined[];
@@ -464,17 +456,12 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLay
     }
   };
   if constexpr (BLOCK) {
-    const bool alone = !a.work && gridDim.x == 1;
-    float* out = a.work ? a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols : joined;
+    float* out = FEW ? joined : a.work + static_cast<long long>(blockIdx.x) * 2 * a.cols;
     each([&](int c, float dw_, float db_) {
-      if (alone) {
-        column_sums(a, c, dw_, db_);
-      } else {
-        out[c] = dw_;
-        out[a.cols + c] = db_;
-      }
+      out[c] = dw_;
+      out[a.cols + c] = db_;
     });
-    if (!a.work && !alone) cluster_sums(a, joined);
+    if constexpr (FEW) cluster_sums(a, joined);
   } else {
     for (int o = lanes; o < 32; o <<= 1)
 #pragma unroll
@@ -482,7 +469,7 @@ __global__ void __launch_bounds__(THREADS, MIN) ln_bwd_one_kernel(const AerisLay
         dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
         db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
       }
-    join_warps(a, joined, lanes, each);
+    join_warps<FEW>(a, joined, lanes, each);
   }
 }
 
@@ -866,12 +853,12 @@ int launch_ln_bwd(const AerisLayerNorm& a, LnCut cut, int threads, cudaStream_t 
   }
   slices = static_cast<int>(blocks);
   const int smem = sums && (!BLOCK || cluster) ? 2 * a.cols * 4 : 0;
-  const auto kernel = [] {
-    if constexpr (W > 1) return ln_bwd_kernel<T, W, NV, R, BLOCK, THREADS, MIN>;
-    else return ln_bwd_one_kernel<T, NV, R, BLOCK, THREADS, MIN>;
-  }();
-  return cluster ? launch_chained_cluster(kernel, slices, threads, smem, stream, a, cut)
-                 : launch_chained(kernel, slices, threads, smem, stream, a, cut);
+  const auto kernel = [](auto few) {
+    if constexpr (W > 1) return ln_bwd_kernel<T, W, NV, R, BLOCK, THREADS, MIN, few.value>;
+    else return ln_bwd_one_kernel<T, NV, R, BLOCK, THREADS, MIN, few.value>;
+  };
+  return cluster ? launch_chained_cluster(kernel(std::true_type{}), slices, threads, smem, stream, a, cut)
+                 : launch_chained(kernel(std::false_type{}), slices, threads, smem, stream, a, cut);
 }
 template <typename T>
 int ln_bwd_fast(const AerisLayerNorm& a, cudaStream_t stream, int& slices) {
