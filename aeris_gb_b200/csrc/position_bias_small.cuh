@@ -9,7 +9,7 @@
 //
 // What bounds it is latency: a CTA waits for a window, works on it and waits for the next, with others of the SM in between. us in a
 // graph against the kernels of large windows, forward / backward with the table's gradient: 2,000 windows of 4 x 4, 16 heads of 64,
-// 56 / 136 (256 / 1,393; their bytes take 40 / 80); 500 of 6 x 5, 8 heads of 64, 19 / 40 (35 / 214); 1,000 of 8 x 8, 4 heads of 32,
+// 56 / 98 (256 / 1,393; their bytes take 40 / 80); 500 of 6 x 5, 8 heads of 64, 19 / 40 (35 / 214); 1,000 of 8 x 8, 4 heads of 32,
 // 30 / 58 (39 / 205); 1,440 of 17 x 4, one head of 72, 24 / 67 (31 / 176); 500 of 9 x 10, 4 heads of 64, 38 / 130 (34 / 148); 500 of
 // 9 x 8, 4 heads of 128, 56 / 190 (50 / 241). Backward, eight sixteens of queries would not have scores, dP and sums in registers.
 #pragma once
@@ -78,7 +78,7 @@ template <int NT> struct SmallCfg {
     return by_memory < most ? by_memory : most;
   }
   // Two where three CTAs still fit on an SM: 2,000 windows of 4 x 4, 16 heads of 64, 68 -> 56 us forward (four CTAs for eight), but
-  // backward 136 -> 254 (two for five); 1,000 of 8 x 8, 4 heads: of 64 47 -> 36 forward (three for six), of 128 67 -> 72 (two for four).
+  // backward with two CTAs for five 1.9 times as long; 1,000 of 8 x 8, 4 heads: of 64 47 -> 36 forward (three for six), of 128 67 -> 72 (two for four).
   static int stages(int d, bool backward) { return held(d, backward, 2) >= 3 ? 2 : 1; }
 };
 
@@ -425,12 +425,13 @@ __global__ void __launch_bounds__(256) small_join_kernel(const float* part, floa
   }
 }
 
-// CTAs of a head: as many as the SMs hold of all heads, each with a window at least for every group.
+// CTAs of a head: no more than the SMs hold of all heads at once (a few more would run behind all others: 1,000 windows of 8 x 8, 8 heads
+// of 32, gradients 169 us, so 105), each with a window at least for every group.
 template <int NT>
 int small_runs(int n_win, int heads, int d, bool backward) {
   using C = SmallCfg<NT>;
-  const int want = (num_sms() * C::held(d, backward, C::stages(d, backward)) + heads - 1) / heads, need = (n_win + C::GROUPS - 1) / C::GROUPS;
-  return want < need ? want : need;
+  const int held = num_sms() * C::held(d, backward, C::stages(d, backward)) / heads, need = (n_win + C::GROUPS - 1) / C::GROUPS;
+  return held < 1 ? 1 : held < need ? held : need;
 }
 int small_runs(int n_win, int n, int heads, int d, bool backward) {
   switch ((n + 15) / 16) {

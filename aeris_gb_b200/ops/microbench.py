@@ -1,5 +1,5 @@
 """Kernel micro-benchmarks: ``python -m aeris_gb_b200.ops.microbench <gemm|attn_fwd|attn_bwd|modnorm|modnorm_bwd|qk_norm|qk_norm_bwd|
-orthogonalise|orthogonal_step|swiglu|adamw|embed|loss> ...``
+orthogonalise|orthogonal_step|layer_norm|layer_norm_bwd|linear|linear_bwd|biased_attn|biased_attn_bwd|swiglu|adamw|embed|loss> ...``
 
 Times one kernel with CUDA events (3 warm-up launches, then ``--iters`` launches, inputs larger than L2) and prints
 one JSON line with achieved TFLOP/s or GB/s and, when ``MEASURED_PEAKS.json`` is present at the repository root, the
@@ -64,7 +64,8 @@ def _time(fn, iters):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["gemm", "attn_fwd", "attn_bwd", "modnorm", "modnorm_bwd", "qk_norm", "qk_norm_bwd",
-                                       "orthogonalise", "orthogonal_step", "swiglu", "adamw",
+                                       "orthogonalise", "orthogonal_step", "layer_norm", "layer_norm_bwd", "linear", "linear_bwd",
+                                       "biased_attn", "biased_attn_bwd", "swiglu", "adamw",
                                        "embed", "loss", "fused_ag_gemm", "fused_rs_gemm", "fused_scatter_heads",
                                        "fused_grad_rs", "fused_shard_adamw", "fused_modnorm_gather"])
     ap.add_argument("--m", type=int, default=32768)
@@ -81,6 +82,9 @@ def main():
     ap.add_argument("--rows", type=int, default=129600)
     ap.add_argument("--dim", type=int, default=1536)
     ap.add_argument("--count", type=int, default=1, help="orthogonalise, orthogonal_step: matrices of --m rows and --n columns")
+    ap.add_argument("--high", type=int, default=30, help="biased_attn, biased_attn_bwd: windows of --high x --wide tokens")
+    ap.add_argument("--wide", type=int, default=30)
+    ap.add_argument("--act", default="none", help="linear, linear_bwd: activation (--m rows, --k to --n channels)")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--one-cta", action="store_true", help="force the one-CTA GEMM kernel")
     ap.add_argument("--fwd-variant", type=int, default=None,
@@ -169,6 +173,44 @@ def main():
                        a.iters)
         by = (2.0 if a.kernel == "qk_norm" else 3.0) * 2 * q.numel() * 2
         out.update(shape=[rows, H, d], ms=ms, gbs=by / ms / 1e6, frac_of_peak=by / ms / 1e6 / bw_peak, peak_source=src)
+    elif a.kernel in ("layer_norm", "layer_norm_bwd"):
+        from . import layer_norm as LN
+        x, dy = (torch.randn(a.rows, a.dim, device=dev).bfloat16() for _ in range(2))
+        w, b = torch.ones(a.dim, device=dev).bfloat16(), torch.zeros(a.dim, device=dev).bfloat16()
+        y, stats = LN.layer_norm_fwd(x, w, b, eps=1e-5)
+        if a.kernel == "layer_norm":
+            ms = _time(lambda: LN.layer_norm_fwd(x, w, b, eps=1e-5, out=y, stats=stats), a.iters)
+        else:
+            ms = _time(lambda: LN.layer_norm_bwd(dy, x, stats, w, dx=y), a.iters)
+        by = (2.0 if a.kernel == "layer_norm" else 3.0) * x.numel() * 2
+        out.update(shape=[a.rows, a.dim], ms=ms, gbs=by / ms / 1e6, frac_of_peak=by / ms / 1e6 / bw_peak, peak_source=src)
+    elif a.kernel in ("linear", "linear_bwd"):
+        from . import linear as LI
+        x, w, dy = (torch.randn(*s, device=dev).bfloat16() for s in ((a.m, a.k), (a.n, a.k), (a.m, a.n)))
+        b = torch.zeros(a.n, device=dev)
+        y, z = LI.linear_fwd(x, w, b, act=a.act, keep=a.act != "none")
+        if a.kernel == "linear":
+            ms = _time(lambda: LI.linear_fwd(x, w, b, act=a.act, out=y), a.iters)
+        else:
+            dx = torch.empty_like(x)
+            ms = _time(lambda: LI.linear_bwd(dy, x, w, z, act=a.act, dx=dx), a.iters)
+        fl = (2.0 if a.kernel == "linear" else 4.0) * a.m * a.n * a.k
+        out.update(shape=[a.m, a.n, a.k], act=a.act, ms=ms, tflops=fl / ms / 1e9, frac_of_peak=fl / ms / 1e9 / tf_peak, peak_source=src)
+    elif a.kernel in ("biased_attn", "biased_attn_bwd"):
+        from . import position_bias as PB
+        nw, win, H, d = a.windows, (a.high, a.wide), a.heads, a.head_dim
+        n = a.high * a.wide
+        qkv, d_o = (torch.randn(nw * n, k * H * d, device=dev).bfloat16() for k in (3, 1))
+        table = torch.randn(PB.relative_positions(win), H, device=dev)
+        o, lse = PB.biased_attn_fwd(qkv, nw, win, H, d, table)
+        if a.kernel == "biased_attn":
+            ms = _time(lambda: PB.biased_attn_fwd(qkv, nw, win, H, d, table, out=o, lse=lse), a.iters)
+        else:
+            g = torch.empty_like(qkv)
+            ms = _time(lambda: PB.biased_attn_bwd(d_o, qkv, o, lse, nw, win, H, d, table, dqkv=g), a.iters)
+        fl = (4.0 if a.kernel == "biased_attn" else 10.0) * nw * H * n * n * d
+        out.update(windows=nw, window=win, heads=H, head_dim=d, ms=ms, tflops=fl / ms / 1e9, frac_of_peak=fl / ms / 1e9 / tf_peak,
+                   peak_source=src)
     elif a.kernel in ("orthogonalise", "orthogonal_step"):
         from . import orthogonalise as OR
         size = a.m * a.n
