@@ -128,7 +128,8 @@ def test_weight_and_bias_may_be_missing_or_in_fp32(rows, cols, parts):
     backward_check(dy, x, stats, w, dx, dw, db)
 
 
-@pytest.mark.parametrize("rows,cols", [(65, 512), (40, 333), (77, 1536), (5, 9000), (900, 48), (2500, 640), (2400, 333)])
+@pytest.mark.parametrize("rows,cols", [(65, 512), (40, 333), (77, 1536), (5, 9000), (900, 48), (2500, 640), (2400, 333), (1300, 4999),
+                                       (1250, 3411), (300, 16001), (20, 4000), (12, 6144)])
 def test_places_that_are_given(rows, cols):
     g = torch.Generator(device=DEV).manual_seed(4)
     x, dy = (rows_of(rows, cols, torch.bfloat16, "whole", g) for _ in range(2))

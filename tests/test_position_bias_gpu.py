@@ -330,3 +330,49 @@ def test_table_gradient_against_differences():
             noise = 4 * HALF * float((do * up).square().sum().sqrt() * 2) / (2 * h)
             size = float((do.abs() * up.abs()).sum())
             assert abs(slope - float(dtable[b, head])) < noise + h * h / 16 * size / 6
+
+
+@pytest.mark.parametrize("window", [(8, 8), (10, 13)])
+def test_offsets_past_32_bits(window):
+    """Rows of one large matrix (8.6 GB) whose last ones are further than 2^32 elements from the first: the same bits as of rows that
+    are close together."""
+    n, heads, d = window[0] * window[1], 2, 24
+    n_win = 4096 // n
+    g = torch.Generator(device=DEV).manual_seed(2)
+    qkv, table, _, d_o = make(n_win, window, heads, d, g)
+    rows, inner = n_win * n, heads * d
+    wide = torch.empty((rows, (2 ** 32 // rows + 4096) // 8 * 8), device=DEV, dtype=BF)
+    assert (rows - 1) * wide.stride(0) > 2 ** 32
+    far = [wide[:, 8 + 256 * i:8 + 256 * i + k * inner] for i, k in enumerate((3, 1, 1, 3))]
+    far[0].copy_(qkv)
+    far[1].copy_(d_o)
+    want, lse = PB.biased_attn_fwd(qkv, n_win, window, heads, d, table)
+    o, again = PB.biased_attn_fwd(far[0], n_win, window, heads, d, table, out=far[2])
+    assert torch.equal(o, want) and torch.equal(again, lse)
+    grad, dtable = PB.biased_attn_bwd(d_o, qkv, want, lse, n_win, window, heads, d, table)
+    g2, dt2 = PB.biased_attn_bwd(far[1], far[0], o, lse, n_win, window, heads, d, table, dqkv=far[3])
+    assert torch.equal(g2, grad) and torch.equal(dt2, dtable)
+
+
+@pytest.mark.parametrize("window,heads,d", [((4, 4), 2, 32), ((7, 7), 3, 64), ((9, 10), 2, 24), ((12, 12), 3, 40), ((20, 20), 2, 64), ((12, 12), 2, 128)])
+def test_two_calls_at_once(window, heads, d):
+    """Other data on two streams, eight times beside one another: the bits of calls by themselves."""
+    n_win, sets = 30, []
+    for i in range(2):
+        g = torch.Generator(device=DEV).manual_seed(i)
+        sets.append(make(n_win, window, heads, d, g))
+
+    def both(qkv, table, _, d_o):
+        o, lse = PB.biased_attn_fwd(qkv, n_win, window, heads, d, table)
+        return o, lse, *PB.biased_attn_bwd(d_o, qkv, o, lse, n_win, window, heads, d, table)
+
+    want = [both(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(8):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(both(*s))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(results, want[i % 2]))
