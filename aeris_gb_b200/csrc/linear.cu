@@ -717,7 +717,11 @@ int launch_product(const void* A, long long lda, const void* B, long long ldb, c
       break;
     default: break;
   }
-  return launch_lin2<A_MN, B_MN, A_MN ? 4 : 8>(A, lda, B, ldb, p, stream);
+  // dw over few rows is its results' way out (eight epilogue warps: 64 x 1536 -> 4096 11 us, four 17), over many the ring's
+  if constexpr (A_MN) {
+    if (p.K > 16 * LIN_BK * p.k_splits) return launch_lin2<A_MN, B_MN, 4>(A, lda, B, ldb, p, stream);
+  }
+  return launch_lin2<A_MN, B_MN, 8>(A, lda, B, ldb, p, stream);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients' own passes
@@ -847,7 +851,7 @@ int launch_both(const Operand& dz, const Operand& w, const Operand& x, LinBoth& 
   int r;
   if ((r = lin_maps<0, 1>(a.dx, dz.p, dz.ld, w.p, w.ld, a.px, LIN_BM, BN))) return r;
   if ((r = lin_maps<1, 1>(a.dw, dz.p, dz.ld, x.p, x.ld, a.pw, LIN_BM, BN))) return r - 1000;
-  a.n_dx = static_cast<int>(lin_tiles(a.px.M, a.px.N, LIN_BM, BN));
+  a.n_dx = static_cast<int>(lin_tiles(a.px.M, a.px.N, LIN_BM, BN) * a.px.k_splits);
   a.n_dw = static_cast<int>(lin_tiles(a.pw.M, a.pw.N, LIN_BM, BN) * a.pw.k_splits);
   return launch_chained(lin_both_kernel<BN>, a.n_dx + a.n_dw + n_db, DZ_THREADS, S::TOTAL, stream, a);
 }
@@ -864,8 +868,8 @@ int both_width(const LinParams& px, const LinParams& pw) {
     apart += best;
   }
   for (int bn : {64, 128}) {
-    const long long tiles = lin_tiles(px.M, px.N, LIN_BM, bn) + lin_tiles(pw.M, pw.N, LIN_BM, bn) * pw.k_splits;
-    const long long cx = lin_cost(px, bn, 1), cw = lin_cost(pw, bn, pw.k_splits);
+    const long long tiles = lin_tiles(px.M, px.N, LIN_BM, bn) * px.k_splits + lin_tiles(pw.M, pw.N, LIN_BM, bn) * pw.k_splits;
+    const long long cx = lin_cost(px, bn, px.k_splits), cw = lin_cost(pw, bn, pw.k_splits);
     if (tiles <= num_sms() && (cx > cw ? cx : cw) < apart) return bn;
   }
   return 0;
@@ -992,8 +996,8 @@ __global__ void __launch_bounds__(DZ_THREADS) lin_join_sums_kernel(const float* 
   }
 }
 
-// dw from the sums of slices of the rows, in their order. `part`: [slices, rows, ld] fp32, ld a multiple of 4.
-__global__ void __launch_bounds__(DZ_THREADS) lin_join_dw_kernel(const float* part, void* dw, long long ld_dw, int f32, int vec,
+// dw or dx from the sums of slices of the reduction, in their order. `part`: [slices, rows, ld] fp32, ld a multiple of 4.
+__global__ void __launch_bounds__(DZ_THREADS) lin_join_kernel(const float* part, void* dw, long long ld_dw, int f32, int vec,
                                                                  int slices, int rows, int cols, long long ld) {
   chain_point();
   const int per_row = (cols + 3) / 4;
@@ -1029,11 +1033,11 @@ __global__ void __launch_bounds__(DZ_THREADS) lin_join_dw_kernel(const float* pa
 // Slices of the reduction over the rows of dw, of which each costs its start and its sums' way through memory as well; at most 8192
 // rows a slice, for the tensor core truncates at every addition and the error of a sum grows with its length (9e-10 of it per
 // row).
-int dw_slices(int rows, int inner, int cols) {
+int slices_of(int M, int N, int K, int least) {
   LinParams p{};
-  p.M = cols; p.N = inner; p.K = rows;
-  const int kb = (rows + LIN_BK - 1) / LIN_BK, least = (kb + 127) / 128;
-  const double sums = 8.0 * cols * inner / 3000;      // cycles to write and read one slice's, 3 KB a cycle
+  p.M = M; p.N = N; p.K = K;
+  const int kb = (K + LIN_BK - 1) / LIN_BK;
+  const double sums = 8.0 * M * N / 3000;      // cycles to write and read one slice's, 3 KB a cycle
   int best = least;
   double cost = 1e30;
   for (int s = least; s <= 64 && (s == least || kb / s >= 4); ++s)
@@ -1043,6 +1047,10 @@ int dw_slices(int rows, int inner, int cols) {
     }
   return best;
 }
+int dw_slices(int rows, int inner, int cols) { return slices_of(cols, inner, rows, (rows + 128 * LIN_BK - 1) / (128 * LIN_BK)); }
+// Slices of the columns for dx, whose tiles are few where rows are: product and join of 64 x 1536 -> 4096 8 us for 14, of 5 x 2048 -> 4096
+// 11 for 19. With the epilogue warps above both gradients take 19.0 us in a graph for 26.7, and 22.2 for 28.4.
+int dx_slices(int rows, int inner, int cols) { return slices_of(rows, inner, cols, 1); }
 
 }  // namespace
 
@@ -1094,10 +1102,8 @@ int db_slices(int rows, int cols) {
   const long long most = 16ll * num_sms() * DZ_COLS / cols + 1, need = (rows + 31ll) / 32;
   return static_cast<int>(most < need ? (most < 4096 ? most : 4096) : (need < 4096 ? need : 4096));
 }
-long long dw_bytes(int rows, int inner, int cols, bool f32) {
-  const int s = dw_slices(rows, inner, cols);
-  return s > 1 || f32 ? 4ll * s * cols * ((inner + 3) / 4 * 4) : 0;
-}
+// fp32 sums of s slices; one slice of bf16 results goes straight to its place.
+long long part_bytes(int s, int rows, int inner, bool f32) { return s > 1 || f32 ? up(4ll * s * rows * ((inner + 3) / 4 * 4)) : 0; }
 
 }  // namespace
 
@@ -1150,16 +1156,26 @@ extern "C" int aeris_linear_fwd(const AerisLinear* a, void* stream_) {
   return r ? r : n;
 }
 
+namespace {
+
+// sx, sw: slices of dx's and dw's sums, 0 where it is not wanted.
+long long bwd_bytes(int rows, int inner, int cols, bool own_dz, bool pad_x, bool pad_w, int sx, int sw, bool db, bool dw_f32) {
+  const int slices = db ? db_slices(rows, cols) : 1;
+  long long n = slices > 1 ? up(4ll * slices * cols) : 0;
+  if (own_dz && (sx || sw)) n += up(2 * padded(cols) * rows);
+  if (sx) n += (pad_w ? up(2 * padded(inner) * cols) : 0) + part_bytes(sx, rows, inner, false);
+  if (sw) n += (pad_x ? up(2 * padded(inner) * rows) : 0) + part_bytes(sw, cols, inner, dw_f32);
+  return n;
+}
+
+}  // namespace
+
 extern "C" long long aeris_linear_bwd_bytes(int rows, int inner, int cols, int own_dz, int pad_x, int pad_w, int dx, int dw, int db,
                                             int dw_f32) {
   if (rows <= 0 || inner <= 0 || cols <= 0) return -1;
   if (small_bwd(rows, inner, cols)) return 0;
-  const int slices = db_slices(rows, cols);
-  long long n = db && slices > 1 ? up(4ll * slices * cols) : 0;
-  if (own_dz && (dx || dw)) n += up(2 * padded(cols) * rows);
-  if (dx && pad_w) n += up(2 * padded(inner) * cols);
-  if (dw) n += (pad_x ? up(2 * padded(inner) * rows) : 0) + up(dw_bytes(rows, inner, cols, dw_f32));
-  return n;
+  return bwd_bytes(rows, inner, cols, own_dz, pad_x, pad_w, dx ? dx_slices(rows, inner, cols) : 0, dw ? dw_slices(rows, inner, cols) : 0, db,
+                   dw_f32);
 }
 
 extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
@@ -1168,9 +1184,6 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   if (rows <= 0 || inner <= 0 || cols <= 0 || !a->dy || a->act < 0 || a->act > LIN_ACT_GELU_TANH) return -1;
   if ((a->act != LIN_ACT_NONE) != (a->z != nullptr)) return -1;
   const bool products = a->dx || a->dw, own_dz = products && (a->z || !tiled(a->dy, a->ld_dy, rows, cols));
-  if (a->work_bytes < aeris_linear_bwd_bytes(rows, inner, cols, own_dz, !tiled(a->x, a->ld_x, rows, inner), !tiled(a->w, a->ld_w, cols, inner),
-                                             a->dx != nullptr, a->dw != nullptr, a->db != nullptr, a->dw_f32))
-    return -2;
   int n = 0, r;
   if (small_bwd(rows, inner, cols)) {
     const long long results = (a->dx ? static_cast<long long>(rows) * inner : 0) + (a->dw ? static_cast<long long>(cols) * inner : 0) + cols;
@@ -1178,16 +1191,22 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
     r = launch_chained(lin_small_bwd_kernel, blocks_for(results * g), DZ_THREADS, 0, stream, *a, g);
     return r ? r : 1;
   }
+  const int sx = a->dx ? dx_slices(rows, inner, cols) : 0, sw = a->dw ? dw_slices(rows, inner, cols) : 0;
+  if (a->work_bytes < bwd_bytes(rows, inner, cols, own_dz, !tiled(a->x, a->ld_x, rows, inner), !tiled(a->w, a->ld_w, cols, inner), sx, sw,
+                                a->db != nullptr, a->dw_f32))
+    return -2;
   uint8_t* work = static_cast<uint8_t*>(a->work);
   long long at = 0;
   Operand dz{a->dy, pitch(a->ld_dy, rows, cols)};
   // [rows, inner] = dz [rows, cols] w [cols, inner], [cols, inner] = dz^T x
   LinBoth both{};
   LinParams &px = both.px, &pw = both.pw;
-  px.M = rows; px.N = inner; px.K = cols; px.mode = LIN_OUT; px.k_splits = 1; px.status = a->status;
+  px.M = rows; px.N = inner; px.K = cols; px.status = a->status;
+  px.k_splits = sx;
+  px.mode = px.k_splits > 1 ? LIN_PART : LIN_OUT;
   px.C = static_cast<__nv_bfloat16*>(a->dx); px.ldc = pitch(a->ld_dx, rows, inner);
   pw.M = cols; pw.N = inner; pw.K = rows; pw.status = a->status;
-  pw.k_splits = a->dw ? dw_slices(rows, inner, cols) : 1;
+  pw.k_splits = sw;
   const bool direct = pw.k_splits == 1 && !a->dw_f32;
   pw.mode = direct ? LIN_OUT : LIN_PART;
   const int slices = db_slices(rows, cols), width = a->dx && a->dw ? both_width(px, pw) : 0;
@@ -1225,11 +1244,20 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
   if (a->dx) w = operands.add(a->w, a->ld_w, cols, inner);
   if (a->dw) x = operands.add(a->x, a->ld_x, rows, inner);
   if ((r = operands.launch(n, stream))) return r;
+  px.ld_part = pw.ld_part = (inner + 3) / 4 * 4;
+  px.part = reinterpret_cast<float*>(work + operands.at);
+  operands.at += part_bytes(sx, rows, inner, false);
   if (direct) {
     pw.C = static_cast<__nv_bfloat16*>(a->dw); pw.ldc = pitch(a->ld_dw, cols, inner);
   } else {
-    pw.part = reinterpret_cast<float*>(work + operands.at); pw.ld_part = (inner + 3) / 4 * 4;
+    pw.part = reinterpret_cast<float*>(work + operands.at);
   }
+  auto join = [&](const LinParams& p, void* out, long long ld, int f32, int size) {
+    const int vec = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && ld % 4 == 0;
+    ++n;
+    return launch_chained(lin_join_kernel, blocks_for(static_cast<long long>(size) * ((inner + 3) / 4)), DZ_THREADS, 0, stream,
+                          static_cast<const float*>(p.part), out, ld, f32, vec, p.k_splits, size, inner, p.ld_part);
+  };
   if (width) {
     const int n_db = db_beside ? static_cast<int>(dz_grid.x) : 0;
     if ((r = width == 64 ? launch_both<64>(dz, w, x, both, n_db, stream) : launch_both<128>(dz, w, x, both, n_db, stream))) return r;
@@ -1239,13 +1267,12 @@ extern "C" int aeris_linear_bwd(const AerisLinearGrad* a, void* stream_) {
       if ((r = launch_product<0, 1>(dz.p, dz.ld, w.p, w.ld, px, stream))) return r;
       ++n;
     }
-    if (!a->dw) return n;
-    if ((r = launch_product<1, 1>(dz.p, dz.ld, x.p, x.ld, pw, stream))) return r - 1000;
-    ++n;
+    if (a->dw) {
+      if ((r = launch_product<1, 1>(dz.p, dz.ld, x.p, x.ld, pw, stream))) return r - 1000;
+      ++n;
+    }
   }
-  if (direct) return n;
-  const int vec = (reinterpret_cast<uintptr_t>(a->dw) & 7) == 0 && a->ld_dw % 4 == 0;
-  r = launch_chained(lin_join_dw_kernel, blocks_for(static_cast<long long>(cols) * ((inner + 3) / 4)), DZ_THREADS, 0, stream,
-                     static_cast<const float*>(pw.part), a->dw, a->ld_dw, a->dw_f32, vec, pw.k_splits, cols, inner, pw.ld_part);
-  return r ? r - 2000 : n + 1;
+  if (px.k_splits > 1 && (r = join(px, a->dx, px.ldc, 0, rows))) return r - 2000;
+  if (a->dw && !direct && (r = join(pw, a->dw, a->ld_dw, a->dw_f32, cols))) return r - 2000;
+  return n;
 }
