@@ -531,9 +531,6 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_long_kernel(const AerisLayerNo
 // 19,366 x 3,411 bf16 88 and 123 (222 and 224), 50,000 x 1,001 bf16 78 and 99 (128 and 157), 20,000 x 333 fp32 17 and 23 (26 and 26),
 // 1,200 x 1,001 bf16 5.3 and 6.2 (6.2 and 7.7).
 struct OddRing {
-  uint64_t* bars;
-  uint8_t* mem;
-  int stages, bytes;            // bytes of a row's place
   static __device__ __forceinline__ uint32_t granules(const void* row, int size) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(row);
     return static_cast<uint32_t>(((at + size + 15) & ~uintptr_t(15)) - (at & ~uintptr_t(15)));
@@ -543,7 +540,8 @@ struct OddRing {
   }
 };
 // A wait gave up: the rounds that were asked for from (st, ph) on are let in (bounded) before the block's memory is another's.
-__device__ __forceinline__ void odd_drain(uint64_t* bars, int stages, int st, uint32_t ph, long long r0, long long step, const AerisLayerNorm& a) {
+__device__ __forceinline__ void odd_drain(uint64_t* bars, int stages, int st, uint32_t ph, long long r0, long long step,
+                                          const AerisLayerNorm& a) {
   for (int i = 0; i < stages && r0 < a.rows; ++i, r0 += step) {
     if (threadIdx.x < 32) mbar_wait_warp(bars + st, ph, a.status, ERR_TIMEOUT_FULL);
     if (++st == stages) { st = 0; ph ^= 1; }
@@ -554,7 +552,7 @@ template <int K>
 __device__ __forceinline__ bool odd_sums(float (&v)[K], bool ok, float* part) {
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-  // everyone has taken the words of the sums before, and its elements of this round's rows
+  // everyone has taken the words of the sums before, and its elements of these rows
   if (!__syncthreads_and(ok)) return false;
   if ((threadIdx.x & 31) == 0)
 #pragma unroll
@@ -741,15 +739,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) ln_bwd_odd_kernel(const AerisLa
   }
 }
 
-// `slices`: null forward; backward it receives how many slices of column sums were written. Returns 1 where the ring would have one
-// stage alone.
+// `slices`: null forward; backward it receives how many slices of column sums were written.
 template <typename T, int NV, int RF, int RB, int TH>
 int launch_ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
   constexpr int PER_SM = 1024 / TH;
   const int R = slices ? RB : RF;
   const int bytes = (a.cols * static_cast<int>(sizeof(T)) + 30) / 16 * 16, row = slices ? 2 * bytes : bytes;
-  int stages = (200 * 1024 / PER_SM - 1024) / (R * row);
-  if (stages < 2) return 1;
+  int stages = (200 * 1024 / PER_SM - 1024) / (R * row);        // three at least
   if (stages > 6) stages = 6;
   const long long need = (a.rows + R - 1) / R;
   long long blocks = static_cast<long long>(num_sms()) * PER_SM;
@@ -766,18 +762,16 @@ int launch_ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
   if (!allow_smem_once(ln_fwd_odd_kernel<T, NV, RF, TH>, 200 * 1024, done)) return -20;
   return launch_chained(ln_fwd_odd_kernel<T, NV, RF, TH>, static_cast<unsigned>(blocks), TH, smem, stream, a, stages, bytes);
 }
-// Where rows are many enough for rounds that follow one another; others, and the widest, go straight from memory.
+// Where rows are many enough for rounds that follow one another; others, and the widest, go straight from memory (returns 1).
 template <typename T>
 int ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
   if (a.rows < 8 * num_sms() || a.cols <= 96 || a.cols > 8192) return 1;
-  int r = 1;
-  if (a.cols <= 256) r = launch_ln_odd<T, 4, 4, 2, 64>(a, stream, slices);
-  else if (a.cols <= 512) r = launch_ln_odd<T, 4, 4, 2, 128>(a, stream, slices);
-  else if (a.cols <= 1024) r = launch_ln_odd<T, 4, 4, 2, 256>(a, stream, slices);
-  else if (a.cols <= 2048) r = launch_ln_odd<T, 4, 4, 2, 512>(a, stream, slices);
-  else if (a.cols <= 4096) r = launch_ln_odd<T, 8, 2, 1, 512>(a, stream, slices);
-  if (r == 1 && a.cols > 2048) r = a.cols <= 4096 ? launch_ln_odd<T, 8, 1, 1, 512>(a, stream, slices) : launch_ln_odd<T, 8, 1, 1, 1024>(a, stream, slices);
-  return r;
+  if (a.cols <= 256) return launch_ln_odd<T, 4, 4, 2, 64>(a, stream, slices);
+  if (a.cols <= 512) return launch_ln_odd<T, 4, 4, 2, 128>(a, stream, slices);
+  if (a.cols <= 1024) return launch_ln_odd<T, 4, 4, 2, 256>(a, stream, slices);
+  if (a.cols <= 2048) return launch_ln_odd<T, 4, 4, 2, 512>(a, stream, slices);
+  if (a.cols <= 4096) return launch_ln_odd<T, 8, 2, 1, 512>(a, stream, slices);
+  return launch_ln_odd<T, 8, 1, 1, 1024>(a, stream, slices);
 }
 
 bool ln_aligned(const void* p, long long ld, int size) {

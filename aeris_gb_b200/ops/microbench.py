@@ -1,5 +1,6 @@
 """Kernel micro-benchmarks: ``python -m aeris_gb_b200.ops.microbench <gemm|attn_fwd|attn_bwd|modnorm|modnorm_bwd|qk_norm|qk_norm_bwd|
-orthogonalise|orthogonal_step|layer_norm|layer_norm_bwd|linear|linear_bwd|biased_attn|biased_attn_bwd|swiglu|adamw|embed|loss> ...``
+orthogonalise|orthogonal_step|layer_norm|layer_norm_bwd|linear|linear_bwd|biased_attn|biased_attn_bwd|
+swiglu|adamw|embed|loss> ...``
 
 Times one kernel with CUDA events (3 warm-up launches, then ``--iters`` launches, inputs larger than L2) and prints
 one JSON line with achieved TFLOP/s or GB/s and, when ``MEASURED_PEAKS.json`` is present at the repository root, the
