@@ -21,7 +21,8 @@ constexpr int ATT_THREADS = 192;
 constexpr int TILE = 128;
 
 // Bias of the scores by relative position: that of query i and key j of head h is table[h * size + zero + at[i] - at[j]], in log2
-// units (position_bias.cu, which lays it out so that 32 queries next to one another are in 32 banks of shared memory); `size` is a multiple of 4. -infinity hides the pair. `at` goes on to the next multiple of 128 behind the window's end.
+// units (position_bias.cu, which lays it out so that 32 queries next to one another are in 32 banks of shared memory); `size` is a
+// multiple of 4. -infinity hides the pair. `at` goes on to the next multiple of 128 behind the window's end.
 struct PairBias {
   const float* table;
   const int* at;
