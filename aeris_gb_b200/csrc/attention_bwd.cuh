@@ -798,13 +798,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
       }
     } else {
       const uint64_t nsl = f2_pack(-p.scale_log2, -p.scale_log2);
-      // Columns past the window's end have zero Q and dO rows and zero statistics (P = 1, dS = 0): they add nothing. Rows
-      // past its end may hold anything: they are not stored.
-      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l, [[maybe_unused]] int a0, [[maybe_unused]] int a1) -> uint32_t {
+      // Columns past the window's end have zero Q and dO rows and zero statistics: without a bias P = 1 and dS = 0 there, which
+      // adds nothing. A bias would make P = 2^bias of it, and infinity times the zero rows NaN: the last tile then has P = 0 from
+      // column `in` of the pair on. Rows past the window's end may hold anything: they are not stored.
+      auto probs = [&](uint32_t& s0, uint32_t& s1, uint64_t l, [[maybe_unused]] int a0, [[maybe_unused]] int a1,
+                       [[maybe_unused]] int in = 2) -> uint32_t {
         float t0, t1;
         uint64_t x = f2_fma(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), nsl, l);             // -(log2 P)
         if constexpr (BIAS) x = f2_sub(x, f2_pack(tab[mine + a0], tab[mine + a1]));
         f2_unpack(x, t0, t1);
+        if constexpr (BIAS) {
+          if (in < 1) t0 = INFINITY;
+          if (in < 2) t1 = INFINITY;
+        }
         t0 = fast_exp2(-t0);
         t1 = fast_exp2(-t1);
         s0 = __float_as_uint(t0);
@@ -869,8 +875,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_i0, const __grid_constant
                 const ulonglong2 l = ls[c / 4 + i], de = ds[c / 4 + i];
                 int4 a = {};
                 if constexpr (BIAS) a = *reinterpret_cast<const int4*>(at + j * BT + c0 + c + 4 * i);
-                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x, a.x, a.y);
-                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y, a.z, a.w);
+                const int in = rem - (c0 + c + 4 * i);
+                pp[2 * i] = probs(sv[4 * i], sv[4 * i + 1], l.x, a.x, a.y, in);
+                pp[2 * i + 1] = probs(sv[4 * i + 2], sv[4 * i + 3], l.y, a.z, a.w, in - 2);
                 dd[2 * i] = grad(sv[4 * i], sv[4 * i + 1], dv[4 * i], dv[4 * i + 1], de.x);
                 dd[2 * i + 1] = grad(sv[4 * i + 2], sv[4 * i + 3], dv[4 * i + 2], dv[4 * i + 3], de.y);
               }

@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(256) bias_expand_kernel(const BiasSource s, fl
 // written to its place, what goes on in the next CTA's to `extra`, which bias_join_kernel adds.
 //
 // With p = 2^(c s + b - lse) the bias b of a pair is the same for all windows: 2^(c s - lse) (dp - delta) is added up and the sum
-// multiplied by 2^b at the end, where every pair of a warp's is visible and |b| is at most 64; else b is added to every score.
+// multiplied by 2^b at the end, where every pair of a warp's is visible and |b| is at most 64 (a probability below 2^-62 may then be
+// taken for zero); else b is added to every score.
 //
 // What bounds it is the operands' way from L2, 64 KB a window: loads and products alone take 0.62 of the 0.75 ms (72 windows of 30 x 30, 24
 // heads of 64), 11 TB/s; the exponentials of a window take 1,024 cycles. Tiles of 128 x 256 read 48 KB for 128 x 128, but two
