@@ -245,7 +245,7 @@ typedef struct AerisLayerNorm {
   const void *x, *dy;
   void* y;
   const void *w, *b;                // [cols], bf16 or fp32 both; null: ones, zeros
-  float *stats;                     // [rows, 2]
+  float *stats;                     // [rows, 2], from an 8-byte boundary on
   float *dw, *db, *work;            // [cols] each, null: not wanted; work: [slices, 2, cols]
   int* status;
   long long rows, ld_x, ld_dy, ld_y;

@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(1024) ln_join_kernel(const AerisLayerNorm a, i
 }
 
 bool ln_fits(const AerisLayerNorm* a) {
-  return a->rows > 0 && a->rows <= 0x7fffffff && a->cols > 0 && a->x && a->y && a->stats && a->ld_x >= 0 && a->ld_y >= a->cols;
+  return a->rows > 0 && a->rows <= 0x7fffffff && a->cols > 0 && a->x && a->y && a->stats && a->ld_x >= 0 && a->ld_y >= a->cols &&
+         (reinterpret_cast<uintptr_t>(a->stats) & 7) == 0;       // read and written as float2
 }
 
 }  // namespace

@@ -93,14 +93,14 @@ def _result(t, shape, dt, index, what: str, *inputs) -> int:
 def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, eps: float,
                    out: torch.Tensor | None = None, stats: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``x`` [rows, cols] bf16 or fp32, rows of any pitch (a section of a wider matrix). Returns (normed rows in x's type, fp32
-    [rows, 2]: mean and 1 / sqrt(var + eps) of every row, which :func:`layer_norm_bwd` takes). ``weight``, ``bias`` [cols] bf16 or
+    [rows, 2]: mean and 1 / sqrt(var + eps) of every row, which :func:`layer_norm_bwd` takes; from an 8-byte boundary on). ``weight``, ``bias`` [cols] bf16 or
     fp32, each may be missing. ``out`` may be ``x`` itself."""
     rows, cols, pitch, dt, index = _check(x, weight, bias)
     if out is not None:
         pitch_out = _result(out, x.shape, dt, index, "out", x, weight, bias)
     if stats is not None:
         if not _stats(stats, rows, index):
-            raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {x.device}, got {_text(stats)}")
+            raise ValueError(f"stats: contiguous fp32 [{rows}, 2] from an 8-byte boundary on, on {x.device}, got {_text(stats)}")
         if any(t is not None and _l.share_memory(stats, t) for t in (x, weight, bias, out)):
             raise ValueError("stats lie over another tensor of the call")
     _l.require_cuda(x)
@@ -117,7 +117,9 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
 
 
 def _stats(t, rows: int, index: int) -> bool:
-    return t.shape == (rows, 2) and t.dtype is torch.float32 and t.get_device() == index and t.is_contiguous()
+    """Mean and reciprocal deviation of a row are read and written as one: from an 8-byte boundary on."""
+    return (t.shape == (rows, 2) and t.dtype is torch.float32 and t.get_device() == index and t.is_contiguous()
+            and t.data_ptr() % 8 == 0)
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: torch.Tensor | None = None, *,
@@ -131,7 +133,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
     shape = x.shape
     pitch_dy = _like(dy, shape, dt, index, "dy")
     if not _stats(stats, rows, index):
-        raise ValueError(f"stats: contiguous fp32 [{rows}, 2] on {x.device}, got {_text(stats)}")
+        raise ValueError(f"stats: contiguous fp32 [{rows}, 2] from an 8-byte boundary on, on {x.device}, got {_text(stats)}")
     add = dw is not None or db is not None
     if add:
         if weight is None and dw is not None or not bias and db is not None:

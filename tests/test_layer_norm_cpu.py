@@ -85,3 +85,16 @@ def test_slices_cover_the_rows_and_the_machine():
     for rows, cols in ((1, 1), (5, 20000), (64800, 1536), (2 ** 31 - 1, 1)):
         s = LN.slices_for(rows, cols, 148)
         assert s <= 65535 and (s == 1) == (rows * cols <= 2 ** 14 and cols <= 4096)
+
+
+@pytest.mark.parametrize("start", [1, 3])
+def test_statistics_between_8_byte_boundaries_are_refused(start):
+    flat = torch.zeros(2 * ROWS + 4)
+    stats = flat[start:start + 2 * ROWS].view(ROWS, 2)
+    assert stats.is_contiguous() and stats.data_ptr() % 8 == 4
+    with pytest.raises(ValueError, match="8-byte"):
+        LN.layer_norm_fwd(mat(), eps=1e-5, stats=stats)
+    with pytest.raises(ValueError, match="8-byte"):
+        LN.layer_norm_bwd(mat(), mat(), stats)
+    with pytest.raises(ValueError, match="GPU"):          # two further on: taken
+        LN.layer_norm_bwd(mat(), mat(), flat[2:2 + 2 * ROWS].view(ROWS, 2))
