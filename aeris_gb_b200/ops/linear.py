@@ -61,12 +61,14 @@ def _matrix(t, shape, index: int, what: str, dtype=_BF16) -> int:
 
 
 def _result(t, shape, index: int, what: str, *others, dtype=_BF16, inside=None) -> int:
-    """``inside``: the one input that the result may take the place of, element by element."""
+    """``inside``: the one input that the result may take the place of, element by element (where it is none of ``others``, too)."""
     pitch = _matrix(t, shape, index, what, dtype)
     if shape[0] > 1 and pitch < shape[1]:
         raise ValueError(f"{what}: rows lie over one another, got {_text(t)}")
+    if inside is not None and not _l.same_memory(t, inside):
+        others += inside,
     for o in others:
-        if o is not None and _l.share_memory(t, o) and not (o is inside and _l.same_memory(t, o)):
+        if o is not None and _l.share_memory(t, o):
             raise ValueError(f"{what} lies over another tensor of the call: {_text(t)}, {_text(o)}")
     return pitch
 
@@ -101,7 +103,7 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     """``resid + act(x @ w^T + bias)`` for ``x`` [rows, inner] and ``w`` [cols, inner], bf16; ``bias`` [cols] fp32 or bf16 and
     ``resid`` [rows, cols] bf16 may be missing. ``act``: one of :data:`ACTIVATIONS` ("gelu" by the error function, "gelu_tanh" by
     the hyperbolic tangent). Returns (the result, and with ``keep`` the values before the activation, bias included, which
-    :func:`linear_bwd` takes: else None). ``out``, ``z``: where to put them; ``out`` may be ``resid`` itself.
+    :func:`linear_bwd` takes: else None). ``out``, ``z``: where to put them; ``out`` may be ``resid`` itself, where that is neither ``x`` nor ``w``.
 
     Any sizes and pitches. Rows that start on 16-byte boundaries are fastest: others of ``x`` and ``w`` are copied first, others of
     the results are written element by element."""
@@ -115,7 +117,7 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
         raise ValueError("z is written with keep=True")
     y_pitch = z_pitch = cols
     if out is not None:
-        y_pitch = _result(out, shape, index, "out", x, w, bias, resid, z, inside=resid)
+        y_pitch = _result(out, shape, index, "out", x, w, bias, z, inside=resid)
     if z is not None:
         z_pitch = _result(z, shape, index, "z", x, w, bias, resid)
     _l.require_cuda(x)

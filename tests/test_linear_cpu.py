@@ -91,3 +91,21 @@ def test_cpu_tensors_are_refused_and_not_computed_elsewhere():
     with pytest.raises(ValueError, match="GPU"):
         backward()
 
+
+
+def test_a_result_over_an_operand_is_refused_where_that_is_the_residual_too():
+    """Rows of x are read by blocks that make other columns of the result."""
+    square, w = mat(INNER, INNER), mat(INNER, INNER)
+    with pytest.raises(ValueError, match="lies over"):
+        forward(x=square, w=w, resid=square, out=square)
+    with pytest.raises(ValueError, match="lies over"):
+        forward(x=square, w=w, resid=square, out=square[:])
+    with pytest.raises(ValueError, match="lies over"):
+        forward(x=square, w=w, resid=w, out=w)
+    with pytest.raises(ValueError, match="lies over"):
+        forward(x=square, w=w, keep=True, resid=square, z=square)
+    with pytest.raises(ValueError, match="GPU"):          # a residual of its own
+        other = mat(INNER, INNER)
+        forward(x=square, w=w, resid=other, out=other)
+    with pytest.raises(ValueError, match="GPU"):          # x is the residual, the result lies elsewhere
+        forward(x=square, w=w, resid=square, out=mat(INNER, INNER))
