@@ -351,7 +351,9 @@ bias_grad2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank()), pair = blockIdx.x >> 1;
+  __shared__ int s_abort;       // an earlier kernel has failed: the pair leaves, as its leader says
   if (threadIdx.x == 0) {
+    s_abort = failed(p.status) ? 1 : 0;
     prefetch_tmap(&tm_q); prefetch_tmap(&tm_do); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v);
     for (int i = 0; i < NST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 2 * C::MATH); }
@@ -363,10 +365,13 @@ bias_grad2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   cluster_sync_all();       // both CTAs' barriers are initialised and tensor memory is allocated before anyone signals
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  const bool gone = ld_shared_cluster_u32(map_to_cta(smem_u32(&s_abort), 0)) != 0;
   chain_point();
 
-  if (warp >= C::MATH) regs_dec<C::REGS_REST>();
-  if (warp == C::W_LOAD) {
+  if (!gone && warp >= C::MATH) regs_dec<C::REGS_REST>();
+  if (gone) {
+    // nothing is under way
+  } else if (warp == C::W_LOAD) {
     if (elect_one_sync()) {
       int st = 0;
       uint32_t ph = 0;

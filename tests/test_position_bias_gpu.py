@@ -376,3 +376,30 @@ def test_two_calls_at_once(window, heads, d):
     torch.cuda.synchronize()
     for i, results in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(results, want[i % 2]))
+
+
+@pytest.mark.parametrize("n_win,window,heads,d", [(2, (5, 6), 2, 32), (2, (9, 13), 2, 64), (2, (12, 16), 3, 64), (3, (10, 16), 2, 128), (1, (20, 20), 5, 72)])
+def test_bucket_outside_the_table_ends_every_kernel_of_the_call(n_win, window, heads, d):
+    """Recorded in both directions, and soon: no kernel of the backward pass waits for what another has left undone (limits of
+    waits are 2 s). Later calls are as before."""
+    from aeris_gb_b200.ops import lib as _l
+    g = torch.Generator(device=DEV).manual_seed(6)
+    qkv, table, buckets, d_o = make(n_win, window, heads, d, g, 5)
+
+    def both(b):
+        o, lse = PB.biased_attn_fwd(qkv, n_win, window, heads, d, table, b)
+        return o, lse, *PB.biased_attn_bwd(d_o, qkv, o, lse, n_win, window, heads, d, table, b)
+
+    want = both(buckets)
+    bad = buckets.clone()
+    bad[7] = 5
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    for call in (lambda: PB.biased_attn_fwd(qkv, n_win, window, heads, d, table, bad),
+                 lambda: PB.biased_attn_bwd(d_o, qkv, want[0], want[1], n_win, window, heads, d, table, bad)):
+        start.record()
+        call()
+        end.record()
+        with pytest.raises(_l.KernelError, match="bounds"):
+            _l.check_status()
+        assert start.elapsed_time(end) < 1000
+    assert all(map(torch.equal, both(buckets), want))
