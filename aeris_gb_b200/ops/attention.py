@@ -41,8 +41,9 @@ def _pad_heads(t: torch.Tensor, parts: int, H: int, d: int, dp: int) -> torch.Te
 
 
 def _unpad_heads(t: torch.Tensor, parts: int, H: int, d: int, dp: int) -> torch.Tensor:
+    """Rows without the padding, one behind the other (of one channel, or one head in one part, a reshape alone would be a view)."""
     T = t.shape[0]
-    return t.view(T, parts, H, dp)[..., :d].reshape(T, parts * H * d)
+    return t.view(T, parts, H, dp)[..., :d].reshape(T, parts * H * d).contiguous()
 
 
 def attn_fwd(qkv: torch.Tensor, n_win: int, N: int, H: int, d: int, *, out: torch.Tensor | None = None,

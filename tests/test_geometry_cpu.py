@@ -105,3 +105,11 @@ def test_separable_position_tables_rebuild_the_full_encoding():
     ch = ty.shape[1]
     both = torch.cat([ty.unsqueeze(1).expand(H, W, ch), tx.unsqueeze(0).expand(H, W, ch)], dim=-1)[..., :C]
     assert torch.allclose(full, both)
+
+
+def test_heads_without_their_padding_lie_in_rows():
+    """Of one channel, or one head, a reshape alone leaves the padding between them: what the backward passes do not take."""
+    for parts, H, d, dp in ((1, 5, 1, 8), (3, 2, 1, 8), (1, 1, 20, 64), (3, 1, 20, 64), (1, 1, 1, 8), (1, 4, 12, 16)):
+        t = torch.randn(6, parts * H * d)
+        back = A._unpad_heads(A._pad_heads(t, parts, H, d, dp), parts, H, d, dp)
+        assert torch.equal(back, t) and back.stride() == t.stride()

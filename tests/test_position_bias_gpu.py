@@ -403,3 +403,24 @@ def test_bucket_outside_the_table_ends_every_kernel_of_the_call(n_win, window, h
             _l.check_status()
         assert start.elapsed_time(end) < 1000
     assert all(map(torch.equal, both(buckets), want))
+
+
+@pytest.mark.parametrize("window", [(3, 5), (10, 11)])
+@pytest.mark.parametrize("heads,d", [(5, 1), (1, 1), (1, 5), (1, 20), (2, 7)])
+def test_results_of_padded_heads_go_on_into_the_backward_pass(heads, d, window):
+    g = torch.Generator(device=DEV).manual_seed(heads + d)
+    o, _, dqkv, _ = run_both(*make(3, window, heads, d, g), 3, window, heads, d)
+    assert o.is_contiguous() and dqkv.is_contiguous()
+
+
+@pytest.mark.parametrize("heads,d", [(1, 20), (3, 1), (1, 1), (2, 20)])
+def test_plain_attention_of_padded_heads_goes_on_into_its_backward_pass(heads, d):
+    """The same by the kernels without a bias, whose backward pass takes o and its gradient in rows of one pitch."""
+    g = torch.Generator(device=DEV).manual_seed(heads + d)
+    n_win, window = 3, (10, 13)
+    qkv, table, _, d_o = make(n_win, window, heads, d, g)
+    o, lse = A.attn_fwd(qkv, n_win, 130, heads, d)
+    dqkv = A.attn_bwd(qkv, o, d_o, lse, n_win, 130, heads, d)
+    f = formula(qkv, window, heads, d, 0 * table, None, 1 / math.sqrt(d))
+    forward_check(o, lse, f)
+    backward_check(d_o, o, dqkv, None, f, window, heads, d, 1 / math.sqrt(d), len(table))
