@@ -106,7 +106,7 @@ def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     :func:`linear_bwd` takes: else None). ``out``, ``z``: where to put them; ``out`` may be ``resid`` itself, where that is neither ``x`` nor ``w``.
 
     Any sizes and pitches. Rows that start on 16-byte boundaries are fastest: others of ``x`` and ``w`` are copied first, others of
-    the results are written element by element."""
+    the results, and those of columns that are no multiple of 8, are written element by element."""
     rows, inner, cols, x_pitch, w_pitch, index = _check(x, w)
     code = _act_code(act)
     shape = (rows, cols)

@@ -306,3 +306,35 @@ def test_offsets_past_32_bits():
     dx, dw, db = LI.linear_bwd(y, x, w)
     backward_check(y[-200:], x[-200:], w, None, "none", dx[-200:], None, None)
     backward_check(y, x, w, None, "none", None, dw, db)
+
+
+def place(rows, cols, pitch, value=7.0):
+    """A matrix whose rows start on 16-byte boundaries, and what lies between and behind them."""
+    buf = torch.full((rows * pitch + 64,), value, device=DEV, dtype=BF)
+    inside = torch.zeros_like(buf, dtype=torch.bool)
+    inside[:rows * pitch].view(rows, pitch)[:, :cols] = True
+    return buf[:rows * pitch].view(rows, pitch)[:, :cols], buf, ~inside
+
+
+@pytest.mark.parametrize("cols", [1, 35, 70, 100, 147, 1015, 2047])
+@pytest.mark.parametrize("rows,inner", [(1, 25000), (10, 48), (64, 512), (200, 512), (1035, 96), (3000, 512), (9000, 264)])
+def test_rows_that_end_between_16_byte_boundaries_leave_what_lies_behind(rows, inner, cols):
+    """Results whose rows start on 16-byte boundaries, of any width: the elements up to the next boundary are not theirs."""
+    g = torch.Generator(device=DEV).manual_seed(rows + inner + cols)
+    x, w, b = rnd(g, rows, inner).to(BF), (rnd(g, cols, inner) / math.sqrt(inner)).to(BF), rnd(g, cols)
+    r = rnd(g, rows, cols).to(BF)
+    for pitch in ((cols + 7) // 8 * 8, (cols + 7) // 8 * 8 + 8):
+        (out, ob, out_rest), (z, zb, z_rest) = (place(rows, cols, pitch) for _ in range(2))
+        out.copy_(r)                                   # the residual is the result's place
+        LI.linear_fwd(x, w, b, act="gelu", resid=out, keep=True, out=out, z=z)
+        forward_check(x, w, b, "gelu", r, out, z)
+        assert bool((ob[out_rest] == 7).all()) and bool((zb[z_rest] == 7).all())
+        y, _ = LI.linear_fwd(x, w, b, act="gelu", resid=r, out=place(rows, cols, pitch)[0])
+        assert torch.equal(y, out)
+        # of dx: dy [rows, inner], w [inner, cols]
+        dy, xx, ww = rnd(g, rows, inner).to(BF), rnd(g, rows, cols).to(BF), (rnd(g, inner, cols) / math.sqrt(inner)).to(BF)
+        for need_dw in (False, True):
+            dx, gb, dx_rest = place(rows, cols, pitch)
+            _, dw, db = LI.linear_bwd(dy, xx, ww, dx=dx, need_dw=need_dw)
+            backward_check(dy, xx, ww, None, "none", dx, dw, db)
+            assert bool((gb[dx_rest] == 7).all())
