@@ -175,9 +175,11 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
 
 
 def slices_for(rows: int, cols: int, multiprocessors: int) -> int:
-    """Slices of the rows whose column sums may be taken apart: four blocks on every multiprocessor, four rows each (one where they are
-    wide). One for what a cluster of blocks, which joins its own sums, is through with before a second launch would begin (221 x 35,
-    bf16: 15.7 us a call for 20.1; 250 x 200: 14.0 for 18.9, in a graph 9.4 for 9.6)."""
+    """Slices of the rows whose column sums may be taken apart: four blocks on every multiprocessor, four rows each; one block and
+    one row where rows are wide, for a slice is as large as two of them (2,000 x 65,536 bf16: 868 us a call and 74 MB of sums, with four
+    blocks 1,489 and 296; 4,000 x 5,000 51 us and 6 MB, 51 and 23). One slice for what a cluster of blocks, which joins its own
+    sums, is through with before a second launch would begin (221 x 35, bf16: 15.7 us a call for 20.1; 250 x 200: 14.0 for 18.9, in a
+    graph 9.4 for 9.6)."""
     if rows <= 256 and rows * cols <= 2 ** 16 and cols <= 4096:
         return 1
-    return max(2, min(4 * multiprocessors, -(-rows // (4 if cols <= 4096 else 1))))
+    return max(2, min(4 * multiprocessors, -(-rows // 4)) if cols <= 4096 else min(multiprocessors, rows))

@@ -98,3 +98,12 @@ def test_statistics_between_8_byte_boundaries_are_refused(start):
         LN.layer_norm_bwd(mat(), mat(), stats)
     with pytest.raises(ValueError, match="GPU"):          # two further on: taken
         LN.layer_norm_bwd(mat(), mat(), flat[2:2 + 2 * ROWS].view(ROWS, 2))
+
+
+@pytest.mark.parametrize("rows,cols,slices", [
+    (1, 1, 1), (256, 256, 1), (256, 257, 64), (257, 8, 65), (250, 200, 1), (1000, 10, 250), (16, 4096, 1), (17, 4096, 5), (15, 4097, 15),
+    (1, 4097, 2), (2368, 64, 592), (2369, 64, 592), (147, 16384, 147), (149, 16384, 148), (64800, 1536, 592), (1000, 10 ** 6, 148), (2, 2 ** 31 - 2 ** 10, 2)])
+def test_slices_of_the_rows(rows, cols, slices):
+    """One (a cluster's) up to 256 rows and 2^16 elements of rows of up to 4,096; at most four a multiprocessor, of four rows; of
+    wider rows one a multiprocessor, of one row. Two at least where there is a workspace."""
+    assert LN.slices_for(rows, cols, 148) == slices
