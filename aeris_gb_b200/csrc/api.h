@@ -239,17 +239,17 @@ long long aeris_ortho_work_bytes(const AerisOrtho* a);          // of its groups
 int aeris_orthogonalise(const AerisOrtho* a, void* stream);     // the number of kernels launched, or a negative code
 
 // Layer norm (csrc/layer_norm.cu; mirrored in ops/layer_norm.py). Pitches in elements; columns lie side by side. Forward: y and
-// stats (mean, 1 / sqrt(var + eps)) of x. Backward: y receives the gradient of x, dw and db (both or neither is null only with
-// the other's flag) the column sums. y may be x or dy itself.
+// stats (mean, 1 / sqrt(var + eps)) of x. Backward: y receives the gradient of x, dw and db the column sums, each where it is
+// given. y may be x or dy itself.
 typedef struct AerisLayerNorm {
   const void *x, *dy;
   void* y;
   const void *w, *b;                // [cols], bf16 or fp32 both; null: ones, zeros
   float *stats;                     // [rows, 2], from an 8-byte boundary on
-  float *dw, *db, *work;            // [cols] each, null: not wanted; work: [slices, 2, cols]
+  float *dw, *db, *work;            // [cols] each, null: not wanted; work: [slices, 2, cols], null where slices are one at most
   int* status;
   long long rows, ld_x, ld_dy, ld_y;
-  int cols, f32, w_f32, add, slices;            // f32: type of x, dy, y; add: dw, db are added to
+  int cols, f32, w_f32, add, slices;            // f32: type of x, dy, y; add: both of dw, db that are given are added to
   float eps;
 } AerisLayerNorm;
 // Both return the number of kernels launched, or a negative code.

@@ -745,7 +745,8 @@ int launch_ln_odd(const AerisLayerNorm& a, cudaStream_t stream, int* slices) {
   constexpr int PER_SM = 1024 / TH;
   const int R = slices ? RB : RF;
   const int bytes = (a.cols * static_cast<int>(sizeof(T)) + 30) / 16 * 16, row = slices ? 2 * bytes : bytes;
-  int stages = (200 * 1024 / PER_SM - 1024) / (R * row);        // three at least
+  // three at least, but for the widest fp32 rows of 64 and of 128 threads (241 to 256, 509 to 512 columns): two
+  int stages = (200 * 1024 / PER_SM - 1024) / (R * row);
   if (stages > 6) stages = 6;
   const long long need = (a.rows + R - 1) / R;
   long long blocks = static_cast<long long>(num_sms()) * PER_SM;
@@ -787,7 +788,7 @@ int launch_ln_fwd(const AerisLayerNorm& a, LnCut cut, int threads, cudaStream_t 
     return launch_chained(ln_fwd_one_kernel<T, NV, BLOCK>, static_cast<unsigned>(blocks), threads, 0, stream, a, cut);
 }
 
-// The cut of rows of `vecs` vectors into lanes: groups of a warp as far as `most` vectors a lane go.
+// The cut of rows of `vecs` vectors into lanes: groups of a warp, as many lanes as there are vectors, up to all of them.
 LnCut ln_cut(int vecs) {
   LnCut c;
   c.group = 1;

@@ -36,7 +36,9 @@ struct LinParams {
 
 // exp(-z^2 / 2) and the Gaussian distribution function of z: erfc by the rational approximation in 1 / (1 + p x) times exp(-x^2)
 // of Abramowitz and Stegun, 7.1.26, whose absolute error is below 1.5e-7. Next to CUDA's erff it takes half the instructions,
-// shares its exponential with the derivative and does not cancel far below zero.
+// shares its exponential with the derivative and does not cancel far below zero. Relative to z cdf(z) it is off by up to 5e-5 at
+// z = -3, 1.6e-3 at -5, 3.6e-3 at -6 (half a step of bf16, of values of 6e-9), 1e-2 at -8; the absolute error of GELU is at most
+// 2.1e-7 everywhere.
 __device__ __forceinline__ void gauss(float z, float& e, float& cdf) {
   const float x = fabsf(z) * 0.70710678118654752f;
   const float t = 1.f / fmaf(0.3275911f, x, 1.f);
@@ -103,7 +105,7 @@ __device__ __forceinline__ void act32(uint32_t (&v)[32]) {
 }
 
 // bf16 columns of a warp's 32 rows on their way out, 32 at a time: two buffers each for y and z, which one lane hands to the TMA
-// unit as 32 x 32 tiles (64-byte swizzle); what lies past the matrix is clipped.
+// unit as 32 x 32 tiles (64-byte swizzle); what lies past the matrix is clipped (see lin_maps).
 struct LinOut {
   uint8_t* stage;        // 8 KB: y, y, z, z of 2 KB
   int lane, n = 0;
@@ -741,7 +743,9 @@ struct DzParams {
   long long ld_dy, ld_z, ld_dz;
   int rows, cols;
 };
-// dz = dy act'(z) and the column sums of one slice of the rows. A thread takes V columns (one 16-byte vector, or one column
+// dz = dy act'(z) and the column sums of one slice of the rows. dz is rounded to bf16, half a step of it at most (2^-8), for the tensor
+// core multiplies bf16 by bf16 and the other operands are bf16: dx and dw end 2.3e-3 off where fp32 products of an unrounded dz end
+// 1.7e-3 off, which is their own rounding. The sums are of the fp32 values. A thread takes V columns (one 16-byte vector, or one column
 // where rows start anywhere) of every R-th row of its slice; a block 64 columns. 28,800 x 2048, GELU by tanh: 73 us, 4.9 TB/s, with
 // half as many slices 78; four rows at a time and two blocks an SM 85, one row and five 92; column sums alone 24 (4.8 TB/s).
 template <int V> constexpr int DZ_ROWS = DZ_THREADS / (DZ_COLS / V);

@@ -3,7 +3,7 @@
     y = (x - mean) / sqrt(var + eps) * w + b          over the columns of a row
 
 The norm of the plain window transformer block; this framework's own blocks use the modulated RMS norm of
-:mod:`.elementwise`.
+:mod:`.elementwise`. As all front ends here they record nothing for autograd: the backward pass is a call of its own.
 """
 from __future__ import annotations
 
@@ -128,7 +128,8 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weigh
     """Gradients of :func:`layer_norm_fwd` for ``dy`` with respect to its rows; ``x`` and ``stats`` are its input and its second
     result. Returns (gradient of x in x's type, fp32 gradient of the weight or None without one, fp32 gradient of the bias or None
     with ``bias=False``). ``dx`` may be ``dy`` or ``x`` itself; ``dw``, ``db`` [cols] fp32 are added to where given. The same
-    bits on every run; tensors whose rows start elsewhere may be added up in another order."""
+    bits on every run; tensors whose rows start elsewhere may be added up in another order. Allocates :func:`slices_for` times 8
+    bytes a column for the sums while it runs."""
     rows, cols, pitch, dt, index = _check(x, weight, None)
     shape = x.shape
     pitch_dy = _like(dy, shape, dt, index, "dy")

@@ -4,7 +4,12 @@
 
 Windows of ``high x wide`` tokens in rows. The relative position of query i and key j is the whole number
 ``(y_i - y_j + high - 1) * (2 * wide - 1) + x_i - x_j + wide - 1``; ``buckets`` maps it to a row of the table. The attention of
-:mod:`.attention` is the same without a bias.
+:mod:`.attention` is the same without a bias. As all front ends here they record nothing for autograd: the backward pass is a call
+of its own.
+
+Scores, softmax statistics and sums are fp32. Probabilities go into the product with v, and into that with dO, in bf16, and so does
+the scores' gradient into those with q and k: 2^-8 of every term, for the tensor core multiplies bf16 by bf16 (results 2.0e-3 to
+2.5e-3 off where fp32 products end 1.7e-3 off, which is their own rounding). The table's gradient is taken from fp32 values.
 """
 from __future__ import annotations
 
@@ -163,7 +168,10 @@ def biased_attn_bwd(d_o: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, lse: 
                     scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Gradients of :func:`biased_attn_fwd` for ``d_o`` with respect to its first result; ``o``, ``lse`` are its results. Returns
     (gradient of qkv, in its layout; fp32 gradient of the table [rows, heads], or None without ``need_dtable``). ``dqkv``: where to
-    put it; ``dtable`` fp32 is added to where given. Rows that hide their pairs get zero. The same bits on every run."""
+    put it; ``dtable`` fp32 is added to where given. Rows that hide their pairs get zero. The same bits on every run.
+
+    Allocates while it runs, in windows of more than 96 tokens, 20 bytes a token and head and, for the table's gradient, sums of
+    the scores' gradient of one head (4 bytes a pair of tokens: 4.3 GB in the largest windows) or of more, up to 256 MB."""
     high, wide, n, pitch, scale, index = _check(qkv, n_win, window, heads, d, table, buckets, scale)
     tokens, inner = n_win * n, heads * d
     o_pitch, do_pitch = _rows(o, (tokens, inner), index, "o"), _rows(d_o, (tokens, inner), index, "d_o")
