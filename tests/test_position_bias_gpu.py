@@ -424,3 +424,11 @@ def test_plain_attention_of_padded_heads_goes_on_into_its_backward_pass(heads, d
     f = formula(qkv, window, heads, d, 0 * table, None, 1 / math.sqrt(d))
     forward_check(o, lse, f)
     backward_check(d_o, o, dqkv, None, f, window, heads, d, 1 / math.sqrt(d), len(table))
+
+
+@pytest.mark.parametrize("window,heads,d", [((95, 95), 1, 64), ((1, 9000), 1, 40), ((9001, 1), 1, 128), ((1, 15700), 1, 64), ((126, 125), 1, 128)])
+def test_windows_whose_tables_do_not_fit_beside_the_tiles(window, heads, d):
+    """Slices of a head's table, and beyond them (15,000 tokens and more) the table in memory."""
+    g = torch.Generator(device=DEV).manual_seed(window[0])
+    run_both(*make(1, window, heads, d, g), 1, window, heads, d)
+    torch.cuda.empty_cache()
