@@ -246,3 +246,17 @@ def test_offsets_past_32_bits():
     dx, _, db = LN.layer_norm_bwd(y, y, again)
     backward_check(y[-50:], y[-50:], again[-50:], None, dx[-50:], None, None)
     assert bool((db.double() - y.double().sum(0)).abs().lt((2 ** 16 + 17) * U * y.double().abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 5), (7, 64), (300, 333), (2500, 333), (1300, 1001), (40, 1536), (1200, 3411), (330, 12544), (30, 20001)])
+@pytest.mark.parametrize("gap,start", [(8, 0), (3, 0), (8, 1)])
+def test_what_lies_between_rows_is_not_read_into_results(rows, cols, gap, start, dt):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    x, dy = (torch.full((rows, cols + gap), math.nan, device=DEV, dtype=dt)[:, start:start + cols] for _ in range(2))
+    for t in (x, dy):
+        t.copy_(torch.randn((rows, cols), generator=g, device=DEV))
+    w, b = (torch.randn(cols, generator=g, device=DEV) for _ in range(2))
+    y, stats = LN.layer_norm_fwd(x, w, b, eps=EPS)
+    forward_check(x, w, b, y, stats)
+    backward_check(dy, x, stats, w, *LN.layer_norm_bwd(dy, x, stats, w))

@@ -338,3 +338,23 @@ def test_rows_that_end_between_16_byte_boundaries_leave_what_lies_behind(rows, i
             _, dw, db = LI.linear_bwd(dy, xx, ww, dx=dx, need_dw=need_dw)
             backward_check(dy, xx, ww, None, "none", dx, dw, db)
             assert bool((gb[dx_rest] == 7).all())
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(1, 35, 70), (5, 100, 33), (10, 48, 147), (200, 295, 100), (1035, 515, 777), (3000, 70, 1015), (9000, 333, 260)])
+@pytest.mark.parametrize("gap", [0, 8, 3])
+def test_what_lies_between_rows_is_not_read_into_results(rows, inner, cols, gap):
+    g = torch.Generator(device=DEV).manual_seed(rows + inner + cols + gap)
+
+    def of(r, c):
+        t, buf, rest = place(r, c, (c + 7) // 8 * 8 + gap, math.nan)
+        t.copy_(rnd(g, r, c))
+        return t
+
+    x, w, dy, resid, z = of(rows, inner), of(cols, inner), of(rows, cols), of(rows, cols), of(rows, cols)
+    w.mul_(1 / math.sqrt(inner))
+    b = rnd(g, cols)
+    y, kept = LI.linear_fwd(x, w, b, act="silu", resid=resid, keep=True)
+    forward_check(x, w, b, "silu", resid, y, kept)
+    for act, zz in (("silu", z), ("none", None)):
+        dx, dw, db = LI.linear_bwd(dy, x, w, zz, act=act)
+        backward_check(dy, x, w, zz, act, dx, dw, db)

@@ -432,3 +432,16 @@ def test_windows_whose_tables_do_not_fit_beside_the_tiles(window, heads, d):
     g = torch.Generator(device=DEV).manual_seed(window[0])
     run_both(*make(1, window, heads, d, g), 1, window, heads, d)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("window,heads,d", [((3, 5), 2, 24), ((9, 13), 3, 40), ((12, 13), 2, 128), ((17, 19), 2, 64), ((5, 7), 1, 20)])
+@pytest.mark.parametrize("gap", [8, 3])
+def test_what_lies_between_rows_is_not_read_into_results(window, heads, d, gap):
+    g = torch.Generator(device=DEV).manual_seed(d + gap)
+    n_win, n = 3, window[0] * window[1]
+    tight = make(n_win, window, heads, d, g)
+    qkv, d_o = (torch.full((t.shape[0] + 1, t.shape[1] + gap), math.nan, device=DEV, dtype=BF)[:-1, :t.shape[1]] for t in (tight[0], tight[3]))
+    qkv.copy_(tight[0])
+    d_o.copy_(tight[3])
+    assert n_win * n == len(qkv)
+    run_both(qkv, tight[1], None, d_o, n_win, window, heads, d)
