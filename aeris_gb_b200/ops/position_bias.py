@@ -170,6 +170,9 @@ def biased_attn_bwd(d_o: torch.Tensor, qkv: torch.Tensor, o: torch.Tensor, lse: 
     (gradient of qkv, in its layout; fp32 gradient of the table [rows, heads], or None without ``need_dtable``). ``dqkv``: where to
     put it; ``dtable`` fp32 is added to where given. Rows that hide their pairs get zero. The same bits on every run.
 
+    Probabilities are made anew from ``lse``, in fp32: where all that a query sees has biases of a size B, they are off by about
+    1e-7 B of themselves. Entries that are to hide are :data:`HIDDEN` or less.
+
     Allocates while it runs, in windows of more than 96 tokens, 20 bytes a token and head and, for the table's gradient, sums of
     the scores' gradient of one head (4 bytes a pair of tokens: 4.3 GB in the largest windows) or of more, up to 256 MB."""
     high, wide, n, pitch, scale, index = _check(qkv, n_win, window, heads, d, table, buckets, scale)
